@@ -350,6 +350,99 @@ NTOPS_API int ntops_sdpa_ws(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64
 NTOPS_API int64_t ntops_sdpa_workspace(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Skv,
                int64_t D, int has_mask);
 
+/* ---- MXFP4 (microscaled 4-bit floating point) ---------------------------- */
+/* No ntops counterparts.  A row of `cols` values is cut into ceil(cols / 32)
+ * blocks of 32 (the last one padded with zeros).  A block's scale is 2^e, e =
+ * max(-127, floor(log2(max |x|)) - 2), stored as the byte e + 127; its values
+ * are x / 2^e rounded to the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 (ties to the
+ * even code) and cut at 6, stored as 4-bit codes (sign in bit 3), two a byte,
+ * the first in the low half.  A block with a NaN or an infinity has the scale
+ * byte 255 and zero codes, and stands for NaN.
+ *
+ * codes: rows of 16 * ceil(cols / 32) bytes, scales: rows of ceil(cols / 32)
+ * bytes, both without gaps; codes 4-byte aligned.  x: F32 / F16 / BF16 with
+ * unit column stride. */
+NTOPS_API int ntops_quantize_mxfp4(int dtype, int64_t rows, int64_t cols, const void* x, int64_t x_row_stride,
+               void* codes, void* scales, void* stream);
+
+/* y (rows x cols, without gaps, F32 / F16 / BF16) = the values of the codes and
+ * scales, rounded once to dtype; row strides in bytes, codes and their row
+ * stride multiples of 4.  cols may be less than the blocks hold. */
+NTOPS_API int ntops_dequantize_mxfp4(int dtype, int64_t rows, int64_t cols,
+               const void* codes, int64_t codes_row_stride,
+               const void* scales, int64_t scales_row_stride, void* y, void* stream);
+
+/* out (M, N) = A B^T (+ bias) for MXFP4 A (M, K) and B (N, K): fp32 sums, bias
+ * (N values of out_dtype, may be NULL) added in fp32, one rounding to out_dtype
+ * (F32 / F16 / BF16).  Code rows 16-byte aligned; strides of codes and scales
+ * in bytes, of out in elements (unit column stride).  The workspace (16-byte
+ * aligned) holds fp32 partial products where K is split over the GPU (a missing
+ * or short one: not split), and a copy of scale rows that are not whole groups
+ * of 8 bytes on 4-byte addresses (required then). */
+NTOPS_API int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K,
+               const void* a, int64_t a_row_stride, const void* a_scales, int64_t as_row_stride,
+               const void* b, int64_t b_row_stride, const void* b_scales, int64_t bs_row_stride,
+               const void* bias, void* out, int64_t out_row_stride,
+               void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace ntops_mxfp4_mm uses for this problem on the current device
+ * (0: none). */
+NTOPS_API int64_t ntops_mxfp4_mm_workspace(int64_t M, int64_t N, int64_t K,
+               const void* a_scales, int64_t as_row_stride,
+               const void* b_scales, int64_t bs_row_stride);
+
+/* ---- key / value cache in 8 bits ------------------------------------------ */
+/* No ntops counterparts (its KV cache, kernels/scaled_dot_product_attention.py:
+ * 139-140, is of the query's type).  key_cache and value_cache (B, H, C, D)
+ * hold e4m3 values in units of an fp32 scale for each block of `block` (a power
+ * of two >= 16) consecutive tokens of a head: key_scale and value_scale (B, H,
+ * ceil(C / block)).  Strides in elements: 4 of a cache, 3 of its scales; the
+ * last dims have unit strides.
+ *
+ * ntops_store_kv_cache stores key and value (B, H, S, D; F32 / F16 / BF16):
+ * sequence b's first lengths[b] tokens (all S where lengths is NULL) go to
+ * positions[b] (`position` where positions is NULL) and on; tokens that would
+ * lie outside of 0 .. C - 1 are dropped.  A block's scale is 2^e, e the least
+ * integer >= -126 with max |x| <= 448 2^e over the finite new values, and the
+ * values are x / 2^e rounded to e4m3 (NaN for what is not finite).  Where the
+ * new tokens start inside a block, the larger of its scale and theirs is kept,
+ * and the block's earlier tokens are rounded again if that raises it.  What the
+ * cache holds behind the new tokens stays as it is (and means nothing in the
+ * rest of their last block).  Indices are I32 or I64. */
+NTOPS_API int ntops_store_kv_cache(int dtype, int64_t B, int64_t H, int64_t S, int64_t D, int64_t C, int64_t block,
+               const void* key, const int64_t* key_strides,
+               const void* value, const int64_t* value_strides,
+               void* key_cache, const int64_t* key_cache_strides,
+               void* value_cache, const int64_t* value_cache_strides,
+               float* key_scale, const int64_t* key_scale_strides,
+               float* value_scale, const int64_t* value_scale_strides,
+               const void* positions, int positions_dtype, int64_t position,
+               const void* lengths, int lengths_dtype, void* stream);
+
+/* out (B, Hq, Sq, D) = softmax(q k^T * scale) v over the first lengths[b] (I32
+ * or I64; NULL: C) tokens of sequence b's cache; lengths outside of 0 .. C count
+ * as the nearer of the two.  causal 1: query row i sees the keys up to lengths[b]
+ * - Sq + i.  A row that sees no key is 0.  Query head h reads cache head h /
+ * (Hq / H).  Nothing behind a sequence's length is read.  fp32 sums; 16-bit q
+ * with D a multiple of 16 up to 128 runs on the matrix cores (probabilities,
+ * times the scale of their value block, rounded to bf16), D <= 256 and F32 on a
+ * kernel of one wave per row.  The workspace (16-byte aligned; may be NULL)
+ * spreads the keys of few query rows over the GPU. */
+NTOPS_API int ntops_kv_cache_attention(int dtype, int64_t B, int64_t Hq, int64_t H, int64_t Sq, int64_t C, int64_t D,
+               int64_t block, const void* q, const int64_t* q_strides,
+               const void* key_cache, const int64_t* key_cache_strides,
+               const void* value_cache, const int64_t* value_cache_strides,
+               const float* key_scale, const int64_t* key_scale_strides,
+               const float* value_scale, const int64_t* value_scale_strides,
+               const void* lengths, int lengths_dtype, int causal, double scale,
+               void* out, const int64_t* out_strides,
+               void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace ntops_kv_cache_attention uses for this problem on the
+ * current device (0: none). */
+NTOPS_API int64_t ntops_kv_cache_attention_workspace(int dtype, int64_t B, int64_t Hq, int64_t H, int64_t Sq,
+               int64_t C, int64_t D);
+
 /* ---- fused variants ------------------------------------------------------- */
 /* residual_out = x + residual (rounded to dtype) and y = rms_norm(residual_out)
  * over rows x cols with the conventions of ntops_rms_norm (weight of dtype or

@@ -124,6 +124,22 @@ _SIGNATURES = {
          _vp],
     ),
     "ntops_gemm_workspace": (_i64, [_i, _i64, _i64, _i64, _i64]),
+    "ntops_quantize_mxfp4": (_i, [_i, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "ntops_dequantize_mxfp4": (_i, [_i, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),
+    "ntops_mxfp4_mm": (
+        _i,
+        [_i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp],
+    ),
+    "ntops_mxfp4_mm_workspace": (_i64, [_i64, _i64, _i64, _vp, _i64, _vp, _i64]),
+    "ntops_store_kv_cache": (
+        _i,
+        [_i] + [_i64] * 6 + [_vp, _c_i64p] * 6 + [_vp, _i, _i64, _vp, _i, _vp],
+    ),
+    "ntops_kv_cache_attention": (
+        _i,
+        [_i] + [_i64] * 7 + [_vp, _c_i64p] * 5 + [_vp, _i, _i, _d, _vp, _c_i64p, _vp, _i64, _vp],
+    ),
+    "ntops_kv_cache_attention_workspace": (_i64, [_i] + [_i64] * 6),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -1,0 +1,29 @@
+// Shared by the attention kernels on a cache in 8 bits (attn_cache*.hip).
+#pragma once
+
+#include "attention.h"
+#include "kv_cache.h"
+
+namespace ntops {
+
+struct CacheAttnArgs {
+  const void* q;       // (B, Hq, Sq, D)
+  const uint8_t* k;    // (B, Hkv, C, D) e4m3
+  const uint8_t* v;
+  const float* ks;     // (B, Hkv, blocks)
+  const float* vs;
+  void* o;
+  int64_t qst[3], kst[3], vst[3], kss[2], vss[2], ost[3];
+  const void* lengths;  // tokens of each sequence (null: C)
+  int lengths_dtype;
+  int64_t C;
+  int B, Hq, Hkv, Sq, D, shift;  // a block of scales: 1 << shift tokens
+  int causal;            // row i sees keys up to length - Sq + i
+  float scale_log2;      // scale * log2(e)
+};
+
+__device__ __forceinline__ int64_t length_of(const CacheAttnArgs& a, int b) {
+  return max(int64_t(0), min(a.C, index_at(a.lengths, a.lengths_dtype, b, a.C)));
+}
+
+}  // namespace ntops

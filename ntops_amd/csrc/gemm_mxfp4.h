@@ -1,0 +1,60 @@
+// Shared by the MXFP4 product's kernels (gemm_mxfp4*.hip): out = A B^T (+ a
+// bias row) for A (M, K) and B (N, K) of 4-bit codes with a scale byte per 32.
+//
+// v_mfma_scale_f32_16x16x128_f8f6f4 on 4-bit data: lane l holds the 16 bytes
+// (32 codes, one block) of row l & 15 and k block l >> 4 of A / B, and that
+// block's scale in one byte of a register; of the result it holds column l & 15
+// and rows 4 (l >> 4) .. + 3.  Which blocks make up the instruction's four does
+// not matter as long as A and B agree: a lane takes neighbouring blocks in
+// consecutive instructions, so that their scales are neighbouring bytes of one
+// register and the instruction's byte select picks them.
+#pragma once
+
+#include "mfma.h"
+
+namespace ntops {
+
+struct Mx4Args {
+  const uint8_t* a;    // codes: 16 bytes a block
+  const uint8_t* as;   // scales: a byte a block
+  const uint8_t* b;
+  const uint8_t* bs;
+  const void* bias;    // N values of the output's type, or null
+  void* d;
+  int64_t lda, ldas, ldb, ldbs;  // row strides in bytes
+  int64_t ldd;         // elements
+  int M, N, kb;        // kb: blocks of 32 along K
+  float* part;         // split K: fp32 partial products, slice s at s * M * N
+  int split, kchunk;   // slices, and the blocks of each
+};
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// c += A B over 4 blocks; SA / SB: the byte of sa / sb that holds the scales.
+template <int SA, int SB>
+__device__ __forceinline__ f32x4 mfma_mx4(u32x4 a, uint32_t sa, u32x4 b, uint32_t sb, f32x4 c) {
+  // (4-bit data fills the first half of the 256-bit operands)
+  const i32x8 x = {static_cast<int>(a.x), static_cast<int>(a.y), static_cast<int>(a.z), static_cast<int>(a.w), 0, 0, 0, 0};
+  const i32x8 y = {static_cast<int>(b.x), static_cast<int>(b.y), static_cast<int>(b.z), static_cast<int>(b.w), 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, SA, static_cast<int>(sa), SB, static_cast<int>(sb));
+}
+
+__device__ __forceinline__ u32x4 mx4_rsrc(const void* base, int64_t bytes) {
+  const uint64_t addr = reinterpret_cast<uint64_t>(base);
+  u32x4 r;
+  r.x = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(addr));
+  r.y = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(addr >> 32) & 0xffffu);
+  r.z = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(bytes));
+  r.w = 0x00020000u;
+  return r;
+}
+
+// 4-byte global -> LDS copy per lane: lane l's dword lands at lds_dst + 4 l.
+__device__ __forceinline__ void dma4(u32x4 rsrc, uint32_t lds_dst, uint32_t voffset) {
+  asm volatile("buffer_load_dword %0, %1, 0 offen lds"
+               :
+               : "v"(voffset), "s"(rsrc), "{m0}"(lds_dst)
+               : "memory");
+}
+
+}  // namespace ntops

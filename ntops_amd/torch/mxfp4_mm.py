@@ -1,0 +1,58 @@
+"""mxfp4_mm -- the product of two MXFP4 matrices (see quantize_mxfp4) that share
+their last dim, as a linear layer's activations and weight do:
+
+    output = input @ mat2.T (+ bias)
+
+No ntops counterpart (its products, torch/mm.py:7-18 and addmm.py:7-18, take 16
+and 32 bits).  input (M, K) and mat2 (N, K) are codes with their scales; with
+input_scale None, input is a float tensor (M, K) that is quantized first.  Sums
+are fp32, bias (N,) of `dtype` is added in fp32, and the result is rounded once
+to `dtype` (bfloat16, float16 or float32)."""
+
+import torch
+
+from ntops_amd import _lib
+from ntops_amd.torch.dequantize_mxfp4 import _checked_pair
+from ntops_amd.torch.quantize_mxfp4 import quantize_mxfp4
+from ntops_amd.torch.utils import _DeviceGuard, _cast_into, _contiguous
+
+
+def _code_rows(t):
+    """t with rows that the kernels can read: unit stride, 16-byte aligned."""
+    if t.stride(1) == 1 and t.stride(0) >= 0 and t.stride(0) % 16 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return _cast_into(t, torch.empty(t.shape, dtype=t.dtype, device=t.device))
+
+
+def mxfp4_mm(input, input_scale, mat2, mat2_scale, bias=None, *, dtype=torch.bfloat16):
+    if input.dim() != 2 or mat2.dim() != 2:
+        raise RuntimeError("mxfp4_mm: expected 2-D tensors")
+    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise RuntimeError(f"mxfp4_mm: unsupported dtype {dtype}")
+    blocks = _checked_pair(mat2, mat2_scale, "mxfp4_mm")
+    dev = _lib.require_cuda(input, input_scale, mat2, mat2_scale, bias)
+    m, n = input.shape[0], mat2.shape[0]
+    if input_scale is None:
+        if -(-input.shape[1] // 32) != blocks:
+            raise RuntimeError(f"mxfp4_mm: rows of {input.shape[1]} values do not have mat2's {blocks} blocks of 32")
+        input, input_scale = quantize_mxfp4(input)
+    elif _checked_pair(input, input_scale, "mxfp4_mm") != blocks:
+        raise RuntimeError(f"mxfp4_mm: {input_scale.shape[1]} and {blocks} blocks cannot be multiplied")
+    if bias is not None and (bias.shape != (n,) or bias.dtype != dtype):
+        raise RuntimeError(f"mxfp4_mm: expected a bias of shape ({n},) and dtype {dtype}, got {tuple(bias.shape)}, {bias.dtype}")
+
+    output = torch.empty((m, n), dtype=dtype, device=dev)
+    lib = _lib.load()
+    with _DeviceGuard(dev):
+        a, b = _code_rows(input), _code_rows(mat2)
+        sa, sb = (s if s.stride(1) == 1 and s.stride(0) >= 0 else _contiguous(s) for s in (input_scale, mat2_scale))
+        bias = None if bias is None else _contiguous(bias)
+        scales = (sa.data_ptr(), sa.stride(0)), (sb.data_ptr(), sb.stride(0))
+        ws_bytes = lib.ntops_mxfp4_mm_workspace(m, n, 32 * blocks, *scales[0], *scales[1])
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
+        rc = lib.ntops_mxfp4_mm(
+            _lib.dtype_code(dtype), m, n, 32 * blocks, a.data_ptr(), a.stride(0), *scales[0], b.data_ptr(), b.stride(0),
+            *scales[1], None if bias is None else bias.data_ptr(), output.data_ptr(), n,
+            None if ws is None else ws.data_ptr(), ws_bytes, _lib.stream_of(output))
+    _lib.check(rc, "ntops_amd.mxfp4_mm")
+    return output

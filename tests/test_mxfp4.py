@@ -1,0 +1,102 @@
+"""MXFP4 without a GPU: the oracle against closed forms, and what the entry
+points refuse."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import ntops_amd.torch as nt
+from ntops_amd import _lib
+from oracle import narrow as N
+
+
+def test_oracle_rounds_to_the_nearest_code():
+    grid = np.concatenate([N.E2M1, -N.E2M1])
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((50, 96)) * np.exp(3 * rng.standard_normal((50, 1)))
+    codes, scales = N.quantize_mxfp4(x)
+    v = N.dequantize_mxfp4(codes, scales)
+    s = np.repeat(np.exp2(scales.astype(float) - 127), 32, -1)
+    best = np.abs(x[..., None] / s[..., None] - grid).min(-1)
+    assert np.allclose(np.abs(x - v) / s, best, rtol=0, atol=1e-12)
+    top = np.abs(x).reshape(50, 3, 32).max(-1)
+    assert ((top / np.exp2(scales.astype(float) - 127) >= 4) & (top / np.exp2(scales.astype(float) - 127) < 8)).all()
+
+
+def test_oracle_ties_go_to_the_even_code():
+    x = np.zeros((1, 32))
+    x[0, :9] = [0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0, -0.25]
+    codes, scales = N.quantize_mxfp4(x)
+    assert scales[0, 0] == 127
+    assert N.dequantize_mxfp4(codes, scales)[0, :9].tolist() == [0, 1, 1, 2, 2, 4, 4, 6, 0]
+
+
+def test_oracle_packs_the_first_value_low():
+    x = np.zeros((1, 32))
+    x[0, :4] = [4.0, -0.5, 1.0, 6.0]
+    codes, _ = N.quantize_mxfp4(x)
+    assert codes[0, 0] == 6 | 9 << 4 and codes[0, 1] == 2 | 7 << 4
+
+
+def test_oracle_zeros_and_not_finite():
+    x = np.zeros((1, 96))
+    x[0, 40], x[0, 70] = np.inf, np.nan
+    codes, scales = N.quantize_mxfp4(x)
+    assert scales.tolist() == [[0, 255, 255]] and not codes.any()
+
+
+def test_refusals():
+    u8 = lambda *s: torch.zeros(s, dtype=torch.uint8)
+    with pytest.raises(RuntimeError, match="at least one dim"):
+        nt.quantize_mxfp4(torch.tensor(1.0))
+    with pytest.raises(RuntimeError, match="unsupported dtype"):
+        nt.quantize_mxfp4(torch.zeros(2, 32, dtype=torch.float64))
+    with pytest.raises(RuntimeError, match="expected a GPU tensor"):
+        nt.quantize_mxfp4(torch.zeros(2, 32))
+    with pytest.raises(RuntimeError, match="codes"):
+        nt.dequantize_mxfp4(u8(2, 32), u8(2, 1))
+    with pytest.raises(RuntimeError, match="uint8"):
+        nt.dequantize_mxfp4(u8(2, 32).int(), u8(2, 2))
+    with pytest.raises(RuntimeError, match="blocks of 32"):
+        nt.dequantize_mxfp4(u8(2, 32), u8(2, 2), 32)
+    with pytest.raises(RuntimeError, match="blocks of 32"):
+        nt.dequantize_mxfp4(u8(2, 32), u8(2, 2), 65)
+    with pytest.raises(RuntimeError, match="unsupported dtype"):
+        nt.dequantize_mxfp4(u8(2, 32), u8(2, 2), dtype=torch.float64)
+    with pytest.raises(RuntimeError, match="2-D"):
+        nt.mxfp4_mm(u8(1, 2, 32), u8(1, 2, 2), u8(4, 32), u8(4, 2))
+    with pytest.raises(RuntimeError, match="expected a GPU tensor"):
+        nt.mxfp4_mm(u8(2, 32), u8(2, 2), u8(4, 32), u8(4, 2))
+    with pytest.raises(RuntimeError, match="unsupported dtype"):
+        nt.mxfp4_mm(u8(2, 32), u8(2, 2), u8(4, 32), u8(4, 2), dtype=torch.float64)
+
+
+P = ctypes.c_void_p
+
+
+def _mm(lib, m=2, n=4, k=64, a=256, lda=32, as_=512, ldas=2, b=1024, ldb=32, bs=2048, ldbs=2, bias=None, out=4096, ldd=4, ws=None, wsb=0, dtype=_lib.BF16):
+    return lib.ntops_mxfp4_mm(dtype, m, n, k, P(a), lda, P(as_), ldas, P(b), ldb, P(bs), ldbs, P(bias), P(out), ldd, P(ws), wsb, None)
+
+
+def test_c_entry_points_refuse():
+    lib = _lib.load()
+    err = lambda: lib.ntops_last_error().decode()
+    assert lib.ntops_quantize_mxfp4(_lib.BF16, -1, 32, P(256), 32, P(256), P(256), None) == 1 and "negative" in err()
+    assert lib.ntops_quantize_mxfp4(_lib.F64, 1, 32, P(256), 32, P(256), P(256), None) == 2
+    assert lib.ntops_quantize_mxfp4(_lib.BF16, 1, 32, None, 32, P(256), P(256), None) == 1 and "null" in err()
+    assert lib.ntops_quantize_mxfp4(_lib.BF16, 1, 32, P(256), 32, P(258), P(256), None) == 1 and "aligned" in err()
+    assert lib.ntops_quantize_mxfp4(_lib.BF16, 1 << 40, 1 << 40, P(256), 32, P(256), P(256), None) == 2
+    assert lib.ntops_dequantize_mxfp4(_lib.BF16, 1, 32, P(256), 18, P(256), 1, P(256), None) == 1 and "aligned" in err()
+    assert lib.ntops_dequantize_mxfp4(_lib.I32, 1, 32, P(256), 16, P(256), 1, P(256), None) == 2
+    assert _mm(lib, m=-1) == 1
+    assert _mm(lib, dtype=_lib.F64) == 2
+    assert _mm(lib, a=264) == 1 and "16 bytes" in err()
+    assert _mm(lib, ldb=40) == 1
+    assert _mm(lib, ldas=-4) == 1 and "negative" in err()
+    assert _mm(lib, out=None) == 1 and "null" in err()
+    assert _mm(lib, k=1 << 40, lda=1 << 35, ldb=1 << 35) == 2 and "too large" in err()
+    # scale rows of 2 bytes need a workspace
+    assert _mm(lib) == 1 and "workspace" in err()
+    assert _mm(lib, m=0) == 0 and lib.ntops_quantize_mxfp4(_lib.BF16, 0, 32, None, 32, None, None, None) == 0
