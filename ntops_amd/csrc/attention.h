@@ -34,6 +34,52 @@ __device__ __forceinline__ int vslot(int r, int c) {
     return c ^ (((r >> 1) & 1) << 2);
 }
 
+// max(a, b, c) in one instruction, without the NaN-quieting moves the
+// compiler puts in front of fmaxf in IEEE mode (a NaN operand may be
+// dropped; a NaN score still reaches the output through its exponential).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// From here on a result cut to [0, 1] keeps a NaN (it is 0 by default): the
+// wave's MODE register, bit 8 (DX10_CLAMP).
+__device__ __forceinline__ void clamp_keeps_nan() { __builtin_amdgcn_s_setreg(1 | 8 << 6 | 0 << 11, 0); }
+
+// B fragment of S = Q K^T: key rows n0 .. n0 + 31 (lane l: row n0 + (l & 31)),
+// d = 16 ks + 8 (l >> 5) .. + 7.
+template <int D>
+__device__ __forceinline__ u32x4 k_frag(const char* tile, int n0, int ks, int lane) {
+  const int r = n0 + (lane & 31);
+  const int c = ks * 2 + (lane >> 5);
+  return *reinterpret_cast<const u32x4*>(tile + r * (D * 2) + kslot<D>(r, c) * 16);
+}
+
+// B fragment of O += P V for the 16-key slice sl and output columns
+// n0 .. n0 + 31: lane l receives column n0 + (l & 31) at keys
+// 16 sl + 4 (l >> 5) + 0..3 (elements 0..3) and 16 sl + 8 + 4 (l >> 5) + 0..3
+// (elements 4..7) -- the key order in which the S accumulator holds P.
+template <int D>
+__device__ __forceinline__ u32x4 v_frag(const char* tile, int n0, int sl, int lane) {
+  const int i = lane & 15;
+  const int n = n0 + ((lane >> 4) & 1) * 16 + (i & 3) * 4;
+  const int c = n >> 3, half = (n >> 2) & 1;
+  s16x4 v[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int k = sl * 16 + h * 8 + (lane >> 5) * 4 + (i >> 2);
+    const char* p = tile + k * (D * 2) + vslot<D>(k, c) * 16 + half * 8;
+    v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(p));
+  }
+  u32x4 r;
+  r.x = static_cast<uint16_t>(v[0][0]) | (static_cast<uint32_t>(static_cast<uint16_t>(v[0][1])) << 16);
+  r.y = static_cast<uint16_t>(v[0][2]) | (static_cast<uint32_t>(static_cast<uint16_t>(v[0][3])) << 16);
+  r.z = static_cast<uint16_t>(v[1][0]) | (static_cast<uint32_t>(static_cast<uint16_t>(v[1][1])) << 16);
+  r.w = static_cast<uint16_t>(v[1][2]) | (static_cast<uint32_t>(static_cast<uint16_t>(v[1][3])) << 16);
+  return r;
+}
+
 // True when attn_decode serves this problem: 16-bit data whose head dim and
 // rows suit the matrix cores, no explicit mask, at most 16 query rows per key
 // / value head, and more than kDecodeMinKeys keys -- or any but none, where

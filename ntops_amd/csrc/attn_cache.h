@@ -26,4 +26,16 @@ __device__ __forceinline__ int64_t length_of(const CacheAttnArgs& a, int b) {
   return max(int64_t(0), min(a.C, index_at(a.lengths, a.lengths_dtype, b, a.C)));
 }
 
+// 16-bit queries of head dims and layouts that the matrix cores' kernels read.
+bool cache_matrix_layout(const CacheAttnArgs& a, int dtype);
+
+// True when cache_decode serves this problem: such a layout, and at most 16
+// query rows per cache head.
+bool cache_decode_serves(const CacheAttnArgs& a, int dtype);
+// Bytes of workspace with which it spreads the keys over more blocks (0: one
+// block per cache head is as good).
+int64_t cache_decode_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t C, int64_t D);
+// Runs it; a missing or short workspace runs one block per cache head.
+int cache_decode(int dtype, const CacheAttnArgs& a, void* workspace, int64_t workspace_bytes, hipStream_t st);
+
 }  // namespace ntops

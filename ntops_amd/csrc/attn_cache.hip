@@ -19,6 +19,7 @@ namespace {
 // lane every 64th column for P V.  For head dims and layouts that the matrix
 // cores' kernels do not take, and fp32 queries.
 constexpr int kMaxDim = 256;
+constexpr int64_t kMaxCount = 0x7fffffff;
 
 template <typename T>
 __global__ __launch_bounds__(64) void k_cache_attn_rows(CacheAttnArgs a) {
@@ -91,7 +92,11 @@ using namespace ntops;
 
 extern "C" int64_t ntops_kv_cache_attention_workspace(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq,
                                                       int64_t C, int64_t D) {
-  return 0;
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || C <= 0 || D <= 0 || Hq % Hkv != 0 || dtype == NTOPS_F32) return 0;
+  if (B > kMaxCount || Hq > kMaxCount || Sq > kMaxCount || C > (int64_t(1) << 40) || B * Hq > kMaxCount ||
+      B * Hq * Sq > (int64_t(1) << 34))
+    return 0;  // (the call is refused)
+  return cache_decode_workspace(B, Hq, Hkv, Sq, C, D);
 }
 
 extern "C" int ntops_kv_cache_attention(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t C, int64_t D,
@@ -119,9 +124,8 @@ extern "C" int ntops_kv_cache_attention(int dtype, int64_t B, int64_t Hq, int64_
   if (C > 0 && (!key_cache || !value_cache || !key_scale || !value_scale || !key_cache_strides || !value_cache_strides ||
                 !key_scale_strides || !value_scale_strides))
     return set_error(NTOPS_ERR_INVALID, "kv_cache_attention: null pointer");
-  const int64_t lim = 0x7fffffff;
   if (D > kMaxDim) return set_error(NTOPS_ERR_UNSUPPORTED, "kv_cache_attention: head dim over %d", kMaxDim);
-  if (B > lim || Hq > lim || Sq > lim || C > (int64_t(1) << 40) || B * Hq > lim || B * Hq * Sq > (int64_t(1) << 34))
+  if (B > kMaxCount || Hq > kMaxCount || Sq > kMaxCount || C > (int64_t(1) << 40) || B * Hq > kMaxCount || B * Hq * Sq > (int64_t(1) << 34))
     return set_error(NTOPS_ERR_UNSUPPORTED, "kv_cache_attention: problem too large");
   CacheAttnArgs a{};
   a.q = q;
@@ -161,5 +165,8 @@ extern "C" int ntops_kv_cache_attention(int dtype, int64_t B, int64_t Hq, int64_
   a.causal = causal;
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (workspace_bytes < 0 || (workspace != nullptr && !aligned16(workspace)))
+    return set_error(NTOPS_ERR_INVALID, "kv_cache_attention: workspace not aligned to 16 bytes");
+  if (cache_decode_serves(a, dtype)) return cache_decode(dtype, a, workspace, workspace_bytes, st);
   return dispatch_float16_32(dtype, "kv_cache_attention", [&](auto tag) { return run_rows<decltype(tag)>(a, st); });
 }

@@ -1,0 +1,492 @@
+// A few query rows over an 8-bit cache (decode): Sq * (Hq / Hkv) <= 16 rows per
+// cache head.
+//
+// Bound by streaming the cache once.  A work item is (batch, cache head, slice
+// of the sequence's tokens); the rows that share the head fill the 16 columns
+// of v_mfma_f32_16x16x32 (S^T = K Q^T, O^T += V^T P^T).  Every wave owns its own
+// key tiles, 8 KiB of keys and of values each (64 keys at a head dim of 128),
+// in its own part of the LDS: direct non-temporal DMA two tiles ahead, refilled
+// as soon as the tile's keys, then its values, have been read, and no barrier
+// before the waves' merge.
+//
+// e4m3 becomes bf16 (f16 for the keys of f16 queries) in registers, exactly: a
+// key fragment is a 16-byte read whose halves feed two instructions, a value
+// fragment a transposing 8-byte read.  The scale of a key's block times the
+// softmax scale multiplies its scores, that of a value's block its
+// probabilities, which are then rounded to bf16 whatever the query's type: only
+// bf16 holds them under scales of any size.
+//
+// Slices are parts of the sequence's own length, known on the device only, so
+// the number of slices is set by the GPU's size and an empty slice leaves an
+// empty partial result.
+#include <algorithm>
+#include <atomic>
+
+#include "attn_cache.h"
+
+namespace ntops {
+namespace {
+
+constexpr int kMaxSplit = 64;
+
+template <typename T>
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (std::is_same<T, __bf16>::value)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+}
+
+// 16-byte slot of chunk c of row r in the tiles (D / 16 chunks a row): the
+// reads of a key fragment (16 rows at one chunk) and of a value fragment (rows
+// 0 .. 7 and 16 .. 23, or 8 .. 15 and 24 .. 31 of 32 in half a wave) each
+// touch every bank once.  Involutions.
+template <int D>
+__device__ __forceinline__ int kslot8(int r, int c) {
+  return kslot<D / 2>(r, c);
+}
+template <int D>
+__device__ __forceinline__ int vslot8(int r, int c) {
+  return D == 128 ? c ^ (((r >> 1) & 3) | ((r >> 4) & 1) << 2) : c ^ (((r >> 2) & 1) | ((r >> 4) & 1) << 1);
+}
+
+__device__ __forceinline__ void dma16_nt(u32x4 rsrc, uint32_t lds_dst, uint32_t voffset) {
+  asm volatile("buffer_load_dwordx4 %0, %1, 0 offen nt lds"
+               :
+               : "v"(voffset), "s"(rsrc), "{m0}"(lds_dst)
+               : "memory");
+}
+__device__ __forceinline__ void dma4(u32x4 rsrc, uint32_t lds_dst, uint32_t voffset) {
+  asm volatile("buffer_load_dword %0, %1, 0 offen lds"
+               :
+               : "v"(voffset), "s"(rsrc), "{m0}"(lds_dst)
+               : "memory");
+}
+__device__ __forceinline__ u32x4 make_rsrc(const void* base, uint32_t bytes) {
+  const uint64_t addr = reinterpret_cast<uint64_t>(base);
+  u32x4 r;
+  r.x = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(addr));
+  r.y = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(addr >> 32) & 0xffffu);
+  r.z = __builtin_amdgcn_readfirstlane(bytes);
+  r.w = 0x00020000u;
+  return r;
+}
+
+// Loads of a tile's key (or value) rows, 8 instructions of 1 KiB, and of the
+// scales of its 16-token parts, one instruction.
+template <int D, bool IS_V>
+struct TileDma {
+  static constexpr int kInst = 8;
+  static constexpr int kRows = 1024 / D;  // rows per instruction
+  u32x4 rows, scales;
+  uint32_t voff[kInst];
+  uint32_t part;  // this lane's 16-token part, in tokens
+  int first_part, shift;
+
+  // base: the slice's first row (token t0, a multiple of 16); n: tokens from there on
+  __device__ __forceinline__ void init(const uint8_t* base, int64_t ld, const float* scale, int64_t t0, int n, int lane,
+                                       int dt, int block_shift) {
+    rows = make_rsrc(base, n > 0 ? static_cast<uint32_t>((n - 1) * ld + dt) : 0u);
+    shift = block_shift;
+    const int64_t b0 = t0 >> shift;
+    first_part = static_cast<int>(t0 - (b0 << shift));
+    scales = make_rsrc(scale + b0, n > 0 ? static_cast<uint32_t>(((first_part + n - 1) >> shift) * 4 + 4) : 0u);
+    part = static_cast<uint32_t>(lane * 16);
+    constexpr int cpr = D / 16;
+#pragma unroll
+    for (int i = 0; i < kInst; ++i) {
+      const int row = i * kRows + lane / cpr;
+      const int c = IS_V ? vslot8<D>(row, lane % cpr) : kslot8<D>(row, lane % cpr);
+      voff[i] = c * 16 < dt ? static_cast<uint32_t>(row * ld + c * 16) : kOOB;
+    }
+  }
+  // The tile at token t of the slice (byte offset off) to dst, its scales to
+  // sdst; valid false: loads that count but bring nothing.
+  __device__ __forceinline__ void issue(uint32_t dst, uint32_t sdst, uint32_t off, int t, bool valid) const {
+#pragma unroll
+    for (int i = 0; i < kInst; ++i)
+      dma16_nt(rows, dst + i * 1024, !valid || voff[i] == kOOB ? kOOB : voff[i] + off);
+    const uint32_t at = static_cast<uint32_t>(first_part + t) + part;
+    dma4(scales, sdst, valid ? (at >> shift) * 4 : kOOB);
+  }
+};
+
+template <int N>
+__device__ __forceinline__ void wait_dma() {
+  __builtin_amdgcn_sched_barrier(0);
+  wait_vmcnt<N>();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// 8 e4m3 values (two words) as an operand of 8 T.
+template <typename T>
+__device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi) {
+  if constexpr (std::is_same<T, __bf16>::value)
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true))};
+  else
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true))};
+}
+
+constexpr int kStage = 16384 + 512;  // keys, values, their scales
+
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2 lds_i32x2_t;
+
+// part: fp32, per query row and slice the unnormalised O row, then (max in base
+// 2, sum) pairs; null: one slice, O normalised into a.o.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, int nsplit, float* part) {
+  constexpr int NK = 8192 / D;  // keys per tile
+  constexpr int KB = NK / 16;   // 16-key parts of a tile
+  constexpr int KC = D / 64;    // 16-byte key reads of a lane per part: two k-steps each
+  constexpr int DT = D / 16;    // 16-row tiles of O^T
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // [wave][2 stages]
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4;
+  const int64_t blk = block_id();
+  if (blk >= static_cast<int64_t>(nsplit) * a.B * a.Hkv) return;  // the tail of a 2-D grid (the whole block)
+  const int bh = static_cast<int>(blk / nsplit);
+  const int sp = static_cast<int>(blk - static_cast<int64_t>(bh) * nsplit);
+  const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const int group = a.Hq / a.Hkv;
+  const int rows = group * a.Sq;  // <= 16
+  const int64_t n_all = length_of(a, b);
+  // this slice: whole rounds of the waves' tiles
+  const int64_t step = NK * NW;
+  const int64_t chunk = (n_all + nsplit * step - 1) / (nsplit * step) * step;
+  const int64_t t0 = sp * chunk;
+  const int n = __builtin_amdgcn_readfirstlane(static_cast<int>(max(int64_t(0), min(n_all - t0, chunk))));
+  // query row of this lane's column: head hk * group + r / Sq, position r % Sq
+  const int r = lane & 15;
+  const int h = hk * group + r / a.Sq, qi = r % a.Sq;
+  // keys of the slice that the row sees, and that every row sees
+  const int lim = a.causal ? static_cast<int>(max(int64_t(-1), min(int64_t(n), n_all - a.Sq + qi + 1 - t0))) : n;
+  const int lim_min = a.causal ? static_cast<int>(max(int64_t(-1), min(int64_t(n), n_all - a.Sq + 1 - t0))) : n;
+
+  u32x4 qf[2 * KC];
+#pragma unroll
+  for (int s = 0; s < 2 * KC; ++s) {
+    const int d0 = ((s >> 1) * 4 + g) * 16 + (s & 1) * 8;  // the key bytes of k-step s in this lane
+    if (r < rows && d0 < a.D)
+      qf[s] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.q) + b * a.qst[0] + h * a.qst[1] + qi * a.qst[2] + d0);
+    else
+      qf[s] = u32x4{0, 0, 0, 0};
+  }
+  // settled here, so that no wait for it is placed among the tile loads
+#pragma unroll
+  for (int s = 0; s < 2 * KC; ++s) asm volatile("" ::"v"(qf[s]));
+
+  TileDma<D, false> kd;
+  TileDma<D, true> vd;
+  kd.init(a.k + b * a.kst[0] + hk * a.kst[1] + t0 * a.kst[2], a.kst[2], a.ks + b * a.kss[0] + hk * a.kss[1], t0, n, lane,
+          a.D, a.shift);
+  vd.init(a.v + b * a.vst[0] + hk * a.vst[1] + t0 * a.vst[2], a.vst[2], a.vs + b * a.vss[0] + hk * a.vss[1], t0, n, lane,
+          a.D, a.shift);
+  const int nt = (n + NK - 1) / NK;
+  const int mine_n = nt > wave ? (nt - wave + NW - 1) / NW : 0;  // tiles wave, wave + NW, ..
+  char* mine = smem + wave * (2 * kStage);
+  const uint32_t mine_addr = lds_addr(mine);
+  auto issue_k = [&](int j) {
+    const int t = (wave + j * NW) * NK;
+    const uint32_t st = mine_addr + (j & 1) * kStage;
+    kd.issue(st, st + 16384, static_cast<uint32_t>(t * a.kst[2]), t, j < mine_n);
+  };
+  auto issue_v = [&](int j) {
+    const int t = (wave + j * NW) * NK;
+    const uint32_t st = mine_addr + (j & 1) * kStage;
+    vd.issue(st + 8192, st + 16384 + 256, static_cast<uint32_t>(t * a.vst[2]), t, j < mine_n);
+  };
+
+  f32x4 o[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = neg_inf(), l = 0.f;  // running max (base 2) of row r; this lane's part of its sum
+
+  issue_k(0);
+  issue_v(0);
+  issue_k(1);
+  issue_v(1);
+  for (int j = 0; j < mine_n; ++j) {
+    const char* sk = mine + (j & 1) * kStage;
+    const char* sv = sk + 8192;
+    wait_dma<27>();  // keys of tile j are in; its values and tile j + 1 may be in flight
+    f32x4 s[KB];
+    float ks[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+      ks[kb] = *reinterpret_cast<const float*>(sk + 16384 + kb * 4);
+    }
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const int row = kb * 16 + (lane & 15);
+        const u32x4 w = *reinterpret_cast<const u32x4*>(sk + row * D + kslot8<D>(row, c * 4 + g) * 16);
+        s[kb] = mfma16<T>(widen8<T>(w.x, w.y), qf[2 * c], s[kb]);
+        s[kb] = mfma16<T>(widen8<T>(w.z, w.w), qf[2 * c + 1], s[kb]);
+      }
+    wait_lgkmcnt0();
+    issue_k(j + 2);
+
+    // scores of the slice's keys kt + 16 kb + 4 g + e
+    const int kt = (wave + j * NW) * NK;
+    float mx = neg_inf();
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[kb][e] *= ks[kb] * a.scale_log2;
+    if (kt + NK > lim_min) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[kb][e] = kt + kb * 16 + 4 * g + e < lim ? s[kb][e] : neg_inf();
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[kb][e]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float m_new = fmaxf(m, mx);
+    const float m_use = m_new == neg_inf() ? 0.f : m_new;  // nothing seen so far: P = 0
+    if (__any(m_new > m)) {
+      const float alpha = fast_exp2(m - m_use);
+      l *= alpha;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[t][e] *= alpha;
+      m = m_new;
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[kb][e] = fast_exp2(s[kb][e] - m_use);
+        l += s[kb][e];
+      }
+    wait_dma<27>();  // values of tile j are in
+    u32x4 pf[KB / 2];
+#pragma unroll
+    for (int p = 0; p < KB / 2; ++p) {
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float vs = *reinterpret_cast<const float*>(sk + 16384 + 256 + (2 * p + u) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * u + e] = s[2 * p + u][e] * vs;
+      }
+      pf[p] = pack8<__bf16>(x);  // keys 32 p + 4 g + 0..3 and 32 p + 16 + 4 g + 0..3
+    }
+#pragma unroll
+    for (int p = 0; p < KB / 2; ++p)
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        // V^T: lane row 16 t + (l & 15) at the keys of pf[p]: of the 16 lanes
+        // of a read, two hold 8 columns each of one of its 8 rows
+        const int i = lane & 15;
+        const int row = p * 32 + ((i >> 3) & 1) * 16 + g * 4 + ((i >> 1) & 3);
+        const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (lds_i32x2_t*)(sv + row * D + vslot8<D>(row, t) * 16 + (i & 1) * 8));
+        o[t] = mfma16<__bf16>(widen8<__bf16>(w.x, w.y), pf[p], o[t]);
+      }
+    wait_lgkmcnt0();
+    issue_v(j + 2);
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  wait_dma<0>();  // no DMA may land in the LDS the merge reuses
+  __syncthreads();
+
+  // merge the waves: per-wave (max, sum) of every row, then O scaled to the
+  // block's max
+  float* sm = reinterpret_cast<float*>(smem);  // [wave][16] max, [wave][16] sum, then [wave][16][D + 4] O
+  float* so = sm + 2 * NW * 16;
+  constexpr int LD = D + 4;
+  if (g == 0) {
+    sm[wave * 16 + r] = m;
+    sm[(NW + wave) * 16 + r] = l;
+  }
+  __syncthreads();
+  float mb = sm[r];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) mb = fmaxf(mb, sm[w * 16 + r]);
+  // (a wave whose scores are all NaN has a NaN sum and no max)
+  const float f = m == neg_inf() ? 0.f : fast_exp2(m - mb);
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) so[(wave * 16 + r) * LD + t * 16 + 4 * g + e] = o[t][e] * f;
+  __syncthreads();
+  const int64_t nrow = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
+  float* part_ml = part + nrow * nsplit * a.D;
+  for (int i = threadIdx.x; i < rows * (D / 4); i += 64 * NW) {
+    const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
+    if (d >= a.D) continue;
+    float mm = sm[row];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) mm = fmaxf(mm, sm[w * 16 + row]);
+    float sum = 0.f;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float mw = sm[w * 16 + row], lw = sm[(NW + w) * 16 + row];
+      sum += mw == neg_inf() ? lw : lw * fast_exp2(mw - mm);  // (no max: 0, or NaN)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += so[(w * 16 + row) * LD + d + e];
+    }
+    const int hh = hk * group + row / a.Sq, qq = row % a.Sq;
+    if (part) {
+      const int64_t at = ((static_cast<int64_t>(b) * a.Hq + hh) * a.Sq + qq) * nsplit + sp;
+      if (d == 0) {
+        part_ml[2 * at] = mm;
+        part_ml[2 * at + 1] = sum;
+      }
+      *reinterpret_cast<f32x4*>(part + at * a.D + d) = f32x4{v[0], v[1], v[2], v[3]};
+    } else {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      T w4[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w4[e] = static_cast<T>(v[e] * inv);
+      *reinterpret_cast<u32x2*>(static_cast<T*>(a.o) + b * a.ost[0] + hh * a.ost[1] + qq * a.ost[2] + d) =
+          __builtin_bit_cast(u32x2, w4);
+    }
+  }
+}
+
+// Combines the slices of every query row in slice order: one wave per row.
+template <typename T>
+__global__ __launch_bounds__(256) void k_cache_merge(CacheAttnArgs a, int nsplit, const float* part) {
+  const int lane = threadIdx.x & 63;
+  const int64_t nrow = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
+  const int64_t row = block_id() * 4 + (threadIdx.x >> 6);
+  if (row >= nrow) return;
+  const float* po = part + row * nsplit * a.D;
+  const float* ml = part + nrow * nsplit * a.D + 2 * row * nsplit;
+  const int d = lane * 2;
+  const auto load4 = [&](int s0, float2 (&v)[4]) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      v[u] = s0 + u < nsplit && d < a.D ? *reinterpret_cast<const float2*>(po + static_cast<int64_t>(s0 + u) * a.D + d)
+                                        : float2{0.f, 0.f};
+  };
+  float2 v[4];
+  load4(0, v);  // in flight while the weights are formed
+  float m = neg_inf(), l = 0.f;
+  if (lane < nsplit) {
+    m = ml[2 * lane];
+    l = ml[2 * lane + 1];
+  }
+  const float mm = wave_max(m);
+  const float w = m == neg_inf() ? 0.f : fast_exp2(m - mm);
+  const float sum = wave_sum(m == neg_inf() ? l : l * w);  // (no max: 0, or NaN)
+  float x = 0.f, y = 0.f;
+  for (int s0 = 0; s0 < nsplit; s0 += 4) {
+    if (s0 > 0) load4(s0, v);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float ws = s0 + u < nsplit ? lane_read(w, s0 + u) : 0.f;
+      x += ws * v[u].x;
+      y += ws * v[u].y;
+    }
+  }
+  if (d < a.D) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int q = static_cast<int>(row % a.Sq);
+    const int64_t bh = row / a.Sq;
+    T* O = static_cast<T*>(a.o) + (bh / a.Hq) * a.ost[0] + (bh % a.Hq) * a.ost[1] + q * a.ost[2];
+    T v2[2] = {static_cast<T>(x * inv), static_cast<T>(y * inv)};
+    *reinterpret_cast<uint32_t*>(O + d) = __builtin_bit_cast(uint32_t, v2);
+  }
+}
+
+// Waves of a block and slices of a sequence.  The sequences' lengths are not
+// known here: as many slices as leave about one two-wave block per CU, none
+// shorter than four tiles a wave at full length.
+void decode_split(int64_t heads, int64_t C, int64_t D, int& waves, int& nsplit) {
+  waves = heads < 2 * cu_count_cached() ? 2 : 1;
+  const int64_t step = (D > 64 ? 64 : 128) * waves;
+  int64_t n = std::min({static_cast<int64_t>(kMaxSplit), cu_count_cached() / heads, ceil_div(C, 4 * step)});
+  if (n <= 2 && C <= 8 * step) n = 1;  // two short slices gain what the merge's launch costs
+  nsplit = static_cast<int>(std::max<int64_t>(n, 1));
+}
+
+template <typename T, int D, int NW>
+int launch_decode(const CacheAttnArgs& a, int nsplit, float* part, hipStream_t st) {
+  constexpr int kLds = NW * 2 * kStage;
+  static_assert((2 * NW * 16 + NW * 16 * (D + 4)) * 4 <= kLds, "LDS");
+  auto kern = k_cache_decode<T, D, NW>;
+  static std::atomic<bool> attr_set{false};  // (threads may get here together)
+  if (!attr_set.load(std::memory_order_relaxed)) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) !=
+        hipSuccess)
+      return set_error(NTOPS_ERR_HIP, "kv_cache_attention: cannot reserve %d bytes of LDS", kLds);
+    attr_set.store(true, std::memory_order_relaxed);
+  }
+  const int64_t blocks = static_cast<int64_t>(nsplit) * a.B * a.Hkv;
+  note_kernel("kv_cache_decode d%d waves%d split%d", D, NW, nsplit);
+  hipLaunchKernelGGL(kern, blocks_2d(blocks), dim3(64 * NW), kLds, st, a, nsplit, part);
+  if (part) {
+    const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
+    hipLaunchKernelGGL((k_cache_merge<T>), blocks_2d(ceil_div(rows, 4)), dim3(256), 0, st, a, nsplit, part);
+  }
+  return check_launch("kv_cache_attention");
+}
+
+template <typename T>
+int run_decode(const CacheAttnArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
+  int waves, nsplit;
+  decode_split(static_cast<int64_t>(a.B) * a.Hkv, a.C, a.D, waves, nsplit);
+  const int64_t need = cache_decode_workspace(a.B, a.Hq, a.Hkv, a.Sq, a.C, a.D);
+  if (need == 0 || ws == nullptr || ws_bytes < need) {
+    nsplit = 1;
+    ws = nullptr;
+  }
+  float* part = static_cast<float*>(ws);
+  if (waves == 1)
+    return a.D > 64 ? launch_decode<T, 128, 1>(a, nsplit, part, st) : launch_decode<T, 64, 1>(a, nsplit, part, st);
+  return a.D > 64 ? launch_decode<T, 128, 2>(a, nsplit, part, st) : launch_decode<T, 64, 2>(a, nsplit, part, st);
+}
+
+}  // namespace
+
+bool cache_matrix_layout(const CacheAttnArgs& a, int dtype) {
+  const auto q8 = [](const int64_t* s) { return s[2] % 8 == 0 && s[1] % 8 == 0 && s[0] % 8 == 0; };
+  const auto c16 = [](const int64_t* s) { return s[2] % 16 == 0 && s[1] % 16 == 0 && s[0] % 16 == 0; };
+  const int64_t ld = std::max(a.kst[2], a.vst[2]);
+  return (dtype == NTOPS_BF16 || dtype == NTOPS_F16) && a.C > 0 && a.D % 16 == 0 && a.D <= 128 && q8(a.qst) &&
+         a.ost[2] % 4 == 0 && a.ost[1] % 4 == 0 && a.ost[0] % 4 == 0 && c16(a.kst) && c16(a.vst) && aligned16(a.q) &&
+         aligned16(a.k) && aligned16(a.v) && (reinterpret_cast<uintptr_t>(a.o) & 7u) == 0 && a.kst[2] >= a.D &&
+         a.vst[2] >= a.D && (a.C + 1024) * ld < 0x7fffffffLL && a.C < (int64_t(1) << 30);
+}
+
+bool cache_decode_serves(const CacheAttnArgs& a, int dtype) {
+  return cache_matrix_layout(a, dtype) && static_cast<int64_t>(a.Sq) * (a.Hq / a.Hkv) <= 16 &&
+         static_cast<int64_t>(a.B) * a.Hkv <= 0x7fffffffLL / kMaxSplit;
+}
+
+int64_t cache_decode_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t C, int64_t D) {
+  if (Sq * (Hq / Hkv) > 16 || D % 16 != 0 || D > 128 || C == 0) return 0;
+  int waves, nsplit;
+  decode_split(B * Hkv, C, D, waves, nsplit);
+  return nsplit > 1 ? B * Hq * Sq * nsplit * (D + 2) * 4 : 0;
+}
+
+int cache_decode(int dtype, const CacheAttnArgs& a, void* workspace, int64_t workspace_bytes, hipStream_t st) {
+  return dtype == NTOPS_BF16 ? run_decode<__bf16>(a, workspace, workspace_bytes, st)
+                             : run_decode<_Float16>(a, workspace, workspace_bytes, st);
+}
+
+}  // namespace ntops
