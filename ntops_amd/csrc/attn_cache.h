@@ -26,6 +26,8 @@ __device__ __forceinline__ int64_t length_of(const CacheAttnArgs& a, int b) {
   return max(int64_t(0), min(a.C, index_at(a.lengths, a.lengths_dtype, b, a.C)));
 }
 
+constexpr int kDecodeRows = 16;  // most query rows per cache head of cache_decode
+
 // 16-bit queries of head dims and layouts that the matrix cores' kernels read.
 bool cache_matrix_layout(const CacheAttnArgs& a, int dtype);
 
@@ -37,5 +39,15 @@ bool cache_decode_serves(const CacheAttnArgs& a, int dtype);
 int64_t cache_decode_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t C, int64_t D);
 // Runs it; a missing or short workspace runs one block per cache head.
 int cache_decode(int dtype, const CacheAttnArgs& a, void* workspace, int64_t workspace_bytes, hipStream_t st);
+
+// The same for any number of query rows.
+bool cache_tile_serves(const CacheAttnArgs& a, int dtype);
+int64_t cache_tile_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t C, int64_t D);
+int cache_tile(int dtype, const CacheAttnArgs& a, void* workspace, int64_t workspace_bytes, hipStream_t st);
+
+// Combines the slices' partial results of every query row in slice order: part
+// holds, per row (batch, head, position) and slice, the unnormalised O row, then
+// for each the pair (max in base 2, sum).
+void cache_merge(int dtype, const CacheAttnArgs& a, int nsplit, const float* part, hipStream_t st);
 
 }  // namespace ntops

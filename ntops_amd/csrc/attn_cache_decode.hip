@@ -438,10 +438,7 @@ int launch_decode(const CacheAttnArgs& a, int nsplit, float* part, hipStream_t s
   const int64_t blocks = static_cast<int64_t>(nsplit) * a.B * a.Hkv;
   note_kernel("kv_cache_decode d%d waves%d split%d", D, NW, nsplit);
   hipLaunchKernelGGL(kern, blocks_2d(blocks), dim3(64 * NW), kLds, st, a, nsplit, part);
-  if (part) {
-    const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
-    hipLaunchKernelGGL((k_cache_merge<T>), blocks_2d(ceil_div(rows, 4)), dim3(256), 0, st, a, nsplit, part);
-  }
+  if (part) cache_merge(std::is_same<T, __bf16>::value ? NTOPS_BF16 : NTOPS_F16, a, nsplit, part, st);
   return check_launch("kv_cache_attention");
 }
 
@@ -462,6 +459,12 @@ int run_decode(const CacheAttnArgs& a, void* ws, int64_t ws_bytes, hipStream_t s
 
 }  // namespace
 
+void cache_merge(int dtype, const CacheAttnArgs& a, int nsplit, const float* part, hipStream_t st) {
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
+  const auto kern = dtype == NTOPS_BF16 ? &k_cache_merge<__bf16> : &k_cache_merge<_Float16>;
+  hipLaunchKernelGGL(kern, blocks_2d(ceil_div(rows, 4)), dim3(256), 0, st, a, nsplit, part);
+}
+
 bool cache_matrix_layout(const CacheAttnArgs& a, int dtype) {
   const auto q8 = [](const int64_t* s) { return s[2] % 8 == 0 && s[1] % 8 == 0 && s[0] % 8 == 0; };
   const auto c16 = [](const int64_t* s) { return s[2] % 16 == 0 && s[1] % 16 == 0 && s[0] % 16 == 0; };
@@ -473,12 +476,12 @@ bool cache_matrix_layout(const CacheAttnArgs& a, int dtype) {
 }
 
 bool cache_decode_serves(const CacheAttnArgs& a, int dtype) {
-  return cache_matrix_layout(a, dtype) && static_cast<int64_t>(a.Sq) * (a.Hq / a.Hkv) <= 16 &&
+  return cache_matrix_layout(a, dtype) && static_cast<int64_t>(a.Sq) * (a.Hq / a.Hkv) <= kDecodeRows &&
          static_cast<int64_t>(a.B) * a.Hkv <= 0x7fffffffLL / kMaxSplit;
 }
 
 int64_t cache_decode_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t C, int64_t D) {
-  if (Sq * (Hq / Hkv) > 16 || D % 16 != 0 || D > 128 || C == 0) return 0;
+  if (Sq * (Hq / Hkv) > kDecodeRows || D % 16 != 0 || D > 128 || C == 0) return 0;
   int waves, nsplit;
   decode_split(B * Hkv, C, D, waves, nsplit);
   return nsplit > 1 ? B * Hq * Sq * nsplit * (D + 2) * 4 : 0;

@@ -1,0 +1,369 @@
+// Many query rows over an 8-bit cache (prompts, chunks of prompts).
+//
+// Rows are those of all query heads that share a cache head, in the order
+// (position, head): row r is position r / group of head r % group, so a tile of
+// 128 rows sees one cache head up to nearly the same key, and the tile's keys
+// are widened once for all of them.  Four waves of 32 rows; key tiles of 64.
+//
+//  * A tile's e4m3 keys and values come through registers (16-byte loads a tile
+//    ahead) and go to the LDS widened to 16 bits, in the layouts that the
+//    fragment reads of attention.h expect: each byte is converted once per block
+//    where converting fragments would do it in each of the four waves.
+//  * Values are widened to bf16 times the power of two in their block's scale
+//    (exact), whatever the query's type; what is left of a scale that is no
+//    power of two, in [1, 2), multiplies the probabilities, in a branch that
+//    stores made by this library never take.  The probabilities are rounded to
+//    bf16 for the product: only bf16 holds values under scales of any size.
+//  * The scale of a key's block times the softmax scale is a factor per 16 keys:
+//    the maximum is taken over raw scores in each 16 and scaled then, and the
+//    exponent is one fma per score.
+//  * Few tiles over many keys are split over slices of the keys, fp32 partial
+//    results combined in slice order (k_cache_merge).
+#include <algorithm>
+#include <atomic>
+
+#include "attn_cache.h"
+
+namespace ntops {
+namespace {
+
+constexpr int kRows = 128;
+constexpr int kKeys = 64;
+constexpr int kAhead = 4;  // fragments read ahead of the MFMA that uses them
+
+// Two e4m3 values of a word to 16-bit ones; bf16: times the power of two in scale.
+template <typename T, bool HI>
+__device__ __forceinline__ uint32_t widen2(uint32_t w, float scale) {
+  if constexpr (std::is_same<T, __bf16>::value)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
+}
+
+// The 16 values of a 16-byte chunk, as two 16-byte chunks.
+template <typename T>
+__device__ __forceinline__ void widen16(u32x4 c, float scale, u32x4 (&o)[2]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    o[i] = u32x4{widen2<T, false>(c[2 * i], scale), widen2<T, true>(c[2 * i], scale),
+                 widen2<T, false>(c[2 * i + 1], scale), widen2<T, true>(c[2 * i + 1], scale)};
+}
+
+__device__ __forceinline__ float max8(const float* v) {
+  return max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[7]));
+}
+
+// part: fp32 partial results (null: one slice, O normalised into a.o).
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb, int total, int nsplit, float* part) {
+  constexpr int KS = D / 16;          // k-steps of S = Q K^T
+  constexpr int DT = D / 32;          // 32-column tiles of O
+  constexpr int kTile = kKeys * D * 2;  // bytes of a widened tile
+  constexpr int CPR = D / 16;         // 16-byte chunks of a cache row
+  constexpr int NL = kKeys * CPR / 256;  // chunks a thread loads of a tile's keys (and values)
+  __shared__ __attribute__((aligned(1024))) char smem[2 * 2 * kTile];  // [stage][keys, values]
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int64_t pid = block_id();
+  if (pid >= total) return;  // the tail of a 2-D grid (the whole block)
+  // an XCD (workgroups go round them) walks whole cache heads; the tiles with
+  // the most keys first
+  if ((total & 7) == 0) pid = (pid & 7) * (total >> 3) + (pid >> 3);
+  const int per = nqb * nsplit;
+  const int bh = static_cast<int>(pid / per);
+  const int in = static_cast<int>(pid - static_cast<int64_t>(bh) * per);
+  const int qb = nqb - 1 - in / nsplit, sp = in % nsplit;
+  const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const int group = a.Hq / a.Hkv;
+  const int nrows = group * a.Sq;
+  const int64_t n_all = length_of(a, b);
+  // keys that the tile's last row sees
+  const int r_last = min(qb * kRows + kRows, nrows) - 1;
+  const int64_t seen = a.causal ? max(int64_t(0), n_all - a.Sq + r_last / group + 1) : n_all;
+  const int64_t chunk = (seen + nsplit * kKeys - 1) / (nsplit * kKeys) * kKeys;
+  const int64_t t0 = sp * chunk;
+  const int n = __builtin_amdgcn_readfirstlane(static_cast<int>(max(int64_t(0), min(seen - t0, chunk))));
+  const int nt = (n + kKeys - 1) / kKeys;
+
+  const int my_r = qb * kRows + wave * 32 + (lane & 31);
+  const bool in_rows = my_r < nrows;
+  const int my_q = my_r / group, my_h = hk * group + my_r - my_q * group;
+  // last key of the slice that this lane's row sees
+  const int my_lim = a.causal ? static_cast<int>(max(int64_t(-1), min(int64_t(n), n_all - a.Sq + my_q + 1 - t0))) - 1 : n - 1;
+  const int w_first = min(qb * kRows + wave * 32, nrows - 1) / group;  // the wave's first position
+  const int w_lim = a.causal ? static_cast<int>(max(int64_t(-1), min(int64_t(n), n_all - a.Sq + w_first + 1 - t0))) - 1 : n - 1;
+
+  // Q fragments (A operand of S); a negative softmax scale: -Q under its magnitude
+  u32x4 qf[KS];
+  const T* Q = static_cast<const T*>(a.q) + b * a.qst[0] + my_h * a.qst[1] + my_q * a.qst[2];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    const int d0 = ks * 16 + 8 * (lane >> 5);
+    qf[ks] = in_rows && d0 < a.D ? *reinterpret_cast<const u32x4*>(Q + d0) : u32x4{0, 0, 0, 0};
+    if (a.scale_log2 < 0.f) qf[ks] ^= 0x80008000u;
+  }
+  const float c0 = fabsf(a.scale_log2);
+
+  // this thread's chunks of a tile: chunk id threadIdx.x + 256 i, row id / CPR
+  const __amdgpu_buffer_rsrc_t rk = buffer_rsrc_uniform(
+      a.k + b * a.kst[0] + hk * a.kst[1] + t0 * a.kst[2], n > 0 ? static_cast<uint32_t>((n - 1) * a.kst[2] + a.D) : 0u);
+  const __amdgpu_buffer_rsrc_t rv = buffer_rsrc_uniform(
+      a.v + b * a.vst[0] + hk * a.vst[1] + t0 * a.vst[2], n > 0 ? static_cast<uint32_t>((n - 1) * a.vst[2] + a.D) : 0u);
+  const int64_t blk0 = t0 >> a.shift;
+  const int first_part = static_cast<int>(t0 - (blk0 << a.shift));
+  const uint32_t sbytes = n > 0 ? static_cast<uint32_t>(((first_part + n - 1) >> a.shift) * 4 + 4) : 0u;
+  const __amdgpu_buffer_rsrc_t rks = buffer_rsrc_uniform(a.ks + b * a.kss[0] + hk * a.kss[1] + blk0, sbytes);
+  const __amdgpu_buffer_rsrc_t rvs = buffer_rsrc_uniform(a.vs + b * a.vss[0] + hk * a.vss[1] + blk0, sbytes);
+  uint32_t koff[NL], voff[NL];
+  int lrow[NL], lchunk[NL];
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int id = threadIdx.x + 256 * i;
+    lrow[i] = id / CPR;
+    lchunk[i] = id % CPR;
+    const bool ok = lchunk[i] * 16 < a.D;
+    koff[i] = ok ? static_cast<uint32_t>(lrow[i] * a.kst[2] + lchunk[i] * 16) : kOOB;
+    voff[i] = ok ? static_cast<uint32_t>(lrow[i] * a.vst[2] + lchunk[i] * 16) : kOOB;
+  }
+  u32x4 kc[NL], vc[NL];
+  float kscale[4], vscale[4], vrow[NL];  // of the tile's four 16-key parts; of this thread's value rows
+  const auto load = [&](int j) {
+    const uint32_t kt = static_cast<uint32_t>(j) * static_cast<uint32_t>(kKeys * a.kst[2]);
+    const uint32_t vt = static_cast<uint32_t>(j) * static_cast<uint32_t>(kKeys * a.vst[2]);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      kc[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, koff[i] == kOOB ? kOOB : koff[i] + kt, 0, 0));
+      vc[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, voff[i] == kOOB ? kOOB : voff[i] + vt, 0, 0));
+      vrow[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                                              rvs, ((first_part + j * kKeys + lrow[i]) >> a.shift) * 4, 0, 0));
+    }
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const int at = ((first_part + j * kKeys + p * 16) >> a.shift) * 4;
+      kscale[p] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rks, at, 0, 0));
+      vscale[p] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rvs, at, 0, 0));
+    }
+  };
+  const auto put = [&](int stage) {
+    char* sk = smem + stage * 2 * kTile;
+    char* sv = sk + kTile;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      u32x4 w[2];
+      widen16<T>(kc[i], 1.f, w);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        *reinterpret_cast<u32x4*>(sk + lrow[i] * (D * 2) + kslot<D>(lrow[i], lchunk[i] * 2 + u) * 16) = w[u];
+      widen16<__bf16>(vc[i], vrow[i], w);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        *reinterpret_cast<u32x4*>(sv + lrow[i] * (D * 2) + vslot<D>(lrow[i], lchunk[i] * 2 + u) * 16) = w[u];
+    }
+  };
+
+  f32x16 o[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
+  float m_i = neg_inf(), l_i = 0.f;  // running max (base 2) of row my_r; this lane's half of its sum
+  float c[4], f[4];  // of the current tile's parts: the scores' factor, the rest of the values' scale
+  const auto factors = [&]() {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      // at least a tiny factor, so that a masked score (-inf) stays one under a zero scale
+      const float x = kscale[p] * c0;
+      c[p] = x < 0x1p-120f ? 0x1p-120f : x;
+      f[p] = vscale[p] < 0x1p-126f ? 0.f
+                                   : __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, vscale[p]) & 0x7fffffu) | 0x3f800000u);
+    }
+  };
+  if (nt > 0) {
+    load(0);
+    put(0);
+    factors();
+  }
+  __syncthreads();
+
+  for (int j = 0; j < nt; ++j) {
+    const char* sk = smem + (j & 1) * 2 * kTile;
+    const char* sv = sk + kTile;
+    if (j + 1 < nt) load(j + 1);
+    f32x16 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
+    {
+      constexpr int nm = 2 * KS;  // MFMA i: d slice i / 2, key half i % 2
+      u32x4 fr[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) fr[i] = k_frag<D>(sk, (i % 2) * 32, i / 2, lane);
+#pragma unroll
+      for (int i = 0; i < nm; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        s[i % 2] = mfma32<T>(fr[i % kAhead], qf[i / 2], s[i % 2]);
+        if (i + kAhead < nm) fr[i % kAhead] = k_frag<D>(sk, ((i + kAhead) % 2) * 32, (i + kAhead) / 2, lane);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // element 4q + e of half t is key 64 j + 32 t + 8 q + 4 (lane >> 5) + e
+    if (j * kKeys + kKeys - 1 > w_lim) {
+      const int rel = my_lim - j * kKeys - 4 * (lane >> 5);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[t][e] = 32 * t + 8 * (e >> 2) + (e & 3) <= rel ? s[t][e] : neg_inf();
+    }
+    float x[2][16];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[t][e] = s[t][e];
+    const float th = fmaxf(max3(max8(&x[0][0]) * c[0], max8(&x[0][8]) * c[1], max8(&x[1][0]) * c[2]), max8(&x[1][8]) * c[3]);
+    if (__any(th > m_i)) {
+      const auto h2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(th), __float_as_uint(th), false, false);
+      const float tmax = fmaxf(__uint_as_float(h2[0]), __uint_as_float(h2[1]));  // of lanes l and l ^ 32
+      const bool up = tmax > m_i;
+      const float alpha = up ? fast_exp2(m_i - tmax) : 1.f;
+      m_i = up ? tmax : m_i;
+      l_i *= alpha;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[t][e] *= alpha;
+    }
+    const float mb = m_i == neg_inf() ? 0.f : m_i;  // nothing seen so far: P = 0
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[t][e] = fast_exp2(fmaf(s[t][e], c[2 * t + (e >> 3)], -mb));
+    {
+      float r[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) r[e] = x[0][e] + x[1][e];
+#pragma unroll
+      for (int w = 8; w >= 1; w >>= 1)
+#pragma unroll
+        for (int e = 0; e < w; ++e) r[e] += r[e + w];
+      l_i += r[0];
+    }
+    if (f[0] != 1.f || f[1] != 1.f || f[2] != 1.f || f[3] != 1.f) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[t][e] *= f[2 * t + (e >> 3)];
+    }
+    {
+      u32x4 pf[4];
+#pragma unroll
+      for (int sl = 0; sl < 4; ++sl) pf[sl] = pack8<__bf16>(&x[sl >> 1][8 * (sl & 1)]);
+      constexpr int nm = 4 * DT;  // MFMA i: key slice i / DT, d tile i % DT
+      u32x4 fr[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) fr[i] = v_frag<D>(sv, (i % DT) * 32, i / DT, lane);
+#pragma unroll
+      for (int i = 0; i < nm; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        o[i % DT] = mfma32<__bf16>(fr[i % kAhead], pf[i / DT], o[i % DT]);
+        if (i + kAhead < nm) fr[i % kAhead] = v_frag<D>(sv, ((i + kAhead) % DT) * 32, (i + kAhead) / DT, lane);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // the other stage was last read before the barrier that ended the previous tile
+    if (j + 1 < nt) {
+      put((j + 1) & 1);
+      factors();
+    }
+    __syncthreads();
+  }
+
+  l_i += __shfl_xor(l_i, 32, 64);
+  if (!in_rows) return;
+  if (part) {
+    const int64_t nrow = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
+    const int64_t at = ((static_cast<int64_t>(b) * a.Hq + my_h) * a.Sq + my_q) * nsplit + sp;
+    float* ml = part + nrow * nsplit * a.D;
+    if (lane < 32) {
+      ml[2 * at] = m_i;
+      ml[2 * at + 1] = l_i;
+    }
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int qq = 0; qq < 4; ++qq) {
+        const int col = t * 32 + 8 * qq + 4 * (lane >> 5);
+        if (col < a.D)
+          *reinterpret_cast<f32x4*>(part + at * a.D + col) =
+              f32x4{o[t][4 * qq], o[t][4 * qq + 1], o[t][4 * qq + 2], o[t][4 * qq + 3]};
+      }
+    return;
+  }
+  const float inv = l_i == 0.f ? 0.f : 1.f / l_i;  // (a NaN sum passes through)
+  T* O = static_cast<T*>(a.o) + b * a.ost[0] + my_h * a.ost[1] + my_q * a.ost[2];
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int qq = 0; qq < 4; ++qq) {
+      T v4[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v4[e] = static_cast<T>(o[t][4 * qq + e] * inv);
+      const int col = t * 32 + 8 * qq + 4 * (lane >> 5);
+      if (col < a.D)  // a.D % 16 == 0: the 4 columns are all in or all out
+        *reinterpret_cast<u32x2*>(O + col) = __builtin_bit_cast(u32x2, v4);
+    }
+}
+
+// Slices of the keys: as many as bring the tiles to two per CU, none under four
+// key tiles at full length.
+int tile_split(int64_t heads, int64_t rows, int64_t C) {
+  const int64_t tiles = heads * ceil_div(rows, kRows);
+  const int64_t n = std::min({static_cast<int64_t>(64), 2 * cu_count_cached() / tiles, ceil_div(C, 4 * kKeys)});
+  return static_cast<int>(std::max<int64_t>(n, 1));
+}
+
+template <typename T, int D>
+int launch_tile(const CacheAttnArgs& a, int nsplit, float* part, hipStream_t st) {
+  const int64_t rows = static_cast<int64_t>(a.Hq / a.Hkv) * a.Sq;
+  const int64_t nqb = ceil_div(rows, kRows);
+  const int64_t total = nqb * nsplit * a.B * a.Hkv;
+  note_kernel("kv_cache_tile d%d split%d", D, nsplit);
+  hipLaunchKernelGGL((k_cache_tile<T, D>), blocks_2d(total), dim3(256), 0, st, a, static_cast<int>(nqb),
+                     static_cast<int>(total), nsplit, part);
+  if (part) cache_merge(std::is_same<T, __bf16>::value ? NTOPS_BF16 : NTOPS_F16, a, nsplit, part, st);
+  return check_launch("kv_cache_attention");
+}
+
+template <typename T>
+int run_tile(const CacheAttnArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
+  int nsplit = tile_split(static_cast<int64_t>(a.B) * a.Hkv, static_cast<int64_t>(a.Hq / a.Hkv) * a.Sq, a.C);
+  const int64_t need = cache_tile_workspace(a.B, a.Hq, a.Hkv, a.Sq, a.C, a.D);
+  if (need == 0 || ws == nullptr || ws_bytes < need) {
+    nsplit = 1;
+    ws = nullptr;
+  }
+  float* part = static_cast<float*>(ws);
+  return a.D > 64 ? launch_tile<T, 128>(a, nsplit, part, st) : launch_tile<T, 64>(a, nsplit, part, st);
+}
+
+}  // namespace
+
+bool cache_tile_serves(const CacheAttnArgs& a, int dtype) {
+  const int64_t rows = static_cast<int64_t>(a.Hq / a.Hkv) * a.Sq;
+  return cache_matrix_layout(a, dtype) && rows < (int64_t(1) << 30) &&
+         ceil_div(rows, kRows) * a.B * a.Hkv <= 0x7fffffffLL / 64;
+}
+
+int64_t cache_tile_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t C, int64_t D) {
+  if (D % 16 != 0 || D > 128 || C == 0) return 0;
+  const int nsplit = tile_split(B * Hkv, Hq / Hkv * Sq, C);
+  return nsplit > 1 ? B * Hq * Sq * nsplit * (D + 2) * 4 : 0;
+}
+
+int cache_tile(int dtype, const CacheAttnArgs& a, void* workspace, int64_t workspace_bytes, hipStream_t st) {
+  return dtype == NTOPS_BF16 ? run_tile<__bf16>(a, workspace, workspace_bytes, st)
+                             : run_tile<_Float16>(a, workspace, workspace_bytes, st);
+}
+
+}  // namespace ntops
