@@ -375,10 +375,9 @@ NTOPS_API int ntops_dequantize_mxfp4(int dtype, int64_t rows, int64_t cols,
 /* out (M, N) = A B^T (+ bias) for MXFP4 A (M, K) and B (N, K): fp32 sums, bias
  * (N values of out_dtype, may be NULL) added in fp32, one rounding to out_dtype
  * (F32 / F16 / BF16).  Code rows 16-byte aligned; strides of codes and scales
- * in bytes, of out in elements (unit column stride).  The workspace (16-byte
- * aligned) holds fp32 partial products where K is split over the GPU (a missing
- * or short one: not split), and a copy of scale rows that are not whole groups
- * of 8 bytes on 4-byte addresses (required then). */
+ * in bytes, of out in elements (unit column stride); scale rows may start
+ * anywhere.  The workspace (16-byte aligned; may be NULL) holds fp32 partial
+ * products where K is split over the GPU. */
 NTOPS_API int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K,
                const void* a, int64_t a_row_stride, const void* a_scales, int64_t as_row_stride,
                const void* b, int64_t b_row_stride, const void* b_scales, int64_t bs_row_stride,
@@ -387,9 +386,7 @@ NTOPS_API int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K,
 
 /* Bytes of workspace ntops_mxfp4_mm uses for this problem on the current device
  * (0: none). */
-NTOPS_API int64_t ntops_mxfp4_mm_workspace(int64_t M, int64_t N, int64_t K,
-               const void* a_scales, int64_t as_row_stride,
-               const void* b_scales, int64_t bs_row_stride);
+NTOPS_API int64_t ntops_mxfp4_mm_workspace(int64_t M, int64_t N, int64_t K);
 
 /* ---- key / value cache in 8 bits ------------------------------------------ */
 /* No ntops counterparts (its KV cache, kernels/scaled_dot_product_attention.py:

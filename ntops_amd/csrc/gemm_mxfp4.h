@@ -57,4 +57,32 @@ __device__ __forceinline__ void dma4(u32x4 rsrc, uint32_t lds_dst, uint32_t voff
                : "memory");
 }
 
+// A lane's 4 consecutive columns n .. n + 3 of row m, rounded; whole: the output's
+// rows are runs that 4 elements at a time can be stored to.
+template <typename T>
+__device__ __forceinline__ void store4(T* d, int64_t ldd, int m, int n, int M, int N, f32x4 v, const T* bias, bool whole) {
+  if (m >= M) return;
+  T* at = d + static_cast<int64_t>(m) * ldd + n;
+  T o[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float b = bias != nullptr && n + e < N ? static_cast<float>(bias[n + e]) : 0.f;
+    o[e] = static_cast<T>(v[e] + b);
+  }
+  if (whole && n + 4 <= N) {
+    if constexpr (sizeof(T) == 2)
+      *reinterpret_cast<u32x2*>(at) = __builtin_bit_cast(u32x2, o);
+    else
+      *reinterpret_cast<u32x4*>(at) = __builtin_bit_cast(u32x4, o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < N) at[e] = o[e];
+  }
+}
+
+constexpr int kSkinnyRows = 16;
+// out for M <= kSkinnyRows, bound by streaming B.
+int mx4_skinny(int out_dtype, const Mx4Args& g, hipStream_t st);
+
 }  // namespace ntops

@@ -1,9 +1,15 @@
 // The MXFP4 product's tile kernel, its split over K, and the C entry points.
 //
-// 128 x 128 output tiles, four waves of 64 x 64, K tiles of 256 values (128
+// BT x BT output tiles, four waves of BT / 2 x BT / 2, K tiles of 256 values (128
 // bytes a row, whole lines) through a ring of four stages filled by direct DMA
-// three tiles ahead; one barrier per K tile.  A stage is 32 KiB of codes and 2
-// KiB of scales.
+// three tiles ahead; one barrier per K tile.
+//
+// Scales come as dwords.  Where a row's scales do not start on one, or K tiles
+// end inside a dword (FIT false), a lane loads the three dwords that its row's 8
+// bytes lie in and reads single bytes; bytes behind the row's last block, which
+// may belong to another row and be 255 (NaN), become 0 there.  Such a dword may
+// reach up to 3 bytes past the scales' end or before their start; being aligned
+// it lies within what the memory's page holds.
 #include <algorithm>
 #include <atomic>
 
@@ -12,40 +18,26 @@
 namespace ntops {
 namespace {
 
-constexpr int kTile = 128;                  // rows and columns of an output tile
 constexpr int kStages = 4;
-constexpr int kCodes = 2 * kTile * 128;     // A's rows, then B's
-constexpr int kScales = 2 * kTile * 8;
-constexpr int kStage = kCodes + kScales;
-constexpr int kLds = kStages * kStage;
-constexpr int kLoads = 8 + 2;               // DMA instructions per wave and stage
 
-// out rows m0 .. of one lane's 4 consecutive columns n .. n + 3.
-template <typename T>
-__device__ __forceinline__ void store4(T* d, int64_t ldd, int m, int n, int M, int N, f32x4 v, const T* bias, bool whole) {
-  if (m >= M) return;
-  T* at = d + static_cast<int64_t>(m) * ldd + n;
-  T o[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float b = bias != nullptr && n + e < N ? static_cast<float>(bias[n + e]) : 0.f;
-    o[e] = static_cast<T>(v[e] + b);
-  }
-  if (whole && n + 4 <= N) {
-    if constexpr (sizeof(T) == 2)
-      *reinterpret_cast<u32x2*>(at) = __builtin_bit_cast(u32x2, o);
-    else
-      *reinterpret_cast<u32x4*>(at) = __builtin_bit_cast(u32x4, o);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n + e < N) at[e] = o[e];
-  }
-}
+template <int BT, bool FIT>
+struct TileShape {
+  static constexpr int kRowsPerWave = BT / 4;                  // rows of an operand that a wave loads
+  static constexpr int kCodes = BT * 128;                      // bytes of an operand's codes per stage
+  static constexpr int kDwords = FIT ? 2 : 3;                  // of a row's scales
+  static constexpr int kScaleInst = (kRowsPerWave * kDwords + 63) / 64;
+  static constexpr int kScales = 4 * kScaleInst * 256;         // bytes of an operand's scales
+  static constexpr int kStage = 2 * (kCodes + kScales);
+  static constexpr int kLds = kStages * kStage;
+  static constexpr int kLoads = 2 * (kRowsPerWave / 8 + kScaleInst);  // DMA instructions per wave and stage
+};
 
 // whole: the output's rows are runs that 4 elements at a time can be stored to.
-template <typename T>
-__global__ __launch_bounds__(256, 1) void k_mx4_tile(Mx4Args g, int tm_count, int tn_count, int whole) {
+template <typename T, int BT, bool FIT>
+__global__ __launch_bounds__(256, BT == 64 ? 2 : 1) void k_mx4_tile(Mx4Args g, int tm_count, int tn_count, int whole) {
+  using S = TileShape<BT, FIT>;
+  constexpr int TW = BT / 32;  // 16-row (and column) pieces of a wave's tile
+  constexpr int ND = S::kDwords;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -56,74 +48,108 @@ __global__ __launch_bounds__(256, 1) void k_mx4_tile(Mx4Args g, int tm_count, in
   const int band = t / (8 * tn_count);
   const int rows_here = min(8, tm_count - band * 8);
   const int in = t - band * 8 * tn_count;
-  const int m0 = (band * 8 + in % rows_here) * kTile, n0 = in / rows_here * kTile;
+  const int m0 = (band * 8 + in % rows_here) * BT, n0 = in / rows_here * BT;
   const int slice = blockIdx.y;
   const int kb0 = slice * g.kchunk, kb1 = min(g.kb, kb0 + g.kchunk);
   const int nt = (kb1 - kb0 + 7) / 8;
 
-  const int mv = min(kTile, g.M - m0), nv = min(kTile, g.N - n0);
+  const int mv = min(BT, g.M - m0), nv = min(BT, g.N - n0);
   const u32x4 ra = mx4_rsrc(g.a + m0 * g.lda, (mv - 1) * g.lda + g.kb * 16);
   const u32x4 rb = mx4_rsrc(g.b + n0 * g.ldb, (nv - 1) * g.ldb + g.kb * 16);
-  const int kb4 = (g.kb + 3) & ~3;  // (padded rows: zeros behind their blocks)
-  const u32x4 rsa = mx4_rsrc(g.as + m0 * g.ldas, (mv - 1) * g.ldas + kb4);
-  const u32x4 rsb = mx4_rsrc(g.bs + n0 * g.ldbs, (nv - 1) * g.ldbs + kb4);
+  // scales from the dword on that holds the tile's first byte
+  const uint8_t* sa0 = g.as + m0 * g.ldas;
+  const uint8_t* sb0 = g.bs + n0 * g.ldbs;
+  const int oa = FIT ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(sa0) & 3u);
+  const int ob = FIT ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(sb0) & 3u);
+  const u32x4 rsa = mx4_rsrc(sa0 - oa, (oa + (mv - 1) * g.ldas + g.kb + 3) & ~3ll);
+  const u32x4 rsb = mx4_rsrc(sb0 - ob, (ob + (nv - 1) * g.ldbs + g.kb + 3) & ~3ll);
   const uint32_t smem_addr = lds_addr(smem);
 
-  // this wave's loads of K tile j: rows 32 wave .. + 31 of A and of B (8 rows
-  // an instruction), their scales in one instruction each (row l / 2, dword l % 2)
+  // this wave's loads of K tile j: BT / 4 rows of A and of B (8 rows an
+  // instruction), and their scales (row l / ND, dword l % ND)
   auto issue = [&](int j) {
-    const uint32_t st = smem_addr + static_cast<uint32_t>((j & (kStages - 1)) * kStage);
+    const uint32_t st = smem_addr + static_cast<uint32_t>((j & (kStages - 1)) * S::kStage);
     const int b0 = kb0 + j * 8;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int row = wave * 32 + u * 8 + (lane >> 3);
+    for (int u = 0; u < S::kRowsPerWave / 8; ++u) {
+      const int row = wave * S::kRowsPerWave + u * 8 + (lane >> 3);
       const int blk = b0 + kslot<64>(row, lane & 7);
-      const uint32_t dst = st + static_cast<uint32_t>((wave * 32 + u * 8) * 128);
+      const uint32_t dst = st + static_cast<uint32_t>((wave * S::kRowsPerWave + u * 8) * 128);
       dma16(ra, dst, blk < kb1 && row < mv ? static_cast<uint32_t>(row * g.lda + blk * 16) : kOOB);
-      dma16(rb, dst + kTile * 128, blk < kb1 && row < nv ? static_cast<uint32_t>(row * g.ldb + blk * 16) : kOOB);
+      dma16(rb, dst + S::kCodes, blk < kb1 && row < nv ? static_cast<uint32_t>(row * g.ldb + blk * 16) : kOOB);
     }
-    const int row = wave * 32 + (lane >> 1), blk = b0 + (lane & 1) * 4;
-    const uint32_t dst = st + kCodes + static_cast<uint32_t>(wave * 256);
-    dma4(rsa, dst, blk < kb1 && row < mv ? static_cast<uint32_t>(row * g.ldas + blk) : kOOB);
-    dma4(rsb, dst + kTile * 8, blk < kb1 && row < nv ? static_cast<uint32_t>(row * g.ldbs + blk) : kOOB);
+#pragma unroll
+    for (int u = 0; u < S::kScaleInst; ++u) {
+      const int id = u * 64 + lane;
+      const int in_wave = id / ND, row = wave * S::kRowsPerWave + in_wave;
+      const int blk = b0 + (id - in_wave * ND) * 4;
+      const bool ok = in_wave < S::kRowsPerWave && b0 < kb1;
+      const uint32_t dst = st + 2 * S::kCodes + static_cast<uint32_t>((wave * S::kScaleInst + u) * 256);
+      // (past the row's last dword: the next row's, masked below; past the last row's: zeros)
+      dma4(rsa, dst, ok && row < mv ? static_cast<uint32_t>(oa + row * g.ldas + blk) & ~3u : kOOB);
+      dma4(rsb, dst + S::kScales, ok && row < nv ? static_cast<uint32_t>(ob + row * g.ldbs + blk) & ~3u : kOOB);
+    }
   };
+  // LDS offset of scale byte 0 (K block 2q of a K tile) of row r's area
+  auto scale_at = [&](int r, int o, int64_t ld) {
+    const int w = r / S::kRowsPerWave, in_wave = r - w * S::kRowsPerWave;
+    return w * S::kScaleInst * 256 + in_wave * ND * 4 + (FIT ? 0 : static_cast<int>((o + r * ld) & 3)) + 2 * q;
+  };
+  int sat[TW], sbt[TW];
+#pragma unroll
+  for (int i = 0; i < TW; ++i) {
+    sat[i] = 2 * S::kCodes + scale_at(wm * (BT / 2) + i * 16 + i16, oa, g.ldas);
+    sbt[i] = 2 * S::kCodes + S::kScales + scale_at(wn * (BT / 2) + i * 16 + i16, ob, g.ldbs);
+  }
 
-  f32x4 acc[4][4];
+  f32x4 acc[TW][TW];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < TW; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < TW; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   issue(0);
   issue(1);
   issue(2);
   for (int j = 0; j < nt; ++j) {
     __builtin_amdgcn_sched_barrier(0);
-    wait_vmcnt<2 * kLoads>();  // K tile j is in (past the last tile the loads are empty, but count)
-    block_barrier();           // for every wave; and tile j - 1's stage is free
+    wait_vmcnt<2 * S::kLoads>();  // K tile j is in (past the last tile the loads are empty, but count)
+    block_barrier();              // for every wave; and tile j - 1's stage is free
     asm volatile("" ::: "memory");
     issue(j + 3);
-    const char* st = smem + (j & (kStages - 1)) * kStage;
-    uint32_t sa[4], sb[4];
+    const char* st = smem + (j & (kStages - 1)) * S::kStage;
+    uint32_t sa[TW], sb[TW];
+    if constexpr (FIT) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sa[i] = *reinterpret_cast<const uint16_t*>(st + kCodes + (wm * 64 + i * 16 + i16) * 8 + q * 2);
-      sb[i] = *reinterpret_cast<const uint16_t*>(st + kCodes + (kTile + wn * 64 + i * 16 + i16) * 8 + q * 2);
+      for (int i = 0; i < TW; ++i) {
+        sa[i] = *reinterpret_cast<const uint16_t*>(st + sat[i]);
+        sb[i] = *reinterpret_cast<const uint16_t*>(st + sbt[i]);
+      }
+    } else {
+      const uint32_t left = static_cast<uint32_t>(max(0, kb1 - kb0 - j * 8 - 2 * q));  // blocks from this lane's first on
+      const uint32_t mask = left >= 2 ? 0xffffu : left == 1 ? 0xffu : 0u;
+#pragma unroll
+      for (int i = 0; i < TW; ++i) {
+        const uint8_t* pa = reinterpret_cast<const uint8_t*>(st + sat[i]);
+        const uint8_t* pb = reinterpret_cast<const uint8_t*>(st + sbt[i]);
+        sa[i] = (pa[0] | static_cast<uint32_t>(pa[1]) << 8) & mask;
+        sb[i] = (pb[0] | static_cast<uint32_t>(pb[1]) << 8) & mask;
+      }
     }
     const auto frag = [&](int area, int r, int ks) {
-      return *reinterpret_cast<const u32x4*>(st + area * (kTile * 128) + r * 128 + kslot<64>(r, 2 * q + ks) * 16);
+      return *reinterpret_cast<const u32x4*>(st + area * S::kCodes + r * 128 + kslot<64>(r, 2 * q + ks) * 16);
     };
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      u32x4 fa[4], fb[4];
+      u32x4 fa[TW], fb[TW];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        fa[i] = frag(0, wm * 64 + i * 16 + i16, ks);
-        fb[i] = frag(1, wn * 64 + i * 16 + i16, ks);
+      for (int i = 0; i < TW; ++i) {
+        fa[i] = frag(0, wm * (BT / 2) + i * 16 + i16, ks);
+        fb[i] = frag(1, wn * (BT / 2) + i * 16 + i16, ks);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < TW; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < TW; ++k)
           acc[i][k] = ks == 0 ? mfma_mx4<0, 0>(fb[k], sb[k], fa[i], sa[i], acc[i][k])
                               : mfma_mx4<1, 1>(fb[k], sb[k], fa[i], sa[i], acc[i][k]);
     }
@@ -131,10 +157,10 @@ __global__ __launch_bounds__(256, 1) void k_mx4_tile(Mx4Args g, int tm_count, in
   }
   wait_vmcnt<0>();  // no DMA may land after the workgroup ends
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < TW; ++i)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int m = m0 + wm * 64 + i * 16 + i16, n = n0 + wn * 64 + k * 16 + 4 * q;
+    for (int k = 0; k < TW; ++k) {
+      const int m = m0 + wm * (BT / 2) + i * 16 + i16, n = n0 + wn * (BT / 2) + k * 16 + 4 * q;
       if (g.split > 1)
         store4<float>(g.part + static_cast<int64_t>(slice) * g.M * g.N, g.N, m, n, g.M, g.N, acc[i][k], nullptr, (g.N & 3) == 0);
       else
@@ -155,51 +181,30 @@ __global__ __launch_bounds__(256) void k_mx4_reduce(Mx4Args g) {
   static_cast<T*>(g.d)[m * g.ldd + n] = static_cast<T>(v);
 }
 
-// Scale rows copied to rows of `to_ld` bytes, a multiple of 16, zeros behind
-// their `kb` bytes: blockIdx.y 0 the a rows, 1 the b rows.
-__global__ __launch_bounds__(256) void k_mx4_pad_scales(Mx4Args g, uint8_t* a, uint8_t* b, int to_ld) {
-  const bool second = blockIdx.y != 0;
-  const int rows = second ? g.N : g.M;
-  uint8_t* to = second ? b : a;
-  if (to == nullptr) return;
-  const uint8_t* from = second ? g.bs : g.as;
-  const int64_t ld = second ? g.ldbs : g.ldas;
-  const int words = to_ld / 4;
-  const int64_t total = static_cast<int64_t>(rows) * words;
-  for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t row = i / words;
-    const int c = static_cast<int>(i - row * words) * 4;
-    uint32_t w = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (c + e < g.kb) w |= static_cast<uint32_t>(from[row * ld + c + e]) << (8 * e);
-    *reinterpret_cast<uint32_t*>(to + row * to_ld + c) = w;
-  }
-}
+constexpr int64_t kMaxSize = int64_t(1) << 30;
 
-int64_t round16(int64_t n) { return (n + 15) & ~int64_t(15); }
-
-// Whether the kernels can read these scale rows as they are: whole groups of 8
-// blocks (what follows a row's last block would count as a scale, and 255 is
-// NaN), dwords aligned.
+// Whether K tiles of 8 blocks are whole dwords of these scale rows.
 bool scales_fit(int64_t kb, const void* s, int64_t ld) {
   return kb % 8 == 0 && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(s) & 3u) == 0;
 }
 
-// Slices of K: as many as bring the blocks near the number of CUs, none under
-// four K tiles.
-void split_k(int64_t M, int64_t N, int64_t kb, int& split, int& kchunk) {
-  const int64_t tiles = ceil_div(M, kTile) * ceil_div(N, kTile);
+// The tile's size, and slices of K: as many as bring the blocks near the number
+// of CUs, none under four K tiles.
+void plan(int64_t M, int64_t N, int64_t kb, int& bt, int& split, int& kchunk) {
+  const int64_t cus = cu_count_cached();
+  const auto tiles = [&](int64_t t) { return ceil_div(M, t) * ceil_div(N, t); };
+  bt = tiles(128) >= cus ? 128 : 64;
   const int64_t kt = ceil_div(kb, 8);
-  int64_t s = std::max<int64_t>(1, std::min<int64_t>({cu_count_cached() / tiles, kt / 4, 16}));
+  int64_t s = std::max<int64_t>(1, std::min<int64_t>({cus / tiles(bt), kt / 4, 16}));
   const int64_t per = ceil_div(kt, s);
   kchunk = static_cast<int>(per * 8);
   split = static_cast<int>(ceil_div(kt, per));
 }
 
-template <typename T>
-int run_tile(const Mx4Args& g, hipStream_t st) {
-  auto kern = k_mx4_tile<T>;
+template <typename T, int BT, bool FIT>
+int launch_tile(const Mx4Args& g, hipStream_t st) {
+  auto kern = k_mx4_tile<T, BT, FIT>;
+  constexpr int kLds = TileShape<BT, FIT>::kLds;
   static std::atomic<bool> attr_set{false};  // (threads may get here together)
   if (!attr_set.load(std::memory_order_relaxed)) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) !=
@@ -207,9 +212,9 @@ int run_tile(const Mx4Args& g, hipStream_t st) {
       return set_error(NTOPS_ERR_HIP, "mxfp4_mm: cannot reserve %d bytes of LDS", kLds);
     attr_set.store(true, std::memory_order_relaxed);
   }
-  const int tm = static_cast<int>(ceil_div(g.M, kTile)), tn = static_cast<int>(ceil_div(g.N, kTile));
+  const int tm = static_cast<int>(ceil_div(g.M, BT)), tn = static_cast<int>(ceil_div(g.N, BT));
   const int whole = (g.ldd & 3) == 0 && (reinterpret_cast<uintptr_t>(g.d) & (4 * sizeof(T) - 1)) == 0;
-  note_kernel("mxfp4_tile split%d", g.split);
+  note_kernel("mxfp4_tile%d split%d%s", BT, g.split, FIT ? "" : " bytes");
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(tm * tn), static_cast<unsigned>(g.split)), dim3(256), kLds, st, g,
                      tm, tn, whole);
   if (g.split > 1)
@@ -217,22 +222,24 @@ int run_tile(const Mx4Args& g, hipStream_t st) {
   return check_launch("mxfp4_mm");
 }
 
+template <typename T>
+int run_tile(const Mx4Args& g, int bt, hipStream_t st) {
+  const bool fit = scales_fit(g.kb, g.as, g.ldas) && scales_fit(g.kb, g.bs, g.ldbs);
+  if (bt == 128) return fit ? launch_tile<T, 128, true>(g, st) : launch_tile<T, 128, false>(g, st);
+  return fit ? launch_tile<T, 64, true>(g, st) : launch_tile<T, 64, false>(g, st);
+}
+
 }  // namespace
 }  // namespace ntops
 
 using namespace ntops;
 
-extern "C" int64_t ntops_mxfp4_mm_workspace(int64_t M, int64_t N, int64_t K, const void* a_scales, int64_t as_row_stride,
-                                            const void* b_scales, int64_t bs_row_stride) {
-  if (M <= 0 || N <= 0 || K <= 0 || M > 0x7fffffff || N > 0x7fffffff || K > 0x7fffffff) return 0;
-  const int64_t kb = ceil_div(K, 32);
-  int split, kchunk;
-  split_k(M, N, kb, split, kchunk);
-  int64_t bytes = split > 1 ? split * M * N * 4 : 0;
-  bytes = round16(bytes);
-  if (!scales_fit(kb, a_scales, as_row_stride)) bytes += M * round16(kb);
-  if (!scales_fit(kb, b_scales, bs_row_stride)) bytes += N * round16(kb);
-  return bytes;
+extern "C" int64_t ntops_mxfp4_mm_workspace(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0 || M > kMaxSize || N > kMaxSize || K > kMaxSize) return 0;
+  if (M <= kSkinnyRows) return 0;
+  int bt, split, kchunk;
+  plan(M, N, ceil_div(K, 32), bt, split, kchunk);
+  return split > 1 ? split * M * N * 4 : 0;
 }
 
 extern "C" int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K, const void* a, int64_t a_row_stride,
@@ -250,11 +257,11 @@ extern "C" int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K, co
     return set_error(NTOPS_ERR_INVALID, "mxfp4_mm: code rows not aligned to 16 bytes");
   if (a_row_stride < 0 || b_row_stride < 0 || as_row_stride < 0 || bs_row_stride < 0)
     return set_error(NTOPS_ERR_INVALID, "mxfp4_mm: negative row stride");
-  const int64_t lim = int64_t(1) << 30;
+  const int64_t lim = kMaxSize;
   const auto span = [&](int64_t ld, int64_t row) { return 256 * ld + row; };  // bytes that one tile's rows cover
   if (M > lim || N > lim || kb * 16 > lim || span(a_row_stride, kb * 16) > lim || span(b_row_stride, kb * 16) > lim ||
       span(as_row_stride, kb) > lim || span(bs_row_stride, kb) > lim ||
-      ceil_div(M, kTile) * ceil_div(N, kTile) > 0x7fffff)
+      ceil_div(M, 64) * ceil_div(N, 64) > 0x7fffff)
     return set_error(NTOPS_ERR_UNSUPPORTED, "mxfp4_mm: operands too large");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   Mx4Args g{};
@@ -272,39 +279,18 @@ extern "C" int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K, co
   g.M = static_cast<int>(M);
   g.N = static_cast<int>(N);
   g.kb = static_cast<int>(kb);
-  const bool pad_a = kb > 0 && !scales_fit(kb, a_scales, as_row_stride);
-  const bool pad_b = kb > 0 && !scales_fit(kb, b_scales, bs_row_stride);
-  split_k(M, N, std::max<int64_t>(kb, 1), g.split, g.kchunk);
-  const int64_t part_bytes = g.split > 1 ? round16(g.split * M * N * 4) : 0;
-  const int64_t ld = round16(kb);
-  const int64_t pad_bytes = (pad_a ? M * ld : 0) + (pad_b ? N * ld : 0);
   if (workspace_bytes < 0 || (workspace != nullptr && !aligned16(workspace)))
     return set_error(NTOPS_ERR_INVALID, "mxfp4_mm: workspace not aligned to 16 bytes");
-  if (pad_bytes > 0 && (workspace == nullptr || workspace_bytes < pad_bytes))
-    return set_error(NTOPS_ERR_INVALID, "mxfp4_mm: these scale rows need %lld bytes of workspace",
-                     static_cast<long long>(pad_bytes));
-  if (g.split > 1 && (workspace == nullptr || workspace_bytes < part_bytes + pad_bytes)) {
-    g.split = 1;
-    g.kchunk = std::max(8, g.kb);
-  } else if (g.split > 1) {
+  return dispatch_float16_32(out_dtype, "mxfp4_mm", [&](auto tag) -> int {
+    using T = decltype(tag);
+    if (M <= kSkinnyRows && kb > 0) return mx4_skinny(out_dtype, g, st);
+    int bt;
+    plan(M, N, std::max<int64_t>(kb, 1), bt, g.split, g.kchunk);
+    if (g.split > 1 && (workspace == nullptr || workspace_bytes < g.split * M * N * 4)) {
+      g.split = 1;
+      g.kchunk = (g.kb + 7) / 8 * 8;
+    }
     g.part = static_cast<float*>(workspace);
-  }
-  if (pad_bytes > 0) {
-    uint8_t* at = static_cast<uint8_t*>(workspace) + (g.split > 1 ? part_bytes : 0);
-    uint8_t* pa = pad_a ? at : nullptr;
-    uint8_t* pb = pad_b ? at + (pad_a ? M * ld : 0) : nullptr;
-    const int64_t words = std::max(pad_a ? M : 0, pad_b ? N : 0) * (ld / 4);
-    const int64_t blocks = std::min<int64_t>(ceil_div(words, 256), 4096);
-    hipLaunchKernelGGL(k_mx4_pad_scales, dim3(static_cast<unsigned>(blocks), 2), dim3(256), 0, st, g, pa, pb,
-                       static_cast<int>(ld));
-    if (pad_a) {
-      g.as = pa;
-      g.ldas = ld;
-    }
-    if (pad_b) {
-      g.bs = pb;
-      g.ldbs = ld;
-    }
-  }
-  return dispatch_float16_32(out_dtype, "mxfp4_mm", [&](auto tag) { return run_tile<decltype(tag)>(g, st); });
+    return run_tile<T>(g, bt, st);
+  });
 }

@@ -1,0 +1,224 @@
+// MXFP4 products of up to 16 rows (decode projections): bound by streaming B,
+// (16 + 1) / 32 bytes a value, once.
+//
+// A block covers 16 J columns; its four waves each own K steps of their own and
+// stream them through their own part of the LDS by direct DMA, two or three steps
+// ahead, with no barrier before their fp32 sums are merged.  A step is 8 KiB of B
+// (16 J rows of 512 / J bytes, non-temporal, whole lines), the same columns of
+// A's 16 rows, and the scales.
+//
+// A lane takes CPR / 4 neighbouring blocks of its row, one per instruction, so
+// that it needs CPR / 4 neighbouring bytes of the row's scales.  Those are loaded
+// as the dwords that the step's CPR bytes lie in (one more than they fill, as a
+// row may start inside one) and shifted into place; bytes behind the row's last
+// block become 0, as they may be another row's 255.  Such a dword may reach up to
+// 3 bytes past the scales' end or before their start; being aligned it lies
+// within what the memory's page holds.
+#include <atomic>
+
+#include "gemm_mxfp4.h"
+
+namespace ntops {
+namespace {
+
+constexpr int kWaves = 4;
+
+// 16-byte slot of chunk c of row r, CPR chunks a row: the 16 rows of a fragment
+// read touch 16 different slots of the LDS's 256 bytes.
+template <int CPR>
+__device__ __forceinline__ int sk_slot(int r, int c) {
+  return c ^ (r & 15);
+}
+
+template <bool NT>
+__device__ __forceinline__ void sk_dma(u32x4 rsrc, uint32_t dst, uint32_t off) {
+  if constexpr (NT)
+    asm volatile("buffer_load_dwordx4 %0, %1, 0 offen nt lds" : : "v"(off), "s"(rsrc), "{m0}"(dst) : "memory");
+  else
+    dma16(rsrc, dst, off);
+}
+
+// One operand's steps: ROWS rows of CPR blocks, and their scales.
+template <int ROWS, int CPR, bool NT>
+struct Loader {
+  static constexpr int kInst = ROWS * CPR / 64;
+  static constexpr int kRpi = 64 / CPR;  // rows per instruction
+  static constexpr int ND = CPR / 4 + 1;  // dwords of a row's scales
+  static constexpr int kScaleInst = (ROWS * ND + 63) / 64;
+  static constexpr int kBytes = ROWS * CPR * 16, kScaleBytes = kScaleInst * 256;
+  u32x4 codes, scales;
+  uint32_t voff[kInst], soff[kScaleInst];
+  int kb;
+
+  __device__ __forceinline__ static int chunk(int lane, int i) {
+    return sk_slot<CPR>(i * kRpi + lane / CPR, lane % CPR);
+  }
+  // rows: valid ones
+  __device__ __forceinline__ void init(const uint8_t* c, int64_t ld, const uint8_t* s, int64_t lds, int rows, int blocks,
+                                       int lane) {
+    kb = blocks;
+    codes = mx4_rsrc(c, (rows - 1) * ld + blocks * 16ll);
+    const int o = static_cast<int>(reinterpret_cast<uintptr_t>(s) & 3u);
+    scales = mx4_rsrc(s - o, (o + (rows - 1) * lds + blocks + 3) & ~3ll);
+#pragma unroll
+    for (int i = 0; i < kInst; ++i) {
+      const int r = i * kRpi + lane / CPR;
+      voff[i] = r < rows ? static_cast<uint32_t>(r * ld + chunk(lane, i) * 16) : kOOB;
+    }
+#pragma unroll
+    for (int i = 0; i < kScaleInst; ++i) {
+      const int id = i * 64 + lane, r = id / ND;
+      soff[i] = r < rows && r < ROWS ? (static_cast<uint32_t>(o + r * lds) & ~3u) + (id - r * ND) * 4 : kOOB;
+    }
+  }
+  __device__ __forceinline__ void issue(uint32_t dst, int b0, bool valid, int lane) const {
+#pragma unroll
+    for (int i = 0; i < kInst; ++i)
+      sk_dma<NT>(codes, dst + i * 1024,
+                 valid && voff[i] != kOOB && b0 + chunk(lane, i) < kb ? voff[i] + static_cast<uint32_t>(b0) * 16 : kOOB);
+#pragma unroll
+    for (int i = 0; i < kScaleInst; ++i)
+      dma4(scales, dst + kBytes + i * 256, valid && soff[i] != kOOB ? soff[i] + static_cast<uint32_t>(b0) : kOOB);
+  }
+};
+
+template <typename T, int J>
+__global__ __launch_bounds__(64 * kWaves, 1) void k_mx4_skinny(Mx4Args g, int whole) {
+  constexpr int CPR = 32 / J;        // blocks of a row per step
+  constexpr int S = J == 1 ? 2 : 3;  // steps in the ring
+  constexpr int NB = CPR / 4;        // blocks of a lane, and bytes of its scales (8 or 4)
+  using LA = Loader<16, CPR, false>;
+  using LB = Loader<16 * J, CPR, true>;
+  constexpr int kStepA = LA::kBytes + LA::kScaleBytes, kStepB = LB::kBytes + LB::kScaleBytes;
+  constexpr int kStep = kStepA + kStepB;
+  constexpr int kInst = LA::kInst + LA::kScaleInst + LB::kInst + LB::kScaleInst;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * (16 * J);
+  const int nv = min(16 * J, g.N - n0);
+  const int i16 = lane & 15, q = lane >> 4;
+
+  LA la;
+  LB lb;
+  la.init(g.a, g.lda, g.as, g.ldas, g.M, g.kb, lane);
+  lb.init(g.b + n0 * g.ldb, g.ldb, g.bs + n0 * g.ldbs, g.ldbs, nv, g.kb, lane);
+  const int steps = (g.kb + CPR - 1) / CPR;
+  const int n = steps > wave ? (steps - wave + kWaves - 1) / kWaves : 0;  // this wave's: wave, wave + kWaves, ..
+  char* mine = smem + wave * (S * kStep);
+  const uint32_t mine_addr = lds_addr(mine);
+  int slot_in = 0;
+  // step j of this wave into ring slot j % S (past the end: empty loads, so that the waits count the same)
+  auto issue = [&](int j) {
+    const int b0 = (wave + j * kWaves) * CPR;
+    const uint32_t dst = mine_addr + slot_in * kStep;
+    lb.issue(dst, b0, j < n, lane);
+    la.issue(dst + kStepB, b0, j < n, lane);
+    slot_in = slot_in + 1 == S ? 0 : slot_in + 1;
+  };
+  // bits that this lane's scales are shifted by
+  const uint32_t sha = (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(g.as) + i16 * g.ldas) & 3u) * 8;
+  uint32_t shb[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+    shb[j] = (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(g.bs) + (n0 + j * 16 + i16) * g.ldbs) & 3u) * 8;
+  // the lane's NB scale bytes of row r
+  auto scales = [&](const char* at, int r, uint32_t shift, int left, uint32_t (&o)[NB / 4]) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(at) + r * LB::ND + q * (NB / 4);
+#pragma unroll
+    for (int u = 0; u < NB / 4; ++u) {
+      o[u] = __builtin_amdgcn_alignbit(w[u + 1], w[u], shift);
+      const int valid = left - 4 * u;  // blocks of this word
+      if (valid < 4) o[u] &= valid <= 0 ? 0u : (1u << (8 * valid)) - 1;
+    }
+  };
+  f32x4 acc[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < S; ++s) issue(s);
+  int slot = 0;
+  for (int i = 0; i < n; ++i) {
+    __builtin_amdgcn_sched_barrier(0);
+    wait_vmcnt<(S - 1) * kInst>();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    const char* tb = mine + slot * kStep;
+    const char* ta = tb + kStepB;
+    const int left = g.kb - (wave + i * kWaves) * CPR - q * NB;  // blocks from this lane's first on
+    uint32_t sa[NB / 4], sb[J][NB / 4];
+    scales(ta + LA::kBytes, i16, sha, left, sa);
+#pragma unroll
+    for (int j = 0; j < J; ++j) scales(tb + LB::kBytes, j * 16 + i16, shb[j], left, sb[j]);
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      const int c = q * NB + u;
+      const u32x4 a = *reinterpret_cast<const u32x4*>(ta + i16 * (CPR * 16) + sk_slot<CPR>(i16, c) * 16);
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int r = j * 16 + i16;
+        const u32x4 b = *reinterpret_cast<const u32x4*>(tb + r * (CPR * 16) + sk_slot<CPR>(r, c) * 16);
+        switch (u & 3) {
+          case 0: acc[j] = mfma_mx4<0, 0>(b, sb[j][u >> 2], a, sa[u >> 2], acc[j]); break;
+          case 1: acc[j] = mfma_mx4<1, 1>(b, sb[j][u >> 2], a, sa[u >> 2], acc[j]); break;
+          case 2: acc[j] = mfma_mx4<2, 2>(b, sb[j][u >> 2], a, sa[u >> 2], acc[j]); break;
+          default: acc[j] = mfma_mx4<3, 3>(b, sb[j][u >> 2], a, sa[u >> 2], acc[j]); break;
+        }
+      }
+    }
+    wait_lgkmcnt0();
+    issue(i + S);
+    slot = slot + 1 == S ? 0 : slot + 1;
+  }
+  wait_vmcnt<0>();  // no DMA may land in the LDS the merge reuses
+  __syncthreads();
+  // lane l holds row l & 15, columns 16 j + 4 (l >> 4) .. + 3
+  f32x4* red = reinterpret_cast<f32x4*>(smem);  // [wave][j][lane]
+#pragma unroll
+  for (int j = 0; j < J; ++j) red[(wave * J + j) * 64 + lane] = acc[j];
+  __syncthreads();
+  if (wave < J) {
+    f32x4 v = red[wave * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) {
+      const f32x4 x = red[(w * J + wave) * 64 + lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += x[e];
+    }
+    store4<T>(static_cast<T*>(g.d), g.ldd, i16, n0 + wave * 16 + 4 * q, g.M, g.N, v, static_cast<const T*>(g.bias), whole != 0);
+  }
+}
+
+template <typename T, int J>
+int launch_skinny(const Mx4Args& g, hipStream_t st) {
+  constexpr int CPR = 32 / J;
+  using LA = Loader<16, CPR, false>;
+  using LB = Loader<16 * J, CPR, true>;
+  constexpr int kLds = kWaves * (J == 1 ? 2 : 3) * (LA::kBytes + LA::kScaleBytes + LB::kBytes + LB::kScaleBytes);
+  static_assert(kLds <= 163840, "LDS");
+  auto kern = k_mx4_skinny<T, J>;
+  static std::atomic<bool> attr_set{false};  // (threads may get here together)
+  if (!attr_set.load(std::memory_order_relaxed)) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) !=
+        hipSuccess)
+      return set_error(NTOPS_ERR_HIP, "mxfp4_mm: cannot reserve %d bytes of LDS", kLds);
+    attr_set.store(true, std::memory_order_relaxed);
+  }
+  const int whole = (g.ldd & 3) == 0 && (reinterpret_cast<uintptr_t>(g.d) & (4 * sizeof(T) - 1)) == 0;
+  note_kernel("mxfp4_skinny j%d", J);
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((g.N + 16 * J - 1) / (16 * J))), dim3(64 * kWaves), kLds, st, g, whole);
+  return check_launch("mxfp4_mm");
+}
+
+}  // namespace
+
+int mx4_skinny(int out_dtype, const Mx4Args& g, hipStream_t st) {
+  // 32 columns a block from a block per CU on
+  const bool wide = g.N >= 32 * cu_count_cached();
+  return dispatch_float16_32(out_dtype, "mxfp4_mm", [&](auto tag) {
+    using T = decltype(tag);
+    return wide ? launch_skinny<T, 2>(g, st) : launch_skinny<T, 1>(g, st);
+  });
+}
+
+}  // namespace ntops

@@ -48,7 +48,7 @@ def mxfp4_mm(input, input_scale, mat2, mat2_scale, bias=None, *, dtype=torch.bfl
         sa, sb = (s if s.stride(1) == 1 and s.stride(0) >= 0 else _contiguous(s) for s in (input_scale, mat2_scale))
         bias = None if bias is None else _contiguous(bias)
         scales = (sa.data_ptr(), sa.stride(0)), (sb.data_ptr(), sb.stride(0))
-        ws_bytes = lib.ntops_mxfp4_mm_workspace(m, n, 32 * blocks, *scales[0], *scales[1])
+        ws_bytes = lib.ntops_mxfp4_mm_workspace(m, n, 32 * blocks)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
         rc = lib.ntops_mxfp4_mm(
             _lib.dtype_code(dtype), m, n, 32 * blocks, a.data_ptr(), a.stride(0), *scales[0], b.data_ptr(), b.stride(0),

@@ -97,6 +97,5 @@ def test_c_entry_points_refuse():
     assert _mm(lib, ldas=-4) == 1 and "negative" in err()
     assert _mm(lib, out=None) == 1 and "null" in err()
     assert _mm(lib, k=1 << 40, lda=1 << 35, ldb=1 << 35) == 2 and "too large" in err()
-    # scale rows of 2 bytes need a workspace
-    assert _mm(lib) == 1 and "workspace" in err()
+    assert _mm(lib, ws=264) == 1 and "workspace" in err()
     assert _mm(lib, m=0) == 0 and lib.ntops_quantize_mxfp4(_lib.BF16, 0, 32, None, 32, None, None, None) == 0
