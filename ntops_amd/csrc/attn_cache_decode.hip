@@ -58,21 +58,6 @@ __device__ __forceinline__ void dma16_nt(u32x4 rsrc, uint32_t lds_dst, uint32_t 
                : "v"(voffset), "s"(rsrc), "{m0}"(lds_dst)
                : "memory");
 }
-__device__ __forceinline__ void dma4(u32x4 rsrc, uint32_t lds_dst, uint32_t voffset) {
-  asm volatile("buffer_load_dword %0, %1, 0 offen lds"
-               :
-               : "v"(voffset), "s"(rsrc), "{m0}"(lds_dst)
-               : "memory");
-}
-__device__ __forceinline__ u32x4 make_rsrc(const void* base, uint32_t bytes) {
-  const uint64_t addr = reinterpret_cast<uint64_t>(base);
-  u32x4 r;
-  r.x = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(addr));
-  r.y = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(addr >> 32) & 0xffffu);
-  r.z = __builtin_amdgcn_readfirstlane(bytes);
-  r.w = 0x00020000u;
-  return r;
-}
 
 // Loads of a tile's key (or value) rows, 8 instructions of 1 KiB, and of the
 // scales of its 16-token parts, one instruction.

@@ -41,25 +41,18 @@
 #include <atomic>
 
 #include "gemm.h"
+#include "gemm_halves.h"
 #include "gemm_tile.h"
 
 namespace ntops {
 namespace {
 
-constexpr int kHalf = 128 * 64 * 2;      // bytes of a half tile: 128 rows / columns x 64 k
 // LDS: half h of the K tile in buffer b at (2 b + h) * kHalf of A's area, and
 // of B's: every fragment read is one per-lane base plus an immediate.
 constexpr int kAreaB = 4 * kHalf;
 constexpr int kStageOff = 8 * kHalf;             // per wave: 16 rows x 64 rounded outputs
 constexpr int kBiasOff = kStageOff + 8 * 2048;   // per wave: the tile's 2 x 64 columns of a bias row
 constexpr int kLargeLds = kBiasOff + 8 * 256;
-
-// The lane id through an empty asm: what is computed from it is computed where
-// it is used, not hoisted out of the tile loops to sit in registers.
-__device__ __forceinline__ int here(int lane) {
-  asm volatile("" : "+v"(lane));
-  return lane;
-}
 
 // v_mfma_f32_16x16x32: lane l holds row / column l & 15 at k = 8 (l >> 4) ..
 // + 7 of A / B; of the result column l & 15 and rows 4 (l >> 4) .. + 3.
@@ -118,50 +111,6 @@ struct FragReader {
   }
 };
 
-// Loads of an operand's half tiles: 2 instructions of 1 KiB per wave.
-template <bool KMAJ>
-struct HalfLoader {
-  uint32_t voff[2];
-  uint32_t kbytes;   // byte distance of consecutive k
-  uint32_t lds_off;  // of this wave's first instruction
-
-  __device__ __forceinline__ static int lane_k(int wave, int lane, int i) {
-    const int q = wave * 2 + i;
-    if constexpr (KMAJ) {
-      const int row = q * 8 + lane / 8;
-      return kslot<64>(row, lane % 8) * 8;
-    } else {
-      return q * 4 + lane / 16;
-    }
-  }
-  __device__ __forceinline__ void init(int64_t ld, int wave, int lane) {
-    lds_off = static_cast<uint32_t>(wave * 2048);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int q = wave * 2 + i;
-      if constexpr (KMAJ)
-        voff[i] = static_cast<uint32_t>((q * 8 + lane / 8) * ld * 2 + lane_k(wave, lane, i) * 2);
-      else
-        voff[i] = static_cast<uint32_t>((q * 4 + lane / 16) * ld * 2 + mnslot(q * 4 + lane / 16, lane % 16) * 16);
-    }
-    kbytes = static_cast<uint32_t>(KMAJ ? 2 : ld * 2);
-  }
-  // TAIL: the K tile at k0 may reach past K; its chunks there read as zero.
-  template <bool TAIL>
-  __device__ __forceinline__ void issue(u32x4 rsrc, uint32_t lds, int k0, int K, int wave, int lane) const {
-    // (opaque, so that no sum of a fixed tile's is kept in a register)
-    uint32_t koff = static_cast<uint32_t>(k0) * kbytes;
-    asm volatile("" : "+s"(koff));
-    const int l = TAIL ? here(lane) : 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t off = voff[i] + koff;
-      if constexpr (TAIL) off = k0 + lane_k(wave, l, i) < K ? off : kOOB;
-      dma16(rsrc, lds + lds_off + i * 1024, off);
-    }
-  }
-};
-
 // The same for a channels-last convolution's pixels (see GemmArgs): a K tile
 // is one 64-channel block under one tap, a row one output pixel.
 struct PixelLoader {
@@ -201,16 +150,6 @@ struct PixelLoader {
   }
 };
 
-__device__ __forceinline__ u32x4 make_rsrc(const void* base, int64_t bytes) {
-  const uint64_t addr = reinterpret_cast<uint64_t>(base);
-  u32x4 r;
-  r.x = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(addr));
-  r.y = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(addr >> 32) & 0xffffu);
-  r.z = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(bytes));
-  r.w = 0x00020000u;
-  return r;
-}
-
 // Resources of an output tile's operand halves (what lies past an edge reads
 // as zero, or as some other row's or column's data: such rows and columns of
 // the product are never stored); a convolution's pixel offsets.
@@ -219,11 +158,6 @@ struct TileRsrc {
   u32x4 a[2], b[2];
   uint32_t pix[CONV ? 2 : 1][2];  // [column half][instruction]
 };
-
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-  wait_vmcnt<(N < 63 ? N : 63)>();
-}
 
 // CONV: B is the channels-last convolution operand, the bias a value per row.
 template <typename T, bool AK, bool BKM, bool BIAS, bool CONV = false>

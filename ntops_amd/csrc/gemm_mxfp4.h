@@ -39,24 +39,6 @@ __device__ __forceinline__ f32x4 mfma_mx4(u32x4 a, uint32_t sa, u32x4 b, uint32_
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, SA, static_cast<int>(sa), SB, static_cast<int>(sb));
 }
 
-__device__ __forceinline__ u32x4 mx4_rsrc(const void* base, int64_t bytes) {
-  const uint64_t addr = reinterpret_cast<uint64_t>(base);
-  u32x4 r;
-  r.x = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(addr));
-  r.y = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(addr >> 32) & 0xffffu);
-  r.z = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(bytes));
-  r.w = 0x00020000u;
-  return r;
-}
-
-// 4-byte global -> LDS copy per lane: lane l's dword lands at lds_dst + 4 l.
-__device__ __forceinline__ void dma4(u32x4 rsrc, uint32_t lds_dst, uint32_t voffset) {
-  asm volatile("buffer_load_dword %0, %1, 0 offen lds"
-               :
-               : "v"(voffset), "s"(rsrc), "{m0}"(lds_dst)
-               : "memory");
-}
-
 // A lane's 4 consecutive columns n .. n + 3 of row m, rounded; whole: the output's
 // rows are runs that 4 elements at a time can be stored to.
 template <typename T>
@@ -80,6 +62,11 @@ __device__ __forceinline__ void store4(T* d, int64_t ldd, int m, int n, int M, i
       if (n + e < N) at[e] = o[e];
   }
 }
+
+// 16-bit out on 256 x 256 tiles: more than 32 blocks of K, in whole K tiles of 8,
+// and scale rows of whole dwords.
+bool mx4_large_serves(int out_dtype, const Mx4Args& g);
+int mx4_large(int out_dtype, const Mx4Args& g, hipStream_t st);
 
 constexpr int kSkinnyRows = 16;
 // out for M <= kSkinnyRows, bound by streaming B.

@@ -54,15 +54,15 @@ __global__ __launch_bounds__(256, BT == 64 ? 2 : 1) void k_mx4_tile(Mx4Args g, i
   const int nt = (kb1 - kb0 + 7) / 8;
 
   const int mv = min(BT, g.M - m0), nv = min(BT, g.N - n0);
-  const u32x4 ra = mx4_rsrc(g.a + m0 * g.lda, (mv - 1) * g.lda + g.kb * 16);
-  const u32x4 rb = mx4_rsrc(g.b + n0 * g.ldb, (nv - 1) * g.ldb + g.kb * 16);
+  const u32x4 ra = make_rsrc(g.a + m0 * g.lda, (mv - 1) * g.lda + g.kb * 16);
+  const u32x4 rb = make_rsrc(g.b + n0 * g.ldb, (nv - 1) * g.ldb + g.kb * 16);
   // scales from the dword on that holds the tile's first byte
   const uint8_t* sa0 = g.as + m0 * g.ldas;
   const uint8_t* sb0 = g.bs + n0 * g.ldbs;
   const int oa = FIT ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(sa0) & 3u);
   const int ob = FIT ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(sb0) & 3u);
-  const u32x4 rsa = mx4_rsrc(sa0 - oa, (oa + (mv - 1) * g.ldas + g.kb + 3) & ~3ll);
-  const u32x4 rsb = mx4_rsrc(sb0 - ob, (ob + (nv - 1) * g.ldbs + g.kb + 3) & ~3ll);
+  const u32x4 rsa = make_rsrc(sa0 - oa, (oa + (mv - 1) * g.ldas + g.kb + 3) & ~3ll);
+  const u32x4 rsb = make_rsrc(sb0 - ob, (ob + (nv - 1) * g.ldbs + g.kb + 3) & ~3ll);
   const uint32_t smem_addr = lds_addr(smem);
 
   // this wave's loads of K tile j: BT / 4 rows of A and of B (8 rows an
@@ -188,6 +188,9 @@ bool scales_fit(int64_t kb, const void* s, int64_t ld) {
   return kb % 8 == 0 && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(s) & 3u) == 0;
 }
 
+// 256 x 256 tiles for about a round of the GPU or more.
+bool large_suits(int64_t M, int64_t N) { return ceil_div(M, 256) * ceil_div(N, 256) >= cu_count_cached() / 2; }
+
 // The tile's size, and slices of K: as many as bring the blocks near the number
 // of CUs, none under four K tiles.
 void plan(int64_t M, int64_t N, int64_t kb, int& bt, int& split, int& kchunk) {
@@ -284,6 +287,7 @@ extern "C" int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K, co
   return dispatch_float16_32(out_dtype, "mxfp4_mm", [&](auto tag) -> int {
     using T = decltype(tag);
     if (M <= kSkinnyRows && kb > 0) return mx4_skinny(out_dtype, g, st);
+    if (large_suits(M, N) && mx4_large_serves(out_dtype, g)) return mx4_large(out_dtype, g, st);
     int bt;
     plan(M, N, std::max<int64_t>(kb, 1), bt, g.split, g.kchunk);
     if (g.split > 1 && (workspace == nullptr || workspace_bytes < g.split * M * N * 4)) {

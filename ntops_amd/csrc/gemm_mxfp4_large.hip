@@ -1,0 +1,457 @@
+// Large MXFP4 products: out (16 bits) = A B^T (+ a bias row).
+//
+// The persistent 256 x 256 schedule of gemm_large.hip: 4-bit data has the same
+// bytes per fragment and per matrix instruction cycle as 16-bit data, so a K tile
+// is again 128 bytes a row (256 values) in four half tiles (A0, A1, B0, B1) that
+// are refilled one by one, the two waves of a SIMD half a phase apart, and a
+// finished quadrant leaves between the next tile's MFMAs.  K is a quarter as many
+// tiles as for 16 bits, so what surrounds the K loop weighs four times as much.
+//
+// Scales, a byte per 32 values, ride along: 8 bytes a row and K tile, two DMA
+// instructions of dwords per wave, into a ring of three K tiles.  A phase reads
+// those of its rows' blocks (k-step ks of lane group g: block 2 g + ks), two 16-row
+// slices to a register; 12 registers that held a pair of K tiles' scales cost 209
+// spilled ones.
+#include <algorithm>
+#include <atomic>
+
+#include "gemm_halves.h"
+#include "gemm_mxfp4.h"
+
+namespace ntops {
+namespace {
+
+// LDS: half h of the K tile in buffer b at (2 b + h) * kHalf of A's area, and of
+// B's; per wave 16 rows x 64 rounded outputs, and 2 x 64 columns of the bias; three
+// K tiles' scales, 256 rows of A and 256 of B each.
+constexpr int kAreaB = 4 * kHalf;
+constexpr int kStageOff = 8 * kHalf;
+constexpr int kBiasOff = kStageOff + 8 * 2048;
+constexpr int kScaleOff = kBiasOff + 8 * 256;
+constexpr int kScales = 512 * 8;
+constexpr int kLds = kScaleOff + 3 * kScales;
+static_assert(kLds <= 163840, "LDS");
+
+typedef __attribute__((address_space(3))) const u32x4 lds_cu32x4_t;
+typedef __attribute__((address_space(3))) const u32x2 lds_cu32x2_t;
+typedef __attribute__((address_space(3))) u32x2 lds_u32x2_t;
+typedef __attribute__((address_space(3))) const uint16_t lds_cu16_t;
+
+// Resources of an output tile's operand halves and of this wave's 64 scale rows
+// (what lies past an edge reads as zero).
+struct TileRsrc {
+  u32x4 a[2], b[2], s;
+};
+
+template <typename T, bool BIAS>
+__global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 1, wn = wave & 1;  // 32 rows of a half, 64 columns of a half
+  const int grp = wave >> 2;
+  const int tm_count = (g.M + 255) / 256, tn_count = (g.N + 255) / 256;
+  const int np = (g.kb + 15) / 16;  // pairs of K tiles
+  const int K = g.kb * 8;    // in 16-bit units, as the loaders count
+
+  // tile `i` of this block: (row, column) or false past the end
+  const int nx = (gridDim.x & 7) == 0 ? 8 : 1;
+  const int per_x = (total + nx - 1) / nx;
+  auto tile_at = [&](int i, int& m0, int& n0) __attribute__((always_inline)) {
+    const int x = static_cast<int>(blockIdx.x) % nx;
+    const int pos = i * (static_cast<int>(gridDim.x) / nx) + static_cast<int>(blockIdx.x) / nx;
+    const int t = x * per_x + pos;
+    if (pos >= per_x || t >= total) return false;
+    constexpr int kGroupM = 4;
+    const int gsz = kGroupM * tn_count;
+    const int gi = t / gsz;
+    const int gm = min(tm_count - gi * kGroupM, kGroupM);
+    const int r = t - gi * gsz;
+    n0 = (r / gm) * 256;
+    m0 = (gi * kGroupM + r % gm) * 256;
+    return true;
+  };
+  auto rsrc_of = [&](bool ok, int m0, int n0) __attribute__((always_inline)) {
+    TileRsrc r;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int mh = m0 + h * 128, nh = n0 + h * 128;
+      const int mv = ok ? min(g.M - mh, 128) : 0, nv = ok ? min(g.N - nh, 128) : 0;
+      r.a[h] = make_rsrc(g.a + (mv > 0 ? mh * g.lda : 0), mv > 0 ? (mv - 1) * g.lda + g.kb * 16ll : 0);
+      r.b[h] = make_rsrc(g.b + (nv > 0 ? nh * g.ldb : 0), nv > 0 ? (nv - 1) * g.ldb + g.kb * 16ll : 0);
+    }
+    const bool of_b = wave >= 4;
+    const int row = (of_b ? n0 : m0) + (wave & 3) * 64, rows = of_b ? g.N : g.M;
+    const int64_t ld = of_b ? g.ldbs : g.ldas;
+    const int v = ok ? min(rows - row, 64) : 0;
+    r.s = make_rsrc((of_b ? g.bs : g.as) + (v > 0 ? row * ld : 0), v > 0 ? (v - 1) * ld + g.kb : 0);
+    return r;
+  };
+
+  HalfLoader<true> la, lb;
+  la.init(g.lda / 2, wave, lane);
+  lb.init(g.ldb / 2, wave, lane);
+  const uint32_t smem_addr = lds_addr(smem);
+  // this lane's dwords of the scales: rows l / 2 and 32 + l / 2 of the wave's 64
+  const uint32_t scale_ld = static_cast<uint32_t>(wave >= 4 ? g.ldbs : g.ldas);
+  const uint32_t scale_off = static_cast<uint32_t>(lane >> 1) * scale_ld + (lane & 1) * 4;
+
+  int m0, n0, nm0 = 0, nn0 = 0;
+  if (!tile_at(0, m0, n0)) return;  // (the whole block)
+  TileRsrc cur = rsrc_of(true, m0, n0), nxt;
+
+  constexpr auto yes = std::true_type{};
+  constexpr auto no = std::false_type{};
+  // loads of half tile `half` of operand A / B of K tile t (buffer t & 1)
+  auto dma_a = [&](auto tail, const TileRsrc& rs, int half, int t) __attribute__((always_inline)) {
+    la.template issue<decltype(tail)::value>(
+        rs.a[half], smem_addr + static_cast<uint32_t>(((t & 1) * 2 + half) * kHalf), t * 64, K, wave, lane);
+  };
+  auto dma_b = [&](auto tail, const TileRsrc& rs, int half, int t) __attribute__((always_inline)) {
+    lb.template issue<decltype(tail)::value>(
+        rs.b[half], smem_addr + static_cast<uint32_t>(kAreaB + ((t & 1) * 2 + half) * kHalf), t * 64, K, wave, lane);
+  };
+  // the scales of K tile t into ring slot `slot`
+  auto dma_s = [&](auto tail, const TileRsrc& rs, int t, int slot) __attribute__((always_inline)) {
+    uint32_t koff = static_cast<uint32_t>(t * 8);
+    asm volatile("" : "+s"(koff));
+    const bool in = !decltype(tail)::value || t * 8 < g.kb;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      dma4(rs.s, smem_addr + static_cast<uint32_t>(kScaleOff + slot * kScales + wave * 512 + u * 256),
+           in ? scale_off + u * 32 * scale_ld + koff : kOOB);
+  };
+
+  // [quadrant][row tile][column tile]; quadrants 00, 10, 11, 01 (row half,
+  // column half), 32 x 64 per wave
+  f32x4 acc[4][2][4];
+  u32x4 ax[4], ay[4], bx[4][2];  // A0, A1, one half of B
+  // scales: A's [half], one half of B's [column tiles 0 and 1, 2 and 3]; byte 2 (tile & 1) + k-step
+  uint32_t sa[2], sb[2];
+  int slot = 0;  // of the current K tile's scales
+  // LDS addresses of this lane's fragments at half 0 of buffer 0, per k-step: row
+  // l & 15 of the wave's part, block 2 (l >> 4) + ks of the K tile
+  uint32_t abase[2], bbase[2];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    const int q = lane >> 4, ra = wm * 32 + (lane & 15), rb = wn * 64 + (lane & 15);
+    abase[ks] = smem_addr + static_cast<uint32_t>(ra * 128 + kslot<64>(ra, 2 * q + ks) * 16);
+    bbase[ks] = smem_addr + static_cast<uint32_t>(kAreaB + rb * 128 + kslot<64>(rb, 2 * q + ks) * 16);
+    asm volatile("" : "+v"(abase[ks]), "+v"(bbase[ks]));
+  }
+  auto read_a = [&](u32x4 (&f)[4], int buf, int half) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)  // [k-step][row tile]
+      f[e] = *reinterpret_cast<lds_cu32x4_t*>(abase[e >> 1] + static_cast<uint32_t>((buf * 2 + half) * kHalf + (e & 1) * 2048));
+  };
+  auto read_b = [&](int buf, int half) __attribute__((always_inline)) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        bx[j][ks] = *reinterpret_cast<lds_cu32x4_t*>(bbase[ks] + static_cast<uint32_t>((buf * 2 + half) * kHalf + j * 2048));
+  };
+  // rows row .. + 15 and row + 16 .. + 31 of the K tile's scales (A's first, then B's)
+  auto read_scales = [&](int row) __attribute__((always_inline)) {
+    const int l = here(lane);
+    const uint32_t at = smem_addr + static_cast<uint32_t>(kScaleOff + slot * kScales + (row + (l & 15)) * 8 + (l >> 4) * 2);
+    return *reinterpret_cast<lds_cu16_t*>(at) | static_cast<uint32_t>(*reinterpret_cast<lds_cu16_t*>(at + 128)) << 16;
+  };
+  auto read_sb = [&](int half) __attribute__((always_inline)) {
+    sb[0] = read_scales(256 + half * 128 + wn * 64);
+    sb[1] = read_scales(256 + half * 128 + wn * 64 + 32);
+  };
+
+  // ---- epilogue: a finished quadrant (32 x 64 per wave) is rounded, 16 x 16
+  // pieces between the MFMAs of the next K step, into the wave's 2 KiB of
+  // staging (16 rows of 128 bytes, chunk c of row r at slot c ^ (r >> 1)) and
+  // leaves as 128-byte row segments.  (A wave's LDS operations are in order:
+  // the second row tile may be written once the first's reads are issued.)
+  const uint32_t ep = smem_addr + static_cast<uint32_t>(kStageOff + wave * 2048);
+  const uint32_t bias_lds = smem_addr + static_cast<uint32_t>(kBiasOff + wave * 256);
+  int pm0 = 0, pn0 = 0;  // the tile being stored
+  bool pend = false;
+  auto row_half = [&](int q) __attribute__((always_inline)) { return q == 1 || q == 2; };
+  auto col_half = [&](int q) __attribute__((always_inline)) { return q >= 2; };
+  // the bias columns of the tile at n: lanes 0-31 the first half's, 32-63 the
+  // second's, two per lane (past N: zero; an odd N's last pair is one dword)
+  auto bias_dma = [&](int n) __attribute__((always_inline)) {
+    const int l = here(lane);
+    dma4(make_rsrc(g.bias, (static_cast<int64_t>(g.N) * 2 + 3) & ~3ll), bias_lds,
+         static_cast<uint32_t>((n + (l >> 5) * 128 + wn * 64 + (l & 31) * 2) * 2));
+  };
+  // LDS address of this lane's 4 columns in column tile 0; column tile ct
+  // flips chunk bits 1 and 2: address ^ (ct << 5)
+  auto ep_base = [&](int l) __attribute__((always_inline)) {
+    const int r = l & 15, c = l >> 5, half = (l >> 4) & 1;
+    return ep + static_cast<uint32_t>(r * 128 + ((c ^ (r >> 1)) << 4) + half * 8);
+  };
+  auto bias_of = [&](int q, int l, u32x2 (&bias)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct)
+      bias[ct] = *reinterpret_cast<lds_cu32x2_t*>(bias_lds + static_cast<uint32_t>(col_half(q) * 128 + ct * 32 + (l >> 4) * 8));
+  };
+  // rounds row tile i / 4, column tile i % 4 of quadrant q into the staging
+  auto convert = [&](int q, int i, uint32_t base, const u32x2 (&bias)[4]) __attribute__((always_inline)) {
+    const int rt = i >> 2, ct = i & 3;
+    T o[4];
+    if constexpr (BIAS) {
+      const u32x2 raw = bias[ct];
+      const T* t = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(acc[q][rt][ct][e] + static_cast<float>(t[e]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(acc[q][rt][ct][e]);
+    }
+    *reinterpret_cast<lds_u32x2_t*>(base ^ static_cast<uint32_t>(ct << 5)) = __builtin_bit_cast(u32x2, o);
+  };
+  // 16 staged rows back, 8 lanes per row: rows l / 8 and l / 8 + 8
+  auto load_rows = [&](u32x4 (&rows)[2], int l) __attribute__((always_inline)) {
+    const int r = l >> 3, c = l & 7;
+    const uint32_t at = ep + static_cast<uint32_t>(r * 128 + ((c ^ (r >> 1)) << 4));
+    rows[0] = *reinterpret_cast<lds_cu32x4_t*>(at);
+    rows[1] = *reinterpret_cast<lds_cu32x4_t*>((at ^ 64u) + 1024u);
+  };
+  // Row tile rt of quadrant q to memory: at least 2 store instructions
+  // whatever the edges (a lane with nothing to store stores past the
+  // resource), which the waits of the following phases count on.  Rows may
+  // start at any 2-byte address.
+  auto put_rows = [&](const u32x4 (&rows)[2], int q, int rt, int l) __attribute__((always_inline)) {
+    const int m = pm0 + row_half(q) * 128 + wm * 32 + rt * 16;
+    const int n = pn0 + col_half(q) * 128 + wn * 64;
+    const T* D = static_cast<const T*>(g.d) + static_cast<int64_t>(m) * g.ldd + n;
+    const __amdgpu_buffer_rsrc_t r = buffer_rsrc_uniform(D, 0x7fffffffu);
+    const int c0 = (l & 7) * 8;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int row = (l >> 3) + 8 * u;
+      const bool in = m + row < g.M;
+      const uint32_t at = static_cast<uint32_t>(row) * static_cast<uint32_t>(g.ldd) * 2 + c0 * 2;
+      __builtin_amdgcn_raw_buffer_store_b128(rows[u], r, in && n + c0 + 8 <= g.N ? at : kOOB, 0, kBufNT);
+      if ((g.N & 7) && pn0 + 256 > g.N) {  // the tile of the row's last, partial chunk
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+          __builtin_amdgcn_raw_buffer_store_b16(
+              static_cast<uint16_t>(rows[u][e >> 1] >> (16 * (e & 1))), r,
+              in && n + c0 + 8 > g.N && n + c0 + e < g.N ? at + 2 * e : kOOB, 0, 0);
+      }
+    }
+  };
+
+  // the quadrant's 16 MFMAs, A of half ah; LEAVE: finished quadrant cq leaves between them -- its first row tile's
+  // rows are stored under its second's conversion, its second's are left in
+  // `rows` (put_rows by the caller)
+  u32x4 rows[2];
+  auto mfma16x = [&](auto first, auto leave, int q, const u32x4 (&af)[4], int ah, int cq) __attribute__((always_inline)) {
+    constexpr bool FIRST = decltype(first)::value, LEAVE = decltype(leave)::value;
+    int l = 0;
+    uint32_t base = 0;
+    u32x2 bias[4];
+    if constexpr (LEAVE) {
+      l = here(lane);
+      base = ep_base(l);
+      if constexpr (BIAS) bias_of(cq, l, bias);
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+        for (int ct = 0; ct < 4; ++ct) {
+          f32x4 c = acc[q][rt][ct];
+          if (FIRST && ks == 0) c = f32x4{0.f, 0.f, 0.f, 0.f};
+          const auto one = [&](auto bb, auto ab) {
+            return mfma_mx4<decltype(bb)::value, decltype(ab)::value>(bx[ct][ks], sb[ct >> 1], af[ks * 2 + rt], sa[ah], c);
+          };
+          constexpr std::integral_constant<int, 0> i0{};
+          constexpr std::integral_constant<int, 1> i1{};
+          constexpr std::integral_constant<int, 2> i2{};
+          constexpr std::integral_constant<int, 3> i3{};
+          if (ks == 0)
+            acc[q][rt][ct] = ct & 1 ? (rt ? one(i2, i2) : one(i2, i0)) : (rt ? one(i0, i2) : one(i0, i0));
+          else
+            acc[q][rt][ct] = ct & 1 ? (rt ? one(i3, i3) : one(i3, i1)) : (rt ? one(i1, i3) : one(i1, i1));
+          if constexpr (LEAVE) {
+            const int i = ks * 8 + rt * 4 + ct;  // piece i / 2 after every second MFMA
+            if (i & 1) {
+              __builtin_amdgcn_sched_barrier(0);
+              convert(cq, i >> 1, base, bias);
+              if (i == 7) load_rows(rows, l);
+              if (i == 11) put_rows(rows, cq, 0, l);
+              if (i == 15) load_rows(rows, l);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+        }
+    // The compiler takes the scaled MFMA for code that it may move past barriers
+    // to the result's use: here the results are used.
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(acc[q][i >> 2][i & 3]));
+  };
+  // ends a memory phase: its fragments are in registers, and all but the
+  // wave's N youngest memory operations are done
+  auto end_mem = [&](auto n_tag) __attribute__((always_inline)) {
+    constexpr int N = decltype(n_tag)::value;
+    __builtin_amdgcn_sched_barrier(0);
+    if (N > 10 && pend)
+      wait_vm<N>();
+    else
+      wait_vm<10>();
+    wait_lgkmcnt0();
+    block_barrier();
+    __builtin_amdgcn_s_setprio(1);
+  };
+  auto end_mfma = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_s_setprio(0);
+    block_barrier();
+  };
+#define NTOPS_W(n) std::integral_constant<int, (n)> {}
+
+  // One K tile (buffer BUF): two phases.  KIND 0: the first K tile of an
+  // output tile (quadrants 1 - 3 of the previous one leave), 3: the second,
+  // 1: between, 2: the last (quadrant 0 leaves).  Loads issued: the scales of the
+  // K tile after the next (rs2 / t2; into the slot of the K tile before this
+  // one, which both groups of waves have read two barriers ago) and B1 of the next
+  // (rs1 / t1), then A0, B0, A1 of the one after it.  The waits allow for the 10
+  // loads issued since the ones the next phase reads, plus the stores among them
+  // while a tile leaves (two per put_rows: 4, 8, 5 and 1 of them).
+  auto ktile = [&](auto kind_tag, auto buf_tag, auto tail, const TileRsrc& rs1, int t1, const TileRsrc& rs2, int t2)
+                   __attribute__((always_inline)) {
+    constexpr int KIND = decltype(kind_tag)::value, BUF = decltype(buf_tag)::value;
+    constexpr auto first = std::bool_constant<KIND == 0>{};
+    // ---- phase A: quadrants 0 and 1
+    sa[0] = read_scales(wm * 32);
+    sa[1] = read_scales(128 + wm * 32);
+    read_sb(0);
+    read_a(ax, BUF, 0);
+    read_b(BUF, 0);
+    read_a(ay, BUF, 1);
+    dma_s(tail, rs2, t2, slot == 0 ? 2 : slot - 1);
+    dma_b(tail, rs1, 1, t1);
+    if constexpr (KIND == 0)
+      if (pend) put_rows(rows, 1, 1, here(lane));
+    end_mem(NTOPS_W(KIND == 0 ? 18 : KIND == 3 ? 20 : 10));
+    if (KIND == 0 && pend) {
+      mfma16x(first, yes, 0, ax, 0, 2);
+      put_rows(rows, 2, 1, here(lane));
+      mfma16x(first, yes, 1, ay, 1, 3);
+    } else {
+      mfma16x(first, no, 0, ax, 0, 0);
+      mfma16x(first, no, 1, ay, 1, 0);
+    }
+    end_mfma();
+    // ---- phase B: quadrants 2 and 3
+    read_sb(1);
+    read_b(BUF, 1);
+    dma_a(tail, rs2, 0, t2);
+    dma_b(tail, rs2, 0, t2);
+    dma_a(tail, rs2, 1, t2);
+    if constexpr (KIND == 0)
+      if (pend) put_rows(rows, 3, 1, here(lane));
+    end_mem(NTOPS_W(KIND == 0 ? 26 : KIND == 3 ? 12 : 10));
+    if constexpr (KIND == 2) {
+      pm0 = m0;
+      pn0 = n0;
+      mfma16x(no, yes, 2, ay, 1, 0);
+      put_rows(rows, 0, 1, here(lane));
+      mfma16x(no, yes, 3, ax, 0, 1);
+    } else {
+      mfma16x(first, no, 2, ay, 1, 0);
+      mfma16x(first, no, 3, ax, 0, 0);
+    }
+    end_mfma();
+    slot = slot == 2 ? 0 : slot + 1;
+  };
+
+  // prologue: the first K tile and the scales, A0, B0, A1 of the second in flight
+  dma_s(no, cur, 0, 0);
+  dma_a(no, cur, 0, 0);
+  dma_b(no, cur, 0, 0);
+  dma_a(no, cur, 1, 0);
+  dma_s(no, cur, 1, 1);
+  dma_b(no, cur, 1, 0);
+  dma_a(no, cur, 0, 1);
+  dma_b(no, cur, 0, 1);
+  dma_a(no, cur, 1, 1);
+  wait_vmcnt<10>();
+  block_barrier();
+  if (grp == 1) block_barrier();
+
+  constexpr auto b0 = NTOPS_W(0);
+  constexpr auto b1 = NTOPS_W(1);
+  for (int it = 0;; ++it) {
+    ktile(NTOPS_W(0), b0, no, cur, 1, cur, 2);
+    ktile(NTOPS_W(3), b1, no, cur, 2, cur, 3);
+    int t = 2;
+    for (; t < 2 * np - 4; t += 2) {
+      ktile(NTOPS_W(1), b0, no, cur, t + 1, cur, t + 2);
+      ktile(NTOPS_W(1), b1, no, cur, t + 2, cur, t + 3);
+    }
+    // the loads of the last two K tiles, which may reach past K
+    ktile(NTOPS_W(1), b0, yes, cur, t + 1, cur, t + 2);
+    ktile(NTOPS_W(1), b1, yes, cur, t + 2, cur, t + 3);
+    if constexpr (BIAS) bias_dma(n0);
+    const bool more = tile_at(it + 1, nm0, nn0);
+    nxt = rsrc_of(more, nm0, nn0);
+    ktile(NTOPS_W(1), b0, yes, cur, t + 3, nxt, 0);
+    ktile(NTOPS_W(2), b1, no, nxt, 0, nxt, 1);
+    pend = true;
+    if (!more) break;
+    cur = nxt;
+    m0 = nm0;
+    n0 = nn0;
+  }
+#undef NTOPS_W
+  if (grp == 0) block_barrier();
+  put_rows(rows, 1, 1, lane);
+#pragma unroll
+  for (int q = 2; q < 4; ++q) {
+    u32x2 bias[4];
+    if constexpr (BIAS) bias_of(q, lane, bias);
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt) {
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) convert(q, rt * 4 + ct, ep_base(lane), bias);
+      load_rows(rows, lane);
+      put_rows(rows, q, rt, lane);
+    }
+  }
+  wait_vmcnt<0>();  // no DMA may land after the workgroup ends
+}
+
+template <typename T, bool BIAS>
+int launch_large(const Mx4Args& g, hipStream_t st) {
+  auto kern = k_mx4_large<T, BIAS>;
+  static std::atomic<bool> attr_set{false};  // (threads may get here together)
+  if (!attr_set.load(std::memory_order_relaxed)) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) !=
+        hipSuccess)
+      return set_error(NTOPS_ERR_HIP, "mxfp4_mm: cannot reserve %d bytes of LDS", kLds);
+    attr_set.store(true, std::memory_order_relaxed);
+  }
+  const int64_t total = ceil_div(g.M, 256) * ceil_div(g.N, 256);
+  const int64_t grid = std::min<int64_t>(total, cu_count_cached());
+  note_kernel("mxfp4_large");
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(grid)), dim3(512), kLds, st, g, static_cast<int>(total));
+  return check_launch("mxfp4_mm");
+}
+
+template <typename T>
+int run_large(const Mx4Args& g, hipStream_t st) {
+  return g.bias != nullptr ? launch_large<T, true>(g, st) : launch_large<T, false>(g, st);
+}
+
+}  // namespace
+
+bool mx4_large_serves(int out_dtype, const Mx4Args& g) {
+  const auto dwords = [](const uint8_t* s, int64_t ld) { return (reinterpret_cast<uintptr_t>(s) & 3u) == 0 && ld % 4 == 0; };
+  return out_dtype != NTOPS_F32 && g.kb % 8 == 0 && g.kb > 32 && dwords(g.as, g.ldas) && dwords(g.bs, g.ldbs) &&
+         (reinterpret_cast<uintptr_t>(g.bias) & 3u) == 0 && g.ldd >= 0 && (16 * g.ldd + 64) * 2 < (int64_t(1) << 31);
+}
+
+int mx4_large(int out_dtype, const Mx4Args& g, hipStream_t st) {
+  return out_dtype == NTOPS_BF16 ? run_large<__bf16>(g, st) : run_large<_Float16>(g, st);
+}
+
+}  // namespace ntops

@@ -57,9 +57,9 @@ struct Loader {
   __device__ __forceinline__ void init(const uint8_t* c, int64_t ld, const uint8_t* s, int64_t lds, int rows, int blocks,
                                        int lane) {
     kb = blocks;
-    codes = mx4_rsrc(c, (rows - 1) * ld + blocks * 16ll);
+    codes = make_rsrc(c, (rows - 1) * ld + blocks * 16ll);
     const int o = static_cast<int>(reinterpret_cast<uintptr_t>(s) & 3u);
-    scales = mx4_rsrc(s - o, (o + (rows - 1) * lds + blocks + 3) & ~3ll);
+    scales = make_rsrc(s - o, (o + (rows - 1) * lds + blocks + 3) & ~3ll);
 #pragma unroll
     for (int i = 0; i < kInst; ++i) {
       const int r = i * kRpi + lane / CPR;

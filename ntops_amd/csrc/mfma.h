@@ -84,6 +84,26 @@ __device__ __forceinline__ void dma16(u32x4 rsrc, uint32_t lds_dst, uint32_t vof
                : "memory");
 }
 
+// 4-byte global -> LDS copy per lane: lane l's dword lands at lds_dst + 4 l.
+__device__ __forceinline__ void dma4(u32x4 rsrc, uint32_t lds_dst, uint32_t voffset) {
+  asm volatile("buffer_load_dword %0, %1, 0 offen lds"
+               :
+               : "v"(voffset), "s"(rsrc), "{m0}"(lds_dst)
+               : "memory");
+}
+
+// Buffer resource of `bytes` bytes at `base` for the copies above (both
+// wave-uniform).
+__device__ __forceinline__ u32x4 make_rsrc(const void* base, int64_t bytes) {
+  const uint64_t addr = reinterpret_cast<uint64_t>(base);
+  u32x4 r;
+  r.x = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(addr));
+  r.y = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(addr >> 32) & 0xffffu);
+  r.z = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(bytes));
+  r.w = 0x00020000u;
+  return r;
+}
+
 // 32-bit LDS address of a pointer into the block's LDS (wave-uniform).
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
   return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void_t*)p)));

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import ntops_amd.torch as nt
+from ntops_amd import _lib
 from oracle import narrow as N
 
 pytestmark = pytest.mark.gpu
@@ -152,6 +153,18 @@ SIZES = [
 def test_product(m, n, k, dtype):
     bias = torch.randn(n).to(dtype).cuda() if (m + n) % 2 else None
     check_product(*operands(m, n, k), bias, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", [(2048, 4096, 1280), (2000, 4090, 1792), (1900, 4099, 2048), (2300, 7700, 1536), (8200, 4100, 1312)])
+def test_product_large(m, n, k, dtype):
+    bias = torch.randn(n).to(dtype).cuda() if n % 4 else None
+    args = operands(m, n, k)
+    out = check_product(*args, bias, dtype)
+    if k % 256 == 0:
+        assert _lib.last_kernel() == "mxfp4_large"
+    for _ in range(3):
+        assert torch.equal(nt.mxfp4_mm(*args, bias, dtype=dtype), out)
 
 
 @pytest.mark.parametrize("m,n,k", [(3, 50, 4096), (64, 200, 512), (260, 300, 1056)])
