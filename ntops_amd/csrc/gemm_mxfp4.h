@@ -28,6 +28,15 @@ struct Mx4Args {
   int split, kchunk;   // slices, and the blocks of each
 };
 
+// Of B neighbouring blocks in the LDS, the one kept at place p of its row: lane
+// group q reads places 4 u + q in instruction u = 0 .. B / 4 - 1 -- reads that touch
+// every bank once under the swizzles of mfma.h -- and gets the neighbouring blocks
+// q B / 4 + u.
+template <int B>
+__device__ __forceinline__ int mx4_block(int p) {
+  return (p & 3) * (B / 4) + (p >> 2);
+}
+
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 // c += A B over 4 blocks; SA / SB: the byte of sa / sb that holds the scales.

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256, BT == 64 ? 2 : 1) void k_mx4_tile(Mx4Args g, i
 #pragma unroll
     for (int u = 0; u < S::kRowsPerWave / 8; ++u) {
       const int row = wave * S::kRowsPerWave + u * 8 + (lane >> 3);
-      const int blk = b0 + kslot<64>(row, lane & 7);
+      const int blk = b0 + mx4_block<8>(kslot<64>(row, lane & 7));
       const uint32_t dst = st + static_cast<uint32_t>((wave * S::kRowsPerWave + u * 8) * 128);
       dma16(ra, dst, blk < kb1 && row < mv ? static_cast<uint32_t>(row * g.lda + blk * 16) : kOOB);
       dma16(rb, dst + S::kCodes, blk < kb1 && row < nv ? static_cast<uint32_t>(row * g.ldb + blk * 16) : kOOB);
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256, BT == 64 ? 2 : 1) void k_mx4_tile(Mx4Args g, i
       }
     }
     const auto frag = [&](int area, int r, int ks) {
-      return *reinterpret_cast<const u32x4*>(st + area * S::kCodes + r * 128 + kslot<64>(r, 2 * q + ks) * 16);
+      return *reinterpret_cast<const u32x4*>(st + area * S::kCodes + r * 128 + kslot<64>(r, 4 * ks + q) * 16);
     };
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {

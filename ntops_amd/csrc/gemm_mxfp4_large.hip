@@ -37,6 +37,39 @@ typedef __attribute__((address_space(3))) const u32x2 lds_cu32x2_t;
 typedef __attribute__((address_space(3))) u32x2 lds_u32x2_t;
 typedef __attribute__((address_space(3))) const uint16_t lds_cu16_t;
 
+// Loads of an operand's half tiles: 2 instructions of 1 KiB per wave, one whole
+// line of 8 blocks a row.
+struct CodeLoader {
+  uint32_t voff[2];
+  uint32_t lds_off;  // of this wave's first instruction
+
+  // the K tile's block that this lane brings with instruction i
+  __device__ __forceinline__ static int block(int wave, int lane, int i) {
+    const int row = (wave * 2 + i) * 8 + lane / 8;
+    return mx4_block<8>(kslot<64>(row, lane % 8));
+  }
+  __device__ __forceinline__ void init(int64_t ld, int wave, int lane) {
+    lds_off = static_cast<uint32_t>(wave * 2048);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      voff[i] = static_cast<uint32_t>(((wave * 2 + i) * 8 + lane / 8) * ld + block(wave, lane, i) * 16);
+  }
+  // TAIL: K tile t may reach past the row's kb blocks, which read as zero.
+  template <bool TAIL>
+  __device__ __forceinline__ void issue(u32x4 rsrc, uint32_t lds, int t, int kb, int wave, int lane) const {
+    // (opaque, so that no sum of a fixed tile's is kept in a register)
+    uint32_t koff = static_cast<uint32_t>(t * 128);
+    asm volatile("" : "+s"(koff));
+    const int l = TAIL ? here(lane) : 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t off = voff[i] + koff;
+      if constexpr (TAIL) off = t * 8 + block(wave, l, i) < kb ? off : kOOB;
+      dma16(rsrc, lds + lds_off + i * 1024, off);
+    }
+  }
+};
+
 // Resources of an output tile's operand halves and of this wave's 64 scale rows
 // (what lies past an edge reads as zero).
 struct TileRsrc {
@@ -52,7 +85,6 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
   const int grp = wave >> 2;
   const int tm_count = (g.M + 255) / 256, tn_count = (g.N + 255) / 256;
   const int np = (g.kb + 15) / 16;  // pairs of K tiles
-  const int K = g.kb * 8;    // in 16-bit units, as the loaders count
 
   // tile `i` of this block: (row, column) or false past the end
   const int nx = (gridDim.x & 7) == 0 ? 8 : 1;
@@ -88,9 +120,9 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
     return r;
   };
 
-  HalfLoader<true> la, lb;
-  la.init(g.lda / 2, wave, lane);
-  lb.init(g.ldb / 2, wave, lane);
+  CodeLoader la, lb;
+  la.init(g.lda, wave, lane);
+  lb.init(g.ldb, wave, lane);
   const uint32_t smem_addr = lds_addr(smem);
   // this lane's dwords of the scales: rows l / 2 and 32 + l / 2 of the wave's 64
   const uint32_t scale_ld = static_cast<uint32_t>(wave >= 4 ? g.ldbs : g.ldas);
@@ -105,11 +137,11 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
   // loads of half tile `half` of operand A / B of K tile t (buffer t & 1)
   auto dma_a = [&](auto tail, const TileRsrc& rs, int half, int t) __attribute__((always_inline)) {
     la.template issue<decltype(tail)::value>(
-        rs.a[half], smem_addr + static_cast<uint32_t>(((t & 1) * 2 + half) * kHalf), t * 64, K, wave, lane);
+        rs.a[half], smem_addr + static_cast<uint32_t>(((t & 1) * 2 + half) * kHalf), t, g.kb, wave, lane);
   };
   auto dma_b = [&](auto tail, const TileRsrc& rs, int half, int t) __attribute__((always_inline)) {
     lb.template issue<decltype(tail)::value>(
-        rs.b[half], smem_addr + static_cast<uint32_t>(kAreaB + ((t & 1) * 2 + half) * kHalf), t * 64, K, wave, lane);
+        rs.b[half], smem_addr + static_cast<uint32_t>(kAreaB + ((t & 1) * 2 + half) * kHalf), t, g.kb, wave, lane);
   };
   // the scales of K tile t into ring slot `slot`
   auto dma_s = [&](auto tail, const TileRsrc& rs, int t, int slot) __attribute__((always_inline)) {
@@ -130,13 +162,13 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
   uint32_t sa[2], sb[2];
   int slot = 0;  // of the current K tile's scales
   // LDS addresses of this lane's fragments at half 0 of buffer 0, per k-step: row
-  // l & 15 of the wave's part, block 2 (l >> 4) + ks of the K tile
+  // l & 15 of the wave's part, place 4 ks + (l >> 4) of the K tile
   uint32_t abase[2], bbase[2];
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
     const int q = lane >> 4, ra = wm * 32 + (lane & 15), rb = wn * 64 + (lane & 15);
-    abase[ks] = smem_addr + static_cast<uint32_t>(ra * 128 + kslot<64>(ra, 2 * q + ks) * 16);
-    bbase[ks] = smem_addr + static_cast<uint32_t>(kAreaB + rb * 128 + kslot<64>(rb, 2 * q + ks) * 16);
+    abase[ks] = smem_addr + static_cast<uint32_t>(ra * 128 + kslot<64>(ra, 4 * ks + q) * 16);
+    bbase[ks] = smem_addr + static_cast<uint32_t>(kAreaB + rb * 128 + kslot<64>(rb, 4 * ks + q) * 16);
     asm volatile("" : "+v"(abase[ks]), "+v"(bbase[ks]));
   }
   auto read_a = [&](u32x4 (&f)[4], int buf, int half) __attribute__((always_inline)) {
@@ -151,15 +183,20 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
       for (int j = 0; j < 4; ++j)
         bx[j][ks] = *reinterpret_cast<lds_cu32x4_t*>(bbase[ks] + static_cast<uint32_t>((buf * 2 + half) * kHalf + j * 2048));
   };
-  // rows row .. + 15 and row + 16 .. + 31 of the K tile's scales (A's first, then B's)
-  auto read_scales = [&](int row) __attribute__((always_inline)) {
-    const int l = here(lane);
-    const uint32_t at = smem_addr + static_cast<uint32_t>(kScaleOff + slot * kScales + (row + (l & 15)) * 8 + (l >> 4) * 2);
-    return *reinterpret_cast<lds_cu16_t*>(at) | static_cast<uint32_t>(*reinterpret_cast<lds_cu16_t*>(at + 128)) << 16;
+  // Scales of the 16-row slices 2 i and 2 i + 1 of a wave's rows in half `half` of A
+  // (of_b: of B), as read: the halves of a register are put together by `pack` once
+  // they have landed, behind the fragments' reads.
+  uint32_t raw[8];
+  auto read_scales = [&](int l, bool of_b, int half, int i, uint32_t& x, uint32_t& y) __attribute__((always_inline)) {
+    const uint32_t base = smem_addr + static_cast<uint32_t>(kScaleOff + slot * kScales + (of_b ? 256 * 8 + wn * 512 : wm * 256));
+    const uint32_t at = base + static_cast<uint32_t>((l & 15) * 8 + (l >> 4) * 2);
+    x = *reinterpret_cast<lds_cu16_t*>(at + half * 1024 + i * 256);
+    y = *reinterpret_cast<lds_cu16_t*>(at + half * 1024 + i * 256 + 128);
   };
-  auto read_sb = [&](int half) __attribute__((always_inline)) {
-    sb[0] = read_scales(256 + half * 128 + wn * 64);
-    sb[1] = read_scales(256 + half * 128 + wn * 64 + 32);
+  // (opaque, so that it is not moved up to where its parts are read)
+  auto pack = [](uint32_t x, uint32_t y) __attribute__((always_inline)) {
+    asm volatile("" : "+v"(x), "+v"(y));
+    return x | y << 16;
   };
 
   // ---- epilogue: a finished quadrant (32 x 64 per wave) is rounded, 16 x 16
@@ -291,7 +328,7 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
   };
   // ends a memory phase: its fragments are in registers, and all but the
   // wave's N youngest memory operations are done
-  auto end_mem = [&](auto n_tag) __attribute__((always_inline)) {
+  auto end_mem = [&](auto n_tag, auto packs) __attribute__((always_inline)) {
     constexpr int N = decltype(n_tag)::value;
     __builtin_amdgcn_sched_barrier(0);
     if (N > 10 && pend)
@@ -299,6 +336,8 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
     else
       wait_vm<10>();
     wait_lgkmcnt0();
+    __builtin_amdgcn_sched_barrier(0);
+    packs();
     block_barrier();
     __builtin_amdgcn_s_setprio(1);
   };
@@ -321,17 +360,25 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
     constexpr int KIND = decltype(kind_tag)::value, BUF = decltype(buf_tag)::value;
     constexpr auto first = std::bool_constant<KIND == 0>{};
     // ---- phase A: quadrants 0 and 1
-    sa[0] = read_scales(wm * 32);
-    sa[1] = read_scales(128 + wm * 32);
-    read_sb(0);
     read_a(ax, BUF, 0);
     read_b(BUF, 0);
     read_a(ay, BUF, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    const int l = here(lane);
+    read_scales(l, false, 0, 0, raw[0], raw[1]);
+    read_scales(l, false, 1, 0, raw[2], raw[3]);
+    read_scales(l, true, 0, 0, raw[4], raw[5]);
+    read_scales(l, true, 0, 1, raw[6], raw[7]);
     dma_s(tail, rs2, t2, slot == 0 ? 2 : slot - 1);
     dma_b(tail, rs1, 1, t1);
     if constexpr (KIND == 0)
       if (pend) put_rows(rows, 1, 1, here(lane));
-    end_mem(NTOPS_W(KIND == 0 ? 18 : KIND == 3 ? 20 : 10));
+    end_mem(NTOPS_W(KIND == 0 ? 18 : KIND == 3 ? 20 : 10), [&]() __attribute__((always_inline)) {
+      sa[0] = pack(raw[0], raw[1]);
+      sa[1] = pack(raw[2], raw[3]);
+      sb[0] = pack(raw[4], raw[5]);
+      sb[1] = pack(raw[6], raw[7]);
+    });
     if (KIND == 0 && pend) {
       mfma16x(first, yes, 0, ax, 0, 2);
       put_rows(rows, 2, 1, here(lane));
@@ -342,14 +389,20 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
     }
     end_mfma();
     // ---- phase B: quadrants 2 and 3
-    read_sb(1);
     read_b(BUF, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    const int l2 = here(lane);
+    read_scales(l2, true, 1, 0, raw[4], raw[5]);
+    read_scales(l2, true, 1, 1, raw[6], raw[7]);
     dma_a(tail, rs2, 0, t2);
     dma_b(tail, rs2, 0, t2);
     dma_a(tail, rs2, 1, t2);
     if constexpr (KIND == 0)
       if (pend) put_rows(rows, 3, 1, here(lane));
-    end_mem(NTOPS_W(KIND == 0 ? 26 : KIND == 3 ? 12 : 10));
+    end_mem(NTOPS_W(KIND == 0 ? 26 : KIND == 3 ? 12 : 10), [&]() __attribute__((always_inline)) {
+      sb[0] = pack(raw[4], raw[5]);
+      sb[1] = pack(raw[6], raw[7]);
+    });
     if constexpr (KIND == 2) {
       pm0 = m0;
       pn0 = n0;

@@ -50,8 +50,9 @@ struct Loader {
   uint32_t voff[kInst], soff[kScaleInst];
   int kb;
 
+  // the step's block that this lane brings with instruction i
   __device__ __forceinline__ static int chunk(int lane, int i) {
-    return sk_slot<CPR>(i * kRpi + lane / CPR, lane % CPR);
+    return mx4_block<CPR>(sk_slot<CPR>(i * kRpi + lane / CPR, lane % CPR));
   }
   // rows: valid ones
   __device__ __forceinline__ void init(const uint8_t* c, int64_t ld, const uint8_t* s, int64_t lds, int rows, int blocks,
@@ -152,7 +153,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_mx4_skinny(Mx4Args g, int wh
     for (int j = 0; j < J; ++j) scales(tb + LB::kBytes, j * 16 + i16, shb[j], left, sb[j]);
 #pragma unroll
     for (int u = 0; u < NB; ++u) {
-      const int c = q * NB + u;
+      const int c = 4 * u + q;  // holds block q NB + u
       const u32x4 a = *reinterpret_cast<const u32x4*>(ta + i16 * (CPR * 16) + sk_slot<CPR>(i16, c) * 16);
 #pragma unroll
       for (int j = 0; j < J; ++j) {
