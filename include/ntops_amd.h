@@ -377,7 +377,8 @@ NTOPS_API int ntops_dequantize_mxfp4(int dtype, int64_t rows, int64_t cols,
  * (F32 / F16 / BF16).  Code rows 16-byte aligned; strides of codes and scales
  * in bytes, of out in elements (unit column stride); scale rows may start
  * anywhere.  The workspace (16-byte aligned; may be NULL) holds fp32 partial
- * products where K is split over the GPU. */
+ * products where K is split over the GPU, and the scales of large products, laid
+ * out anew (without it those run on a slower kernel). */
 NTOPS_API int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K,
                const void* a, int64_t a_row_stride, const void* a_scales, int64_t as_row_stride,
                const void* b, int64_t b_row_stride, const void* b_scales, int64_t bs_row_stride,

@@ -72,10 +72,10 @@ __device__ __forceinline__ void store4(T* d, int64_t ldd, int m, int n, int M, i
   }
 }
 
-// 16-bit out on 256 x 256 tiles: more than 32 blocks of K, in whole K tiles of 8,
-// and scale rows of whole dwords.
+// 16-bit out on 256 x 256 tiles, from 33 blocks of K on, with a workspace.
 bool mx4_large_serves(int out_dtype, const Mx4Args& g);
-int mx4_large(int out_dtype, const Mx4Args& g, hipStream_t st);
+int64_t mx4_large_workspace(int64_t M, int64_t N, int64_t kb);
+int mx4_large(int out_dtype, Mx4Args g, void* workspace, hipStream_t st);
 
 constexpr int kSkinnyRows = 16;
 // out for M <= kSkinnyRows, bound by streaming B.

@@ -240,6 +240,7 @@ using namespace ntops;
 extern "C" int64_t ntops_mxfp4_mm_workspace(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0 || M > kMaxSize || N > kMaxSize || K > kMaxSize) return 0;
   if (M <= kSkinnyRows) return 0;
+  if (large_suits(M, N)) return mx4_large_workspace(M, N, ceil_div(K, 32));
   int bt, split, kchunk;
   plan(M, N, ceil_div(K, 32), bt, split, kchunk);
   return split > 1 ? split * M * N * 4 : 0;
@@ -287,7 +288,9 @@ extern "C" int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K, co
   return dispatch_float16_32(out_dtype, "mxfp4_mm", [&](auto tag) -> int {
     using T = decltype(tag);
     if (M <= kSkinnyRows && kb > 0) return mx4_skinny(out_dtype, g, st);
-    if (large_suits(M, N) && mx4_large_serves(out_dtype, g)) return mx4_large(out_dtype, g, st);
+    if (large_suits(M, N) && mx4_large_serves(out_dtype, g) && workspace != nullptr &&
+        workspace_bytes >= mx4_large_workspace(M, N, kb))
+      return mx4_large(out_dtype, g, workspace, st);
     int bt;
     plan(M, N, std::max<int64_t>(kb, 1), bt, g.split, g.kchunk);
     if (g.split > 1 && (workspace == nullptr || workspace_bytes < g.split * M * N * 4)) {

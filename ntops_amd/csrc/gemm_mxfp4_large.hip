@@ -7,11 +7,13 @@
 // finished quadrant leaves between the next tile's MFMAs.  K is a quarter as many
 // tiles as for 16 bits, so what surrounds the K loop weighs four times as much.
 //
-// Scales, a byte per 32 values, ride along: 8 bytes a row and K tile, two DMA
-// instructions of dwords per wave, into a ring of three K tiles.  A phase reads
-// those of its rows' blocks (k-step ks of lane group g: block 2 g + ks), two 16-row
-// slices to a register; 12 registers that held a pair of K tiles' scales cost 209
-// spilled ones.
+// Scales, a byte per 32 values, ride along, 4 KiB a K tile, in a ring of three.  A
+// kernel before this one lays them out by (256 rows, K tile), so that they arrive
+// as whole lines: read from the tensors, 8 bytes a row were as many requests as
+// the codes' lines, and 8192 x 4096 x 14336 took 246 us.  A phase reads those of
+// its rows' blocks (k-step ks of lane group q: block 2 q + ks), two 16-row slices
+// to a register; 12 registers that held a pair of K tiles' scales cost 209 spilled
+// ones.
 #include <algorithm>
 #include <atomic>
 
@@ -29,7 +31,8 @@ constexpr int kStageOff = 8 * kHalf;
 constexpr int kBiasOff = kStageOff + 8 * 2048;
 constexpr int kScaleOff = kBiasOff + 8 * 256;
 constexpr int kScales = 512 * 8;
-constexpr int kLds = kScaleOff + 3 * kScales;
+constexpr int kNoneOff = kScaleOff + 3 * kScales;
+constexpr int kLds = kNoneOff + 1024;
 static_assert(kLds <= 163840, "LDS");
 
 typedef __attribute__((address_space(3))) const u32x4 lds_cu32x4_t;
@@ -70,8 +73,8 @@ struct CodeLoader {
   }
 };
 
-// Resources of an output tile's operand halves and of this wave's 64 scale rows
-// (what lies past an edge reads as zero).
+// Resources of an output tile's operand halves (what lies past an edge reads as
+// zero) and of what this wave loads of its scales (nothing in waves 4 to 7).
 struct TileRsrc {
   u32x4 a[2], b[2], s;
 };
@@ -85,6 +88,7 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
   const int grp = wave >> 2;
   const int tm_count = (g.M + 255) / 256, tn_count = (g.N + 255) / 256;
   const int np = (g.kb + 15) / 16;  // pairs of K tiles
+  const int kt = (g.kb + 7) / 8;    // K tiles that have scales
 
   // tile `i` of this block: (row, column) or false past the end
   const int nx = (gridDim.x & 7) == 0 ? 8 : 1;
@@ -112,11 +116,10 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
       r.a[h] = make_rsrc(g.a + (mv > 0 ? mh * g.lda : 0), mv > 0 ? (mv - 1) * g.lda + g.kb * 16ll : 0);
       r.b[h] = make_rsrc(g.b + (nv > 0 ? nh * g.ldb : 0), nv > 0 ? (nv - 1) * g.ldb + g.kb * 16ll : 0);
     }
-    const bool of_b = wave >= 4;
-    const int row = (of_b ? n0 : m0) + (wave & 3) * 64, rows = of_b ? g.N : g.M;
-    const int64_t ld = of_b ? g.ldbs : g.ldas;
-    const int v = ok ? min(rows - row, 64) : 0;
-    r.s = make_rsrc((of_b ? g.bs : g.as) + (v > 0 ? row * ld : 0), v > 0 ? (v - 1) * ld + g.kb : 0);
+    // waves 0 and 1: halves of A's 2 KiB a K tile, 2 and 3: of B's
+    const int64_t panel = static_cast<int64_t>(kt) * 2048;
+    const uint8_t* sc = wave < 2 ? g.as + (m0 >> 8) * panel : g.bs + (n0 >> 8) * panel;
+    r.s = make_rsrc(sc, ok && wave < 4 ? panel : 0);
     return r;
   };
 
@@ -124,9 +127,7 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
   la.init(g.lda, wave, lane);
   lb.init(g.ldb, wave, lane);
   const uint32_t smem_addr = lds_addr(smem);
-  // this lane's dwords of the scales: rows l / 2 and 32 + l / 2 of the wave's 64
-  const uint32_t scale_ld = static_cast<uint32_t>(wave >= 4 ? g.ldbs : g.ldas);
-  const uint32_t scale_off = static_cast<uint32_t>(lane >> 1) * scale_ld + (lane & 1) * 4;
+  const uint32_t scale_off = static_cast<uint32_t>((wave & 1) * 1024 + lane * 16);
 
   int m0, n0, nm0 = 0, nn0 = 0;
   if (!tile_at(0, m0, n0)) return;  // (the whole block)
@@ -143,15 +144,13 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
     lb.template issue<decltype(tail)::value>(
         rs.b[half], smem_addr + static_cast<uint32_t>(kAreaB + ((t & 1) * 2 + half) * kHalf), t, g.kb, wave, lane);
   };
-  // the scales of K tile t into ring slot `slot`
-  auto dma_s = [&](auto tail, const TileRsrc& rs, int t, int slot) __attribute__((always_inline)) {
-    uint32_t koff = static_cast<uint32_t>(t * 8);
+  // the scales of K tile t (past the last: zeros) into ring slot `slot`
+  auto dma_s = [&](const TileRsrc& rs, int t, int slot) __attribute__((always_inline)) {
+    uint32_t koff = static_cast<uint32_t>(t * 2048);
     asm volatile("" : "+s"(koff));
-    const bool in = !decltype(tail)::value || t * 8 < g.kb;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-      dma4(rs.s, smem_addr + static_cast<uint32_t>(kScaleOff + slot * kScales + wave * 512 + u * 256),
-           in ? scale_off + u * 32 * scale_ld + koff : kOOB);
+    // (waves 4 to 7, whose waits count alike, bring zeros that nobody reads)
+    dma16(rs.s, smem_addr + static_cast<uint32_t>(wave < 4 ? kScaleOff + slot * kScales + wave * 1024 : kNoneOff),
+          scale_off + koff);
   };
 
   // [quadrant][row tile][column tile]; quadrants 00, 10, 11, 01 (row half,
@@ -331,10 +330,10 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
   auto end_mem = [&](auto n_tag, auto packs) __attribute__((always_inline)) {
     constexpr int N = decltype(n_tag)::value;
     __builtin_amdgcn_sched_barrier(0);
-    if (N > 10 && pend)
+    if (N > 9 && pend)
       wait_vm<N>();
     else
-      wait_vm<10>();
+      wait_vm<9>();
     wait_lgkmcnt0();
     __builtin_amdgcn_sched_barrier(0);
     packs();
@@ -352,7 +351,7 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
   // 1: between, 2: the last (quadrant 0 leaves).  Loads issued: the scales of the
   // K tile after the next (rs2 / t2; into the slot of the K tile before this
   // one, which both groups of waves have read two barriers ago) and B1 of the next
-  // (rs1 / t1), then A0, B0, A1 of the one after it.  The waits allow for the 10
+  // (rs1 / t1), then A0, B0, A1 of the one after it.  The waits allow for the 9
   // loads issued since the ones the next phase reads, plus the stores among them
   // while a tile leaves (two per put_rows: 4, 8, 5 and 1 of them).
   auto ktile = [&](auto kind_tag, auto buf_tag, auto tail, const TileRsrc& rs1, int t1, const TileRsrc& rs2, int t2)
@@ -369,11 +368,11 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
     read_scales(l, false, 1, 0, raw[2], raw[3]);
     read_scales(l, true, 0, 0, raw[4], raw[5]);
     read_scales(l, true, 0, 1, raw[6], raw[7]);
-    dma_s(tail, rs2, t2, slot == 0 ? 2 : slot - 1);
+    dma_s(rs2, t2, slot == 0 ? 2 : slot - 1);
     dma_b(tail, rs1, 1, t1);
     if constexpr (KIND == 0)
       if (pend) put_rows(rows, 1, 1, here(lane));
-    end_mem(NTOPS_W(KIND == 0 ? 18 : KIND == 3 ? 20 : 10), [&]() __attribute__((always_inline)) {
+    end_mem(NTOPS_W(KIND == 0 ? 17 : KIND == 3 ? 19 : 9), [&]() __attribute__((always_inline)) {
       sa[0] = pack(raw[0], raw[1]);
       sa[1] = pack(raw[2], raw[3]);
       sb[0] = pack(raw[4], raw[5]);
@@ -399,7 +398,7 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
     dma_a(tail, rs2, 1, t2);
     if constexpr (KIND == 0)
       if (pend) put_rows(rows, 3, 1, here(lane));
-    end_mem(NTOPS_W(KIND == 0 ? 26 : KIND == 3 ? 12 : 10), [&]() __attribute__((always_inline)) {
+    end_mem(NTOPS_W(KIND == 0 ? 25 : KIND == 3 ? 11 : 9), [&]() __attribute__((always_inline)) {
       sb[0] = pack(raw[4], raw[5]);
       sb[1] = pack(raw[6], raw[7]);
     });
@@ -418,16 +417,16 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
   };
 
   // prologue: the first K tile and the scales, A0, B0, A1 of the second in flight
-  dma_s(no, cur, 0, 0);
+  dma_s(cur, 0, 0);
   dma_a(no, cur, 0, 0);
   dma_b(no, cur, 0, 0);
   dma_a(no, cur, 1, 0);
-  dma_s(no, cur, 1, 1);
+  dma_s(cur, 1, 1);
   dma_b(no, cur, 1, 0);
   dma_a(no, cur, 0, 1);
   dma_b(no, cur, 0, 1);
   dma_a(no, cur, 1, 1);
-  wait_vmcnt<10>();
+  wait_vmcnt<9>();
   block_barrier();
   if (grp == 1) block_barrier();
 
@@ -473,6 +472,30 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
   wait_vmcnt<0>();  // no DMA may land after the workgroup ends
 }
 
+// The scales of 256 rows and a K tile of 8 blocks to 2 KiB in a row, by panels of
+// 256 rows, then K tiles; zeros past the rows' last block and the last row.  A
+// thread a row and K tile; blockIdx.z 0: A's, 1: B's.
+__global__ __launch_bounds__(256) void k_mx4_lay_scales(Mx4Args g, uint8_t* a, uint8_t* b) {
+  const bool of_b = blockIdx.z != 0;
+  const int rows = of_b ? g.N : g.M, kt = (g.kb + 7) / 8;
+  const int panel = blockIdx.x, t = blockIdx.y;
+  if (panel * 256 >= rows) return;
+  const int row = panel * 256 + threadIdx.x;
+  const int64_t ld = of_b ? g.ldbs : g.ldas;
+  const uint8_t* from = (of_b ? g.bs : g.as) + row * ld + t * 8;
+  const int n = row < rows ? min(8, g.kb - t * 8) : 0;
+  uint32_t w[2] = {0, 0};
+  if (n == 8 && (reinterpret_cast<uintptr_t>(from) & 7u) == 0) {
+    const u32x2 v = *reinterpret_cast<const u32x2*>(from);
+    w[0] = v.x;
+    w[1] = v.y;
+  } else {
+    for (int e = 0; e < n; ++e) w[e >> 2] |= static_cast<uint32_t>(from[e]) << (8 * (e & 3));
+  }
+  uint8_t* to = (of_b ? b : a) + ((static_cast<int64_t>(panel) * kt + t) * 256 + threadIdx.x) * 8;
+  *reinterpret_cast<u32x2*>(to) = u32x2{w[0], w[1]};
+}
+
 template <typename T, bool BIAS>
 int launch_large(const Mx4Args& g, hipStream_t st) {
   auto kern = k_mx4_large<T, BIAS>;
@@ -498,12 +521,21 @@ int run_large(const Mx4Args& g, hipStream_t st) {
 }  // namespace
 
 bool mx4_large_serves(int out_dtype, const Mx4Args& g) {
-  const auto dwords = [](const uint8_t* s, int64_t ld) { return (reinterpret_cast<uintptr_t>(s) & 3u) == 0 && ld % 4 == 0; };
-  return out_dtype != NTOPS_F32 && g.kb % 8 == 0 && g.kb > 32 && dwords(g.as, g.ldas) && dwords(g.bs, g.ldbs) &&
-         (reinterpret_cast<uintptr_t>(g.bias) & 3u) == 0 && g.ldd >= 0 && (16 * g.ldd + 64) * 2 < (int64_t(1) << 31);
+  return out_dtype != NTOPS_F32 && g.kb > 32 && g.kb <= 65535 * 8 && (reinterpret_cast<uintptr_t>(g.bias) & 3u) == 0 && g.ldd >= 0 &&
+         (16 * g.ldd + 64) * 2 < (int64_t(1) << 31);
 }
 
-int mx4_large(int out_dtype, const Mx4Args& g, hipStream_t st) {
+int64_t mx4_large_workspace(int64_t M, int64_t N, int64_t kb) {
+  return (ceil_div(M, 256) + ceil_div(N, 256)) * ceil_div(kb, 8) * 2048;
+}
+
+int mx4_large(int out_dtype, Mx4Args g, void* workspace, hipStream_t st) {
+  uint8_t* a = static_cast<uint8_t*>(workspace);
+  uint8_t* b = a + ceil_div(g.M, 256) * ceil_div(g.kb, 8) * 2048;
+  const unsigned panels = static_cast<unsigned>(ceil_div(std::max(g.M, g.N), 256));
+  hipLaunchKernelGGL(k_mx4_lay_scales, dim3(panels, static_cast<unsigned>(ceil_div(g.kb, 8)), 2), dim3(256), 0, st, g, a, b);
+  g.as = a;
+  g.bs = b;
   return out_dtype == NTOPS_BF16 ? run_large<__bf16>(g, st) : run_large<_Float16>(g, st);
 }
 

@@ -156,15 +156,19 @@ def test_product(m, n, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("m,n,k", [(2048, 4096, 1280), (2000, 4090, 1792), (1900, 4099, 2048), (2300, 7700, 1536), (8200, 4100, 1312)])
+@pytest.mark.parametrize("m,n,k", [(2048, 4096, 1280), (2000, 4090, 1792), (1900, 4099, 2048), (2300, 7700, 1536), (8200, 4100, 1312), (2100, 4200, 1100), (2050, 4097, 1024)])
 def test_product_large(m, n, k, dtype):
     bias = torch.randn(n).to(dtype).cuda() if n % 4 else None
     args = operands(m, n, k)
     out = check_product(*args, bias, dtype)
-    if k % 256 == 0:
+    if k > 1024:
         assert _lib.last_kernel() == "mxfp4_large"
     for _ in range(3):
         assert torch.equal(nt.mxfp4_mm(*args, bias, dtype=dtype), out)
+    a, sa, b, sb = args
+    wide = torch.full((m, sa.shape[1] + 9), 255, dtype=torch.uint8, device="cuda")
+    wide[:, 3:-6] = sa
+    assert torch.equal(nt.mxfp4_mm(a, wide[:, 3:-6], b, sb, bias, dtype=dtype), out)
 
 
 @pytest.mark.parametrize("m,n,k", [(3, 50, 4096), (64, 200, 512), (260, 300, 1056)])
