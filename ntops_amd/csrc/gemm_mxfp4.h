@@ -3,11 +3,12 @@
 //
 // v_mfma_scale_f32_16x16x128_f8f6f4 on 4-bit data: lane l holds the 16 bytes
 // (32 codes, one block) of row l & 15 and k block l >> 4 of A / B, and that
-// block's scale in one byte of a register; of the result it holds column l & 15
-// and rows 4 (l >> 4) .. + 3.  Which blocks make up the instruction's four does
-// not matter as long as A and B agree: a lane takes neighbouring blocks in
-// consecutive instructions, so that their scales are neighbouring bytes of one
-// register and the instruction's byte select picks them.
+// block's scale in one byte of a register, which the instruction selects; of the
+// result it holds column l & 15 and rows 4 (l >> 4) .. + 3.
+//
+// Blocks keep their order in the LDS: with neighbouring blocks in one lane, whose
+// scales would be neighbouring bytes, the DMA's lanes gathered every second (or
+// eighth) 16 bytes of a line: (16, 4096, 14336) 10.9 -> 13.1 us.
 #pragma once
 
 #include "mfma.h"
@@ -27,15 +28,6 @@ struct Mx4Args {
   float* part;         // split K: fp32 partial products, slice s at s * M * N
   int split, kchunk;   // slices, and the blocks of each
 };
-
-// Of B neighbouring blocks in the LDS, the one kept at place p of its row: lane
-// group q reads places 4 u + q in instruction u = 0 .. B / 4 - 1 -- reads that touch
-// every bank once under the swizzles of mfma.h -- and gets the neighbouring blocks
-// q B / 4 + u.
-template <int B>
-__device__ __forceinline__ int mx4_block(int p) {
-  return (p & 3) * (B / 4) + (p >> 2);
-}
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256, BT == 64 ? 2 : 1) void k_mx4_tile(Mx4Args g, i
 #pragma unroll
     for (int u = 0; u < S::kRowsPerWave / 8; ++u) {
       const int row = wave * S::kRowsPerWave + u * 8 + (lane >> 3);
-      const int blk = b0 + mx4_block<8>(kslot<64>(row, lane & 7));
+      const int blk = b0 + kslot<64>(row, lane & 7);
       const uint32_t dst = st + static_cast<uint32_t>((wave * S::kRowsPerWave + u * 8) * 128);
       dma16(ra, dst, blk < kb1 && row < mv ? static_cast<uint32_t>(row * g.lda + blk * 16) : kOOB);
       dma16(rb, dst + S::kCodes, blk < kb1 && row < nv ? static_cast<uint32_t>(row * g.ldb + blk * 16) : kOOB);
@@ -90,10 +90,10 @@ __global__ __launch_bounds__(256, BT == 64 ? 2 : 1) void k_mx4_tile(Mx4Args g, i
       dma4(rsb, dst + S::kScales, ok && row < nv ? static_cast<uint32_t>(ob + row * g.ldbs + blk) & ~3u : kOOB);
     }
   };
-  // LDS offset of scale byte 0 (K block 2q of a K tile) of row r's area
+  // LDS offset of row r's scales of a K tile (not FIT: of the byte of block q)
   auto scale_at = [&](int r, int o, int64_t ld) {
     const int w = r / S::kRowsPerWave, in_wave = r - w * S::kRowsPerWave;
-    return w * S::kScaleInst * 256 + in_wave * ND * 4 + (FIT ? 0 : static_cast<int>((o + r * ld) & 3)) + 2 * q;
+    return w * S::kScaleInst * 256 + in_wave * ND * 4 + (FIT ? 0 : static_cast<int>((o + r * ld) & 3) + q);
   };
   int sat[TW], sbt[TW];
 #pragma unroll
@@ -118,21 +118,27 @@ __global__ __launch_bounds__(256, BT == 64 ? 2 : 1) void k_mx4_tile(Mx4Args g, i
     issue(j + 3);
     const char* st = smem + (j & (kStages - 1)) * S::kStage;
     uint32_t sa[TW], sb[TW];
+    // the scales of blocks q and q + 4 of each row, in bytes 0 and 1
     if constexpr (FIT) {
+      const uint32_t sel = 0x0400u + q * 0x0101u;
+      const auto two = [&](int at) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(st + at);
+        return __builtin_amdgcn_perm(w.y, w.x, sel);
+      };
 #pragma unroll
       for (int i = 0; i < TW; ++i) {
-        sa[i] = *reinterpret_cast<const uint16_t*>(st + sat[i]);
-        sb[i] = *reinterpret_cast<const uint16_t*>(st + sbt[i]);
+        sa[i] = two(sat[i]);
+        sb[i] = two(sbt[i]);
       }
     } else {
-      const uint32_t left = static_cast<uint32_t>(max(0, kb1 - kb0 - j * 8 - 2 * q));  // blocks from this lane's first on
-      const uint32_t mask = left >= 2 ? 0xffffu : left == 1 ? 0xffu : 0u;
+      const int left = kb1 - kb0 - j * 8 - q;  // blocks from this lane's first on
+      const uint32_t mask = left > 4 ? 0xffffu : left > 0 ? 0xffu : 0u;
 #pragma unroll
       for (int i = 0; i < TW; ++i) {
         const uint8_t* pa = reinterpret_cast<const uint8_t*>(st + sat[i]);
         const uint8_t* pb = reinterpret_cast<const uint8_t*>(st + sbt[i]);
-        sa[i] = (pa[0] | static_cast<uint32_t>(pa[1]) << 8) & mask;
-        sb[i] = (pb[0] | static_cast<uint32_t>(pb[1]) << 8) & mask;
+        sa[i] = (pa[0] | static_cast<uint32_t>(pa[4]) << 8) & mask;
+        sb[i] = (pb[0] | static_cast<uint32_t>(pb[4]) << 8) & mask;
       }
     }
     const auto frag = [&](int area, int r, int ks) {

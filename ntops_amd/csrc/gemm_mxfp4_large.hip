@@ -11,8 +11,8 @@
 // kernel before this one lays them out by (256 rows, K tile), so that they arrive
 // as whole lines: read from the tensors, 8 bytes a row were as many requests as
 // the codes' lines, and 8192 x 4096 x 14336 took 246 us.  A phase reads those of
-// its rows' blocks (k-step ks of lane group q: block 2 q + ks), two 16-row slices
-// to a register; 12 registers that held a pair of K tiles' scales cost 209 spilled
+// its rows' blocks (k-step ks of lane group q: block 4 ks + q; the two are laid next
+// to each other), two 16-row slices to a register; 12 registers that held a pair of K tiles' scales cost 209 spilled
 // ones.
 #include <algorithm>
 #include <atomic>
@@ -49,7 +49,7 @@ struct CodeLoader {
   // the K tile's block that this lane brings with instruction i
   __device__ __forceinline__ static int block(int wave, int lane, int i) {
     const int row = (wave * 2 + i) * 8 + lane / 8;
-    return mx4_block<8>(kslot<64>(row, lane % 8));
+    return kslot<64>(row, lane % 8);
   }
   __device__ __forceinline__ void init(int64_t ld, int wave, int lane) {
     lds_off = static_cast<uint32_t>(wave * 2048);
@@ -473,7 +473,8 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
 }
 
 // The scales of 256 rows and a K tile of 8 blocks to 2 KiB in a row, by panels of
-// 256 rows, then K tiles; zeros past the rows' last block and the last row.  A
+// 256 rows, then K tiles; of a row's 8 those of blocks q and q + 4 are next to each
+// other; zeros past the rows' last block and the last row.  A
 // thread a row and K tile; blockIdx.z 0: A's, 1: B's.
 __global__ __launch_bounds__(256) void k_mx4_lay_scales(Mx4Args g, uint8_t* a, uint8_t* b) {
   const bool of_b = blockIdx.z != 0;
@@ -493,7 +494,8 @@ __global__ __launch_bounds__(256) void k_mx4_lay_scales(Mx4Args g, uint8_t* a, u
     for (int e = 0; e < n; ++e) w[e >> 2] |= static_cast<uint32_t>(from[e]) << (8 * (e & 3));
   }
   uint8_t* to = (of_b ? b : a) + ((static_cast<int64_t>(panel) * kt + t) * 256 + threadIdx.x) * 8;
-  *reinterpret_cast<u32x2*>(to) = u32x2{w[0], w[1]};
+  // bytes 0, 4, 1, 5 and 2, 6, 3, 7
+  *reinterpret_cast<u32x2*>(to) = u32x2{__builtin_amdgcn_perm(w[1], w[0], 0x05010400u), __builtin_amdgcn_perm(w[1], w[0], 0x07030602u)};
 }
 
 template <typename T, bool BIAS>

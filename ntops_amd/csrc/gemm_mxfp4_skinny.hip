@@ -2,18 +2,18 @@
 // (16 + 1) / 32 bytes a value, once.
 //
 // A block covers 16 J columns; its four waves each own K steps of their own and
-// stream them through their own part of the LDS by direct DMA, two or three steps
-// ahead, with no barrier before their fp32 sums are merged.  A step is 8 KiB of B
-// (16 J rows of 512 / J bytes, non-temporal, whole lines), the same columns of
-// A's 16 rows, and the scales.
+// stream them through their own part of the LDS by direct DMA, as many steps ahead
+// as the LDS holds (two to four), with no barrier before their fp32 sums are
+// merged.  A step is 8 KiB of B (16 J rows of 512 / J bytes, non-temporal, whole
+// lines), the same columns of A's rows, and the scales.  Up to 4 rows (MR 4) A's
+// part of a step is a quarter, and the ring a step longer; the instruction's other
+// rows read the four again.
 //
-// A lane takes CPR / 4 neighbouring blocks of its row, one per instruction, so
-// that it needs CPR / 4 neighbouring bytes of the row's scales.  Those are loaded
-// as the dwords that the step's CPR bytes lie in (one more than they fill, as a
-// row may start inside one) and shifted into place; bytes behind the row's last
-// block become 0, as they may be another row's 255.  Such a dword may reach up to
-// 3 bytes past the scales' end or before their start; being aligned it lies
-// within what the memory's page holds.
+// The scales are loaded as the dwords that the step's CPR bytes of a row lie in (one
+// more than they fill, as a row may start inside one) and read as single bytes;
+// bytes behind the row's last block count as 0, as they may be another row's 255.
+// Such a dword may reach up to 3 bytes past the scales' end or before their start;
+// being aligned it lies within what the memory's page holds.
 #include <atomic>
 
 #include "gemm_mxfp4.h"
@@ -27,7 +27,7 @@ constexpr int kWaves = 4;
 // read touch 16 different slots of the LDS's 256 bytes.
 template <int CPR>
 __device__ __forceinline__ int sk_slot(int r, int c) {
-  return c ^ (r & 15);
+  return CPR == 8 ? kslot<64>(r, c) : c ^ (r & 15);
 }
 
 template <bool NT>
@@ -41,18 +41,18 @@ __device__ __forceinline__ void sk_dma(u32x4 rsrc, uint32_t dst, uint32_t off) {
 // One operand's steps: ROWS rows of CPR blocks, and their scales.
 template <int ROWS, int CPR, bool NT>
 struct Loader {
-  static constexpr int kInst = ROWS * CPR / 64;
+  static constexpr int kInst = (ROWS * CPR + 63) / 64;
   static constexpr int kRpi = 64 / CPR;  // rows per instruction
   static constexpr int ND = CPR / 4 + 1;  // dwords of a row's scales
   static constexpr int kScaleInst = (ROWS * ND + 63) / 64;
-  static constexpr int kBytes = ROWS * CPR * 16, kScaleBytes = kScaleInst * 256;
+  static constexpr int kBytes = kInst * 1024, kScaleBytes = kScaleInst * 256;
   u32x4 codes, scales;
   uint32_t voff[kInst], soff[kScaleInst];
   int kb;
 
   // the step's block that this lane brings with instruction i
   __device__ __forceinline__ static int chunk(int lane, int i) {
-    return mx4_block<CPR>(sk_slot<CPR>(i * kRpi + lane / CPR, lane % CPR));
+    return sk_slot<CPR>(i * kRpi + lane / CPR, lane % CPR);
   }
   // rows: valid ones
   __device__ __forceinline__ void init(const uint8_t* c, int64_t ld, const uint8_t* s, int64_t lds, int rows, int blocks,
@@ -64,7 +64,7 @@ struct Loader {
 #pragma unroll
     for (int i = 0; i < kInst; ++i) {
       const int r = i * kRpi + lane / CPR;
-      voff[i] = r < rows ? static_cast<uint32_t>(r * ld + chunk(lane, i) * 16) : kOOB;
+      voff[i] = r < rows && r < ROWS ? static_cast<uint32_t>(r * ld + chunk(lane, i) * 16) : kOOB;
     }
 #pragma unroll
     for (int i = 0; i < kScaleInst; ++i) {
@@ -83,15 +83,26 @@ struct Loader {
   }
 };
 
-template <typename T, int J>
-__global__ __launch_bounds__(64 * kWaves, 1) void k_mx4_skinny(Mx4Args g, int whole) {
-  constexpr int CPR = 32 / J;        // blocks of a row per step
-  constexpr int S = J == 1 ? 2 : 3;  // steps in the ring
-  constexpr int NB = CPR / 4;        // blocks of a lane, and bytes of its scales (8 or 4)
-  using LA = Loader<16, CPR, false>;
+// Steps in the ring: what fits into a CU's LDS.
+template <int J, int MR>
+struct Ring {
+  static constexpr int CPR = 32 / J;  // blocks of a row per step
+  using LA = Loader<MR, CPR, false>;
   using LB = Loader<16 * J, CPR, true>;
-  constexpr int kStepA = LA::kBytes + LA::kScaleBytes, kStepB = LB::kBytes + LB::kScaleBytes;
-  constexpr int kStep = kStepA + kStepB;
+  static constexpr int kStepB = LB::kBytes + LB::kScaleBytes;
+  static constexpr int kStep = kStepB + LA::kBytes + LA::kScaleBytes;
+  static constexpr int kFit = 163840 / (kWaves * kStep);
+  static constexpr int S = kFit < 4 ? kFit : 4;
+  static constexpr int kLds = kWaves * S * kStep;
+};
+
+template <typename T, int J, int MR>
+__global__ __launch_bounds__(64 * kWaves, 1) void k_mx4_skinny(Mx4Args g, int whole) {
+  using R = Ring<J, MR>;
+  using LA = typename R::LA;
+  using LB = typename R::LB;
+  constexpr int CPR = R::CPR, S = R::S, kStep = R::kStep, kStepB = R::kStepB;
+  constexpr int NB = CPR / 4;  // instructions of a step: block 4 u + q in lane group q
   constexpr int kInst = LA::kInst + LA::kScaleInst + LB::kInst + LB::kScaleInst;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63;
@@ -117,22 +128,14 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_mx4_skinny(Mx4Args g, int wh
     la.issue(dst + kStepB, b0, j < n, lane);
     slot_in = slot_in + 1 == S ? 0 : slot_in + 1;
   };
-  // bits that this lane's scales are shifted by
-  const uint32_t sha = (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(g.as) + i16 * g.ldas) & 3u) * 8;
-  uint32_t shb[J];
+  // this lane's first scale byte in a step's dwords: of its row of A, of its columns
+  const int ar = i16 & (MR - 1);
+  const int sat = LA::kBytes + ar * (LA::ND * 4) + static_cast<int>((reinterpret_cast<uintptr_t>(g.as) + ar * g.ldas) & 3u) + q;
+  int sbt[J];
 #pragma unroll
   for (int j = 0; j < J; ++j)
-    shb[j] = (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(g.bs) + (n0 + j * 16 + i16) * g.ldbs) & 3u) * 8;
-  // the lane's NB scale bytes of row r
-  auto scales = [&](const char* at, int r, uint32_t shift, int left, uint32_t (&o)[NB / 4]) {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(at) + r * LB::ND + q * (NB / 4);
-#pragma unroll
-    for (int u = 0; u < NB / 4; ++u) {
-      o[u] = __builtin_amdgcn_alignbit(w[u + 1], w[u], shift);
-      const int valid = left - 4 * u;  // blocks of this word
-      if (valid < 4) o[u] &= valid <= 0 ? 0u : (1u << (8 * valid)) - 1;
-    }
-  };
+    sbt[j] = LB::kBytes + (j * 16 + i16) * (LB::ND * 4) +
+             static_cast<int>((reinterpret_cast<uintptr_t>(g.bs) + (n0 + j * 16 + i16) * g.ldbs) & 3u) + q;
   f32x4 acc[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -146,25 +149,20 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_mx4_skinny(Mx4Args g, int wh
     __builtin_amdgcn_sched_barrier(0);
     const char* tb = mine + slot * kStep;
     const char* ta = tb + kStepB;
-    const int left = g.kb - (wave + i * kWaves) * CPR - q * NB;  // blocks from this lane's first on
-    uint32_t sa[NB / 4], sb[J][NB / 4];
-    scales(ta + LA::kBytes, i16, sha, left, sa);
-#pragma unroll
-    for (int j = 0; j < J; ++j) scales(tb + LB::kBytes, j * 16 + i16, shb[j], left, sb[j]);
+    const int left = g.kb - (wave + i * kWaves) * CPR;  // blocks of the row from the step's first on
 #pragma unroll
     for (int u = 0; u < NB; ++u) {
-      const int c = 4 * u + q;  // holds block q NB + u
-      const u32x4 a = *reinterpret_cast<const u32x4*>(ta + i16 * (CPR * 16) + sk_slot<CPR>(i16, c) * 16);
+      const int c = 4 * u + q;
+      const u32x4 a = *reinterpret_cast<const u32x4*>(ta + ar * (CPR * 16) + sk_slot<CPR>(ar, c) * 16);
+      uint32_t sa = *reinterpret_cast<const uint8_t*>(ta + sat + 4 * u);
+      if (left < CPR) sa = c < left ? sa : 0;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const int r = j * 16 + i16;
         const u32x4 b = *reinterpret_cast<const u32x4*>(tb + r * (CPR * 16) + sk_slot<CPR>(r, c) * 16);
-        switch (u & 3) {
-          case 0: acc[j] = mfma_mx4<0, 0>(b, sb[j][u >> 2], a, sa[u >> 2], acc[j]); break;
-          case 1: acc[j] = mfma_mx4<1, 1>(b, sb[j][u >> 2], a, sa[u >> 2], acc[j]); break;
-          case 2: acc[j] = mfma_mx4<2, 2>(b, sb[j][u >> 2], a, sa[u >> 2], acc[j]); break;
-          default: acc[j] = mfma_mx4<3, 3>(b, sb[j][u >> 2], a, sa[u >> 2], acc[j]); break;
-        }
+        uint32_t sb = *reinterpret_cast<const uint8_t*>(tb + sbt[j] + 4 * u);
+        if (left < CPR) sb = c < left ? sb : 0;
+        acc[j] = mfma_mx4<0, 0>(b, sb, a, sa, acc[j]);
       }
     }
     wait_lgkmcnt0();
@@ -190,14 +188,10 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_mx4_skinny(Mx4Args g, int wh
   }
 }
 
-template <typename T, int J>
+template <typename T, int J, int MR>
 int launch_skinny(const Mx4Args& g, hipStream_t st) {
-  constexpr int CPR = 32 / J;
-  using LA = Loader<16, CPR, false>;
-  using LB = Loader<16 * J, CPR, true>;
-  constexpr int kLds = kWaves * (J == 1 ? 2 : 3) * (LA::kBytes + LA::kScaleBytes + LB::kBytes + LB::kScaleBytes);
-  static_assert(kLds <= 163840, "LDS");
-  auto kern = k_mx4_skinny<T, J>;
+  constexpr int kLds = Ring<J, MR>::kLds;
+  auto kern = k_mx4_skinny<T, J, MR>;
   static std::atomic<bool> attr_set{false};  // (threads may get here together)
   if (!attr_set.load(std::memory_order_relaxed)) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) !=
@@ -206,19 +200,39 @@ int launch_skinny(const Mx4Args& g, hipStream_t st) {
     attr_set.store(true, std::memory_order_relaxed);
   }
   const int whole = (g.ldd & 3) == 0 && (reinterpret_cast<uintptr_t>(g.d) & (4 * sizeof(T) - 1)) == 0;
-  note_kernel("mxfp4_skinny j%d", J);
+  note_kernel("mxfp4_skinny j%d m%d", J, MR);
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((g.N + 16 * J - 1) / (16 * J))), dim3(64 * kWaves), kLds, st, g, whole);
   return check_launch("mxfp4_mm");
+}
+
+template <typename T, int MR>
+int run_skinny(const Mx4Args& g, int j, hipStream_t st) {
+  return j == 4 ? launch_skinny<T, 4, MR>(g, st) : j == 2 ? launch_skinny<T, 2, MR>(g, st) : launch_skinny<T, 1, MR>(g, st);
+}
+
+// Columns of a block, in 16s: a CU takes its blocks one after the other, each at
+// the cost of its start (as much as 48 KiB of B) and its bytes.
+int columns(int64_t N, int64_t kb) {
+  int best = 1;
+  int64_t least = 0;
+  for (int j = 1; j <= 4; j *= 2) {
+    const int64_t rounds = ceil_div(ceil_div(N, 16 * j), cu_count_cached());
+    const int64_t cost = rounds * (48 * 1024 + 16 * j * kb * 16);
+    if (j == 1 || cost <= least) {
+      least = cost;
+      best = j;
+    }
+  }
+  return best;
 }
 
 }  // namespace
 
 int mx4_skinny(int out_dtype, const Mx4Args& g, hipStream_t st) {
-  // 32 columns a block from a block per CU on
-  const bool wide = g.N >= 32 * cu_count_cached();
+  const int j = columns(g.N, g.kb);
   return dispatch_float16_32(out_dtype, "mxfp4_mm", [&](auto tag) {
     using T = decltype(tag);
-    return wide ? launch_skinny<T, 2>(g, st) : launch_skinny<T, 1>(g, st);
+    return g.M <= 4 ? run_skinny<T, 4>(g, j, st) : run_skinny<T, 16>(g, j, st);
   });
 }
 
