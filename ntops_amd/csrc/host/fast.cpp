@@ -22,6 +22,7 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/core/DispatchKeySet.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -43,6 +44,13 @@ decltype(&ntops_gemm_workspace) f_gemm_workspace;
 decltype(&ntops_sdpa_ws) f_sdpa_ws;
 decltype(&ntops_sdpa_workspace) f_sdpa_workspace;
 decltype(&ntops_copy2) f_copy2;
+decltype(&ntops_quantize_mxfp4) f_quantize_mxfp4;
+decltype(&ntops_dequantize_mxfp4) f_dequantize_mxfp4;
+decltype(&ntops_mxfp4_mm) f_mxfp4_mm;
+decltype(&ntops_mxfp4_mm_workspace) f_mxfp4_mm_workspace;
+decltype(&ntops_store_kv_cache) f_store_kv_cache;
+decltype(&ntops_kv_cache_attention) f_kv_cache_attention;
+decltype(&ntops_kv_cache_attention_workspace) f_kv_cache_attention_workspace;
 bool ready = false;
 PyObject* get_device = nullptr;  // torch._C._cuda_getDevice
 PyObject* get_stream = nullptr;  // torch._C._cuda_getCurrentRawStream
@@ -504,6 +512,259 @@ PyObject* sdpa(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NTOPS_END
 }
 
+// A torch.dtype's code in the C ABI (F32 / F16 / BF16) and scalar type.
+bool float_dtype(PyObject* o, int& code, at::ScalarType& type) {
+  if (!THPDtype_Check(o)) return false;
+  type = reinterpret_cast<THPDtype*>(o)->scalar_type;
+  code = type == at::kFloat ? NTOPS_F32 : type == at::kHalf ? NTOPS_F16 : type == at::kBFloat16 ? NTOPS_BF16 : -1;
+  return code >= 0;
+}
+
+at::Tensor bytes_like(const at::Tensor& t, c10::IntArrayRef sizes) {
+  return at::empty(sizes, at::TensorOptions().dtype(at::kByte).device(t.device()));
+}
+
+// quantize_mxfp4(input): a contiguous input
+PyObject* quantize_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NTOPS_TRY
+  if (n != 1 || !usable()) return none();
+  const at::Tensor* x = plain(a[0]);
+  int64_t dev;
+  void* st;
+  if (!x || code16_32(*x) < 0 || x->dim() < 1 || !x->is_contiguous() || x->numel() == 0 || !current(dev, st) ||
+      x->get_device() != dev)
+    return none();
+  const int64_t cols = x->size(-1), rows = x->numel() / cols, blocks = (cols + 31) / 32;
+  auto sizes = x->sizes().vec();
+  at::Tensor codes, scales;
+  int rc;
+  {
+    NoGil free;
+    sizes.back() = 16 * blocks;
+    codes = bytes_like(*x, sizes);
+    sizes.back() = blocks;
+    scales = bytes_like(*x, sizes);
+    rc = f_quantize_mxfp4(code16_32(*x), rows, cols, x->data_ptr(), cols, codes.data_ptr(), scales.data_ptr(), st);
+  }
+  return rc == NTOPS_OK ? wrap2(codes, scales) : none();
+  NTOPS_END
+}
+
+// Blocks along the last dim of an MXFP4 pair on `dev`; -1: the Python path.
+int64_t mx4_blocks(const at::Tensor* codes, const at::Tensor* scales, int64_t dev) {
+  if (!codes || !scales || codes->scalar_type() != at::kByte || scales->scalar_type() != at::kByte || codes->dim() < 1 ||
+      scales->dim() != codes->dim() || codes->get_device() != dev || scales->get_device() != dev)
+    return -1;
+  for (int64_t i = 0; i + 1 < codes->dim(); ++i)
+    if (codes->size(i) != scales->size(i)) return -1;
+  return codes->size(-1) == 16 * scales->size(-1) ? scales->size(-1) : -1;
+}
+
+// dequantize_mxfp4(codes, scales, size, dtype): contiguous codes and scales
+PyObject* dequantize_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NTOPS_TRY
+  int code;
+  at::ScalarType type;
+  int64_t dev;
+  void* st;
+  if (n != 4 || !usable() || !float_dtype(a[3], code, type) || !current(dev, st)) return none();
+  const at::Tensor *codes = plain(a[0]), *scales = plain(a[1]);
+  const int64_t blocks = mx4_blocks(codes, scales, dev);
+  if (blocks <= 0 || !codes->is_contiguous() || !scales->is_contiguous() || codes->numel() == 0 ||
+      (reinterpret_cast<uintptr_t>(codes->data_ptr()) & 3u) != 0)
+    return none();
+  int64_t cols = 32 * blocks;
+  if (a[2] != Py_None) {
+    if (!PyLong_CheckExact(a[2])) return none();
+    cols = PyLong_AsLongLong(a[2]);
+    if (cols == -1 && PyErr_Occurred()) PyErr_Clear();
+    if (cols <= 0 || (cols + 31) / 32 != blocks) return none();
+  }
+  auto sizes = codes->sizes().vec();
+  sizes.back() = cols;
+  at::Tensor y;
+  int rc;
+  {
+    NoGil free;
+    y = at::empty(sizes, at::TensorOptions().dtype(type).device(codes->device()));
+    rc = f_dequantize_mxfp4(code, scales->numel() / blocks, cols, codes->data_ptr(), 16 * blocks, scales->data_ptr(), blocks,
+                            y.data_ptr(), st);
+  }
+  return rc == NTOPS_OK ? wrap(y) : none();
+  NTOPS_END
+}
+
+// mxfp4_mm(input, input_scale or None, mat2, mat2_scale, bias or None, dtype):
+// code rows the kernels read in place; a float input contiguous.  Its codes and
+// scales and the product's workspace are one allocation.
+PyObject* mxfp4_mm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NTOPS_TRY
+  int code;
+  at::ScalarType type;
+  int64_t dev;
+  void* st;
+  if (n != 6 || !usable() || !float_dtype(a[5], code, type) || !current(dev, st)) return none();
+  const at::Tensor *x = plain(a[0]), *w = plain(a[2]), *ws = plain(a[3]);
+  const int64_t blocks = mx4_blocks(w, ws, dev);
+  if (!x || x->dim() != 2 || x->get_device() != dev || blocks <= 0 || w->dim() != 2) return none();
+  const auto rows16 = [](const at::Tensor& t) { return t.stride(1) == 1 && t.stride(0) >= 0 && t.stride(0) % 16 == 0 && aligned16(t); };
+  const auto rows1 = [](const at::Tensor& t) { return t.stride(1) == 1 && t.stride(0) >= 0; };
+  const int64_t M = x->size(0), N = w->size(0), K = 32 * blocks;
+  if (M <= 0 || N <= 0 || !rows16(*w) || !rows1(*ws)) return none();
+  const at::Tensor* xs = nullptr;
+  if (a[1] != Py_None) {
+    xs = plain(a[1]);
+    if (mx4_blocks(x, xs, dev) != blocks || !rows16(*x) || !rows1(*xs)) return none();
+  } else if (code16_32(*x) < 0 || !x->is_contiguous() || (x->size(1) + 31) / 32 != blocks) {
+    return none();
+  }
+  const at::Tensor* bias = nullptr;
+  if (a[4] != Py_None) {
+    bias = plain(a[4]);
+    if (!bias || bias->get_device() != dev || bias->scalar_type() != type || bias->dim() != 1 || bias->size(0) != N ||
+        !bias->is_contiguous())
+      return none();
+  }
+  at::Tensor out;
+  int rc = NTOPS_OK;
+  {
+    NoGil free;
+    out = at::empty({M, N}, at::TensorOptions().dtype(type).device(x->device()));
+    const int64_t bytes = f_mxfp4_mm_workspace(M, N, K);
+    const int64_t codes = xs ? 0 : M * 16 * blocks, scales = xs ? 0 : (M * blocks + 15) / 16 * 16;
+    at::Tensor tmp;
+    char* at = nullptr;
+    if (codes + scales + bytes > 0) {
+      tmp = workspace(*x, codes + scales + bytes);
+      at = static_cast<char*>(tmp.data_ptr());
+    }
+    if (!xs)
+      rc = f_quantize_mxfp4(code16_32(*x), M, x->size(1), x->data_ptr(), x->size(1), at, at + codes, st);
+    if (rc == NTOPS_OK)
+      rc = f_mxfp4_mm(code, M, N, K, xs ? x->data_ptr() : at, xs ? x->stride(0) : 16 * blocks, xs ? xs->data_ptr() : at + codes,
+                      xs ? xs->stride(0) : blocks, w->data_ptr(), w->stride(0), ws->data_ptr(), ws->stride(0),
+                      bias ? bias->data_ptr() : nullptr, out.data_ptr(), N, bytes > 0 ? at + codes + scales : nullptr, bytes, st);
+  }
+  return rc == NTOPS_OK ? wrap(out) : none();
+  NTOPS_END
+}
+
+// A cache (key_cache, value_cache, key_scale, value_scale) at a[0 ..] in layouts
+// that need no copy.
+struct Cache {
+  const at::Tensor* t[4];
+  int64_t B, H, C, D;
+  bool read(PyObject* const* a, int64_t block, int64_t dev) {
+    if (block < 16 || (block & (block - 1)) != 0) return false;
+    for (int i = 0; i < 4; ++i) {
+      t[i] = plain(a[i]);
+      if (!t[i] || t[i]->get_device() != dev || t[i]->scalar_type() != (i < 2 ? at::kFloat8_e4m3fn : at::kFloat) ||
+          t[i]->dim() != (i < 2 ? 4 : 3) || t[i]->numel() == 0 || t[i]->stride(-1) != 1)
+        return false;
+      for (int64_t d = 0; d < t[i]->dim(); ++d)
+        if (t[i]->stride(d) == 0 && t[i]->size(d) > 1) return false;
+    }
+    B = t[0]->size(0);
+    H = t[0]->size(1);
+    C = t[0]->size(2);
+    D = t[0]->size(3);
+    const int64_t s[3] = {B, H, (C + block - 1) / block};
+    return t[1]->sizes() == t[0]->sizes() && t[2]->sizes() == c10::IntArrayRef(s, 3) && t[3]->sizes() == t[2]->sizes();
+  }
+};
+
+// An index vector (batch,) or None; false: the Python path.
+bool index_vector(PyObject* o, int64_t batch, int64_t dev, const at::Tensor*& t, int& code) {
+  t = nullptr;
+  code = 0;
+  if (o == Py_None) return true;
+  t = plain(o);
+  if (!t || t->get_device() != dev || t->dim() != 1 || t->size(0) != batch || !t->is_contiguous()) return false;
+  code = t->scalar_type() == at::kInt ? NTOPS_I32 : t->scalar_type() == at::kLong ? NTOPS_I64 : -1;
+  return code >= 0;
+}
+
+// store_kv_cache(key, value, key_cache, value_cache, key_scale, value_scale,
+// positions (int or tensor), lengths or None, block_size): True when stored
+PyObject* store_kv_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NTOPS_TRY
+  int64_t dev;
+  void* st;
+  if (n != 9 || !usable() || !PyLong_CheckExact(a[8]) || !current(dev, st)) return none();
+  const int64_t block = PyLong_AsLongLong(a[8]);
+  Cache c;
+  const at::Tensor *k = plain(a[0]), *v = plain(a[1]), *pos = nullptr, *len = nullptr;
+  if (!k || !v || !c.read(a + 2, block, dev) || k->dim() != 4 || v->sizes() != k->sizes() || code16_32(*k) < 0 ||
+      v->scalar_type() != k->scalar_type() || k->get_device() != dev || v->get_device() != dev || k->size(0) != c.B ||
+      k->size(1) != c.H || k->size(2) <= 0 || k->size(3) != c.D || k->stride(3) != 1 || v->stride(3) != 1)
+    return none();
+  int64_t position = 0;
+  int pcode = 0, lcode;
+  if (PyLong_CheckExact(a[6])) {
+    position = PyLong_AsLongLong(a[6]);
+    if (position == -1 && PyErr_Occurred()) {
+      PyErr_Clear();
+      return none();
+    }
+  } else if (a[6] == Py_None || !index_vector(a[6], c.B, dev, pos, pcode)) {
+    return none();
+  }
+  if (!index_vector(a[7], c.B, dev, len, lcode)) return none();
+  int rc;
+  {
+    NoGil free;
+    rc = f_store_kv_cache(code16_32(*k), c.B, c.H, k->size(2), c.D, c.C, block, k->data_ptr(), k->strides().data(), v->data_ptr(),
+                          v->strides().data(), c.t[0]->data_ptr(), c.t[0]->strides().data(), c.t[1]->data_ptr(),
+                          c.t[1]->strides().data(), static_cast<float*>(c.t[2]->data_ptr()), c.t[2]->strides().data(),
+                          static_cast<float*>(c.t[3]->data_ptr()), c.t[3]->strides().data(), pos ? pos->data_ptr() : nullptr,
+                          pcode, position, len ? len->data_ptr() : nullptr, lcode, st);
+  }
+  if (rc != NTOPS_OK) return none();
+  Py_RETURN_TRUE;
+  NTOPS_END
+}
+
+// kv_cache_attention(query, key_cache, value_cache, key_scale, value_scale,
+// lengths or None, is_causal, scale (None: 1 / sqrt(D)), block_size)
+PyObject* kv_cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NTOPS_TRY
+  int64_t dev;
+  void* st;
+  if (n != 9 || !usable() || !PyBool_Check(a[6]) || !PyLong_CheckExact(a[8]) || !current(dev, st)) return none();
+  const int64_t block = PyLong_AsLongLong(a[8]);
+  Cache c;
+  const at::Tensor *q = plain(a[0]), *len = nullptr;
+  int lcode;
+  if (!q || !c.read(a + 1, block, dev) || q->dim() != 4 || code16_32(*q) < 0 || q->get_device() != dev || q->numel() == 0 ||
+      q->size(0) != c.B || q->size(3) != c.D || q->stride(3) != 1 || q->size(1) % c.H != 0 ||
+      !index_vector(a[5], c.B, dev, len, lcode))
+    return none();
+  double scale;
+  if (a[7] == Py_None)
+    scale = 1.0 / std::sqrt(static_cast<double>(c.D));
+  else if (!number(a[7], scale))
+    return none();
+  const int code = code16_32(*q);
+  const int64_t Hq = q->size(1), Sq = q->size(2);
+  at::Tensor out;
+  int rc;
+  {
+    NoGil free;
+    out = new_like(*q, q->sizes());
+    const int64_t bytes = f_kv_cache_attention_workspace(code, c.B, Hq, c.H, Sq, c.C, c.D);
+    at::Tensor ws;
+    if (bytes > 0) ws = workspace(*q, bytes);
+    rc = f_kv_cache_attention(code, c.B, Hq, c.H, Sq, c.C, c.D, block, q->data_ptr(), q->strides().data(), c.t[0]->data_ptr(),
+                              c.t[0]->strides().data(), c.t[1]->data_ptr(), c.t[1]->strides().data(),
+                              static_cast<const float*>(c.t[2]->data_ptr()), c.t[2]->strides().data(),
+                              static_cast<const float*>(c.t[3]->data_ptr()), c.t[3]->strides().data(),
+                              len ? len->data_ptr() : nullptr, lcode, a[6] == Py_True ? 1 : 0, scale, out.data_ptr(),
+                              out.strides().data(), bytes > 0 ? ws.data_ptr() : nullptr, bytes, st);
+  }
+  return rc == NTOPS_OK ? wrap(out) : none();
+  NTOPS_END
+}
+
 // init({name: address}, get_device, get_stream)
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 3 || !PyDict_Check(a[0])) {
@@ -521,7 +782,11 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
                    set("ntops_layer_norm", f_layer_norm) & set("ntops_add_rms_norm", f_add_rms_norm) &
                    set("ntops_rope_qk", f_rope_qk) & set("ntops_gemm_ws", f_gemm_ws) &
                    set("ntops_gemm_workspace", f_gemm_workspace) & set("ntops_sdpa_ws", f_sdpa_ws) &
-                   set("ntops_sdpa_workspace", f_sdpa_workspace) & set("ntops_copy2", f_copy2);
+                   set("ntops_sdpa_workspace", f_sdpa_workspace) & set("ntops_copy2", f_copy2) &
+                   set("ntops_quantize_mxfp4", f_quantize_mxfp4) & set("ntops_dequantize_mxfp4", f_dequantize_mxfp4) &
+                   set("ntops_mxfp4_mm", f_mxfp4_mm) & set("ntops_mxfp4_mm_workspace", f_mxfp4_mm_workspace) &
+                   set("ntops_store_kv_cache", f_store_kv_cache) & set("ntops_kv_cache_attention", f_kv_cache_attention) &
+                   set("ntops_kv_cache_attention_workspace", f_kv_cache_attention_workspace);
   if (PyErr_Occurred()) return nullptr;
   Py_INCREF(a[1]);
   Py_INCREF(a[2]);
@@ -536,7 +801,8 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define NTOPS_M(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {NTOPS_M(init),         NTOPS_M(unary),   NTOPS_M(softmax), NTOPS_M(rms_norm), NTOPS_M(layer_norm),
                          NTOPS_M(add_rms_norm), NTOPS_M(rope_qk), NTOPS_M(mm),      NTOPS_M(addmm),    NTOPS_M(sdpa),
-                         {nullptr, nullptr, 0, nullptr}};
+                         NTOPS_M(quantize_mxfp4), NTOPS_M(dequantize_mxfp4), NTOPS_M(mxfp4_mm), NTOPS_M(store_kv_cache),
+                         NTOPS_M(kv_cache_attention), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", "native host path of the torch wrappers", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 

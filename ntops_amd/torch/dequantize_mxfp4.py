@@ -27,6 +27,10 @@ def _checked_pair(codes, scales, what):
 
 
 def dequantize_mxfp4(codes, scales, size=None, *, dtype=torch.bfloat16):
+    if _lib.fast is not None:
+        r = _lib.fast.dequantize_mxfp4(codes, scales, size, dtype)
+        if r is not None:
+            return r
     blocks = _checked_pair(codes, scales, "dequantize_mxfp4")
     if dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise RuntimeError(f"dequantize_mxfp4: unsupported dtype {dtype}")

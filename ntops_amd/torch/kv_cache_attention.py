@@ -23,6 +23,11 @@ from ntops_amd.torch.utils import _DeviceGuard, _contiguous, _strides
 def kv_cache_attention(
     query, key_cache, value_cache, key_scale, value_scale, lengths=None, is_causal=False, scale=None, *, block_size=64
 ):
+    if _lib.fast is not None:
+        r = _lib.fast.kv_cache_attention(
+            query, key_cache, value_cache, key_scale, value_scale, lengths, is_causal, scale, block_size)
+        if r is not None:
+            return r
     what = "kv_cache_attention"
     b, hkv, c, d = _checked_cache(key_cache, value_cache, key_scale, value_scale, block_size, what)
     if query.dim() != 4 or query.shape[0] != b or query.shape[3] != d:

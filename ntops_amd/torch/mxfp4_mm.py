@@ -25,6 +25,10 @@ def _code_rows(t):
 
 
 def mxfp4_mm(input, input_scale, mat2, mat2_scale, bias=None, *, dtype=torch.bfloat16):
+    if _lib.fast is not None:
+        r = _lib.fast.mxfp4_mm(input, input_scale, mat2, mat2_scale, bias, dtype)
+        if r is not None:
+            return r
     if input.dim() != 2 or mat2.dim() != 2:
         raise RuntimeError("mxfp4_mm: expected 2-D tensors")
     if dtype not in (torch.float32, torch.float16, torch.bfloat16):

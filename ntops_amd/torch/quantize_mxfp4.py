@@ -31,6 +31,10 @@ def _rows(t):
 
 
 def quantize_mxfp4(input):
+    if _lib.fast is not None:
+        r = _lib.fast.quantize_mxfp4(input)
+        if r is not None:
+            return r
     if input.dim() == 0:
         raise RuntimeError("quantize_mxfp4: expected a tensor of at least one dim")
     if input.dtype not in _DTYPES:

@@ -48,6 +48,10 @@ def _check_index(t, batch, name, what):
 
 
 def store_kv_cache(key, value, key_cache, value_cache, key_scale, value_scale, positions, lengths=None, *, block_size=64):
+    if _lib.fast is not None and _lib.fast.store_kv_cache(
+        key, value, key_cache, value_cache, key_scale, value_scale, positions, lengths, block_size
+    ):
+        return
     what = "store_kv_cache"
     b, h, c, d = _checked_cache(key_cache, value_cache, key_scale, value_scale, block_size, what)
     if key.dim() != 4 or key.shape != value.shape or key.shape[:2] != (b, h) or key.shape[3] != d:
