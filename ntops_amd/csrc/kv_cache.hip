@@ -30,7 +30,7 @@ struct StoreArgs {
   int64_t position;      // of every sequence, without positions
   int64_t B, H, S, C;
   int D, shift;          // block = 1 << shift tokens
-  int64_t units;         // blocks that a sequence's tokens can lie in
+  int64_t units;         // blocks that a sequence's tokens can lie in: the grid is (units, H, B), a wave for keys and one for values
 };
 
 constexpr int kSlots = 16;  // packs of 8 values a lane keeps
@@ -51,111 +51,231 @@ struct Divide {
   __device__ __forceinline__ float operator()(float x) const { return pow2 ? x * inv : x / s; }
 };
 
-// VEC: 8 values at a time (head dim a multiple of 8, aligned rows), else one.
-template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void k_store_kv_cache(StoreArgs a) {
-  constexpr int N = VEC ? 8 : 1;
-  const int lane = threadIdx.x & 63;
-  int64_t id = block_id() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int which = static_cast<int>(id & 1);
-  id >>= 1;
-  const int64_t unit = id % a.units;
-  id /= a.units;
-  const int64_t h = id % a.H, b = id / a.H;
-  if (b >= a.B) return;
-  int64_t start = index_at(a.positions, a.positions_dtype, b, a.position);
-  start = max(-a.S, min(a.C, start));
-  const int64_t count = max(int64_t(0), min(a.S, index_at(a.lengths, a.lengths_dtype, b, a.S)));
-  const int64_t lo = max(int64_t(0), start), hi = min(a.C, start + count);
-  const int64_t j = (lo >> a.shift) + unit;
-  const int64_t first = j << a.shift;  // of the block
-  const int64_t p0 = max(lo, first), p1 = min(hi, first + (int64_t(1) << a.shift));
-  if (p0 >= p1) return;
-
-  const T* x = static_cast<const T*>(a.x[which]) + b * a.xs[which][0] + h * a.xs[which][1] + (p0 - start) * a.xs[which][2];
-  uint8_t* c = a.cache[which] + b * a.cs[which][0] + h * a.cs[which][1] + p0 * a.cs[which][2];
-  float* sp = a.scale[which] + b * a.ss[which][0] + h * a.ss[which][1] + j;
-  const int per = a.D / N;  // slots of a token
-  const int total = static_cast<int>(p1 - p0) * per;
-  const auto load = [&](int s, float (&v)[8]) {
-    const int t = s / per, d = (s - t * per) * N;
-    const T* at = x + t * a.xs[which][2] + d;
-    if constexpr (VEC) {
-#pragma unroll
-      for (int k = 0; k < static_cast<int>(sizeof(T)) / 2; ++k) {
-        const Pack16<T> p = load16(at + k * Pack16<T>::N);
-#pragma unroll
-        for (int e = 0; e < Pack16<T>::N; ++e) v[k * Pack16<T>::N + e] = static_cast<float>(p.v[e]);
-      }
-    } else {
-      v[0] = static_cast<float>(*at);
-    }
-  };
-  uint32_t top = 0;
-  const auto grow = [&](const float (&v)[8]) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const uint32_t m = __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu;
-      top = max(top, m < 0x7f800000u ? m : 0u);
-    }
-  };
-  const auto store = [&](int s, const float (&v)[8], const Divide& by) {
-    const int t = s / per, d = (s - t * per) * N;
-    uint8_t* at = c + t * a.cs[which][2] + d;
-    float r[8];
-#pragma unroll
-    for (int e = 0; e < N; ++e) r[e] = by(v[e]);
-    if constexpr (VEC)
-      *reinterpret_cast<u32x2*>(at) = to_e4m3(r);
-    else
-      *at = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(r[0], 0.f, 0, false));
-  };
-  constexpr int kKept = VEC ? kSlots : 1;
-  float v[kKept][8];
-  const float old = p0 > first ? *sp : 0.f;
-#pragma unroll
-  for (int i = 0; i < kKept; ++i)
-    if (i * 64 + lane < total) load(i * 64 + lane, v[i]);
-#pragma unroll
-  for (int i = 0; i < kKept; ++i)
-    if (i * 64 + lane < total) grow(v[i]);
-  for (int s = kKept * 64 + lane; s < total; s += 64) {
-    float w[8];
-    load(s, w);
-    grow(w);
+// What a wave's lanes do next: slot l, l + 64, .. of rows of `per` slots.
+struct Walk {
+  int row, col, per, drow, dcol;
+  __device__ __forceinline__ Walk(int first, int per_row) : per(per_row) {
+    row = first / per;
+    col = first - row * per;
+    drow = 64 / per;
+    dcol = 64 - drow * per;
   }
+  __device__ __forceinline__ void next() {
+    row += drow;
+    col += dcol;
+    if (col >= per) {
+      col -= per;
+      ++row;
+    }
+  }
+};
+
+// Where a wave's tokens lie.
+struct Unit {
+  int which;
+  int64_t b, h, j;         // sequence, head, block
+  int64_t start, p0, p1;   // position of the sequence's first token; positions of the block's new tokens
+  int64_t first;           // of the block
+  __device__ __forceinline__ bool find(const StoreArgs& a) {
+    which = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    h = blockIdx.y;
+    b = blockIdx.z;
+    start = max(-a.S, min(a.C, index_at(a.positions, a.positions_dtype, b, a.position)));
+    const int64_t count = max(int64_t(0), min(a.S, index_at(a.lengths, a.lengths_dtype, b, a.S)));
+    const int64_t lo = max(int64_t(0), start), hi = min(a.C, start + count);
+    j = (lo >> a.shift) + blockIdx.x;
+    first = j << a.shift;
+    p0 = max(lo, first);
+    p1 = min(hi, first + (int64_t(1) << a.shift));
+    return p0 < p1;
+  }
+};
+
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+  // (bits of a non-negative float: the float's order)
+  return __builtin_bit_cast(uint32_t, wave_max(__builtin_bit_cast(float, v)));
+}
+
+__device__ __forceinline__ void grow(uint32_t& top, float v) {
+  const uint32_t m = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
+  top = max(top, m < 0x7f800000u ? m : 0u);
+}
+
+// Largest |x| so far, of 2 16-bit values in a register or of one fp32, as its bits
+// (a NaN's above an infinity's above any number's).
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void grow_word(u16x2& top, uint32_t w, _Float16) {
+  top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w & 0x7fff7fffu));
+}
+__device__ __forceinline__ void grow_word(u16x2& top, uint32_t w, __bf16) { grow_word(top, w, _Float16{}); }
+__device__ __forceinline__ void grow_word(uint32_t& top, uint32_t w, float) { top = max(top, w & 0x7fffffffu); }
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(u16x2 t) {  // as fp32 bits
+  const uint16_t m = max(t.x, t.y);
+  return __builtin_bit_cast(uint32_t, static_cast<float>(__builtin_bit_cast(T, m)));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(uint32_t t) { return t; }
+
+// 8 finite values over a power of two, at most 448 of it, to e4m3.
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+template <typename T>
+__device__ __forceinline__ u32x2 scaled_e4m3(const Pack16<T> (&v)[sizeof(T) / 2], float scale) {
+  u32x2 c;
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), m, 64)));
+  for (int i = 0; i < 2; ++i) {
+    s16x2 w = {0, 0};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int e = 4 * i + 2 * h;
+      const T x = v[e / Pack16<T>::N].v[e % Pack16<T>::N], y = v[e / Pack16<T>::N].v[e % Pack16<T>::N + 1];
+      if constexpr (std::is_same<T, __bf16>::value)
+        w = h ? __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, bf16x2{x, y}, scale, true)
+              : __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, bf16x2{x, y}, scale, false);
+      else if constexpr (std::is_same<T, _Float16>::value)
+        w = h ? __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, f16x2{x, y}, scale, true)
+              : __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, f16x2{x, y}, scale, false);
+      else
+        w = h ? __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x, y, scale, true)
+              : __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x, y, scale, false);
+    }
+    c[i] = __builtin_bit_cast(uint32_t, w);
+  }
+  return c;
+}
+
+// 8 values at a time: head dim a multiple of 8, aligned rows, a block's rows within
+// 31-bit byte offsets.  Buffer loads and stores, which end at the block's last
+// value, so that no branch stands between a lane's loads.
+template <typename T>
+__global__ __launch_bounds__(128) void k_store_kv_cache(StoreArgs a) {
+  constexpr int ES = sizeof(T);
+  const int lane = threadIdx.x & 63;
+  Unit u;
+  if (!u.find(a)) return;
+  const int per = a.D / 8;
+  const int rows = static_cast<int>(u.p1 - u.p0), slots = rows * per;
+  const T* x = static_cast<const T*>(a.x[u.which]) + u.b * a.xs[u.which][0] + u.h * a.xs[u.which][1] +
+               (u.p0 - u.start) * a.xs[u.which][2];
+  uint8_t* c = a.cache[u.which] + u.b * a.cs[u.which][0] + u.h * a.cs[u.which][1] + u.p0 * a.cs[u.which][2];
+  float* sp = a.scale[u.which] + u.b * a.ss[u.which][0] + u.h * a.ss[u.which][1] + u.j;
+  const uint32_t xld = static_cast<uint32_t>(a.xs[u.which][2] * ES), cld = static_cast<uint32_t>(a.cs[u.which][2]);
+  const __amdgpu_buffer_rsrc_t rx = buffer_rsrc_uniform(x, (rows - 1) * xld + a.D * ES);
+  const __amdgpu_buffer_rsrc_t rc = buffer_rsrc_uniform(c, (rows - 1) * cld + a.D);
+  const auto load = [&](const Walk& w, bool in, Pack16<T> (&v)[ES / 2]) {
+    const uint32_t at = in ? w.row * xld + w.col * (8 * ES) : kOOB;
+#pragma unroll
+    for (int k = 0; k < ES / 2; ++k)
+      v[k] = __builtin_bit_cast(Pack16<T>, __builtin_amdgcn_raw_buffer_load_b128(rx, at, k * 16, 0));
+  };
+  const auto value = [](const Pack16<T> (&v)[ES / 2], int e) { return static_cast<float>(v[e / Pack16<T>::N].v[e % Pack16<T>::N]); };
+  Pack16<T> v[kSlots][ES / 2];
+  const float old = u.p0 > u.first ? *sp : 0.f;
+  {
+    Walk w(lane, per);
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      load(w, i * 64 + lane < slots, v[i]);
+      w.next();
+    }
+  }
+  const auto words = [](const Pack16<T> (&y)[ES / 2], auto& t) {
+#pragma unroll
+    for (int k = 0; k < ES / 2; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) grow_word(t, __builtin_bit_cast(u32x4, y[k])[e], T{});
+  };
+  std::conditional_t<ES == 2, u16x2, uint32_t> most{};
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i) words(v[i], most);  // (slots past the end read as zero)
+  for (Walk w(lane + kSlots * 64, per); w.row < rows; w.next()) {
+    Pack16<T> y[ES / 2];
+    load(w, true, y);
+    words(y, most);
+  }
+  uint32_t top = wave_max_bits(top_bits<T>(most));
+  const bool finite = top < 0x7f800000u;
+  if (!finite) {  // once more, over the finite values
+    top = 0;
+    for (Walk w(lane, per); w.row < rows; w.next()) {
+      Pack16<T> y[ES / 2];
+      load(w, true, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) grow(top, value(y, e));
+    }
+    top = wave_max_bits(top);
+  }
   const float fits = least_scale(top);
   const bool keeps = old > fits;
   const float scale = keeps ? old : fits;
   const Divide by(scale);
+  if (finite && by.pow2) {
+    Walk w(lane, per);
 #pragma unroll
-  for (int i = 0; i < kKept; ++i)
-    if (i * 64 + lane < total) store(i * 64 + lane, v[i], by);
-  for (int s = kKept * 64 + lane; s < total; s += 64) {
-    float w[8];
-    load(s, w);
-    store(s, w, by);
-  }
-  if (p0 > first && !keeps && old != fits) {
-    const float ratio = old / fits;
-    uint8_t* o = a.cache[which] + b * a.cs[which][0] + h * a.cs[which][1] + first * a.cs[which][2];
-    const int before = static_cast<int>(p0 - first) * per;
-    for (int s = lane; s < before; s += 64) {
-      const int t = s / per, d = (s - t * per) * N;
-      uint8_t* at = o + t * a.cs[which][2] + d;
-      float w[8];
-      if constexpr (VEC) {
-        from_e4m3(*reinterpret_cast<const u32x2*>(at), w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] *= ratio;
-        *reinterpret_cast<u32x2*>(at) = to_e4m3(w);
-      } else {
-        w[0] = __builtin_amdgcn_cvt_f32_fp8(*at, 0) * ratio;
-        *at = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(w[0], 0.f, 0, false));
-      }
+    for (int i = 0; i < kSlots; ++i) {
+      if (i * 64 < slots)
+        __builtin_amdgcn_raw_buffer_store_b64(scaled_e4m3<T>(v[i], scale), rc, i * 64 + lane < slots ? w.row * cld + w.col * 8 : kOOB, 0, 0);
+      w.next();
     }
+    for (; w.row < rows; w.next()) {
+      Pack16<T> y[ES / 2];
+      load(w, true, y);
+      __builtin_amdgcn_raw_buffer_store_b64(scaled_e4m3<T>(y, scale), rc, w.row * cld + w.col * 8, 0, 0);
+    }
+  } else {
+    for (Walk w(lane, per); w.row < rows; w.next()) {
+      Pack16<T> y[ES / 2];
+      load(w, true, y);
+      float r[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = by(value(y, e));
+      __builtin_amdgcn_raw_buffer_store_b64(to_e4m3(r), rc, w.row * cld + w.col * 8, 0, 0);
+    }
+  }
+  if (u.p0 > u.first && !keeps && old != fits) {
+    const float ratio = old / fits;
+    uint8_t* o = c - (u.p0 - u.first) * a.cs[u.which][2];
+    const int before = static_cast<int>(u.p0 - u.first);
+    for (Walk r(lane, per); r.row < before; r.next()) {
+      u32x2* at = reinterpret_cast<u32x2*>(o + static_cast<int64_t>(r.row) * a.cs[u.which][2] + r.col * 8);
+      float y[8];
+      from_e4m3(*at, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] *= ratio;
+      *at = to_e4m3(y);
+    }
+  }
+  if (lane == 0) *sp = scale;
+}
+
+// One value at a time, for any head dim and alignment.
+template <typename T>
+__global__ __launch_bounds__(128) void k_store_kv_cache_any(StoreArgs a) {
+  const int lane = threadIdx.x & 63;
+  Unit u;
+  if (!u.find(a)) return;
+  const int rows = static_cast<int>(u.p1 - u.p0);
+  const int64_t xld = a.xs[u.which][2], cld = a.cs[u.which][2];
+  const T* x = static_cast<const T*>(a.x[u.which]) + u.b * a.xs[u.which][0] + u.h * a.xs[u.which][1] + (u.p0 - u.start) * xld;
+  uint8_t* c = a.cache[u.which] + u.b * a.cs[u.which][0] + u.h * a.cs[u.which][1] + u.p0 * cld;
+  float* sp = a.scale[u.which] + u.b * a.ss[u.which][0] + u.h * a.ss[u.which][1] + u.j;
+  const auto code = [](float v) { return static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(v, 0.f, 0, false)); };
+  const float old = u.p0 > u.first ? *sp : 0.f;
+  uint32_t top = 0;
+  for (Walk w(lane, a.D); w.row < rows; w.next()) grow(top, static_cast<float>(x[w.row * xld + w.col]));
+  const float fits = least_scale(wave_max_bits(top));
+  const bool keeps = old > fits;
+  const float scale = keeps ? old : fits;
+  const Divide by(scale);
+  for (Walk w(lane, a.D); w.row < rows; w.next()) c[w.row * cld + w.col] = code(by(static_cast<float>(x[w.row * xld + w.col])));
+  if (u.p0 > u.first && !keeps && old != fits) {
+    const float ratio = old / fits;
+    uint8_t* o = c - (u.p0 - u.first) * cld;
+    const int before = static_cast<int>(u.p0 - u.first);
+    for (Walk w(lane, a.D); w.row < before; w.next())
+      o[w.row * cld + w.col] = code(__builtin_amdgcn_cvt_f32_fp8(o[w.row * cld + w.col], 0) * ratio);
   }
   if (lane == 0) *sp = scale;
 }
@@ -203,6 +323,9 @@ extern "C" int ntops_store_kv_cache(int dtype, int64_t B, int64_t H, int64_t S, 
         a.cs[i][d] = cs[i][d];
         vec = vec && xs[i][d] % (16 / static_cast<int>(sizeof(T))) == 0 && cs[i][d] % 8 == 0;
       }
+      const int64_t most = std::min(block, S);
+      vec = vec && xs[i][2] >= 0 && cs[i][2] >= 0 && most * xs[i][2] * static_cast<int64_t>(sizeof(T)) + D * 4 < 0x7fffffff &&
+            most * cs[i][2] + D < 0x7fffffff;
       a.ss[i][0] = ss[i][0];
       a.ss[i][1] = ss[i][1];
       vec = vec && aligned16(a.x[i]) && (reinterpret_cast<uintptr_t>(a.cache[i]) & 7u) == 0;
@@ -219,11 +342,11 @@ extern "C" int ntops_store_kv_cache(int dtype, int64_t B, int64_t H, int64_t S, 
     a.D = static_cast<int>(D);
     a.shift = __builtin_ctzll(static_cast<unsigned long long>(block));
     a.units = std::min(ceil_div(S - 1, block) + 1, ceil_div(C, block));
-    if (B > (int64_t(1) << 31) || H > (int64_t(1) << 31) || B * H > (int64_t(1) << 33) / a.units)
-      return set_error(NTOPS_ERR_UNSUPPORTED, "store_kv_cache: too many blocks");
-    const int64_t blocks = ceil_div(2 * B * H * a.units, 4);
-    const auto kern = vec ? &k_store_kv_cache<T, true> : &k_store_kv_cache<T, false>;
-    hipLaunchKernelGGL(kern, blocks_2d(blocks), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    if (B > 65535 || H > 65535 || a.units > (1 << 24))
+      return set_error(NTOPS_ERR_UNSUPPORTED, "store_kv_cache: over 65535 sequences or heads, or too many tokens");
+    const dim3 grid(static_cast<unsigned>(a.units), static_cast<unsigned>(H), static_cast<unsigned>(B));
+    const auto kern = vec ? &k_store_kv_cache<T> : &k_store_kv_cache_any<T>;
+    hipLaunchKernelGGL(kern, grid, dim3(128), 0, static_cast<hipStream_t>(stream), a);
     return check_launch("store_kv_cache");
   });
 }

@@ -119,7 +119,7 @@ def test_c_entry_points_refuse():
     assert store(cs=bad4) == 1 and "unit strides" in err()
     assert store(pos=256, pdt=_lib.F32) == 1 and "I32 or I64" in err()
     assert store(lens=256, ldt=_lib.I16) == 1
-    assert store(d=1 << 20) == 2 and store(b=1 << 33) == 2
+    assert store(d=1 << 20) == 2 and store(b=1 << 33) == 2 and store(h=70000) == 2
     assert store(b=0, key=None) == 0 and store(s=0, key=None) == 0
 
     def attend(dtype=_lib.BF16, b=2, hq=4, h=2, sq=3, c=40, d=16, block=16, q=256, qs=s4, cs=s4, lens=None, ldt=0, causal=0, out=512):
