@@ -4,10 +4,15 @@
 // Bound by streaming the cache once.  A work item is (batch, cache head, slice
 // of the sequence's tokens); the rows that share the head fill the 16 columns
 // of v_mfma_f32_16x16x32 (S^T = K Q^T, O^T += V^T P^T).  Every wave owns its own
-// key tiles, 8 KiB of keys and of values each (64 keys at a head dim of 128),
-// in its own part of the LDS: direct non-temporal DMA two tiles ahead, refilled
-// as soon as the tile's keys, then its values, have been read, and no barrier
-// before the waves' merge.
+// key tiles, 4 KiB of keys and of values each (32 keys at a head dim of 128), in
+// its own part of the LDS: direct non-temporal DMA two tiles ahead, refilled as
+// soon as the tile's keys, then its values, have been read, and no barrier
+// before the waves' merge.  A byte is a value here, so that per byte there is
+// twice the work of 16-bit caches; a wave alone on its SIMD issues a vector
+// instruction every 8 to 9 clocks at best, and two waves a SIMD hide that: (16, 32
+// / 8 heads, 1, 2048 .. 4096, 128) bf16 in two waves a block of 8 KiB tiles 32.4
+// us, in four 26.5, in eight of 4 KiB tiles 25.6; (1, 32 / 8, 1, 131072, 128) f16
+// 59.5, 53.4, 51.4 (5.2 TB/s).
 //
 // e4m3 becomes bf16 (f16 for the keys of f16 queries) in registers, exactly: a
 // key fragment is a 16-byte read whose halves feed two instructions, a value
@@ -59,11 +64,15 @@ __device__ __forceinline__ void dma16_nt(u32x4 rsrc, uint32_t lds_dst, uint32_t 
                : "memory");
 }
 
-// Loads of a tile's key (or value) rows, 8 instructions of 1 KiB, and of the
+constexpr int kTileBytes = 4096;                  // a tile's keys, or its values
+constexpr int kStage = 2 * kTileBytes + 2 * 256;  // and the scales of each
+constexpr int kTileInst = kTileBytes / 1024 + 1;  // instructions of one, with its scales
+
+// Loads of a tile's key (or value) rows, 4 instructions of 1 KiB, and of the
 // scales of its 16-token parts, one instruction.
 template <int D, bool IS_V>
 struct TileDma {
-  static constexpr int kInst = 8;
+  static constexpr int kInst = kTileBytes / 1024;
   static constexpr int kRows = 1024 / D;  // rows per instruction
   u32x4 rows, scales;
   uint32_t voff[kInst];
@@ -121,8 +130,6 @@ __device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi) {
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true))};
 }
 
-constexpr int kStage = 16384 + 512;  // keys, values, their scales
-
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2_t;
 
@@ -130,7 +137,7 @@ typedef __attribute__((address_space(3))) i32x2 lds_i32x2_t;
 // 2, sum) pairs; null: one slice, O normalised into a.o.
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, int nsplit, float* part) {
-  constexpr int NK = 8192 / D;  // keys per tile
+  constexpr int NK = kTileBytes / D;  // keys per tile
   constexpr int KB = NK / 16;   // 16-key parts of a tile
   constexpr int KC = D / 64;    // 16-byte key reads of a lane per part: two k-steps each
   constexpr int DT = D / 16;    // 16-row tiles of O^T
@@ -154,23 +161,28 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
   const int n = __builtin_amdgcn_readfirstlane(static_cast<int>(max(int64_t(0), min(n_all - t0, chunk))));
   // query row of this lane's column: head hk * group + r / Sq, position r % Sq
   const int r = lane & 15;
-  const int h = hk * group + r / a.Sq, qi = r % a.Sq;
+  const int qi = r % a.Sq;
   // keys of the slice that the row sees, and that every row sees
   const int lim = a.causal ? static_cast<int>(max(int64_t(-1), min(int64_t(n), n_all - a.Sq + qi + 1 - t0))) : n;
   const int lim_min = a.causal ? static_cast<int>(max(int64_t(-1), min(int64_t(n), n_all - a.Sq + 1 - t0))) : n;
 
-  u32x4 qf[2 * KC];
+  // The query rows ahead of the first tiles, by DMA too (rows of D values, chunk c
+  // of row r at slot c ^ r): as loads of their own they would be waited for first.
+  // Every wave brings them all, to one place.
+  constexpr int kQInst = D / 32;          // instructions of 1 KiB
+  constexpr int kQRows = 512 / D;         // rows of one
+  const uint32_t q_lds = lds_addr(smem) + NW * 2 * kStage;
+  {
+    const T* Q = static_cast<const T*>(a.q) + b * a.qst[0] + static_cast<int64_t>(hk) * group * a.qst[1];
+    const u32x4 rq = make_rsrc(Q, static_cast<uint32_t>(((group - 1) * a.qst[1] + (a.Sq - 1) * a.qst[2] + a.D) * 2));
 #pragma unroll
-  for (int s = 0; s < 2 * KC; ++s) {
-    const int d0 = ((s >> 1) * 4 + g) * 16 + (s & 1) * 8;  // the key bytes of k-step s in this lane
-    if (r < rows && d0 < a.D)
-      qf[s] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.q) + b * a.qst[0] + h * a.qst[1] + qi * a.qst[2] + d0);
-    else
-      qf[s] = u32x4{0, 0, 0, 0};
+    for (int i = 0; i < kQInst; ++i) {
+      const int row = i * kQRows + lane / (D / 8);
+      const int c = (lane % (D / 8)) ^ (row & (D / 8 - 1));
+      const uint32_t at = static_cast<uint32_t>((row / a.Sq * a.qst[1] + row % a.Sq * a.qst[2]) * 2 + c * 16);
+      dma16(rq, q_lds + i * 1024, row < rows && c * 8 < a.D ? at : kOOB);
+    }
   }
-  // settled here, so that no wait for it is placed among the tile loads
-#pragma unroll
-  for (int s = 0; s < 2 * KC; ++s) asm volatile("" ::"v"(qf[s]));
 
   TileDma<D, false> kd;
   TileDma<D, true> vd;
@@ -185,12 +197,12 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
   auto issue_k = [&](int j) {
     const int t = (wave + j * NW) * NK;
     const uint32_t st = mine_addr + (j & 1) * kStage;
-    kd.issue(st, st + 16384, static_cast<uint32_t>(t * a.kst[2]), t, j < mine_n);
+    kd.issue(st, st + 2 * kTileBytes, static_cast<uint32_t>(t * a.kst[2]), t, j < mine_n);
   };
   auto issue_v = [&](int j) {
     const int t = (wave + j * NW) * NK;
     const uint32_t st = mine_addr + (j & 1) * kStage;
-    vd.issue(st + 8192, st + 16384 + 256, static_cast<uint32_t>(t * a.vst[2]), t, j < mine_n);
+    vd.issue(st + kTileBytes, st + 2 * kTileBytes + 256, static_cast<uint32_t>(t * a.vst[2]), t, j < mine_n);
   };
 
   f32x4 o[DT];
@@ -202,16 +214,23 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
   issue_v(0);
   issue_k(1);
   issue_v(1);
+  wait_dma<3 * kTileInst>();  // the queries, and the keys of tile 0
+  u32x4 qf[2 * KC];
+#pragma unroll
+  for (int s = 0; s < 2 * KC; ++s) {
+    const int c = ((s >> 1) * 4 + g) * 2 + (s & 1);  // the key bytes of k-step s in this lane
+    qf[s] = *reinterpret_cast<const u32x4*>(smem + NW * 2 * kStage + r * (D * 2) + (c ^ (r & (D / 8 - 1))) * 16);
+  }
   for (int j = 0; j < mine_n; ++j) {
     const char* sk = mine + (j & 1) * kStage;
-    const char* sv = sk + 8192;
-    wait_dma<27>();  // keys of tile j are in; its values and tile j + 1 may be in flight
+    const char* sv = sk + kTileBytes;
+    wait_dma<3 * kTileInst>();  // keys of tile j are in; its values and tile j + 1 may be in flight
     f32x4 s[KB];
     float ks[KB];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-      ks[kb] = *reinterpret_cast<const float*>(sk + 16384 + kb * 4);
+      ks[kb] = *reinterpret_cast<const float*>(sk + 2 * kTileBytes + kb * 4);
     }
 #pragma unroll
     for (int c = 0; c < KC; ++c)
@@ -262,14 +281,14 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
         s[kb][e] = fast_exp2(s[kb][e] - m_use);
         l += s[kb][e];
       }
-    wait_dma<27>();  // values of tile j are in
+    wait_dma<3 * kTileInst>();  // values of tile j are in
     u32x4 pf[KB / 2];
 #pragma unroll
     for (int p = 0; p < KB / 2; ++p) {
       float x[8];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const float vs = *reinterpret_cast<const float*>(sk + 16384 + 256 + (2 * p + u) * 4);
+        const float vs = *reinterpret_cast<const float*>(sk + 2 * kTileBytes + 256 + (2 * p + u) * 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[4 * u + e] = s[2 * p + u][e] * vs;
       }
@@ -361,14 +380,15 @@ __global__ __launch_bounds__(256) void k_cache_merge(CacheAttnArgs a, int nsplit
   const float* po = part + row * nsplit * a.D;
   const float* ml = part + nrow * nsplit * a.D + 2 * row * nsplit;
   const int d = lane * 2;
-  const auto load4 = [&](int s0, float2 (&v)[4]) {
+  constexpr int kAtOnce = 16;
+  const auto load = [&](int s0, float2 (&v)[kAtOnce]) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < kAtOnce; ++u)
       v[u] = s0 + u < nsplit && d < a.D ? *reinterpret_cast<const float2*>(po + static_cast<int64_t>(s0 + u) * a.D + d)
                                         : float2{0.f, 0.f};
   };
-  float2 v[4];
-  load4(0, v);  // in flight while the weights are formed
+  float2 v[kAtOnce];
+  load(0, v);  // in flight while the weights are formed
   float m = neg_inf(), l = 0.f;
   if (lane < nsplit) {
     m = ml[2 * lane];
@@ -378,10 +398,10 @@ __global__ __launch_bounds__(256) void k_cache_merge(CacheAttnArgs a, int nsplit
   const float w = m == neg_inf() ? 0.f : fast_exp2(m - mm);
   const float sum = wave_sum(m == neg_inf() ? l : l * w);  // (no max: 0, or NaN)
   float x = 0.f, y = 0.f;
-  for (int s0 = 0; s0 < nsplit; s0 += 4) {
-    if (s0 > 0) load4(s0, v);
+  for (int s0 = 0; s0 < nsplit; s0 += kAtOnce) {
+    if (s0 > 0) load(s0, v);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kAtOnce; ++u) {
       const float ws = s0 + u < nsplit ? lane_read(w, s0 + u) : 0.f;
       x += ws * v[u].x;
       y += ws * v[u].y;
@@ -398,19 +418,22 @@ __global__ __launch_bounds__(256) void k_cache_merge(CacheAttnArgs a, int nsplit
 }
 
 // Waves of a block and slices of a sequence.  The sequences' lengths are not
-// known here: as many slices as leave about one two-wave block per CU, none
-// shorter than four tiles a wave at full length.
+// known here: as many slices as leave about one eight-wave block per CU, none
+// shorter than two tiles a wave at full length (twice the slices: (16, 32 / 8, 1,
+// 2048 .. 4096, 128) 26.5 -> 30.3 us with four-wave blocks).  From two heads per CU
+// on nothing is split, and two-wave blocks, four to a CU, hide each other's start
+// ((64, 32 / 32, 1, 512 .. 1024, 128): eight-wave ones 85.1 us, two-wave ones 73.8).
 void decode_split(int64_t heads, int64_t C, int64_t D, int& waves, int& nsplit) {
-  waves = heads < 2 * cu_count_cached() ? 2 : 1;
-  const int64_t step = (D > 64 ? 64 : 128) * waves;
-  int64_t n = std::min({static_cast<int64_t>(kMaxSplit), cu_count_cached() / heads, ceil_div(C, 4 * step)});
+  waves = heads < 2 * cu_count_cached() ? 8 : 2;
+  const int64_t step = (D > 64 ? 32 : 64) * waves;
+  int64_t n = std::min({static_cast<int64_t>(kMaxSplit), cu_count_cached() / heads, ceil_div(C, 2 * step)});
   if (n <= 2 && C <= 8 * step) n = 1;  // two short slices gain what the merge's launch costs
   nsplit = static_cast<int>(std::max<int64_t>(n, 1));
 }
 
 template <typename T, int D, int NW>
 int launch_decode(const CacheAttnArgs& a, int nsplit, float* part, hipStream_t st) {
-  constexpr int kLds = NW * 2 * kStage;
+  constexpr int kLds = NW * 2 * kStage + 32 * D;
   static_assert((2 * NW * 16 + NW * 16 * (D + 4)) * 4 <= kLds, "LDS");
   auto kern = k_cache_decode<T, D, NW>;
   static std::atomic<bool> attr_set{false};  // (threads may get here together)
@@ -437,8 +460,8 @@ int run_decode(const CacheAttnArgs& a, void* ws, int64_t ws_bytes, hipStream_t s
     ws = nullptr;
   }
   float* part = static_cast<float*>(ws);
-  if (waves == 1)
-    return a.D > 64 ? launch_decode<T, 128, 1>(a, nsplit, part, st) : launch_decode<T, 64, 1>(a, nsplit, part, st);
+  if (waves == 8)
+    return a.D > 64 ? launch_decode<T, 128, 8>(a, nsplit, part, st) : launch_decode<T, 64, 8>(a, nsplit, part, st);
   return a.D > 64 ? launch_decode<T, 128, 2>(a, nsplit, part, st) : launch_decode<T, 64, 2>(a, nsplit, part, st);
 }
 
@@ -456,7 +479,8 @@ bool cache_matrix_layout(const CacheAttnArgs& a, int dtype) {
   const int64_t ld = std::max(a.kst[2], a.vst[2]);
   return (dtype == NTOPS_BF16 || dtype == NTOPS_F16) && a.C > 0 && a.D % 16 == 0 && a.D <= 128 && q8(a.qst) &&
          a.ost[2] % 4 == 0 && a.ost[1] % 4 == 0 && a.ost[0] % 4 == 0 && c16(a.kst) && c16(a.vst) && aligned16(a.q) &&
-         aligned16(a.k) && aligned16(a.v) && (reinterpret_cast<uintptr_t>(a.o) & 7u) == 0 && a.kst[2] >= a.D &&
+         aligned16(a.k) && aligned16(a.v) && (reinterpret_cast<uintptr_t>(a.o) & 7u) == 0 && a.qst[1] >= 0 && a.qst[2] >= 0 &&
+         (a.Hq / a.Hkv) * a.qst[1] + static_cast<int64_t>(a.Sq) * a.qst[2] < (int64_t(1) << 29) && a.kst[2] >= a.D &&
          a.vst[2] >= a.D && (a.C + 1024) * ld < 0x7fffffffLL && a.C < (int64_t(1) << 30);
 }
 
