@@ -67,12 +67,19 @@ __global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb,
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int64_t pid = block_id();
   if (pid >= total) return;  // the tail of a 2-D grid (the whole block)
-  // an XCD (workgroups go round them) walks whole cache heads; the tiles with
-  // the most keys first
-  if ((total & 7) == 0) pid = (pid & 7) * (total >> 3) + (pid >> 3);
+  // An XCD (workgroups go round them) walks whole cache heads, every eighth one, so
+  // that sequences of different lengths spread over the XCDs; the tiles with the
+  // most keys first.
   const int per = nqb * nsplit;
-  const int bh = static_cast<int>(pid / per);
-  const int in = static_cast<int>(pid - static_cast<int64_t>(bh) * per);
+  int bh, in;
+  if (((a.B * a.Hkv) & 7) == 0) {
+    const int at = static_cast<int>(pid >> 3);
+    bh = at / per * 8 + static_cast<int>(pid & 7);
+    in = at % per;
+  } else {
+    bh = static_cast<int>(pid / per);
+    in = static_cast<int>(pid - static_cast<int64_t>(bh) * per);
+  }
   const int qb = nqb - 1 - in / nsplit, sp = in % nsplit;
   const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
   const int group = a.Hq / a.Hkv;
@@ -127,7 +134,7 @@ __global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb,
     voff[i] = ok ? static_cast<uint32_t>(lrow[i] * a.vst[2] + lchunk[i] * 16) : kOOB;
   }
   u32x4 kc[NL], vc[NL];
-  float kscale[4], vscale[4], vrow[NL];  // of the tile's four 16-key parts; of this thread's value rows
+  float kscale, vscale;  // of the tile's 16-key part lane & 3
   const auto load = [&](int j) {
     const uint32_t kt = static_cast<uint32_t>(j) * static_cast<uint32_t>(kKeys * a.kst[2]);
     const uint32_t vt = static_cast<uint32_t>(j) * static_cast<uint32_t>(kKeys * a.vst[2]);
@@ -135,15 +142,10 @@ __global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb,
     for (int i = 0; i < NL; ++i) {
       kc[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, koff[i] == kOOB ? kOOB : koff[i] + kt, 0, 0));
       vc[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, voff[i] == kOOB ? kOOB : voff[i] + vt, 0, 0));
-      vrow[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
-                                              rvs, ((first_part + j * kKeys + lrow[i]) >> a.shift) * 4, 0, 0));
     }
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const int at = ((first_part + j * kKeys + p * 16) >> a.shift) * 4;
-      kscale[p] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rks, at, 0, 0));
-      vscale[p] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rvs, at, 0, 0));
-    }
+    const int at = ((first_part + j * kKeys + (lane & 3) * 16) >> a.shift) * 4;
+    kscale = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rks, at, 0, 0));
+    vscale = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rvs, at, 0, 0));
   };
   const auto put = [&](int stage) {
     char* sk = smem + stage * 2 * kTile;
@@ -155,7 +157,8 @@ __global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb,
 #pragma unroll
       for (int u = 0; u < 2; ++u)
         *reinterpret_cast<u32x4*>(sk + lrow[i] * (D * 2) + kslot<D>(lrow[i], lchunk[i] * 2 + u) * 16) = w[u];
-      widen16<__bf16>(vc[i], vrow[i], w);
+      // (a wave's value rows of one i lie in one part: its first lane's)
+      widen16<__bf16>(vc[i], lane_read(vscale, (i * (256 / CPR) + wave * (64 / CPR)) >> 4), w);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
         *reinterpret_cast<u32x4*>(sv + lrow[i] * (D * 2) + vslot<D>(lrow[i], lchunk[i] * 2 + u) * 16) = w[u];
@@ -173,10 +176,9 @@ __global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb,
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       // at least a tiny factor, so that a masked score (-inf) stays one under a zero scale
-      const float x = kscale[p] * c0;
+      const float x = lane_read(kscale, p) * c0, y = lane_read(vscale, p);
       c[p] = x < 0x1p-120f ? 0x1p-120f : x;
-      f[p] = vscale[p] < 0x1p-126f ? 0.f
-                                   : __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, vscale[p]) & 0x7fffffu) | 0x3f800000u);
+      f[p] = y < 0x1p-126f ? 0.f : __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, y) & 0x7fffffu) | 0x3f800000u);
     }
   };
   if (nt > 0) {
