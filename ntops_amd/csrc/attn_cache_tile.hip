@@ -30,6 +30,11 @@ namespace {
 constexpr int kRows = 128;
 constexpr int kKeys = 64;
 constexpr int kAhead = 4;  // fragments read ahead of the MFMA that uses them
+// A row's reference, which its exponents are taken from, follows its maximum when
+// that is past it by more than this (base 2): the largest probability is then at
+// most 2^8, in fp32 sums and in bf16 products as good as 1, and O is rescaled on
+// few tiles instead of most.
+constexpr float kSlack = 8.f;
 
 // Two e4m3 values of a word to 16-bit ones; bf16: times the power of two in scale.
 template <typename T, bool HI>
@@ -170,7 +175,7 @@ __global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb,
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
-  float m_i = neg_inf(), l_i = 0.f;  // running max (base 2) of row my_r; this lane's half of its sum
+  float m_i = neg_inf(), l_i = 0.f;  // reference (base 2) of row my_r; this lane's half of its sum
   float c[4], f[4];  // of the current tile's parts: the scores' factor, the rest of the values' scale
   const auto factors = [&]() {
 #pragma unroll
@@ -193,6 +198,8 @@ __global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb,
     const char* sv = sk + kTile;
     if (j + 1 < nt) load(j + 1);
     f32x16 s[2];
+    // (the other block's wave on this SIMD has its vector work under these MFMAs)
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -210,6 +217,7 @@ __global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb,
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     // element 4q + e of half t is key 64 j + 32 t + 8 q + 4 (lane >> 5) + e
     if (j * kKeys + kKeys - 1 > w_lim) {
       const int rel = my_lim - j * kKeys - 4 * (lane >> 5);
@@ -224,10 +232,10 @@ __global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb,
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[t][e] = s[t][e];
     const float th = fmaxf(max3(max8(&x[0][0]) * c[0], max8(&x[0][8]) * c[1], max8(&x[1][0]) * c[2]), max8(&x[1][8]) * c[3]);
-    if (__any(th > m_i)) {
+    if (__any(th > m_i + kSlack)) {
       const auto h2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(th), __float_as_uint(th), false, false);
       const float tmax = fmaxf(__uint_as_float(h2[0]), __uint_as_float(h2[1]));  // of lanes l and l ^ 32
-      const bool up = tmax > m_i;
+      const bool up = tmax > m_i + kSlack;
       const float alpha = up ? fast_exp2(m_i - tmax) : 1.f;
       m_i = up ? tmax : m_i;
       l_i *= alpha;
@@ -251,16 +259,21 @@ __global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb,
         for (int e = 0; e < w; ++e) r[e] += r[e + w];
       l_i += r[0];
     }
-    if (f[0] != 1.f || f[1] != 1.f || f[2] != 1.f || f[3] != 1.f) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[t][e] *= f[2 * t + (e >> 3)];
-    }
     {
       u32x4 pf[4];
+      if (f[0] == 1.f && f[1] == 1.f && f[2] == 1.f && f[3] == 1.f) {
 #pragma unroll
-      for (int sl = 0; sl < 4; ++sl) pf[sl] = pack8<__bf16>(&x[sl >> 1][8 * (sl & 1)]);
+        for (int sl = 0; sl < 4; ++sl) pf[sl] = pack8<__bf16>(&x[sl >> 1][8 * (sl & 1)]);
+      } else {
+#pragma unroll
+        for (int sl = 0; sl < 4; ++sl) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = x[sl >> 1][8 * (sl & 1) + e] * f[sl];
+          pf[sl] = pack8<__bf16>(y);
+        }
+      }
+      __builtin_amdgcn_s_setprio(1);
       constexpr int nm = 4 * DT;  // MFMA i: key slice i / DT, d tile i % DT
       u32x4 fr[kAhead];
 #pragma unroll
@@ -273,6 +286,7 @@ __global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb,
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     // the other stage was last read before the barrier that ended the previous tile
     if (j + 1 < nt) {
       put((j + 1) & 1);
