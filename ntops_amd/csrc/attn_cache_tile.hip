@@ -138,32 +138,35 @@ __global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb,
     koff[i] = ok ? static_cast<uint32_t>(lrow[i] * a.kst[2] + lchunk[i] * 16) : kOOB;
     voff[i] = ok ? static_cast<uint32_t>(lrow[i] * a.vst[2] + lchunk[i] * 16) : kOOB;
   }
-  u32x4 kc[NL], vc[NL];
-  float kscale, vscale;  // of the tile's 16-key part lane & 3
-  const auto load = [&](int j) {
+  // two tiles on their way: tile j's chunks in set j & 1
+  u32x4 kc[2][NL], vc[2][NL];
+  float kscale[2], vscale[2];  // of the tile's 16-key part lane & 3
+  const auto load = [&](auto set, int j) __attribute__((always_inline)) {
+    constexpr int S = decltype(set)::value;
     const uint32_t kt = static_cast<uint32_t>(j) * static_cast<uint32_t>(kKeys * a.kst[2]);
     const uint32_t vt = static_cast<uint32_t>(j) * static_cast<uint32_t>(kKeys * a.vst[2]);
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      kc[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, koff[i] == kOOB ? kOOB : koff[i] + kt, 0, 0));
-      vc[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, voff[i] == kOOB ? kOOB : voff[i] + vt, 0, 0));
+      kc[S][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, koff[i] == kOOB ? kOOB : koff[i] + kt, 0, 0));
+      vc[S][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, voff[i] == kOOB ? kOOB : voff[i] + vt, 0, 0));
     }
     const int at = ((first_part + j * kKeys + (lane & 3) * 16) >> a.shift) * 4;
-    kscale = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rks, at, 0, 0));
-    vscale = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rvs, at, 0, 0));
+    kscale[S] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rks, at, 0, 0));
+    vscale[S] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rvs, at, 0, 0));
   };
-  const auto put = [&](int stage) {
-    char* sk = smem + stage * 2 * kTile;
+  const auto put = [&](auto set) __attribute__((always_inline)) {  // into the stage of the same number
+    constexpr int S = decltype(set)::value;
+    char* sk = smem + S * 2 * kTile;
     char* sv = sk + kTile;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       u32x4 w[2];
-      widen16<T>(kc[i], 1.f, w);
+      widen16<T>(kc[S][i], 1.f, w);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
         *reinterpret_cast<u32x4*>(sk + lrow[i] * (D * 2) + kslot<D>(lrow[i], lchunk[i] * 2 + u) * 16) = w[u];
       // (a wave's value rows of one i lie in one part: its first lane's)
-      widen16<__bf16>(vc[i], lane_read(vscale, (i * (256 / CPR) + wave * (64 / CPR)) >> 4), w);
+      widen16<__bf16>(vc[S][i], lane_read(vscale[S], (i * (256 / CPR) + wave * (64 / CPR)) >> 4), w);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
         *reinterpret_cast<u32x4*>(sv + lrow[i] * (D * 2) + vslot<D>(lrow[i], lchunk[i] * 2 + u) * 16) = w[u];
@@ -177,26 +180,31 @@ __global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb,
     for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
   float m_i = neg_inf(), l_i = 0.f;  // reference (base 2) of row my_r; this lane's half of its sum
   float c[4], f[4];  // of the current tile's parts: the scores' factor, the rest of the values' scale
-  const auto factors = [&]() {
+  const auto factors = [&](auto set) __attribute__((always_inline)) {
+    constexpr int S = decltype(set)::value;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       // at least a tiny factor, so that a masked score (-inf) stays one under a zero scale
-      const float x = lane_read(kscale, p) * c0, y = lane_read(vscale, p);
+      const float x = lane_read(kscale[S], p) * c0, y = lane_read(vscale[S], p);
       c[p] = x < 0x1p-120f ? 0x1p-120f : x;
       f[p] = y < 0x1p-126f ? 0.f : __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, y) & 0x7fffffu) | 0x3f800000u);
     }
   };
+  constexpr std::integral_constant<int, 0> even{};
+  constexpr std::integral_constant<int, 1> odd{};
   if (nt > 0) {
-    load(0);
-    put(0);
-    factors();
+    load(even, 0);
+    load(odd, 1);
+    put(even);
+    factors(even);
   }
   __syncthreads();
 
-  for (int j = 0; j < nt; ++j) {
-    const char* sk = smem + (j & 1) * 2 * kTile;
+  // tile j, of stage set; other: the other one (loads past the last tile bring zeros)
+  const auto tile = [&](auto set, auto other, int j) __attribute__((always_inline)) {
+    const char* sk = smem + decltype(set)::value * 2 * kTile;
     const char* sv = sk + kTile;
-    if (j + 1 < nt) load(j + 1);
+    load(set, j + 2);
     f32x16 s[2];
     // (the other block's wave on this SIMD has its vector work under these MFMAs)
     __builtin_amdgcn_s_setprio(1);
@@ -289,10 +297,14 @@ __global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb,
     __builtin_amdgcn_s_setprio(0);
     // the other stage was last read before the barrier that ended the previous tile
     if (j + 1 < nt) {
-      put((j + 1) & 1);
-      factors();
+      put(other);
+      factors(other);
     }
     __syncthreads();
+  };
+  for (int j = 0; j < nt; j += 2) {
+    tile(even, odd, j);
+    if (j + 1 < nt) tile(odd, even, j + 1);
   }
 
   l_i += __shfl_xor(l_i, 32, 64);
