@@ -197,14 +197,18 @@ bool scales_fit(int64_t kb, const void* s, int64_t ld) {
 // 256 x 256 tiles for about a round of the GPU or more.
 bool large_suits(int64_t M, int64_t N) { return ceil_div(M, 256) * ceil_div(N, 256) >= cu_count_cached() / 2; }
 
-// The tile's size, and slices of K: as many as bring the blocks near the number
-// of CUs, none under four K tiles.
+// The tile's size: 128 from a tile per CU on ((1024, 4096, 4096) bf16 25.2 us, on 64
+// x 64 tiles 30.9; (512, 4096, 4096), 128 large tiles, 23.6 and 17.8).  Slices of K:
+// as many as bring the blocks near the number of CUs (twice as many: (256, 4096,
+// 4096) 11.2 -> 16.1), none under eight K tiles, whose time a reduction's launch
+// takes ((500, 1001, 2080) in slices of four 12.3 us, whole 9.1; (64, 4096, 14336) in
+// slices of eight or more 17.6, of sixteen or more 19.1).
 void plan(int64_t M, int64_t N, int64_t kb, int& bt, int& split, int& kchunk) {
   const int64_t cus = cu_count_cached();
   const auto tiles = [&](int64_t t) { return ceil_div(M, t) * ceil_div(N, t); };
   bt = tiles(128) >= cus ? 128 : 64;
   const int64_t kt = ceil_div(kb, 8);
-  int64_t s = std::max<int64_t>(1, std::min<int64_t>({cus / tiles(bt), kt / 4, 16}));
+  int64_t s = std::max<int64_t>(1, std::min<int64_t>({cus / tiles(bt), kt / 8, 16}));
   const int64_t per = ceil_div(kt, s);
   kchunk = static_cast<int>(per * 8);
   split = static_cast<int>(ceil_div(kt, per));
