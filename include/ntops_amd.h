@@ -423,7 +423,7 @@ NTOPS_API int ntops_store_kv_cache(int dtype, int64_t B, int64_t H, int64_t S, i
  * - Sq + i.  A row that sees no key is 0.  Query head h reads cache head h /
  * (Hq / H).  Nothing behind a sequence's length is read.  fp32 sums; 16-bit q
  * with D a multiple of 16 up to 128 runs on the matrix cores (probabilities,
- * times the scale of their value block, rounded to bf16), D <= 256 and F32 on a
+ * times the scale of their value block, rounded to bf16, for F16 to two bf16 parts), D <= 256 and F32 on a
  * kernel of one wave per row.  The workspace (16-byte aligned; may be NULL)
  * spreads the keys of few query rows over the GPU. */
 NTOPS_API int ntops_kv_cache_attention(int dtype, int64_t B, int64_t Hq, int64_t H, int64_t Sq, int64_t C, int64_t D,

@@ -22,6 +22,22 @@ struct CacheAttnArgs {
   float scale_log2;      // scale * log2(e)
 };
 
+// 8 probabilities as bf16 operands: rounded, and for f16 queries, whose results
+// keep 11 bits, what the rounding left as a second operand (17 bits in all).
+template <bool LO>
+__device__ __forceinline__ void pack_p(const float* x, u32x4& hi, u32x4& lo) {
+  hi = pack8<__bf16>(x);
+  if constexpr (LO) {
+    float d[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t w = hi[e >> 1];
+      d[e] = x[e] - __builtin_bit_cast(float, e & 1 ? w & 0xffff0000u : w << 16);
+    }
+    lo = pack8<__bf16>(d);
+  }
+}
+
 __device__ __forceinline__ int64_t length_of(const CacheAttnArgs& a, int b) {
   return max(int64_t(0), min(a.C, index_at(a.lengths, a.lengths_dtype, b, a.C)));
 }

@@ -19,7 +19,8 @@
 // fragment a transposing 8-byte read.  The scale of a key's block times the
 // softmax scale multiplies its scores, that of a value's block its
 // probabilities, which are then rounded to bf16 whatever the query's type: only
-// bf16 holds them under scales of any size.
+// bf16 holds them under scales of any size.  For f16 queries the rest of the
+// rounding is a second operand of the same product (pack_p).
 //
 // Slices are parts of the sequence's own length, known on the device only, so
 // the number of slices is set by the GPU's size and an empty slice leaves an
@@ -282,7 +283,8 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
         l += s[kb][e];
       }
     wait_dma<3 * kTileInst>();  // values of tile j are in
-    u32x4 pf[KB / 2];
+    constexpr bool LO = std::is_same<T, _Float16>::value;
+    u32x4 pf[KB / 2], pl[KB / 2];
 #pragma unroll
     for (int p = 0; p < KB / 2; ++p) {
       float x[8];
@@ -292,7 +294,7 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[4 * u + e] = s[2 * p + u][e] * vs;
       }
-      pf[p] = pack8<__bf16>(x);  // keys 32 p + 4 g + 0..3 and 32 p + 16 + 4 g + 0..3
+      pack_p<LO>(x, pf[p], pl[p]);  // keys 32 p + 4 g + 0..3 and 32 p + 16 + 4 g + 0..3
     }
 #pragma unroll
     for (int p = 0; p < KB / 2; ++p)
@@ -304,7 +306,9 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
         const int row = p * 32 + ((i >> 3) & 1) * 16 + g * 4 + ((i >> 1) & 3);
         const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
             (lds_i32x2_t*)(sv + row * D + vslot8<D>(row, t) * 16 + (i & 1) * 8));
-        o[t] = mfma16<__bf16>(widen8<__bf16>(w.x, w.y), pf[p], o[t]);
+        const u32x4 vf = widen8<__bf16>(w.x, w.y);
+        o[t] = mfma16<__bf16>(vf, pf[p], o[t]);
+        if constexpr (LO) o[t] = mfma16<__bf16>(vf, pl[p], o[t]);
       }
     wait_lgkmcnt0();
     issue_v(j + 2);

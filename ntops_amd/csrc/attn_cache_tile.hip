@@ -13,7 +13,8 @@
 //    (exact), whatever the query's type; what is left of a scale that is no
 //    power of two, in [1, 2), multiplies the probabilities, in a branch that
 //    stores made by this library never take.  The probabilities are rounded to
-//    bf16 for the product: only bf16 holds values under scales of any size.
+//    bf16 for the product (f16 queries: with the rest as a second operand): only
+//    bf16 holds values under scales of any size.
 //  * The scale of a key's block times the softmax scale is a factor per 16 keys:
 //    the maximum is taken over raw scores in each 16 and scaled then, and the
 //    exponent is one fma per score.
@@ -63,6 +64,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb, int total, int nsplit, float* part) {
   constexpr int KS = D / 16;          // k-steps of S = Q K^T
   constexpr int DT = D / 32;          // 32-column tiles of O
+  constexpr bool LO = std::is_same<T, _Float16>::value;  // probabilities in two operands
   constexpr int kTile = kKeys * D * 2;  // bytes of a widened tile
   constexpr int CPR = D / 16;         // 16-byte chunks of a cache row
   constexpr int NL = kKeys * CPR / 256;  // chunks a thread loads of a tile's keys (and values)
@@ -268,29 +270,31 @@ __global__ __launch_bounds__(256, 2) void k_cache_tile(CacheAttnArgs a, int nqb,
       l_i += r[0];
     }
     {
-      u32x4 pf[4];
+      u32x4 pf[4], pl[4];
       if (f[0] == 1.f && f[1] == 1.f && f[2] == 1.f && f[3] == 1.f) {
 #pragma unroll
-        for (int sl = 0; sl < 4; ++sl) pf[sl] = pack8<__bf16>(&x[sl >> 1][8 * (sl & 1)]);
+        for (int sl = 0; sl < 4; ++sl) pack_p<LO>(&x[sl >> 1][8 * (sl & 1)], pf[sl], pl[sl]);
       } else {
 #pragma unroll
         for (int sl = 0; sl < 4; ++sl) {
           float y[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) y[e] = x[sl >> 1][8 * (sl & 1) + e] * f[sl];
-          pf[sl] = pack8<__bf16>(y);
+          pack_p<LO>(y, pf[sl], pl[sl]);
         }
       }
       __builtin_amdgcn_s_setprio(1);
+      constexpr int kAheadV = LO ? 2 : kAhead;  // (two MFMAs a fragment)
       constexpr int nm = 4 * DT;  // MFMA i: key slice i / DT, d tile i % DT
-      u32x4 fr[kAhead];
+      u32x4 fr[kAheadV];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) fr[i] = v_frag<D>(sv, (i % DT) * 32, i / DT, lane);
+      for (int i = 0; i < kAheadV; ++i) fr[i] = v_frag<D>(sv, (i % DT) * 32, i / DT, lane);
 #pragma unroll
       for (int i = 0; i < nm; ++i) {
         __builtin_amdgcn_sched_barrier(0);
-        o[i % DT] = mfma32<__bf16>(fr[i % kAhead], pf[i / DT], o[i % DT]);
-        if (i + kAhead < nm) fr[i % kAhead] = v_frag<D>(sv, ((i + kAhead) % DT) * 32, (i + kAhead) / DT, lane);
+        o[i % DT] = mfma32<__bf16>(fr[i % kAheadV], pf[i / DT], o[i % DT]);
+        if constexpr (LO) o[i % DT] = mfma32<__bf16>(fr[i % kAheadV], pl[i / DT], o[i % DT]);
+        if (i + kAheadV < nm) fr[i % kAheadV] = v_frag<D>(sv, ((i + kAheadV) % DT) * 32, (i + kAheadV) / DT, lane);
       }
       __builtin_amdgcn_sched_barrier(0);
     }

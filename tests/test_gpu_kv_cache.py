@@ -146,8 +146,8 @@ def check_attention(query, caches, lengths, causal, block, scale=None, kernel=No
     size = N.kv_cache_attention(q, k, np.abs(v), ks, vs, n, block, causal, scale)
     # a score is off by delta: fp32 sums of d products, its scaling, the
     # subtraction of the maximum and the exponential; a probability by e^delta,
-    # and by half a step of bf16 where it meets the values; the sum of the
-    # probabilities by e^delta; the result is rounded once
+    # and by half a step of bf16 where it meets the values (f16: its square, in two
+    # operands); the sum of the probabilities by e^delta; the result is rounded once
     at = np.arange(c)
     top = 0.0
     for i in range(b):
@@ -157,7 +157,7 @@ def check_attention(query, caches, lengths, causal, block, scale=None, kernel=No
         kk = np.abs(np.nan_to_num(k[i, :, :m])) * ks[i][:, at[:m] // block][..., None]
         top = max(top, float((np.abs(q[i]).reshape(k.shape[1], -1, d) @ kk.transpose(0, 2, 1)).max()) * abs(scale))
     delta = (d + 16) * 2.0**-23 * top + 2.0**-20
-    rel = 2 * math.expm1(delta) + 2.0**-8 + c * 2.0**-24
+    rel = 2 * math.expm1(delta) + (2.0**-16 if query.dtype == torch.float16 else 2.0**-8) + c * 2.0**-24
     bound = rel * size + HALF_STEP[query.dtype] * (np.abs(want) + rel * size) + 2.0**-140
     if query.dtype == torch.float16:
         bound = bound + 2.0**-25
