@@ -8,12 +8,13 @@
 // tiles as for 16 bits, so what surrounds the K loop weighs four times as much.
 //
 // Scales, a byte per 32 values, ride along, 4 KiB a K tile, in a ring of three.  A
-// kernel before this one lays them out by (256 rows, K tile), so that they arrive
-// as whole lines: read from the tensors, 8 bytes a row were as many requests as
-// the codes' lines, and 8192 x 4096 x 14336 took 246 us.  A phase reads those of
-// its rows' blocks (k-step ks of lane group q: block 4 ks + q; the two are laid next
-// to each other), two 16-row slices to a register; 12 registers that held a pair of K tiles' scales cost 209 spilled
-// ones.
+// kernel before this one lays them out by (256 rows, K tile), and within these 2
+// KiB by the lane that needs them, four bytes (two 16-row slices, two k-steps) to
+// a register of the MFMAs: they arrive as whole lines and are read by one
+// instruction for A and one for each half of B.  Read from the tensors, 8 bytes a
+// row were as many requests as the codes' lines (8192 x 4096 x 14336: 246 us against
+// 224), and read from the LDS by 2 bytes, twelve reads and six combinations a K
+// tile, they took a tenth of the time.
 #include <algorithm>
 #include <atomic>
 
@@ -38,7 +39,6 @@ static_assert(kLds <= 163840, "LDS");
 typedef __attribute__((address_space(3))) const u32x4 lds_cu32x4_t;
 typedef __attribute__((address_space(3))) const u32x2 lds_cu32x2_t;
 typedef __attribute__((address_space(3))) u32x2 lds_u32x2_t;
-typedef __attribute__((address_space(3))) const uint16_t lds_cu16_t;
 
 // Loads of an operand's half tiles: 2 instructions of 1 KiB per wave, one whole
 // line of 8 blocks a row.
@@ -157,7 +157,8 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
   // column half), 32 x 64 per wave
   f32x4 acc[4][2][4];
   u32x4 ax[4], ay[4], bx[4][2];  // A0, A1, one half of B
-  // scales: A's [half], one half of B's [column tiles 0 and 1, 2 and 3]; byte 2 (tile & 1) + k-step
+  // scales: A's [half], one half of B's [column tiles 0 and 1, 2 and 3]; byte 2 (tile & 1)
+  // + k-step (lane group q: K tile's block 4 k-step + q)
   uint32_t sa[2], sb[2];
   int slot = 0;  // of the current K tile's scales
   // LDS addresses of this lane's fragments at half 0 of buffer 0, per k-step: row
@@ -182,20 +183,10 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
       for (int j = 0; j < 4; ++j)
         bx[j][ks] = *reinterpret_cast<lds_cu32x4_t*>(bbase[ks] + static_cast<uint32_t>((buf * 2 + half) * kHalf + j * 2048));
   };
-  // Scales of the 16-row slices 2 i and 2 i + 1 of a wave's rows in half `half` of A
-  // (of_b: of B), as read: the halves of a register are put together by `pack` once
-  // they have landed, behind the fragments' reads.
-  uint32_t raw[8];
-  auto read_scales = [&](int l, bool of_b, int half, int i, uint32_t& x, uint32_t& y) __attribute__((always_inline)) {
-    const uint32_t base = smem_addr + static_cast<uint32_t>(kScaleOff + slot * kScales + (of_b ? 256 * 8 + wn * 512 : wm * 256));
-    const uint32_t at = base + static_cast<uint32_t>((l & 15) * 8 + (l >> 4) * 2);
-    x = *reinterpret_cast<lds_cu16_t*>(at + half * 1024 + i * 256);
-    y = *reinterpret_cast<lds_cu16_t*>(at + half * 1024 + i * 256 + 128);
-  };
-  // (opaque, so that it is not moved up to where its parts are read)
-  auto pack = [](uint32_t x, uint32_t y) __attribute__((always_inline)) {
-    asm volatile("" : "+v"(x), "+v"(y));
-    return x | y << 16;
+  auto read_scales = [&](int off, uint32_t (&to)[2]) __attribute__((always_inline)) {
+    const u32x2 w = *reinterpret_cast<lds_cu32x2_t*>(smem_addr + static_cast<uint32_t>(kScaleOff + slot * kScales + off + here(lane) * 8));
+    to[0] = w.x;
+    to[1] = w.y;
   };
 
   // ---- epilogue: a finished quadrant (32 x 64 per wave) is rounded, 16 x 16
@@ -327,7 +318,7 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
   };
   // ends a memory phase: its fragments are in registers, and all but the
   // wave's N youngest memory operations are done
-  auto end_mem = [&](auto n_tag, auto packs) __attribute__((always_inline)) {
+  auto end_mem = [&](auto n_tag) __attribute__((always_inline)) {
     constexpr int N = decltype(n_tag)::value;
     __builtin_amdgcn_sched_barrier(0);
     if (N > 9 && pend)
@@ -335,8 +326,6 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
     else
       wait_vm<9>();
     wait_lgkmcnt0();
-    __builtin_amdgcn_sched_barrier(0);
-    packs();
     block_barrier();
     __builtin_amdgcn_s_setprio(1);
   };
@@ -363,21 +352,13 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
     read_b(BUF, 0);
     read_a(ay, BUF, 1);
     __builtin_amdgcn_sched_barrier(0);
-    const int l = here(lane);
-    read_scales(l, false, 0, 0, raw[0], raw[1]);
-    read_scales(l, false, 1, 0, raw[2], raw[3]);
-    read_scales(l, true, 0, 0, raw[4], raw[5]);
-    read_scales(l, true, 0, 1, raw[6], raw[7]);
+    read_scales(wm * 512, sa);
+    read_scales(2048 + wn * 512, sb);
     dma_s(rs2, t2, slot == 0 ? 2 : slot - 1);
     dma_b(tail, rs1, 1, t1);
     if constexpr (KIND == 0)
       if (pend) put_rows(rows, 1, 1, here(lane));
-    end_mem(NTOPS_W(KIND == 0 ? 17 : KIND == 3 ? 19 : 9), [&]() __attribute__((always_inline)) {
-      sa[0] = pack(raw[0], raw[1]);
-      sa[1] = pack(raw[2], raw[3]);
-      sb[0] = pack(raw[4], raw[5]);
-      sb[1] = pack(raw[6], raw[7]);
-    });
+    end_mem(NTOPS_W(KIND == 0 ? 17 : KIND == 3 ? 19 : 9));
     if (KIND == 0 && pend) {
       mfma16x(first, yes, 0, ax, 0, 2);
       put_rows(rows, 2, 1, here(lane));
@@ -390,18 +371,13 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
     // ---- phase B: quadrants 2 and 3
     read_b(BUF, 1);
     __builtin_amdgcn_sched_barrier(0);
-    const int l2 = here(lane);
-    read_scales(l2, true, 1, 0, raw[4], raw[5]);
-    read_scales(l2, true, 1, 1, raw[6], raw[7]);
+    read_scales(2048 + 1024 + wn * 512, sb);
     dma_a(tail, rs2, 0, t2);
     dma_b(tail, rs2, 0, t2);
     dma_a(tail, rs2, 1, t2);
     if constexpr (KIND == 0)
       if (pend) put_rows(rows, 3, 1, here(lane));
-    end_mem(NTOPS_W(KIND == 0 ? 25 : KIND == 3 ? 11 : 9), [&]() __attribute__((always_inline)) {
-      sb[0] = pack(raw[4], raw[5]);
-      sb[1] = pack(raw[6], raw[7]);
-    });
+    end_mem(NTOPS_W(KIND == 0 ? 25 : KIND == 3 ? 11 : 9));
     if constexpr (KIND == 2) {
       pm0 = m0;
       pn0 = n0;
@@ -472,30 +448,49 @@ __global__ __launch_bounds__(512, 1) void k_mx4_large(Mx4Args g, int total) {
   wait_vmcnt<0>();  // no DMA may land after the workgroup ends
 }
 
-// The scales of 256 rows and a K tile of 8 blocks to 2 KiB in a row, by panels of
-// 256 rows, then K tiles; of a row's 8 those of blocks q and q + 4 are next to each
-// other; zeros past the rows' last block and the last row.  A
-// thread a row and K tile; blockIdx.z 0: A's, 1: B's.
-__global__ __launch_bounds__(256) void k_mx4_lay_scales(Mx4Args g, uint8_t* a, uint8_t* b) {
+// The scales of 256 rows and a K tile of 8 blocks to 2 KiB, by panels of 256 rows,
+// then K tiles, in the order of k_mx4_large's registers: A's dword (wave row wm,
+// lane, half) has rows 128 half + 32 wm + l & 15 and 16 on, B's (half, wave column
+// wn, lane, pair) columns 128 half + 64 wn + 32 pair + l & 15 and 16 on; of each the
+// blocks q and q + 4, q = l >> 4.  Zeros past the row's last block and the last
+// row.  blockIdx.z 0: A's, 1: B's.  A block takes four K tiles, 32 bytes a row,
+// through the LDS (byte by byte from memory: 10.3 us for 8192 + 14336 rows of 128).
+constexpr int kLayTiles = 4;
+__global__ __launch_bounds__(512) void k_mx4_lay_scales(Mx4Args g, uint8_t* a, uint8_t* b) {
+  constexpr int kPitch = kLayTiles * 8 + 4;
+  __shared__ uint32_t lds[256 * kPitch / 4];
   const bool of_b = blockIdx.z != 0;
   const int rows = of_b ? g.N : g.M, kt = (g.kb + 7) / 8;
-  const int panel = blockIdx.x, t = blockIdx.y;
-  if (panel * 256 >= rows) return;
-  const int row = panel * 256 + threadIdx.x;
-  const int64_t ld = of_b ? g.ldbs : g.ldas;
-  const uint8_t* from = (of_b ? g.bs : g.as) + row * ld + t * 8;
-  const int n = row < rows ? min(8, g.kb - t * 8) : 0;
-  uint32_t w[2] = {0, 0};
-  if (n == 8 && (reinterpret_cast<uintptr_t>(from) & 7u) == 0) {
-    const u32x2 v = *reinterpret_cast<const u32x2*>(from);
-    w[0] = v.x;
-    w[1] = v.y;
-  } else {
-    for (int e = 0; e < n; ++e) w[e >> 2] |= static_cast<uint32_t>(from[e]) << (8 * (e & 3));
+  const int panel = blockIdx.x, t0 = blockIdx.y * kLayTiles;
+  if (panel * 256 >= rows) return;  // (the whole block)
+  {
+    const int r = threadIdx.x >> 1, k = t0 * 8 + (threadIdx.x & 1) * 16;
+    const uint8_t* from = (of_b ? g.bs : g.as) + (panel * 256 + r) * (of_b ? g.ldbs : g.ldas) + k;
+    const int n = panel * 256 + r < rows ? min(16, g.kb - k) : 0;
+    u32x4 w = {0, 0, 0, 0};
+    if (n == 16 && (reinterpret_cast<uintptr_t>(from) & 15u) == 0) {
+      w = *reinterpret_cast<const u32x4*>(from);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (e < n) w[e >> 2] |= static_cast<uint32_t>(from[e]) << (8 * (e & 3));
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) lds[r * (kPitch / 4) + (threadIdx.x & 1) * 4 + e] = w[e];
   }
-  uint8_t* to = (of_b ? b : a) + ((static_cast<int64_t>(panel) * kt + t) * 256 + threadIdx.x) * 8;
-  // bytes 0, 4, 1, 5 and 2, 6, 3, 7
-  *reinterpret_cast<u32x2*>(to) = u32x2{__builtin_amdgcn_perm(w[1], w[0], 0x05010400u), __builtin_amdgcn_perm(w[1], w[0], 0x07030602u)};
+  __syncthreads();
+  const int d = threadIdx.x, l = (d >> 1) & 63, low = d & 1, high = d >> 7;
+  const int row = (of_b ? (high >> 1) * 128 + (high & 1) * 64 + low * 32 : low * 128 + high * 32) + (l & 15);
+  const uint8_t* at = reinterpret_cast<const uint8_t*>(lds) + row * kPitch + (l >> 4);
+  uint32_t* to = reinterpret_cast<uint32_t*>(of_b ? b : a) + (static_cast<int64_t>(panel) * kt + t0) * 512 + d;
+#pragma unroll
+  for (int t = 0; t < kLayTiles; ++t) {
+    if (t0 + t >= kt) break;
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w |= static_cast<uint32_t>(at[(e >> 1) * 16 * kPitch + t * 8 + (e & 1) * 4]) << (8 * e);
+    to[t * 512] = w;
+  }
 }
 
 template <typename T, bool BIAS>
@@ -535,7 +530,7 @@ int mx4_large(int out_dtype, Mx4Args g, void* workspace, hipStream_t st) {
   uint8_t* a = static_cast<uint8_t*>(workspace);
   uint8_t* b = a + ceil_div(g.M, 256) * ceil_div(g.kb, 8) * 2048;
   const unsigned panels = static_cast<unsigned>(ceil_div(std::max(g.M, g.N), 256));
-  hipLaunchKernelGGL(k_mx4_lay_scales, dim3(panels, static_cast<unsigned>(ceil_div(g.kb, 8)), 2), dim3(256), 0, st, g, a, b);
+  hipLaunchKernelGGL(k_mx4_lay_scales, dim3(panels, static_cast<unsigned>(ceil_div(g.kb, 8 * kLayTiles)), 2), dim3(512), 0, st, g, a, b);
   g.as = a;
   g.bs = b;
   return out_dtype == NTOPS_BF16 ? run_large<__bf16>(g, st) : run_large<_Float16>(g, st);
