@@ -58,7 +58,7 @@ int cache_decode(int dtype, const CacheAttnArgs& a, void* workspace, int64_t wor
 
 // The same for any number of query rows.
 bool cache_tile_serves(const CacheAttnArgs& a, int dtype);
-int64_t cache_tile_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t C, int64_t D);
+int64_t cache_tile_workspace(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t C, int64_t D);
 int cache_tile(int dtype, const CacheAttnArgs& a, void* workspace, int64_t workspace_bytes, hipStream_t st);
 
 // Combines the slices' partial results of every query row in slice order: part

@@ -96,7 +96,7 @@ extern "C" int64_t ntops_kv_cache_attention_workspace(int dtype, int64_t B, int6
   if (B > kMaxCount || Hq > kMaxCount || Sq > kMaxCount || C > (int64_t(1) << 40) || B * Hq > kMaxCount ||
       B * Hq * Sq > (int64_t(1) << 34))
     return 0;  // (the call is refused)
-  return Sq * (Hq / Hkv) <= kDecodeRows ? cache_decode_workspace(B, Hq, Hkv, Sq, C, D) : cache_tile_workspace(B, Hq, Hkv, Sq, C, D);
+  return Sq * (Hq / Hkv) <= kDecodeRows ? cache_decode_workspace(B, Hq, Hkv, Sq, C, D) : cache_tile_workspace(dtype, B, Hq, Hkv, Sq, C, D);
 }
 
 extern "C" int ntops_kv_cache_attention(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t C, int64_t D,

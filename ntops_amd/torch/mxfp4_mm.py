@@ -17,9 +17,13 @@ from ntops_amd.torch.quantize_mxfp4 import quantize_mxfp4
 from ntops_amd.torch.utils import _DeviceGuard, _cast_into, _contiguous
 
 
+# (a tile's rows have to lie within 2^30 bytes)
+_FARTHEST_ROWS = (1 << 30) // 257
+
+
 def _code_rows(t):
     """t with rows that the kernels can read: unit stride, 16-byte aligned."""
-    if t.stride(1) == 1 and t.stride(0) >= 0 and t.stride(0) % 16 == 0 and t.data_ptr() % 16 == 0:
+    if t.stride(1) == 1 and 0 <= t.stride(0) <= _FARTHEST_ROWS and t.stride(0) % 16 == 0 and t.data_ptr() % 16 == 0:
         return t
     return _cast_into(t, torch.empty(t.shape, dtype=t.dtype, device=t.device))
 
@@ -49,7 +53,7 @@ def mxfp4_mm(input, input_scale, mat2, mat2_scale, bias=None, *, dtype=torch.bfl
     lib = _lib.load()
     with _DeviceGuard(dev):
         a, b = _code_rows(input), _code_rows(mat2)
-        sa, sb = (s if s.stride(1) == 1 and s.stride(0) >= 0 else _contiguous(s) for s in (input_scale, mat2_scale))
+        sa, sb = (s if s.stride(1) == 1 and 0 <= s.stride(0) <= _FARTHEST_ROWS else _contiguous(s) for s in (input_scale, mat2_scale))
         bias = None if bias is None else _contiguous(bias)
         scales = (sa.data_ptr(), sa.stride(0)), (sb.data_ptr(), sb.stride(0))
         ws_bytes = lib.ntops_mxfp4_mm_workspace(m, n, 32 * blocks)
