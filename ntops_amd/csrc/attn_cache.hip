@@ -94,7 +94,7 @@ extern "C" int64_t ntops_kv_cache_attention_workspace(int dtype, int64_t B, int6
                                                       int64_t C, int64_t D) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || C <= 0 || D <= 0 || Hq % Hkv != 0 || dtype == NTOPS_F32) return 0;
   if (B > kMaxCount || Hq > kMaxCount || Sq > kMaxCount || C > (int64_t(1) << 40) || B * Hq > kMaxCount ||
-      B * Hq * Sq > (int64_t(1) << 34))
+      B * Hq * Sq > kMaxCount)
     return 0;  // (the call is refused)
   return Sq * (Hq / Hkv) <= kDecodeRows ? cache_decode_workspace(B, Hq, Hkv, Sq, C, D) : cache_tile_workspace(dtype, B, Hq, Hkv, Sq, C, D);
 }
@@ -125,7 +125,7 @@ extern "C" int ntops_kv_cache_attention(int dtype, int64_t B, int64_t Hq, int64_
                 !key_scale_strides || !value_scale_strides))
     return set_error(NTOPS_ERR_INVALID, "kv_cache_attention: null pointer");
   if (D > kMaxDim) return set_error(NTOPS_ERR_UNSUPPORTED, "kv_cache_attention: head dim over %d", kMaxDim);
-  if (B > kMaxCount || Hq > kMaxCount || Sq > kMaxCount || C > (int64_t(1) << 40) || B * Hq > kMaxCount || B * Hq * Sq > (int64_t(1) << 34))
+  if (B > kMaxCount || Hq > kMaxCount || Sq > kMaxCount || C > (int64_t(1) << 40) || B * Hq > kMaxCount || B * Hq * Sq > kMaxCount)
     return set_error(NTOPS_ERR_UNSUPPORTED, "kv_cache_attention: problem too large");
   CacheAttnArgs a{};
   a.q = q;

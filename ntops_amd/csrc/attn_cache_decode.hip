@@ -440,13 +440,8 @@ int launch_decode(const CacheAttnArgs& a, int nsplit, float* part, hipStream_t s
   constexpr int kLds = NW * 2 * kStage + 32 * D;
   static_assert((2 * NW * 16 + NW * 16 * (D + 4)) * 4 <= kLds, "LDS");
   auto kern = k_cache_decode<T, D, NW>;
-  static std::atomic<bool> attr_set{false};  // (threads may get here together)
-  if (!attr_set.load(std::memory_order_relaxed)) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) !=
-        hipSuccess)
-      return set_error(NTOPS_ERR_HIP, "kv_cache_attention: cannot reserve %d bytes of LDS", kLds);
-    attr_set.store(true, std::memory_order_relaxed);
-  }
+  static std::atomic<uint64_t> reserved{0};
+  if (const int rc = reserve_lds(reinterpret_cast<const void*>(kern), kLds, reserved, "kv_cache_attention"); rc != NTOPS_OK) return rc;
   const int64_t blocks = static_cast<int64_t>(nsplit) * a.B * a.Hkv;
   note_kernel("kv_cache_decode d%d waves%d split%d", D, NW, nsplit);
   hipLaunchKernelGGL(kern, blocks_2d(blocks), dim3(64 * NW), kLds, st, a, nsplit, part);

@@ -45,6 +45,17 @@ int cu_count_cached() {
   return n;
 }
 
+int reserve_lds(const void* kern, int bytes, std::atomic<uint64_t>& done, const char* what) {
+  int dev = 0;
+  const bool known = hipGetDevice(&dev) == hipSuccess && dev >= 0 && dev < 64;
+  const uint64_t bit = known ? uint64_t(1) << dev : 0;
+  if (known && (done.load(std::memory_order_relaxed) & bit)) return NTOPS_OK;  // (threads may get here together)
+  if (hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+    return set_error(NTOPS_ERR_HIP, "%s: cannot reserve %d bytes of LDS", what, bytes);
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return NTOPS_OK;
+}
+
 }  // namespace ntops
 
 extern "C" int ntops_abi_version(void) { return 2; }

@@ -9,6 +9,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "../../include/ntops_amd.h"
@@ -26,6 +27,10 @@ void note_kernel(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
 // Number of CUs of the current device (queried once per device; 256 if the
 // query fails).
 int cu_count_cached();
+
+// Lets `kern` launch with `bytes` of dynamic LDS on the current device (once per
+// device: `done` is the kernel's own).  NTOPS_OK, or an error of `what`.
+int reserve_lds(const void* kern, int bytes, std::atomic<uint64_t>& done, const char* what);
 
 // ------------------------------------------------------------ wave size --
 constexpr int kWave = 64;

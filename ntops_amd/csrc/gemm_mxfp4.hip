@@ -187,7 +187,8 @@ __global__ __launch_bounds__(256) void k_mx4_reduce(Mx4Args g) {
   static_cast<T*>(g.d)[m * g.ldd + n] = static_cast<T>(v);
 }
 
-constexpr int64_t kMaxSize = int64_t(1) << 30;
+constexpr int64_t kMaxSize = int64_t(1) << 30;   // bytes of a tile's rows, or of a row
+constexpr int64_t kMaxCount = int64_t(1) << 29;  // rows
 
 // Whether K tiles of 8 blocks are whole dwords of these scale rows.
 bool scales_fit(int64_t kb, const void* s, int64_t ld) {
@@ -218,13 +219,8 @@ template <typename T, int BT, bool FIT>
 int launch_tile(const Mx4Args& g, hipStream_t st) {
   auto kern = k_mx4_tile<T, BT, FIT>;
   constexpr int kLds = TileShape<BT, FIT>::kLds;
-  static std::atomic<bool> attr_set{false};  // (threads may get here together)
-  if (!attr_set.load(std::memory_order_relaxed)) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) !=
-        hipSuccess)
-      return set_error(NTOPS_ERR_HIP, "mxfp4_mm: cannot reserve %d bytes of LDS", kLds);
-    attr_set.store(true, std::memory_order_relaxed);
-  }
+  static std::atomic<uint64_t> reserved{0};
+  if (const int rc = reserve_lds(reinterpret_cast<const void*>(kern), kLds, reserved, "mxfp4_mm"); rc != NTOPS_OK) return rc;
   const int tm = static_cast<int>(ceil_div(g.M, BT)), tn = static_cast<int>(ceil_div(g.N, BT));
   const int whole = (g.ldd & 3) == 0 && (reinterpret_cast<uintptr_t>(g.d) & (4 * sizeof(T) - 1)) == 0;
   note_kernel("mxfp4_tile%d split%d%s", BT, g.split, FIT ? "" : " bytes");
@@ -248,7 +244,7 @@ int run_tile(const Mx4Args& g, int bt, hipStream_t st) {
 using namespace ntops;
 
 extern "C" int64_t ntops_mxfp4_mm_workspace(int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0 || M > kMaxSize || N > kMaxSize || K > kMaxSize) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || M > kMaxCount || N > kMaxCount || K > kMaxSize) return 0;
   if (M <= kSkinnyRows) return 0;
   if (large_suits(M, N)) return mx4_large_workspace(M, N, ceil_div(K, 32));
   int bt, split, kchunk;
@@ -273,7 +269,7 @@ extern "C" int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K, co
     return set_error(NTOPS_ERR_INVALID, "mxfp4_mm: negative row stride");
   const int64_t lim = kMaxSize;
   const auto span = [&](int64_t ld, int64_t row) { return 256 * ld + row; };  // bytes that one tile's rows cover
-  if (M > lim || N > lim || kb * 16 > lim || span(a_row_stride, kb * 16) > lim || span(b_row_stride, kb * 16) > lim ||
+  if (M > kMaxCount || N > kMaxCount || kb * 16 > lim || span(a_row_stride, kb * 16) > lim || span(b_row_stride, kb * 16) > lim ||
       span(as_row_stride, kb) > lim || span(bs_row_stride, kb) > lim ||
       ceil_div(M, 64) * ceil_div(N, 64) > 0x7fffff)
     return set_error(NTOPS_ERR_UNSUPPORTED, "mxfp4_mm: operands too large");

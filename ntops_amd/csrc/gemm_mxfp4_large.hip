@@ -496,13 +496,8 @@ __global__ __launch_bounds__(512) void k_mx4_lay_scales(Mx4Args g, uint8_t* a, u
 template <typename T, bool BIAS>
 int launch_large(const Mx4Args& g, hipStream_t st) {
   auto kern = k_mx4_large<T, BIAS>;
-  static std::atomic<bool> attr_set{false};  // (threads may get here together)
-  if (!attr_set.load(std::memory_order_relaxed)) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) !=
-        hipSuccess)
-      return set_error(NTOPS_ERR_HIP, "mxfp4_mm: cannot reserve %d bytes of LDS", kLds);
-    attr_set.store(true, std::memory_order_relaxed);
-  }
+  static std::atomic<uint64_t> reserved{0};
+  if (const int rc = reserve_lds(reinterpret_cast<const void*>(kern), kLds, reserved, "mxfp4_mm"); rc != NTOPS_OK) return rc;
   const int64_t total = ceil_div(g.M, 256) * ceil_div(g.N, 256);
   const int64_t grid = std::min<int64_t>(total, cu_count_cached());
   note_kernel("mxfp4_large");

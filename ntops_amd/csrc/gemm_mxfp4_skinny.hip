@@ -192,13 +192,8 @@ template <typename T, int J, int MR>
 int launch_skinny(const Mx4Args& g, hipStream_t st) {
   constexpr int kLds = Ring<J, MR>::kLds;
   auto kern = k_mx4_skinny<T, J, MR>;
-  static std::atomic<bool> attr_set{false};  // (threads may get here together)
-  if (!attr_set.load(std::memory_order_relaxed)) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) !=
-        hipSuccess)
-      return set_error(NTOPS_ERR_HIP, "mxfp4_mm: cannot reserve %d bytes of LDS", kLds);
-    attr_set.store(true, std::memory_order_relaxed);
-  }
+  static std::atomic<uint64_t> reserved{0};
+  if (const int rc = reserve_lds(reinterpret_cast<const void*>(kern), kLds, reserved, "mxfp4_mm"); rc != NTOPS_OK) return rc;
   const int whole = (g.ldd & 3) == 0 && (reinterpret_cast<uintptr_t>(g.d) & (4 * sizeof(T) - 1)) == 0;
   note_kernel("mxfp4_skinny j%d m%d", J, MR);
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((g.N + 16 * J - 1) / (16 * J))), dim3(64 * kWaves), kLds, st, g, whole);
