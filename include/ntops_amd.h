@@ -389,6 +389,18 @@ NTOPS_API int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K,
  * (0: none). */
 NTOPS_API int64_t ntops_mxfp4_mm_workspace(int64_t M, int64_t N, int64_t K);
 
+/* ntops_mxfp4_mm with A as F32 / F16 / BF16 activations x (M, K), which are
+ * quantized first (as ntops_quantize_mxfp4 does; for up to 4 rows of 16-bit values
+ * on 16-byte addresses inside the product's own kernel, otherwise into the
+ * workspace, which is then required). */
+NTOPS_API int ntops_mxfp4_linear(int x_dtype, int out_dtype, int64_t M, int64_t N, int64_t K,
+               const void* x, int64_t x_row_stride,
+               const void* b, int64_t b_row_stride, const void* b_scales, int64_t bs_row_stride,
+               const void* bias, void* out, int64_t out_row_stride,
+               void* workspace, int64_t workspace_bytes, void* stream);
+NTOPS_API int64_t ntops_mxfp4_linear_workspace(int x_dtype, int64_t M, int64_t N, int64_t K,
+               const void* x, int64_t x_row_stride);
+
 /* ---- key / value cache in 8 bits ------------------------------------------ */
 /* No ntops counterparts (its KV cache, kernels/scaled_dot_product_attention.py:
  * 139-140, is of the query's type).  key_cache and value_cache (B, H, C, D)

@@ -131,6 +131,11 @@ _SIGNATURES = {
         [_i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp],
     ),
     "ntops_mxfp4_mm_workspace": (_i64, [_i64, _i64, _i64]),
+    "ntops_mxfp4_linear": (
+        _i,
+        [_i, _i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp],
+    ),
+    "ntops_mxfp4_linear_workspace": (_i64, [_i, _i64, _i64, _i64, _vp, _i64]),
     "ntops_store_kv_cache": (
         _i,
         [_i] + [_i64] * 6 + [_vp, _c_i64p] * 6 + [_vp, _i, _i64, _vp, _i, _vp],

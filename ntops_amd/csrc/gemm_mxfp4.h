@@ -25,6 +25,9 @@ struct Mx4Args {
   int64_t lda, ldas, ldb, ldbs;  // row strides in bytes
   int64_t ldd;         // elements
   int M, N, kb;        // kb: blocks of 32 along K
+  const void* x;       // A not yet quantized: 16-bit rows of K values, ldx apart (elements)
+  int64_t ldx;
+  int K;
   float* part;         // split K: fp32 partial products, slice s at s * M * N
   int split, kchunk;   // slices, and the blocks of each
 };
@@ -72,5 +75,9 @@ int mx4_large(int out_dtype, Mx4Args g, void* workspace, hipStream_t st);
 constexpr int kSkinnyRows = 16;
 // out for M <= kSkinnyRows, bound by streaming B.
 int mx4_skinny(int out_dtype, const Mx4Args& g, hipStream_t st);
+// The same with A quantized by the blocks themselves (g.x), for up to kFusedRows
+// rows.
+constexpr int kFusedRows = 4;
+int mx4_skinny_fused(int x_dtype, int out_dtype, const Mx4Args& g, hipStream_t st);
 
 }  // namespace ntops

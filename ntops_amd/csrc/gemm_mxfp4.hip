@@ -252,14 +252,16 @@ extern "C" int64_t ntops_mxfp4_mm_workspace(int64_t M, int64_t N, int64_t K) {
   return split > 1 ? split * M * N * 4 : 0;
 }
 
-extern "C" int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K, const void* a, int64_t a_row_stride,
-                              const void* a_scales, int64_t as_row_stride, const void* b, int64_t b_row_stride,
-                              const void* b_scales, int64_t bs_row_stride, const void* bias, void* out,
-                              int64_t out_row_stride, void* workspace, int64_t workspace_bytes, void* stream) {
+namespace ntops {
+namespace {
+
+// The arguments of ntops_mxfp4_mm, checked (M, N > 0), in g.
+int mx4_args(int out_dtype, int64_t M, int64_t N, int64_t K, const void* a, int64_t a_row_stride, const void* a_scales,
+             int64_t as_row_stride, const void* b, int64_t b_row_stride, const void* b_scales, int64_t bs_row_stride,
+             const void* bias, void* out, int64_t out_row_stride, const void* workspace, int64_t workspace_bytes, Mx4Args& g) {
   if (M < 0 || N < 0 || K < 0) return set_error(NTOPS_ERR_INVALID, "mxfp4_mm: negative size");
   if (out_dtype != NTOPS_F32 && out_dtype != NTOPS_F16 && out_dtype != NTOPS_BF16)
     return set_error(NTOPS_ERR_UNSUPPORTED, "mxfp4_mm: unsupported output dtype %d (F32/F16/BF16 only)", out_dtype);
-  if (M == 0 || N == 0) return NTOPS_OK;
   if (!out || (K > 0 && (!a || !a_scales || !b || !b_scales))) return set_error(NTOPS_ERR_INVALID, "mxfp4_mm: null pointer");
   const int64_t kb = ceil_div(K, 32);
   if (K == 0) a_row_stride = b_row_stride = as_row_stride = bs_row_stride = 0;  // no rows to read
@@ -273,8 +275,6 @@ extern "C" int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K, co
       span(as_row_stride, kb) > lim || span(bs_row_stride, kb) > lim ||
       ceil_div(M, 64) * ceil_div(N, 64) > 0x7fffff)
     return set_error(NTOPS_ERR_UNSUPPORTED, "mxfp4_mm: operands too large");
-  const hipStream_t st = static_cast<hipStream_t>(stream);
-  Mx4Args g{};
   g.a = static_cast<const uint8_t*>(a);
   g.as = static_cast<const uint8_t*>(a_scales);
   g.b = static_cast<const uint8_t*>(b);
@@ -291,6 +291,26 @@ extern "C" int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K, co
   g.kb = static_cast<int>(kb);
   if (workspace_bytes < 0 || (workspace != nullptr && !aligned16(workspace)))
     return set_error(NTOPS_ERR_INVALID, "mxfp4_mm: workspace not aligned to 16 bytes");
+  return NTOPS_OK;
+}
+
+}  // namespace
+}  // namespace ntops
+
+extern "C" int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K, const void* a, int64_t a_row_stride,
+                              const void* a_scales, int64_t as_row_stride, const void* b, int64_t b_row_stride,
+                              const void* b_scales, int64_t bs_row_stride, const void* bias, void* out,
+                              int64_t out_row_stride, void* workspace, int64_t workspace_bytes, void* stream) {
+  if ((M == 0 || N == 0) && M >= 0 && N >= 0 && K >= 0 &&
+      (out_dtype == NTOPS_F32 || out_dtype == NTOPS_F16 || out_dtype == NTOPS_BF16))
+    return NTOPS_OK;
+  Mx4Args g{};
+  if (const int rc = mx4_args(out_dtype, M, N, K, a, a_row_stride, a_scales, as_row_stride, b, b_row_stride, b_scales, bs_row_stride,
+                              bias, out, out_row_stride, workspace, workspace_bytes, g);
+      rc != NTOPS_OK)
+    return rc;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t kb = g.kb;
   return dispatch_float16_32(out_dtype, "mxfp4_mm", [&](auto tag) -> int {
     using T = decltype(tag);
     if (M <= kSkinnyRows && kb > 0) return mx4_skinny(out_dtype, g, st);
@@ -306,4 +326,59 @@ extern "C" int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K, co
     g.part = static_cast<float*>(workspace);
     return run_tile<T>(g, bt, st);
   });
+}
+
+namespace ntops {
+namespace {
+
+// Whether a product's blocks quantize these activations themselves.
+bool fused(int x_dtype, int64_t M, int64_t K, const void* x, int64_t x_row_stride) {
+  return (x_dtype == NTOPS_BF16 || x_dtype == NTOPS_F16) && M <= kFusedRows && K % 8 == 0 && aligned16(x) &&
+         (M == 1 || (x_row_stride % 8 == 0 && x_row_stride >= 0 && x_row_stride < kMaxSize / (2 * kFusedRows) - K));
+}
+
+int64_t round16(int64_t n) { return (n + 15) & ~int64_t(15); }
+
+}  // namespace
+}  // namespace ntops
+
+extern "C" int64_t ntops_mxfp4_linear_workspace(int x_dtype, int64_t M, int64_t N, int64_t K, const void* x,
+                                                int64_t x_row_stride) {
+  if (M <= 0 || N <= 0 || K <= 0 || M > kMaxCount || N > kMaxCount || K > kMaxSize || fused(x_dtype, M, K, x, x_row_stride)) return 0;
+  const int64_t kb = ceil_div(K, 32);
+  return round16(M * kb * 16) + round16(M * kb) + ntops_mxfp4_mm_workspace(M, N, K);
+}
+
+extern "C" int ntops_mxfp4_linear(int x_dtype, int out_dtype, int64_t M, int64_t N, int64_t K, const void* x,
+                                  int64_t x_row_stride, const void* b, int64_t b_row_stride, const void* b_scales,
+                                  int64_t bs_row_stride, const void* bias, void* out, int64_t out_row_stride, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  if (M < 0 || N < 0 || K < 0) return set_error(NTOPS_ERR_INVALID, "mxfp4_mm: negative size");
+  if (x_dtype != NTOPS_F32 && x_dtype != NTOPS_F16 && x_dtype != NTOPS_BF16)
+    return set_error(NTOPS_ERR_UNSUPPORTED, "mxfp4_mm: unsupported input dtype %d (F32/F16/BF16 only)", x_dtype);
+  if (M > kMaxCount || N > kMaxCount || K > kMaxSize) return set_error(NTOPS_ERR_UNSUPPORTED, "mxfp4_mm: operands too large");
+  if (K > 0 && M > 0 && !x) return set_error(NTOPS_ERR_INVALID, "mxfp4_mm: null pointer");
+  const int64_t kb = ceil_div(K, 32);
+  if (M == 0 || N == 0 || K == 0)
+    return ntops_mxfp4_mm(out_dtype, M, N, 0, nullptr, 0, nullptr, 0, nullptr, 0, nullptr, 0, bias, out, out_row_stride, nullptr, 0, stream);
+  // (all but x checked before a kernel starts; A stands in for the codes to come)
+  Mx4Args g{};
+  if (const int rc = mx4_args(out_dtype, M, N, K, b, kb * 16, b_scales, kb, b, b_row_stride, b_scales, bs_row_stride, bias, out,
+                              out_row_stride, nullptr, 0, g);
+      rc != NTOPS_OK)
+    return rc;
+  if (fused(x_dtype, M, K, x, x_row_stride)) {
+    g.x = x;
+    g.ldx = M == 1 ? 0 : x_row_stride;
+    g.K = static_cast<int>(K);
+    return mx4_skinny_fused(x_dtype, out_dtype, g, static_cast<hipStream_t>(stream));
+  }
+  const int64_t codes = round16(M * kb * 16), scales = round16(M * kb);
+  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < codes + scales)
+    return set_error(NTOPS_ERR_INVALID, "mxfp4_mm: needs %lld bytes of workspace, aligned to 16",
+                     static_cast<long long>(codes + scales));
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  if (const int rc = ntops_quantize_mxfp4(x_dtype, M, K, x, x_row_stride, at, at + codes, stream); rc != NTOPS_OK) return rc;
+  return ntops_mxfp4_mm(out_dtype, M, N, K, at, kb * 16, at + codes, kb, b, b_row_stride, b_scales, bs_row_stride, bias, out,
+                        out_row_stride, at + codes + scales, workspace_bytes - codes - scales, stream);
 }

@@ -14,9 +14,19 @@
 // bytes behind the row's last block count as 0, as they may be another row's 255.
 // Such a dword may reach up to 3 bytes past the scales' end or before their start;
 // being aligned it lies within what the memory's page holds.
+//
+// Activations that are still 16-bit (X) are quantized here, up to 4 rows: a step's
+// A is then its raw values, a lane rounds whole blocks of them (mxfp4.h), and the
+// codes go to the LDS, where the fragments are read as ever.  Every block rounds the
+// same rows again, which pays for up to 4 of them: a kernel before this one and then
+// this one, against this one alone, in a captured graph, took 1 row of 4096 values
+// 6.4 against 5.1 us for 640 columns and 12.0 against 10.7 for 14336; 4 rows 6.4
+// against 5.4 and 12.1 against 11.0, and 4 rows of 14336 values, the most a wave has
+// to round, 12.1 against 12.5 for 4096 columns.
 #include <atomic>
 
 #include "gemm_mxfp4.h"
+#include "mxfp4.h"
 
 namespace ntops {
 namespace {
@@ -83,23 +93,63 @@ struct Loader {
   }
 };
 
-// Steps in the ring: what fits into a CU's LDS.
-template <int J, int MR>
+// Raw rows of 32 CPR 16-bit values: 16-byte piece p of block c at piece p ^ (c & 3),
+// for reads of whole blocks by neighbouring lanes.
+template <int ROWS, int CPR>
+struct RawLoader {
+  static constexpr int kInst = ROWS * CPR / 16;
+  static constexpr int kBytes = kInst * 1024, kScaleBytes = 0, kScaleInst = 0;
+  u32x4 rows;
+  uint32_t voff[kInst];
+  int row_bytes;
+  __device__ __forceinline__ static int in_row(int lane, int i) {  // the lane's byte of its row of the step
+    const int at = (i * 1024 + lane * 16) % (CPR * 64);
+    return (at & ~63) + (((at >> 4) ^ (at >> 6)) & 3) * 16;
+  }
+  __device__ __forceinline__ void init(const void* x, int64_t ld, int n, int K, int lane) {
+    row_bytes = K * 2;
+    rows = make_rsrc(x, (n - 1) * ld * 2 + row_bytes);
+#pragma unroll
+    for (int i = 0; i < kInst; ++i) {
+      const int r = (i * 1024 + lane * 16) / (CPR * 64);
+      voff[i] = r < n ? static_cast<uint32_t>(r * ld * 2 + in_row(lane, i)) : kOOB;
+    }
+  }
+  __device__ __forceinline__ void issue(uint32_t dst, int b0, bool valid, int lane) const {
+#pragma unroll
+    for (int i = 0; i < kInst; ++i)
+      dma16(rows, dst + i * 1024,
+            valid && voff[i] != kOOB && b0 * 64 + in_row(lane, i) < row_bytes ? voff[i] + static_cast<uint32_t>(b0) * 64 : kOOB);
+  }
+  // block c of row r
+  __device__ __forceinline__ static void block(const char* t, int r, int c, u32x4 (&x)[4]) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) x[p] = *reinterpret_cast<const u32x4*>(t + (r * CPR + c) * 64 + (p ^ (c & 3)) * 16);
+  }
+};
+
+// Steps in the ring: what fits into a CU's LDS.  X: A is raw, and a wave keeps the
+// codes and scales of one step.
+template <typename X, int J, int MR>
 struct Ring {
+  static constexpr bool kRaw = !std::is_same<X, void>::value;
   static constexpr int CPR = 32 / J;  // blocks of a row per step
-  using LA = Loader<MR, CPR, false>;
+  using LC = Loader<MR, CPR, false>;
+  using LA = std::conditional_t<kRaw, RawLoader<MR, CPR>, LC>;
   using LB = Loader<16 * J, CPR, true>;
   static constexpr int kStepB = LB::kBytes + LB::kScaleBytes;
   static constexpr int kStep = kStepB + LA::kBytes + LA::kScaleBytes;
-  static constexpr int kFit = 163840 / (kWaves * kStep);
+  static constexpr int kOwn = kRaw ? LC::kBytes + LC::kScaleBytes : 0;
+  static constexpr int kFit = (163840 / kWaves - kOwn) / kStep;
   static constexpr int S = kFit < 4 ? kFit : 4;
-  static constexpr int kLds = kWaves * S * kStep;
+  static constexpr int kLds = kWaves * (S * kStep + kOwn);
 };
 
-template <typename T, int J, int MR>
+template <typename T, typename X, int J, int MR>
 __global__ __launch_bounds__(64 * kWaves, 1) void k_mx4_skinny(Mx4Args g, int whole) {
-  using R = Ring<J, MR>;
+  using R = Ring<X, J, MR>;
   using LA = typename R::LA;
+  using LC = typename R::LC;
   using LB = typename R::LB;
   constexpr int CPR = R::CPR, S = R::S, kStep = R::kStep, kStepB = R::kStepB;
   constexpr int NB = CPR / 4;  // instructions of a step: block 4 u + q in lane group q
@@ -113,11 +163,15 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_mx4_skinny(Mx4Args g, int wh
 
   LA la;
   LB lb;
-  la.init(g.a, g.lda, g.as, g.ldas, g.M, g.kb, lane);
+  if constexpr (R::kRaw)
+    la.init(g.x, g.ldx, g.M, g.K, lane);
+  else
+    la.init(g.a, g.lda, g.as, g.ldas, g.M, g.kb, lane);
   lb.init(g.b + n0 * g.ldb, g.ldb, g.bs + n0 * g.ldbs, g.ldbs, nv, g.kb, lane);
   const int steps = (g.kb + CPR - 1) / CPR;
   const int n = steps > wave ? (steps - wave + kWaves - 1) / kWaves : 0;  // this wave's: wave, wave + kWaves, ..
-  char* mine = smem + wave * (S * kStep);
+  char* mine = smem + wave * (S * kStep + R::kOwn);
+  char* own = mine + S * kStep;  // X: the step's codes and scales
   const uint32_t mine_addr = lds_addr(mine);
   int slot_in = 0;
   // step j of this wave into ring slot j % S (past the end: empty loads, so that the waits count the same)
@@ -130,7 +184,8 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_mx4_skinny(Mx4Args g, int wh
   };
   // this lane's first scale byte in a step's dwords: of its row of A, of its columns
   const int ar = i16 & (MR - 1);
-  const int sat = LA::kBytes + ar * (LA::ND * 4) + static_cast<int>((reinterpret_cast<uintptr_t>(g.as) + ar * g.ldas) & 3u) + q;
+  const int sat = LC::kBytes + ar * (LC::ND * 4) + q +
+                  (R::kRaw ? 0 : static_cast<int>((reinterpret_cast<uintptr_t>(g.as) + ar * g.ldas) & 3u));
   int sbt[J];
 #pragma unroll
   for (int j = 0; j < J; ++j)
@@ -149,6 +204,24 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_mx4_skinny(Mx4Args g, int wh
     __builtin_amdgcn_sched_barrier(0);
     const char* tb = mine + slot * kStep;
     const char* ta = tb + kStepB;
+    if constexpr (R::kRaw) {
+      // (the step's blocks by lanes; rows that all lie past M are left as they are:
+      // what they give is never stored)
+#pragma unroll
+      for (int id0 = 0; id0 < MR * CPR; id0 += 64) {
+        const int id = id0 + lane, r = id / CPR, c = id - r * CPR;
+        if (id0 / CPR < g.M && id < MR * CPR) {
+          u32x4 x[4];
+          LA::block(ta, r, c, x);
+          uint32_t s;
+          const u32x4 codes = quantize32<X>(x, s);
+          *reinterpret_cast<u32x4*>(own + r * (CPR * 16) + sk_slot<CPR>(r, c) * 16) = codes;
+          *reinterpret_cast<uint8_t*>(own + LC::kBytes + r * (LC::ND * 4) + c) = static_cast<uint8_t>(s);
+        }
+      }
+      asm volatile("" ::: "memory");  // a wave's LDS operations run in order: written, then read by other lanes
+      ta = own;
+    }
     const int left = g.kb - (wave + i * kWaves) * CPR;  // blocks of the row from the step's first on
 #pragma unroll
     for (int u = 0; u < NB; ++u) {
@@ -188,21 +261,23 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_mx4_skinny(Mx4Args g, int wh
   }
 }
 
-template <typename T, int J, int MR>
+template <typename T, typename X, int J, int MR>
 int launch_skinny(const Mx4Args& g, hipStream_t st) {
-  constexpr int kLds = Ring<J, MR>::kLds;
-  auto kern = k_mx4_skinny<T, J, MR>;
+  constexpr int kLds = Ring<X, J, MR>::kLds;
+  auto kern = k_mx4_skinny<T, X, J, MR>;
   static std::atomic<uint64_t> reserved{0};
   if (const int rc = reserve_lds(reinterpret_cast<const void*>(kern), kLds, reserved, "mxfp4_mm"); rc != NTOPS_OK) return rc;
   const int whole = (g.ldd & 3) == 0 && (reinterpret_cast<uintptr_t>(g.d) & (4 * sizeof(T) - 1)) == 0;
-  note_kernel("mxfp4_skinny j%d m%d", J, MR);
+  note_kernel("mxfp4_skinny j%d m%d%s", J, MR, Ring<X, J, MR>::kRaw ? " fused" : "");
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((g.N + 16 * J - 1) / (16 * J))), dim3(64 * kWaves), kLds, st, g, whole);
   return check_launch("mxfp4_mm");
 }
 
-template <typename T, int MR>
+template <typename T, typename X, int MR>
 int run_skinny(const Mx4Args& g, int j, hipStream_t st) {
-  return j == 4 ? launch_skinny<T, 4, MR>(g, st) : j == 2 ? launch_skinny<T, 2, MR>(g, st) : launch_skinny<T, 1, MR>(g, st);
+  return j == 4   ? launch_skinny<T, X, 4, MR>(g, st)
+         : j == 2 ? launch_skinny<T, X, 2, MR>(g, st)
+                  : launch_skinny<T, X, 1, MR>(g, st);
 }
 
 // Columns of a block, in 16s: a CU takes its blocks one after the other, each at
@@ -227,7 +302,15 @@ int mx4_skinny(int out_dtype, const Mx4Args& g, hipStream_t st) {
   const int j = columns(g.N, g.kb);
   return dispatch_float16_32(out_dtype, "mxfp4_mm", [&](auto tag) {
     using T = decltype(tag);
-    return g.M <= 4 ? run_skinny<T, 4>(g, j, st) : run_skinny<T, 16>(g, j, st);
+    return g.M <= 4 ? run_skinny<T, void, 4>(g, j, st) : run_skinny<T, void, 16>(g, j, st);
+  });
+}
+
+int mx4_skinny_fused(int x_dtype, int out_dtype, const Mx4Args& g, hipStream_t st) {
+  const int j = columns(g.N, g.kb);
+  return dispatch_float16_32(out_dtype, "mxfp4_mm", [&](auto tag) {
+    using T = decltype(tag);
+    return x_dtype == NTOPS_BF16 ? run_skinny<T, __bf16, kFusedRows>(g, j, st) : run_skinny<T, _Float16, kFusedRows>(g, j, st);
   });
 }
 

@@ -48,6 +48,8 @@ decltype(&ntops_quantize_mxfp4) f_quantize_mxfp4;
 decltype(&ntops_dequantize_mxfp4) f_dequantize_mxfp4;
 decltype(&ntops_mxfp4_mm) f_mxfp4_mm;
 decltype(&ntops_mxfp4_mm_workspace) f_mxfp4_mm_workspace;
+decltype(&ntops_mxfp4_linear) f_mxfp4_linear;
+decltype(&ntops_mxfp4_linear_workspace) f_mxfp4_linear_workspace;
 decltype(&ntops_store_kv_cache) f_store_kv_cache;
 decltype(&ntops_kv_cache_attention) f_kv_cache_attention;
 decltype(&ntops_kv_cache_attention_workspace) f_kv_cache_attention_workspace;
@@ -595,8 +597,7 @@ PyObject* dequantize_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // mxfp4_mm(input, input_scale or None, mat2, mat2_scale, bias or None, dtype):
-// code rows the kernels read in place; a float input contiguous.  Its codes and
-// scales and the product's workspace are one allocation.
+// code rows the kernels read in place; a float input contiguous.
 PyObject* mxfp4_mm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NTOPS_TRY
   int code;
@@ -626,24 +627,21 @@ PyObject* mxfp4_mm(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return none();
   }
   at::Tensor out;
-  int rc = NTOPS_OK;
+  int rc;
   {
     NoGil free;
     out = at::empty({M, N}, at::TensorOptions().dtype(type).device(x->device()));
-    const int64_t bytes = f_mxfp4_mm_workspace(M, N, K);
-    const int64_t codes = xs ? 0 : M * 16 * blocks, scales = xs ? 0 : (M * blocks + 15) / 16 * 16;
+    const int64_t cols = x->size(1);
+    const int64_t bytes = xs ? f_mxfp4_mm_workspace(M, N, K)
+                             : f_mxfp4_linear_workspace(code16_32(*x), M, N, cols, x->data_ptr(), cols);
     at::Tensor tmp;
-    char* at = nullptr;
-    if (codes + scales + bytes > 0) {
-      tmp = workspace(*x, codes + scales + bytes);
-      at = static_cast<char*>(tmp.data_ptr());
-    }
-    if (!xs)
-      rc = f_quantize_mxfp4(code16_32(*x), M, x->size(1), x->data_ptr(), x->size(1), at, at + codes, st);
-    if (rc == NTOPS_OK)
-      rc = f_mxfp4_mm(code, M, N, K, xs ? x->data_ptr() : at, xs ? x->stride(0) : 16 * blocks, xs ? xs->data_ptr() : at + codes,
-                      xs ? xs->stride(0) : blocks, w->data_ptr(), w->stride(0), ws->data_ptr(), ws->stride(0),
-                      bias ? bias->data_ptr() : nullptr, out.data_ptr(), N, bytes > 0 ? at + codes + scales : nullptr, bytes, st);
+    if (bytes > 0) tmp = workspace(*x, bytes);
+    void* at = bytes > 0 ? tmp.data_ptr() : nullptr;
+    const void* b = bias ? bias->data_ptr() : nullptr;
+    rc = xs ? f_mxfp4_mm(code, M, N, K, x->data_ptr(), x->stride(0), xs->data_ptr(), xs->stride(0), w->data_ptr(), w->stride(0),
+                         ws->data_ptr(), ws->stride(0), b, out.data_ptr(), N, at, bytes, st)
+            : f_mxfp4_linear(code16_32(*x), code, M, N, cols, x->data_ptr(), cols, w->data_ptr(), w->stride(0), ws->data_ptr(),
+                             ws->stride(0), b, out.data_ptr(), N, at, bytes, st);
   }
   return rc == NTOPS_OK ? wrap(out) : none();
   NTOPS_END
@@ -785,6 +783,7 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
                    set("ntops_sdpa_workspace", f_sdpa_workspace) & set("ntops_copy2", f_copy2) &
                    set("ntops_quantize_mxfp4", f_quantize_mxfp4) & set("ntops_dequantize_mxfp4", f_dequantize_mxfp4) &
                    set("ntops_mxfp4_mm", f_mxfp4_mm) & set("ntops_mxfp4_mm_workspace", f_mxfp4_mm_workspace) &
+                   set("ntops_mxfp4_linear", f_mxfp4_linear) & set("ntops_mxfp4_linear_workspace", f_mxfp4_linear_workspace) &
                    set("ntops_store_kv_cache", f_store_kv_cache) & set("ntops_kv_cache_attention", f_kv_cache_attention) &
                    set("ntops_kv_cache_attention_workspace", f_kv_cache_attention_workspace);
   if (PyErr_Occurred()) return nullptr;

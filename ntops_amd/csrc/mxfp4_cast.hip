@@ -15,46 +15,14 @@
 // than an infinity and that than any number.
 #include <algorithm>
 
-#include "mfma.h"
+#include "mxfp4.h"
 
 namespace ntops {
 namespace {
 
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
-
-// fp32 value of scale byte s (< 255): 2^(s - 127).
-__device__ __forceinline__ float scale_value(uint32_t s) {
-  return __builtin_bit_cast(float, s == 0 ? 0x00400000u : s << 23);
-}
-
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
   return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false));
-}
-
-// 8 values to 8 codes (value i in nibble i) under `scale`.
-template <typename T>
-__device__ __forceinline__ uint32_t codes8(const T (&v)[8], float scale) {
-  uint32_t r = 0;
-  if constexpr (std::is_same<T, __bf16>::value) {
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, bf16x2_t{v[0], v[1]}, scale, 0);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, bf16x2_t{v[2], v[3]}, scale, 1);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, bf16x2_t{v[4], v[5]}, scale, 2);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, bf16x2_t{v[6], v[7]}, scale, 3);
-  } else if constexpr (std::is_same<T, _Float16>::value) {
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, f16x2_t{v[0], v[1]}, scale, 0);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, f16x2_t{v[2], v[3]}, scale, 1);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, f16x2_t{v[4], v[5]}, scale, 2);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, f16x2_t{v[6], v[7]}, scale, 3);
-  } else {
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], scale, 0);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], scale, 1);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], scale, 2);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], scale, 3);
-  }
-  return r;
 }
 
 // Index type I: 32 bits where every count fits.  VEC: rows of whole 16-byte
@@ -96,8 +64,7 @@ __global__ __launch_bounds__(256) void k_quantize_mxfp4(const T* x, int64_t ld, 
       top = max(top, __builtin_bit_cast(uint32_t, static_cast<float>(v[u][e])) & 0x7fffffffu);
     top = max(top, dpp_u32<kDppXor1>(top));  // (a block's four lanes are in a quad, whole waves active)
     top = max(top, dpp_u32<kDppXor2>(top));
-    const uint32_t exponent = top >> 23;
-    const uint32_t s = exponent == 255 ? 255 : exponent > 2 ? exponent - 2 : 0;
+    const uint32_t s = scale_byte(top);
     if (p < total) {
       codes[p] = s == 255 ? 0 : codes8<T>(v[u], scale_value(s));
       if ((threadIdx.x & 3) == 0) scales[p >> 2] = static_cast<uint8_t>(s);

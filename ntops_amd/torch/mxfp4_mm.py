@@ -13,7 +13,7 @@ import torch
 
 from ntops_amd import _lib
 from ntops_amd.torch.dequantize_mxfp4 import _checked_pair
-from ntops_amd.torch.quantize_mxfp4 import quantize_mxfp4
+from ntops_amd.torch.quantize_mxfp4 import _DTYPES, _rows
 from ntops_amd.torch.utils import _DeviceGuard, _cast_into, _contiguous
 
 
@@ -26,6 +26,10 @@ def _code_rows(t):
     if t.stride(1) == 1 and 0 <= t.stride(0) <= _FARTHEST_ROWS and t.stride(0) % 16 == 0 and t.data_ptr() % 16 == 0:
         return t
     return _cast_into(t, torch.empty(t.shape, dtype=t.dtype, device=t.device))
+
+
+def _scale_rows(t):
+    return t if t.stride(1) == 1 and 0 <= t.stride(0) <= _FARTHEST_ROWS else _contiguous(t)
 
 
 def mxfp4_mm(input, input_scale, mat2, mat2_scale, bias=None, *, dtype=torch.bfloat16):
@@ -43,7 +47,8 @@ def mxfp4_mm(input, input_scale, mat2, mat2_scale, bias=None, *, dtype=torch.bfl
     if input_scale is None:
         if -(-input.shape[1] // 32) != blocks:
             raise RuntimeError(f"mxfp4_mm: rows of {input.shape[1]} values do not have mat2's {blocks} blocks of 32")
-        input, input_scale = quantize_mxfp4(input)
+        if input.dtype not in _DTYPES:
+            raise RuntimeError(f"quantize_mxfp4: unsupported dtype {input.dtype}")
     elif _checked_pair(input, input_scale, "mxfp4_mm") != blocks:
         raise RuntimeError(f"mxfp4_mm: {input_scale.shape[1]} and {blocks} blocks cannot be multiplied")
     if bias is not None and (bias.shape != (n,) or bias.dtype != dtype):
@@ -52,15 +57,24 @@ def mxfp4_mm(input, input_scale, mat2, mat2_scale, bias=None, *, dtype=torch.bfl
     output = torch.empty((m, n), dtype=dtype, device=dev)
     lib = _lib.load()
     with _DeviceGuard(dev):
-        a, b = _code_rows(input), _code_rows(mat2)
-        sa, sb = (s if s.stride(1) == 1 and 0 <= s.stride(0) <= _FARTHEST_ROWS else _contiguous(s) for s in (input_scale, mat2_scale))
+        b, sb = _code_rows(mat2), _scale_rows(mat2_scale)
         bias = None if bias is None else _contiguous(bias)
-        scales = (sa.data_ptr(), sa.stride(0)), (sb.data_ptr(), sb.stride(0))
-        ws_bytes = lib.ntops_mxfp4_mm_workspace(m, n, 32 * blocks)
+        weight = b.data_ptr(), b.stride(0), sb.data_ptr(), sb.stride(0), None if bias is None else bias.data_ptr(), output.data_ptr(), n
+        if input_scale is None:
+            x, _, stride = _rows(input)
+            k = x.shape[1]
+            a = x.data_ptr(), stride
+            ws_bytes = lib.ntops_mxfp4_linear_workspace(_lib.dtype_code(x.dtype), m, n, k, *a)
+        else:
+            x, sx = _code_rows(input), _scale_rows(input_scale)
+            k = 32 * blocks
+            a = x.data_ptr(), x.stride(0), sx.data_ptr(), sx.stride(0)
+            ws_bytes = lib.ntops_mxfp4_mm_workspace(m, n, k)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
-        rc = lib.ntops_mxfp4_mm(
-            _lib.dtype_code(dtype), m, n, 32 * blocks, a.data_ptr(), a.stride(0), *scales[0], b.data_ptr(), b.stride(0),
-            *scales[1], None if bias is None else bias.data_ptr(), output.data_ptr(), n,
-            None if ws is None else ws.data_ptr(), ws_bytes, _lib.stream_of(output))
+        rest = *a, *weight, None if ws is None else ws.data_ptr(), ws_bytes, _lib.stream_of(output)
+        if input_scale is None:
+            rc = lib.ntops_mxfp4_linear(_lib.dtype_code(x.dtype), _lib.dtype_code(dtype), m, n, k, *rest)
+        else:
+            rc = lib.ntops_mxfp4_mm(_lib.dtype_code(dtype), m, n, k, *rest)
     _lib.check(rc, "ntops_amd.mxfp4_mm")
     return output

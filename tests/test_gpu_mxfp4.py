@@ -203,6 +203,51 @@ def test_product_of_activations():
         assert torch.equal(nt.mxfp4_mm(x, None, b, sb), nt.mxfp4_mm(*nt.quantize_mxfp4(x), b, sb))
 
 
+# Up to 4 rows of 16 bits on 16-byte addresses are rounded inside the product's
+# kernel: the same codes, so the same sums, bit for bit.  One column group of a block,
+# two and four; last blocks and steps that the row fills in part or not at all.
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("n,k", [(70, 8), (1, 32), (33, 1000), (200, 1024), (40, 4096 + 40), (5000, 264), (20000, 2056), (130, 4104)])
+def test_product_of_few_activations(m, n, k):
+    b, sb = nt.quantize_mxfp4(torch.randn(n, k).cuda())
+    for dtype in DTYPES:
+        x = spread(m, k, dtype=dtype).cuda()
+        if n == 33:
+            x[0, -1], x[m - 1, 40] = float("nan"), float("-inf")
+        bias = torch.randn(n).to(dtype).cuda() if n % 3 else None
+        want = nt.mxfp4_mm(*nt.quantize_mxfp4(x), b, sb, bias, dtype=dtype)
+        fused = m <= 4 and dtype != torch.float32
+        wide = torch.full((m, k + 24), float("nan"), dtype=dtype, device="cuda")
+        for left in (8, 3, 0, None):  # on 16-byte addresses and off them, between values that are not numbers
+            view = x
+            if left is not None:
+                view = wide.fill_(float("nan"))[:, left : left + k]
+                view.copy_(x)
+            got = nt.mxfp4_mm(view, None, b, sb, bias, dtype=dtype)
+            assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0), want.nan_to_num(0)), (dtype, left)
+            assert ("fused" in _lib.last_kernel()) == (fused and left != 3), (dtype, left, _lib.last_kernel())
+
+
+def test_product_of_few_activations_graph_and_stream():
+    b, sb = nt.quantize_mxfp4(torch.randn(640, 2048).cuda())
+    x = torch.randn(3, 2048, device="cuda").half()
+    want = nt.mxfp4_mm(x, None, b, sb)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = nt.mxfp4_mm(x, None, b, sb)
+    side.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = nt.mxfp4_mm(x, None, b, sb)
+    for _ in range(3):
+        x.copy_(torch.randn(3, 2048))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, nt.mxfp4_mm(*nt.quantize_mxfp4(x), b, sb))
+
+
 @pytest.mark.parametrize("m", [2, 40, 200])
 def test_product_keeps_nan_blocks_apart(m):
     x, w = torch.randn(m, 512), torch.randn(60, 512)

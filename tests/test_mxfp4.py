@@ -99,3 +99,34 @@ def test_c_entry_points_refuse():
     assert _mm(lib, k=1 << 40, lda=1 << 35, ldb=1 << 35) == 2 and "too large" in err()
     assert _mm(lib, ws=264) == 1 and "workspace" in err()
     assert _mm(lib, m=0) == 0 and lib.ntops_quantize_mxfp4(_lib.BF16, 0, 32, None, 32, None, None, None) == 0
+
+
+def _linear(lib, x_dtype=_lib.BF16, dtype=_lib.BF16, m=2, n=4, k=64, x=256, ldx=64, b=1024, ldb=32, bs=2048, ldbs=2, bias=None, out=4096, ldd=4, ws=None, wsb=0):
+    return lib.ntops_mxfp4_linear(x_dtype, dtype, m, n, k, P(x), ldx, P(b), ldb, P(bs), ldbs, P(bias), P(out), ldd, P(ws), wsb, None)
+
+
+def test_linear_refuses():
+    lib = _lib.load()
+    err = lambda: lib.ntops_last_error().decode()
+    for m in (2, 9):  # rounded by the product's kernel, and into the workspace
+        assert _linear(lib, m=-m) == 1 and "negative" in err()
+        assert _linear(lib, x_dtype=_lib.F64, m=m) == 2 and "input dtype" in err()
+        ws = dict(ws=8192, wsb=1 << 20)
+        assert _linear(lib, dtype=_lib.F64, m=m, **ws) == 2
+        assert _linear(lib, x=None, m=m, **ws) == 1 and "null" in err()
+        assert _linear(lib, out=None, m=m, **ws) == 1 and "null" in err()
+        assert _linear(lib, b=None, m=m, **ws) == 1 and "null" in err()
+        assert _linear(lib, b=1032, m=m, **ws) == 1 and "16 bytes" in err()
+        assert _linear(lib, ldbs=-2, m=m, **ws) == 1 and "negative" in err()
+        assert _linear(lib, m=m, k=1 << 40, ldx=1 << 40, **ws) == 2 and "too large" in err()
+        assert _linear(lib, m=m, n=1 << 40, **ws) == 2 and "too large" in err()
+        assert _linear(lib, m=0, x=None) == 0 and _linear(lib, n=0, m=m) == 0
+    assert _linear(lib, m=9) == 1 and "workspace" in err()
+    assert _linear(lib, m=9, ws=8192, wsb=9 * 34) == 1 and "workspace" in err()
+    assert _linear(lib, m=9, ws=8196, wsb=1 << 20) == 1 and "workspace" in err()
+    need = lib.ntops_mxfp4_linear_workspace
+    assert need(_lib.BF16, 4, 4, 64, P(256), 64) == 0
+    for args in ((_lib.F32, 4, 4, 64, P(256), 64), (_lib.BF16, 5, 4, 64, P(256), 64), (_lib.F16, 4, 4, 64, P(264), 64), (_lib.F16, 4, 4, 62, P(256), 64)):
+        assert need(*args) >= args[1] * 34, args
+    assert need(_lib.F16, 2, 4, 64, P(256), 65) >= 2 * 34 and need(_lib.F16, 1, 4, 64, P(256), 65) == 0
+    assert need(_lib.BF16, 0, 4, 64, None, 64) == 0 and need(_lib.BF16, 4, 4, 0, None, 0) == 0
