@@ -3,11 +3,14 @@
 //
 // A block covers 16 J columns; its four waves each own K steps of their own and
 // stream them through their own part of the LDS by direct DMA, as many steps ahead
-// as the LDS holds (two to four), with no barrier before their fp32 sums are
-// merged.  A step is 8 KiB of B (16 J rows of 512 / J bytes, non-temporal, whole
-// lines), the same columns of A's rows, and the scales.  Up to 4 rows (MR 4) A's
-// part of a step is a quarter, and the ring a step longer; the instruction's other
-// rows read the four again.
+// as half a CU's LDS holds (one to three), with no barrier before their fp32 sums are
+// merged.  Two blocks share a CU, so that one streams while the other starts or
+// merges: 1 row, 100000 x 4096 took 52.2 us with one block of twice the ring a CU and
+// 38.7 with two, 28672 x 4096 17.8 and 15.1.  A step is 4 or (J 4) 8 KiB of B (16 J
+// rows of 256 or 128 bytes, non-temporal, whole lines), the same columns of A's
+// rows, and the scales; steps of 8 KiB for J 1 left the ring one step shorter, 8.2 us
+// -> 10.4 at 1 row, 4096 x 14336.  Up to 4 rows (MR 4) A's part of a step is a
+// quarter, and the ring longer; the instruction's other rows read the four again.
 //
 // The scales are loaded as the dwords that the step's CPR bytes of a row lie in (one
 // more than they fill, as a row may start inside one) and read as single bytes;
@@ -20,9 +23,10 @@
 // codes go to the LDS, where the fragments are read as ever.  Every block rounds the
 // same rows again, which pays for up to 4 of them: a kernel before this one and then
 // this one, against this one alone, in a captured graph, took 1 row of 4096 values
-// 6.4 against 5.1 us for 640 columns and 12.0 against 10.7 for 14336; 4 rows 6.4
-// against 5.4 and 12.1 against 11.0, and 4 rows of 14336 values, the most a wave has
-// to round, 12.1 against 12.5 for 4096 columns.
+// 5.9 against 4.4 us for 640 columns and 11.2 against 9.9 for 14336; 4 rows 5.8
+// against 4.7 and 11.2 against 10.6, and 4 rows of 14336 values, the most a wave has
+// to round, 10.8 against 10.4 for 4096 columns.
+#include <algorithm>
 #include <atomic>
 
 #include "gemm_mxfp4.h"
@@ -133,20 +137,21 @@ struct RawLoader {
 template <typename X, int J, int MR>
 struct Ring {
   static constexpr bool kRaw = !std::is_same<X, void>::value;
-  static constexpr int CPR = 32 / J;  // blocks of a row per step
+  static constexpr int CPR = J == 1 ? 16 : 8;  // blocks of a row per step
   using LC = Loader<MR, CPR, false>;
   using LA = std::conditional_t<kRaw, RawLoader<MR, CPR>, LC>;
   using LB = Loader<16 * J, CPR, true>;
   static constexpr int kStepB = LB::kBytes + LB::kScaleBytes;
   static constexpr int kStep = kStepB + LA::kBytes + LA::kScaleBytes;
   static constexpr int kOwn = kRaw ? LC::kBytes + LC::kScaleBytes : 0;
-  static constexpr int kFit = (163840 / kWaves - kOwn) / kStep;
+  static constexpr int kFit = (163840 / 2 / kWaves - kOwn) / kStep;  // two blocks a CU
   static constexpr int S = kFit < 4 ? kFit : 4;
   static constexpr int kLds = kWaves * (S * kStep + kOwn);
+  static_assert(S >= 1 && kLds >= kWaves * J * 1024, "a step, and the sums to merge");
 };
 
 template <typename T, typename X, int J, int MR>
-__global__ __launch_bounds__(64 * kWaves, 1) void k_mx4_skinny(Mx4Args g, int whole) {
+__global__ __launch_bounds__(64 * kWaves, 2) void k_mx4_skinny(Mx4Args g, int whole) {
   using R = Ring<X, J, MR>;
   using LA = typename R::LA;
   using LC = typename R::LC;
@@ -280,26 +285,32 @@ int run_skinny(const Mx4Args& g, int j, hipStream_t st) {
                   : launch_skinny<T, X, 1, MR>(g, st);
 }
 
-// Columns of a block, in 16s: a CU takes its blocks one after the other, each at
-// the cost of its start (as much as 48 KiB of B) and its bytes.
-int columns(int64_t N, int64_t kb) {
+// Columns of a block, in 16s.  A CU's blocks, counted in halves as two run at once
+// and one alone has the CU's bandwidth, cost their bytes and their starts, as much
+// as 20 KiB of B each.  A ring of one step (lone) needs the CU's other block to
+// cover its waits; two columns give the same sums as four.
+// Measured with 1, 2 and 4 (us): 1 row, 4096 x 4096 4.8, 5.3, 7.1; 14336 x 4096
+// 11.2, 9.6, 9.2; 100000 x 4096 52.4, 42.0, 38.7; 24000 x 2048 12.1, 10.5, 9.4;
+// 8 rows, 14336 x 4096 12.3, 9.9, 11.0; 16 rows, 100000 x 4096 60.4, 47.7, 45.4.
+int columns(int64_t N, int64_t kb, bool lone) {
   int best = 1;
   int64_t least = 0;
+  const int64_t cus = cu_count_cached();
   for (int j = 1; j <= 4; j *= 2) {
-    const int64_t rounds = ceil_div(ceil_div(N, 16 * j), cu_count_cached());
-    const int64_t cost = rounds * (48 * 1024 + 16 * j * kb * 16);
+    const int64_t halves = std::max<int64_t>(2, ceil_div(2 * ceil_div(N, 16 * j), cus));
+    const int64_t cost = halves * (20 * 1024 + 16 * j * kb * 17);
     if (j == 1 || cost <= least) {
       least = cost;
       best = j;
     }
   }
-  return best;
+  return best == 4 && lone && ceil_div(N, 64) <= cus ? 2 : best;
 }
 
 }  // namespace
 
 int mx4_skinny(int out_dtype, const Mx4Args& g, hipStream_t st) {
-  const int j = columns(g.N, g.kb);
+  const int j = columns(g.N, g.kb, g.M > 4);
   return dispatch_float16_32(out_dtype, "mxfp4_mm", [&](auto tag) {
     using T = decltype(tag);
     return g.M <= 4 ? run_skinny<T, void, 4>(g, j, st) : run_skinny<T, void, 16>(g, j, st);
@@ -307,7 +318,7 @@ int mx4_skinny(int out_dtype, const Mx4Args& g, hipStream_t st) {
 }
 
 int mx4_skinny_fused(int x_dtype, int out_dtype, const Mx4Args& g, hipStream_t st) {
-  const int j = columns(g.N, g.kb);
+  const int j = columns(g.N, g.kb, true);
   return dispatch_float16_32(out_dtype, "mxfp4_mm", [&](auto tag) {
     using T = decltype(tag);
     return x_dtype == NTOPS_BF16 ? run_skinny<T, __bf16, kFusedRows>(g, j, st) : run_skinny<T, _Float16, kFusedRows>(g, j, st);
