@@ -425,12 +425,16 @@ __global__ __launch_bounds__(256) void k_cache_merge(CacheAttnArgs a, int nsplit
 // known here: as many slices as leave about one eight-wave block per CU, none
 // shorter than two tiles a wave at full length (twice the slices: (16, 32 / 8, 1,
 // 2048 .. 4096, 128) 26.5 -> 30.3 us with four-wave blocks).  From two heads per CU
-// on nothing is split, and two-wave blocks, four to a CU, hide each other's start
-// ((64, 32 / 32, 1, 512 .. 1024, 128): eight-wave ones 85.1 us, two-wave ones 73.8).
+// on nothing is split, and four-wave blocks, two to a CU, hide each other's start
+// ((64, 32 / 32, 1, 512 .. 1024, 128): eight-wave ones 85.1 us, four 68.7, two 73.8;
+// (100, 32 / 8, 1, 2048 .. 4096, 128): four 114, two 124).  Between one head a CU and
+// two they do for short caches: 264 and 448 heads at 500 .. 1000 tokens 19.7 -> 18.0
+// us and 24.8 -> 21.9, but at 2048 .. 4096 49.1 -> 52.1 and 66.1 -> 67.3.
 void decode_split(int64_t heads, int64_t C, int64_t D, int& waves, int& nsplit) {
-  waves = heads < 2 * cu_count_cached() ? 8 : 2;
+  const int64_t cus = cu_count_cached();
+  waves = heads >= 2 * cus || (heads > cus && C <= 2048) ? 4 : 8;
   const int64_t step = (D > 64 ? 32 : 64) * waves;
-  int64_t n = std::min({static_cast<int64_t>(kMaxSplit), cu_count_cached() / heads, ceil_div(C, 2 * step)});
+  int64_t n = std::min({static_cast<int64_t>(kMaxSplit), cus / heads, ceil_div(C, 2 * step)});
   if (n <= 2 && C <= 8 * step) n = 1;  // two short slices gain what the merge's launch costs
   nsplit = static_cast<int>(std::max<int64_t>(n, 1));
 }
@@ -461,7 +465,7 @@ int run_decode(const CacheAttnArgs& a, void* ws, int64_t ws_bytes, hipStream_t s
   float* part = static_cast<float*>(ws);
   if (waves == 8)
     return a.D > 64 ? launch_decode<T, 128, 8>(a, nsplit, part, st) : launch_decode<T, 64, 8>(a, nsplit, part, st);
-  return a.D > 64 ? launch_decode<T, 128, 2>(a, nsplit, part, st) : launch_decode<T, 64, 2>(a, nsplit, part, st);
+  return a.D > 64 ? launch_decode<T, 128, 4>(a, nsplit, part, st) : launch_decode<T, 64, 4>(a, nsplit, part, st);
 }
 
 }  // namespace
