@@ -424,18 +424,21 @@ __global__ __launch_bounds__(256) void k_cache_merge(CacheAttnArgs a, int nsplit
 // Waves of a block and slices of a sequence.  The sequences' lengths are not
 // known here: as many slices as leave about one eight-wave block per CU, none
 // shorter than two tiles a wave at full length (twice the slices: (16, 32 / 8, 1,
-// 2048 .. 4096, 128) 26.5 -> 30.3 us with four-wave blocks).  From two heads per CU
-// on nothing is split, and four-wave blocks, two to a CU, hide each other's start
-// ((64, 32 / 32, 1, 512 .. 1024, 128): eight-wave ones 85.1 us, four 68.7, two 73.8;
-// (100, 32 / 8, 1, 2048 .. 4096, 128): four 114, two 124).  Between one head a CU and
-// two they do for short caches: 264 and 448 heads at 500 .. 1000 tokens 19.7 -> 18.0
-// us and 24.8 -> 21.9, but at 2048 .. 4096 49.1 -> 52.1 and 66.1 -> 67.3.
+// 2048 .. 4096, 128) 26.5 -> 30.3 us with four-wave blocks).  From one head per CU
+// on four-wave blocks, two to a CU, hide each other's start ((64, 32 / 32, 1, 512 ..
+// 1024, 128): eight-wave ones 85.1 us, four 68.7, two 73.8; (100, 32 / 8, 1, 2048 ..
+// 4096, 128): four 114, two 124; (33, 32 / 8, 1, 500 .. 1000, 128): eight 19.7, four
+// 17.9; 448 heads over 2048 .. 4096: 66.1, 67.3).  Up to one and a half heads per CU
+// that leaves half the CUs idle at the end, and a long sequence goes in three
+// slices: 264 heads over 4096 67.5 -> 59.8 us, over 2048 .. 4096 48.9 -> 46.5, 320
+// 70.6 -> 61.3 and 55.9 -> 51.8, 384 73.9 -> 73.2, but 448 78.7 -> 85.0.
 void decode_split(int64_t heads, int64_t C, int64_t D, int& waves, int& nsplit) {
   const int64_t cus = cu_count_cached();
-  waves = heads >= 2 * cus || (heads > cus && C <= 2048) ? 4 : 8;
+  waves = heads > cus ? 4 : 8;
   const int64_t step = (D > 64 ? 32 : 64) * waves;
   int64_t n = std::min({static_cast<int64_t>(kMaxSplit), cus / heads, ceil_div(C, 2 * step)});
   if (n <= 2 && C <= 8 * step) n = 1;  // two short slices gain what the merge's launch costs
+  if (heads > cus && 2 * heads <= 3 * cus && C > 2048) n = 3;
   nsplit = static_cast<int>(std::max<int64_t>(n, 1));
 }
 

@@ -197,14 +197,14 @@ def test_attention(b, hq, h, sq, c, d, block, dtype, causal):
     check_attention(query, caches, lengths, causal, block, 0.3)
 
 
-# More heads than compute units: nothing is split, and blocks of fewer waves share a
-# unit; with long caches only from two heads a unit on.
+# More heads than compute units: blocks of fewer waves share a unit, and only long
+# caches of few more heads are split.
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize(
-    "b,hq,h,sq,c,d,block,waves",
-    [(66, 16, 8, 1, 130, 128, 32, 4), (40, 24, 8, 2, 300, 64, 16, 4), (9, 64, 64, 1, 1030, 80, 64, 4), (37, 8, 8, 3, 2050, 16, 128, 8), (520, 2, 1, 1, 2100, 32, 64, 4)],
+    "b,hq,h,sq,c,d,block,split",
+    [(66, 16, 8, 1, 130, 128, 32, 1), (40, 24, 8, 2, 300, 64, 16, 1), (9, 64, 64, 1, 1030, 80, 64, 1), (37, 8, 8, 3, 2050, 16, 128, 3), (520, 2, 1, 1, 2100, 32, 64, 1)],
 )
-def test_attention_many_heads(b, hq, h, sq, c, d, block, waves, dtype):
+def test_attention_many_heads(b, hq, h, sq, c, d, block, split, dtype):
     caches = filled(b, h, c, d, block, dtype)
     query = torch.randn(b, hq, sq, d).to(dtype).cuda()
     lengths = torch.randint(0, c + 1, (b,), dtype=torch.int32)
@@ -212,7 +212,7 @@ def test_attention_many_heads(b, hq, h, sq, c, d, block, waves, dtype):
     check_attention(query, caches, lengths.cuda(), True, block)
     nt.kv_cache_attention(query, *caches, lengths.cuda(), block_size=block)
     if torch.cuda.get_device_properties(0).multi_processor_count == 256:
-        assert f"waves{waves} split1" in _lib.last_kernel(), _lib.last_kernel()
+        assert f"waves4 split{split}" in _lib.last_kernel(), _lib.last_kernel()
 
 
 @pytest.mark.parametrize("b,hq,h,sq,c,d,block", SHAPES[1:18:4])
