@@ -1,15 +1,20 @@
 // The MXFP4 product's tile kernel, its split over K, and the C entry points.
 //
-// BT x BT output tiles, four waves of BT / 2 x BT / 2, K tiles of 256 values (128
-// bytes a row, whole lines) through a ring of four stages filled by direct DMA
-// three tiles ahead; one barrier per K tile.
+// BT x BT output tiles, four waves of 32 x 32 or eight of 64 x 32, two a SIMD either
+// way (a block of 64 x 64 shares its CU with another), so that one issues where the
+// other waits: (1024, 4096, 4096) bf16 with four waves of 64 x 64 23.8 us, with eight
+// 20.1.  K tiles of 256 values (128 bytes a row, whole lines) go through a ring of
+// four stages filled by direct DMA three tiles ahead; one barrier per K tile.  What
+// bounds it is the delivery of the tiles into the LDS, some 35 bytes a ns and CU.
 //
-// Scales come as dwords.  Where a row's scales do not start on one, or K tiles
-// end inside a dword (FIT false), a lane loads the three dwords that its row's 8
-// bytes lie in and reads single bytes; bytes behind the row's last block, which
-// may belong to another row and be 255 (NaN), become 0 there.  Such a dword may
-// reach up to 3 bytes past the scales' end or before their start; being aligned
-// it lies within what the memory's page holds.
+// Scales come as dwords, those of two K tiles together: a row's 8 bytes a K tile are
+// a request as a line of codes is ((512, 4096, 14336) a K tile's at a time 55.6 us,
+// two 46.4, four, which read the LDS in conflict, 47.4).  Where a row's scales do not
+// start on a dword, or K tiles end inside one (FIT false), a lane loads the three
+// dwords that its row's 8 bytes of a K tile lie in and reads single bytes; bytes
+// behind the row's last block, which may belong to another row and be 255 (NaN),
+// become 0 there.  Such a dword may reach up to 3 bytes past the scales' end or
+// before their start; being aligned it lies within what the memory's page holds.
 #include <algorithm>
 #include <atomic>
 
@@ -22,29 +27,39 @@ constexpr int kStages = 4;
 
 template <int BT, bool FIT>
 struct TileShape {
-  static constexpr int kRowsPerWave = BT / 4;                  // rows of an operand that a wave loads
+  static constexpr int kWaves = BT == 128 ? 8 : 4;
+  static constexpr int kWN = kWaves / 2;  // waves along a tile's columns
+  static constexpr int kRowsPerWave = BT / kWaves;                  // rows of an operand that a wave loads
   static constexpr int kCodes = BT * 128;                      // bytes of an operand's codes per stage
-  static constexpr int kDwords = FIT ? 2 : 3;                  // of a row's scales
+  static constexpr int kStage = 2 * kCodes;
+  static constexpr int kGroup = FIT ? 2 : 1;                   // K tiles whose scales are loaded together
+  static constexpr int kDwords = FIT ? 4 : 3;                  // of a row's scales in a group
   static constexpr int kScaleInst = (kRowsPerWave * kDwords + 63) / 64;
-  static constexpr int kScales = 4 * kScaleInst * 256;         // bytes of an operand's scales
-  static constexpr int kStage = 2 * (kCodes + kScales);
-  static constexpr int kLds = kStages * kStage;
-  static constexpr int kLoads = 2 * (kRowsPerWave / 8 + kScaleInst);  // DMA instructions per wave and stage
+  static constexpr int kScales = kWaves * kScaleInst * 256;    // bytes of an operand's scales in a group
+  static constexpr int kScaleRing = 8;                         // groups
+  static constexpr int kScalesPerTile = 2 * kScaleInst / kGroup;
+  static constexpr int kScalesAt = kStages * kStage;
+  static constexpr int kLds = kScalesAt + kScaleRing * 2 * kScales;
+  static constexpr int kLoads = 2 * kRowsPerWave / 8 + kScalesPerTile;  // DMA instructions per wave and K tile
+  static_assert(kRowsPerWave == 16 && kScalesPerTile * kGroup == 2 * kScaleInst && kLds * (BT == 64 ? 2 : 1) <= 163840, "tile");
 };
 
 // whole: the output's rows are runs that 4 elements at a time can be stored to.
 template <typename T, int BT, bool FIT>
-__global__ __launch_bounds__(256, BT == 64 ? 2 : 1) void k_mx4_tile(Mx4Args g, int tm_count, int tn_count, int whole) {
+__global__ __launch_bounds__(64 * (BT == 128 ? 8 : 4), BT == 64 ? 2 : 1) void k_mx4_tile(Mx4Args g, int tm_count, int tn_count, int whole) {
   using S = TileShape<BT, FIT>;
-  constexpr int TW = BT / 32;  // 16-row (and column) pieces of a wave's tile
+  constexpr int TW = BT / 32, TN = BT / S::kWN / 16;  // 16-row and 16-column pieces of a wave's tile
   constexpr int ND = S::kDwords;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave / S::kWN, wn = wave % S::kWN;
   const int q = lane >> 4, i16 = lane & 15;
-  // tiles by columns of up to 8 row tiles, so that neighbouring blocks share operands
-  const int t = blockIdx.x;
+  // Tiles by columns of up to 8 row tiles, so that neighbours share operands, and an
+  // XCD (workgroups go round the eight) takes a run of them: (512, 4096, 4096) 17.6 ->
+  // 16.2 us.
+  const int xcd = blockIdx.x & 7;
+  const int t = xcd * static_cast<int>(gridDim.x >> 3) + min(xcd, static_cast<int>(gridDim.x & 7)) + static_cast<int>(blockIdx.x >> 3);
   const int band = t / (8 * tn_count);
   const int rows_here = min(8, tm_count - band * 8);
   const int in = t - band * 8 * tn_count;
@@ -65,8 +80,23 @@ __global__ __launch_bounds__(256, BT == 64 ? 2 : 1) void k_mx4_tile(Mx4Args g, i
   const u32x4 rsb = make_rsrc(sb0 - ob, (ob + (nv - 1) * g.ldbs + g.kb + 3) & ~3ll);
   const uint32_t smem_addr = lds_addr(smem);
 
-  // this wave's loads of K tile j: BT / 4 rows of A and of B (8 rows an
-  // instruction), and their scales (row l / ND, dword l % ND)
+  // this wave's load id of scale group gr: 16 rows of A's or B's (row l / ND, dword l % ND)
+  auto issue_scales = [&](int gr, int id) {
+    const int u = id % S::kScaleInst;
+    const bool of_b = id >= S::kScaleInst;
+    const int l = u * 64 + lane;
+    const int in_wave = l / ND, row = wave * S::kRowsPerWave + in_wave;
+    const int b0 = kb0 + gr * (S::kGroup * 8), blk = b0 + (l - in_wave * ND) * 4;
+    const bool ok = in_wave < S::kRowsPerWave && b0 < kb1 && row < (of_b ? nv : mv);
+    // (past the row's last dword: the next row's, masked or not read below; past the last row's: zeros)
+    const uint32_t off = static_cast<uint32_t>((of_b ? ob + row * g.ldbs : oa + row * g.ldas) + blk) & ~3u;
+    const uint32_t dst = smem_addr + S::kScalesAt +
+                         static_cast<uint32_t>((gr & (S::kScaleRing - 1)) * (2 * S::kScales) + (of_b ? S::kScales : 0) +
+                                               (wave * S::kScaleInst + u) * 256);
+    dma4(of_b ? rsb : rsa, dst, ok ? off : kOOB);
+  };
+  // this wave's loads of K tile j: 16 rows of A and of B, 8 an instruction, and its
+  // part of the scales of the next group
   auto issue = [&](int j) {
     const uint32_t st = smem_addr + static_cast<uint32_t>((j & (kStages - 1)) * S::kStage);
     const int b0 = kb0 + j * 8;
@@ -79,34 +109,26 @@ __global__ __launch_bounds__(256, BT == 64 ? 2 : 1) void k_mx4_tile(Mx4Args g, i
       dma16(rb, dst + S::kCodes, blk < kb1 && row < nv ? static_cast<uint32_t>(row * g.ldb + blk * 16) : kOOB);
     }
 #pragma unroll
-    for (int u = 0; u < S::kScaleInst; ++u) {
-      const int id = u * 64 + lane;
-      const int in_wave = id / ND, row = wave * S::kRowsPerWave + in_wave;
-      const int blk = b0 + (id - in_wave * ND) * 4;
-      const bool ok = in_wave < S::kRowsPerWave && b0 < kb1;
-      const uint32_t dst = st + 2 * S::kCodes + static_cast<uint32_t>((wave * S::kScaleInst + u) * 256);
-      // (past the row's last dword: the next row's, masked below; past the last row's: zeros)
-      dma4(rsa, dst, ok && row < mv ? static_cast<uint32_t>(oa + row * g.ldas + blk) & ~3u : kOOB);
-      dma4(rsb, dst + S::kScales, ok && row < nv ? static_cast<uint32_t>(ob + row * g.ldbs + blk) & ~3u : kOOB);
-    }
+    for (int u = 0; u < S::kScalesPerTile; ++u) issue_scales(j / S::kGroup + 1, j % S::kGroup * S::kScalesPerTile + u);
   };
   // LDS offset of row r's scales of a K tile (not FIT: of the byte of block q)
   auto scale_at = [&](int r, int o, int64_t ld) {
     const int w = r / S::kRowsPerWave, in_wave = r - w * S::kRowsPerWave;
     return w * S::kScaleInst * 256 + in_wave * ND * 4 + (FIT ? 0 : static_cast<int>((o + r * ld) & 3) + q);
   };
-  int sat[TW], sbt[TW];
+  int sat[TW], sbt[TN];
 #pragma unroll
-  for (int i = 0; i < TW; ++i) {
-    sat[i] = 2 * S::kCodes + scale_at(wm * (BT / 2) + i * 16 + i16, oa, g.ldas);
-    sbt[i] = 2 * S::kCodes + S::kScales + scale_at(wn * (BT / 2) + i * 16 + i16, ob, g.ldbs);
-  }
+  for (int i = 0; i < TW; ++i) sat[i] = scale_at(wm * (BT / 2) + i * 16 + i16, oa, g.ldas);
+#pragma unroll
+  for (int i = 0; i < TN; ++i) sbt[i] = S::kScales + scale_at((wn * TN + i) * 16 + i16, ob, g.ldbs);
 
-  f32x4 acc[TW][TW];
+  f32x4 acc[TW][TN];
 #pragma unroll
   for (int i = 0; i < TW; ++i)
 #pragma unroll
-    for (int j = 0; j < TW; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < 2 * S::kScaleInst; ++u) issue_scales(0, u);
   issue(0);
   issue(1);
   issue(2);
@@ -117,45 +139,45 @@ __global__ __launch_bounds__(256, BT == 64 ? 2 : 1) void k_mx4_tile(Mx4Args g, i
     asm volatile("" ::: "memory");
     issue(j + 3);
     const char* st = smem + (j & (kStages - 1)) * S::kStage;
-    uint32_t sa[TW], sb[TW];
+    const char* sc = smem + S::kScalesAt + (j / S::kGroup & (S::kScaleRing - 1)) * (2 * S::kScales) + j % S::kGroup * 8;
+    uint32_t sa[TW], sb[TN];
     // the scales of blocks q and q + 4 of each row, in bytes 0 and 1
     if constexpr (FIT) {
       const uint32_t sel = 0x0400u + q * 0x0101u;
       const auto two = [&](int at) {
-        const u32x2 w = *reinterpret_cast<const u32x2*>(st + at);
+        const u32x2 w = *reinterpret_cast<const u32x2*>(sc + at);
         return __builtin_amdgcn_perm(w.y, w.x, sel);
       };
 #pragma unroll
-      for (int i = 0; i < TW; ++i) {
-        sa[i] = two(sat[i]);
-        sb[i] = two(sbt[i]);
-      }
+      for (int i = 0; i < TW; ++i) sa[i] = two(sat[i]);
+#pragma unroll
+      for (int i = 0; i < TN; ++i) sb[i] = two(sbt[i]);
     } else {
       const int left = kb1 - kb0 - j * 8 - q;  // blocks from this lane's first on
       const uint32_t mask = left > 4 ? 0xffffu : left > 0 ? 0xffu : 0u;
+      const auto two = [&](int at) {
+        const uint8_t* p = reinterpret_cast<const uint8_t*>(sc + at);
+        return (p[0] | static_cast<uint32_t>(p[4]) << 8) & mask;
+      };
 #pragma unroll
-      for (int i = 0; i < TW; ++i) {
-        const uint8_t* pa = reinterpret_cast<const uint8_t*>(st + sat[i]);
-        const uint8_t* pb = reinterpret_cast<const uint8_t*>(st + sbt[i]);
-        sa[i] = (pa[0] | static_cast<uint32_t>(pa[4]) << 8) & mask;
-        sb[i] = (pb[0] | static_cast<uint32_t>(pb[4]) << 8) & mask;
-      }
+      for (int i = 0; i < TW; ++i) sa[i] = two(sat[i]);
+#pragma unroll
+      for (int i = 0; i < TN; ++i) sb[i] = two(sbt[i]);
     }
     const auto frag = [&](int area, int r, int ks) {
       return *reinterpret_cast<const u32x4*>(st + area * S::kCodes + r * 128 + kslot<64>(r, 4 * ks + q) * 16);
     };
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      u32x4 fa[TW], fb[TW];
+      u32x4 fa[TW], fb[TN];
 #pragma unroll
-      for (int i = 0; i < TW; ++i) {
-        fa[i] = frag(0, wm * (BT / 2) + i * 16 + i16, ks);
-        fb[i] = frag(1, wn * (BT / 2) + i * 16 + i16, ks);
-      }
+      for (int i = 0; i < TW; ++i) fa[i] = frag(0, wm * (BT / 2) + i * 16 + i16, ks);
+#pragma unroll
+      for (int i = 0; i < TN; ++i) fb[i] = frag(1, (wn * TN + i) * 16 + i16, ks);
 #pragma unroll
       for (int i = 0; i < TW; ++i)
 #pragma unroll
-        for (int k = 0; k < TW; ++k)
+        for (int k = 0; k < TN; ++k)
           acc[i][k] = ks == 0 ? mfma_mx4<0, 0>(fb[k], sb[k], fa[i], sa[i], acc[i][k])
                               : mfma_mx4<1, 1>(fb[k], sb[k], fa[i], sa[i], acc[i][k]);
     }
@@ -165,8 +187,8 @@ __global__ __launch_bounds__(256, BT == 64 ? 2 : 1) void k_mx4_tile(Mx4Args g, i
 #pragma unroll
   for (int i = 0; i < TW; ++i)
 #pragma unroll
-    for (int k = 0; k < TW; ++k) {
-      const int m = m0 + wm * (BT / 2) + i * 16 + i16, n = n0 + wn * (BT / 2) + k * 16 + 4 * q;
+    for (int k = 0; k < TN; ++k) {
+      const int m = m0 + wm * (BT / 2) + i * 16 + i16, n = n0 + (wn * TN + k) * 16 + 4 * q;
       if (g.split > 1)
         store4<float>(g.part + static_cast<int64_t>(slice) * g.M * g.N, g.N, m, n, g.M, g.N, acc[i][k], nullptr, (g.N & 3) == 0);
       else
@@ -174,17 +196,23 @@ __global__ __launch_bounds__(256, BT == 64 ? 2 : 1) void k_mx4_tile(Mx4Args g, i
     }
 }
 
-// The slices' partial products summed in their order, and the bias.
-template <typename T>
+// The slices' partial products summed in their order, and the bias: V elements a
+// thread, of one row.
+template <typename T, int V>
 __global__ __launch_bounds__(256) void k_mx4_reduce(Mx4Args g) {
-  const int64_t i = block_id() * 256 + threadIdx.x;
   const int64_t mn = static_cast<int64_t>(g.M) * g.N;
+  const int64_t i = (block_id() * 256 + threadIdx.x) * V;
   if (i >= mn) return;
-  float v = 0.f;
-  for (int s = 0; s < g.split; ++s) v += g.part[s * mn + i];
+  typedef float vec __attribute__((ext_vector_type(V)));
+  typedef T out __attribute__((ext_vector_type(V)));
+  vec v = 0.f;
+  for (int s = 0; s < g.split; ++s) v += *reinterpret_cast<const vec*>(g.part + s * mn + i);
   const int64_t m = i / g.N, n = i - m * g.N;
-  if (g.bias != nullptr) v += static_cast<float>(static_cast<const T*>(g.bias)[n]);
-  static_cast<T*>(g.d)[m * g.ldd + n] = static_cast<T>(v);
+  out o;
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    o[e] = static_cast<T>(g.bias == nullptr ? v[e] : v[e] + static_cast<float>(static_cast<const T*>(g.bias)[n + e]));
+  *reinterpret_cast<out*>(static_cast<T*>(g.d) + m * g.ldd + n) = o;
 }
 
 constexpr int64_t kMaxSize = int64_t(1) << 30;   // bytes of a tile's rows, or of a row
@@ -195,24 +223,42 @@ bool scales_fit(int64_t kb, const void* s, int64_t ld) {
   return kb % 8 == 0 && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(s) & 3u) == 0;
 }
 
-// 256 x 256 tiles for about a round of the GPU or more.
-bool large_suits(int64_t M, int64_t N) { return ceil_div(M, 256) * ceil_div(N, 256) >= cu_count_cached() / 2; }
+// 256 x 256 tiles where 128 x 128 ones are more than a round of the GPU: (1024, 4352,
+// 8192) bf16 52.1 us, on 128 x 128 tiles 57.6; (384, 14336, 4096) 33.1 and 37.4; (2048,
+// 4096, 4096) 31.4 and 35.0; but (1024, 4096, 14336), one round, 83.0 and 60.6.  Up to
+// 128 rows they are half empty: (128, 100000, 4096) 80.4 and 78.4, (64, 100000, 4096)
+// 76.9 and, on 64 x 64, 61.7.
+bool large_suits(int64_t M, int64_t N) { return M > 128 && ceil_div(M, 128) * ceil_div(N, 128) > cu_count_cached(); }
 
-// The tile's size: 128 from a tile per CU on ((1024, 4096, 4096) bf16 25.2 us, on 64
-// x 64 tiles 30.9; (512, 4096, 4096), 128 large tiles, 23.6 and 17.8).  Slices of K:
-// as many as bring the blocks near the number of CUs (twice as many: (256, 4096,
-// 4096) 11.2 -> 16.1), none under eight K tiles, whose time a reduction's launch
-// takes ((500, 1001, 2080) in slices of four 12.3 us, whole 9.1; (64, 4096, 14336) in
-// slices of eight or more 17.6, of sixteen or more 19.1).
+// The tile's size and the slices of K: as many slices as bring the blocks near the
+// number of CUs (twice as many: (256, 4096, 4096) 11.2 -> 16.1 us), none under eight
+// K tiles of 64 x 64 or fourteen of 128 x 128, whose time a reduction's launch takes
+// ((500, 1001, 2080) in slices of four 12.3 us, whole 9.1; (64, 4096, 14336) in slices
+// of eight or more 17.6, of sixteen or more 19.1; (512, 4096, 4096) on 128 x 128 in
+// slices of eight 25.1, whole 18.5).  128 x 128 where they, sliced so, fill three
+// quarters of the CUs: with and without, (768, 4096, 4096) 19.3 and 22.5, (192, 14336,
+// 4096) 20.8 and 25.5, (256, 4096, 14336) in four slices 26.6 and 29.0; short of that,
+// (512, 4096, 4096) 18.5 and 14.7, (128, 4096, 14336) 23.8 and 20.2.
 void plan(int64_t M, int64_t N, int64_t kb, int& bt, int& split, int& kchunk) {
   const int64_t cus = cu_count_cached();
   const auto tiles = [&](int64_t t) { return ceil_div(M, t) * ceil_div(N, t); };
-  bt = tiles(128) >= cus ? 128 : 64;
   const int64_t kt = ceil_div(kb, 8);
-  int64_t s = std::max<int64_t>(1, std::min<int64_t>({cus / tiles(bt), kt / 8, 16}));
+  const auto slices = [&](int64_t t, int64_t least) { return std::max<int64_t>(1, std::min<int64_t>({cus / tiles(t), kt / least, 16})); };
+  int64_t s = slices(128, 14);
+  bt = M > 64 && 4 * tiles(128) * s >= 3 * cus ? 128 : 64;
+  if (bt == 64) s = slices(64, 8);
   const int64_t per = ceil_div(kt, s);
   kchunk = static_cast<int>(per * 8);
   split = static_cast<int>(ceil_div(kt, per));
+}
+
+template <typename T>
+void launch_reduce(const Mx4Args& g, bool fours, hipStream_t st) {
+  const int64_t mn = static_cast<int64_t>(g.M) * g.N;
+  if (fours)
+    hipLaunchKernelGGL((k_mx4_reduce<T, 4>), blocks_2d(ceil_div(mn, 1024)), dim3(256), 0, st, g);
+  else
+    hipLaunchKernelGGL((k_mx4_reduce<T, 1>), blocks_2d(ceil_div(mn, 256)), dim3(256), 0, st, g);
 }
 
 template <typename T, int BT, bool FIT>
@@ -224,10 +270,10 @@ int launch_tile(const Mx4Args& g, hipStream_t st) {
   const int tm = static_cast<int>(ceil_div(g.M, BT)), tn = static_cast<int>(ceil_div(g.N, BT));
   const int whole = (g.ldd & 3) == 0 && (reinterpret_cast<uintptr_t>(g.d) & (4 * sizeof(T) - 1)) == 0;
   note_kernel("mxfp4_tile%d split%d%s", BT, g.split, FIT ? "" : " bytes");
-  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(tm * tn), static_cast<unsigned>(g.split)), dim3(256), kLds, st, g,
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(tm * tn), static_cast<unsigned>(g.split)), dim3(64 * TileShape<BT, FIT>::kWaves), kLds, st, g,
                      tm, tn, whole);
   if (g.split > 1)
-    hipLaunchKernelGGL((k_mx4_reduce<T>), blocks_2d(ceil_div(static_cast<int64_t>(g.M) * g.N, 256)), dim3(256), 0, st, g);
+    launch_reduce<T>(g, whole && g.N % 4 == 0, st);
   return check_launch("mxfp4_mm");
 }
 

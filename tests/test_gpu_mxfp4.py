@@ -155,6 +155,23 @@ def test_product(m, n, k, dtype):
     check_product(*operands(m, n, k), bias, dtype)
 
 
+# Each tile in a round and in more, whole and in slices of K, scales in dwords and not.
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize(
+    "m,n,k,kernel",
+    [(130, 6100, 7424, "tile128 split2"), (130, 6100, 7200, "tile128 split2"), (200, 12300, 1056, "tile128 split1"), (300, 8300, 768, "tile128 split1"),
+     (40, 33000, 544, "tile64 split1"), (64, 300, 4096, "tile64 split2"), (70, 302, 4128, "tile64 split2"), (120, 40000, 256, "tile128 split1")],
+)
+def test_product_tiles(m, n, k, kernel, dtype):
+    bias = torch.randn(n).to(dtype).cuda() if m % 3 else None
+    args = operands(m, n, k)
+    out = check_product(*args, bias, dtype)
+    if torch.cuda.get_device_properties(0).multi_processor_count == 256:
+        assert kernel in _lib.last_kernel(), _lib.last_kernel()
+    for _ in range(3):
+        assert torch.equal(nt.mxfp4_mm(*args, bias, dtype=dtype), out)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("m,n,k", [(2048, 4096, 1280), (2000, 4090, 1792), (1900, 4099, 2048), (2300, 7700, 1536), (8200, 4100, 1312), (2100, 4200, 1100), (2050, 4097, 1024)])
 def test_product_large(m, n, k, dtype):
