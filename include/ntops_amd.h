@@ -405,7 +405,7 @@ NTOPS_API int64_t ntops_mxfp4_linear_workspace(int x_dtype, int64_t M, int64_t N
 /* No ntops counterparts (its KV cache, kernels/scaled_dot_product_attention.py:
  * 139-140, is of the query's type).  key_cache and value_cache (B, H, C, D)
  * hold e4m3 values in units of an fp32 scale for each block of `block` (a power
- * of two >= 16) consecutive tokens of a head: key_scale and value_scale (B, H,
+ * of two, 16 to 2^24) consecutive tokens of a head: key_scale and value_scale (B, H,
  * ceil(C / block)).  Strides in elements: 4 of a cache, 3 of its scales; the
  * last dims have unit strides.
  *
@@ -418,7 +418,8 @@ NTOPS_API int64_t ntops_mxfp4_linear_workspace(int x_dtype, int64_t M, int64_t N
  * new tokens start inside a block, the larger of its scale and theirs is kept,
  * and the block's earlier tokens are rounded again if that raises it.  What the
  * cache holds behind the new tokens stays as it is (and means nothing in the
- * rest of their last block).  Indices are I32 or I64. */
+ * rest of their last block).  Indices are I32 or I64.  Keys and values share
+ * neither cache nor scales. */
 NTOPS_API int ntops_store_kv_cache(int dtype, int64_t B, int64_t H, int64_t S, int64_t D, int64_t C, int64_t block,
                const void* key, const int64_t* key_strides,
                const void* value, const int64_t* value_strides,

@@ -112,7 +112,7 @@ extern "C" int ntops_kv_cache_attention(int dtype, int64_t B, int64_t Hq, int64_
   if (dtype != NTOPS_F32 && dtype != NTOPS_F16 && dtype != NTOPS_BF16)
     return set_error(NTOPS_ERR_UNSUPPORTED, "kv_cache_attention: unsupported dtype %d (F32/F16/BF16 only)", dtype);
   if (!block_ok(block))
-    return set_error(NTOPS_ERR_INVALID, "kv_cache_attention: a block is a power of two of at least 16 tokens");
+    return set_error(NTOPS_ERR_INVALID, "kv_cache_attention: a block is a power of two of 16 to 2^24 tokens");
   if (lengths && !index_dtype(lengths_dtype))
     return set_error(NTOPS_ERR_INVALID, "kv_cache_attention: lengths are I32 or I64");
   if (causal != 0 && causal != 1) return set_error(NTOPS_ERR_INVALID, "kv_cache_attention: causal is 0 or 1");

@@ -671,6 +671,13 @@ struct Cache {
   }
 };
 
+// A block size given as an int; -1, which no cache has, if it is past 64 bits.
+int64_t block_of(PyObject* o) {
+  const int64_t block = PyLong_AsLongLong(o);
+  if (block == -1 && PyErr_Occurred()) PyErr_Clear();
+  return block;
+}
+
 // An index vector (batch,) or None; false: the Python path.
 bool index_vector(PyObject* o, int64_t batch, int64_t dev, const at::Tensor*& t, int& code) {
   t = nullptr;
@@ -689,7 +696,7 @@ PyObject* store_kv_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int64_t dev;
   void* st;
   if (n != 9 || !usable() || !PyLong_CheckExact(a[8]) || !current(dev, st)) return none();
-  const int64_t block = PyLong_AsLongLong(a[8]);
+  const int64_t block = block_of(a[8]);
   Cache c;
   const at::Tensor *k = plain(a[0]), *v = plain(a[1]), *pos = nullptr, *len = nullptr;
   if (!k || !v || !c.read(a + 2, block, dev) || k->dim() != 4 || v->sizes() != k->sizes() || code16_32(*k) < 0 ||
@@ -729,7 +736,7 @@ PyObject* kv_cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int64_t dev;
   void* st;
   if (n != 9 || !usable() || !PyBool_Check(a[6]) || !PyLong_CheckExact(a[8]) || !current(dev, st)) return none();
-  const int64_t block = PyLong_AsLongLong(a[8]);
+  const int64_t block = block_of(a[8]);
   Cache c;
   const at::Tensor *q = plain(a[0]), *len = nullptr;
   int lcode;

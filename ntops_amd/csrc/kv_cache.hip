@@ -293,7 +293,7 @@ extern "C" int ntops_store_kv_cache(int dtype, int64_t B, int64_t H, int64_t S, 
                                     const int64_t* value_scale_strides, const void* positions, int positions_dtype,
                                     int64_t position, const void* lengths, int lengths_dtype, void* stream) {
   if (B < 0 || H < 0 || S < 0 || D < 0 || C < 0) return set_error(NTOPS_ERR_INVALID, "store_kv_cache: negative size");
-  if (!block_ok(block)) return set_error(NTOPS_ERR_INVALID, "store_kv_cache: a block is a power of two of at least 16 tokens");
+  if (!block_ok(block)) return set_error(NTOPS_ERR_INVALID, "store_kv_cache: a block is a power of two of 16 to 2^24 tokens");
   if ((positions && !index_dtype(positions_dtype)) || (lengths && !index_dtype(lengths_dtype)))
     return set_error(NTOPS_ERR_INVALID, "store_kv_cache: positions and lengths are I32 or I64");
   return dispatch_float16_32(dtype, "store_kv_cache", [&](auto tag) -> int {
@@ -302,6 +302,8 @@ extern "C" int ntops_store_kv_cache(int dtype, int64_t B, int64_t H, int64_t S, 
     if (!key || !value || !key_cache || !value_cache || !key_scale || !value_scale || !key_strides || !value_strides ||
         !key_cache_strides || !value_cache_strides || !key_scale_strides || !value_scale_strides)
       return set_error(NTOPS_ERR_INVALID, "store_kv_cache: null pointer");
+    if (key_cache == value_cache || key_scale == value_scale)
+      return set_error(NTOPS_ERR_INVALID, "store_kv_cache: keys and values share their cache or its scales");
     if (D > 65536 || (D * std::min(block, S) > (int64_t(1) << 30)))
       return set_error(NTOPS_ERR_UNSUPPORTED, "store_kv_cache: blocks too large");
     StoreArgs a{};

@@ -7,7 +7,7 @@ is of the query's type.  The cache of a layer is four tensors of the caller's:
   key_scale, value_scale   float32 (batch, heads, ceil(capacity / block_size))
 
 A token's values are its codes times the scale of its block of `block_size` (a
-power of two of at least 16) tokens.  key and value (batch, heads, tokens,
+power of two of 16 to 2^24) tokens.  key and value (batch, heads, tokens,
 head_dim; float32, float16 or bfloat16) go to `positions` and on: an int, or an
 int32 / int64 tensor (batch,).  With `lengths` (batch,) only each sequence's
 first lengths[b] tokens are stored.  Tokens outside of the cache are dropped.
@@ -19,6 +19,8 @@ raises it, the block's earlier tokens are rounded again.  What the cache holds
 behind the new tokens stays as it is, and means nothing in the rest of their last
 block: a sequence grows at its end, or is cut and grows from there."""
 
+import operator
+
 import torch
 
 from ntops_amd import _lib
@@ -27,8 +29,8 @@ from ntops_amd.torch.utils import _DeviceGuard, _contiguous, _strides
 
 def _checked_cache(key_cache, value_cache, key_scale, value_scale, block_size, what):
     """The cache's shape (batch, heads, capacity, head_dim)."""
-    if block_size < 16 or block_size & (block_size - 1):
-        raise RuntimeError(f"{what}: block_size must be a power of two of at least 16, got {block_size}")
+    if not 16 <= block_size <= 1 << 24 or block_size & (block_size - 1):
+        raise RuntimeError(f"{what}: block_size must be a power of two of 16 to 2^24, got {block_size}")
     if key_cache.dim() != 4 or key_cache.shape != value_cache.shape:
         raise RuntimeError(f"{what}: expected two 4-D caches of one shape, got {tuple(key_cache.shape)} and {tuple(value_cache.shape)}")
     if key_cache.dtype != torch.float8_e4m3fn or value_cache.dtype != torch.float8_e4m3fn:
@@ -64,7 +66,7 @@ def store_kv_cache(key, value, key_cache, value_cache, key_scale, value_scale, p
         _check_index(positions, b, "positions", what)
         tensors.append(positions)
     else:
-        at, positions = int(positions), None
+        at, positions = max(-(1 << 62), min(1 << 62, operator.index(positions))), None
     if lengths is not None:
         _check_index(lengths, b, "lengths", what)
     for t in (key_cache, value_cache, key_scale, value_scale):

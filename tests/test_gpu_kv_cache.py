@@ -77,6 +77,28 @@ def test_store(b, h, s, d, c, block, dtype):
     check_store(key, value, caches, positions.long(), None, block)
 
 
+def test_numbers_past_64_bits_and_shared_caches():
+    b, h, c, d = 2, 2, 50, 64
+    caches = caches_of(b, h, c, d, 16)
+    x = tokens(b, h, 3, d).cuda()
+    before = [t.clone() for t in caches]
+    for position in (1 << 70, -(1 << 70), c, -3):
+        nt.store_kv_cache(x, x, *caches, position, block_size=16)
+        assert all(torch.equal(s.view(torch.uint8), t.view(torch.uint8)) for s, t in zip(before, caches))
+    for block in (1 << 70, 1 << 64, -(1 << 70), 1 << 25):
+        with pytest.raises(RuntimeError, match="power of two"):
+            nt.store_kv_cache(x, x, *caches, 0, block_size=block)
+        with pytest.raises(RuntimeError, match="power of two"):
+            nt.kv_cache_attention(x, *caches, block_size=block)
+    with pytest.raises(TypeError):
+        nt.store_kv_cache(x, x, *caches, 1.5, block_size=16)
+    kc, vc, ks, vs = caches
+    for shared in ((kc, kc, ks, vs), (kc, vc, ks, ks)):
+        with pytest.raises(RuntimeError, match="share"):
+            nt.store_kv_cache(x, x, *shared, 0, block_size=16)
+    nt.kv_cache_attention(x, kc, kc, ks, ks, block_size=16)  # read only
+
+
 @pytest.mark.parametrize("first", [2.0**-20, 1.0, 2.0**12])
 def test_store_token_by_token(first):
     b, h, c, d, block = 2, 2, 50, 64, 16

@@ -280,7 +280,10 @@ def test_product_empty():
     e = lambda *s: torch.empty(s, dtype=torch.uint8, device="cuda")
     assert nt.mxfp4_mm(e(0, 64), e(0, 4), e(5, 64), e(5, 4)).shape == (0, 5)
     assert nt.mxfp4_mm(e(3, 64), e(3, 4), e(0, 64), e(0, 4)).shape == (3, 0)
+    f = lambda *s: torch.empty(s, device="cuda").bfloat16()
+    assert nt.mxfp4_mm(f(0, 64), None, e(5, 32), e(5, 2)).shape == (0, 5) and nt.mxfp4_mm(f(3, 64), None, e(0, 32), e(0, 2)).shape == (3, 0)
     bias = torch.randn(5, device="cuda").bfloat16()
+    assert torch.equal(nt.mxfp4_mm(f(3, 0), None, e(5, 0), e(5, 0), bias), bias.expand(3, 5))
     assert torch.equal(nt.mxfp4_mm(e(3, 0), e(3, 0), e(5, 0), e(5, 0), bias), bias.expand(3, 5))
 
 

@@ -138,3 +138,15 @@ def test_c_entry_points_refuse():
     assert attend(causal=2) == 1
     assert attend(d=257) == 2 and "head dim" in err()
     assert attend(b=0, q=None) == 0 and attend(sq=0, q=None) == 0
+
+
+def test_store_refuses_one_cache_for_both():
+    lib = _lib.load()
+    arr = lambda *v: (ctypes.c_int64 * len(v))(*v)
+    s4, s3 = arr(2048, 1024, 16, 1), arr(8, 4, 1)
+
+    def go(vc=2048, vs=8192):
+        return lib.ntops_store_kv_cache(_lib.BF16, 2, 2, 1, 16, 64, 16, P(256), s4, P(512), s4, P(1024), s4, P(vc), s4, P(4096), s3, P(vs), s3, None, 0, 0, None, 0, None)
+
+    for same in (dict(vc=1024), dict(vs=4096)):
+        assert go(**same) == 1 and "share" in lib.ntops_last_error().decode()
