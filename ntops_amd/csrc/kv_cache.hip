@@ -10,8 +10,13 @@
 //
 // Bound by memory (es read, 1 byte written per value), or for single tokens by
 // latency: a wave owns the block of a head -- its new values stay in registers
-// between the maximum and the rounding, nothing is shared, no barrier.  Blocks
-// of more than kSlots * 64 * 8 values are read twice.
+// between the maximum and the rounding, nothing is shared, no barrier: (32, 8, 1,
+// 128) bf16 3.9 us, (4, 8, 2048, 128) 11.4 us and (1, 8, 16384, 128) 23.0 us (4.4
+// TB/s) in blocks of 64.  Blocks of more values than a wave's lanes keep are shared
+// by eight waves (in blocks of 512 (4, 8, 2048, 128) took one wave 66.4 us, eight
+// 12.4; of 4096 tokens 420 and 51.8), and so are those of head dims that are no
+// multiple of 8, which go value by value ((4, 8, 2041, 100) 43.6 us and 30.0); past
+// what eight waves keep, the values are read twice.
 #include <algorithm>
 
 #include "kv_cache.h"
@@ -34,6 +39,7 @@ struct StoreArgs {
 };
 
 constexpr int kSlots = 16;  // packs of 8 values a lane keeps
+constexpr int kWide = 8;    // waves that share a block of more values than a wave's lanes keep
 
 __device__ __forceinline__ float least_scale(uint32_t top) {
   const int e = static_cast<int>(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
@@ -51,14 +57,15 @@ struct Divide {
   __device__ __forceinline__ float operator()(float x) const { return pow2 ? x * inv : x / s; }
 };
 
-// What a wave's lanes do next: slot l, l + 64, .. of rows of `per` slots.
+// What the lanes of W waves do next: slot l, l + 64 W, .. of rows of `per` slots.
+template <int W>
 struct Walk {
   int row, col, per, drow, dcol;
   __device__ __forceinline__ Walk(int first, int per_row) : per(per_row) {
     row = first / per;
     col = first - row * per;
-    drow = 64 / per;
-    dcol = 64 - drow * per;
+    drow = 64 * W / per;
+    dcol = 64 * W - drow * per;
   }
   __device__ __forceinline__ void next() {
     row += drow;
@@ -70,20 +77,24 @@ struct Walk {
   }
 };
 
-// Where a wave's tokens lie.
+// Where a block's tokens lie.  W 1: keys in one wave, values in another; else the
+// W waves take the values of a block of tokens together.
+template <int W>
 struct Unit {
-  int which;
+  int which, lane;
   int64_t b, h, j;         // sequence, head, block
   int64_t start, p0, p1;   // position of the sequence's first token; positions of the block's new tokens
   int64_t first;           // of the block
   __device__ __forceinline__ bool find(const StoreArgs& a) {
-    which = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    which = W == 1 ? wave : blockIdx.x & 1;
+    lane = W == 1 ? threadIdx.x & 63 : threadIdx.x;
     h = blockIdx.y;
     b = blockIdx.z;
     start = max(-a.S, min(a.C, index_at(a.positions, a.positions_dtype, b, a.position)));
     const int64_t count = max(int64_t(0), min(a.S, index_at(a.lengths, a.lengths_dtype, b, a.S)));
     const int64_t lo = max(int64_t(0), start), hi = min(a.C, start + count);
-    j = (lo >> a.shift) + blockIdx.x;
+    j = (lo >> a.shift) + (W == 1 ? blockIdx.x : blockIdx.x >> 1);
     first = j << a.shift;
     p0 = max(lo, first);
     p1 = min(hi, first + (int64_t(1) << a.shift));
@@ -94,6 +105,21 @@ struct Unit {
 __device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
   // (bits of a non-negative float: the float's order)
   return __builtin_bit_cast(uint32_t, wave_max(__builtin_bit_cast(float, v)));
+}
+
+// The largest of all the lanes of a block of tokens (and what each has read of the
+// cache before, it has).
+template <int W>
+__device__ __forceinline__ uint32_t group_max_bits(uint32_t v) {
+  v = wave_max_bits(v);
+  if constexpr (W > 1) {
+    __shared__ uint32_t most[W];
+    __syncthreads();  // (an earlier call's reads are over)
+    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = v;
+    __syncthreads();
+    for (int w = 0; w < W; ++w) v = max(v, most[w]);
+  }
+  return v;
 }
 
 __device__ __forceinline__ void grow(uint32_t& top, float v) {
@@ -149,12 +175,13 @@ __device__ __forceinline__ u32x2 scaled_e4m3(const Pack16<T> (&v)[sizeof(T) / 2]
 // 8 values at a time: head dim a multiple of 8, aligned rows, a block's rows within
 // 31-bit byte offsets.  Buffer loads and stores, which end at the block's last
 // value, so that no branch stands between a lane's loads.
-template <typename T>
-__global__ __launch_bounds__(128) void k_store_kv_cache(StoreArgs a) {
+template <typename T, int W>
+__global__ __launch_bounds__(W == 1 ? 128 : 64 * W) void k_store_kv_cache(StoreArgs a) {
   constexpr int ES = sizeof(T);
-  const int lane = threadIdx.x & 63;
-  Unit u;
+  using Walk = Walk<W>;
+  Unit<W> u;
   if (!u.find(a)) return;
+  const int lane = u.lane;
   const int per = a.D / 8;
   const int rows = static_cast<int>(u.p1 - u.p0), slots = rows * per;
   const T* x = static_cast<const T*>(a.x[u.which]) + u.b * a.xs[u.which][0] + u.h * a.xs[u.which][1] +
@@ -177,7 +204,7 @@ __global__ __launch_bounds__(128) void k_store_kv_cache(StoreArgs a) {
     Walk w(lane, per);
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
-      load(w, i * 64 + lane < slots, v[i]);
+      load(w, i * (64 * W) + lane < slots, v[i]);
       w.next();
     }
   }
@@ -190,12 +217,12 @@ __global__ __launch_bounds__(128) void k_store_kv_cache(StoreArgs a) {
   std::conditional_t<ES == 2, u16x2, uint32_t> most{};
 #pragma unroll
   for (int i = 0; i < kSlots; ++i) words(v[i], most);  // (slots past the end read as zero)
-  for (Walk w(lane + kSlots * 64, per); w.row < rows; w.next()) {
+  for (Walk w(lane + kSlots * 64 * W, per); w.row < rows; w.next()) {
     Pack16<T> y[ES / 2];
     load(w, true, y);
     words(y, most);
   }
-  uint32_t top = wave_max_bits(top_bits<T>(most));
+  uint32_t top = group_max_bits<W>(top_bits<T>(most));
   const bool finite = top < 0x7f800000u;
   if (!finite) {  // once more, over the finite values
     top = 0;
@@ -205,7 +232,7 @@ __global__ __launch_bounds__(128) void k_store_kv_cache(StoreArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) grow(top, value(y, e));
     }
-    top = wave_max_bits(top);
+    top = group_max_bits<W>(top);
   }
   const float fits = least_scale(top);
   const bool keeps = old > fits;
@@ -215,8 +242,8 @@ __global__ __launch_bounds__(128) void k_store_kv_cache(StoreArgs a) {
     Walk w(lane, per);
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
-      if (i * 64 < slots)
-        __builtin_amdgcn_raw_buffer_store_b64(scaled_e4m3<T>(v[i], scale), rc, i * 64 + lane < slots ? w.row * cld + w.col * 8 : kOOB, 0, 0);
+      if (i * (64 * W) < slots)
+        __builtin_amdgcn_raw_buffer_store_b64(scaled_e4m3<T>(v[i], scale), rc, i * (64 * W) + lane < slots ? w.row * cld + w.col * 8 : kOOB, 0, 0);
       w.next();
     }
     for (; w.row < rows; w.next()) {
@@ -251,11 +278,12 @@ __global__ __launch_bounds__(128) void k_store_kv_cache(StoreArgs a) {
 }
 
 // One value at a time, for any head dim and alignment.
-template <typename T>
-__global__ __launch_bounds__(128) void k_store_kv_cache_any(StoreArgs a) {
-  const int lane = threadIdx.x & 63;
-  Unit u;
+template <typename T, int W>
+__global__ __launch_bounds__(W == 1 ? 128 : 64 * W) void k_store_kv_cache_any(StoreArgs a) {
+  using Walk = Walk<W>;
+  Unit<W> u;
   if (!u.find(a)) return;
+  const int lane = u.lane;
   const int rows = static_cast<int>(u.p1 - u.p0);
   const int64_t xld = a.xs[u.which][2], cld = a.cs[u.which][2];
   const T* x = static_cast<const T*>(a.x[u.which]) + u.b * a.xs[u.which][0] + u.h * a.xs[u.which][1] + (u.p0 - u.start) * xld;
@@ -265,7 +293,7 @@ __global__ __launch_bounds__(128) void k_store_kv_cache_any(StoreArgs a) {
   const float old = u.p0 > u.first ? *sp : 0.f;
   uint32_t top = 0;
   for (Walk w(lane, a.D); w.row < rows; w.next()) grow(top, static_cast<float>(x[w.row * xld + w.col]));
-  const float fits = least_scale(wave_max_bits(top));
+  const float fits = least_scale(group_max_bits<W>(top));
   const bool keeps = old > fits;
   const float scale = keeps ? old : fits;
   const Divide by(scale);
@@ -346,9 +374,12 @@ extern "C" int ntops_store_kv_cache(int dtype, int64_t B, int64_t H, int64_t S, 
     a.units = std::min(ceil_div(S - 1, block) + 1, ceil_div(C, block));
     if (B > 65535 || H > 65535 || a.units > (1 << 24))
       return set_error(NTOPS_ERR_UNSUPPORTED, "store_kv_cache: over 65535 sequences or heads, or too many tokens");
-    const dim3 grid(static_cast<unsigned>(a.units), static_cast<unsigned>(H), static_cast<unsigned>(B));
-    const auto kern = vec ? &k_store_kv_cache<T> : &k_store_kv_cache_any<T>;
-    hipLaunchKernelGGL(kern, grid, dim3(128), 0, static_cast<hipStream_t>(stream), a);
+    // a lane's registers hold kSlots packs; of single values a wave takes a few turns
+    const bool wide = std::min(block, S) * D > (vec ? kSlots * 64 * 8 : 8 * 64);
+    const dim3 grid(static_cast<unsigned>(a.units * (wide ? 2 : 1)), static_cast<unsigned>(H), static_cast<unsigned>(B));
+    const auto kern = vec ? (wide ? &k_store_kv_cache<T, kWide> : &k_store_kv_cache<T, 1>)
+                          : (wide ? &k_store_kv_cache_any<T, kWide> : &k_store_kv_cache_any<T, 1>);
+    hipLaunchKernelGGL(kern, grid, dim3(wide ? 64 * kWide : 128), 0, static_cast<hipStream_t>(stream), a);
     return check_launch("store_kv_cache");
   });
 }

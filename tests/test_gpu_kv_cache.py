@@ -108,6 +108,23 @@ def test_store_token_by_token(first):
         check_store((tokens(b, h, 1, d) * size).cuda(), tokens(b, h, 1, d).cuda(), caches, torch.tensor([t, t + 7]).cuda(), None, block)
 
 
+# Blocks of more values than a wave takes: several waves share one, within what
+# their registers hold and past it; the parts of a block arrive one after the other.
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,h,c,d,block", [(2, 2, 1300, 128, 1024), (1, 3, 400, 100, 64), (1, 1, 5000, 64, 4096), (1, 2, 300, 200, 128), (1, 1, 40, 257, 16)])
+def test_store_large_blocks_in_parts(b, h, c, d, block, dtype):
+    caches = caches_of(b, h, c, d, block)
+    at = 0
+    for i, s in enumerate((c // 2, 1, 37 % c, c // 3)):
+        s = min(s, c - at)
+        key, value = (tokens(b, h, s, d, dtype=dtype) * 2.0 ** (3 * (i % 3) - 3) for _ in range(2))
+        if i == 2:
+            key[0, 0, 0, 0], value[0, h - 1, s - 1, d - 1], value[0, 0, s // 2, 3] = float("inf"), float("nan"), float("-inf")
+        check_store(key.cuda(), value.cuda(), caches, at, None, block)
+        at += s
+    check_store(key.cuda(), value.cuda(), caches, torch.tensor([c // 4] * b).cuda(), torch.arange(1, b + 1).cuda(), block)
+
+
 def test_store_drops_what_lies_outside():
     b, h, c, d, block = 6, 2, 40, 16, 16
     caches = caches_of(b, h, c, d, block)
