@@ -1,10 +1,11 @@
 // The MXFP4 product's tile kernel, its split over K, and the C entry points.
 //
-// BT x BT output tiles, four waves of 32 x 32 or eight of 64 x 32, two a SIMD either
-// way (a block of 64 x 64 shares its CU with another), so that one issues where the
+// BT x BT output tiles, four waves of 32 x 32 or eight of 64 x 32, two a SIMD at
+// least (a block of 64 x 64 shares its CU with another), so that one issues where the
 // other waits: (1024, 4096, 4096) bf16 with four waves of 64 x 64 23.8 us, with eight
 // 20.1.  K tiles of 256 values (128 bytes a row, whole lines) go through a ring of
-// four stages filled by direct DMA three tiles ahead; one barrier per K tile.  What
+// four stages filled by direct DMA three tiles ahead, or of two; one barrier per K
+// tile.  What
 // bounds it is the delivery of the tiles into the LDS, some 35 bytes a ns and CU.
 //
 // Scales come as dwords, those of two K tiles together: a row's 8 bytes a K tile are
@@ -23,9 +24,10 @@
 namespace ntops {
 namespace {
 
-constexpr int kStages = 4;
+// Blocks that share a CU.
+constexpr int tile_blocks(int bt, int stages) { return (bt == 64 ? 2 : 1) * 4 / stages; }
 
-template <int BT, bool FIT>
+template <int BT, bool FIT, int STAGES>
 struct TileShape {
   static constexpr int kWaves = BT == 128 ? 8 : 4;
   static constexpr int kWN = kWaves / 2;  // waves along a tile's columns
@@ -36,18 +38,18 @@ struct TileShape {
   static constexpr int kDwords = FIT ? 4 : 3;                  // of a row's scales in a group
   static constexpr int kScaleInst = (kRowsPerWave * kDwords + 63) / 64;
   static constexpr int kScales = kWaves * kScaleInst * 256;    // bytes of an operand's scales in a group
-  static constexpr int kScaleRing = 8;                         // groups
+  static constexpr int kScaleRing = STAGES == 2 ? 4 : 8;       // groups
   static constexpr int kScalesPerTile = 2 * kScaleInst / kGroup;
-  static constexpr int kScalesAt = kStages * kStage;
+  static constexpr int kScalesAt = STAGES * kStage;
   static constexpr int kLds = kScalesAt + kScaleRing * 2 * kScales;
   static constexpr int kLoads = 2 * kRowsPerWave / 8 + kScalesPerTile;  // DMA instructions per wave and K tile
-  static_assert(kRowsPerWave == 16 && kScalesPerTile * kGroup == 2 * kScaleInst && kLds * (BT == 64 ? 2 : 1) <= 163840, "tile");
+  static_assert(kRowsPerWave == 16 && kScalesPerTile * kGroup == 2 * kScaleInst && kLds * tile_blocks(BT, STAGES) <= 163840, "tile");
 };
 
 // whole: the output's rows are runs that 4 elements at a time can be stored to.
-template <typename T, int BT, bool FIT>
-__global__ __launch_bounds__(64 * (BT == 128 ? 8 : 4), BT == 64 ? 2 : 1) void k_mx4_tile(Mx4Args g, int tm_count, int tn_count, int whole) {
-  using S = TileShape<BT, FIT>;
+template <typename T, int BT, bool FIT, int STAGES>
+__global__ __launch_bounds__(64 * (BT == 128 ? 8 : 4), tile_blocks(BT, STAGES)) void k_mx4_tile(Mx4Args g, int tm_count, int tn_count, int whole) {
+  using S = TileShape<BT, FIT, STAGES>;
   constexpr int TW = BT / 32, TN = BT / S::kWN / 16;  // 16-row and 16-column pieces of a wave's tile
   constexpr int ND = S::kDwords;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -98,7 +100,7 @@ __global__ __launch_bounds__(64 * (BT == 128 ? 8 : 4), BT == 64 ? 2 : 1) void k_
   // this wave's loads of K tile j: 16 rows of A and of B, 8 an instruction, and its
   // part of the scales of the next group
   auto issue = [&](int j) {
-    const uint32_t st = smem_addr + static_cast<uint32_t>((j & (kStages - 1)) * S::kStage);
+    const uint32_t st = smem_addr + static_cast<uint32_t>((j & (STAGES - 1)) * S::kStage);
     const int b0 = kb0 + j * 8;
 #pragma unroll
     for (int u = 0; u < S::kRowsPerWave / 8; ++u) {
@@ -129,16 +131,15 @@ __global__ __launch_bounds__(64 * (BT == 128 ? 8 : 4), BT == 64 ? 2 : 1) void k_
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int u = 0; u < 2 * S::kScaleInst; ++u) issue_scales(0, u);
-  issue(0);
-  issue(1);
-  issue(2);
+#pragma unroll
+  for (int j = 0; j < STAGES - 1; ++j) issue(j);
   for (int j = 0; j < nt; ++j) {
     __builtin_amdgcn_sched_barrier(0);
-    wait_vmcnt<2 * S::kLoads>();  // K tile j is in (past the last tile the loads are empty, but count)
+    wait_vmcnt<(STAGES - 2) * S::kLoads>();  // K tile j is in (past the last tile the loads are empty, but count)
     block_barrier();              // for every wave; and tile j - 1's stage is free
     asm volatile("" ::: "memory");
-    issue(j + 3);
-    const char* st = smem + (j & (kStages - 1)) * S::kStage;
+    issue(j + STAGES - 1);
+    const char* st = smem + (j & (STAGES - 1)) * S::kStage;
     const char* sc = smem + S::kScalesAt + (j / S::kGroup & (S::kScaleRing - 1)) * (2 * S::kScales) + j % S::kGroup * 8;
     uint32_t sa[TW], sb[TN];
     // the scales of blocks q and q + 4 of each row, in bytes 0 and 1
@@ -223,12 +224,16 @@ bool scales_fit(int64_t kb, const void* s, int64_t ld) {
   return kb % 8 == 0 && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(s) & 3u) == 0;
 }
 
-// 256 x 256 tiles where 128 x 128 ones are more than a round of the GPU: (1024, 4352,
-// 8192) bf16 52.1 us, on 128 x 128 tiles 57.6; (384, 14336, 4096) 33.1 and 37.4; (2048,
-// 4096, 4096) 31.4 and 35.0; but (1024, 4096, 14336), one round, 83.0 and 60.6.  Up to
-// 128 rows they are half empty: (128, 100000, 4096) 80.4 and 78.4, (64, 100000, 4096)
-// 76.9 and, on 64 x 64, 61.7.
-bool large_suits(int64_t M, int64_t N) { return M > 128 && ceil_div(M, 128) * ceil_div(N, 128) > cu_count_cached(); }
+// 256 x 256 tiles where 128 x 128 ones, two a CU, are more than a round of the GPU:
+// (1500, 6000, 8192) bf16 58.5 us, on 128 x 128 tiles 74.8; (3000, 3000, 3000) 33.5 and
+// 38.9; but (2048, 4096, 4096), one round, 32.7 and 29.2, and (1100, 4000, 4096) 31.0
+// and 25.7.  Over a long K already where they are more than one a CU: (2048, 4096,
+// 14336) 86.2 and 93.0, (1024, 6144, 8192) 52.8 and 52.6; but (1024, 4096, 14336), one
+// a CU, 83.0 and 53.5.  Up to 128 rows they are half empty: (128, 100000, 4096) 80.4
+// and 78.4.
+bool large_suits(int64_t M, int64_t N, int64_t kb) {
+  return M > 128 && ceil_div(M, 128) * ceil_div(N, 128) > cu_count_cached() * (kb >= 256 ? 1 : 2);
+}
 
 // The tile's size and the slices of K: as many slices as bring the blocks near the
 // number of CUs (twice as many: (256, 4096, 4096) 11.2 -> 16.1 us), none under eight
@@ -261,27 +266,37 @@ void launch_reduce(const Mx4Args& g, bool fours, hipStream_t st) {
     hipLaunchKernelGGL((k_mx4_reduce<T, 1>), blocks_2d(ceil_div(mn, 256)), dim3(256), 0, st, g);
 }
 
-template <typename T, int BT, bool FIT>
+// Rings of two stages, and twice the blocks a CU: where there are more tiles than
+// one round of blocks with four ((8192, 8192, 512) 79.8 -> 62.6 us, (2048, 4096, 4096)
+// 35.6 -> 29.2; of 64 x 64 (8192, 14336, 100) 174 -> 97.8), and for up to four K tiles
+// ((1000, 1000, 200) 4.8 -> 4.4).  In one round four are needed ((1024, 4096, 14336)
+// 53.5, with two 68.3; (64, 14336, 4096) 13.8 and 17.1).
+bool two_stages(int64_t M, int64_t N, int64_t kchunk, int64_t split, int bt) {
+  return kchunk <= 32 || ceil_div(M, bt) * ceil_div(N, bt) * split > cu_count_cached() * tile_blocks(bt, 4);
+}
+
+template <typename T, int BT, bool FIT, int STAGES>
 int launch_tile(const Mx4Args& g, hipStream_t st) {
-  auto kern = k_mx4_tile<T, BT, FIT>;
-  constexpr int kLds = TileShape<BT, FIT>::kLds;
+  auto kern = k_mx4_tile<T, BT, FIT, STAGES>;
+  using S = TileShape<BT, FIT, STAGES>;
+  constexpr int kLds = S::kLds;
   static std::atomic<uint64_t> reserved{0};
   if (const int rc = reserve_lds(reinterpret_cast<const void*>(kern), kLds, reserved, "mxfp4_mm"); rc != NTOPS_OK) return rc;
   const int tm = static_cast<int>(ceil_div(g.M, BT)), tn = static_cast<int>(ceil_div(g.N, BT));
   const int whole = (g.ldd & 3) == 0 && (reinterpret_cast<uintptr_t>(g.d) & (4 * sizeof(T) - 1)) == 0;
-  note_kernel("mxfp4_tile%d split%d%s", BT, g.split, FIT ? "" : " bytes");
-  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(tm * tn), static_cast<unsigned>(g.split)), dim3(64 * TileShape<BT, FIT>::kWaves), kLds, st, g,
+  note_kernel("mxfp4_tile%d split%d stages%d%s", BT, g.split, STAGES, FIT ? "" : " bytes");
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(tm * tn), static_cast<unsigned>(g.split)), dim3(64 * S::kWaves), kLds, st, g,
                      tm, tn, whole);
   if (g.split > 1)
     launch_reduce<T>(g, whole && g.N % 4 == 0, st);
   return check_launch("mxfp4_mm");
 }
 
-template <typename T>
-int run_tile(const Mx4Args& g, int bt, hipStream_t st) {
+template <typename T, int BT>
+int run_tile(const Mx4Args& g, hipStream_t st) {
   const bool fit = scales_fit(g.kb, g.as, g.ldas) && scales_fit(g.kb, g.bs, g.ldbs);
-  if (bt == 128) return fit ? launch_tile<T, 128, true>(g, st) : launch_tile<T, 128, false>(g, st);
-  return fit ? launch_tile<T, 64, true>(g, st) : launch_tile<T, 64, false>(g, st);
+  if (two_stages(g.M, g.N, g.kchunk, g.split, BT)) return fit ? launch_tile<T, BT, true, 2>(g, st) : launch_tile<T, BT, false, 2>(g, st);
+  return fit ? launch_tile<T, BT, true, 4>(g, st) : launch_tile<T, BT, false, 4>(g, st);
 }
 
 }  // namespace
@@ -292,7 +307,7 @@ using namespace ntops;
 extern "C" int64_t ntops_mxfp4_mm_workspace(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0 || M > kMaxCount || N > kMaxCount || K > kMaxSize) return 0;
   if (M <= kSkinnyRows) return 0;
-  if (large_suits(M, N)) return mx4_large_workspace(M, N, ceil_div(K, 32));
+  if (large_suits(M, N, ceil_div(K, 32))) return mx4_large_workspace(M, N, ceil_div(K, 32));
   int bt, split, kchunk;
   plan(M, N, ceil_div(K, 32), bt, split, kchunk);
   return split > 1 ? split * M * N * 4 : 0;
@@ -360,7 +375,7 @@ extern "C" int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K, co
   return dispatch_float16_32(out_dtype, "mxfp4_mm", [&](auto tag) -> int {
     using T = decltype(tag);
     if (M <= kSkinnyRows && kb > 0) return mx4_skinny(out_dtype, g, st);
-    if (large_suits(M, N) && mx4_large_serves(out_dtype, g) && workspace != nullptr &&
+    if (large_suits(M, N, kb) && mx4_large_serves(out_dtype, g) && workspace != nullptr &&
         workspace_bytes >= mx4_large_workspace(M, N, kb))
       return mx4_large(out_dtype, g, workspace, st);
     int bt;
@@ -370,7 +385,7 @@ extern "C" int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K, co
       g.kchunk = (g.kb + 7) / 8 * 8;
     }
     g.part = static_cast<float*>(workspace);
-    return run_tile<T>(g, bt, st);
+    return bt == 128 ? run_tile<T, 128>(g, st) : run_tile<T, 64>(g, st);
   });
 }
 

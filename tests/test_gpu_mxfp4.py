@@ -159,8 +159,10 @@ def test_product(m, n, k, dtype):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize(
     "m,n,k,kernel",
-    [(130, 6100, 7424, "tile128 split2"), (130, 6100, 7200, "tile128 split2"), (200, 12300, 1056, "tile128 split1"), (300, 8300, 768, "tile128 split1"),
-     (40, 33000, 544, "tile64 split1"), (64, 300, 4096, "tile64 split2"), (70, 302, 4128, "tile64 split2"), (120, 40000, 256, "tile128 split1")],
+    [(130, 6100, 7424, "tile128 split2 stages4"), (130, 6100, 7200, "tile128 split2 stages4"), (200, 12300, 1056, "tile128 split1 stages4"),
+     (300, 8300, 768, "tile128 split1 stages2"), (300, 12000, 2048, "tile128 split1 stages2"), (300, 12001, 2080, "tile128 split1 stages2"),
+     (120, 40000, 256, "tile128 split1 stages2"), (64, 300, 4096, "tile64 split2 stages4"), (70, 302, 4128, "tile64 split2 stages4"),
+     (40, 33000, 544, "tile64 split1 stages2"), (50, 33000, 1536, "tile64 split1 stages2"), (50, 33000, 1600, "tile64 split1 stages2"), (300, 1000, 544, "tile64 split1 stages2")],
 )
 def test_product_tiles(m, n, k, kernel, dtype):
     bias = torch.randn(n).to(dtype).cuda() if m % 3 else None
@@ -173,12 +175,12 @@ def test_product_tiles(m, n, k, kernel, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("m,n,k", [(2048, 4096, 1280), (2000, 4090, 1792), (1900, 4099, 2048), (2300, 7700, 1536), (8200, 4100, 1312), (2100, 4200, 1100), (2050, 4097, 1024)])
+@pytest.mark.parametrize("m,n,k", [(2048, 4096, 1280), (2000, 4090, 1792), (1900, 4099, 2048), (2300, 7700, 1536), (8200, 4100, 1312), (2100, 4200, 1100), (2050, 4097, 1024), (2048, 8192, 1280), (2000, 8190, 1792), (1900, 8199, 2048), (1500, 2900, 8192)])
 def test_product_large(m, n, k, dtype):
     bias = torch.randn(n).to(dtype).cuda() if n % 4 else None
     args = operands(m, n, k)
     out = check_product(*args, bias, dtype)
-    if k > 1024:
+    if -(-m // 128) * -(-n // 128) > (256 if k >= 8192 else 512) and k > 1024:
         assert _lib.last_kernel() == "mxfp4_large"
     for _ in range(3):
         assert torch.equal(nt.mxfp4_mm(*args, bias, dtype=dtype), out)
