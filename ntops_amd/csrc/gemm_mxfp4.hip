@@ -276,15 +276,11 @@ bool scales_fit(int64_t kb, const void* s, int64_t ld) {
 }
 
 // 256 x 256 tiles where 128 x 128 ones, two a CU, are more than a round of the GPU:
-// (1500, 6000, 8192) bf16 58.5 us, on 128 x 128 tiles 74.8; (3000, 3000, 3000) 33.5 and
-// 38.9; but (2048, 4096, 4096), one round, 32.7 and 29.2, and (1100, 4000, 4096) 31.0
-// and 25.7.  Over a long K already where they are more than one a CU: (2048, 4096,
-// 14336) 86.2 and 93.0, (1024, 6144, 8192) 52.8 and 52.6; but (1024, 4096, 14336), one
-// a CU, 83.0 and 53.5.  Up to 128 rows they are half empty: (128, 100000, 4096) 80.4
-// and 78.4.
-bool large_suits(int64_t M, int64_t N, int64_t kb) {
-  return M > 128 && ceil_div(M, 128) * ceil_div(N, 128) > cu_count_cached() * (kb >= 256 ? 1 : 2);
-}
+// (1500, 6000, 8192) bf16 58.2 us, on 128 x 128 tiles 73.2; (3000, 3000, 3000) 32.5 and
+// 34.2; (4096, 8192, 1400) 43.4 and 47.1; but one round of those, (2048, 4096, 4096),
+// 33.0 and 27.7, (1024, 4352, 8192) 51.3 and 41.7, (2048, 4096, 14336) 84.8 and 88.4.
+// Up to 128 rows they are half empty: (128, 100000, 4096) 80.4 and 78.4.
+bool large_suits(int64_t M, int64_t N) { return M > 128 && ceil_div(M, 128) * ceil_div(N, 128) > 2 * cu_count_cached(); }
 
 // The tile's size and the slices of K: as many slices as bring the blocks near the
 // number of CUs (twice as many: (256, 4096, 4096) 11.2 -> 16.1 us), none under eight
@@ -358,7 +354,7 @@ using namespace ntops;
 extern "C" int64_t ntops_mxfp4_mm_workspace(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0 || M > kMaxCount || N > kMaxCount || K > kMaxSize) return 0;
   if (M <= kSkinnyRows) return 0;
-  if (large_suits(M, N, ceil_div(K, 32))) return mx4_large_workspace(M, N, ceil_div(K, 32));
+  if (large_suits(M, N)) return mx4_large_workspace(M, N, ceil_div(K, 32));
   int bt, split, kchunk;
   plan(M, N, ceil_div(K, 32), bt, split, kchunk);
   return split > 1 ? split * M * N * 4 : 0;
@@ -426,7 +422,7 @@ extern "C" int ntops_mxfp4_mm(int out_dtype, int64_t M, int64_t N, int64_t K, co
   return dispatch_float16_32(out_dtype, "mxfp4_mm", [&](auto tag) -> int {
     using T = decltype(tag);
     if (M <= kSkinnyRows && kb > 0) return mx4_skinny(out_dtype, g, st);
-    if (large_suits(M, N, kb) && mx4_large_serves(out_dtype, g) && workspace != nullptr &&
+    if (large_suits(M, N) && mx4_large_serves(out_dtype, g) && workspace != nullptr &&
         workspace_bytes >= mx4_large_workspace(M, N, kb))
       return mx4_large(out_dtype, g, workspace, st);
     int bt;

@@ -175,12 +175,12 @@ def test_product_tiles(m, n, k, kernel, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("m,n,k", [(2048, 4096, 1280), (2000, 4090, 1792), (1900, 4099, 2048), (2300, 7700, 1536), (8200, 4100, 1312), (2100, 4200, 1100), (2050, 4097, 1024), (2048, 8192, 1280), (2000, 8190, 1792), (1900, 8199, 2048), (1500, 2900, 8192)])
+@pytest.mark.parametrize("m,n,k", [(2048, 4096, 1280), (2000, 4090, 1792), (1900, 4099, 2048), (2300, 7700, 1536), (8200, 4100, 1312), (2100, 4200, 1100), (2050, 4097, 1024), (2048, 8192, 1280), (2000, 8190, 1792), (1900, 8199, 2048), (1500, 2900, 8192), (1500, 5700, 7680)])
 def test_product_large(m, n, k, dtype):
     bias = torch.randn(n).to(dtype).cuda() if n % 4 else None
     args = operands(m, n, k)
     out = check_product(*args, bias, dtype)
-    if -(-m // 128) * -(-n // 128) > (256 if k >= 8192 else 512) and k > 1024:
+    if -(-m // 128) * -(-n // 128) > 512 and k > 1024:
         assert _lib.last_kernel() == "mxfp4_large"
     for _ in range(3):
         assert torch.equal(nt.mxfp4_mm(*args, bias, dtype=dtype), out)
