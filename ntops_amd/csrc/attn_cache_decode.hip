@@ -97,14 +97,13 @@ struct TileDma {
       voff[i] = c * 16 < dt ? static_cast<uint32_t>(row * ld + c * 16) : kOOB;
     }
   }
-  // The tile at token t of the slice (byte offset off) to dst, its scales to
-  // sdst; valid false: loads that count but bring nothing.
-  __device__ __forceinline__ void issue(uint32_t dst, uint32_t sdst, uint32_t off, int t, bool valid) const {
+  // The tile at token t of the slice (byte offset off) to dst, its scales to sdst.
+  __device__ __forceinline__ void issue(uint32_t dst, uint32_t sdst, uint32_t off, int t) const {
 #pragma unroll
     for (int i = 0; i < kInst; ++i)
-      dma16_nt(rows, dst + i * 1024, !valid || voff[i] == kOOB ? kOOB : voff[i] + off);
+      dma16_nt(rows, dst + i * 1024, voff[i] == kOOB ? kOOB : voff[i] + off);
     const uint32_t at = static_cast<uint32_t>(first_part + t) + part;
-    dma4(scales, sdst, valid ? (at >> shift) * 4 : kOOB);
+    dma4(scales, sdst, (at >> shift) * 4);
   }
 };
 
@@ -196,14 +195,16 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
   char* mine = smem + wave * (2 * kStage);
   const uint32_t mine_addr = lds_addr(mine);
   auto issue_k = [&](int j) {
+    if (j >= mine_n) return;
     const int t = (wave + j * NW) * NK;
     const uint32_t st = mine_addr + (j & 1) * kStage;
-    kd.issue(st, st + 2 * kTileBytes, static_cast<uint32_t>(t * a.kst[2]), t, j < mine_n);
+    kd.issue(st, st + 2 * kTileBytes, static_cast<uint32_t>(t * a.kst[2]), t);
   };
   auto issue_v = [&](int j) {
+    if (j >= mine_n) return;
     const int t = (wave + j * NW) * NK;
     const uint32_t st = mine_addr + (j & 1) * kStage;
-    vd.issue(st + kTileBytes, st + 2 * kTileBytes + 256, static_cast<uint32_t>(t * a.vst[2]), t, j < mine_n);
+    vd.issue(st + kTileBytes, st + 2 * kTileBytes + 256, static_cast<uint32_t>(t * a.vst[2]), t);
   };
 
   f32x4 o[DT];
@@ -215,7 +216,16 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
   issue_v(0);
   issue_k(1);
   issue_v(1);
-  wait_dma<3 * kTileInst>();  // the queries, and the keys of tile 0
+  // all but what was issued behind tile j's keys: its values, and the tile after it
+  const auto wait_keys = [&](int j) {
+    if (j + 1 < mine_n)
+      wait_dma<3 * kTileInst>();
+    else if (j < mine_n)
+      wait_dma<kTileInst>();
+    else
+      wait_dma<0>();
+  };
+  wait_keys(0);  // and the queries
   u32x4 qf[2 * KC];
 #pragma unroll
   for (int s = 0; s < 2 * KC; ++s) {
@@ -225,7 +235,7 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
   for (int j = 0; j < mine_n; ++j) {
     const char* sk = mine + (j & 1) * kStage;
     const char* sv = sk + kTileBytes;
-    wait_dma<3 * kTileInst>();  // keys of tile j are in; its values and tile j + 1 may be in flight
+    wait_keys(j);
     f32x4 s[KB];
     float ks[KB];
 #pragma unroll
@@ -282,7 +292,13 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
         s[kb][e] = fast_exp2(s[kb][e] - m_use);
         l += s[kb][e];
       }
-    wait_dma<3 * kTileInst>();  // values of tile j are in
+    // values of tile j are in; behind them came tile j + 1, and the keys of j + 2
+    if (j + 2 < mine_n)
+      wait_dma<3 * kTileInst>();
+    else if (j + 1 < mine_n)
+      wait_dma<2 * kTileInst>();
+    else
+      wait_dma<0>();
     constexpr bool LO = std::is_same<T, _Float16>::value;
     u32x4 pf[KB / 2], pl[KB / 2];
 #pragma unroll

@@ -166,13 +166,20 @@ __global__ __launch_bounds__(64 * (BT == 128 ? 8 : 4), tile_blocks(BT, STAGES)) 
 #pragma unroll
   for (int u = 0; u < 2 * S::kScaleInst; ++u) issue_scales(0, u);
 #pragma unroll
-  for (int j = 0; j < STAGES - 1; ++j) issue(j);
+  for (int j = 0; j < STAGES - 1; ++j)
+    if (j < nt) issue(j);
   for (int j = 0; j < nt; ++j) {
     __builtin_amdgcn_sched_barrier(0);
-    wait_vmcnt<(STAGES - 2) * S::kLoads>();  // K tile j is in (past the last tile the loads are empty, but count)
+    // K tile j is in: all but the tiles behind it, STAGES - 2 until the last ones
+    if (STAGES == 4 && nt - 1 - j >= 2)
+      wait_vmcnt<2 * S::kLoads>();
+    else if (STAGES == 4 && nt - 1 - j == 1)
+      wait_vmcnt<S::kLoads>();
+    else
+      wait_vmcnt<0>();
     block_barrier();              // for every wave; and tile j - 1's stage is free
     asm volatile("" ::: "memory");
-    issue(j + STAGES - 1);
+    if (j + STAGES - 1 < nt) issue(j + STAGES - 1);
     const char* st = smem + (j & (STAGES - 1)) * S::kStage;
     const char* sc = smem + S::kScalesAt + (j / S::kGroup & (S::kScaleRing - 1)) * (2 * S::kScales) + j % S::kGroup * 8;
     uint32_t sa[TW], sb[TN];

@@ -6,7 +6,7 @@
 // as half a CU's LDS holds (one to three), with no barrier before their fp32 sums are
 // merged.  Two blocks share a CU, so that one streams while the other starts or
 // merges: 1 row, 100000 x 4096 took 52.2 us with one block of twice the ring a CU and
-// 38.7 with two, 28672 x 4096 17.8 and 15.1.  A step is 4 or (J 4) 8 KiB of B (16 J
+// 38.7 with two (now 36.1, 6.0 TB/s), 28672 x 4096 17.8 and 15.1.  A step is 4 or (J 4) 8 KiB of B (16 J
 // rows of 256 or 128 bytes, non-temporal, whole lines), the same columns of A's
 // rows, and the scales; steps of 8 KiB for J 1 left the ring one step shorter, 8.2 us
 // -> 10.4 at 1 row, 4096 x 14336.  Up to 4 rows (MR 4) A's part of a step is a
@@ -23,9 +23,9 @@
 // codes go to the LDS, where the fragments are read as ever.  Every block rounds the
 // same rows again, which pays for up to 4 of them: a kernel before this one and then
 // this one, against this one alone, in a captured graph, took 1 row of 4096 values
-// 5.9 against 4.4 us for 640 columns and 11.2 against 9.9 for 14336; 4 rows 5.8
-// against 4.7 and 11.2 against 10.6, and 4 rows of 14336 values, the most a wave has
-// to round, 10.8 against 10.4 for 4096 columns.
+// 5.5 against 4.2 us for 640 columns and 10.9 against 9.5 for 14336; 4 rows 5.6
+// against 4.5 and 11.0 against 9.9, and 4 rows of 14336 values, the most a wave has
+// to round, 10.7 against 10.2 for 4096 columns.
 #include <algorithm>
 #include <atomic>
 
@@ -86,14 +86,14 @@ struct Loader {
       soff[i] = r < rows && r < ROWS ? (static_cast<uint32_t>(o + r * lds) & ~3u) + (id - r * ND) * 4 : kOOB;
     }
   }
-  __device__ __forceinline__ void issue(uint32_t dst, int b0, bool valid, int lane) const {
+  __device__ __forceinline__ void issue(uint32_t dst, int b0, int lane) const {
 #pragma unroll
     for (int i = 0; i < kInst; ++i)
       sk_dma<NT>(codes, dst + i * 1024,
-                 valid && voff[i] != kOOB && b0 + chunk(lane, i) < kb ? voff[i] + static_cast<uint32_t>(b0) * 16 : kOOB);
+                 voff[i] != kOOB && b0 + chunk(lane, i) < kb ? voff[i] + static_cast<uint32_t>(b0) * 16 : kOOB);
 #pragma unroll
     for (int i = 0; i < kScaleInst; ++i)
-      dma4(scales, dst + kBytes + i * 256, valid && soff[i] != kOOB ? soff[i] + static_cast<uint32_t>(b0) : kOOB);
+      dma4(scales, dst + kBytes + i * 256, soff[i] != kOOB ? soff[i] + static_cast<uint32_t>(b0) : kOOB);
   }
 };
 
@@ -119,11 +119,11 @@ struct RawLoader {
       voff[i] = r < n ? static_cast<uint32_t>(r * ld * 2 + in_row(lane, i)) : kOOB;
     }
   }
-  __device__ __forceinline__ void issue(uint32_t dst, int b0, bool valid, int lane) const {
+  __device__ __forceinline__ void issue(uint32_t dst, int b0, int lane) const {
 #pragma unroll
     for (int i = 0; i < kInst; ++i)
       dma16(rows, dst + i * 1024,
-            valid && voff[i] != kOOB && b0 * 64 + in_row(lane, i) < row_bytes ? voff[i] + static_cast<uint32_t>(b0) * 64 : kOOB);
+            voff[i] != kOOB && b0 * 64 + in_row(lane, i) < row_bytes ? voff[i] + static_cast<uint32_t>(b0) * 64 : kOOB);
   }
   // block c of row r
   __device__ __forceinline__ static void block(const char* t, int r, int c, u32x4 (&x)[4]) {
@@ -179,12 +179,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_mx4_skinny(Mx4Args g, int wh
   char* own = mine + S * kStep;  // X: the step's codes and scales
   const uint32_t mine_addr = lds_addr(mine);
   int slot_in = 0;
-  // step j of this wave into ring slot j % S (past the end: empty loads, so that the waits count the same)
+  // step j of this wave into ring slot j % S
   auto issue = [&](int j) {
+    if (j >= n) return;
     const int b0 = (wave + j * kWaves) * CPR;
     const uint32_t dst = mine_addr + slot_in * kStep;
-    lb.issue(dst, b0, j < n, lane);
-    la.issue(dst + kStepB, b0, j < n, lane);
+    lb.issue(dst, b0, lane);
+    la.issue(dst + kStepB, b0, lane);
     slot_in = slot_in + 1 == S ? 0 : slot_in + 1;
   };
   // this lane's first scale byte in a step's dwords: of its row of A, of its columns
@@ -204,7 +205,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_mx4_skinny(Mx4Args g, int wh
   int slot = 0;
   for (int i = 0; i < n; ++i) {
     __builtin_amdgcn_sched_barrier(0);
-    wait_vmcnt<(S - 1) * kInst>();
+    // step i is in: all but the steps behind it, S - 1 until the last ones
+    const int behind = n - 1 - i;
+    if (behind >= S - 1)
+      wait_vmcnt<(S - 1) * kInst>();
+    else if (S > 3 && behind == 2)
+      wait_vmcnt<2 * kInst>();
+    else if (S > 2 && behind == 1)
+      wait_vmcnt<kInst>();
+    else
+      wait_vmcnt<0>();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     const char* tb = mine + slot * kStep;
@@ -289,7 +299,8 @@ int run_skinny(const Mx4Args& g, int j, hipStream_t st) {
 // and one alone has the CU's bandwidth, cost their bytes and their starts, as much
 // as 20 KiB of B each.  A ring of one step (lone) needs the CU's other block to
 // cover its waits; two columns give the same sums as four.
-// Measured with 1, 2 and 4 (us): 1 row, 4096 x 4096 4.8, 5.3, 7.1; 14336 x 4096
+// Measured with 1, 2 and 4 (us, with empty loads past a wave's last step, which are
+// gone): 1 row, 4096 x 4096 4.8, 5.3, 7.1; 14336 x 4096
 // 11.2, 9.6, 9.2; 100000 x 4096 52.4, 42.0, 38.7; 24000 x 2048 12.1, 10.5, 9.4;
 // 8 rows, 14336 x 4096 12.3, 9.9, 11.0; 16 rows, 100000 x 4096 60.4, 47.7, 45.4.
 int columns(int64_t N, int64_t kb, bool lone) {
