@@ -2,6 +2,7 @@
 e4m3 and attention, and what the entry points refuse."""
 
 import ctypes
+import inspect
 
 import numpy as np
 import pytest
@@ -50,6 +51,55 @@ def test_oracle_attention_is_softmax():
     want = torch.nn.functional.scaled_dot_product_attention(torch.from_numpy(q), kk, vv, mask, scale=0.3)
     assert np.allclose(out[0], want[0].numpy())
     assert not out[1, :, 0].any() and np.allclose(out[1, :, 1], vv[1, :, 0].numpy())
+
+
+def test_oracle_attention_scales_each_block():
+    rng = np.random.default_rng(3)
+    q, k, v = rng.standard_normal((1, 2, 2, 8)), rng.standard_normal((1, 1, 40, 8)), rng.standard_normal((1, 1, 40, 8))
+    ks, vs = np.array([[[0.5, 2.0, 0.125]]]), np.array([[[4.0, 0.25, 1.5]]])
+    out = N.kv_cache_attention(q, k, v, ks, vs, [37], 16, False, 0.5)
+    at = np.arange(37) // 16
+    kk, vv = (torch.from_numpy(x[:, :, :37] * s[..., at][..., None]).expand(1, 2, 37, 8) for x, s in ((k, ks), (v, vs)))
+    assert np.allclose(out, torch.nn.functional.scaled_dot_product_attention(torch.from_numpy(q), kk, vv, scale=0.5).numpy())
+
+
+def planted(monkeypatch, right, wrong):
+    """The oracle with one mistake in it."""
+    source = inspect.getsource(N)
+    assert source.count(right) == 1
+    names = {}
+    exec(compile(source.replace(right, wrong), "planted", "exec"), names)
+    for name, value in names.items():
+        if inspect.isfunction(value):
+            monkeypatch.setattr(N, name, value)
+
+
+def catches(check):
+    try:
+        check()
+    except AssertionError:
+        return True
+    return False
+
+
+@pytest.mark.parametrize(
+    "right,wrong",
+    [
+        ("-6).astype(np.float64) - 3", "-5).astype(np.float64) - 3"),
+        ("np.rint(a / unit)", "np.floor(a / unit)"),
+        ("1.0)) - 8, -126)", "1.0)) - 7, -126)"),
+        ("(old / s)", "(s / old)"),
+        ("if old > s:", "if old < s:"),
+        ("np.arange(Sq)[:, None] + n - Sq if", "np.arange(Sq)[:, None] + n - Sq - 1 if"),
+        ("g = h // group", "g = h % k.shape[1]"),
+        ("[at // block][:, None]\n            s = ", "[at // block - 1][:, None]\n            s = "),
+    ],
+)
+def test_oracle_checks_catch(right, wrong, monkeypatch):
+    planted(monkeypatch, right, wrong)
+    checks = (test_oracle_rounds_as_torch_does, test_oracle_scale_is_the_least, test_oracle_store_reads_back, test_oracle_attention_is_softmax,
+              test_oracle_attention_scales_each_block)
+    assert any(catches(c) for c in checks)
 
 
 def caches(b=2, h=2, c=40, d=16, block=16, dtype=E4M3):

@@ -2,6 +2,7 @@
 points refuse."""
 
 import ctypes
+import inspect
 
 import numpy as np
 import pytest
@@ -45,6 +46,43 @@ def test_oracle_zeros_and_not_finite():
     x[0, 40], x[0, 70] = np.inf, np.nan
     codes, scales = N.quantize_mxfp4(x)
     assert scales.tolist() == [[0, 255, 255]] and not codes.any()
+
+
+def planted(monkeypatch, right, wrong):
+    """The oracle with one mistake in it."""
+    source = inspect.getsource(N)
+    assert source.count(right) == 1
+    names = {}
+    exec(compile(source.replace(right, wrong), "planted", "exec"), names)
+    for name, value in names.items():
+        if inspect.isfunction(value):
+            monkeypatch.setattr(N, name, value)
+
+
+def catches(check):
+    try:
+        check()
+    except AssertionError:
+        return True
+    return False
+
+
+@pytest.mark.parametrize(
+    "right,wrong",
+    [
+        ("_floor_log2(top) - 2, -127)", "_floor_log2(top) - 1, -127)"),
+        ("(i % 2 == 1)", "(i % 2 == 0)"),
+        ("code[..., 0] + 16 * code[..., 1]", "code[..., 1] + 16 * code[..., 0]"),
+        ("np.where(bad, 255, e + 127)", "np.where(bad, 254, e + 127)"),
+        ("np.where(nibbles < 8, 1.0, -1.0)", "np.where(nibbles > 8, 1.0, -1.0)"),
+        ("[codes & 15, codes >> 4]", "[codes >> 4, codes & 15]"),
+        ("E2M1[i] + E2M1[i + 1]) / 2", "E2M1[i] + 2 * E2M1[i + 1]) / 3"),
+    ],
+)
+def test_oracle_checks_catch(right, wrong, monkeypatch):
+    planted(monkeypatch, right, wrong)
+    checks = (test_oracle_rounds_to_the_nearest_code, test_oracle_ties_go_to_the_even_code, test_oracle_packs_the_first_value_low, test_oracle_zeros_and_not_finite)
+    assert any(catches(c) for c in checks)
 
 
 def test_refusals():
