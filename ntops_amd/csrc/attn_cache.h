@@ -42,12 +42,16 @@ __device__ __forceinline__ int64_t length_of(const CacheAttnArgs& a, int b) {
   return max(int64_t(0), min(a.C, index_at(a.lengths, a.lengths_dtype, b, a.C)));
 }
 
-constexpr int kDecodeRows = 16;  // most query rows per cache head of cache_decode
+// Most query rows per cache head of cache_decode: with more, its registers are spent.
+// 5 positions of 4 heads, bf16 of 128: (16, 32 / 8, 5, 2048 .. 4096) 30.7 us, by
+// cache_tile 46.3; (1, 32 / 8, 8, 131000) 57.5 and 92.6; (64, 32 / 8, 8, 1024 .. 2048)
+// 48.6 and 76.3.
+constexpr int kDecodeRows = 32;
 
 // 16-bit queries of head dims and layouts that the matrix cores' kernels read.
 bool cache_matrix_layout(const CacheAttnArgs& a, int dtype);
 
-// True when cache_decode serves this problem: such a layout, and at most 16
+// True when cache_decode serves this problem: such a layout, and at most kDecodeRows
 // query rows per cache head.
 bool cache_decode_serves(const CacheAttnArgs& a, int dtype);
 // Bytes of workspace with which it spreads the keys over more blocks (0: one

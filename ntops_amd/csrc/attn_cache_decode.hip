@@ -1,9 +1,10 @@
-// A few query rows over an 8-bit cache (decode): Sq * (Hq / Hkv) <= 16 rows per
+// A few query rows over an 8-bit cache (decode): Sq * (Hq / Hkv) <= 32 rows per
 // cache head.
 //
 // Bound by streaming the cache once.  A work item is (batch, cache head, slice
 // of the sequence's tokens); the rows that share the head fill the 16 columns
-// of v_mfma_f32_16x16x32 (S^T = K Q^T, O^T += V^T P^T).  Every wave owns its own
+// of v_mfma_f32_16x16x32 (S^T = K Q^T, O^T += V^T P^T), or twice 16 (RB 2), for
+// which the cache's fragments are read and widened once.  Every wave owns its own
 // key tiles, 4 KiB of keys and of values each (32 keys at a head dim of 128), in
 // its own part of the LDS: direct non-temporal DMA two tiles ahead, refilled as
 // soon as the tile's keys, then its values, have been read, and no barrier
@@ -135,7 +136,7 @@ typedef __attribute__((address_space(3))) i32x2 lds_i32x2_t;
 
 // part: fp32, per query row and slice the unnormalised O row, then (max in base
 // 2, sum) pairs; null: one slice, O normalised into a.o.
-template <typename T, int D, int NW>
+template <typename T, int D, int NW, int RB>
 __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, int nsplit, float* part) {
   constexpr int NK = kTileBytes / D;  // keys per tile
   constexpr int KB = NK / 16;   // 16-key parts of a tile
@@ -152,24 +153,27 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
   const int sp = static_cast<int>(blk - static_cast<int64_t>(bh) * nsplit);
   const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
   const int group = a.Hq / a.Hkv;
-  const int rows = group * a.Sq;  // <= 16
+  constexpr int ROWS = 16 * RB;
+  const int rows = group * a.Sq;  // <= ROWS
   const int64_t n_all = length_of(a, b);
   // this slice: whole rounds of the waves' tiles
   const int64_t step = NK * NW;
   const int64_t chunk = (n_all + nsplit * step - 1) / (nsplit * step) * step;
   const int64_t t0 = sp * chunk;
   const int n = __builtin_amdgcn_readfirstlane(static_cast<int>(max(int64_t(0), min(n_all - t0, chunk))));
-  // query row of this lane's column: head hk * group + r / Sq, position r % Sq
+  // query row of this lane's column, in each 16 rows: head hk * group + r / Sq, position r % Sq
   const int r = lane & 15;
-  const int qi = r % a.Sq;
-  // keys of the slice that the row sees, and that every row sees
-  const int lim = a.causal ? static_cast<int>(max(int64_t(-1), min(int64_t(n), n_all - a.Sq + qi + 1 - t0))) : n;
+  // keys of the slice that the rows see, and that every row sees
+  int lim[RB];
+#pragma unroll
+  for (int x = 0; x < RB; ++x)
+    lim[x] = a.causal ? static_cast<int>(max(int64_t(-1), min(int64_t(n), n_all - a.Sq + (16 * x + r) % a.Sq + 1 - t0))) : n;
   const int lim_min = a.causal ? static_cast<int>(max(int64_t(-1), min(int64_t(n), n_all - a.Sq + 1 - t0))) : n;
 
   // The query rows ahead of the first tiles, by DMA too (rows of D values, chunk c
   // of row r at slot c ^ r): as loads of their own they would be waited for first.
   // Every wave brings them all, to one place.
-  constexpr int kQInst = D / 32;          // instructions of 1 KiB
+  constexpr int kQInst = ROWS * D / 512;  // instructions of 1 KiB
   constexpr int kQRows = 512 / D;         // rows of one
   const uint32_t q_lds = lds_addr(smem) + NW * 2 * kStage;
   {
@@ -207,10 +211,15 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
     vd.issue(st + kTileBytes, st + 2 * kTileBytes + 256, static_cast<uint32_t>(t * a.vst[2]), t);
   };
 
-  f32x4 o[DT];
+  f32x4 o[RB][DT];
+  float m[RB], l[RB];  // running max (base 2) of each row; this lane's part of its sum
 #pragma unroll
-  for (int t = 0; t < DT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = neg_inf(), l = 0.f;  // running max (base 2) of row r; this lane's part of its sum
+  for (int x = 0; x < RB; ++x) {
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[x][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m[x] = neg_inf();
+    l[x] = 0.f;
+  }
 
   issue_k(0);
   issue_v(0);
@@ -226,21 +235,24 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
       wait_dma<0>();
   };
   wait_keys(0);  // and the queries
-  u32x4 qf[2 * KC];
+  u32x4 qf[RB][2 * KC];
 #pragma unroll
-  for (int s = 0; s < 2 * KC; ++s) {
-    const int c = ((s >> 1) * 4 + g) * 2 + (s & 1);  // the key bytes of k-step s in this lane
-    qf[s] = *reinterpret_cast<const u32x4*>(smem + NW * 2 * kStage + r * (D * 2) + (c ^ (r & (D / 8 - 1))) * 16);
-  }
+  for (int x = 0; x < RB; ++x)
+#pragma unroll
+    for (int s = 0; s < 2 * KC; ++s) {
+      const int c = ((s >> 1) * 4 + g) * 2 + (s & 1), row = 16 * x + r;  // the key bytes of k-step s in this lane
+      qf[x][s] = *reinterpret_cast<const u32x4*>(smem + NW * 2 * kStage + row * (D * 2) + (c ^ (row & (D / 8 - 1))) * 16);
+    }
   for (int j = 0; j < mine_n; ++j) {
     const char* sk = mine + (j & 1) * kStage;
     const char* sv = sk + kTileBytes;
     wait_keys(j);
-    f32x4 s[KB];
+    f32x4 s[RB][KB];
     float ks[KB];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < RB; ++x) s[x][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
       ks[kb] = *reinterpret_cast<const float*>(sk + 2 * kTileBytes + kb * 4);
     }
 #pragma unroll
@@ -249,49 +261,56 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
       for (int kb = 0; kb < KB; ++kb) {
         const int row = kb * 16 + (lane & 15);
         const u32x4 w = *reinterpret_cast<const u32x4*>(sk + row * D + kslot8<D>(row, c * 4 + g) * 16);
-        s[kb] = mfma16<T>(widen8<T>(w.x, w.y), qf[2 * c], s[kb]);
-        s[kb] = mfma16<T>(widen8<T>(w.z, w.w), qf[2 * c + 1], s[kb]);
+        const u32x4 k0 = widen8<T>(w.x, w.y), k1 = widen8<T>(w.z, w.w);
+#pragma unroll
+        for (int x = 0; x < RB; ++x) {
+          s[x][kb] = mfma16<T>(k0, qf[x][2 * c], s[x][kb]);
+          s[x][kb] = mfma16<T>(k1, qf[x][2 * c + 1], s[x][kb]);
+        }
       }
     wait_lgkmcnt0();
     issue_k(j + 2);
 
     // scores of the slice's keys kt + 16 kb + 4 g + e
     const int kt = (wave + j * NW) * NK;
-    float mx = neg_inf();
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[kb][e] *= ks[kb] * a.scale_log2;
-    if (kt + NK > lim_min) {
+    for (int x = 0; x < RB; ++x) {
+      float mx = neg_inf();
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[kb][e] = kt + kb * 16 + 4 * g + e < lim ? s[kb][e] : neg_inf();
-    }
+        for (int e = 0; e < 4; ++e) s[x][kb][e] *= ks[kb] * a.scale_log2;
+      if (kt + NK > lim_min) {
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[kb][e]);
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float m_new = fmaxf(m, mx);
-    const float m_use = m_new == neg_inf() ? 0.f : m_new;  // nothing seen so far: P = 0
-    if (__any(m_new > m)) {
-      const float alpha = fast_exp2(m - m_use);
-      l *= alpha;
-#pragma unroll
-      for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[t][e] *= alpha;
-      m = m_new;
-    }
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[kb][e] = fast_exp2(s[kb][e] - m_use);
-        l += s[kb][e];
+          for (int e = 0; e < 4; ++e) s[x][kb][e] = kt + kb * 16 + 4 * g + e < lim[x] ? s[x][kb][e] : neg_inf();
       }
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[x][kb][e]);
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float m_new = fmaxf(m[x], mx);
+      const float m_use = m_new == neg_inf() ? 0.f : m_new;  // nothing seen so far: P = 0
+      if (__any(m_new > m[x])) {
+        const float alpha = fast_exp2(m[x] - m_use);
+        l[x] *= alpha;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[x][t][e] *= alpha;
+        m[x] = m_new;
+      }
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[x][kb][e] = fast_exp2(s[x][kb][e] - m_use);
+          l[x] += s[x][kb][e];
+        }
+    }
     // values of tile j are in; behind them came tile j + 1, and the keys of j + 2
     if (j + 2 < mine_n)
       wait_dma<3 * kTileInst>();
@@ -300,17 +319,20 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
     else
       wait_dma<0>();
     constexpr bool LO = std::is_same<T, _Float16>::value;
-    u32x4 pf[KB / 2], pl[KB / 2];
+    u32x4 pf[RB][KB / 2], pl[RB][KB / 2];
 #pragma unroll
     for (int p = 0; p < KB / 2; ++p) {
-      float x[8];
+      float v[RB][8];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const float vs = *reinterpret_cast<const float*>(sk + 2 * kTileBytes + 256 + (2 * p + u) * 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 * u + e] = s[2 * p + u][e] * vs;
+        for (int x = 0; x < RB; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[x][4 * u + e] = s[x][2 * p + u][e] * vs;
       }
-      pack_p<LO>(x, pf[p], pl[p]);  // keys 32 p + 4 g + 0..3 and 32 p + 16 + 4 g + 0..3
+#pragma unroll
+      for (int x = 0; x < RB; ++x) pack_p<LO>(v[x], pf[x][p], pl[x][p]);  // keys 32 p + 4 g + 0..3 and 32 p + 16 + 4 g + 0..3
     }
 #pragma unroll
     for (int p = 0; p < KB / 2; ++p)
@@ -323,36 +345,48 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
         const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
             (lds_i32x2_t*)(sv + row * D + vslot8<D>(row, t) * 16 + (i & 1) * 8));
         const u32x4 vf = widen8<__bf16>(w.x, w.y);
-        o[t] = mfma16<__bf16>(vf, pf[p], o[t]);
-        if constexpr (LO) o[t] = mfma16<__bf16>(vf, pl[p], o[t]);
+#pragma unroll
+        for (int x = 0; x < RB; ++x) {
+          o[x][t] = mfma16<__bf16>(vf, pf[x][p], o[x][t]);
+          if constexpr (LO) o[x][t] = mfma16<__bf16>(vf, pl[x][p], o[x][t]);
+        }
       }
     wait_lgkmcnt0();
     issue_v(j + 2);
   }
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
+#pragma unroll
+  for (int x = 0; x < RB; ++x) {
+    l[x] += __shfl_xor(l[x], 16, 64);
+    l[x] += __shfl_xor(l[x], 32, 64);
+  }
   wait_dma<0>();  // no DMA may land in the LDS the merge reuses
   __syncthreads();
 
   // merge the waves: per-wave (max, sum) of every row, then O scaled to the
   // block's max
-  float* sm = reinterpret_cast<float*>(smem);  // [wave][16] max, [wave][16] sum, then [wave][16][D + 4] O
-  float* so = sm + 2 * NW * 16;
+  float* sm = reinterpret_cast<float*>(smem);  // [wave][ROWS] max, [wave][ROWS] sum, then [wave][ROWS][D + 4] O
+  float* so = sm + 2 * NW * ROWS;
   constexpr int LD = D + 4;
-  if (g == 0) {
-    sm[wave * 16 + r] = m;
-    sm[(NW + wave) * 16 + r] = l;
-  }
+  if (g == 0)
+#pragma unroll
+    for (int x = 0; x < RB; ++x) {
+      sm[wave * ROWS + 16 * x + r] = m[x];
+      sm[(NW + wave) * ROWS + 16 * x + r] = l[x];
+    }
   __syncthreads();
-  float mb = sm[r];
 #pragma unroll
-  for (int w = 1; w < NW; ++w) mb = fmaxf(mb, sm[w * 16 + r]);
-  // (a wave whose scores are all NaN has a NaN sum and no max)
-  const float f = m == neg_inf() ? 0.f : fast_exp2(m - mb);
+  for (int x = 0; x < RB; ++x) {
+    const int row = 16 * x + r;
+    float mb = sm[row];
 #pragma unroll
-  for (int t = 0; t < DT; ++t)
+    for (int w = 1; w < NW; ++w) mb = fmaxf(mb, sm[w * ROWS + row]);
+    // (a wave whose scores are all NaN has a NaN sum and no max)
+    const float f = m[x] == neg_inf() ? 0.f : fast_exp2(m[x] - mb);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) so[(wave * 16 + r) * LD + t * 16 + 4 * g + e] = o[t][e] * f;
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) so[(wave * ROWS + row) * LD + t * 16 + 4 * g + e] = o[x][t][e] * f;
+  }
   __syncthreads();
   const int64_t nrow = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
   float* part_ml = part + nrow * nsplit * a.D;
@@ -361,15 +395,15 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
     if (d >= a.D) continue;
     float mm = sm[row];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) mm = fmaxf(mm, sm[w * 16 + row]);
+    for (int w = 1; w < NW; ++w) mm = fmaxf(mm, sm[w * ROWS + row]);
     float sum = 0.f;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const float mw = sm[w * 16 + row], lw = sm[(NW + w) * 16 + row];
+      const float mw = sm[w * ROWS + row], lw = sm[(NW + w) * ROWS + row];
       sum += mw == neg_inf() ? lw : lw * fast_exp2(mw - mm);  // (no max: 0, or NaN)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += so[(w * 16 + row) * LD + d + e];
+      for (int e = 0; e < 4; ++e) v[e] += so[(w * ROWS + row) * LD + d + e];
     }
     const int hh = hk * group + row / a.Sq, qq = row % a.Sq;
     if (part) {
@@ -458,15 +492,15 @@ void decode_split(int64_t heads, int64_t C, int64_t D, int& waves, int& nsplit) 
   nsplit = static_cast<int>(std::max<int64_t>(n, 1));
 }
 
-template <typename T, int D, int NW>
+template <typename T, int D, int NW, int RB>
 int launch_decode(const CacheAttnArgs& a, int nsplit, float* part, hipStream_t st) {
-  constexpr int kLds = NW * 2 * kStage + 32 * D;
-  static_assert((2 * NW * 16 + NW * 16 * (D + 4)) * 4 <= kLds, "LDS");
-  auto kern = k_cache_decode<T, D, NW>;
+  constexpr int kLds = NW * 2 * kStage + 32 * D * RB;
+  static_assert((2 * NW + NW * (D + 4)) * 16 * RB * 4 <= kLds && kLds * 8 / NW <= 163840, "LDS");
+  auto kern = k_cache_decode<T, D, NW, RB>;
   static std::atomic<uint64_t> reserved{0};
   if (const int rc = reserve_lds(reinterpret_cast<const void*>(kern), kLds, reserved, "kv_cache_attention"); rc != NTOPS_OK) return rc;
   const int64_t blocks = static_cast<int64_t>(nsplit) * a.B * a.Hkv;
-  note_kernel("kv_cache_decode d%d waves%d split%d", D, NW, nsplit);
+  note_kernel("kv_cache_decode d%d rows%d waves%d split%d", D, 16 * RB, NW, nsplit);
   hipLaunchKernelGGL(kern, blocks_2d(blocks), dim3(64 * NW), kLds, st, a, nsplit, part);
   if (part) cache_merge(std::is_same<T, __bf16>::value ? NTOPS_BF16 : NTOPS_F16, a, nsplit, part, st);
   return check_launch("kv_cache_attention");
@@ -482,9 +516,12 @@ int run_decode(const CacheAttnArgs& a, void* ws, int64_t ws_bytes, hipStream_t s
     ws = nullptr;
   }
   float* part = static_cast<float*>(ws);
-  if (waves == 8)
-    return a.D > 64 ? launch_decode<T, 128, 8>(a, nsplit, part, st) : launch_decode<T, 64, 8>(a, nsplit, part, st);
-  return a.D > 64 ? launch_decode<T, 128, 4>(a, nsplit, part, st) : launch_decode<T, 64, 4>(a, nsplit, part, st);
+  const auto go = [&](auto rb) {
+    constexpr int RB = decltype(rb)::value;
+    if (waves == 8) return a.D > 64 ? launch_decode<T, 128, 8, RB>(a, nsplit, part, st) : launch_decode<T, 64, 8, RB>(a, nsplit, part, st);
+    return a.D > 64 ? launch_decode<T, 128, 4, RB>(a, nsplit, part, st) : launch_decode<T, 64, 4, RB>(a, nsplit, part, st);
+  };
+  return a.Sq * (a.Hq / a.Hkv) <= 16 ? go(std::integral_constant<int, 1>{}) : go(std::integral_constant<int, 2>{});
 }
 
 }  // namespace

@@ -236,6 +236,27 @@ def test_attention(b, hq, h, sq, c, d, block, dtype, causal):
     check_attention(query, caches, lengths, causal, block, 0.3)
 
 
+# 17 to 32 query rows a cache head: positions and heads in the second sixteen.
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize(
+    "b,hq,h,sq,c,d,block",
+    [(2, 8, 2, 5, 333, 128, 16), (1, 32, 1, 1, 2049, 128, 64), (3, 6, 2, 9, 200, 64, 32), (66, 24, 8, 7, 130, 80, 64), (1, 17, 1, 1, 40, 16, 16),
+     (2, 2, 2, 32, 31, 96, 128), (37, 16, 8, 10, 2100, 48, 64), (1, 8, 2, 8, 6000, 112, 128)],
+)
+def test_attention_two_sixteens(b, hq, h, sq, c, d, block, dtype, causal):
+    caches = filled(b, h, c, d, block, dtype)
+    query = torch.randn(b, hq, sq, d).to(dtype).cuda()
+    check_attention(query, caches, None, causal, block)
+    assert "kv_cache_decode" in _lib.last_kernel() and "rows32" in _lib.last_kernel(), _lib.last_kernel()
+    lengths = torch.randint(0, c + 1, (b,), dtype=torch.int32)
+    lengths[0] = min(sq, c) // 2
+    check_attention(query, caches, lengths.cuda(), causal, block, -0.3)
+    query[0, hq - 1, sq - 1, 1] = float("nan")  # stays in its row
+    out = check_attention(query, caches, None, causal, block)
+    assert torch.isnan(out[0, hq - 1, sq - 1]).all() and torch.isnan(out).sum() == d
+
+
 # More heads than compute units: blocks of fewer waves share a unit, and only long
 # caches of few more heads are split.
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
