@@ -72,7 +72,7 @@ bool mx4_large_serves(int out_dtype, const Mx4Args& g);
 int64_t mx4_large_workspace(int64_t M, int64_t N, int64_t kb);
 int mx4_large(int out_dtype, Mx4Args g, void* workspace, hipStream_t st);
 
-constexpr int kSkinnyRows = 16;
+constexpr int kSkinnyRows = 32;
 // out for M <= kSkinnyRows, bound by streaming B.
 int mx4_skinny(int out_dtype, const Mx4Args& g, hipStream_t st);
 // The same with A quantized by the blocks themselves (g.x), for up to kFusedRows

@@ -1,4 +1,4 @@
-// MXFP4 products of up to 16 rows (decode projections): bound by streaming B,
+// MXFP4 products of up to 32 rows (decode projections): bound by streaming B,
 // (16 + 1) / 32 bytes a value, once.
 //
 // A block covers 16 J columns; its four waves each own K steps of their own and
@@ -10,7 +10,10 @@
 // rows of 256 or 128 bytes, non-temporal, whole lines), the same columns of A's
 // rows, and the scales; steps of 8 KiB for J 1 left the ring one step shorter, 8.2 us
 // -> 10.4 at 1 row, 4096 x 14336.  Up to 4 rows (MR 4) A's part of a step is a
-// quarter, and the ring longer; the instruction's other rows read the four again.
+// quarter, and the ring longer; the instruction's other rows read the four again.  From
+// 17 rows on (MR 32) two sixteens use B's fragments: 17 rows, 4096 x 4096 6.2 us (in
+// 64 x 64 tiles 8.8), 32 rows, 14336 x 4096 11.5 (12.6), 4096 x 14336 13.7 (15.8), 1000
+// x 2000 4.5 (6.9).
 //
 // The scales are loaded as the dwords that the step's CPR bytes of a row lie in (one
 // more than they fill, as a row may start inside one) and read as single bytes;
@@ -147,7 +150,7 @@ struct Ring {
   static constexpr int kFit = (163840 / 2 / kWaves - kOwn) / kStep;  // two blocks a CU
   static constexpr int S = kFit < 4 ? kFit : 4;
   static constexpr int kLds = kWaves * (S * kStep + kOwn);
-  static_assert(S >= 1 && kLds >= kWaves * J * 1024, "a step, and the sums to merge");
+  static_assert(S >= 1 && kLds >= kWaves * J * (MR > 16 ? MR / 16 : 1) * 1024, "a step, and the sums to merge");
 };
 
 template <typename T, typename X, int J, int MR>
@@ -188,18 +191,25 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_mx4_skinny(Mx4Args g, int wh
     la.issue(dst + kStepB, b0, lane);
     slot_in = slot_in + 1 == S ? 0 : slot_in + 1;
   };
-  // this lane's first scale byte in a step's dwords: of its row of A, of its columns
-  const int ar = i16 & (MR - 1);
-  const int sat = LC::kBytes + ar * (LC::ND * 4) + q +
-                  (R::kRaw ? 0 : static_cast<int>((reinterpret_cast<uintptr_t>(g.as) + ar * g.ldas) & 3u));
+  // this lane's first scale byte in a step's dwords: of its rows of A, of its columns
+  constexpr int RB = MR > 16 ? MR / 16 : 1;
+  int ar[RB], sat[RB];
+#pragma unroll
+  for (int x = 0; x < RB; ++x) {
+    ar[x] = 16 * x + (i16 & (MR - 1));
+    sat[x] = LC::kBytes + ar[x] * (LC::ND * 4) + q +
+             (R::kRaw ? 0 : static_cast<int>((reinterpret_cast<uintptr_t>(g.as) + ar[x] * g.ldas) & 3u));
+  }
   int sbt[J];
 #pragma unroll
   for (int j = 0; j < J; ++j)
     sbt[j] = LB::kBytes + (j * 16 + i16) * (LB::ND * 4) +
              static_cast<int>((reinterpret_cast<uintptr_t>(g.bs) + (n0 + j * 16 + i16) * g.ldbs) & 3u) + q;
-  f32x4 acc[J];
+  f32x4 acc[RB][J];
 #pragma unroll
-  for (int j = 0; j < J; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int x = 0; x < RB; ++x)
+#pragma unroll
+    for (int j = 0; j < J; ++j) acc[x][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int s = 0; s < S; ++s) issue(s);
   int slot = 0;
@@ -241,16 +251,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_mx4_skinny(Mx4Args g, int wh
 #pragma unroll
     for (int u = 0; u < NB; ++u) {
       const int c = 4 * u + q;
-      const u32x4 a = *reinterpret_cast<const u32x4*>(ta + ar * (CPR * 16) + sk_slot<CPR>(ar, c) * 16);
-      uint32_t sa = *reinterpret_cast<const uint8_t*>(ta + sat + 4 * u);
-      if (left < CPR) sa = c < left ? sa : 0;
+      u32x4 a[RB];
+      uint32_t sa[RB];
+#pragma unroll
+      for (int x = 0; x < RB; ++x) {
+        a[x] = *reinterpret_cast<const u32x4*>(ta + ar[x] * (CPR * 16) + sk_slot<CPR>(ar[x], c) * 16);
+        sa[x] = *reinterpret_cast<const uint8_t*>(ta + sat[x] + 4 * u);
+        if (left < CPR) sa[x] = c < left ? sa[x] : 0;
+      }
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const int r = j * 16 + i16;
         const u32x4 b = *reinterpret_cast<const u32x4*>(tb + r * (CPR * 16) + sk_slot<CPR>(r, c) * 16);
         uint32_t sb = *reinterpret_cast<const uint8_t*>(tb + sbt[j] + 4 * u);
         if (left < CPR) sb = c < left ? sb : 0;
-        acc[j] = mfma_mx4<0, 0>(b, sb, a, sa, acc[j]);
+#pragma unroll
+        for (int x = 0; x < RB; ++x) acc[x][j] = mfma_mx4<0, 0>(b, sb, a[x], sa[x], acc[x][j]);
       }
     }
     wait_lgkmcnt0();
@@ -259,20 +275,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_mx4_skinny(Mx4Args g, int wh
   }
   wait_vmcnt<0>();  // no DMA may land in the LDS the merge reuses
   __syncthreads();
-  // lane l holds row l & 15, columns 16 j + 4 (l >> 4) .. + 3
-  f32x4* red = reinterpret_cast<f32x4*>(smem);  // [wave][j][lane]
+  // lane l holds rows 16 x + l & 15, columns 16 j + 4 (l >> 4) .. + 3
+  f32x4* red = reinterpret_cast<f32x4*>(smem);  // [wave][x][j][lane]
 #pragma unroll
-  for (int j = 0; j < J; ++j) red[(wave * J + j) * 64 + lane] = acc[j];
+  for (int x = 0; x < RB; ++x)
+#pragma unroll
+    for (int j = 0; j < J; ++j) red[((wave * RB + x) * J + j) * 64 + lane] = acc[x][j];
   __syncthreads();
-  if (wave < J) {
-    f32x4 v = red[wave * 64 + lane];
+  for (int i = wave; i < RB * J; i += kWaves) {
+    f32x4 v = red[i * 64 + lane];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) {
-      const f32x4 x = red[(w * J + wave) * 64 + lane];
+      const f32x4 y = red[(w * (RB * J) + i) * 64 + lane];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += x[e];
+      for (int e = 0; e < 4; ++e) v[e] += y[e];
     }
-    store4<T>(static_cast<T*>(g.d), g.ldd, i16, n0 + wave * 16 + 4 * q, g.M, g.N, v, static_cast<const T*>(g.bias), whole != 0);
+    store4<T>(static_cast<T*>(g.d), g.ldd, i / J * 16 + i16, n0 + i % J * 16 + 4 * q, g.M, g.N, v, static_cast<const T*>(g.bias), whole != 0);
   }
 }
 
@@ -324,7 +342,7 @@ int mx4_skinny(int out_dtype, const Mx4Args& g, hipStream_t st) {
   const int j = columns(g.N, g.kb, g.M > 4);
   return dispatch_float16_32(out_dtype, "mxfp4_mm", [&](auto tag) {
     using T = decltype(tag);
-    return g.M <= 4 ? run_skinny<T, void, 4>(g, j, st) : run_skinny<T, void, 16>(g, j, st);
+    return g.M <= 4 ? run_skinny<T, void, 4>(g, j, st) : g.M <= 16 ? run_skinny<T, void, 16>(g, j, st) : run_skinny<T, void, 32>(g, j, st);
   });
 }
 

@@ -144,6 +144,7 @@ def operands(m, n, k, dtype=torch.float32):
 SIZES = [
     (1, 1, 1), (1, 1, 32), (1, 16, 33), (2, 17, 256), (5, 100, 300), (16, 64, 1024), (17, 33, 96), (1, 4096, 768),
     (4, 1000, 4096), (8, 515, 2080), (16, 256, 8192), (33, 129, 512), (64, 300, 1600), (100, 1001, 2080), (128, 128, 256),
+    (17, 4100, 2080), (32, 300, 4096), (25, 20000, 1030), (31, 1, 64), (32, 5000, 8200), (20, 70001, 96),
     (129, 257, 288), (200, 640, 4096), (256, 512, 1024), (300, 1000, 544), (512, 512, 2048), (1000, 777, 1056),
 ]
 
