@@ -380,12 +380,15 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
     float mb = sm[row];
 #pragma unroll
     for (int w = 1; w < NW; ++w) mb = fmaxf(mb, sm[w * ROWS + row]);
-    // (a wave whose scores are all NaN has a NaN sum and no max)
-    const float f = m[x] == neg_inf() ? 0.f : fast_exp2(m[x] - mb);
+    // A row that sees none of the wave's keys has no max, and 0 whatever it met of
+    // the values: a NaN among them times P = 0 is NaN.  (One whose scores are all
+    // NaN has a NaN sum.)
+    const bool none = m[x] == neg_inf();
+    const float f = fast_exp2(m[x] - mb);
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) so[(wave * ROWS + row) * LD + t * 16 + 4 * g + e] = o[x][t][e] * f;
+      for (int e = 0; e < 4; ++e) so[(wave * ROWS + row) * LD + t * 16 + 4 * g + e] = none ? 0.f : o[x][t][e] * f;
   }
   __syncthreads();
   const int64_t nrow = static_cast<int64_t>(a.B) * a.Hq * a.Sq;

@@ -316,6 +316,13 @@ __global__ __launch_bounds__(256, blocks_per_cu(std::is_same<T, __bf16>::value, 
 
   l_i += __shfl_xor(l_i, 32, 64);
   if (!in_rows) return;
+  // A row that sees none of these keys is 0 whatever it met of the values: a NaN
+  // among them times P = 0 is NaN.  (One whose scores are all NaN has a NaN sum.)
+  const bool none = m_i == neg_inf();
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[t][e] = none ? 0.f : o[t][e];
   if (part) {
     const int64_t nrow = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
     const int64_t at = ((static_cast<int64_t>(b) * a.Hq + my_h) * a.Sq + my_q) * nsplit + sp;
