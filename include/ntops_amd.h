@@ -433,7 +433,8 @@ NTOPS_API int ntops_store_kv_cache(int dtype, int64_t B, int64_t H, int64_t S, i
 /* out (B, Hq, Sq, D) = softmax(q k^T * scale) v over the first lengths[b] (I32
  * or I64; NULL: C) tokens of sequence b's cache; lengths outside of 0 .. C count
  * as the nearer of the two.  causal 1: query row i sees the keys up to lengths[b]
- * - Sq + i.  A row that sees no key is 0.  Query head h reads cache head h /
+ * - Sq + i.  A row that sees no key is 0; a NaN value reaches the rows that see its
+ * token and no others.  Query head h reads cache head h /
  * (Hq / H).  Nothing behind a sequence's length is read.  fp32 sums; 16-bit q
  * with D a multiple of 16 up to 128 runs on the matrix cores (probabilities,
  * times the scale of their value block, rounded to bf16, for F16 to two bf16 parts), D <= 256 and F32 on a

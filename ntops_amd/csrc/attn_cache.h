@@ -38,6 +38,13 @@ __device__ __forceinline__ void pack_p(const float* x, u32x4& hi, u32x4& lo) {
   }
 }
 
+// 1 in every byte of w that is a NaN of e4m3 (all of its low 7 bits set).
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  return (((w & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
+}
+// Bits 0, 8, 16 and 24 as bits 0 .. 3.
+__device__ __forceinline__ uint32_t byte_bits(uint32_t w) { return (w * 0x01020408u) >> 24; }
+
 __device__ __forceinline__ int64_t length_of(const CacheAttnArgs& a, int b) {
   return max(int64_t(0), min(a.C, index_at(a.lengths, a.lengths_dtype, b, a.C)));
 }

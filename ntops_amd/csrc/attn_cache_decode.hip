@@ -23,6 +23,10 @@
 // bf16 holds them under scales of any size.  For f16 queries the rest of the
 // rounding is a second operand of the same product (pack_p).
 //
+// A NaN value reaches the rows that see it and no others, though P = 0 times it is
+// NaN: in a tile that not every row sees whole (several positions, causal), NaN codes
+// are noted for the rows that see them and cleared before the product.
+//
 // Slices are parts of the sequence's own length, known on the device only, so
 // the number of slices is set by the GPU's size and an empty slice leaves an
 // empty partial result.
@@ -318,6 +322,34 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
       wait_dma<2 * kTileInst>();
     else
       wait_dma<0>();
+    uint32_t nan[RB] = {};  // columns 16 t + 4 g + e (bit 4 t + e) that a NaN value reaches
+    if (lim_min < n && kt + NK > lim_min) {
+      char* own = const_cast<char*>(sv) + lane * 16;
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < kTileBytes / 1024; ++i) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(own + i * 1024);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) any |= nan_bytes(w[e]);
+      }
+      if (__any(any != 0)) {
+        for (int k = 0; k < NK; ++k) {
+          uint32_t bits = 0;
+#pragma unroll
+          for (int t = 0; t < DT; ++t)
+            bits |= byte_bits(nan_bytes(*reinterpret_cast<const uint32_t*>(sv + k * D + vslot8<D>(k, t) * 16 + 4 * g))) << (4 * t);
+#pragma unroll
+          for (int x = 0; x < RB; ++x) nan[x] |= kt + k < lim[x] ? bits : 0;
+        }
+        for (int i = 0; i < kTileBytes / 1024; ++i) {
+          u32x4 w = *reinterpret_cast<const u32x4*>(own + i * 1024);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] &= ~(nan_bytes(w[e]) * 0xffu);
+          *reinterpret_cast<u32x4*>(own + i * 1024) = w;
+        }
+        asm volatile("" ::: "memory");  // a wave's LDS operations run in order: written, then read by other lanes
+      }
+    }
     constexpr bool LO = std::is_same<T, _Float16>::value;
     u32x4 pf[RB][KB / 2], pl[RB][KB / 2];
 #pragma unroll
@@ -351,6 +383,15 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
           if constexpr (LO) o[x][t] = mfma16<__bf16>(vf, pl[x][p], o[x][t]);
         }
       }
+    if (lim_min < n && kt + NK > lim_min)
+#pragma unroll
+      for (int x = 0; x < RB; ++x)
+        if (__any(nan[x] != 0))
+#pragma unroll
+          for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (nan[x] >> (4 * t + e) & 1) o[x][t][e] = __builtin_nanf("");
     wait_lgkmcnt0();
     issue_v(j + 2);
   }
@@ -381,8 +422,7 @@ __global__ __launch_bounds__(64 * NW, 1) void k_cache_decode(CacheAttnArgs a, in
 #pragma unroll
     for (int w = 1; w < NW; ++w) mb = fmaxf(mb, sm[w * ROWS + row]);
     // A row that sees none of the wave's keys has no max, and 0 whatever it met of
-    // the values: a NaN among them times P = 0 is NaN.  (One whose scores are all
-    // NaN has a NaN sum.)
+    // the values.  (One whose scores are all NaN has a NaN sum.)
     const bool none = m[x] == neg_inf();
     const float f = fast_exp2(m[x] - mb);
 #pragma unroll

@@ -6,7 +6,8 @@ reads a cache of the query's type).  query (batch, query heads, tokens, head_dim
 attends the first lengths[b] tokens of sequence b (int32 or int64 (batch,);
 None: the whole capacity; query head h reads cache head h // (query heads / cache
 heads)).  With is_causal the last query row is the sequence's last token: row i
-sees the keys up to lengths[b] - tokens + i.  A row that sees no key is 0.
+sees the keys up to lengths[b] - tokens + i.  A row that sees no key is 0; a
+NaN value reaches the rows that see its token and no others.
 scale defaults to 1 / sqrt(head_dim).  float16, bfloat16 or float32 queries, head
 dims up to 256; 16-bit queries of head dims that are multiples of 16 up to 128
 run on the matrix cores."""

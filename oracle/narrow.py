@@ -91,7 +91,8 @@ def store_kv_cache(new, cache, scale, positions, lengths, block):
 
 
 def kv_cache_attention(q, k, v, k_scale, v_scale, lengths, block, causal, scale):
-    """q (B, Hq, Sq, D), k and v (B, Hkv, C, D) in units of their scales."""
+    """q (B, Hq, Sq, D), k and v (B, Hkv, C, D) in units of their scales.  A NaN of v
+    reaches the rows that see its token."""
     q = np.asarray(q, np.float64)
     B, Hq, Sq, D = q.shape
     group = Hq // k.shape[1]
@@ -108,6 +109,8 @@ def kv_cache_attention(q, k, v, k_scale, v_scale, lengths, block, causal, scale)
             top = s.max(-1, keepdims=True, initial=-np.inf)
             p = np.exp(s - np.where(np.isneginf(top), 0.0, top))
             total = p.sum(-1, keepdims=True)
+            bad = np.isnan(vv)  # reaches the rows that see it
             with np.errstate(invalid="ignore", divide="ignore"):
-                out[b, h] = np.where(total == 0, 0.0, p @ vv / total)
+                mean = np.where((seen @ bad.astype(np.float64)) > 0, np.nan, p @ np.where(bad, 0.0, vv) / total)
+            out[b, h] = np.where(total == 0, 0.0, mean)
     return out

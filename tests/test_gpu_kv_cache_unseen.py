@@ -46,3 +46,30 @@ def test_rows_that_see_nothing_are_zero(b, hq, h, sq, c, d, block, kernel, dtype
         assert torch.isnan(out[i, :, sq - n :, d // 2 :]).all() and torch.isnan(out[i, :, sq - n :, 0]).all()
     again = nt.kv_cache_attention(query.float(), *caches, lengths.cuda(), True, block_size=block)
     assert torch.equal(torch.isnan(out), torch.isnan(again))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("b,hq,h,sq,c,d,block,kernel", KERNELS)
+def test_nan_values_reach_the_rows_that_see_them(b, hq, h, sq, c, d, block, kernel, dtype, causal):
+    """All else is, bit for bit, what zeros in their place give."""
+    caches = cache(b, h, c, d, block)
+    lengths = [(c, min(c, sq + c // 2), sq // 2 + 1, min(c, sq + 3))[i % 4] for i in range(b)]
+    query = torch.randn(b, hq, sq, d).to(dtype).cuda()
+    # (sequence, token, columns) of the last cache head: the last token, one that about
+    # half of the rows see, and an early one
+    bad = [(i, max(0, n - 1 - back), at) for i, n in enumerate(lengths) for back, at in ((0, slice(0, 1)), ((sq - 1) // 2, slice(d // 2, d // 2 + 9)), (c, slice(d - 1, d)))]
+    codes = caches[1].view(torch.uint8)
+    for i, t, at in bad:
+        codes[i, h - 1, t, at] = 0
+    n = torch.tensor(lengths).cuda()
+    want = nt.kv_cache_attention(query, *caches, n, causal, block_size=block)
+    assert kernel in _lib.last_kernel(), _lib.last_kernel()
+    assert torch.isfinite(want).all()
+    for i, t, at in bad:
+        codes[i, h - 1, t, at] = 127 + 128 * (i % 2)
+        first = max(0, t - lengths[i] + sq) if causal else 0
+        want[i, hq - hq // h :, first:, at] = float("nan")
+    out = nt.kv_cache_attention(query, *caches, n, causal, block_size=block)
+    assert torch.equal(torch.isnan(out), torch.isnan(want))
+    assert torch.equal(out.nan_to_num(), want.nan_to_num())
