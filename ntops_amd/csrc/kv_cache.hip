@@ -374,8 +374,10 @@ extern "C" int ntops_store_kv_cache(int dtype, int64_t B, int64_t H, int64_t S, 
     a.units = std::min(ceil_div(S - 1, block) + 1, ceil_div(C, block));
     if (B > 65535 || H > 65535 || a.units > (1 << 24))
       return set_error(NTOPS_ERR_UNSUPPORTED, "store_kv_cache: over 65535 sequences or heads, or too many tokens");
-    // a lane's registers hold kSlots packs; of single values a wave takes a few turns
-    const bool wide = std::min(block, S) * D > (vec ? kSlots * 64 * 8 : 8 * 64);
+    // a lane's registers hold kSlots packs; of single values a wave takes a few turns;
+    // two of eight waves for each block have to be under the 2^32 threads of a grid's x
+    // dimension (2^24 of one for keys and one for values are)
+    const bool wide = std::min(block, S) * D > (vec ? kSlots * 64 * 8 : 8 * 64) && a.units * (2 * 64 * kWide) < (int64_t(1) << 32);
     const dim3 grid(static_cast<unsigned>(a.units * (wide ? 2 : 1)), static_cast<unsigned>(H), static_cast<unsigned>(B));
     const auto kern = vec ? (wide ? &k_store_kv_cache<T, kWide> : &k_store_kv_cache<T, 1>)
                           : (wide ? &k_store_kv_cache_any<T, kWide> : &k_store_kv_cache_any<T, 1>);
