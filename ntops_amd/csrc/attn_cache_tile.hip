@@ -202,9 +202,9 @@ __global__ __launch_bounds__(256, blocks_per_cu(std::is_same<T, __bf16>::value, 
     constexpr int S = decltype(set)::value;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-      // at least a tiny factor, so that a masked score (-inf) stays one under a zero scale
+      // at least the least factor there is, so that a masked score (-inf) stays one under a zero scale
       const float x = lane_read(kscale[S], p) * c0, y = lane_read(vscale[S], p);
-      c[p] = x < 0x1p-120f ? 0x1p-120f : x;
+      c[p] = x < 0x1p-149f ? 0x1p-149f : x;
       f[p] = y < 0x1p-126f ? 0.f : __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, y) & 0x7fffffu) | 0x3f800000u);
     }
   };
