@@ -434,10 +434,13 @@ NTOPS_API int ntops_store_kv_cache(int dtype, int64_t B, int64_t H, int64_t S, i
  * or I64; NULL: C) tokens of sequence b's cache; lengths outside of 0 .. C count
  * as the nearer of the two.  causal 1: query row i sees the keys up to lengths[b]
  * - Sq + i.  A row that sees no key is 0; a NaN value reaches the rows that see its
- * token and no others.  Query head h reads cache head h /
- * (Hq / H).  Nothing behind a sequence's length is read.  fp32 sums; 16-bit q
- * with D a multiple of 16 up to 128 runs on the matrix cores (probabilities,
- * times the scale of their value block, rounded to bf16, for F16 to two bf16 parts), D <= 256 and F32 on a
+ * token and no others.  Query head h reads cache head h / (Hq / H).  Nothing behind a
+ * sequence's length is read.  Scales are not negative (the store writes powers of
+ * two; results under negative ones differ between the kernels).  Sums are fp32: q
+ * times the codes before their scale, and values weighted with up to 2^8 before they
+ * are normalized, have to lie in its range.  16-bit q with D a multiple of 16 up to
+ * 128 runs on the matrix cores (probabilities, with what they carry of their value
+ * block's scale, rounded to bf16, for F16 to two bf16 parts), D <= 256 and F32 on a
  * kernel of one wave per row.  The workspace (16-byte aligned; may be NULL)
  * spreads the keys of few query rows over the GPU. */
 NTOPS_API int ntops_kv_cache_attention(int dtype, int64_t B, int64_t Hq, int64_t H, int64_t Sq, int64_t C, int64_t D,

@@ -8,6 +8,7 @@ None: the whole capacity; query head h reads cache head h // (query heads / cach
 heads)).  With is_causal the last query row is the sequence's last token: row i
 sees the keys up to lengths[b] - tokens + i.  A row that sees no key is 0; a
 NaN value reaches the rows that see its token and no others.
+Scales of the cache are not negative.
 scale defaults to 1 / sqrt(head_dim).  float16, bfloat16 or float32 queries, head
 dims up to 256; 16-bit queries of head dims that are multiples of 16 up to 128
 run on the matrix cores."""
