@@ -147,10 +147,9 @@ struct Ring {
   static constexpr int kStepB = LB::kBytes + LB::kScaleBytes;
   static constexpr int kStep = kStepB + LA::kBytes + LA::kScaleBytes;
   static constexpr int kOwn = kRaw ? LC::kBytes + LC::kScaleBytes : 0;
-  static constexpr int kFit = (163840 / 2 / kWaves - kOwn) / kStep;  // two blocks a CU
-  static constexpr int S = kFit < 4 ? kFit : 4;
+  static constexpr int S = (163840 / 2 / kWaves - kOwn) / kStep;  // two blocks a CU
   static constexpr int kLds = kWaves * (S * kStep + kOwn);
-  static_assert(S >= 1 && kLds >= kWaves * J * (MR > 16 ? MR / 16 : 1) * 1024, "a step, and the sums to merge");
+  static_assert(S >= 1 && S <= 3 && kLds >= kWaves * J * (MR > 16 ? MR / 16 : 1) * 1024, "a step, and the sums to merge");
 };
 
 template <typename T, typename X, int J, int MR>
@@ -219,8 +218,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_mx4_skinny(Mx4Args g, int wh
     const int behind = n - 1 - i;
     if (behind >= S - 1)
       wait_vmcnt<(S - 1) * kInst>();
-    else if (S > 3 && behind == 2)
-      wait_vmcnt<2 * kInst>();
     else if (S > 2 && behind == 1)
       wait_vmcnt<kInst>();
     else
