@@ -305,23 +305,34 @@ int launch_skinny(const Mx4Args& g, hipStream_t st) {
 
 template <typename T, typename X, int MR>
 int run_skinny(const Mx4Args& g, int j, hipStream_t st) {
-  return j == 4   ? launch_skinny<T, X, 4, MR>(g, st)
-         : j == 2 ? launch_skinny<T, X, 2, MR>(g, st)
-                  : launch_skinny<T, X, 1, MR>(g, st);
+  if constexpr (MR <= 16)
+    if (j == 4) return launch_skinny<T, X, 4, MR>(g, st);
+  return j == 2 ? launch_skinny<T, X, 2, MR>(g, st) : launch_skinny<T, X, 1, MR>(g, st);
 }
 
 // Columns of a block, in 16s.  A CU's blocks, counted in halves as two run at once
 // and one alone has the CU's bandwidth, cost their bytes and their starts, as much
 // as 20 KiB of B each.  A ring of one step (lone) needs the CU's other block to
-// cover its waits; two columns give the same sums as four.
-// Measured with 1, 2 and 4 (us, with empty loads past a wave's last step, which are
-// gone): 1 row, 4096 x 4096 4.8, 5.3, 7.1; 14336 x 4096
-// 11.2, 9.6, 9.2; 100000 x 4096 52.4, 42.0, 38.7; 24000 x 2048 12.1, 10.5, 9.4;
-// 8 rows, 14336 x 4096 12.3, 9.9, 11.0; 16 rows, 100000 x 4096 60.4, 47.7, 45.4.
-int columns(int64_t N, int64_t kb, bool lone) {
+// cover its waits; two columns give the same sums as four.  From 17 rows on only two
+// have a ring of more than one step, and are taken wherever a CU would get a second
+// block of one.  Measured with 1, 2 and 4 in one graph over weights from memory (us):
+//                    1 row, rounded here  1 row             16 rows           32 rows
+//   4096 x 4096       5.2,  6.0,  9.5      4.4,  4.8,  6.6   4.8,  5.4,  8.4   5.9,  6.3,  9.5
+//   4096 x 14336      9.0, 12.3, 22.7      7.6,  9.6, 17.3   9.2, 12.7, 22.5  12.5, 16.0, 26.6
+//   6144 x 4096       6.3,  6.2,  9.7      5.3,  5.0,  6.9   6.1,  5.7,  8.6   7.8,  6.7,  9.8
+//   14336 x 4096     10.4,  9.3, 11.3      8.9,  7.8,  8.3  10.3,  9.0,  9.9  13.3, 10.8, 11.1
+//   14336 x 14336    24.0, 22.7, 27.0     21.4, 21.3, 22.7  26.6, 26.4, 26.7  36.5, 32.3, 30.8
+//   24000 x 2048     10.3,  8.8,  8.7      9.2,  7.9,  7.7   9.8,  8.2,  8.7  11.8,  9.5,  9.9
+//   28672 x 4096     16.9, 15.3, 14.6     14.9, 13.4, 13.1  17.6, 15.4, 15.4  23.4, 18.2, 17.5
+//   100000 x 4096    54.0, 42.3, 40.9     46.0, 37.1, 37.5  55.2, 43.8, 46.5  70.7, 53.1, 52.9
+// Starts of 44 KiB would take two columns in the third and fifth row, and four at
+// 18944 x 3584, which lose up to 14 % there; without four from 5 rows on 49152 x 1536
+// of 16 rows took 11.9 instead of 10.3.
+int columns(int64_t M, int64_t N, int64_t kb, bool lone) {
   int best = 1;
   int64_t least = 0;
   const int64_t cus = cu_count_cached();
+  if (M > 16) return ceil_div(N, 16) <= cus ? 1 : 2;
   for (int j = 1; j <= 4; j *= 2) {
     const int64_t halves = std::max<int64_t>(2, ceil_div(2 * ceil_div(N, 16 * j), cus));
     const int64_t cost = halves * (20 * 1024 + 16 * j * kb * 17);
@@ -336,7 +347,7 @@ int columns(int64_t N, int64_t kb, bool lone) {
 }  // namespace
 
 int mx4_skinny(int out_dtype, const Mx4Args& g, hipStream_t st) {
-  const int j = columns(g.N, g.kb, g.M > 4);
+  const int j = columns(g.M, g.N, g.kb, g.M > 4);
   return dispatch_float16_32(out_dtype, "mxfp4_mm", [&](auto tag) {
     using T = decltype(tag);
     return g.M <= 4 ? run_skinny<T, void, 4>(g, j, st) : g.M <= 16 ? run_skinny<T, void, 16>(g, j, st) : run_skinny<T, void, 32>(g, j, st);
@@ -344,7 +355,7 @@ int mx4_skinny(int out_dtype, const Mx4Args& g, hipStream_t st) {
 }
 
 int mx4_skinny_fused(int x_dtype, int out_dtype, const Mx4Args& g, hipStream_t st) {
-  const int j = columns(g.N, g.kb, true);
+  const int j = columns(g.M, g.N, g.kb, true);
   return dispatch_float16_32(out_dtype, "mxfp4_mm", [&](auto tag) {
     using T = decltype(tag);
     return x_dtype == NTOPS_BF16 ? run_skinny<T, __bf16, kFusedRows>(g, j, st) : run_skinny<T, _Float16, kFusedRows>(g, j, st);
