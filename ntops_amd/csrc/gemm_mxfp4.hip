@@ -282,11 +282,15 @@ bool scales_fit(int64_t kb, const void* s, int64_t ld) {
   return kb % 8 == 0 && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(s) & 3u) == 0;
 }
 
-// 256 x 256 tiles where 128 x 128 ones, two a CU, are more than a round of the GPU:
-// (1500, 6000, 8192) bf16 58.2 us, on 128 x 128 tiles 73.2; (3000, 3000, 3000) 32.5 and
-// 34.2; (4096, 8192, 1400) 43.4 and 47.1; but one round of those, (2048, 4096, 4096),
-// 33.0 and 27.7, (1024, 4352, 8192) 51.3 and 41.7, (2048, 4096, 14336) 84.8 and 88.4.
-// Up to 128 rows they are half empty: (128, 100000, 4096) 80.4 and 78.4.
+// 256 x 256 tiles where 128 x 128 ones, two a CU, are more than a round of the GPU.
+// Measured on 128 x 128 and on 256 x 256 (bf16, us): one round, (2048, 4096) over 4096
+// 28.8 and 33.9, over 14336 81.5 and 81.5, (1024, 8192) over 14336 82.2 and 84.1, (256,
+// 28672) over 14336 104 and 97; more, (1536, 6144) over 4096 38.1 and 34.1, over 14336
+// 114 and 83, (4096, 4096) over 2048 30.8 and 29.2, over 4096 50.8 and 41.6, (8192,
+// 14336) over 1056 155 and 130, over 2048 201 and 159.  It goes by tiles alone, and so
+// wrong over short rows: (1536, 6144) over 1056 19.3 and 23.4, over 2048 23.6 and 25.2,
+// (4096, 5120), a quarter of a second round of 256 x 256, over 2048 35.6 and 43.5.
+// Up to 128 rows those are half empty: (128, 100000) over 4096 69.2 and 81.6.
 bool large_suits(int64_t M, int64_t N) { return M > 128 && ceil_div(M, 128) * ceil_div(N, 128) > 2 * cu_count_cached(); }
 
 // The tile's size and the slices of K: as many slices as bring the blocks near the
