@@ -22,8 +22,12 @@ struct CacheAttnArgs {
   float scale_log2;      // scale * log2(e)
 };
 
-// 8 probabilities as bf16 operands: rounded, and for f16 queries, whose results
-// keep 11 bits, what the rounding left as a second operand (17 bits in all).
+// 8 probabilities as bf16 operands: rounded, as the 16-bit attention of this library
+// rounds them, and for f16 queries, whose results keep 11 bits, what the rounding left
+// as a second operand (17 bits in all).  Against 64 bits, relative to the whole result:
+// bf16 prompts (4, 32 / 8, 2048 over 2048, 128) 0.0017, with fp32 probabilities, of
+// which only the result's own rounding is left, 0.0014; (16, 32 / 8, 1 over 2048 ..
+// 4096, 128) 0.0015 and 0.0015; f16 prompts 0.00018 and 0.00018.
 template <bool LO>
 __device__ __forceinline__ void pack_p(const float* x, u32x4& hi, u32x4& lo) {
   hi = pack8<__bf16>(x);

@@ -6,6 +6,10 @@
 // are refilled one by one, the two waves of a SIMD half a phase apart, and a
 // finished quadrant leaves between the next tile's MFMAs.  K is a quarter as many
 // tiles as for 16 bits, so what surrounds the K loop weighs four times as much.
+// In an output tile's first K tile, where the previous one leaves, the compiler keeps
+// 16 to 20 registers in scratch (52 to 68 bytes a lane; gemm_large.hip's kernel none):
+// up to four reloads between its MFMAs, each behind a wait for all of the wave's memory
+// operations, so that there the loads do not run ahead and the stores are waited for.
 //
 // Scales, a byte per 32 values, ride along, 4 KiB a K tile, in a ring of three.  A
 // kernel before this one lays them out by (256 rows, K tile), and within these 2
