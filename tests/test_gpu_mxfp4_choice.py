@@ -30,3 +30,21 @@ def test_columns_of_17_to_32_rows(m, n, k, kernel):
     v = [np.abs(N.dequantize_mxfp4(*operands[i : i + 2])) for i in (0, 2)]
     # fp32 sums of k exact products, in any order
     assert (np.abs(out.double().cpu().numpy() - want) <= (k + 8) * 2.0**-24 * (v[0] @ v[1].T) + 2.0**-140).all()
+
+
+@pytest.mark.parametrize("m", [1, 16, 17])
+def test_as_many_columns_as_are_allowed(m):
+    """One row of the weight for all of them: their blocks come near the threads of a grid."""
+    n = 64 * 0x7FFFFF
+    a, sa = nt.quantize_mxfp4(torch.randn(m, 32, device="cuda"))
+    b, sb = nt.quantize_mxfp4(torch.randn(1, 32, device="cuda"))
+    want = nt.mxfp4_mm(a, sa, b, sb)
+    try:
+        out = nt.mxfp4_mm(a, sa, b.expand(n, -1), sb.expand(n, -1))
+        assert "skinny" in _lib.last_kernel(), _lib.last_kernel()
+        assert all(bool((part == want).all()) for part in out.split(1 << 26, 1))
+        with pytest.raises(RuntimeError, match="too large"):
+            nt.mxfp4_mm(a, sa, b.expand(n + 1, -1), sb.expand(n + 1, -1))
+    finally:
+        out = None
+        torch.cuda.empty_cache()
