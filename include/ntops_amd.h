@@ -458,6 +458,54 @@ NTOPS_API int ntops_kv_cache_attention(int dtype, int64_t B, int64_t Hq, int64_t
 NTOPS_API int64_t ntops_kv_cache_attention_workspace(int dtype, int64_t B, int64_t Hq, int64_t H, int64_t Sq,
                int64_t C, int64_t D);
 
+/* ---- attention over long and shared contexts ------------------------------- */
+/* O (B, Hq, Sq, D) = softmax(scale * Q K^T) V in a sliding window: query row i of
+ * sequence b is its token p = lengths[b] - Sq + i and sees the keys j <= p with
+ * j > p - window or j < sinks (the first tokens, which stay visible).  K and V
+ * (B, Hkv, C, D) are of Q's type, query head h reads key / value head
+ * h / (Hq / Hkv).  lengths (B values, I32 or I64 by lengths_dtype; NULL: C tokens
+ * each) are read on the device and cut to 0 .. C; keys that no row sees are not
+ * read.  A row that sees no key is 0, and what a row does not see does not reach
+ * it, whatever it holds.  window >= 1, sinks >= 0.  fp32 statistics and sums; F16
+ * and BF16 with D a multiple of 8 up to 128, unit strides along D and rows at
+ * multiples of 16 bytes run on the matrix cores (probabilities rounded to the
+ * type), other layouts, D <= 256 and F32 on a kernel of one wave per row.  The
+ * workspace (16-byte aligned; may be NULL) spreads the keys of few query rows over
+ * the GPU. */
+NTOPS_API int ntops_sliding_window_attention(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t C, int64_t D,
+               const void* q, const int64_t* q_strides,
+               const void* key, const int64_t* key_strides,
+               const void* value, const int64_t* value_strides,
+               const void* lengths, int lengths_dtype, int64_t window, int64_t sinks, double scale,
+               void* out, const int64_t* out_strides,
+               void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace ntops_sliding_window_attention uses for this problem on the
+ * current device (0: none). */
+NTOPS_API int64_t ntops_sliding_window_attention_workspace(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq,
+               int64_t C, int64_t D, int64_t window, int64_t sinks);
+
+/* The same over a prefix that sequences share: sequences b of group b / (B / G) see
+ * the first prefix_lengths[group] of its P prefix tokens (prefix_key and
+ * prefix_value (G, Hkv, P, D)) and, row i, their own keys up to
+ * lengths[b] - Sq + i.  The prefix is read once for all rows of a group where that
+ * saves more than joining the two parts costs. */
+NTOPS_API int ntops_shared_prefix_attention(int dtype, int64_t G, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq,
+               int64_t P, int64_t C, int64_t D, const void* q, const int64_t* q_strides,
+               const void* prefix_key, const int64_t* prefix_key_strides,
+               const void* prefix_value, const int64_t* prefix_value_strides,
+               const void* prefix_lengths, int prefix_lengths_dtype,
+               const void* key, const int64_t* key_strides,
+               const void* value, const int64_t* value_strides,
+               const void* lengths, int lengths_dtype, double scale,
+               void* out, const int64_t* out_strides,
+               void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace ntops_shared_prefix_attention uses for this problem on the
+ * current device (0: none). */
+NTOPS_API int64_t ntops_shared_prefix_attention_workspace(int dtype, int64_t G, int64_t B, int64_t Hq, int64_t Hkv,
+               int64_t Sq, int64_t P, int64_t C, int64_t D);
+
 /* ---- fused variants ------------------------------------------------------- */
 /* residual_out = x + residual (rounded to dtype) and y = rms_norm(residual_out)
  * over rows x cols with the conventions of ntops_rms_norm (weight of dtype or
@@ -482,6 +530,24 @@ NTOPS_API int ntops_rope_qk(int dtype, int64_t B, int64_t S, int64_t Hq, int64_t
                const void* k, const int64_t* k_strides,
                const void* sin_table, const void* cos_table,
                int64_t table_row_stride, int64_t table_cols, int interleaved,
+               void* q_out, const int64_t* q_out_strides,
+               void* k_out, const int64_t* k_out_strides, void* stream);
+
+/* Rotary positions with several axes on q (B, S, Hq, D) and k (B, S, Hk, D) (either
+ * head count may be 0): pair i -- elements (i, i + D / 2), or (2 i, 2 i + 1)
+ * interleaved -- is rotated by the angle of row positions[axis][b][s] of the tables,
+ * where section s of `sections`, which add up to D / 2, belongs to axis s % axes.
+ * positions (axes, B, S) by 3 element strides, I32 or I64, are read on the device; a
+ * pair whose position lies outside of the table_rows rows is NaN.  Tables of F32 or
+ * of dtype, of D / 2 columns (column i) or D (each element its own).  fp32, one
+ * rounding.  D <= 512.  In place per tensor with equal strides. */
+NTOPS_API int ntops_rope_axes_qk(int dtype, int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D,
+               const void* q, const int64_t* q_strides,
+               const void* k, const int64_t* k_strides,
+               int table_dtype, const void* sin_table, int64_t sin_row_stride,
+               const void* cos_table, int64_t cos_row_stride, int64_t table_rows, int64_t table_cols,
+               int64_t axes, const void* positions, int positions_dtype, const int64_t* position_strides,
+               int64_t n_sections, const int64_t* sections, int interleaved,
                void* q_out, const int64_t* q_out_strides,
                void* k_out, const int64_t* k_out_strides, void* stream);
 

@@ -145,6 +145,21 @@ _SIGNATURES = {
         [_i] + [_i64] * 7 + [_vp, _c_i64p] * 5 + [_vp, _i, _i, _d, _vp, _c_i64p, _vp, _i64, _vp],
     ),
     "ntops_kv_cache_attention_workspace": (_i64, [_i] + [_i64] * 6),
+    "ntops_sliding_window_attention": (
+        _i,
+        [_i] + [_i64] * 6 + [_vp, _c_i64p] * 3 + [_vp, _i, _i64, _i64, _d, _vp, _c_i64p, _vp, _i64, _vp],
+    ),
+    "ntops_sliding_window_attention_workspace": (_i64, [_i] + [_i64] * 8),
+    "ntops_shared_prefix_attention": (
+        _i,
+        [_i] + [_i64] * 8 + [_vp, _c_i64p] * 3 + [_vp, _i] + [_vp, _c_i64p] * 2 + [_vp, _i, _d, _vp, _c_i64p, _vp, _i64, _vp],
+    ),
+    "ntops_shared_prefix_attention_workspace": (_i64, [_i] + [_i64] * 8),
+    "ntops_rope_axes_qk": (
+        _i,
+        [_i] + [_i64] * 5 + [_vp, _c_i64p] * 2 + [_i, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i, _c_i64p, _i64, _c_i64p, _i]
+        + [_vp, _c_i64p] * 2 + [_vp],
+    ),
 }
 
 EXPORTED = tuple(_SIGNATURES)

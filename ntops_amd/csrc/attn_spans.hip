@@ -1,0 +1,288 @@
+// sliding_window_attention and shared_prefix_attention: the kernel for any head
+// dim and layout, the merge of partial results, and the C entry points.
+//
+//   O = softmax(scale Q K^T) V over the keys that a row sees.  Row t of a sequence
+//   of n tokens is its token p = n - Sq + t.
+//     window: keys j <= p with j > p - window or j < sinks
+//     prefix: every key of the prefix, and its own sequence's keys j <= p
+//   A row that sees no key is 0.
+#include <algorithm>
+
+#include "attn_spans.h"
+
+namespace ntops {
+namespace {
+
+constexpr int kMaxDim = 256;
+constexpr int kMaxSlices = 64;
+constexpr int64_t kMaxCount = 0x7fffffff;
+
+// One wave per query row and slice of what it sees (front and main keys in equal
+// parts of both).
+template <typename T, int EL>
+__global__ __launch_bounds__(256) void k_span_rows(SpanArgs a, int mode, int slices, SpanPart part, int64_t total) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t id = block_id() * 4 + wave;
+  if (id >= total) return;
+  const int64_t rows = static_cast<int64_t>(a.Hq / a.Hkv) * a.Sq * (mode == kFront ? a.B / a.G : 1);
+  const int slice = static_cast<int>(id % slices);
+  const int64_t at = id / slices, set = at / rows;
+  const int r = static_cast<int>(at - set * rows);
+  const int t = r / (a.Hq / a.Hkv) % a.Sq;
+  const Spans s = make_spans<sizeof(T)>(a, mode, set, t, t);
+  const SpanRow x = span_row(a, s, r);
+  const int fc = (s.n[0] + slices - 1) / slices, mc = (s.n[1] + slices - 1) / slices;
+  float o[EL], m, l;
+  span_attend_row<T, EL>(a, s, x, min(slice * fc, s.n[0]), min(slice * fc + fc, s.n[0]), min(slice * mc, s.n[1]), min(slice * mc + mc, s.n[1]),
+                         o, m, l);
+  span_write_row<T, EL>(a, part, x, slice, o, m, l);
+}
+
+// Combines the slices of every query row in slice order: one wave per row, W lanes
+// a slice and 64 / W slices side by side.
+template <typename T, int W>
+__global__ __launch_bounds__(256) void k_span_merge(SpanArgs a, SpanPart part) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = block_id() * 4 + (threadIdx.x >> 6);
+  if (row >= static_cast<int64_t>(a.B) * a.Hq * a.Sq) return;
+  constexpr int NS = 64 / W;
+  const int d = (lane % W) * 4, g = lane / W;
+  float m = neg_inf(), l = 0.f;
+  if (lane < part.slices) {
+    const float* ml = part.ml(a, row * part.slices + lane);
+    m = ml[0];
+    l = ml[1];
+  }
+  const float mm = wave_max(m);
+  const float w = m == neg_inf() ? 0.f : fast_exp2(m - mm);
+  const float sum = wave_sum(l * w);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < part.slices; s0 += NS) {
+    const int s = s0 + g;
+    const float ws = __shfl(w, s & 63, 64);
+    // (a slice of weight 0 holds nothing that the row has seen, or nothing beside the others)
+    if (s < part.slices && d < part.ld && ws != 0.f)
+      o += ws * *reinterpret_cast<const f32x4*>(part.row(row * part.slices + s) + d);
+  }
+#pragma unroll
+  for (int step = W; step < 64; step <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], step, 64);
+  if (g != 0) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int t = static_cast<int>(row % a.Sq);
+  const int64_t bh = row / a.Sq;
+  T* O = static_cast<T*>(a.o) + (bh / a.Hq) * a.ost[0] + (bh % a.Hq) * a.ost[1] + t * a.ost[2];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (d + e < a.D) O[(d + e) * a.ost[3]] = static_cast<T>(o[e] * inv);
+}
+
+int merge(int dtype, const SpanArgs& a, const SpanPart& part, hipStream_t st) {
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
+  return dispatch_float16_32(dtype, "attention", [&](auto tag) {
+    using T = decltype(tag);
+    const dim3 grid = blocks_2d(ceil_div(rows, 4)), block(256);
+    if (part.ld <= 64)
+      hipLaunchKernelGGL((k_span_merge<T, 16>), grid, block, 0, st, a, part);
+    else if (part.ld <= 128)
+      hipLaunchKernelGGL((k_span_merge<T, 32>), grid, block, 0, st, a, part);
+    else
+      hipLaunchKernelGGL((k_span_merge<T, 64>), grid, block, 0, st, a, part);
+    return check_launch("attention");
+  });
+}
+
+template <typename T, int EL>
+int launch_rows(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
+  const int64_t total = static_cast<int64_t>(a.B) * a.Hq * a.Sq * slices;
+  hipLaunchKernelGGL((k_span_rows<T, EL>), blocks_2d(ceil_div(total, 4)), dim3(256), 0, st, a, mode, slices, part, total);
+  return check_launch("attention");
+}
+
+// How a problem is served: how many slices of the keys, in which launches.
+struct Plan {
+  int slices;  // of rows over all their keys
+};
+
+// Most keys that a row sees.
+int64_t most_keys(const SpanArgs& a) {
+  return a.P + std::min<int64_t>(a.C, static_cast<int64_t>(a.window) + a.sinks);
+}
+
+Plan make_plan(int dtype, const SpanArgs& a) {
+  (void)dtype;
+  Plan p;
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
+  p.slices = static_cast<int>(std::max<int64_t>(1, std::min({static_cast<int64_t>(kMaxSlices), cu_count_cached() * 8 / rows, most_keys(a) / 128})));
+  return p;
+}
+
+int64_t plan_bytes(const SpanArgs& a, const Plan& p) {
+  if (p.slices <= 1) return 0;
+  return static_cast<int64_t>(a.B) * a.Hq * a.Sq * p.slices * ((a.D + 3) / 4 * 4 + 2) * 4;
+}
+
+int run(int dtype, const SpanArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
+  Plan p = make_plan(dtype, a);
+  if (ws == nullptr || ws_bytes < plan_bytes(a, p)) p.slices = 1;
+  SpanPart part{p.slices > 1 ? static_cast<float*>(ws) : nullptr, p.slices, 0, (a.D + 3) / 4 * 4};
+  if (int e = span_rows_run(dtype, a, kBoth, p.slices, part, st)) return e;
+  return part.p ? merge(dtype, a, part, st) : NTOPS_OK;
+}
+
+bool sizes_fit(int64_t B, int64_t Hq, int64_t Sq, int64_t C, int64_t P) {
+  return B <= kMaxCount && Hq <= kMaxCount && Sq <= kMaxCount / 2 && C <= kMaxCount / 2 && P <= kMaxCount / 2 && B * Hq <= kMaxCount &&
+         B * Hq * Sq <= kMaxCount;
+}
+
+}  // namespace
+
+int span_rows_run(int dtype, const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
+  note_kernel("%s rows split%d", a.pk ? "shared_prefix" : "sliding_window", slices);
+  return dispatch_float16_32(dtype, "attention", [&](auto tag) {
+    using T = decltype(tag);
+    if (a.D <= 64) return launch_rows<T, 4>(a, mode, slices, part, st);
+    if (a.D <= 128) return launch_rows<T, 8>(a, mode, slices, part, st);
+    return launch_rows<T, 16>(a, mode, slices, part, st);
+  });
+}
+
+}  // namespace ntops
+
+using namespace ntops;
+
+namespace {
+
+// Checks what both operators share, and fills in the arguments.
+int span_args(const char* what, SpanArgs& a, int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t C, int64_t D,
+              int64_t P, const void* q, const int64_t* q_strides, const void* key, const int64_t* key_strides,
+              const void* value, const int64_t* value_strides, const void* lengths, int lengths_dtype, double scale, void* out,
+              const int64_t* out_strides, void* workspace, int64_t workspace_bytes) {
+  if (dtype != NTOPS_F32 && dtype != NTOPS_F16 && dtype != NTOPS_BF16)
+    return set_error(NTOPS_ERR_UNSUPPORTED, "%s: unsupported dtype %d (F32/F16/BF16 only)", what, dtype);
+  if (lengths && !index_dtype(lengths_dtype)) return set_error(NTOPS_ERR_INVALID, "%s: lengths are I32 or I64", what);
+  if (Hkv <= 0 || Hq % Hkv != 0)
+    return set_error(NTOPS_ERR_INVALID, "%s: query heads are not a multiple of key / value heads", what);
+  if (!q || !out || !q_strides || !out_strides || (C > 0 && (!key || !value || !key_strides || !value_strides)))
+    return set_error(NTOPS_ERR_INVALID, "%s: null pointer", what);
+  if (D > kMaxDim) return set_error(NTOPS_ERR_UNSUPPORTED, "%s: head dim over %d", what, kMaxDim);
+  if (!sizes_fit(B, Hq, Sq, C, P)) return set_error(NTOPS_ERR_UNSUPPORTED, "%s: problem too large", what);
+  if (workspace_bytes < 0 || (workspace != nullptr && !aligned16(workspace)))
+    return set_error(NTOPS_ERR_INVALID, "%s: workspace not aligned to 16 bytes", what);
+  a.q = q;
+  a.o = out;
+  a.k = key;
+  a.v = value;
+  for (int i = 0; i < 4; ++i) {
+    a.qst[i] = q_strides[i];
+    a.ost[i] = out_strides[i];
+    if (C > 0) {
+      a.kst[i] = key_strides[i];
+      a.vst[i] = value_strides[i];
+    }
+  }
+  a.lengths = lengths;
+  a.lengths_dtype = lengths_dtype;
+  a.B = static_cast<int>(B);
+  a.Hq = static_cast<int>(Hq);
+  a.Hkv = static_cast<int>(Hkv);
+  a.Sq = static_cast<int>(Sq);
+  a.C = static_cast<int>(C);
+  a.D = static_cast<int>(D);
+  a.G = a.B;
+  a.window = static_cast<int>(kMaxCount / 2);
+  a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  return NTOPS_OK;
+}
+
+// Sizes alone, for the workspaces; false: nothing to attend, or a call that is refused.
+bool span_sizes(SpanArgs& a, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t C, int64_t D, int64_t P) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || C < 0 || P < 0 || D <= 0 || D > kMaxDim || Hq % Hkv != 0 || !sizes_fit(B, Hq, Sq, C, P))
+    return false;
+  a.B = static_cast<int>(B);
+  a.Hq = static_cast<int>(Hq);
+  a.Hkv = static_cast<int>(Hkv);
+  a.Sq = static_cast<int>(Sq);
+  a.C = static_cast<int>(C);
+  a.D = static_cast<int>(D);
+  a.G = a.B;
+  a.P = static_cast<int>(P);
+  a.window = static_cast<int>(kMaxCount / 2);
+  return true;
+}
+
+int clamp_count(int64_t n) { return static_cast<int>(std::min<int64_t>(n, kMaxCount / 2)); }
+
+}  // namespace
+
+extern "C" int64_t ntops_sliding_window_attention_workspace(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq,
+                                                            int64_t C, int64_t D, int64_t window, int64_t sinks) {
+  SpanArgs a{};
+  if (!span_sizes(a, B, Hq, Hkv, Sq, C, D, 0) || window < 1 || sinks < 0) return 0;
+  a.window = clamp_count(window);
+  a.sinks = clamp_count(sinks);
+  return plan_bytes(a, make_plan(dtype, a));
+}
+
+extern "C" int ntops_sliding_window_attention(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t C, int64_t D,
+                                              const void* q, const int64_t* q_strides, const void* key,
+                                              const int64_t* key_strides, const void* value, const int64_t* value_strides,
+                                              const void* lengths, int lengths_dtype, int64_t window, int64_t sinks,
+                                              double scale, void* out, const int64_t* out_strides, void* workspace,
+                                              int64_t workspace_bytes, void* stream) {
+  constexpr const char* what = "sliding_window_attention";
+  if (B < 0 || Hq < 0 || Hkv < 0 || Sq < 0 || C < 0 || D < 0) return set_error(NTOPS_ERR_INVALID, "%s: negative size", what);
+  if (window < 1 || sinks < 0) return set_error(NTOPS_ERR_INVALID, "%s: a window of at least 1, sinks of at least 0", what);
+  if (B == 0 || Hq == 0 || Sq == 0 || D == 0) return NTOPS_OK;
+  SpanArgs a{};
+  if (int e = span_args(what, a, dtype, B, Hq, Hkv, Sq, C, D, 0, q, q_strides, key, key_strides, value, value_strides, lengths,
+                        lengths_dtype, scale, out, out_strides, workspace, workspace_bytes))
+    return e;
+  a.window = clamp_count(window);
+  a.sinks = clamp_count(sinks);
+  return run(dtype, a, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int64_t ntops_shared_prefix_attention_workspace(int dtype, int64_t G, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq,
+                                                           int64_t P, int64_t C, int64_t D) {
+  SpanArgs a{};
+  if (!span_sizes(a, B, Hq, Hkv, Sq, C, D, P) || G <= 0 || B % G != 0) return 0;
+  a.G = static_cast<int>(G);
+  a.pk = &a;  // (a prefix there is)
+  return plan_bytes(a, make_plan(dtype, a));
+}
+
+extern "C" int ntops_shared_prefix_attention(int dtype, int64_t G, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t P,
+                                             int64_t C, int64_t D, const void* q, const int64_t* q_strides,
+                                             const void* prefix_key, const int64_t* prefix_key_strides,
+                                             const void* prefix_value, const int64_t* prefix_value_strides,
+                                             const void* prefix_lengths, int prefix_lengths_dtype, const void* key,
+                                             const int64_t* key_strides, const void* value, const int64_t* value_strides,
+                                             const void* lengths, int lengths_dtype, double scale, void* out,
+                                             const int64_t* out_strides, void* workspace, int64_t workspace_bytes, void* stream) {
+  constexpr const char* what = "shared_prefix_attention";
+  if (G < 0 || B < 0 || Hq < 0 || Hkv < 0 || Sq < 0 || P < 0 || C < 0 || D < 0)
+    return set_error(NTOPS_ERR_INVALID, "%s: negative size", what);
+  if (B == 0 || Hq == 0 || Sq == 0 || D == 0) return NTOPS_OK;
+  if (G == 0 || B % G != 0) return set_error(NTOPS_ERR_INVALID, "%s: the batch is not a multiple of the prefixes", what);
+  SpanArgs a{};
+  if (int e = span_args(what, a, dtype, B, Hq, Hkv, Sq, C, D, P, q, q_strides, key, key_strides, value, value_strides, lengths,
+                        lengths_dtype, scale, out, out_strides, workspace, workspace_bytes))
+    return e;
+  if (P > 0 && (!prefix_key || !prefix_value || !prefix_key_strides || !prefix_value_strides))
+    return set_error(NTOPS_ERR_INVALID, "%s: null pointer", what);
+  if (prefix_lengths && !index_dtype(prefix_lengths_dtype))
+    return set_error(NTOPS_ERR_INVALID, "%s: prefix lengths are I32 or I64", what);
+  a.G = static_cast<int>(G);
+  a.P = static_cast<int>(P);
+  a.pk = P > 0 ? prefix_key : out;  // (no key of it is read)
+  a.pv = P > 0 ? prefix_value : out;
+  for (int i = 0; i < 4 && P > 0; ++i) {
+    a.pkst[i] = prefix_key_strides[i];
+    a.pvst[i] = prefix_value_strides[i];
+  }
+  a.plengths = prefix_lengths;
+  a.plengths_dtype = prefix_lengths_dtype;
+  return run(dtype, a, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}

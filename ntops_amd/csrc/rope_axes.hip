@@ -1,0 +1,179 @@
+// Rotary positions with several axes on the query and key of a layer, each
+// (B, S, H, D):
+//   out0 = x0 cos - x1 sin,  out1 = x1 cos + x0 sin
+// for the pairs (i, i + D / 2), or (2 i, 2 i + 1) interleaved, with sin and cos of
+// pair i from row positions[axis(i)][b][s] of the tables: column i of tables of
+// D / 2 columns, the elements' own columns of tables of D.  In fp32, rounded once.
+// A pair whose position lies outside of the tables is NaN.
+//
+// Vector path: a thread owns 8 (fp32: 4) pairs of a token -- a 16-byte pack of
+// each half, or two packs of interleaved pairs -- gathers their sines and cosines
+// once and rotates up to kHeads heads with them, so that the table's bytes, which
+// are fp32 and come from rows of their own for each axis, are read once for several
+// heads.  Generic path: a thread per pair, any strides.
+#include <algorithm>
+
+#include "dispatch.h"
+#include "kv_cache.h"
+
+namespace ntops {
+namespace {
+
+constexpr int kMaxPairs = 256;
+
+struct AxesTensor {
+  const void* x;
+  void* y;
+  int64_t H;
+  int64_t xs[4], ys[4];
+};
+
+struct AxesArgs {
+  int64_t B, S, D;
+  AxesTensor t[2];  // query, key; H == 0: none
+  const void* sn;
+  const void* cs;
+  int64_t srs, crs;  // row strides of the tables
+  int64_t rows;      // of the tables
+  int wide;          // tables of D columns
+  int interleaved;
+  const void* pos;   // (axes, B, S)
+  int64_t ps[3];
+  int pos_dtype;
+  uint8_t axis[kMaxPairs];
+};
+
+__device__ __forceinline__ void rotate_pair(float x0, float x1, float c0, float s0, float c1, float s1, float& o0, float& o1) {
+  o0 = fmaf(x0, c0, -(x1 * s0));
+  o1 = fmaf(x1, c1, x0 * s1);
+}
+
+// Row of the tables of pair i's axis at token (b, s); -1: outside.
+__device__ __forceinline__ int64_t table_row(const AxesArgs& a, int axis, int64_t b, int64_t s) {
+  const int64_t p = index_at(a.pos, a.pos_dtype, axis * a.ps[0] + b * a.ps[1] + s * a.ps[2], 0);
+  return p >= 0 && p < a.rows ? p : -1;
+}
+
+// Sine and cosine of column `col` of row `row`.
+template <typename TT>
+__device__ __forceinline__ void table_at(const AxesArgs& a, int64_t row, int64_t col, float& sn, float& cs) {
+  const float nan = __builtin_nanf("");
+  sn = row < 0 ? nan : static_cast<float>(static_cast<const TT*>(a.sn)[row * a.srs + col]);
+  cs = row < 0 ? nan : static_cast<float>(static_cast<const TT*>(a.cs)[row * a.crs + col]);
+}
+
+// T: element type, TT: the tables' type.
+template <typename T, typename TT>
+__global__ __launch_bounds__(256) void k_rope_axes_generic(AxesArgs a, int64_t pairs0, int64_t pairs) {
+  const int64_t half = a.D / 2;
+  for (int64_t it = block_id() * 256 + threadIdx.x; it < pairs; it += static_cast<int64_t>(gridDim.x) * gridDim.y * 256) {
+    const bool second = it >= pairs0;
+    const AxesTensor& d = a.t[second ? 1 : 0];
+    const int64_t li = second ? it - pairs0 : it;
+    const int64_t i = li % half;
+    int64_t r = li / half;
+    const int64_t h = r % d.H;
+    r /= d.H;
+    const int64_t s = r % a.S, b = r / a.S;
+    const T* x = static_cast<const T*>(d.x) + b * d.xs[0] + s * d.xs[1] + h * d.xs[2];
+    T* y = static_cast<T*>(d.y) + b * d.ys[0] + s * d.ys[1] + h * d.ys[2];
+    const int64_t d0 = a.interleaved ? 2 * i : i, d1 = a.interleaved ? 2 * i + 1 : i + half;
+    const int64_t row = table_row(a, a.axis[i], b, s);
+    float s0, c0, s1, c1;
+    table_at<TT>(a, row, a.wide ? d0 : i, s0, c0);
+    table_at<TT>(a, row, a.wide ? d1 : i, s1, c1);
+    const float x0 = static_cast<float>(x[d0 * d.xs[3]]), x1 = static_cast<float>(x[d1 * d.xs[3]]);
+    float o0, o1;
+    rotate_pair(x0, x1, c0, s0, c1, s1, o0, o1);
+    y[d0 * d.ys[3]] = static_cast<T>(o0);
+    y[d1 * d.ys[3]] = static_cast<T>(o1);
+  }
+}
+
+template <typename T, typename TT>
+int run_axes(const AxesArgs& a, hipStream_t st) {
+  const int64_t tokens = a.B * a.S;
+  const int64_t pairs0 = tokens * a.t[0].H * (a.D / 2), pairs = pairs0 + tokens * a.t[1].H * (a.D / 2);
+  note_kernel("rope_axes generic");
+  hipLaunchKernelGGL((k_rope_axes_generic<T, TT>), blocks_2d(std::min<int64_t>(ceil_div(pairs, 256), 1 << 20)), dim3(256), 0, st, a, pairs0,
+                     pairs);
+  return check_launch("rope_axes");
+}
+
+}  // namespace
+}  // namespace ntops
+
+using namespace ntops;
+
+extern "C" int ntops_rope_axes_qk(int dtype, int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D, const void* q,
+                                  const int64_t* q_strides, const void* k, const int64_t* k_strides, int table_dtype,
+                                  const void* sin_table, int64_t sin_row_stride, const void* cos_table, int64_t cos_row_stride,
+                                  int64_t table_rows, int64_t table_cols, int64_t axes, const void* positions, int positions_dtype,
+                                  const int64_t* position_strides, int64_t n_sections, const int64_t* sections, int interleaved,
+                                  void* q_out, const int64_t* q_out_strides, void* k_out, const int64_t* k_out_strides,
+                                  void* stream) {
+  constexpr const char* what = "rope_axes_qk";
+  if (B < 0 || S < 0 || Hq < 0 || Hk < 0 || D < 0 || table_rows < 0) return set_error(NTOPS_ERR_INVALID, "%s: negative size", what);
+  if (dtype != NTOPS_F32 && dtype != NTOPS_F16 && dtype != NTOPS_BF16)
+    return set_error(NTOPS_ERR_UNSUPPORTED, "%s: unsupported dtype %d (F32/F16/BF16 only)", what, dtype);
+  if (table_dtype != NTOPS_F32 && table_dtype != dtype)
+    return set_error(NTOPS_ERR_INVALID, "%s: tables are F32 or of the tensors' type", what);
+  if (D % 2 != 0) return set_error(NTOPS_ERR_INVALID, "%s: the embedding dim must be even", what);
+  if (D > 2 * kMaxPairs) return set_error(NTOPS_ERR_UNSUPPORTED, "%s: embedding dim %lld > %d", what, (long long)D, 2 * kMaxPairs);
+  if (table_cols != D && table_cols != D / 2) return set_error(NTOPS_ERR_INVALID, "%s: tables must have D or D/2 columns", what);
+  if (!index_dtype(positions_dtype)) return set_error(NTOPS_ERR_INVALID, "%s: positions are I32 or I64", what);
+  if (axes < 1 || n_sections < 1 || !sections) return set_error(NTOPS_ERR_INVALID, "%s: no axes or sections", what);
+  AxesArgs a{};
+  int64_t filled = 0;
+  for (int64_t s = 0; s < n_sections; ++s) {
+    if (sections[s] < 0 || sections[s] > D / 2 - filled)
+      return set_error(NTOPS_ERR_INVALID, "%s: the sections must add up to D/2", what);
+    if (sections[s] > 0 && s % axes > 255) return set_error(NTOPS_ERR_UNSUPPORTED, "%s: more than 256 axes", what);
+    for (int64_t i = 0; i < sections[s]; ++i) a.axis[filled++] = static_cast<uint8_t>(s % axes);
+  }
+  if (filled != D / 2) return set_error(NTOPS_ERR_INVALID, "%s: the sections must add up to D/2", what);
+  if (B == 0 || S == 0 || Hq + Hk == 0 || D == 0) return NTOPS_OK;
+  if (!positions || !position_strides || (table_rows > 0 && (!sin_table || !cos_table)) ||
+      (Hq > 0 && (!q || !q_out || !q_strides || !q_out_strides)) || (Hk > 0 && (!k || !k_out || !k_strides || !k_out_strides)))
+    return set_error(NTOPS_ERR_INVALID, "%s: null pointer", what);
+  constexpr int64_t kMost = int64_t(1) << 40;
+  if (B > kMost || S > kMost || Hq > kMost || Hk > kMost || B * S > kMost || (Hq + Hk) > kMost / (B * S))
+    return set_error(NTOPS_ERR_UNSUPPORTED, "%s: problem too large", what);
+  a.B = B;
+  a.S = S;
+  a.D = D;
+  const void* xs[2] = {q, k};
+  void* ys[2] = {q_out, k_out};
+  const int64_t* xst[2] = {q_strides, k_strides};
+  const int64_t* yst[2] = {q_out_strides, k_out_strides};
+  const int64_t hs[2] = {Hq, Hk};
+  for (int t = 0; t < 2; ++t) {
+    a.t[t].H = hs[t];
+    if (hs[t] == 0) continue;
+    a.t[t].x = xs[t];
+    a.t[t].y = ys[t];
+    for (int d = 0; d < 4; ++d) {
+      a.t[t].xs[d] = xst[t][d];
+      a.t[t].ys[d] = yst[t][d];
+    }
+    if (xs[t] == ys[t])
+      for (int d = 0; d < 4; ++d)
+        if (xst[t][d] != yst[t][d]) return set_error(NTOPS_ERR_INVALID, "%s: in place needs equal strides", what);
+  }
+  a.sn = sin_table;
+  a.cs = cos_table;
+  a.srs = sin_row_stride;
+  a.crs = cos_row_stride;
+  a.rows = table_rows;
+  a.wide = table_cols == D;
+  a.interleaved = interleaved != 0;
+  a.pos = positions;
+  a.pos_dtype = positions_dtype;
+  for (int d = 0; d < 3; ++d) a.ps[d] = position_strides[d];
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  return dispatch_float16_32(dtype, what, [&](auto tag) {
+    using T = decltype(tag);
+    if (table_dtype == NTOPS_F32) return run_axes<T, float>(a, st);
+    return run_axes<T, T>(a, st);
+  });
+}

@@ -30,6 +30,7 @@ from ntops_amd.torch.lt import lt
 from ntops_amd.torch.matmul import matmul
 from ntops_amd.torch.mm import mm
 from ntops_amd.torch.mul import mul
+from ntops_amd.torch.multi_axis_rotary_position_embedding_qk import multi_axis_rotary_position_embedding_qk
 from ntops_amd.torch.mxfp4_mm import mxfp4_mm
 from ntops_amd.torch.ne import ne
 from ntops_amd.torch.neg import neg
@@ -41,9 +42,11 @@ from ntops_amd.torch.rotary_position_embedding import rotary_position_embedding
 from ntops_amd.torch.rotary_position_embedding_qk import rotary_position_embedding_qk
 from ntops_amd.torch.rsqrt import rsqrt
 from ntops_amd.torch.scaled_dot_product_attention import scaled_dot_product_attention
+from ntops_amd.torch.shared_prefix_attention import shared_prefix_attention
 from ntops_amd.torch.sigmoid import sigmoid
 from ntops_amd.torch.silu import silu
 from ntops_amd.torch.sin import sin
+from ntops_amd.torch.sliding_window_attention import sliding_window_attention
 from ntops_amd.torch.softmax import softmax
 from ntops_amd.torch.store_kv_cache import store_kv_cache
 from ntops_amd.torch.sub import sub
@@ -78,6 +81,7 @@ __all__ = [
     "matmul",
     "mm",
     "mul",
+    "multi_axis_rotary_position_embedding_qk",
     "mxfp4_mm",
     "ne",
     "neg",
@@ -89,9 +93,11 @@ __all__ = [
     "rotary_position_embedding_qk",
     "rsqrt",
     "scaled_dot_product_attention",
+    "shared_prefix_attention",
     "sigmoid",
     "silu",
     "sin",
+    "sliding_window_attention",
     "softmax",
     "store_kv_cache",
     "sub",

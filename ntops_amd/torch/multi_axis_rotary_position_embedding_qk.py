@@ -1,0 +1,67 @@
+"""multi_axis_rotary_position_embedding_qk -- rotary positions with several axes (of
+an image or a video: time, height and width) on the query and key of one attention
+layer, in a single launch.
+
+No ntops counterpart (torch/rotary_position_embedding.py:7-29 rotates a whole head by
+one position, the token's place).  q (batch, seq, q_heads, dim) and k (batch, seq,
+k_heads, dim); positions (axes, batch, seq) in int32 or int64, expanded dims as they
+are.  `sections` divides the dim / 2 pairs of a head: section s holds that many pairs
+in order, and belongs to axis s % axes -- (16, 24, 24) for three blocks of pairs,
+(1,) * 64 for axes in turn.  A pair's angle is that of its axis' position: sin_table
+and cos_table (positions, dim / 2), or (positions, dim) with each element's own
+column, in float32 or the tensors' type.  Pairs are elements (2 i, 2 i + 1), or with
+interleaved=False (i, i + dim / 2).
+
+Computed in fp32 and rounded once.  A pair whose position lies outside of the tables
+is NaN (positions are read on the device).  Returns (q_out, k_out); inplace=True
+rotates q and k in place."""
+
+import operator
+
+import torch
+
+from ntops_amd import _lib
+from ntops_amd.torch.utils import _DeviceGuard, _contiguous, _strides, _to_dtype
+
+
+def multi_axis_rotary_position_embedding_qk(q, k, sin_table, cos_table, positions, sections, interleaved=True, inplace=False):
+    what = "multi_axis_rotary_position_embedding_qk"
+    if q.dim() != 4 or k.dim() != 4:
+        raise RuntimeError(f"{what}: q and k must be (batch, seq, heads, dim)")
+    batch, seq, _, dim = q.shape
+    if k.shape[0] != batch or k.shape[1] != seq or k.shape[3] != dim:
+        raise RuntimeError(f"{what}: q and k differ in batch, seq or dim")
+    if k.dtype != q.dtype or q.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise RuntimeError(f"{what}: expected one of float32, float16 and bfloat16, got {q.dtype} and {k.dtype}")
+    if dim % 2 != 0:
+        raise RuntimeError("The embedding dimension must be even.")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 3 or positions.shape[1:] != (batch, seq) or positions.shape[0] < 1:
+        raise RuntimeError(f"{what}: expected positions of shape (axes, {batch}, {seq}) in int32 or int64, got {tuple(positions.shape)}, {positions.dtype}")
+    sections = [operator.index(n) for n in sections]
+    if min(sections, default=-1) < 0 or sum(sections) != dim // 2:
+        raise RuntimeError(f"{what}: sections {sections} do not add up to {dim // 2} pairs")
+    if sin_table.dim() != 2 or sin_table.shape != cos_table.shape or sin_table.shape[1] not in (dim // 2, dim):
+        raise RuntimeError(
+            f"{what}: the tables must both be (positions, {dim // 2}) or (positions, {dim}), got {tuple(sin_table.shape)} and {tuple(cos_table.shape)}")
+    for x in (q, k):
+        if inplace and any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape)):
+            raise RuntimeError(f"{what}: elements that share memory (a stride is 0) cannot be rotated in place")
+    dev = _lib.require_cuda(q, k, sin_table, cos_table, positions)
+    lib = _lib.load()
+    with _DeviceGuard(dev):
+        q_out = q if inplace else torch.empty(q.shape, dtype=q.dtype, device=dev)
+        k_out = k if inplace else torch.empty(k.shape, dtype=k.dtype, device=dev)
+        tables = [sin_table, cos_table]
+        if sin_table.dtype != cos_table.dtype or sin_table.dtype not in (torch.float32, q.dtype):
+            tables = [_to_dtype(t, torch.float32) for t in tables]
+        sin_table, cos_table = (t if t.stride(1) == 1 or t.shape[1] <= 1 else _contiguous(t) for t in tables)
+        rc = lib.ntops_rope_axes_qk(
+            _lib.dtype_code(q.dtype), batch, seq, q.shape[2], k.shape[2], dim,
+            q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), _lib.dtype_code(sin_table.dtype),
+            sin_table.data_ptr(), sin_table.stride(0), cos_table.data_ptr(), cos_table.stride(0),
+            sin_table.shape[0], sin_table.shape[1], positions.shape[0], positions.data_ptr(),
+            _lib.dtype_code(positions.dtype), _strides(positions), len(sections), _lib.i64_array(sections),
+            1 if interleaved else 0, q_out.data_ptr(), _strides(q_out), k_out.data_ptr(), _strides(k_out),
+            _lib.stream_of(q_out))
+    _lib.check(rc, f"ntops_amd.{what}")
+    return q_out, k_out
