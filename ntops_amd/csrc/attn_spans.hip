@@ -100,22 +100,58 @@ int launch_rows(const SpanArgs& a, int mode, int slices, const SpanPart& part, h
   return check_launch("attention");
 }
 
-// How a problem is served: how many slices of the keys, in which launches.
+// Most keys of the main span that a row sees.
+int64_t main_keys(const SpanArgs& a) { return std::min<int64_t>(a.C, static_cast<int64_t>(a.window) + a.sinks); }
+
+// How a problem is served: on which kernels, and in how many slices of the keys.
+enum Path { kRows, kFew };
 struct Plan {
-  int slices;  // of rows over all their keys
+  Path path;
+  int slices;  // of a row, over all launches
+  FewPlan few;
 };
 
-// Most keys that a row sees.
-int64_t most_keys(const SpanArgs& a) {
-  return a.P + std::min<int64_t>(a.C, static_cast<int64_t>(a.window) + a.sinks);
+Plan rows_plan(const SpanArgs& a) {
+  Plan p{kRows, 1, {}};
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
+  p.slices = static_cast<int>(std::max<int64_t>(1, std::min({static_cast<int64_t>(kMaxSlices), cu_count_cached() * 8 / rows, (a.P + main_keys(a)) / 128})));
+  return p;
 }
 
-Plan make_plan(int dtype, const SpanArgs& a) {
-  (void)dtype;
-  Plan p;
-  const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
-  p.slices = static_cast<int>(std::max<int64_t>(1, std::min({static_cast<int64_t>(kMaxSlices), cu_count_cached() * 8 / rows, most_keys(a) / 128})));
+// Slices for `heads` sets of blocks over `keys` keys.
+int few_slices(const SpanArgs& a, int64_t heads, int64_t keys, int waves) {
+  const int step = (a.D > 64 ? 32 : 64) * waves;
+  int64_t n = std::min({static_cast<int64_t>(kMaxSlices), cu_count_cached() * 2 / waves / heads, ceil_div(keys, 4 * step)});
+  if (n <= 2 && keys <= 8 * step) n = 1;  // two short slices gain what the merge's launch costs
+  return static_cast<int>(std::max<int64_t>(n, 1));
+}
+
+Plan few_plan(const SpanArgs& a) {
+  Plan p{kFew, 1, {}};
+  const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv;
+  const int cus = cu_count_cached();
+  p.few.waves = heads < 2 * cus ? 2 : 1;
+  if (a.P > 0 && a.B > a.G) {
+    // as many keys a block of the prefix as of a sequence
+    const int64_t fsets = span_sets(a, kFront) * ceil_div(span_rows(a, kFront), 64);
+    const int64_t total = fsets * a.P + heads * a.C;
+    const int step = (a.D > 64 ? 32 : 64) * p.few.waves;
+    const int64_t chunk = std::max<int64_t>(4 * step, ceil_div(total, cus * 2));
+    p.few.front_slices = static_cast<int>(std::min<int64_t>(kMaxSlices / 2, ceil_div(a.P, chunk)));
+    p.few.slices = static_cast<int>(std::min<int64_t>(kMaxSlices / 2, std::max<int64_t>(1, ceil_div(a.C, chunk))));
+    p.slices = p.few.front_slices + p.few.slices;
+    return p;
+  }
+  p.few.front_slices = 0;
+  p.few.slices = p.slices = few_slices(a, heads, a.P + main_keys(a), p.few.waves);
   return p;
+}
+
+// The plan for this problem where layouts suit the matrix cores, from sizes alone.
+Plan make_plan(int dtype, const SpanArgs& a) {
+  const bool matrix = dtype != NTOPS_F32 && a.D % 8 == 0 && a.D <= 128 && a.C + static_cast<int64_t>(a.P) > 0;
+  if (matrix && span_rows(a, kMain) <= kFewRows) return few_plan(a);
+  return rows_plan(a);
 }
 
 int64_t plan_bytes(const SpanArgs& a, const Plan& p) {
@@ -123,11 +159,38 @@ int64_t plan_bytes(const SpanArgs& a, const Plan& p) {
   return static_cast<int64_t>(a.B) * a.Hq * a.Sq * p.slices * ((a.D + 3) / 4 * 4 + 2) * 4;
 }
 
+// What the matrix cores' kernels read: unit strides along the head dim, rows at
+// multiples of 16 bytes that do not overlap, and every offset within a span of a head
+// below 2^31 bytes.
+bool matrix_layout(const SpanArgs& a) {
+  const auto rows8 = [](const int64_t* s) { return s[3] == 1 && s[2] % 8 == 0 && s[1] % 8 == 0 && s[0] % 8 == 0; };
+  const auto span = [&](const int64_t* s, int64_t keys) { return s[2] >= a.D && (keys + 256) * s[2] * 2 < 0x7fffffffLL; };
+  if (!rows8(a.qst) || !aligned16(a.q) || a.ost[3] != 1 || a.ost[2] % 4 != 0 || a.ost[1] % 4 != 0 || a.ost[0] % 4 != 0 ||
+      (reinterpret_cast<uintptr_t>(a.o) & 7u) != 0)
+    return false;
+  const int64_t keys = std::min<int64_t>(a.C, static_cast<int64_t>(a.window) + a.Sq);
+  if (a.C > 0 && (!rows8(a.kst) || !rows8(a.vst) || !aligned16(a.k) || !aligned16(a.v) || !span(a.kst, keys) || !span(a.vst, keys)))
+    return false;
+  if (a.C > 0 && a.sinks > 0) {
+    const int64_t sinks = std::min<int64_t>(a.C, a.sinks);
+    if (!span(a.kst, sinks) || !span(a.vst, sinks)) return false;
+  }
+  return a.P == 0 || (rows8(a.pkst) && rows8(a.pvst) && aligned16(a.pk) && aligned16(a.pv) && span(a.pkst, a.P) && span(a.pvst, a.P));
+}
+
 int run(int dtype, const SpanArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
   Plan p = make_plan(dtype, a);
-  if (ws == nullptr || ws_bytes < plan_bytes(a, p)) p.slices = 1;
-  SpanPart part{p.slices > 1 ? static_cast<float*>(ws) : nullptr, p.slices, 0, (a.D + 3) / 4 * 4};
-  if (int e = span_rows_run(dtype, a, kBoth, p.slices, part, st)) return e;
+  if (p.path != kRows && !matrix_layout(a)) {
+    const int64_t room = plan_bytes(a, p);
+    p = rows_plan(a);
+    if (plan_bytes(a, p) > room) p.slices = 1;  // (the workspace is sized before the layout is known)
+  }
+  if (p.slices > 1 && (ws == nullptr || ws_bytes < plan_bytes(a, p))) {
+    p.slices = p.few.slices = 1;
+    p.few.front_slices = 0;
+  }
+  const SpanPart part{p.slices > 1 ? static_cast<float*>(ws) : nullptr, p.slices, 0, (a.D + 3) / 4 * 4};
+  if (int e = p.path == kFew ? span_few_run(dtype, a, p.few, part, st) : span_rows_run(dtype, a, kBoth, p.slices, part, st)) return e;
   return part.p ? merge(dtype, a, part, st) : NTOPS_OK;
 }
 

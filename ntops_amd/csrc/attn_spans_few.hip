@@ -1,0 +1,427 @@
+// Few query rows a cache head (single tokens, drafted ones): windowed and
+// shared-prefix attention bound by streaming keys and values once.
+//
+// The rows that share a cache head fill the 16 columns of v_mfma_f32_16x16x32, up to
+// four such groups of them, so that a key that has reached the LDS serves up to 64
+// rows (S^T = K Q^T: a lane's scores all belong to one row, and P^T feeds
+// O^T += V^T P^T from registers).  Every wave owns tiles of 8 KiB of keys and 8 KiB
+// of values in its own part of the LDS, loaded by direct DMA two tiles ahead and
+// refilled as soon as they are read: no barrier before the waves are joined.  Tiles
+// never mix the two spans: those of the front come first.
+//
+// A launch holds two kinds of blocks, one behind the other: those of the rows of
+// all sequences of a group over their shared prefix, and those of each sequence's
+// rows over its own keys, so that neither waits for the other's tail.
+//
+// What a row does not see: masked scores are -inf whatever their key holds.  A
+// value that is not finite times P = 0 is NaN, though; a row whose result is NaN under
+// a sum that is none is computed again by itself, from the keys that it sees.
+#include <algorithm>
+
+#include "attn_spans.h"
+
+namespace ntops {
+namespace {
+
+// v_mfma_f32_16x16x32: lane l holds row / column l & 15 at k = 8 (l >> 4) .. + 7 of
+// A / B, and column l & 15, rows 4 (l >> 4) .. + 3 of the result.
+template <typename T>
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (std::is_same<T, __bf16>::value)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+}
+
+template <int D>
+constexpr int kTileKeys = 4096 / D;  // keys of a wave's tile
+// A row's reference, which its exponents are taken from, follows its maximum when that
+// is past it by more than this (base 2): the largest probability is then at most 2^8,
+// in fp32 sums and in 16-bit products as good as 1, and O is rescaled on few tiles.
+constexpr float kSlack = 8.f;
+
+// The copy of a 16-byte chunk a lane with the non-temporal hint (mfma.h: dma16): each
+// byte is read once.
+__device__ __forceinline__ void dma16_once(u32x4 rsrc, uint32_t lds_dst, uint32_t voffset) {
+  asm volatile("buffer_load_dwordx4 %0, %1, 0 offen nt lds"
+               :
+               : "v"(voffset), "s"(rsrc), "{m0}"(lds_dst)
+               : "memory");
+}
+
+// Loads of one tile's K (or V) rows: 8 instructions of 1 KiB, the swizzle on the global
+// side.
+template <int D, bool IS_V>
+struct TileDma {
+  static constexpr int kInst = 8;
+  static constexpr int kRows = 512 / D;  // rows per instruction
+  u32x4 rsrc;
+  uint32_t ld2;  // bytes from row to row
+  uint32_t voff[kInst];
+
+  __device__ __forceinline__ void init(const void* base, int64_t ld, int n, int lane, int dt) {
+    rsrc = make_rsrc(base, n > 0 ? ((n - 1) * ld + dt) * 2 : 0);
+    ld2 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(ld * 2));
+    constexpr int cpr = D / 8;
+#pragma unroll
+    for (int i = 0; i < kInst; ++i) {
+      const int row = i * kRows + lane / cpr;
+      const int slot = lane % cpr;
+      const int c = IS_V ? vslot<D>(row, slot) : kslot<D>(row, slot);
+      voff[i] = c * 8 < dt ? row * ld2 + c * 16 : kOOB;
+    }
+  }
+  // rows `row0` and on into LDS at `dst`; row0 < 0: an empty load, which still counts
+  // in vmcnt
+  __device__ __forceinline__ void issue(uint32_t dst, int row0) const {
+    const uint32_t off = row0 < 0 ? kOOB : row0 * ld2;
+#pragma unroll
+    for (int i = 0; i < kInst; ++i)
+      // kOOB + kOOB would wrap to 0: keep either one
+      dma16_once(rsrc, dst + i * 1024, (voff[i] | off) & kOOB ? kOOB : voff[i] + off);
+  }
+};
+
+// Reads of LDS filled by DMA must not move across the wait that orders them.
+template <int N>
+__device__ __forceinline__ void wait_dma() {
+  __builtin_amdgcn_sched_barrier(0);
+  wait_vmcnt<N>();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// One kind of blocks of a launch.
+struct FewBlocks {
+  int mode;       // SpanMode
+  int row_blocks;  // of a set
+  int slices;
+  int first;      // slice of the rows that slice 0 is
+  int64_t blocks;
+};
+
+// RG: groups of 16 rows a block has room for.
+template <typename T, int D, int NW, int RG>
+__device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f, SpanPart part, int64_t id, char* smem) {
+  constexpr int NK = kTileKeys<D>;
+  constexpr int KB = NK / 16;  // 16-key blocks of a tile
+  constexpr int KS = D / 32;   // k-steps of S^T = K Q^T
+  constexpr int DT = D / 16;   // 16-row tiles of O^T
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, c16 = lane & 15;
+  const int slice = static_cast<int>(id % f.slices);
+  const int64_t at = id / f.slices;
+  const int64_t set = at / f.row_blocks;
+  const int r0 = static_cast<int>(at - set * f.row_blocks) * (16 * RG);
+  const int group = a.Hq / a.Hkv, ro = group * a.Sq;
+  const int set_rows = f.mode == kFront ? ro * (a.B / a.G) : ro;
+  const int rows = min(16 * RG, set_rows - r0);
+  const int ng = RG == 1 ? 1 : (rows + 15) / 16;
+  const int t0 = f.mode == kFront ? 0 : r0 / group, t1 = f.mode == kFront ? 0 : (r0 + rows - 1) / group;
+  const Spans s = make_spans<2>(a, f.mode, set, t0, t1);
+  part.first = f.first;
+
+  int hi[RG], lo[RG];
+  u32x4 qf[RG][KS];
+#pragma unroll
+  for (int rg = 0; rg < RG; ++rg) {
+    const int r = rg * 16 + c16;
+    const SpanRow x = span_row(a, s, r0 + min(r, rows - 1));
+    hi[rg] = s.hi(x.t);
+    lo[rg] = s.lo(x.t);
+    const T* Q = static_cast<const T*>(a.q) + x.b * a.qst[0] + x.h * a.qst[1] + x.t * a.qst[2];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d0 = ks * 32 + 8 * g;
+      qf[rg][ks] = r < rows && d0 < a.D ? *reinterpret_cast<const u32x4*>(Q + d0) : u32x4{0, 0, 0, 0};
+      if (a.scale_log2 < 0.f) qf[rg][ks] ^= 0x80008000u;
+    }
+  }
+  // settled here, so that no wait for it is placed among the tile loads
+#pragma unroll
+  for (int rg = 0; rg < RG; ++rg)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[rg][ks]));
+  // at least the least factor there is, so that a masked score stays -inf under a zero scale
+  const float c = fabsf(a.scale_log2) < 0x1p-126f ? 0x1p-126f : fabsf(a.scale_log2);
+  const int hi_min = s.hi(t0), lo_max = s.lo(t1);  // a main tile between them is seen whole by every row
+
+  const int nft = (s.n[0] + NK - 1) / NK, nt = nft + (s.n[1] + NK - 1) / NK;
+  const int per = (nt + f.slices - 1) / f.slices;
+  const int i0 = min(slice * per, nt), i1 = min(i0 + per, nt);
+  const int n = i1 - i0 > wave ? (i1 - i0 - wave + NW - 1) / NW : 0;  // tiles of this wave: i0 + wave, + NW, ...
+  char* mine = smem + wave * 32768;
+  const uint32_t mine_addr = lds_addr(mine);
+  TileDma<D, false> kd;
+  TileDma<D, true> vd;
+  const auto tile_at = [&](int j) { return i0 + wave + j * NW; };
+  // (a wave's tiles of the front come first, so each DMA turns to the main span once)
+  int kspan = tile_at(0) < nft ? 0 : 1, vspan = kspan;
+  kd.init(s.k[kspan], s.kld[kspan], s.n[kspan], lane, a.D);
+  vd.init(s.v[vspan], s.vld[vspan], s.n[vspan], lane, a.D);
+  const auto issue_k = [&](int j) __attribute__((always_inline)) {
+    const int i = tile_at(j);
+    if (j < n && kspan == 0 && i >= nft) {
+      kspan = 1;
+      kd.init(s.k[1], s.kld[1], s.n[1], lane, a.D);
+    }
+    kd.issue(mine_addr + (j & 1) * 16384, j < n ? (i < nft ? i : i - nft) * NK : -1);
+  };
+  const auto issue_v = [&](int j) __attribute__((always_inline)) {
+    const int i = tile_at(j);
+    if (j < n && vspan == 0 && i >= nft) {
+      vspan = 1;
+      vd.init(s.v[1], s.vld[1], s.n[1], lane, a.D);
+    }
+    vd.issue(mine_addr + (j & 1) * 16384 + 8192, j < n ? (i < nft ? i : i - nft) * NK : -1);
+  };
+
+  f32x4 o[RG][DT];
+  float m[RG], l[RG];  // reference (base 2) of the lane's row; this lane's part of its sum
+#pragma unroll
+  for (int rg = 0; rg < RG; ++rg) {
+    m[rg] = neg_inf();
+    l[rg] = 0.f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[rg][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  issue_k(0);
+  issue_v(0);
+  issue_k(1);
+  issue_v(1);
+  for (int j = 0; j < n; ++j) {
+    const char* sk = mine + (j & 1) * 16384;
+    const char* sv = sk + 8192;
+    wait_dma<24>();  // K of tile j is in; its V and tile j + 1 may be in flight
+    f32x4 sc[RG][KB];
+#pragma unroll
+    for (int rg = 0; rg < RG; ++rg)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) sc[rg][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const int row = kb * 16 + c16;
+        const u32x4 kf = *reinterpret_cast<const u32x4*>(sk + row * (D * 2) + kslot<D>(row, ks * 4 + g) * 16);
+#pragma unroll
+        for (int rg = 0; rg < RG; ++rg)
+          if (RG == 1 || rg < ng) sc[rg][kb] = mfma16<T>(kf, qf[rg][ks], sc[rg][kb]);
+      }
+    wait_lgkmcnt0();
+    issue_k(j + 2);
+
+    // scores of keys kt + 16 kb + 4 g + e of the tile's span
+    const int i = tile_at(j);
+    const bool front = i < nft;
+    const int kt = (front ? i : i - nft) * NK;
+    const bool whole = front ? kt + NK <= s.n[0] : kt + NK <= hi_min && (kt >= lo_max || kt + NK <= s.sinks);
+    u32x4 pf[RG][KB / 2];
+#pragma unroll
+    for (int rg = 0; rg < RG; ++rg) {
+      if (RG > 1 && rg >= ng) continue;
+      if (!whole) {
+        const int up = (front ? s.n[0] : hi[rg]) - kt - 4 * g, down = front ? 0 : lo[rg] - kt - 4 * g, sink = s.sinks - kt - 4 * g;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k = kb * 16 + e;
+            sc[rg][kb][e] = k < up && (k >= down || k < sink) ? sc[rg][kb][e] : neg_inf();
+          }
+      }
+      float mx = fmaxf(sc[rg][0][0], sc[rg][0][1]);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        mx = max3(mx, sc[rg][kb][0], sc[rg][kb][1]);
+        mx = max3(mx, sc[rg][kb][2], sc[rg][kb][3]);
+      }
+      mx *= c;
+      if (__any(mx > m[rg] + kSlack)) {
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const bool up = mx > m[rg] + kSlack;
+        const float alpha = up ? fast_exp2(m[rg] - mx) : 1.f;
+        m[rg] = up ? mx : m[rg];
+        l[rg] *= alpha;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[rg][t][e] *= alpha;
+      }
+      const float mb = m[rg] == neg_inf() ? 0.f : m[rg];  // nothing seen so far: P = 0
+#pragma unroll
+      for (int p = 0; p < KB / 2; ++p) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = fast_exp2(fmaf(sc[rg][2 * p + (e >> 2)][e & 3], c, -mb));
+        l[rg] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        pf[rg][p] = pack8<T>(x);  // keys 32 p + 4 g + 0..3 and 32 p + 16 + 4 g + 0..3
+      }
+    }
+
+    wait_dma<24>();  // V of tile j is in
+#pragma unroll
+    for (int p = 0; p < KB / 2; ++p)
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        // V^T: lane row 16 t + (l & 15) at the keys of pf[p]
+        const int col = t * 16 + (c16 & 3) * 4;
+        s16x4 w[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int row = p * 32 + u * 16 + g * 4 + (c16 >> 2);
+          w[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_s16x4_t*)(sv + row * (D * 2) + vslot<D>(row, col >> 3) * 16 + ((col >> 2) & 1) * 8));
+        }
+        const u32x2 lw = __builtin_bit_cast(u32x2, w[0]), hw = __builtin_bit_cast(u32x2, w[1]);
+        const u32x4 vf = {lw.x, lw.y, hw.x, hw.y};
+#pragma unroll
+        for (int rg = 0; rg < RG; ++rg)
+          if (RG == 1 || rg < ng) o[rg][t] = mfma16<T>(vf, pf[rg][p], o[rg][t]);
+      }
+    wait_lgkmcnt0();
+    issue_v(j + 2);
+  }
+  wait_dma<0>();  // no DMA may land in the LDS that the joining reuses
+
+  // join the waves, a group of rows after the other: [wave][16] maxima, [wave][16]
+  // sums, a bit per row that has to be computed again, then [wave][16][D + 4] O
+  float* sm = reinterpret_cast<float*>(smem);
+  uint32_t* again = reinterpret_cast<uint32_t*>(sm + 2 * NW * 16);
+  float* so = sm + 2 * NW * 16 + 4;
+  constexpr int LD = D + 4;
+#pragma unroll
+  for (int rg = 0; rg < RG; ++rg) {
+    if (RG > 1 && rg >= ng) continue;
+    __syncthreads();
+    l[rg] += __shfl_xor(l[rg], 16, 64);
+    l[rg] += __shfl_xor(l[rg], 32, 64);
+    if (rg == 0 && threadIdx.x < 2) again[threadIdx.x] = 0;
+    if (g == 0) {
+      sm[wave * 16 + c16] = m[rg];
+      sm[(NW + wave) * 16 + c16] = l[rg];
+    }
+#pragma unroll
+    for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4*>(so + (wave * 16 + c16) * LD + t * 16 + 4 * g) = o[rg][t];
+    __syncthreads();
+    for (int it = threadIdx.x; it < 16 * (D / 4); it += 64 * NW) {
+      const int row = it / (D / 4), d = (it - row * (D / 4)) * 4;
+      if (rg * 16 + row >= rows || d >= a.D) continue;
+      float mm = sm[row];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) mm = fmaxf(mm, sm[w * 16 + row]);
+      float sum = 0.f;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float mw = sm[w * 16 + row];
+        // (a wave of which the row has seen nothing: 0 whatever it met)
+        const float fw = mw == neg_inf() ? 0.f : fast_exp2(mw - mm);
+        sum += sm[(NW + w) * 16 + row] * fw;
+        const f32x4 ow = *reinterpret_cast<const f32x4*>(so + (w * 16 + row) * LD + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += mw == neg_inf() ? 0.f : ow[e] * fw;
+      }
+      const SpanRow x = span_row(a, s, r0 + rg * 16 + row);
+      const float any = (v[0] + v[1]) + (v[2] + v[3]);
+      if (!(any == any) && sum == sum) atomicOr(&again[rg >> 1], 1u << ((rg & 1) * 16 + row));
+      if (part.p) {
+        const int64_t pa = part.at(a, x, slice);
+        if (d == 0) {
+          float* ml = part.ml(a, pa);
+          ml[0] = mm;
+          ml[1] = sum;
+        }
+        *reinterpret_cast<f32x4*>(part.row(pa) + d) = v;
+      } else {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (a NaN sum passes through)
+        T w4[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w4[e] = static_cast<T>(v[e] * inv);
+        *reinterpret_cast<u32x2*>(static_cast<T*>(a.o) + x.b * a.ost[0] + x.h * a.ost[1] + x.t * a.ost[2] + d) =
+            __builtin_bit_cast(u32x2, w4);
+      }
+    }
+  }
+  __syncthreads();
+  const uint32_t bad0 = __builtin_amdgcn_readfirstlane(again[0]), bad1 = __builtin_amdgcn_readfirstlane(again[1]);
+  uint64_t bad = static_cast<uint64_t>(bad1) << 32 | bad0;
+  if (bad == 0) return;  // (the same for every wave)
+  wait_vmcnt<0>();       // what has been written of these rows is written before what follows
+  __syncthreads();
+  while (bad != 0) {
+    const int row = __builtin_ctzll(bad);
+    bad &= bad - 1;
+    if (row % NW != wave) continue;
+    const SpanRow x = span_row(a, s, r0 + row);
+    float ro_[D / 16], rm, rl;
+    span_attend_row<T, D / 16>(a, s, x, min(i0 * NK, s.n[0]), min(i1 * NK, s.n[0]), max(0, min((i0 - nft) * NK, s.n[1])),
+                               max(0, min((i1 - nft) * NK, s.n[1])), ro_, rm, rl);
+    span_write_row<T, D / 16>(a, part, x, slice, ro_, rm, rl);
+  }
+}
+
+// RGF, RGM: groups of rows of the blocks over shared prefixes (0: there are none) and
+// of the others.
+template <typename T, int D, int NW, int RGF, int RGM>
+__global__ __launch_bounds__(64 * NW, 1) void k_span_few(SpanArgs a, FewBlocks front, FewBlocks main, SpanPart part) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // [wave][2 stages][K, V]
+  const int64_t id = block_id();
+  if (id >= front.blocks + main.blocks) return;  // the tail of a 2-D grid (the whole block)
+  if constexpr (RGF > 0) {
+    if (id < front.blocks) {
+      few_block<T, D, NW, RGF>(a, front, part, id, smem);
+      return;
+    }
+  }
+  few_block<T, D, NW, RGM>(a, main, part, id - front.blocks, smem);
+}
+
+template <typename T, int D, int NW, int RGF, int RGM>
+int launch_few(const SpanArgs& a, const FewBlocks& front, const FewBlocks& main, const SpanPart& part, hipStream_t st) {
+  constexpr int kLds = NW * 32768;
+  static_assert(kLds <= 65536 && (2 * NW * 16 + 4 + NW * 16 * (D + 4)) * 4 <= kLds, "LDS");
+  note_kernel("%s few d%d waves%d rows%d+%d split%d", a.pk ? "shared_prefix" : "sliding_window", D, NW, 16 * RGF, 16 * RGM, part.slices);
+  hipLaunchKernelGGL((k_span_few<T, D, NW, RGF, RGM>), blocks_2d(front.blocks + main.blocks), dim3(64 * NW), kLds, st, a, front, main, part);
+  return check_launch("attention");
+}
+
+template <typename T, int D>
+int run_few(const SpanArgs& a, const FewPlan& p, const SpanPart& part, hipStream_t st) {
+  const bool wide = span_rows(a, kMain) > 16;
+  FewBlocks front{}, main{};
+  main.mode = p.front_slices > 0 ? kMain : kBoth;
+  main.row_blocks = static_cast<int>(ceil_div(span_rows(a, main.mode), wide ? 64 : 16));
+  main.slices = p.slices;
+  main.first = p.front_slices;
+  main.blocks = span_sets(a, main.mode) * main.row_blocks * main.slices;
+  if (p.front_slices > 0) {
+    front.mode = kFront;
+    front.row_blocks = static_cast<int>(ceil_div(span_rows(a, kFront), 64));
+    front.slices = p.front_slices;
+    front.blocks = span_sets(a, kFront) * front.row_blocks * front.slices;
+  }
+#define NTOPS_FEW(NW)                                                                             \
+  if (p.front_slices > 0)                                                                         \
+    return wide ? launch_few<T, D, NW, 4, 4>(a, front, main, part, st) : launch_few<T, D, NW, 4, 1>(a, front, main, part, st); \
+  return wide ? launch_few<T, D, NW, 0, 4>(a, front, main, part, st) : launch_few<T, D, NW, 0, 1>(a, front, main, part, st);
+  if (p.waves == 1) {
+    NTOPS_FEW(1)
+  }
+  NTOPS_FEW(2)
+#undef NTOPS_FEW
+}
+
+}  // namespace
+
+int span_few_run(int dtype, const SpanArgs& a, const FewPlan& p, const SpanPart& part, hipStream_t st) {
+  if (dtype == NTOPS_BF16) return a.D > 64 ? run_few<__bf16, 128>(a, p, part, st) : run_few<__bf16, 64>(a, p, part, st);
+  return a.D > 64 ? run_few<_Float16, 128>(a, p, part, st) : run_few<_Float16, 64>(a, p, part, st);
+}
+
+}  // namespace ntops
