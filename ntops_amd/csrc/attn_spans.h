@@ -245,15 +245,18 @@ __device__ __forceinline__ void span_write_row(const SpanArgs& a, const SpanPart
 // Any types, head dims and layouts: a wave per row and slice.
 int span_rows_run(int dtype, const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st);
 
-// 16-bit types, at most kFewRows rows of a sequence a cache head, layouts that
-// span_matrix_layout takes.  front_slices > 0: the rows of all sequences of a group
-// over their prefix in that many slices, and each sequence's rows over its own keys in
-// `slices`; 0: each sequence's rows over both spans.
+// 16-bit types, at most kFewRows rows of a sequence a cache head.  front_slices > 0:
+// with the rows of all sequences of a group over their prefix, in that many slices that
+// come before the others.
 constexpr int kFewRows = 64;
 struct FewPlan {
   int waves;  // a block, 1 or 2
+  int mode;   // of each sequence's rows
   int front_slices, slices;
 };
 int span_few_run(int dtype, const SpanArgs& a, const FewPlan& p, const SpanPart& part, hipStream_t st);
+
+// The same for any number of rows; kBoth: with equal row strides of both spans.
+int span_tile_run(int dtype, const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st);
 
 }  // namespace ntops

@@ -103,19 +103,20 @@ int launch_rows(const SpanArgs& a, int mode, int slices, const SpanPart& part, h
 // Most keys of the main span that a row sees.
 int64_t main_keys(const SpanArgs& a) { return std::min<int64_t>(a.C, static_cast<int64_t>(a.window) + a.sinks); }
 
-// How a problem is served: on which kernels, and in how many slices of the keys.
-enum Path { kRows, kFew };
+// How a problem is served.  With front_slices the rows of all sequences of a group go
+// over their prefix together, in that many slices, and each sequence's rows over its own
+// keys in `slices`; without, each sequence's rows go over both spans.
+enum Path { kRows, kFew, kTile };
 struct Plan {
-  Path path;
-  int slices;  // of a row, over all launches
-  FewPlan few;
+  Path front, main;  // front: kFew (in one launch with a main of kFew) or kTile
+  int front_slices, slices;
+  int waves;  // of a block of kFew
 };
 
 Plan rows_plan(const SpanArgs& a) {
-  Plan p{kRows, 1, {}};
   const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
-  p.slices = static_cast<int>(std::max<int64_t>(1, std::min({static_cast<int64_t>(kMaxSlices), cu_count_cached() * 8 / rows, (a.P + main_keys(a)) / 128})));
-  return p;
+  const int64_t n = std::min({static_cast<int64_t>(kMaxSlices), cu_count_cached() * 8 / rows, (a.P + main_keys(a)) / 128});
+  return {kRows, kRows, 0, static_cast<int>(std::max<int64_t>(1, n)), 0};
 }
 
 // Slices for `heads` sets of blocks over `keys` keys.
@@ -126,37 +127,47 @@ int few_slices(const SpanArgs& a, int64_t heads, int64_t keys, int waves) {
   return static_cast<int>(std::max<int64_t>(n, 1));
 }
 
-Plan few_plan(const SpanArgs& a) {
-  Plan p{kFew, 1, {}};
-  const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv;
-  const int cus = cu_count_cached();
-  p.few.waves = heads < 2 * cus ? 2 : 1;
-  if (a.P > 0 && a.B > a.G) {
-    // as many keys a block of the prefix as of a sequence
-    const int64_t fsets = span_sets(a, kFront) * ceil_div(span_rows(a, kFront), 64);
-    const int64_t total = fsets * a.P + heads * a.C;
-    const int step = (a.D > 64 ? 32 : 64) * p.few.waves;
-    const int64_t chunk = std::max<int64_t>(4 * step, ceil_div(total, cus * 2));
-    p.few.front_slices = static_cast<int>(std::min<int64_t>(kMaxSlices / 2, ceil_div(a.P, chunk)));
-    p.few.slices = static_cast<int>(std::min<int64_t>(kMaxSlices / 2, std::max<int64_t>(1, ceil_div(a.C, chunk))));
-    p.slices = p.few.front_slices + p.few.slices;
-    return p;
-  }
-  p.few.front_slices = 0;
-  p.few.slices = p.slices = few_slices(a, heads, a.P + main_keys(a), p.few.waves);
-  return p;
+// Slices of a tile launch of `items` blocks of rows over `keys` keys.
+int tile_slices(int64_t items, int64_t keys, int most) {
+  const int64_t n = std::min({static_cast<int64_t>(most), cu_count_cached() / items, ceil_div(keys, 256)});
+  return static_cast<int>(std::max<int64_t>(n, 1));
 }
 
+int64_t row_blocks(const SpanArgs& a, int mode, int rows) { return span_sets(a, mode) * ceil_div(span_rows(a, mode), rows); }
+
 // The plan for this problem where layouts suit the matrix cores, from sizes alone.
-Plan make_plan(int dtype, const SpanArgs& a) {
-  const bool matrix = dtype != NTOPS_F32 && a.D % 8 == 0 && a.D <= 128 && a.C + static_cast<int64_t>(a.P) > 0;
-  if (matrix && span_rows(a, kMain) <= kFewRows) return few_plan(a);
-  return rows_plan(a);
+// `joined`: both spans in one pass (without a workspace, they cannot be parted).
+Plan make_plan(int dtype, const SpanArgs& a, bool joined = false) {
+  if (dtype == NTOPS_F32 || a.D % 8 != 0 || a.D > 128 || static_cast<int64_t>(a.C) + a.P == 0) return rows_plan(a);
+  const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv;
+  const int cus = cu_count_cached();
+  const bool few = span_rows(a, kMain) <= kFewRows;
+  const int waves = heads < 2 * cus ? 2 : 1;
+  if (!joined && a.P > 0 && a.B > a.G) {
+    if (few && span_rows(a, kFront) <= 4 * kFewRows) {
+      // as many keys a block of the prefix as of a sequence
+      const int64_t total = row_blocks(a, kFront, 64) * a.P + heads * a.C;
+      const int step = (a.D > 64 ? 32 : 64) * waves;
+      const int64_t chunk = std::max<int64_t>(4 * step, ceil_div(total, cus * 2));
+      return {kFew, kFew, static_cast<int>(std::min<int64_t>(kMaxSlices / 2, ceil_div(a.P, chunk))),
+              static_cast<int>(std::min<int64_t>(kMaxSlices / 2, std::max<int64_t>(1, ceil_div(a.C, chunk)))), waves};
+    }
+    // tiles of 256 rows and 64 keys, of both spans for each sequence or apart
+    const int64_t both = row_blocks(a, kMain, 256) * (a.P + a.C), front = row_blocks(a, kFront, 256) * a.P;
+    if (few || both > (front + row_blocks(a, kMain, 256) * a.C) * 5 / 4) {
+      const int fs = tile_slices(row_blocks(a, kFront, 256), a.P, kMaxSlices / 2);
+      const int ms = few ? few_slices(a, heads, std::max<int64_t>(a.C, 1), waves) : tile_slices(row_blocks(a, kMain, 256), a.C, kMaxSlices / 2);
+      return {kTile, few ? kFew : kTile, fs, std::min(ms, kMaxSlices / 2), waves};
+    }
+  }
+  if (few) return {kFew, kFew, 0, few_slices(a, heads, a.P + main_keys(a), waves), waves};
+  return {kTile, kTile, 0, tile_slices(row_blocks(a, kMain, 256), a.P + std::min<int64_t>(a.C, main_keys(a) + a.Sq), kMaxSlices), 0};
 }
 
 int64_t plan_bytes(const SpanArgs& a, const Plan& p) {
-  if (p.slices <= 1) return 0;
-  return static_cast<int64_t>(a.B) * a.Hq * a.Sq * p.slices * ((a.D + 3) / 4 * 4 + 2) * 4;
+  const int n = p.front_slices + p.slices;
+  if (n <= 1) return 0;
+  return static_cast<int64_t>(a.B) * a.Hq * a.Sq * n * ((a.D + 3) / 4 * 4 + 2) * 4;
 }
 
 // What the matrix cores' kernels read: unit strides along the head dim, rows at
@@ -178,25 +189,43 @@ bool matrix_layout(const SpanArgs& a) {
   return a.P == 0 || (rows8(a.pkst) && rows8(a.pvst) && aligned16(a.pk) && aligned16(a.pv) && span(a.pkst, a.P) && span(a.pvst, a.P));
 }
 
-int run(int dtype, const SpanArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
+int run(int dtype, SpanArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
+  if (ws == nullptr) ws_bytes = 0;
+  // a span without keys has the other's strides
+  for (int i = 0; i < 4; ++i) {
+    if (a.P == 0) a.pkst[i] = a.kst[i], a.pvst[i] = a.vst[i];
+    if (a.C == 0) a.kst[i] = a.pkst[i], a.vst[i] = a.pvst[i];
+  }
   Plan p = make_plan(dtype, a);
-  if (p.path != kRows && !matrix_layout(a)) {
-    const int64_t room = plan_bytes(a, p);
+  if (plan_bytes(a, p) > ws_bytes) {
+    p = make_plan(dtype, a, true);
+    if (plan_bytes(a, p) > ws_bytes) p.slices = 1;
+  }
+  const bool one_stride = a.pk == nullptr || (a.kst[2] == a.pkst[2] && a.vst[2] == a.pvst[2]);
+  if (p.main != kRows && (!matrix_layout(a) || (p.main == kTile && p.front_slices == 0 && !one_stride))) {
     p = rows_plan(a);
-    if (plan_bytes(a, p) > room) p.slices = 1;  // (the workspace is sized before the layout is known)
+    if (plan_bytes(a, p) > ws_bytes) p.slices = 1;
   }
-  if (p.slices > 1 && (ws == nullptr || ws_bytes < plan_bytes(a, p))) {
-    p.slices = p.few.slices = 1;
-    p.few.front_slices = 0;
-  }
-  const SpanPart part{p.slices > 1 ? static_cast<float*>(ws) : nullptr, p.slices, 0, (a.D + 3) / 4 * 4};
-  if (int e = p.path == kFew ? span_few_run(dtype, a, p.few, part, st) : span_rows_run(dtype, a, kBoth, p.slices, part, st)) return e;
+  const int n = p.front_slices + p.slices;
+  SpanPart part{n > 1 ? static_cast<float*>(ws) : nullptr, n, 0, (a.D + 3) / 4 * 4};
+  const int mode = p.front_slices > 0 ? kMain : kBoth;
+  if (p.front_slices > 0 && p.front == kTile)
+    if (int e = span_tile_run(dtype, a, kFront, p.front_slices, part, st)) return e;
+  part.first = p.front_slices;
+  int e;
+  if (p.main == kRows)
+    e = span_rows_run(dtype, a, mode, p.slices, part, st);
+  else if (p.main == kFew)
+    e = span_few_run(dtype, a, {p.waves, mode, p.front == kFew ? p.front_slices : 0, p.slices}, part, st);
+  else
+    e = span_tile_run(dtype, a, mode, p.slices, part, st);
+  if (e) return e;
   return part.p ? merge(dtype, a, part, st) : NTOPS_OK;
 }
 
 bool sizes_fit(int64_t B, int64_t Hq, int64_t Sq, int64_t C, int64_t P) {
   return B <= kMaxCount && Hq <= kMaxCount && Sq <= kMaxCount / 2 && C <= kMaxCount / 2 && P <= kMaxCount / 2 && B * Hq <= kMaxCount &&
-         B * Hq * Sq <= kMaxCount;
+         B * Hq * Sq <= kMaxCount - 4096;
 }
 
 }  // namespace

@@ -395,10 +395,10 @@ template <typename T, int D>
 int run_few(const SpanArgs& a, const FewPlan& p, const SpanPart& part, hipStream_t st) {
   const bool wide = span_rows(a, kMain) > 16;
   FewBlocks front{}, main{};
-  main.mode = p.front_slices > 0 ? kMain : kBoth;
+  main.mode = p.mode;
   main.row_blocks = static_cast<int>(ceil_div(span_rows(a, main.mode), wide ? 64 : 16));
   main.slices = p.slices;
-  main.first = p.front_slices;
+  main.first = part.first;
   main.blocks = span_sets(a, main.mode) * main.row_blocks * main.slices;
   if (p.front_slices > 0) {
     front.mode = kFront;

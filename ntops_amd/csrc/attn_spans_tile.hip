@@ -1,0 +1,376 @@
+// Many query rows a cache head (prompts, chunks of prompts, all sequences of a shared
+// prefix together): windowed and shared-prefix attention on the matrix cores.
+//
+// A work item is 256 of the rows that share a cache head -- with grouped queries 256 /
+// group tokens, so that the keys that a window leaves to a block are little more than
+// the window -- over the 64-key tiles of both spans, or a slice of them.  Wave w owns
+// rows 32 w .. + 31 with their queries in registers; tiles go global -> LDS by direct
+// DMA into a ring of four stages, two tiles ahead.  The two waves that share a SIMD run
+// half a tile apart: while one runs a matrix phase (O += P_j V_j, then S_{j+1} = Q
+// K_{j+1}^T) the other runs a vector phase (mask, maximum, exponentials, sum, pack P),
+// two barriers a tile.  A wave skips the tiles that none of its rows sees.
+//
+// A row's reference (from which its exponents are taken) follows its maximum when that
+// is past it by more than 2^8.  Masked scores are -inf whatever their key holds; a
+// value that is not finite times P = 0 is NaN, so a row whose result is NaN under a sum
+// that is none is computed again by itself, from the keys that it sees.
+#include <algorithm>
+#include <atomic>
+
+#include "attn_spans.h"
+
+namespace ntops {
+namespace {
+
+constexpr int kRowsBlock = 256;
+constexpr int kWaves = 8;
+constexpr int kKeys = 64;
+constexpr int kStages = 4;
+constexpr int kAhead = 4;  // fragments read ahead of the MFMA that uses them
+constexpr float kSlack = 8.f;
+
+// DMA of one tile of 64 keys of D: 1 KiB an instruction, spread evenly over the waves.
+template <int D, bool IS_V>
+struct SpanDma {
+  static constexpr int kRowsPerInst = 1024 / (D * 2);
+  static constexpr int kInst = kKeys / kRowsPerInst / kWaves;
+  static_assert(kInst >= 1 && kInst * kWaves * kRowsPerInst == kKeys, "tile must split evenly over the waves");
+  uint32_t voff[kInst];
+  int lds_off;
+
+  __device__ __forceinline__ void init(int64_t ld, int wave, int lane, int dt) {
+    lds_off = wave * kInst * 1024;
+    constexpr int cpr = D / 8;
+#pragma unroll
+    for (int i = 0; i < kInst; ++i) {
+      const int row = (wave * kInst + i) * kRowsPerInst + lane / cpr;
+      const int slot = lane % cpr;
+      const int c = IS_V ? vslot<D>(row, slot) : kslot<D>(row, slot);
+      voff[i] = c * 8 < dt ? static_cast<uint32_t>(row * ld * 2 + c * 16) : kOOB;
+    }
+  }
+  // 64 rows from row0 on of `n` at `base` (rows past them are zeros) into the LDS
+  __device__ __forceinline__ void issue(const char* base, int64_t ld, int row0, int n, int dt, uint32_t tile) const {
+    const u32x4 r = make_rsrc(base + row0 * ld * 2, n > row0 ? ((n - row0 - 1) * ld + dt) * 2 : 0);
+#pragma unroll
+    for (int i = 0; i < kInst; ++i) dma16(r, __builtin_amdgcn_readfirstlane(tile + lds_off + i * 1024), voff[i]);
+  }
+};
+
+__device__ __forceinline__ float max32(const f32x16 (&s)[2]) {
+  float v[32];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[16 * u + e] = s[u][e];
+  float m[11];
+#pragma unroll
+  for (int i = 0; i < 10; ++i) m[i] = max3(v[3 * i], v[3 * i + 1], v[3 * i + 2]);
+  m[10] = max3(v[30], v[31], v[31]);
+  return max3(max3(max3(m[0], m[1], m[2]), max3(m[3], m[4], m[5]), m[6]), max3(m[7], m[8], m[9]), m[10]);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kWaves, 1) void k_span_tile(SpanArgs a, int mode, int nqb, int slices, int64_t total, SpanPart part) {
+  constexpr int KS = D / 16;  // k-steps of S = Q K^T
+  constexpr int DT = D / 32;  // 32-column tiles of O
+  constexpr int kTile = kKeys * D * 2;
+  constexpr int kStage = 2 * kTile;                      // K tile, then V tile
+  constexpr int L = 2 * SpanDma<D, false>::kInst;  // DMA instructions per lane per tile
+  static_assert(kStages == 4, "the phases refill the stage of tile k - 2 with tile k + 2");
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int grp = wave >> 2;  // 0: leads, 1: one phase behind (one wave of each per SIMD)
+  const int64_t pid = block_id();
+  if (pid >= total) return;  // the tail of a 2-D grid (the whole block)
+  // An XCD (workgroups go round them) walks whole sets, every eighth one, the rows with
+  // the most keys first.
+  const int per = nqb * slices;
+  int64_t set;
+  int in;
+  if ((total / per & 7) == 0) {
+    const int64_t at = pid >> 3;
+    set = at / per * 8 + (pid & 7);
+    in = static_cast<int>(at % per);
+  } else {
+    set = pid / per;
+    in = static_cast<int>(pid - set * per);
+  }
+  const int qb = nqb - 1 - in / slices, slice = in % slices;
+  const int group = a.Hq / a.Hkv, ro = group * a.Sq;
+  const int nrows = mode == kFront ? ro * (a.B / a.G) : ro;
+  const int r0 = qb * kRowsBlock, r1 = min(r0 + kRowsBlock, nrows);
+  const bool front_only = mode == kFront;
+  const Spans s = make_spans<2>(a, mode, set, front_only ? 0 : r0 / group, front_only ? 0 : (r1 - 1) / group);
+  const int64_t kld = s.kld[front_only ? 0 : 1], vld = s.vld[front_only ? 0 : 1];  // (equal where there are both)
+
+  const int qw = r0 + wave * 32;
+  const bool active = qw < nrows;
+  const int my_r = qw + (lane & 31);
+  const bool in_rows = my_r < nrows;
+  const SpanRow x = span_row(a, s, min(my_r, nrows - 1));
+  const int tw0 = front_only ? 0 : min(qw, nrows - 1) / group, tw1 = front_only ? 0 : min(qw + 31, nrows - 1) / group;
+  // main keys [lo, hi) that some row of the wave sees, and between lo_all and hi_all every row
+  const int w_hi = s.hi(tw1), w_lo = s.lo(tw0), w_hi_all = s.hi(tw0), w_lo_all = s.lo(tw1);
+
+  u32x4 qf[KS];  // Q fragments (A operand of S): row my_r, d = 16 ks + 8 (lane >> 5) .. + 7
+  {
+    const T* Q = static_cast<const T*>(a.q) + x.b * a.qst[0] + x.h * a.qst[1] + x.t * a.qst[2];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d0 = ks * 16 + 8 * (lane >> 5);
+      qf[ks] = in_rows && d0 < a.D ? *reinterpret_cast<const u32x4*>(Q + d0) : u32x4{0, 0, 0, 0};
+      if (a.scale_log2 < 0.f) qf[ks] ^= 0x80008000u;
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[ks]));
+  }
+  // at least the least factor there is, so that a masked score stays -inf under a zero scale
+  const float c = fabsf(a.scale_log2) < 0x1p-126f ? 0x1p-126f : fabsf(a.scale_log2);
+
+  const int nft = (s.n[0] + kKeys - 1) / kKeys, nt = nft + (s.n[1] + kKeys - 1) / kKeys;
+  const int share = (nt + slices - 1) / slices;
+  const int i0 = min(slice * share, nt);
+  const int nkv = min(i0 + share, nt) - i0;  // tiles of this item
+
+  SpanDma<D, false> kd;
+  SpanDma<D, true> vd;
+  kd.init(kld, wave, lane, a.D);
+  vd.init(vld, wave, lane, a.D);
+  const uint32_t smem_addr = lds_addr(smem);
+  // tile g of the item into its stage; past the last: loads of nothing, which still
+  // count in vmcnt
+  const auto dma = [&](int g) __attribute__((always_inline)) {
+    const uint32_t st = smem_addr + static_cast<uint32_t>((g & 3) * kStage);
+    const int i = i0 + g, span = i < nft ? 0 : 1;
+    const int row0 = (span == 0 ? i : i - nft) * kKeys, n = g < nkv ? s.n[span] : 0;
+    kd.issue(s.k[span], kld, row0, n, a.D, st);
+    vd.issue(s.v[span], vld, row0, n, a.D, st + kTile);
+  };
+  // whether the wave has rows that see keys of tile g
+  const auto need = [&](int g) __attribute__((always_inline)) {
+    const int i = i0 + g;
+    if (i < nft) return active;
+    const int k0 = (i - nft) * kKeys;
+    return active && k0 < w_hi && (k0 + kKeys > w_lo || k0 < s.sinks);
+  };
+  // limits of row my_r relative to this lane's column group: element (u, e) of a tile is
+  // its key 32 u + 8 (e >> 2) + (e & 3) past that origin
+  const int my_hi = s.hi(x.t) - 4 * (lane >> 5), my_lo = s.lo(x.t) - 4 * (lane >> 5);
+
+  f32x16 o[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
+  float m_run = neg_inf();  // reference (base 2) of row my_r
+  float l_half = 0.f;       // this lane's half of the row's sum of exponentials
+  f32x16 sc[2];             // S of the tile being softmaxed
+  u32x4 pf[4];              // P of that tile, as MFMA A operands per 16-key slice
+
+  // O += P_j V_j; fragment i + kAhead is read while MFMA i runs, and a scheduling fence
+  // per step pins that order
+  const auto pv_part = [&](int j) __attribute__((always_inline)) {
+    const char* sv = smem + (j & 3) * kStage + kTile;
+    constexpr int nm = 4 * DT;  // MFMA i: key slice i / DT, d tile i % DT
+    u32x4 f[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) f[i] = v_frag<D>(sv, (i % DT) * 32, i / DT, lane);
+#pragma unroll
+    for (int i = 0; i < nm; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      o[i % DT] = mfma32<T>(f[i % kAhead], pf[i / DT], o[i % DT]);
+      if (i + kAhead < nm) f[i % kAhead] = v_frag<D>(sv, ((i + kAhead) % DT) * 32, (i + kAhead) / DT, lane);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // S = Q K_j^T
+  const auto qk_part = [&](int j) __attribute__((always_inline)) {
+    const char* sk = smem + (j & 3) * kStage;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[u][e] = 0.f;
+    constexpr int nm = 2 * KS;  // MFMA i: d slice i / 2, key half i % 2
+    u32x4 f[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) f[i] = k_frag<D>(sk, (i % 2) * 32, i / 2, lane);
+#pragma unroll
+    for (int i = 0; i < nm; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      sc[i % 2] = mfma32<T>(f[i % kAhead], qf[i / 2], sc[i % 2]);
+      if (i + kAhead < nm) f[i % kAhead] = k_frag<D>(sk, ((i + kAhead) % 2) * 32, (i + kAhead) / 2, lane);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // at raised priority: the SIMD issues it ahead of the partner wave's vector phase
+  const auto matrix_phase = [&](int j) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_setprio(1);
+    if (j >= 0 && need(j)) pv_part(j);
+    if (j + 1 < nkv && need(j + 1)) qk_part(j + 1);
+    __builtin_amdgcn_s_setprio(0);
+  };
+  const auto vector_phase = [&](int g) __attribute__((always_inline)) {
+    const int i = i0 + g;
+    const bool front = i < nft;
+    const int k0 = (front ? i : i - nft) * kKeys;
+    const bool whole = front ? k0 + kKeys <= s.n[0] : k0 + kKeys <= w_hi_all && (k0 >= w_lo_all || k0 + kKeys <= s.sinks);
+    if (!whole) {
+      const int up = (front ? s.n[0] - 4 * (lane >> 5) : my_hi) - k0, down = front ? -64 : my_lo - k0;
+      const int sink = s.sinks - 4 * (lane >> 5) - k0;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int k = 32 * u + 8 * (e >> 2) + (e & 3);
+          sc[u][e] = k < up && (k >= down || k < sink) ? sc[u][e] : neg_inf();
+        }
+    }
+    const float th = max32(sc) * c;  // of this lane's half of the row (base 2)
+    if (__any(th > m_run + kSlack)) {
+      const float tmax = fmaxf(th, __shfl_xor(th, 32, 64));
+      const bool up = tmax > m_run + kSlack;
+      const float alpha = up ? fast_exp2(m_run - tmax) : 1.f;
+      m_run = up ? tmax : m_run;
+      l_half *= alpha;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[t][e] *= alpha;
+    }
+    const float mb = m_run == neg_inf() ? 0.f : m_run;  // nothing seen so far: P = 0
+    float p[2][16];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) p[u][e] = fast_exp2(fmaf(sc[u][e], c, -mb));
+    float r[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) r[e] = p[0][e] + p[1][e];
+#pragma unroll
+    for (int w = 8; w >= 1; w >>= 1)
+#pragma unroll
+      for (int e = 0; e < w; ++e) r[e] += r[e + w];
+    l_half += r[0];
+#pragma unroll
+    for (int sl = 0; sl < 4; ++sl) pf[sl] = pack8<T>(&p[sl >> 1][8 * (sl & 1)]);
+  };
+
+  // Period k: group 0 runs the matrix phase of tile k - 1, then the vector phase of tile
+  // k; group 1 the vector phase of tile k - 1, then the matrix phase of tile k - 1.  Tile
+  // k is read from the first phase of period k to the second of period k + 1; at the
+  // start of period k it must have landed, and the stage of tile k - 2 is free.
+  const auto period_start = [&](int k) __attribute__((always_inline)) {
+    wait_vmcnt<L>();  // this wave's part of tile k; tile k + 1 may be in flight
+    block_barrier();
+    dma(k + 2);
+  };
+  if (nkv > 0) {
+    dma(0);
+    dma(1);
+    if (grp == 0) {
+      for (int k = 0; k < nkv; ++k) {
+        period_start(k);
+        matrix_phase(k - 1);
+        block_barrier();
+        if (need(k)) vector_phase(k);
+      }
+      period_start(nkv);
+      if (need(nkv - 1)) pv_part(nkv - 1);
+      block_barrier();
+    } else {
+      for (int k = 0; k < nkv; ++k) {
+        period_start(k);
+        if (k >= 1 && need(k - 1)) vector_phase(k - 1);
+        block_barrier();
+        matrix_phase(k - 1);
+      }
+      period_start(nkv);
+      const bool last = need(nkv - 1);
+      if (last) vector_phase(nkv - 1);
+      block_barrier();
+      if (last) pv_part(nkv - 1);
+    }
+  }
+
+  const float l = l_half + __shfl_xor(l_half, 32, 64);
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // (a NaN sum passes through)
+  // what a row met of values without seeing a key of theirs: nothing
+  const bool none = m_run == neg_inf();
+  float any = 0.f;
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      o[t][e] = none ? 0.f : o[t][e];
+      any += o[t][e];
+    }
+  if (in_rows) {
+    if (part.p) {
+      const int64_t at = part.at(a, x, slice);
+      if (lane < 32) {
+        float* ml = part.ml(a, at);
+        ml[0] = m_run;
+        ml[1] = l;
+      }
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int col = t * 32 + 8 * q + 4 * (lane >> 5);
+          if (col < a.D)
+            *reinterpret_cast<f32x4*>(part.row(at) + col) = f32x4{o[t][4 * q], o[t][4 * q + 1], o[t][4 * q + 2], o[t][4 * q + 3]};
+        }
+    } else {
+      T* O = static_cast<T*>(a.o) + x.b * a.ost[0] + x.h * a.ost[1] + x.t * a.ost[2];
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          T v4[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v4[e] = static_cast<T>(o[t][4 * q + e] * inv);
+          const int col = t * 32 + 8 * q + 4 * (lane >> 5);
+          if (col < a.D)  // a.D % 8 == 0: the 4 columns are all in or all out
+            *reinterpret_cast<u32x2*>(O + col) = __builtin_bit_cast(u32x2, v4);
+        }
+    }
+  }
+  wait_vmcnt<0>();  // no DMA may land after the workgroup ends
+  const uint64_t bad = __ballot(in_rows && !(any == any) && l == l);
+  uint32_t rows = static_cast<uint32_t>(bad) | static_cast<uint32_t>(bad >> 32);
+  while (rows != 0) {
+    const int r = qw + __builtin_ctz(rows);
+    rows &= rows - 1;
+    const SpanRow y = span_row(a, s, r);
+    float ro_[D / 16], rm, rl;
+    span_attend_row<T, D / 16>(a, s, y, min(i0 * kKeys, s.n[0]), min((i0 + nkv) * kKeys, s.n[0]),
+                               max(0, min((i0 - nft) * kKeys, s.n[1])), max(0, min((i0 + nkv - nft) * kKeys, s.n[1])), ro_, rm, rl);
+    span_write_row<T, D / 16>(a, part, y, slice, ro_, rm, rl);
+  }
+}
+
+template <typename T, int D>
+int launch_tile(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
+  constexpr int kLds = kStages * 2 * kKeys * D * 2;
+  auto kern = k_span_tile<T, D>;
+  static std::atomic<uint64_t> done{0};
+  if (int e = reserve_lds(reinterpret_cast<const void*>(kern), kLds, done, "attention")) return e;
+  const int64_t nqb = ceil_div(span_rows(a, mode), kRowsBlock);
+  const int64_t total = span_sets(a, mode) * nqb * slices;
+  note_kernel("%s tile d%d mode%d split%d", a.pk ? "shared_prefix" : "sliding_window", D, mode, slices);
+  hipLaunchKernelGGL(kern, blocks_2d(total), dim3(64 * kWaves), kLds, st, a, mode, static_cast<int>(nqb), slices, total, part);
+  return check_launch("attention");
+}
+
+}  // namespace
+
+int span_tile_run(int dtype, const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
+  if (dtype == NTOPS_BF16)
+    return a.D > 64 ? launch_tile<__bf16, 128>(a, mode, slices, part, st) : launch_tile<__bf16, 64>(a, mode, slices, part, st);
+  return a.D > 64 ? launch_tile<_Float16, 128>(a, mode, slices, part, st) : launch_tile<_Float16, 64>(a, mode, slices, part, st);
+}
+
+}  // namespace ntops
