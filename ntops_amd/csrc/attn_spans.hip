@@ -147,7 +147,7 @@ Plan make_plan(int dtype, const SpanArgs& a, bool joined = false) {
     if (few && span_rows(a, kFront) <= 4 * kFewRows) {
       // as many keys a block of the prefix as of a sequence
       const int64_t total = row_blocks(a, kFront, 64) * a.P + heads * a.C;
-      const int step = (a.D > 64 ? 32 : 64) * waves;
+      const int step = (a.D > 64 ? 32 : 64) * 2;
       const int64_t chunk = std::max<int64_t>(4 * step, ceil_div(total, cus * 2));
       return {kFew, kFew, static_cast<int>(std::min<int64_t>(kMaxSlices / 2, ceil_div(a.P, chunk))),
               static_cast<int>(std::min<int64_t>(kMaxSlices / 2, std::max<int64_t>(1, ceil_div(a.C, chunk)))), waves};
@@ -186,6 +186,8 @@ bool matrix_layout(const SpanArgs& a) {
     const int64_t sinks = std::min<int64_t>(a.C, a.sinks);
     if (!span(a.kst, sinks) || !span(a.vst, sinks)) return false;
   }
+  const int64_t per = a.pk ? a.B / a.G : 1;
+  if ((per - 1) * a.qst[0] + (a.Hq / a.Hkv - 1) * a.qst[1] + (a.Sq - 1) * a.qst[2] + a.D >= 0x3fffffffLL) return false;
   return a.P == 0 || (rows8(a.pkst) && rows8(a.pvst) && aligned16(a.pk) && aligned16(a.pv) && span(a.pkst, a.P) && span(a.pvst, a.P));
 }
 

@@ -17,6 +17,7 @@
 // value that is not finite times P = 0 is NaN, though; a row whose result is NaN under
 // a sum that is none is computed again by itself, from the keys that it sees.
 #include <algorithm>
+#include <atomic>
 
 #include "attn_spans.h"
 
@@ -52,36 +53,44 @@ __device__ __forceinline__ void dma16_once(u32x4 rsrc, uint32_t lds_dst, uint32_
 }
 
 // Loads of one tile's K (or V) rows: 8 instructions of 1 KiB, the swizzle on the global
-// side.
+// side.  Instruction i brings rows kRows i and on: lane l's row is lane / cpr past them,
+// its chunk that of instruction 0, for K with 4 (i & 3) (D = 64: 4 (i & 1)) flipped.
 template <int D, bool IS_V>
 struct TileDma {
   static constexpr int kInst = 8;
   static constexpr int kRows = 512 / D;  // rows per instruction
   u32x4 rsrc;
-  uint32_t ld2;  // bytes from row to row
-  uint32_t voff[kInst];
+  uint32_t ld2;    // bytes from row to row
+  uint32_t row, col;  // bytes of the lane's row and chunk
 
   __device__ __forceinline__ void init(const void* base, int64_t ld, int n, int lane, int dt) {
     rsrc = make_rsrc(base, n > 0 ? ((n - 1) * ld + dt) * 2 : 0);
     ld2 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(ld * 2));
     constexpr int cpr = D / 8;
+    const int r = lane / cpr, slot = lane % cpr;
+    row = r * ld2;
+    col = (IS_V ? vslot<D>(r, slot) : kslot<D>(r, slot)) * 16;
+  }
+  // rows `row0` and on into LDS at `dst`; !valid: loads of nothing, which still count in
+  // vmcnt.  Columns past the head dim: of K zeros; of V whatever follows, which reaches
+  // nothing but the columns of O past the head dim.
+  __device__ __forceinline__ void issue(uint32_t dst, int row0, bool valid, int dt) const {
+    u32x4 r = rsrc;
+    r.z = valid ? r.z : 0u;
+    const uint32_t off = row0 * ld2;
+    if (IS_V || dt == D) {
 #pragma unroll
-    for (int i = 0; i < kInst; ++i) {
-      const int row = i * kRows + lane / cpr;
-      const int slot = lane % cpr;
-      const int c = IS_V ? vslot<D>(row, slot) : kslot<D>(row, slot);
-      voff[i] = c * 8 < dt ? row * ld2 + c * 16 : kOOB;
+      for (int i = 0; i < kInst; ++i)
+        dma16_once(r, dst + i * 1024, (IS_V ? col : col ^ flip(i)) + (row + (off + i * kRows * ld2)));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kInst; ++i) {
+        const uint32_t c = col ^ flip(i);
+        dma16_once(r, dst + i * 1024, c < static_cast<uint32_t>(dt * 2) ? c + (row + (off + i * kRows * ld2)) : kOOB);
+      }
     }
   }
-  // rows `row0` and on into LDS at `dst`; row0 < 0: an empty load, which still counts
-  // in vmcnt
-  __device__ __forceinline__ void issue(uint32_t dst, int row0) const {
-    const uint32_t off = row0 < 0 ? kOOB : row0 * ld2;
-#pragma unroll
-    for (int i = 0; i < kInst; ++i)
-      // kOOB + kOOB would wrap to 0: keep either one
-      dma16_once(rsrc, dst + i * 1024, (voff[i] | off) & kOOB ? kOOB : voff[i] + off);
-  }
+  static constexpr uint32_t flip(int i) { return 64 * (i & (D == 128 ? 3 : 1)); }
 };
 
 // Reads of LDS filled by DMA must not move across the wait that orders them.
@@ -102,6 +111,12 @@ struct FewBlocks {
   int64_t blocks;
 };
 
+// Where the queries lie: up to two groups of rows go to registers, through the LDS of a
+// tile that has not been loaded yet; more stay in the LDS behind the waves' tiles, as
+// fragments, shared by the block.
+template <int D, int RG>
+constexpr int kQueryLds = RG > 2 ? RG * (D / 32) * 1024 : 0;
+
 // RG: groups of 16 rows a block has room for.
 template <typename T, int D, int NW, int RG>
 __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f, SpanPart part, int64_t id, char* smem) {
@@ -109,6 +124,8 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
   constexpr int KB = NK / 16;  // 16-key blocks of a tile
   constexpr int KS = D / 32;   // k-steps of S^T = K Q^T
   constexpr int DT = D / 16;   // 16-row tiles of O^T
+  constexpr bool kShared = RG > 2;
+  static_assert(kShared || RG * KS * 1024 <= 8192, "the queries go through a tile's values");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
@@ -119,42 +136,42 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
   const int group = a.Hq / a.Hkv, ro = group * a.Sq;
   const int set_rows = f.mode == kFront ? ro * (a.B / a.G) : ro;
   const int rows = min(16 * RG, set_rows - r0);
-  const int ng = RG == 1 ? 1 : (rows + 15) / 16;
   const int t0 = f.mode == kFront ? 0 : r0 / group, t1 = f.mode == kFront ? 0 : (r0 + rows - 1) / group;
   const Spans s = make_spans<2>(a, f.mode, set, t0, t1);
   part.first = f.first;
 
+  char* mine = smem + wave * 32768;
+  const uint32_t mine_addr = lds_addr(mine);
+  char* sq = kShared ? smem + NW * 32768 : mine + 16384 + 8192;  // [rg][ks][lane]
   int hi[RG], lo[RG];
-  u32x4 qf[RG][KS];
+  {
+    const T* Q = static_cast<const T*>(a.q) + s.b0 * a.qst[0] + static_cast<int64_t>(s.hk) * group * a.qst[1];
+    const u32x4 rq = make_rsrc(Q, 0x7ffffff0);
+    const uint32_t sq_addr = lds_addr(sq);
 #pragma unroll
-  for (int rg = 0; rg < RG; ++rg) {
-    const int r = rg * 16 + c16;
-    const SpanRow x = span_row(a, s, r0 + min(r, rows - 1));
-    hi[rg] = s.hi(x.t);
-    lo[rg] = s.lo(x.t);
-    const T* Q = static_cast<const T*>(a.q) + x.b * a.qst[0] + x.h * a.qst[1] + x.t * a.qst[2];
+    for (int rg = 0; rg < RG; ++rg) {
+      const int r = rg * 16 + c16;
+      const SpanRow x = span_row(a, s, r0 + min(r, rows - 1));
+      hi[rg] = s.hi(x.t);
+      lo[rg] = s.lo(x.t);
+      const uint32_t off = static_cast<uint32_t>(((x.b - s.b0) * a.qst[0] + (x.h - s.hk * group) * a.qst[1] + x.t * a.qst[2]) * 2);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int d0 = ks * 32 + 8 * g;
-      qf[rg][ks] = r < rows && d0 < a.D ? *reinterpret_cast<const u32x4*>(Q + d0) : u32x4{0, 0, 0, 0};
-      if (a.scale_log2 < 0.f) qf[rg][ks] ^= 0x80008000u;
+      for (int ks = 0; ks < KS; ++ks) {
+        const int d0 = ks * 32 + 8 * g;
+        if (!kShared || (rg * KS + ks) % NW == wave)
+          dma16(rq, __builtin_amdgcn_readfirstlane(sq_addr + (rg * KS + ks) * 1024), r < rows && d0 < a.D ? off + d0 * 2 : kOOB);
+      }
     }
   }
-  // settled here, so that no wait for it is placed among the tile loads
-#pragma unroll
-  for (int rg = 0; rg < RG; ++rg)
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[rg][ks]));
   // at least the least factor there is, so that a masked score stays -inf under a zero scale
   const float c = fabsf(a.scale_log2) < 0x1p-126f ? 0x1p-126f : fabsf(a.scale_log2);
+  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // a negative scale: -Q
   const int hi_min = s.hi(t0), lo_max = s.lo(t1);  // a main tile between them is seen whole by every row
 
   const int nft = (s.n[0] + NK - 1) / NK, nt = nft + (s.n[1] + NK - 1) / NK;
   const int per = (nt + f.slices - 1) / f.slices;
   const int i0 = min(slice * per, nt), i1 = min(i0 + per, nt);
   const int n = i1 - i0 > wave ? (i1 - i0 - wave + NW - 1) / NW : 0;  // tiles of this wave: i0 + wave, + NW, ...
-  char* mine = smem + wave * 32768;
-  const uint32_t mine_addr = lds_addr(mine);
   TileDma<D, false> kd;
   TileDma<D, true> vd;
   const auto tile_at = [&](int j) { return i0 + wave + j * NW; };
@@ -168,7 +185,7 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
       kspan = 1;
       kd.init(s.k[1], s.kld[1], s.n[1], lane, a.D);
     }
-    kd.issue(mine_addr + (j & 1) * 16384, j < n ? (i < nft ? i : i - nft) * NK : -1);
+    kd.issue(mine_addr + (j & 1) * 16384, (i < nft ? i : i - nft) * NK, j < n, a.D);
   };
   const auto issue_v = [&](int j) __attribute__((always_inline)) {
     const int i = tile_at(j);
@@ -176,7 +193,7 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
       vspan = 1;
       vd.init(s.v[1], s.vld[1], s.n[1], lane, a.D);
     }
-    vd.issue(mine_addr + (j & 1) * 16384 + 8192, j < n ? (i < nft ? i : i - nft) * NK : -1);
+    vd.issue(mine_addr + (j & 1) * 16384 + 8192, (i < nft ? i : i - nft) * NK, j < n, a.D);
   };
 
   f32x4 o[RG][DT];
@@ -189,56 +206,89 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
     for (int t = 0; t < DT; ++t) o[rg][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
+  const auto query = [&](int rg, int ks) __attribute__((always_inline)) {
+    return *reinterpret_cast<const u32x4*>(sq + (rg * KS + ks) * 1024 + lane * 16);
+  };
+  u32x4 qf[kShared ? 1 : RG][KS];
   issue_k(0);
   issue_v(0);
   issue_k(1);
-  issue_v(1);
+  if constexpr (kShared) {
+    issue_v(1);
+    wait_dma<32>();  // the wave's part of the queries is in
+    if (flip) {
+#pragma unroll
+      for (int i = 0; i < RG * KS; ++i)
+        if (i % NW == wave) *reinterpret_cast<u32x4*>(sq + i * 1024 + lane * 16) ^= flip;
+      wait_lgkmcnt0();
+    }
+    block_barrier();
+  } else {
+    wait_dma<24>();
+#pragma unroll
+    for (int rg = 0; rg < RG; ++rg)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qf[rg][ks] = query(rg, ks) ^ flip;
+    wait_lgkmcnt0();
+    issue_v(1);
+  }
   for (int j = 0; j < n; ++j) {
     const char* sk = mine + (j & 1) * 16384;
     const char* sv = sk + 8192;
     wait_dma<24>();  // K of tile j is in; its V and tile j + 1 may be in flight
-    f32x4 sc[RG][KB];
-#pragma unroll
-    for (int rg = 0; rg < RG; ++rg)
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) sc[rg][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        const int row = kb * 16 + c16;
-        const u32x4 kf = *reinterpret_cast<const u32x4*>(sk + row * (D * 2) + kslot<D>(row, ks * 4 + g) * 16);
-#pragma unroll
-        for (int rg = 0; rg < RG; ++rg)
-          if (RG == 1 || rg < ng) sc[rg][kb] = mfma16<T>(kf, qf[rg][ks], sc[rg][kb]);
-      }
-    wait_lgkmcnt0();
-    issue_k(j + 2);
-
     // scores of keys kt + 16 kb + 4 g + e of the tile's span
     const int i = tile_at(j);
     const bool front = i < nft;
     const int kt = (front ? i : i - nft) * NK;
     const bool whole = front ? kt + NK <= s.n[0] : kt + NK <= hi_min && (kt >= lo_max || kt + NK <= s.sinks);
+    const bool sinks = !front && kt < s.sinks;
     u32x4 pf[RG][KB / 2];
+    // (the keys' fragments are read again for each group of rows: there are registers for
+    // O alone)
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
-      if (RG > 1 && rg >= ng) continue;
-      if (!whole) {
-        const int up = (front ? s.n[0] : hi[rg]) - kt - 4 * g, down = front ? 0 : lo[rg] - kt - 4 * g, sink = s.sinks - kt - 4 * g;
+      if constexpr (RG > 1) __builtin_amdgcn_sched_barrier(0);
+      f32x4 sc[KB];
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+      for (int kb = 0; kb < KB; ++kb) sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int k = kb * 16 + e;
-            sc[rg][kb][e] = k < up && (k >= down || k < sink) ? sc[rg][kb][e] : neg_inf();
-          }
+      for (int ks = 0; ks < KS; ++ks) {
+        const u32x4 q = kShared ? query(rg, ks) : qf[kShared ? 0 : rg][ks];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          const int row = kb * 16 + c16;
+          const u32x4 kf = *reinterpret_cast<const u32x4*>(sk + row * (D * 2) + kslot<D>(row, ks * 4 + g) * 16);
+          sc[kb] = mfma16<T>(kf, q, sc[kb]);
+        }
       }
-      float mx = fmaxf(sc[rg][0][0], sc[rg][0][1]);
+      if (rg == RG - 1) {
+        wait_lgkmcnt0();
+        issue_k(j + 2);
+      }
+      if (!whole) {
+        const int up = (front ? s.n[0] : hi[rg]) - kt - 4 * g, down = front ? -4 * g : lo[rg] - kt - 4 * g;
+        if (sinks) {
+          const int sink = s.sinks - kt - 4 * g;
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int k = kb * 16 + e;
+              sc[kb][e] = k < up && (k >= down || k < sink) ? sc[kb][e] : neg_inf();
+            }
+        } else {
+          const uint32_t seen = static_cast<uint32_t>(max(0, up - down));
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[kb][e] = static_cast<uint32_t>(kb * 16 + e - down) < seen ? sc[kb][e] : neg_inf();
+        }
+      }
+      float mx = fmaxf(sc[0][0], sc[0][1]);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
-        mx = max3(mx, sc[rg][kb][0], sc[rg][kb][1]);
-        mx = max3(mx, sc[rg][kb][2], sc[rg][kb][3]);
+        mx = max3(mx, sc[kb][0], sc[kb][1]);
+        mx = max3(mx, sc[kb][2], sc[kb][3]);
       }
       mx *= c;
       if (__any(mx > m[rg] + kSlack)) {
@@ -258,7 +308,7 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
       for (int p = 0; p < KB / 2; ++p) {
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = fast_exp2(fmaf(sc[rg][2 * p + (e >> 2)][e & 3], c, -mb));
+        for (int e = 0; e < 8; ++e) x[e] = fast_exp2(fmaf(sc[2 * p + (e >> 2)][e & 3], c, -mb));
         l[rg] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
         pf[rg][p] = pack8<T>(x);  // keys 32 p + 4 g + 0..3 and 32 p + 16 + 4 g + 0..3
       }
@@ -281,8 +331,7 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
         const u32x2 lw = __builtin_bit_cast(u32x2, w[0]), hw = __builtin_bit_cast(u32x2, w[1]);
         const u32x4 vf = {lw.x, lw.y, hw.x, hw.y};
 #pragma unroll
-        for (int rg = 0; rg < RG; ++rg)
-          if (RG == 1 || rg < ng) o[rg][t] = mfma16<T>(vf, pf[rg][p], o[rg][t]);
+        for (int rg = 0; rg < RG; ++rg) o[rg][t] = mfma16<T>(vf, pf[rg][p], o[rg][t]);
       }
     wait_lgkmcnt0();
     issue_v(j + 2);
@@ -297,7 +346,7 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
   constexpr int LD = D + 4;
 #pragma unroll
   for (int rg = 0; rg < RG; ++rg) {
-    if (RG > 1 && rg >= ng) continue;
+    if (rg > 0 && rg * 16 >= rows) continue;
     __syncthreads();
     l[rg] += __shfl_xor(l[rg], 16, 64);
     l[rg] += __shfl_xor(l[rg], 32, 64);
@@ -369,8 +418,8 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
 // RGF, RGM: groups of rows of the blocks over shared prefixes (0: there are none) and
 // of the others.
 template <typename T, int D, int NW, int RGF, int RGM>
-__global__ __launch_bounds__(64 * NW, 1) void k_span_few(SpanArgs a, FewBlocks front, FewBlocks main, SpanPart part) {
-  extern __shared__ __attribute__((aligned(1024))) char smem[];  // [wave][2 stages][K, V]
+__global__ __launch_bounds__(64 * NW, 2) void k_span_few(SpanArgs a, FewBlocks front, FewBlocks main, SpanPart part) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // [wave][2 stages][K, V], queries
   const int64_t id = block_id();
   if (id >= front.blocks + main.blocks) return;  // the tail of a 2-D grid (the whole block)
   if constexpr (RGF > 0) {
@@ -384,37 +433,43 @@ __global__ __launch_bounds__(64 * NW, 1) void k_span_few(SpanArgs a, FewBlocks f
 
 template <typename T, int D, int NW, int RGF, int RGM>
 int launch_few(const SpanArgs& a, const FewBlocks& front, const FewBlocks& main, const SpanPart& part, hipStream_t st) {
-  constexpr int kLds = NW * 32768;
-  static_assert(kLds <= 65536 && (2 * NW * 16 + 4 + NW * 16 * (D + 4)) * 4 <= kLds, "LDS");
-  note_kernel("%s few d%d waves%d rows%d+%d split%d", a.pk ? "shared_prefix" : "sliding_window", D, NW, 16 * RGF, 16 * RGM, part.slices);
-  hipLaunchKernelGGL((k_span_few<T, D, NW, RGF, RGM>), blocks_2d(front.blocks + main.blocks), dim3(64 * NW), kLds, st, a, front, main, part);
+  constexpr int kLds = NW * 32768 + std::max(kQueryLds<D, RGF>, kQueryLds<D, RGM>);
+  static_assert((2 * NW * 16 + 4 + NW * 16 * (D + 4)) * 4 <= NW * 32768, "LDS");
+  auto kern = k_span_few<T, D, NW, RGF, RGM>;
+  if constexpr (kLds > 65536) {
+    static std::atomic<uint64_t> done{0};
+    if (int e = reserve_lds(reinterpret_cast<const void*>(kern), kLds, done, "attention")) return e;
+  }
+  note_kernel("%s few d%d waves%d rows%d+%d split%d+%d", a.pk ? "shared_prefix" : "sliding_window", D, NW, 16 * RGF, 16 * RGM, front.slices,
+              main.slices);
+  hipLaunchKernelGGL(kern, blocks_2d(front.blocks + main.blocks), dim3(64 * NW), kLds, st, a, front, main, part);
   return check_launch("attention");
+}
+
+template <typename T, int D, int NW, int RGF>
+int launch_few(const SpanArgs& a, const FewBlocks& front, const FewBlocks& main, int rows, const SpanPart& part, hipStream_t st) {
+  if (rows <= 16) return launch_few<T, D, NW, RGF, 1>(a, front, main, part, st);
+  if (rows <= 32) return launch_few<T, D, NW, RGF, 2>(a, front, main, part, st);
+  return launch_few<T, D, NW, RGF, 4>(a, front, main, part, st);
 }
 
 template <typename T, int D>
 int run_few(const SpanArgs& a, const FewPlan& p, const SpanPart& part, hipStream_t st) {
-  const bool wide = span_rows(a, kMain) > 16;
   FewBlocks front{}, main{};
   main.mode = p.mode;
-  main.row_blocks = static_cast<int>(ceil_div(span_rows(a, main.mode), wide ? 64 : 16));
+  const int rows = static_cast<int>(span_rows(a, main.mode));  // <= kFewRows: one block of rows a set
+  main.row_blocks = 1;
   main.slices = p.slices;
   main.first = part.first;
-  main.blocks = span_sets(a, main.mode) * main.row_blocks * main.slices;
+  main.blocks = span_sets(a, main.mode) * main.slices;
   if (p.front_slices > 0) {
     front.mode = kFront;
     front.row_blocks = static_cast<int>(ceil_div(span_rows(a, kFront), 64));
     front.slices = p.front_slices;
     front.blocks = span_sets(a, kFront) * front.row_blocks * front.slices;
+    return launch_few<T, D, 2, 4>(a, front, main, rows, part, st);
   }
-#define NTOPS_FEW(NW)                                                                             \
-  if (p.front_slices > 0)                                                                         \
-    return wide ? launch_few<T, D, NW, 4, 4>(a, front, main, part, st) : launch_few<T, D, NW, 4, 1>(a, front, main, part, st); \
-  return wide ? launch_few<T, D, NW, 0, 4>(a, front, main, part, st) : launch_few<T, D, NW, 0, 1>(a, front, main, part, st);
-  if (p.waves == 1) {
-    NTOPS_FEW(1)
-  }
-  NTOPS_FEW(2)
-#undef NTOPS_FEW
+  return p.waves == 1 ? launch_few<T, D, 1, 0>(a, front, main, rows, part, st) : launch_few<T, D, 2, 0>(a, front, main, rows, part, st);
 }
 
 }  // namespace

@@ -6,11 +6,11 @@
 // D / 2 columns, the elements' own columns of tables of D.  In fp32, rounded once.
 // A pair whose position lies outside of the tables is NaN.
 //
-// Vector path: a thread owns 8 (fp32: 4) pairs of a token -- a 16-byte pack of
-// each half, or two packs of interleaved pairs -- gathers their sines and cosines
-// once and rotates up to kHeads heads with them, so that the table's bytes, which
-// are fp32 and come from rows of their own for each axis, are read once for several
-// heads.  Generic path: a thread per pair, any strides.
+// Bound by reading and writing the heads once.  Vector path: a thread owns the pairs of
+// a 16-byte pack of each half of a token's head, or of a pack of interleaved pairs,
+// gathers their sines and cosines once and rotates several heads with them: the tables'
+// bytes, fp32 and from a row of its own for each axis, would otherwise pass the L1 as
+// often as the heads' own.  Generic path: a thread per pair, any strides.
 #include <algorithm>
 
 #include "dispatch.h"
@@ -40,7 +40,7 @@ struct AxesArgs {
   const void* pos;   // (axes, B, S)
   int64_t ps[3];
   int pos_dtype;
-  uint8_t axis[kMaxPairs];
+  alignas(8) uint8_t axis[kMaxPairs];
 };
 
 __device__ __forceinline__ void rotate_pair(float x0, float x1, float c0, float s0, float c1, float s1, float& o0, float& o1) {
@@ -60,6 +60,23 @@ __device__ __forceinline__ void table_at(const AxesArgs& a, int64_t row, int64_t
   const float nan = __builtin_nanf("");
   sn = row < 0 ? nan : static_cast<float>(static_cast<const TT*>(a.sn)[row * a.srs + col]);
   cs = row < 0 ? nan : static_cast<float>(static_cast<const TT*>(a.cs)[row * a.crs + col]);
+}
+
+// N columns of a table's row, at any element.
+template <typename TT, int N>
+__device__ __forceinline__ void load_run(const TT* p, float (&v)[N]) {
+  if constexpr (std::is_same<TT, float>::value && N % 4 == 0) {
+    typedef float Run __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const Run r = reinterpret_cast<const Run*>(p)[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * i + e] = r[e];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = static_cast<float>(p[i]);
+  }
 }
 
 // T: element type, TT: the tables' type.
@@ -90,10 +107,144 @@ __global__ __launch_bounds__(256) void k_rope_axes_generic(AxesArgs a, int64_t p
   }
 }
 
+// Vector path.  A block covers 256 work items: (token, pack j of the head, part of the
+// heads); a thread keeps the sines and cosines of its 8 (fp32: 4) pairs -- of an
+// interleaved pack of V elements V / 2 pairs -- and takes the heads hp, hp + parts, ...
+// of the query and then of the key, kUnroll of them in flight.
+template <typename T, typename TT, bool INTER>
+__global__ __launch_bounds__(256) void k_rope_axes(AxesArgs a, int parts, uint32_t items) {
+  constexpr int V = Pack16<T>::N;
+  constexpr int NP = INTER ? V / 2 : V;  // pairs of a thread
+  constexpr int kUnroll = 2;
+  const uint32_t it = static_cast<uint32_t>(block_id()) * 256 + threadIdx.x;
+  if (it >= items) return;
+  const uint32_t half = static_cast<uint32_t>(a.D / 2), packs = half / NP;
+  const uint32_t j = it % packs;
+  uint32_t r = it / packs;
+  const uint32_t hp = r % parts;
+  r /= parts;
+  const uint32_t S = static_cast<uint32_t>(a.S);
+  const uint32_t tb = r / S, ts = r - tb * S;
+  // heads of both tensors as one list: query heads, then key heads
+  const int hq = static_cast<int>(a.t[0].H), heads = hq + static_cast<int>(a.t[1].H);
+  const T* x[2];
+  T* y[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    x[t] = static_cast<const T*>(a.t[t].x) + tb * a.t[t].xs[0] + ts * a.t[t].xs[1] + (INTER ? j * V : j * NP);
+    y[t] = static_cast<T*>(a.t[t].y) + tb * a.t[t].ys[0] + ts * a.t[t].ys[1] + (INTER ? j * V : j * NP);
+  }
+  Pack16<T> p0[kUnroll], p1[kUnroll];
+  const auto load = [&](int h, Pack16<T>& u, Pack16<T>& w) {
+    const bool k = h >= hq;
+    const T* p = k ? x[1] + (h - hq) * a.t[1].xs[2] : x[0] + h * a.t[0].xs[2];
+    u = load16_nt(p);
+    if constexpr (!INTER) w = load16_nt(p + half);
+  };
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u)
+    if (static_cast<int>(hp) + u * parts < heads) load(hp + u * parts, p0[u], p1[u]);
+
+  float s0[NP], c0[NP], s1[NP], c1[NP];
+  using Axes = std::conditional_t<NP == 8, uint64_t, std::conditional_t<NP == 4, uint32_t, uint16_t>>;
+  const Axes axes = reinterpret_cast<const Axes*>(a.axis)[j];  // of the thread's pairs
+  const uint32_t pair0 = j * NP;
+  if (axes == static_cast<Axes>(static_cast<uint8_t>(axes) * static_cast<Axes>(0x0101010101010101ull)) && !(INTER && a.wide)) {
+    // one position, and runs of the tables' columns
+    const int64_t row = table_row(a, static_cast<uint8_t>(axes), tb, ts);
+    const int64_t so = max(row, int64_t(0)) * a.srs + pair0, co = max(row, int64_t(0)) * a.crs + pair0;
+    if (row >= 0) {
+      load_run<TT, NP>(static_cast<const TT*>(a.sn) + so, s0);
+      load_run<TT, NP>(static_cast<const TT*>(a.cs) + co, c0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) s0[i] = c0[i] = __builtin_nanf("");
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      s1[i] = s0[i];
+      c1[i] = c0[i];
+    }
+    if (a.wide && row >= 0) {
+      load_run<TT, NP>(static_cast<const TT*>(a.sn) + so + half, s1);
+      load_run<TT, NP>(static_cast<const TT*>(a.cs) + co + half, c1);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const uint32_t pair = pair0 + i;
+      const int64_t row = table_row(a, static_cast<uint8_t>(axes >> (8 * i)), tb, ts);
+      const uint32_t d0 = INTER ? 2 * pair : pair, d1 = INTER ? 2 * pair + 1 : pair + half;
+      table_at<TT>(a, row, a.wide ? d0 : pair, s0[i], c0[i]);
+      s1[i] = s0[i];
+      c1[i] = c0[i];
+      if (a.wide) table_at<TT>(a, row, d1, s1[i], c1[i]);
+    }
+  }
+  for (int h0 = hp; h0 < heads; h0 += kUnroll * parts) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int h = h0 + u * parts;
+      if (h >= heads) break;
+      const Pack16<T> v0 = p0[u], v1 = p1[u];
+      if (h + kUnroll * parts < heads) load(h + kUnroll * parts, p0[u], p1[u]);
+      const bool k = h >= hq;
+      T* p = k ? y[1] + (h - hq) * a.t[1].ys[2] : y[0] + h * a.t[0].ys[2];
+      Pack16<T> o0, o1;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        float r0, r1;
+        if constexpr (INTER) {
+          rotate_pair(static_cast<float>(v0.v[2 * i]), static_cast<float>(v0.v[2 * i + 1]), c0[i], s0[i], c1[i], s1[i], r0, r1);
+          o0.v[2 * i] = static_cast<T>(r0);
+          o0.v[2 * i + 1] = static_cast<T>(r1);
+        } else {
+          rotate_pair(static_cast<float>(v0.v[i]), static_cast<float>(v1.v[i]), c0[i], s0[i], c1[i], s1[i], r0, r1);
+          o0.v[i] = static_cast<T>(r0);
+          o1.v[i] = static_cast<T>(r1);
+        }
+      }
+      store16_nt(p, o0);
+      if constexpr (!INTER) store16_nt(p + half, o1);
+    }
+  }
+}
+
 template <typename T, typename TT>
 int run_axes(const AxesArgs& a, hipStream_t st) {
-  const int64_t tokens = a.B * a.S;
-  const int64_t pairs0 = tokens * a.t[0].H * (a.D / 2), pairs = pairs0 + tokens * a.t[1].H * (a.D / 2);
+  constexpr int V = Pack16<T>::N;
+  const int64_t tokens = a.B * a.S, heads = a.t[0].H + a.t[1].H;
+  bool vec = (a.D / 2) % (a.interleaved ? V / 2 : V) == 0;
+  for (const AxesTensor& d : a.t) {
+    if (d.H == 0) continue;
+    vec = vec && d.xs[3] == 1 && d.ys[3] == 1 && aligned16(d.x) && aligned16(d.y);
+    for (int k = 0; k < 3; ++k) vec = vec && d.xs[k] % V == 0 && d.ys[k] % V == 0;
+  }
+  const int64_t packs = a.D / 2 / (a.interleaved ? V / 2 : V);
+  if (vec) {
+    // Heads of a thread: as many as leave every CU five blocks, which its registers hold,
+    // at most four -- where a thread's pairs belong to several axes, so that it gathers
+    // each by itself, eight.  (4, 4096, 32 + 8, 128) bf16, 1 / 2 / 4 / 8 / 20 heads: 75.1 /
+    // 63.3 / 60.5 / 62.3 / 71.6 us (344 MB, 5.7 TB/s; a copy of as much takes 64), pairs of
+    // axes in turn 175.9 / 110.7 / 85.7 / 76.5 / 78.9; f32 122.5 / 115.3 / 114.3 / 118.8 / 130.5.
+    const int np = a.interleaved ? V / 2 : V;
+    bool runs = true;
+    for (int i = 0; i < a.D / 2; ++i) runs = runs && a.axis[i] == a.axis[i - i % np];
+    const int64_t blocks = static_cast<int64_t>(cu_count_cached()) * 5;
+    const int64_t per = std::max<int64_t>(1, std::min<int64_t>({heads, tokens * packs * heads / (256 * blocks), runs ? 4 : 8}));
+    const int64_t parts = ceil_div(heads, per);
+    const int64_t items = tokens * packs * parts;
+    if (items < 0xffffff00LL) {
+      note_kernel("rope_axes heads%lld", static_cast<long long>(per));
+      const dim3 grid = blocks_2d(ceil_div(items, 256));
+      if (a.interleaved)
+        hipLaunchKernelGGL((k_rope_axes<T, TT, true>), grid, dim3(256), 0, st, a, static_cast<int>(parts), static_cast<uint32_t>(items));
+      else
+        hipLaunchKernelGGL((k_rope_axes<T, TT, false>), grid, dim3(256), 0, st, a, static_cast<int>(parts), static_cast<uint32_t>(items));
+      return check_launch("rope_axes");
+    }
+  }
+  const int64_t pairs0 = tokens * a.t[0].H * (a.D / 2), pairs = tokens * heads * (a.D / 2);
   note_kernel("rope_axes generic");
   hipLaunchKernelGGL((k_rope_axes_generic<T, TT>), blocks_2d(std::min<int64_t>(ceil_div(pairs, 256), 1 << 20)), dim3(256), 0, st, a, pairs0,
                      pairs);
