@@ -243,74 +243,99 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
     const bool whole = front ? kt + NK <= s.n[0] : kt + NK <= hi_min && (kt >= lo_max || kt + NK <= s.sinks);
     const bool sinks = !front && kt < s.sinks;
     u32x4 pf[RG][KB / 2];
-    // (the keys' fragments are read again for each group of rows: there are registers for
-    // O alone)
+    // Two groups of rows side by side, which hide each other's latencies: a SIMD has this
+    // wave alone.  (The keys' fragments are read again for each pair: there are registers
+    // for O alone.)
+    constexpr int PG = RG > 1 ? 2 : 1;
 #pragma unroll
-    for (int rg = 0; rg < RG; ++rg) {
+    for (int rg0 = 0; rg0 < RG; rg0 += PG) {
       if constexpr (RG > 1) __builtin_amdgcn_sched_barrier(0);
-      f32x4 sc[KB];
+      f32x4 sc[PG][KB];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < PG; ++u)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) sc[u][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const u32x4 q = kShared ? query(rg, ks) : qf[kShared ? 0 : rg][ks];
+        u32x4 q[PG];
+#pragma unroll
+        for (int u = 0; u < PG; ++u) q[u] = kShared ? query(rg0 + u, ks) : qf[kShared ? 0 : rg0 + u][ks];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           const int row = kb * 16 + c16;
           const u32x4 kf = *reinterpret_cast<const u32x4*>(sk + row * (D * 2) + kslot<D>(row, ks * 4 + g) * 16);
-          sc[kb] = mfma16<T>(kf, q, sc[kb]);
+#pragma unroll
+          for (int u = 0; u < PG; ++u) sc[u][kb] = mfma16<T>(kf, q[u], sc[u][kb]);
         }
       }
-      if (rg == RG - 1) {
+      if (rg0 + PG == RG) {
         wait_lgkmcnt0();
         issue_k(j + 2);
       }
       if (!whole) {
-        const int up = (front ? s.n[0] : hi[rg]) - kt - 4 * g, down = front ? -4 * g : lo[rg] - kt - 4 * g;
-        if (sinks) {
-          const int sink = s.sinks - kt - 4 * g;
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
+        for (int u = 0; u < PG; ++u) {
+          const int rg = rg0 + u;
+          const int up = (front ? s.n[0] : hi[rg]) - kt - 4 * g, down = front ? -4 * g : lo[rg] - kt - 4 * g;
+          if (sinks) {
+            const int sink = s.sinks - kt - 4 * g;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int k = kb * 16 + e;
-              sc[kb][e] = k < up && (k >= down || k < sink) ? sc[kb][e] : neg_inf();
-            }
-        } else {
-          const uint32_t seen = static_cast<uint32_t>(max(0, up - down));
+            for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
+              for (int e = 0; e < 4; ++e) {
+                const int k = kb * 16 + e;
+                sc[u][kb][e] = k < up && (k >= down || k < sink) ? sc[u][kb][e] : neg_inf();
+              }
+          } else {
+            const uint32_t seen = static_cast<uint32_t>(max(0, up - down));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[kb][e] = static_cast<uint32_t>(kb * 16 + e - down) < seen ? sc[kb][e] : neg_inf();
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sc[u][kb][e] = static_cast<uint32_t>(kb * 16 + e - down) < seen ? sc[u][kb][e] : neg_inf();
+          }
         }
       }
-      float mx = fmaxf(sc[0][0], sc[0][1]);
+      float mx[PG];
+      bool raise = false;
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        mx = max3(mx, sc[kb][0], sc[kb][1]);
-        mx = max3(mx, sc[kb][2], sc[kb][3]);
+      for (int u = 0; u < PG; ++u) {
+        float top[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          top[kb] = max3(sc[u][kb][0], sc[u][kb][1], sc[u][kb][2]);
+          top[kb] = max3(top[kb], sc[u][kb][3], kb > 0 ? top[kb - 1] : top[kb]);
+        }
+        mx[u] = top[KB - 1] * c;
+        raise = raise || mx[u] > m[rg0 + u] + kSlack;
       }
-      mx *= c;
-      if (__any(mx > m[rg] + kSlack)) {
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const bool up = mx > m[rg] + kSlack;
-        const float alpha = up ? fast_exp2(m[rg] - mx) : 1.f;
-        m[rg] = up ? mx : m[rg];
-        l[rg] *= alpha;
+      if (__any(raise)) {
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+        for (int u = 0; u < PG; ++u) {
+          const int rg = rg0 + u;
+          mx[u] = fmaxf(mx[u], __shfl_xor(mx[u], 16, 64));
+          mx[u] = fmaxf(mx[u], __shfl_xor(mx[u], 32, 64));
+          const bool up = mx[u] > m[rg] + kSlack;
+          const float alpha = up ? fast_exp2(m[rg] - mx[u]) : 1.f;
+          m[rg] = up ? mx[u] : m[rg];
+          l[rg] *= alpha;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[rg][t][e] *= alpha;
+          for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[rg][t][e] *= alpha;
+        }
       }
-      const float mb = m[rg] == neg_inf() ? 0.f : m[rg];  // nothing seen so far: P = 0
 #pragma unroll
-      for (int p = 0; p < KB / 2; ++p) {
-        float x[8];
+      for (int u = 0; u < PG; ++u) {
+        const int rg = rg0 + u;
+        const float mb = m[rg] == neg_inf() ? 0.f : m[rg];  // nothing seen so far: P = 0
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = fast_exp2(fmaf(sc[2 * p + (e >> 2)][e & 3], c, -mb));
-        l[rg] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-        pf[rg][p] = pack8<T>(x);  // keys 32 p + 4 g + 0..3 and 32 p + 16 + 4 g + 0..3
+        for (int p = 0; p < KB / 2; ++p) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = fast_exp2(fmaf(sc[u][2 * p + (e >> 2)][e & 3], c, -mb));
+          l[rg] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+          pf[rg][p] = pack8<T>(x);  // keys 32 p + 4 g + 0..3 and 32 p + 16 + 4 g + 0..3
+        }
       }
     }
 
