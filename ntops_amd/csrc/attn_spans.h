@@ -141,15 +141,14 @@ struct SpanPart {
 
 // One query row by one wave, fp32 throughout, any head dim up to 16 EL and any
 // strides; reads nothing that the row does not see.  Sixteen lanes share a key
-// (lane i the columns i + 16 u), four keys side by side, kUnroll of them in
-// flight each; the four streams of keys are joined at the end.  Every lane ends
-// with the whole row: o[u] of column (lane & 15) + 16 u.
+// (lane i the columns i + 16 u), four keys side by side, UNROLL of them in flight
+// each; the four streams of keys are joined at the end.  Every lane ends with the
+// whole row: o[u] of column (lane & 15) + 16 u.
 //
 // Front keys [f0, f1) and main keys [m0, m1) of what the row sees.
-template <typename T, int EL>
+template <typename T, int EL, int UNROLL>
 __device__ __forceinline__ void span_attend_row(const SpanArgs& a, const Spans& s, const SpanRow x, int f0, int f1, int m0,
                                              int m1, float (&o)[EL], float& m, float& l) {
-  constexpr int kUnroll = EL > 8 ? 2 : 4;
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   float q[EL];
   const T* Q = static_cast<const T*>(a.q) + x.b * a.qst[0] + x.h * a.qst[1] + x.t * a.qst[2];
@@ -170,10 +169,10 @@ __device__ __forceinline__ void span_attend_row(const SpanArgs& a, const Spans& 
     const int k1 = part == 0 ? min(f1, s.n[0]) : part == 1 ? min(m1, min(lo, min(s.sinks, hi))) : min(m1, hi);
     const T* K = reinterpret_cast<const T*>(s.k[sp]);
     const T* V = reinterpret_cast<const T*>(s.v[sp]);
-    for (int k = k0 + g; k < k1; k += 4 * kUnroll) {
-      float kv[kUnroll][EL], vv[kUnroll][EL];
+    for (int k = k0 + g; k < k1; k += 4 * UNROLL) {
+      float kv[UNROLL][EL], vv[UNROLL][EL];
 #pragma unroll
-      for (int w = 0; w < kUnroll; ++w) {
+      for (int w = 0; w < UNROLL; ++w) {
         const int64_t key = k + 4 * w;
         const bool in = key < k1;
 #pragma unroll
@@ -184,7 +183,7 @@ __device__ __forceinline__ void span_attend_row(const SpanArgs& a, const Spans& 
         }
       }
 #pragma unroll
-      for (int w = 0; w < kUnroll; ++w) {
+      for (int w = 0; w < UNROLL; ++w) {
         float d = 0.f;
 #pragma unroll
         for (int u = 0; u < EL; ++u) d = fmaf(q[u], kv[w][u], d);
@@ -258,5 +257,10 @@ int span_few_run(int dtype, const SpanArgs& a, const FewPlan& p, const SpanPart&
 
 // The same for any number of rows; kBoth: with equal row strides of both spans.
 int span_tile_run(int dtype, const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st);
+
+// fp32, head dims up to 128 that are multiples of 4, rows at multiples of 16 bytes: any
+// number of rows, in blocks of kF32Rows.
+constexpr int kF32Rows = 128;
+int span_f32_run(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st);
 
 }  // namespace ntops

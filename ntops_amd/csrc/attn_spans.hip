@@ -7,6 +7,8 @@
 //     prefix: every key of the prefix, and its own sequence's keys j <= p
 //   A row that sees no key is 0.
 #include <algorithm>
+#include <cstdio>
+#include <cstdlib>
 
 #include "attn_spans.h"
 
@@ -33,7 +35,7 @@ __global__ __launch_bounds__(256) void k_span_rows(SpanArgs a, int mode, int sli
   const SpanRow x = span_row(a, s, r);
   const int fc = (s.n[0] + slices - 1) / slices, mc = (s.n[1] + slices - 1) / slices;
   float o[EL], m, l;
-  span_attend_row<T, EL>(a, s, x, min(slice * fc, s.n[0]), min(slice * fc + fc, s.n[0]), min(slice * mc, s.n[1]), min(slice * mc + mc, s.n[1]),
+  span_attend_row<T, EL, (EL > 8 ? 2 : 4)>(a, s, x, min(slice * fc, s.n[0]), min(slice * fc + fc, s.n[0]), min(slice * mc, s.n[1]), min(slice * mc + mc, s.n[1]),
                          o, m, l);
   span_write_row<T, EL>(a, part, x, slice, o, m, l);
 }
@@ -106,7 +108,7 @@ int64_t main_keys(const SpanArgs& a) { return std::min<int64_t>(a.C, static_cast
 // How a problem is served.  With front_slices the rows of all sequences of a group go
 // over their prefix together, in that many slices, and each sequence's rows over its own
 // keys in `slices`; without, each sequence's rows go over both spans.
-enum Path { kRows, kFew, kTile };
+enum Path { kRows, kFew, kTile, kF32 };
 struct Plan {
   Path front, main;  // front: kFew (in one launch with a main of kFew) or kTile
   int front_slices, slices;
@@ -133,12 +135,31 @@ int tile_slices(int64_t items, int64_t keys, int most) {
   return static_cast<int>(std::max<int64_t>(n, 1));
 }
 
+// Blocks of `rows` rows.
 int64_t row_blocks(const SpanArgs& a, int mode, int rows) { return span_sets(a, mode) * ceil_div(span_rows(a, mode), rows); }
+
+// fp32: blocks of kF32Rows rows, two a CU.
+Plan f32_plan(const SpanArgs& a, bool joined) {
+  const int64_t blocks = 2 * cu_count_cached();
+  const auto slices = [&](int64_t items, int64_t keys, int most) {
+    const int64_t n = std::min({static_cast<int64_t>(most), blocks / items, ceil_div(keys, 128)});
+    return static_cast<int>(std::max<int64_t>(n, 1));
+  };
+  const int64_t main = row_blocks(a, kMain, kF32Rows);
+  if (!joined && a.P > 0 && a.B > a.G) {
+    const int64_t front = row_blocks(a, kFront, kF32Rows);
+    if (main * a.P > front * a.P + (front * a.P + main * a.C) / 4)
+      return {kF32, kF32, slices(front, a.P, kMaxSlices / 2), slices(main, a.C, kMaxSlices / 2), 0};
+  }
+  return {kF32, kF32, 0, slices(main, a.P + std::min<int64_t>(a.C, main_keys(a) + a.Sq), kMaxSlices), 0};
+}
 
 // The plan for this problem where layouts suit the matrix cores, from sizes alone.
 // `joined`: both spans in one pass (without a workspace, they cannot be parted).
 Plan make_plan(int dtype, const SpanArgs& a, bool joined = false) {
-  if (dtype == NTOPS_F32 || a.D % 8 != 0 || a.D > 128 || static_cast<int64_t>(a.C) + a.P == 0) return rows_plan(a);
+  if (const char* env = getenv("NT_PLAN")) { int f, m, fs, ms, w; if (sscanf(env, "%d,%d,%d,%d,%d", &f, &m, &fs, &ms, &w) == 5) return {(Path)f, (Path)m, fs, ms, w}; }
+  if (a.D > 128 || a.D % (dtype == NTOPS_F32 ? 4 : 8) != 0 || static_cast<int64_t>(a.C) + a.P == 0) return rows_plan(a);
+  if (dtype == NTOPS_F32) return f32_plan(a, joined);
   const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv;
   const int cus = cu_count_cached();
   const bool few = span_rows(a, kMain) <= kFewRows;
@@ -171,24 +192,26 @@ int64_t plan_bytes(const SpanArgs& a, const Plan& p) {
 }
 
 // What the matrix cores' kernels read: unit strides along the head dim, rows at
-// multiples of 16 bytes that do not overlap, and every offset within a span of a head
-// below 2^31 bytes.
-bool matrix_layout(const SpanArgs& a) {
-  const auto rows8 = [](const int64_t* s) { return s[3] == 1 && s[2] % 8 == 0 && s[1] % 8 == 0 && s[0] % 8 == 0; };
-  const auto span = [&](const int64_t* s, int64_t keys) { return s[2] >= a.D && (keys + 256) * s[2] * 2 < 0x7fffffffLL; };
-  if (!rows8(a.qst) || !aligned16(a.q) || a.ost[3] != 1 || a.ost[2] % 4 != 0 || a.ost[1] % 4 != 0 || a.ost[0] % 4 != 0 ||
-      (reinterpret_cast<uintptr_t>(a.o) & 7u) != 0)
+// multiples of 16 bytes that do not overlap, and for 16-bit types every offset within a
+// span of a head below 2^31 bytes.
+bool matrix_layout(const SpanArgs& a, int dtype) {
+  const bool f32 = dtype == NTOPS_F32;
+  const int pack = f32 ? 4 : 8;
+  const auto rows16 = [&](const int64_t* s) { return s[3] == 1 && s[2] % pack == 0 && s[1] % pack == 0 && s[0] % pack == 0; };
+  const auto span = [&](const int64_t* s, int64_t keys) { return f32 || (s[2] >= a.D && (keys + 256) * s[2] * 2 < 0x7fffffffLL); };
+  if (!rows16(a.qst) || !aligned16(a.q) || a.ost[3] != 1 || a.ost[2] % 4 != 0 || a.ost[1] % 4 != 0 || a.ost[0] % 4 != 0 ||
+      (reinterpret_cast<uintptr_t>(a.o) & (f32 ? 15u : 7u)) != 0)
     return false;
   const int64_t keys = std::min<int64_t>(a.C, static_cast<int64_t>(a.window) + a.Sq);
-  if (a.C > 0 && (!rows8(a.kst) || !rows8(a.vst) || !aligned16(a.k) || !aligned16(a.v) || !span(a.kst, keys) || !span(a.vst, keys)))
+  if (a.C > 0 && (!rows16(a.kst) || !rows16(a.vst) || !aligned16(a.k) || !aligned16(a.v) || !span(a.kst, keys) || !span(a.vst, keys)))
     return false;
   if (a.C > 0 && a.sinks > 0) {
     const int64_t sinks = std::min<int64_t>(a.C, a.sinks);
     if (!span(a.kst, sinks) || !span(a.vst, sinks)) return false;
   }
   const int64_t per = a.pk ? a.B / a.G : 1;
-  if ((per - 1) * a.qst[0] + (a.Hq / a.Hkv - 1) * a.qst[1] + (a.Sq - 1) * a.qst[2] + a.D >= 0x3fffffffLL) return false;
-  return a.P == 0 || (rows8(a.pkst) && rows8(a.pvst) && aligned16(a.pk) && aligned16(a.pv) && span(a.pkst, a.P) && span(a.pvst, a.P));
+  if (!f32 && (per - 1) * a.qst[0] + (a.Hq / a.Hkv - 1) * a.qst[1] + (a.Sq - 1) * a.qst[2] + a.D >= 0x3fffffffLL) return false;
+  return a.P == 0 || (rows16(a.pkst) && rows16(a.pvst) && aligned16(a.pk) && aligned16(a.pv) && span(a.pkst, a.P) && span(a.pvst, a.P));
 }
 
 int run(int dtype, SpanArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
@@ -204,21 +227,24 @@ int run(int dtype, SpanArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
     if (plan_bytes(a, p) > ws_bytes) p.slices = 1;
   }
   const bool one_stride = a.pk == nullptr || (a.kst[2] == a.pkst[2] && a.vst[2] == a.pvst[2]);
-  if (p.main != kRows && (!matrix_layout(a) || (p.main == kTile && p.front_slices == 0 && !one_stride))) {
+  if (p.main != kRows && (!matrix_layout(a, dtype) || (p.main == kTile && p.front_slices == 0 && !one_stride))) {
     p = rows_plan(a);
     if (plan_bytes(a, p) > ws_bytes) p.slices = 1;
   }
   const int n = p.front_slices + p.slices;
   SpanPart part{n > 1 ? static_cast<float*>(ws) : nullptr, n, 0, (a.D + 3) / 4 * 4};
   const int mode = p.front_slices > 0 ? kMain : kBoth;
-  if (p.front_slices > 0 && p.front == kTile)
-    if (int e = span_tile_run(dtype, a, kFront, p.front_slices, part, st)) return e;
+  if (p.front_slices > 0 && p.front != kFew)
+    if (int e = p.front == kF32 ? span_f32_run(a, kFront, p.front_slices, part, st) : span_tile_run(dtype, a, kFront, p.front_slices, part, st))
+      return e;
   part.first = p.front_slices;
   int e;
   if (p.main == kRows)
     e = span_rows_run(dtype, a, mode, p.slices, part, st);
   else if (p.main == kFew)
     e = span_few_run(dtype, a, {p.waves, mode, p.front == kFew ? p.front_slices : 0, p.slices}, part, st);
+  else if (p.main == kF32)
+    e = span_f32_run(a, mode, p.slices, part, st);
   else
     e = span_tile_run(dtype, a, mode, p.slices, part, st);
   if (e) return e;

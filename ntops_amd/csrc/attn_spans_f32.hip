@@ -1,0 +1,249 @@
+// fp32 windowed and shared-prefix attention on the matrix cores: IEEE fp32 products
+// (v_mfma_f32_16x16x4_f32) with fp32 sums.
+//
+// A block is 16 rows a wave of those that share a cache head, over the 32-key tiles of
+// both spans or a slice of them.  The scores are computed transposed, S^T = K Q^T: lane
+// l's accumulator r holds key 4 (l >> 4) + r of a 16-key block for row l & 15, which is
+// the B operand of O^T += V^T P^T for MFMA step r when the keys of that step are taken as
+// 4 (l >> 4) + r (a sum over keys does not depend on their order), so P never leaves the
+// registers, and every accumulator of a lane belongs to one row.  The head dim is walked
+// as d = 16 t + 4 g + e (g = l >> 4, e the step of four), so a lane reads four floats per
+// four MFMAs.  K and V^T tiles are double-buffered in the LDS; a tile's loads go to
+// registers before the previous tile's products and are stored after them, one barrier a
+// tile.  Bound by the fp32 matrix rate, a sixteenth of the 16-bit one, and, with few
+// rows, by the loads.
+//
+// What a row does not see: as in attn_spans_tile.hip.
+#include <algorithm>
+#include <atomic>
+
+#include "attn_spans.h"
+
+namespace ntops {
+namespace {
+
+constexpr int kKeys = 32;
+
+template <int DP>
+constexpr int kLdsBytes = 2 * (kKeys * (DP + 4) + DP * (kKeys + 4)) * 4;
+
+template <int DP, int NW>
+__global__ __launch_bounds__(64 * NW, 4) void k_span_f32(SpanArgs a, int mode, int nqb, int slices, int64_t total, SpanPart part) {
+  constexpr int QB = 16 * NW;
+  constexpr int KP = DP + 4;     // floats per K row in the LDS
+  constexpr int VP = kKeys + 4;  // floats per V^T row
+  constexpr int kKTile = kKeys * KP, kBuf = kKTile + DP * VP;
+  constexpr int kThreads = 64 * NW;
+  constexpr int kF4 = kKeys * DP / 4;                   // 16-byte chunks per operand and tile
+  constexpr int kLd = (kF4 + kThreads - 1) / kThreads;  // per thread
+  extern __shared__ __attribute__((aligned(16))) float sm[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, g = lane >> 4;
+  const int64_t pid = block_id();
+  if (pid >= total) return;  // the tail of a 2-D grid (the whole block)
+  const int per = nqb * slices;
+  const int64_t set = pid / per;
+  const int in = static_cast<int>(pid - set * per);
+  const int qb = nqb - 1 - in / slices, slice = in % slices;
+  const int group = a.Hq / a.Hkv, ro = group * a.Sq;
+  const bool front_only = mode == kFront;
+  const int nrows = front_only ? ro * (a.B / a.G) : ro;
+  const int r0 = qb * QB, r1 = min(r0 + QB, nrows);
+  const Spans s = make_spans<4>(a, mode, set, front_only ? 0 : r0 / group, front_only ? 0 : (r1 - 1) / group);
+
+  const int qw = r0 + wave * 16;
+  const bool active = qw < nrows;
+  const bool in_rows = qw + r16 < nrows;
+  const SpanRow x = span_row(a, s, min(qw + r16, nrows - 1));
+  const int tw0 = front_only ? 0 : min(qw, nrows - 1) / group, tw1 = front_only ? 0 : min(qw + 15, nrows - 1) / group;
+  const int w_hi = s.hi(tw1), w_lo = s.lo(tw0), w_hi_all = s.hi(tw0), w_lo_all = s.lo(tw1);
+  const int my_hi = s.hi(x.t) - 4 * g, my_lo = s.lo(x.t) - 4 * g;
+  f32x4 qf[DP / 16];
+  {
+    const float* Q = static_cast<const float*>(a.q) + x.b * a.qst[0] + x.h * a.qst[1] + x.t * a.qst[2];
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) {
+      const int d = 16 * t + 4 * g;
+      qf[t] = in_rows && d < a.D ? *reinterpret_cast<const f32x4*>(Q + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
+  const int nft = (s.n[0] + kKeys - 1) / kKeys, nt = nft + (s.n[1] + kKeys - 1) / kKeys;
+  const int share = (nt + slices - 1) / slices;
+  const int i0 = min(slice * share, nt);
+  const int nkv = min(i0 + share, nt) - i0;
+
+  f32x4 kst[kLd], vst[kLd];
+  const auto load_tile = [&](int t) __attribute__((always_inline)) {
+    const int i = i0 + t, sp = i < nft ? 0 : 1;
+    const int row0 = (sp == 0 ? i : i - nft) * kKeys;
+    const float* K = reinterpret_cast<const float*>(s.k[sp]);
+    const float* V = reinterpret_cast<const float*>(s.v[sp]);
+#pragma unroll
+    for (int j = 0; j < kLd; ++j) {
+      const int f = threadIdx.x + kThreads * j;
+      const int key = row0 + f / (DP / 4), d = 4 * (f % (DP / 4));
+      const bool ok = f < kF4 && key < s.n[sp] && d < a.D;
+      f32x4 kz = {0.f, 0.f, 0.f, 0.f}, vz = {0.f, 0.f, 0.f, 0.f};
+      if (ok) {
+        kz = *reinterpret_cast<const f32x4*>(K + key * s.kld[sp] + d);
+        vz = *reinterpret_cast<const f32x4*>(V + key * s.vld[sp] + d);
+      }
+      kst[j] = kz;
+      vst[j] = vz;
+    }
+  };
+  const auto store_tile = [&](int buf) __attribute__((always_inline)) {
+    float* kt = sm + buf * kBuf;
+    float* vt = kt + kKTile;
+#pragma unroll
+    for (int j = 0; j < kLd; ++j) {
+      const int f = threadIdx.x + kThreads * j;
+      if (f >= kF4) break;
+      const int kl = f / (DP / 4), d = 4 * (f % (DP / 4));
+      *reinterpret_cast<f32x4*>(kt + kl * KP + d) = kst[j];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) vt[(d + e) * VP + kl] = vst[j][e];
+    }
+  };
+
+  f32x4 o[DP / 16];
+#pragma unroll
+  for (int i = 0; i < DP / 16; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = neg_inf(), l = 0.f;
+  if (nkv > 0) {
+    load_tile(0);
+    store_tile(0);
+  }
+  __syncthreads();
+  for (int t = 0; t < nkv; ++t) {
+    if (t + 1 < nkv) load_tile(t + 1);
+    const float* kt = sm + (t & 1) * kBuf;
+    const float* vt = kt + kKTile;
+    const int i = i0 + t;
+    const bool front = i < nft;
+    const int k0 = (front ? i : i - nft) * kKeys;
+    if (active && (front || (k0 < w_hi && (k0 + kKeys > w_lo || k0 < s.sinks)))) {  // wave-uniform
+      f32x4 sc[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int tt = 0; tt < DP / 16; ++tt)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const f32x4 kf = *reinterpret_cast<const f32x4*>(kt + (kb * 16 + r16) * KP + 16 * tt + 4 * g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[tt][e], sc[kb], 0, 0, 0);
+        }
+      const bool whole = front ? k0 + kKeys <= s.n[0] : k0 + kKeys <= w_hi_all && (k0 >= w_lo_all || k0 + kKeys <= s.sinks);
+      const int up = (front ? s.n[0] - 4 * g : my_hi) - k0, down = front ? -4 * g : my_lo - k0, sink = s.sinks - 4 * g - k0;
+      float mx = neg_inf();
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int k = kb * 16 + r;
+          float v = sc[kb][r] * a.scale_log2;
+          if (!whole) v = k < up && (k >= down || k < sink) ? v : neg_inf();
+          sc[kb][r] = v;
+          mx = fmaxf(mx, v);
+        }
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float m_new = fmaxf(m, mx);
+      const float m_use = m_new == neg_inf() ? 0.f : m_new;  // nothing seen so far: P = 0
+      const float alpha = fast_exp2(m - m_use);
+      float ps = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = fast_exp2(sc[kb][r] - m_use);
+          sc[kb][r] = p;
+          ps += p;
+        }
+      l = l * alpha + ps;  // (this lane's part of the row's sum)
+      m = m_new;
+#pragma unroll
+      for (int u = 0; u < DP / 16; ++u) o[u] *= alpha;
+#pragma unroll
+      for (int u = 0; u < DP / 16; ++u)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const f32x4 vf = *reinterpret_cast<const f32x4*>(vt + (16 * u + r16) * VP + kb * 16 + 4 * g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[e], sc[kb][e], o[u], 0, 0, 0);
+        }
+    }
+    if (t + 1 < nkv) store_tile((t + 1) & 1);  // read last in tile t - 1, before the barrier that ended it
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  const bool none = m == neg_inf();
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // (a NaN sum passes through)
+  float any = 0.f;
+#pragma unroll
+  for (int u = 0; u < DP / 16; ++u)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[u][e] = none ? 0.f : o[u][e];
+      any += 16 * u + 4 * g < a.D ? o[u][e] : 0.f;
+    }
+  if (in_rows) {
+    const int64_t at = part.p ? part.at(a, x, slice) : 0;
+    if (part.p && g == 0) {
+      float* ml = part.ml(a, at);
+      ml[0] = m;
+      ml[1] = l;
+    }
+    float* O = part.p ? part.row(at) : static_cast<float*>(a.o) + x.b * a.ost[0] + x.h * a.ost[1] + x.t * a.ost[2];
+#pragma unroll
+    for (int u = 0; u < DP / 16; ++u) {
+      const int d = 16 * u + 4 * g;
+      if (d < a.D) *reinterpret_cast<f32x4*>(O + d) = part.p ? o[u] : o[u] * inv;
+    }
+  }
+  const uint64_t bad = __ballot(in_rows && !(any == any) && l == l);
+  uint32_t rows = static_cast<uint32_t>(bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffffu;
+  if (rows != 0) wait_vmcnt<0>();  // what has been written of these rows is written before what follows
+  while (rows != 0) {
+    const int r = qw + __builtin_ctz(rows);
+    rows &= rows - 1;
+    const SpanRow y = span_row(a, s, r);
+    float ro_[DP / 16], rm, rl;
+    span_attend_row<float, DP / 16, 1>(a, s, y, min(i0 * kKeys, s.n[0]), min((i0 + nkv) * kKeys, s.n[0]),
+                                    max(0, min((i0 - nft) * kKeys, s.n[1])), max(0, min((i0 + nkv - nft) * kKeys, s.n[1])), ro_, rm, rl);
+    span_write_row<float, DP / 16>(a, part, y, slice, ro_, rm, rl);
+  }
+}
+
+template <int DP, int NW>
+int launch_f32(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
+  auto kern = k_span_f32<DP, NW>;
+  if constexpr (kLdsBytes<DP> > 65536) {
+    static std::atomic<uint64_t> done{0};
+    if (int e = reserve_lds(reinterpret_cast<const void*>(kern), kLdsBytes<DP>, done, "attention")) return e;
+  }
+  const int64_t nqb = ceil_div(span_rows(a, mode), 16 * NW);
+  const int64_t total = span_sets(a, mode) * nqb * slices;
+  note_kernel("%s f32 d%d waves%d mode%d split%d", a.pk ? "shared_prefix" : "sliding_window", DP, NW, mode, slices);
+  hipLaunchKernelGGL(kern, blocks_2d(total), dim3(64 * NW), kLdsBytes<DP>, st, a, mode, static_cast<int>(nqb), slices, total, part);
+  return check_launch("attention");
+}
+
+template <int DP>
+int run_f32(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
+  return launch_f32<DP, 8>(a, mode, slices, part, st);
+}
+
+}  // namespace
+
+int span_f32_run(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
+  if (a.D <= 64) return run_f32<64>(a, mode, slices, part, st);
+  if (a.D <= 96) return run_f32<96>(a, mode, slices, part, st);
+  return run_f32<128>(a, mode, slices, part, st);
+}
+
+}  // namespace ntops

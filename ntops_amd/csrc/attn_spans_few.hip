@@ -107,8 +107,8 @@ struct FewBlocks {
   int mode;       // SpanMode
   int row_blocks;  // of a set
   int slices;
-  int first;      // slice of the rows that slice 0 is
-  int64_t blocks;
+  int first;       // slice of the rows that slice 0 is
+  int64_t sets, blocks;
 };
 
 // Where the queries lie: up to two groups of rows go to registers, through the LDS of a
@@ -129,10 +129,19 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
-  const int slice = static_cast<int>(id % f.slices);
-  const int64_t at = id / f.slices;
-  const int64_t set = at / f.row_blocks;
-  const int r0 = static_cast<int>(at - set * f.row_blocks) * (16 * RG);
+  // Blocks of the same keys and other rows run on one XCD (workgroups go round the 8),
+  // whose L2 then brings the keys in once.
+  int64_t at = id;
+  int rb = 0;
+  if (f.row_blocks > 1) {
+    const int64_t t = id >> 3;
+    rb = static_cast<int>(t % f.row_blocks);
+    at = t / f.row_blocks * 8 + (id & 7);
+  }
+  const int64_t set = at / f.slices;
+  const int slice = static_cast<int>(at - set * f.slices);
+  if (set >= f.sets) return;  // (the whole block: the last eight)
+  const int r0 = rb * (16 * RG);
   const int group = a.Hq / a.Hkv, ro = group * a.Sq;
   const int set_rows = f.mode == kFront ? ro * (a.B / a.G) : ro;
   const int rows = min(16 * RG, set_rows - r0);
@@ -434,7 +443,7 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
     if (row % NW != wave) continue;
     const SpanRow x = span_row(a, s, r0 + row);
     float ro_[D / 16], rm, rl;
-    span_attend_row<T, D / 16>(a, s, x, min(i0 * NK, s.n[0]), min(i1 * NK, s.n[0]), max(0, min((i0 - nft) * NK, s.n[1])),
+    span_attend_row<T, D / 16, 1>(a, s, x, min(i0 * NK, s.n[0]), min(i1 * NK, s.n[0]), max(0, min((i0 - nft) * NK, s.n[1])),
                                max(0, min((i1 - nft) * NK, s.n[1])), ro_, rm, rl);
     span_write_row<T, D / 16>(a, part, x, slice, ro_, rm, rl);
   }
@@ -486,12 +495,15 @@ int run_few(const SpanArgs& a, const FewPlan& p, const SpanPart& part, hipStream
   main.row_blocks = 1;
   main.slices = p.slices;
   main.first = part.first;
-  main.blocks = span_sets(a, main.mode) * main.slices;
+  main.sets = span_sets(a, main.mode);
+  main.blocks = main.sets * main.slices;
   if (p.front_slices > 0) {
     front.mode = kFront;
     front.row_blocks = static_cast<int>(ceil_div(span_rows(a, kFront), 64));
     front.slices = p.front_slices;
-    front.blocks = span_sets(a, kFront) * front.row_blocks * front.slices;
+    front.sets = span_sets(a, kFront);
+    front.blocks = front.sets * front.slices;
+    if (front.row_blocks > 1) front.blocks = ceil_div(front.blocks, 8) * 8 * front.row_blocks;
     return launch_few<T, D, 2, 4>(a, front, main, rows, part, st);
   }
   return p.waves == 1 ? launch_few<T, D, 1, 0>(a, front, main, rows, part, st) : launch_few<T, D, 2, 0>(a, front, main, rows, part, st);

@@ -70,10 +70,11 @@ __device__ __forceinline__ float max32(const f32x16 (&s)[2]) {
   return max3(max3(max3(m[0], m[1], m[2]), max3(m[3], m[4], m[5]), m[6]), max3(m[7], m[8], m[9]), m[10]);
 }
 
-template <typename T, int D>
+// D: columns of a row in the LDS; DM: columns that are multiplied, at least the head dim.
+template <typename T, int D, int DM>
 __global__ __launch_bounds__(64 * kWaves, 1) void k_span_tile(SpanArgs a, int mode, int nqb, int slices, int64_t total, SpanPart part) {
-  constexpr int KS = D / 16;  // k-steps of S = Q K^T
-  constexpr int DT = D / 32;  // 32-column tiles of O
+  constexpr int KS = DM / 16;  // k-steps of S = Q K^T
+  constexpr int DT = DM / 32;  // 32-column tiles of O
   constexpr int kTile = kKeys * D * 2;
   constexpr int kStage = 2 * kTile;                      // K tile, then V tile
   constexpr int L = 2 * SpanDma<D, false>::kInst;  // DMA instructions per lane per tile
@@ -345,32 +346,37 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_span_tile(SpanArgs a, int mo
     const int r = qw + __builtin_ctz(rows);
     rows &= rows - 1;
     const SpanRow y = span_row(a, s, r);
-    float ro_[D / 16], rm, rl;
-    span_attend_row<T, D / 16>(a, s, y, min(i0 * kKeys, s.n[0]), min((i0 + nkv) * kKeys, s.n[0]),
+    float ro_[DM / 16], rm, rl;
+    span_attend_row<T, DM / 16, 1>(a, s, y, min(i0 * kKeys, s.n[0]), min((i0 + nkv) * kKeys, s.n[0]),
                                max(0, min((i0 - nft) * kKeys, s.n[1])), max(0, min((i0 + nkv - nft) * kKeys, s.n[1])), ro_, rm, rl);
-    span_write_row<T, D / 16>(a, part, y, slice, ro_, rm, rl);
+    span_write_row<T, DM / 16>(a, part, y, slice, ro_, rm, rl);
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int DM>
 int launch_tile(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
   constexpr int kLds = kStages * 2 * kKeys * D * 2;
-  auto kern = k_span_tile<T, D>;
+  auto kern = k_span_tile<T, D, DM>;
   static std::atomic<uint64_t> done{0};
   if (int e = reserve_lds(reinterpret_cast<const void*>(kern), kLds, done, "attention")) return e;
   const int64_t nqb = ceil_div(span_rows(a, mode), kRowsBlock);
   const int64_t total = span_sets(a, mode) * nqb * slices;
-  note_kernel("%s tile d%d mode%d split%d", a.pk ? "shared_prefix" : "sliding_window", D, mode, slices);
+  note_kernel("%s tile d%d mode%d split%d", a.pk ? "shared_prefix" : "sliding_window", DM, mode, slices);
   hipLaunchKernelGGL(kern, blocks_2d(total), dim3(64 * kWaves), kLds, st, a, mode, static_cast<int>(nqb), slices, total, part);
   return check_launch("attention");
+}
+
+template <typename T>
+int run_tile(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
+  if (a.D <= 64) return launch_tile<T, 64, 64>(a, mode, slices, part, st);
+  if (a.D <= 96) return launch_tile<T, 128, 96>(a, mode, slices, part, st);
+  return launch_tile<T, 128, 128>(a, mode, slices, part, st);
 }
 
 }  // namespace
 
 int span_tile_run(int dtype, const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
-  if (dtype == NTOPS_BF16)
-    return a.D > 64 ? launch_tile<__bf16, 128>(a, mode, slices, part, st) : launch_tile<__bf16, 64>(a, mode, slices, part, st);
-  return a.D > 64 ? launch_tile<_Float16, 128>(a, mode, slices, part, st) : launch_tile<_Float16, 64>(a, mode, slices, part, st);
+  return dtype == NTOPS_BF16 ? run_tile<__bf16>(a, mode, slices, part, st) : run_tile<_Float16>(a, mode, slices, part, st);
 }
 
 }  // namespace ntops
