@@ -247,7 +247,7 @@ int span_rows_run(int dtype, const SpanArgs& a, int mode, int slices, const Span
 // 16-bit types, at most kFewRows rows of a sequence a cache head.  front_slices > 0:
 // with the rows of all sequences of a group over their prefix, in that many slices that
 // come before the others.
-constexpr int kFewRows = 64;
+constexpr int kFewRows = 32;
 struct FewPlan {
   int waves;  // a block, 1 or 2
   int mode;   // of each sequence's rows
@@ -255,7 +255,9 @@ struct FewPlan {
 };
 int span_few_run(int dtype, const SpanArgs& a, const FewPlan& p, const SpanPart& part, hipStream_t st);
 
-// The same for any number of rows; kBoth: with equal row strides of both spans.
+// The same for any number of rows, in blocks of kTileRows; kBoth: with equal row strides
+// of both spans.
+constexpr int kTileRows = 128;
 int span_tile_run(int dtype, const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st);
 
 // fp32, head dims up to 128 that are multiples of 4, rows at multiples of 16 bytes: any

@@ -7,8 +7,6 @@
 //     prefix: every key of the prefix, and its own sequence's keys j <= p
 //   A row that sees no key is 0.
 #include <algorithm>
-#include <cstdio>
-#include <cstdlib>
 
 #include "attn_spans.h"
 
@@ -121,20 +119,6 @@ Plan rows_plan(const SpanArgs& a) {
   return {kRows, kRows, 0, static_cast<int>(std::max<int64_t>(1, n)), 0};
 }
 
-// Slices for `heads` sets of blocks over `keys` keys.
-int few_slices(const SpanArgs& a, int64_t heads, int64_t keys, int waves) {
-  const int step = (a.D > 64 ? 32 : 64) * waves;
-  int64_t n = std::min({static_cast<int64_t>(kMaxSlices), cu_count_cached() * 2 / waves / heads, ceil_div(keys, 4 * step)});
-  if (n <= 2 && keys <= 8 * step) n = 1;  // two short slices gain what the merge's launch costs
-  return static_cast<int>(std::max<int64_t>(n, 1));
-}
-
-// Slices of a tile launch of `items` blocks of rows over `keys` keys.
-int tile_slices(int64_t items, int64_t keys, int most) {
-  const int64_t n = std::min({static_cast<int64_t>(most), cu_count_cached() / items, ceil_div(keys, 256)});
-  return static_cast<int>(std::max<int64_t>(n, 1));
-}
-
 // Blocks of `rows` rows.
 int64_t row_blocks(const SpanArgs& a, int mode, int rows) { return span_sets(a, mode) * ceil_div(span_rows(a, mode), rows); }
 
@@ -154,35 +138,69 @@ Plan f32_plan(const SpanArgs& a, bool joined) {
   return {kF32, kF32, 0, slices(main, a.P + std::min<int64_t>(a.C, main_keys(a) + a.Sq), kMaxSlices), 0};
 }
 
+// Slices of kFew for `heads` sets of rows over `keys` keys: a block of two waves a CU,
+// none of less than four tiles a wave, below which the partial results and the merge
+// cost what the slices gain; blocks of one wave (two heads a CU or more) are not split.
+// bf16, 128 columns, 4100 keys, 1 / 2 / 4 / 8 / 16 / 32 slices: 8 heads of 8 rows - / - / - /
+// 17.0 / 16.0 / 16.3 us, 64 heads - / 33.4 / 29.7 / 33.9, 256 heads 91.2 / 98.6.
+int few_slices(const SpanArgs& a, int64_t heads, int64_t keys, int waves) {
+  const int step = (a.D > 64 ? 32 : 64) * waves;
+  int64_t n = waves == 1 ? 1 : std::min({static_cast<int64_t>(kMaxSlices), cu_count_cached() / heads, ceil_div(keys, 4 * step)});
+  if (n <= 2 && keys <= 8 * step) n = 1;  // two short slices gain what the merge's launch costs
+  return static_cast<int>(std::max<int64_t>(n, 1));
+}
+
+// Slices of kTile for `items` blocks of rows over `keys` keys: a block a CU, two of 64
+// columns or where each still has 4000 keys (two run side by side, but the partial
+// results cost), none under two tiles.  4100 keys of 128 columns, 1 / 2 / 4 / 8 / 16 / 32
+// slices: 8 blocks of 64 rows 95 / 57 / 37 / 24.8 / 21.5 / 21.1 us, 64 blocks - / 56.6 / 39.5 /
+// 41.3, 256 blocks 110.6 / 113.3; 1100 keys, 256 blocks of 128 rows 36.1 / 46.7; 8700 keys 172 /
+// 148; 2100 keys of 64 columns, 128 blocks - / 30.1 / 26.2 / 32.5.
+int tile_slices(const SpanArgs& a, int64_t items, int64_t keys, int most) {
+  const int64_t cus = cu_count_cached();
+  const int64_t two = 2 * cus / items, n = a.D <= 64 || (two > 1 && keys / two >= 4000) ? two : cus / items;
+  return static_cast<int>(std::max<int64_t>(1, std::min({static_cast<int64_t>(most), n, ceil_div(keys, 128)})));
+}
+
+// Prefix keys and values that sequences may read again through the caches before the
+// prefix is better attended by itself, and the two results joined.  bf16, 32 / 8 heads of
+// 128, one token over a prefix and up to 512 of its own, each sequence over both / apart:
+// 4 over 8192 (100 MB again) 23.3 / 26.5 us, 8 over 8192 (235 MB) 33.9 / 29.7, 16 over 2048
+// (126 MB) 24.1 / 25.5, 64 over 512 (132 MB) 28.9 / 29.2, 2 over 32768 (134 MB) 35.8 / 44.6, 4 over
+// 32768 (403 MB) 56.9 / 46.0, 64 over 2048 (528 MB) 50.5 / 36.5.
+constexpr int64_t kReadAgain = 140 << 20;
+// Rows of a group up to which kFew takes the prefix, in the launch of the sequences' own
+// keys: 256 / 1024 rows over 2048 36.5 / 89.7 us, by kTile 44.3 / 93.2.
+constexpr int64_t kFewFrontRows = 512;
+
 // The plan for this problem where layouts suit the matrix cores, from sizes alone.
 // `joined`: both spans in one pass (without a workspace, they cannot be parted).
 Plan make_plan(int dtype, const SpanArgs& a, bool joined = false) {
-  if (const char* env = getenv("NT_PLAN")) { int f, m, fs, ms, w; if (sscanf(env, "%d,%d,%d,%d,%d", &f, &m, &fs, &ms, &w) == 5) return {(Path)f, (Path)m, fs, ms, w}; }
   if (a.D > 128 || a.D % (dtype == NTOPS_F32 ? 4 : 8) != 0 || static_cast<int64_t>(a.C) + a.P == 0) return rows_plan(a);
   if (dtype == NTOPS_F32) return f32_plan(a, joined);
-  const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv;
-  const int cus = cu_count_cached();
+  const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv, cus = cu_count_cached();
   const bool few = span_rows(a, kMain) <= kFewRows;
-  const int waves = heads < 2 * cus ? 2 : 1;
+  const int64_t again = static_cast<int64_t>(a.B - a.G) * a.Hkv * a.P * a.D * 4;
+  const int64_t blocks = row_blocks(a, kMain, few ? kFewRows : kTileRows);
   if (!joined && a.P > 0 && a.B > a.G) {
-    if (few && span_rows(a, kFront) <= 4 * kFewRows) {
-      // as many keys a block of the prefix as of a sequence
-      const int64_t total = row_blocks(a, kFront, 64) * a.P + heads * a.C;
-      const int step = (a.D > 64 ? 32 : 64) * 2;
-      const int64_t chunk = std::max<int64_t>(4 * step, ceil_div(total, cus * 2));
-      return {kFew, kFew, static_cast<int>(std::min<int64_t>(kMaxSlices / 2, ceil_div(a.P, chunk))),
-              static_cast<int>(std::min<int64_t>(kMaxSlices / 2, std::max<int64_t>(1, ceil_div(a.C, chunk)))), waves};
-    }
-    // tiles of 256 rows and 64 keys, of both spans for each sequence or apart
-    const int64_t both = row_blocks(a, kMain, 256) * (a.P + a.C), front = row_blocks(a, kFront, 256) * a.P;
-    if (few || both > (front + row_blocks(a, kMain, 256) * a.C) * 5 / 4) {
-      const int fs = tile_slices(row_blocks(a, kFront, 256), a.P, kMaxSlices / 2);
-      const int ms = few ? few_slices(a, heads, std::max<int64_t>(a.C, 1), waves) : tile_slices(row_blocks(a, kMain, 256), a.C, kMaxSlices / 2);
-      return {kTile, few ? kFew : kTile, fs, std::min(ms, kMaxSlices / 2), waves};
+    const int64_t front = row_blocks(a, kFront, kTileRows);
+    // many rows: where the rows of a group fill blocks that those of a sequence leave empty
+    const bool apart = few ? again > kReadAgain : blocks * (a.P + a.C) > (front * a.P + blocks * a.C) * 7 / 4 && again > kReadAgain;
+    if (apart) {
+      const bool few_front = few && span_rows(a, kFront) <= kFewFrontRows;
+      const int64_t keys = std::max<int64_t>(128, ceil_div(a.P * (few_front ? row_blocks(a, kFront, 64) : front), cus));
+      const int fs = static_cast<int>(std::min<int64_t>(kMaxSlices / 2, ceil_div(a.P, keys)));
+      // own keys: slices no longer than twice the prefix's
+      const int64_t ms = std::min({static_cast<int64_t>(kMaxSlices / 2), ceil_div(a.C, 2 * ceil_div(a.P, fs)), 2 * cus / blocks});
+      return {few_front ? kFew : kTile, few ? kFew : kTile, fs, static_cast<int>(std::max<int64_t>(1, ms)), 2};
     }
   }
-  if (few) return {kFew, kFew, 0, few_slices(a, heads, a.P + main_keys(a), waves), waves};
-  return {kTile, kTile, 0, tile_slices(row_blocks(a, kMain, 256), a.P + std::min<int64_t>(a.C, main_keys(a) + a.Sq), kMaxSlices), 0};
+  const int64_t keys = a.P + std::min<int64_t>(a.C, main_keys(a) + (few ? 0 : a.Sq));
+  if (few) {
+    const int waves = heads < 2 * cus ? 2 : 1;
+    return {kFew, kFew, 0, few_slices(a, heads, keys, waves), waves};
+  }
+  return {kTile, kTile, 0, tile_slices(a, blocks, keys, kMaxSlices), 0};
 }
 
 int64_t plan_bytes(const SpanArgs& a, const Plan& p) {

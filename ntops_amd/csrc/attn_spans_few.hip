@@ -467,7 +467,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_span_few(SpanArgs a, FewBlocks f
 
 template <typename T, int D, int NW, int RGF, int RGM>
 int launch_few(const SpanArgs& a, const FewBlocks& front, const FewBlocks& main, const SpanPart& part, hipStream_t st) {
-  constexpr int kLds = NW * 32768 + std::max(kQueryLds<D, RGF>, kQueryLds<D, RGM>);
+  constexpr int kLds = NW * 32768 + kQueryLds<D, RGF>;
   static_assert((2 * NW * 16 + 4 + NW * 16 * (D + 4)) * 4 <= NW * 32768, "LDS");
   auto kern = k_span_few<T, D, NW, RGF, RGM>;
   if constexpr (kLds > 65536) {
@@ -483,8 +483,7 @@ int launch_few(const SpanArgs& a, const FewBlocks& front, const FewBlocks& main,
 template <typename T, int D, int NW, int RGF>
 int launch_few(const SpanArgs& a, const FewBlocks& front, const FewBlocks& main, int rows, const SpanPart& part, hipStream_t st) {
   if (rows <= 16) return launch_few<T, D, NW, RGF, 1>(a, front, main, part, st);
-  if (rows <= 32) return launch_few<T, D, NW, RGF, 2>(a, front, main, part, st);
-  return launch_few<T, D, NW, RGF, 4>(a, front, main, part, st);
+  return launch_few<T, D, NW, RGF, 2>(a, front, main, part, st);
 }
 
 template <typename T, int D>

@@ -1,31 +1,32 @@
 // Many query rows a cache head (prompts, chunks of prompts, all sequences of a shared
 // prefix together): windowed and shared-prefix attention on the matrix cores.
 //
-// A work item is 256 of the rows that share a cache head -- with grouped queries 256 /
-// group tokens, so that the keys that a window leaves to a block are little more than
-// the window -- over the 64-key tiles of both spans, or a slice of them.  Wave w owns
-// rows 32 w .. + 31 with their queries in registers; tiles go global -> LDS by direct
-// DMA into a ring of four stages, two tiles ahead.  The two waves that share a SIMD run
-// half a tile apart: while one runs a matrix phase (O += P_j V_j, then S_{j+1} = Q
-// K_{j+1}^T) the other runs a vector phase (mask, maximum, exponentials, sum, pack P),
-// two barriers a tile.  A wave skips the tiles that none of its rows sees.
+// A block is 128 of the rows that share a cache head -- with grouped queries 128 / group
+// tokens, so that the keys that a window leaves to a block are little more than the
+// window -- over the 64-key tiles of both spans, or a slice of them.  Wave w owns rows
+// 32 w .. + 31 with their queries in registers and skips the tiles that none of them
+// sees; tiles go global -> LDS by direct DMA into one of two stages while the other is
+// used, one barrier a tile.  Two blocks a CU (64 columns: three) that nothing
+// synchronizes: the maxima and exponentials of one run under the MFMAs of the other.
+// Eight waves of 32 rows that alternate the two kinds of phase between barriers (256
+// rows, four stages, one block a CU) took 2 % less for long rows of 128 columns -- (16,
+// 32 / 8, 500 over a shared 8192) bf16 1070 against 1088 us -- 28 % more of 64 columns,
+// (1, 32 / 8, 16384, window 4096) 748 against 583, and half as long again for narrow
+// windows, (7, 16, 2001, window 255) of 80 columns 100 against 65.
 //
 // A row's reference (from which its exponents are taken) follows its maximum when that
 // is past it by more than 2^8.  Masked scores are -inf whatever their key holds; a
 // value that is not finite times P = 0 is NaN, so a row whose result is NaN under a sum
 // that is none is computed again by itself, from the keys that it sees.
-#include <algorithm>
-#include <atomic>
-
 #include "attn_spans.h"
 
 namespace ntops {
 namespace {
 
-constexpr int kRowsBlock = 256;
-constexpr int kWaves = 8;
+constexpr int kWaves = 4;
+constexpr int kRowsBlock = 32 * kWaves;
+static_assert(kRowsBlock == kTileRows, "the plans count on it");
 constexpr int kKeys = 64;
-constexpr int kStages = 4;
 constexpr int kAhead = 4;  // fragments read ahead of the MFMA that uses them
 constexpr float kSlack = 8.f;
 
@@ -49,9 +50,9 @@ struct SpanDma {
       voff[i] = c * 8 < dt ? static_cast<uint32_t>(row * ld * 2 + c * 16) : kOOB;
     }
   }
-  // 64 rows from row0 on of `n` at `base` (rows past them are zeros) into the LDS
+  // 64 rows from row0 < n on of `n` at `base` (rows past them are zeros) into the LDS
   __device__ __forceinline__ void issue(const char* base, int64_t ld, int row0, int n, int dt, uint32_t tile) const {
-    const u32x4 r = make_rsrc(base + row0 * ld * 2, n > row0 ? ((n - row0 - 1) * ld + dt) * 2 : 0);
+    const u32x4 r = make_rsrc(base + row0 * ld * 2, ((n - row0 - 1) * ld + dt) * 2);
 #pragma unroll
     for (int i = 0; i < kInst; ++i) dma16(r, __builtin_amdgcn_readfirstlane(tile + lds_off + i * 1024), voff[i]);
   }
@@ -72,18 +73,15 @@ __device__ __forceinline__ float max32(const f32x16 (&s)[2]) {
 
 // D: columns of a row in the LDS; DM: columns that are multiplied, at least the head dim.
 template <typename T, int D, int DM>
-__global__ __launch_bounds__(64 * kWaves, 1) void k_span_tile(SpanArgs a, int mode, int nqb, int slices, int64_t total, SpanPart part) {
+__global__ __launch_bounds__(64 * kWaves, 2) void k_span_tile(SpanArgs a, int mode, int nqb, int slices, int64_t total, SpanPart part) {
   constexpr int KS = DM / 16;  // k-steps of S = Q K^T
   constexpr int DT = DM / 32;  // 32-column tiles of O
   constexpr int kTile = kKeys * D * 2;
   constexpr int kStage = 2 * kTile;                      // K tile, then V tile
-  constexpr int L = 2 * SpanDma<D, false>::kInst;  // DMA instructions per lane per tile
-  static_assert(kStages == 4, "the phases refill the stage of tile k - 2 with tile k + 2");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int grp = wave >> 2;  // 0: leads, 1: one phase behind (one wave of each per SIMD)
   const int64_t pid = block_id();
   if (pid >= total) return;  // the tail of a 2-D grid (the whole block)
   // An XCD (workgroups go round them) walks whole sets, every eighth one, the rows with
@@ -141,14 +139,13 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_span_tile(SpanArgs a, int mo
   kd.init(kld, wave, lane, a.D);
   vd.init(vld, wave, lane, a.D);
   const uint32_t smem_addr = lds_addr(smem);
-  // tile g of the item into its stage; past the last: loads of nothing, which still
-  // count in vmcnt
+  // tile g of the item into its stage
   const auto dma = [&](int g) __attribute__((always_inline)) {
-    const uint32_t st = smem_addr + static_cast<uint32_t>((g & 3) * kStage);
+    const uint32_t st = smem_addr + static_cast<uint32_t>((g & 1) * kStage);
     const int i = i0 + g, span = i < nft ? 0 : 1;
-    const int row0 = (span == 0 ? i : i - nft) * kKeys, n = g < nkv ? s.n[span] : 0;
-    kd.issue(s.k[span], kld, row0, n, a.D, st);
-    vd.issue(s.v[span], vld, row0, n, a.D, st + kTile);
+    const int row0 = (span == 0 ? i : i - nft) * kKeys;
+    kd.issue(s.k[span], kld, row0, s.n[span], a.D, st);
+    vd.issue(s.v[span], vld, row0, s.n[span], a.D, st + kTile);
   };
   // whether the wave has rows that see keys of tile g
   const auto need = [&](int g) __attribute__((always_inline)) {
@@ -174,7 +171,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_span_tile(SpanArgs a, int mo
   // O += P_j V_j; fragment i + kAhead is read while MFMA i runs, and a scheduling fence
   // per step pins that order
   const auto pv_part = [&](int j) __attribute__((always_inline)) {
-    const char* sv = smem + (j & 3) * kStage + kTile;
+    const char* sv = smem + (j & 1) * kStage + kTile;
     constexpr int nm = 4 * DT;  // MFMA i: key slice i / DT, d tile i % DT
     u32x4 f[kAhead];
 #pragma unroll
@@ -189,7 +186,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_span_tile(SpanArgs a, int mo
   };
   // S = Q K_j^T
   const auto qk_part = [&](int j) __attribute__((always_inline)) {
-    const char* sk = smem + (j & 3) * kStage;
+    const char* sk = smem + (j & 1) * kStage;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -205,13 +202,6 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_span_tile(SpanArgs a, int mo
       if (i + kAhead < nm) f[i % kAhead] = k_frag<D>(sk, ((i + kAhead) % 2) * 32, (i + kAhead) / 2, lane);
     }
     __builtin_amdgcn_sched_barrier(0);
-  };
-  // at raised priority: the SIMD issues it ahead of the partner wave's vector phase
-  const auto matrix_phase = [&](int j) __attribute__((always_inline)) {
-    __builtin_amdgcn_s_setprio(1);
-    if (j >= 0 && need(j)) pv_part(j);
-    if (j + 1 < nkv && need(j + 1)) qk_part(j + 1);
-    __builtin_amdgcn_s_setprio(0);
   };
   const auto vector_phase = [&](int g) __attribute__((always_inline)) {
     const int i = i0 + g;
@@ -259,41 +249,20 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_span_tile(SpanArgs a, int mo
     for (int sl = 0; sl < 4; ++sl) pf[sl] = pack8<T>(&p[sl >> 1][8 * (sl & 1)]);
   };
 
-  // Period k: group 0 runs the matrix phase of tile k - 1, then the vector phase of tile
-  // k; group 1 the vector phase of tile k - 1, then the matrix phase of tile k - 1.  Tile
-  // k is read from the first phase of period k to the second of period k + 1; at the
-  // start of period k it must have landed, and the stage of tile k - 2 is free.
-  const auto period_start = [&](int k) __attribute__((always_inline)) {
-    wait_vmcnt<L>();  // this wave's part of tile k; tile k + 1 may be in flight
-    block_barrier();
-    dma(k + 2);
-  };
-  if (nkv > 0) {
-    dma(0);
-    dma(1);
-    if (grp == 0) {
-      for (int k = 0; k < nkv; ++k) {
-        period_start(k);
-        matrix_phase(k - 1);
-        block_barrier();
-        if (need(k)) vector_phase(k);
-      }
-      period_start(nkv);
-      if (need(nkv - 1)) pv_part(nkv - 1);
-      block_barrier();
-    } else {
-      for (int k = 0; k < nkv; ++k) {
-        period_start(k);
-        if (k >= 1 && need(k - 1)) vector_phase(k - 1);
-        block_barrier();
-        matrix_phase(k - 1);
-      }
-      period_start(nkv);
-      const bool last = need(nkv - 1);
-      if (last) vector_phase(nkv - 1);
-      block_barrier();
-      if (last) pv_part(nkv - 1);
-    }
+  if (nkv > 0) dma(0);
+  for (int k = 0; k < nkv; ++k) {
+    wait_vmcnt<0>();
+    block_barrier();  // tile k is in, and every wave is done with tile k - 1
+    if (k + 1 < nkv) dma(k + 1);
+    if (!need(k)) continue;
+    // (the other block's wave on this SIMD has its vector work under these MFMAs)
+    __builtin_amdgcn_s_setprio(1);
+    qk_part(k);
+    __builtin_amdgcn_s_setprio(0);
+    vector_phase(k);
+    __builtin_amdgcn_s_setprio(1);
+    pv_part(k);
+    __builtin_amdgcn_s_setprio(0);
   }
 
   const float l = l_half + __shfl_xor(l_half, 32, 64);
@@ -355,14 +324,12 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_span_tile(SpanArgs a, int mo
 
 template <typename T, int D, int DM>
 int launch_tile(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
-  constexpr int kLds = kStages * 2 * kKeys * D * 2;
-  auto kern = k_span_tile<T, D, DM>;
-  static std::atomic<uint64_t> done{0};
-  if (int e = reserve_lds(reinterpret_cast<const void*>(kern), kLds, done, "attention")) return e;
+  constexpr int kLds = 2 * 2 * kKeys * D * 2;
+  static_assert(kLds <= 65536, "LDS");
   const int64_t nqb = ceil_div(span_rows(a, mode), kRowsBlock);
   const int64_t total = span_sets(a, mode) * nqb * slices;
   note_kernel("%s tile d%d mode%d split%d", a.pk ? "shared_prefix" : "sliding_window", DM, mode, slices);
-  hipLaunchKernelGGL(kern, blocks_2d(total), dim3(64 * kWaves), kLds, st, a, mode, static_cast<int>(nqb), slices, total, part);
+  hipLaunchKernelGGL((k_span_tile<T, D, DM>), blocks_2d(total), dim3(64 * kWaves), kLds, st, a, mode, static_cast<int>(nqb), slices, total, part);
   return check_launch("attention");
 }
 

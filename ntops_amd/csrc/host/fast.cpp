@@ -53,6 +53,11 @@ decltype(&ntops_mxfp4_linear_workspace) f_mxfp4_linear_workspace;
 decltype(&ntops_store_kv_cache) f_store_kv_cache;
 decltype(&ntops_kv_cache_attention) f_kv_cache_attention;
 decltype(&ntops_kv_cache_attention_workspace) f_kv_cache_attention_workspace;
+decltype(&ntops_sliding_window_attention) f_sliding_window_attention;
+decltype(&ntops_sliding_window_attention_workspace) f_sliding_window_attention_workspace;
+decltype(&ntops_shared_prefix_attention) f_shared_prefix_attention;
+decltype(&ntops_shared_prefix_attention_workspace) f_shared_prefix_attention_workspace;
+decltype(&ntops_rope_axes_qk) f_rope_axes_qk;
 bool ready = false;
 PyObject* get_device = nullptr;  // torch._C._cuda_getDevice
 PyObject* get_stream = nullptr;  // torch._C._cuda_getCurrentRawStream
@@ -770,6 +775,150 @@ PyObject* kv_cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NTOPS_END
 }
 
+// A Python int (not a bool); false: the Python path, as for one past 64 bits.
+bool integer(PyObject* o, int64_t& v) {
+  if (!PyLong_CheckExact(o)) return false;
+  v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return true;
+}
+
+// Query, key and value (a[0], a[i], a[i + 1]) of attention in one type, with unit strides
+// along the head dim.
+struct Attention {
+  const at::Tensor *q, *k, *v;
+  int64_t B, Hq, H, Sq, C, D;
+  int code;
+  bool read(PyObject* const* a, int i, int64_t dev) {
+    q = plain(a[0]);
+    k = plain(a[i]);
+    v = plain(a[i + 1]);
+    if (!q || !k || !v || q->dim() != 4 || k->dim() != 4 || v->sizes() != k->sizes() || (code = code16_32(*q)) < 0 ||
+        q->numel() == 0 || k->numel() == 0 || k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type() ||
+        q->get_device() != dev || k->get_device() != dev || v->get_device() != dev || q->stride(3) != 1)
+      return false;
+    B = q->size(0);
+    Hq = q->size(1);
+    Sq = q->size(2);
+    D = q->size(3);
+    H = k->size(1);
+    C = k->size(2);
+    return k->size(0) == B && k->size(3) == D && Hq % H == 0;
+  }
+  bool scale(PyObject* o, double& s) const {
+    if (o != Py_None) return number(o, s);
+    s = 1.0 / std::sqrt(static_cast<double>(D));
+    return true;
+  }
+};
+
+// sliding_window_attention(query, key, value, window, sinks, lengths or None, scale or None)
+PyObject* sliding_window_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NTOPS_TRY
+  int64_t dev, window, sinks;
+  void* st;
+  if (n != 7 || !usable() || !integer(a[3], window) || !integer(a[4], sinks) || window < 1 || sinks < 0 || !current(dev, st))
+    return none();
+  Attention t;
+  const at::Tensor* len;
+  int lcode;
+  double scale;
+  if (!t.read(a, 1, dev) || !index_vector(a[5], t.B, dev, len, lcode) || !t.scale(a[6], scale)) return none();
+  at::Tensor out;
+  int rc;
+  {
+    NoGil free;
+    out = new_like(*t.q, t.q->sizes());
+    const int64_t bytes = f_sliding_window_attention_workspace(t.code, t.B, t.Hq, t.H, t.Sq, t.C, t.D, window, sinks);
+    at::Tensor ws;
+    if (bytes > 0) ws = workspace(*t.q, bytes);
+    rc = f_sliding_window_attention(t.code, t.B, t.Hq, t.H, t.Sq, t.C, t.D, t.q->data_ptr(), t.q->strides().data(), t.k->data_ptr(),
+                                    t.k->strides().data(), t.v->data_ptr(), t.v->strides().data(), len ? len->data_ptr() : nullptr,
+                                    lcode, window, sinks, scale, out.data_ptr(), out.strides().data(),
+                                    bytes > 0 ? ws.data_ptr() : nullptr, bytes, st);
+  }
+  return rc == NTOPS_OK ? wrap(out) : none();
+  NTOPS_END
+}
+
+// shared_prefix_attention(query, prefix_key, prefix_value, key, value, prefix_lengths or
+// None, lengths or None, scale or None)
+PyObject* shared_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NTOPS_TRY
+  int64_t dev;
+  void* st;
+  if (n != 8 || !usable() || !current(dev, st)) return none();
+  Attention t;
+  const at::Tensor *pk = plain(a[1]), *pv = plain(a[2]), *plen, *len;
+  int pcode, lcode;
+  double scale;
+  if (!pk || !pv || !t.read(a, 3, dev) || pk->dim() != 4 || pv->sizes() != pk->sizes() || pk->numel() == 0 ||
+      pk->scalar_type() != t.q->scalar_type() || pv->scalar_type() != t.q->scalar_type() || pk->get_device() != dev ||
+      pv->get_device() != dev || pk->size(1) != t.H || pk->size(3) != t.D || t.B % pk->size(0) != 0 ||
+      !index_vector(a[5], pk->size(0), dev, plen, pcode) || !index_vector(a[6], t.B, dev, len, lcode) || !t.scale(a[7], scale))
+    return none();
+  const int64_t G = pk->size(0), P = pk->size(2);
+  at::Tensor out;
+  int rc;
+  {
+    NoGil free;
+    out = new_like(*t.q, t.q->sizes());
+    const int64_t bytes = f_shared_prefix_attention_workspace(t.code, G, t.B, t.Hq, t.H, t.Sq, P, t.C, t.D);
+    at::Tensor ws;
+    if (bytes > 0) ws = workspace(*t.q, bytes);
+    rc = f_shared_prefix_attention(t.code, G, t.B, t.Hq, t.H, t.Sq, P, t.C, t.D, t.q->data_ptr(), t.q->strides().data(),
+                                   pk->data_ptr(), pk->strides().data(), pv->data_ptr(), pv->strides().data(),
+                                   plen ? plen->data_ptr() : nullptr, pcode, t.k->data_ptr(), t.k->strides().data(), t.v->data_ptr(),
+                                   t.v->strides().data(), len ? len->data_ptr() : nullptr, lcode, scale, out.data_ptr(),
+                                   out.strides().data(), bytes > 0 ? ws.data_ptr() : nullptr, bytes, st);
+  }
+  return rc == NTOPS_OK ? wrap(out) : none();
+  NTOPS_END
+}
+
+// rope_axes_qk(q, k, sin, cos, positions, sections (a list or tuple of ints), interleaved)
+PyObject* rope_axes_qk(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NTOPS_TRY
+  if (n != 7 || !usable() || !PyBool_Check(a[6]) || (!PyTuple_CheckExact(a[5]) && !PyList_CheckExact(a[5]))) return none();
+  const at::Tensor* t[5];
+  int64_t dev;
+  void* st;
+  if (!current(dev, st)) return none();
+  for (int i = 0; i < 5; ++i) {
+    t[i] = plain(a[i]);
+    if (!t[i] || t[i]->get_device() != dev || t[i]->dim() != (i < 2 ? 4 : i < 4 ? 2 : 3) || t[i]->numel() == 0) return none();
+  }
+  const at::Tensor &q = *t[0], &k = *t[1], &sn = *t[2], &cs = *t[3], &pos = *t[4];
+  const int64_t B = q.size(0), S = q.size(1), D = q.size(3), tw = sn.size(1);
+  const int code = code16_32(q), tcode = code16_32(sn);
+  const int pcode = pos.scalar_type() == at::kInt ? NTOPS_I32 : pos.scalar_type() == at::kLong ? NTOPS_I64 : -1;
+  if (code < 0 || k.scalar_type() != q.scalar_type() || k.size(0) != B || k.size(1) != S || k.size(3) != D || D % 2 != 0 ||
+      cs.sizes() != sn.sizes() || cs.scalar_type() != sn.scalar_type() || (tcode != NTOPS_F32 && tcode != code) ||
+      (tw != D && tw != D / 2) || sn.stride(1) != 1 || cs.stride(1) != 1 || pcode < 0 || pos.size(1) != B || pos.size(2) != S)
+    return none();
+  int64_t sections[256];
+  const Py_ssize_t count = PySequence_Fast_GET_SIZE(a[5]);
+  if (count > 256) return none();
+  for (Py_ssize_t i = 0; i < count; ++i)
+    if (!integer(PySequence_Fast_GET_ITEM(a[5], i), sections[i])) return none();
+  at::Tensor qo, ko;
+  int rc;
+  {
+    NoGil free;
+    qo = new_like(q, q.sizes());
+    ko = new_like(k, k.sizes());
+    rc = f_rope_axes_qk(code, B, S, q.size(2), k.size(2), D, q.data_ptr(), q.strides().data(), k.data_ptr(), k.strides().data(), tcode,
+                        sn.data_ptr(), sn.stride(0), cs.data_ptr(), cs.stride(0), sn.size(0), tw, pos.size(0), pos.data_ptr(), pcode,
+                        pos.strides().data(), count, sections, a[6] == Py_True ? 1 : 0, qo.data_ptr(), qo.strides().data(),
+                        ko.data_ptr(), ko.strides().data(), st);
+  }
+  return rc == NTOPS_OK ? wrap2(qo, ko) : none();
+  NTOPS_END
+}
+
 // init({name: address}, get_device, get_stream)
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 3 || !PyDict_Check(a[0])) {
@@ -792,7 +941,12 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
                    set("ntops_mxfp4_mm", f_mxfp4_mm) & set("ntops_mxfp4_mm_workspace", f_mxfp4_mm_workspace) &
                    set("ntops_mxfp4_linear", f_mxfp4_linear) & set("ntops_mxfp4_linear_workspace", f_mxfp4_linear_workspace) &
                    set("ntops_store_kv_cache", f_store_kv_cache) & set("ntops_kv_cache_attention", f_kv_cache_attention) &
-                   set("ntops_kv_cache_attention_workspace", f_kv_cache_attention_workspace);
+                   set("ntops_kv_cache_attention_workspace", f_kv_cache_attention_workspace) &
+                   set("ntops_sliding_window_attention", f_sliding_window_attention) &
+                   set("ntops_sliding_window_attention_workspace", f_sliding_window_attention_workspace) &
+                   set("ntops_shared_prefix_attention", f_shared_prefix_attention) &
+                   set("ntops_shared_prefix_attention_workspace", f_shared_prefix_attention_workspace) &
+                   set("ntops_rope_axes_qk", f_rope_axes_qk);
   if (PyErr_Occurred()) return nullptr;
   Py_INCREF(a[1]);
   Py_INCREF(a[2]);
@@ -808,7 +962,8 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {NTOPS_M(init),         NTOPS_M(unary),   NTOPS_M(softmax), NTOPS_M(rms_norm), NTOPS_M(layer_norm),
                          NTOPS_M(add_rms_norm), NTOPS_M(rope_qk), NTOPS_M(mm),      NTOPS_M(addmm),    NTOPS_M(sdpa),
                          NTOPS_M(quantize_mxfp4), NTOPS_M(dequantize_mxfp4), NTOPS_M(mxfp4_mm), NTOPS_M(store_kv_cache),
-                         NTOPS_M(kv_cache_attention), {nullptr, nullptr, 0, nullptr}};
+                         NTOPS_M(kv_cache_attention), NTOPS_M(sliding_window_attention), NTOPS_M(shared_prefix_attention),
+                         NTOPS_M(rope_axes_qk), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", "native host path of the torch wrappers", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 

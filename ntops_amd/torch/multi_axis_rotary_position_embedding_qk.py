@@ -25,6 +25,10 @@ from ntops_amd.torch.utils import _DeviceGuard, _contiguous, _strides, _to_dtype
 
 
 def multi_axis_rotary_position_embedding_qk(q, k, sin_table, cos_table, positions, sections, interleaved=True, inplace=False):
+    if _lib.fast is not None and not inplace:
+        r = _lib.fast.rope_axes_qk(q, k, sin_table, cos_table, positions, sections, interleaved)
+        if r is not None:
+            return r
     what = "multi_axis_rotary_position_embedding_qk"
     if q.dim() != 4 or k.dim() != 4:
         raise RuntimeError(f"{what}: q and k must be (batch, seq, heads, dim)")

@@ -30,6 +30,10 @@ from ntops_amd.torch.utils import _DeviceGuard, _contiguous, _strides
 
 
 def shared_prefix_attention(query, prefix_key, prefix_value, key, value, prefix_lengths=None, lengths=None, scale=None):
+    if _lib.fast is not None:
+        r = _lib.fast.shared_prefix_attention(query, prefix_key, prefix_value, key, value, prefix_lengths, lengths, scale)
+        if r is not None:
+            return r
     what = "shared_prefix_attention"
     b, hq, hkv, sq, c, d = _check_attention(query, key, value, what)
     if prefix_key.dim() != 4 or prefix_key.shape != prefix_value.shape or prefix_key.shape[1] != hkv or prefix_key.shape[3] != d:

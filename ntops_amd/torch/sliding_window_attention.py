@@ -45,6 +45,10 @@ def _index_args(t):
 
 
 def sliding_window_attention(query, key, value, window, sinks=0, lengths=None, scale=None):
+    if _lib.fast is not None:
+        r = _lib.fast.sliding_window_attention(query, key, value, window, sinks, lengths, scale)
+        if r is not None:
+            return r
     what = "sliding_window_attention"
     b, hq, hkv, sq, c, d = _check_attention(query, key, value, what)
     window, sinks = (min(operator.index(n), 1 << 62) for n in (window, sinks))
