@@ -45,14 +45,26 @@ inline int64_t span_rows(const SpanArgs& a, int mode) {
   return mode == kFront ? rows * (a.B / a.G) : rows;
 }
 
+// Where a set's rows and keys are.
+struct SpanSet {
+  int at;  // sequence, or prefix
+  int b0;  // first sequence
+  int hk;  // cache head
+};
+__device__ __forceinline__ SpanSet span_set(const SpanArgs& a, int mode, int64_t set) {
+  SpanSet s;
+  s.at = static_cast<int>(set / a.Hkv);
+  s.hk = static_cast<int>(set - static_cast<int64_t>(s.at) * a.Hkv);
+  s.b0 = mode == kFront ? s.at * (a.B / a.G) : s.at;
+  return s;
+}
+
 // The spans of a block of rows; wave-uniform.
-struct Spans {
+struct Spans : SpanSet {
   const char* k[2];  // front, main: first key
   const char* v[2];
   int n[2];          // keys
   int64_t kld[2], vld[2];  // strides in elements
-  int b0;            // (first) sequence of the set
-  int hk;
   int place;         // main key of the first token (t = 0) of a row; -Sq or less: before the main span
   int window, sinks;  // sinks: main keys below it are seen whatever the window
   // main keys [lo, hi) are seen by a row of token t, and those below `sinks`
@@ -68,10 +80,8 @@ __device__ __forceinline__ int span_length(const void* p, int dtype, int i, int 
 template <int ES>
 __device__ __forceinline__ Spans make_spans(const SpanArgs& a, int mode, int64_t set, int t0, int t1) {
   Spans s;
-  const int at = static_cast<int>(set / a.Hkv);
-  s.hk = static_cast<int>(set - static_cast<int64_t>(at) * a.Hkv);
-  const int per = a.B / a.G;
-  s.b0 = mode == kFront ? at * per : at;
+  static_cast<SpanSet&>(s) = span_set(a, mode, set);
+  const int at = s.at;
   s.n[0] = s.n[1] = 0;
   s.k[0] = s.k[1] = static_cast<const char*>(a.k);
   s.v[0] = s.v[1] = static_cast<const char*>(a.v);
@@ -98,7 +108,7 @@ __device__ __forceinline__ Spans make_spans(const SpanArgs& a, int mode, int64_t
     }
   }
   if (a.pk != nullptr && mode != kMain) {
-    const int g = mode == kFront ? at : at / per;
+    const int g = mode == kFront ? at : at / (a.B / a.G);
     s.n[0] = span_length(a.plengths, a.plengths_dtype, g, a.P);
     s.k[0] = static_cast<const char*>(a.pk) + (g * a.pkst[0] + s.hk * a.pkst[1]) * ES;
     s.v[0] = static_cast<const char*>(a.pv) + (g * a.pvst[0] + s.hk * a.pvst[1]) * ES;
@@ -112,7 +122,7 @@ __device__ __forceinline__ Spans make_spans(const SpanArgs& a, int mode, int64_t
 struct SpanRow {
   int b, t, h;
 };
-__device__ __forceinline__ SpanRow span_row(const SpanArgs& a, const Spans& s, int r) {
+__device__ __forceinline__ SpanRow span_row(const SpanArgs& a, const SpanSet& s, int r) {
   const int group = a.Hq / a.Hkv, ro = group * a.Sq;
   SpanRow x;
   x.b = r / ro;

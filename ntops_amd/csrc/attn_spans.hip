@@ -45,8 +45,14 @@ __global__ __launch_bounds__(256) void k_span_merge(SpanArgs a, SpanPart part) {
   const int lane = threadIdx.x & 63;
   const int64_t row = block_id() * 4 + (threadIdx.x >> 6);
   if (row >= static_cast<int64_t>(a.B) * a.Hq * a.Sq) return;
-  constexpr int NS = 64 / W;
+  constexpr int NS = 64 / W, kAhead = 4;
   const int d = (lane % W) * 4, g = lane / W;
+  const auto load = [&](int s) {
+    return s < part.slices && d < part.ld ? *reinterpret_cast<const f32x4*>(part.row(row * part.slices + s) + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+  };
+  f32x4 v[kAhead];  // in flight while the weights are formed
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) v[u] = load(u * NS + g);
   float m = neg_inf(), l = 0.f;
   if (lane < part.slices) {
     const float* ml = part.ml(a, row * part.slices + lane);
@@ -57,13 +63,16 @@ __global__ __launch_bounds__(256) void k_span_merge(SpanArgs a, SpanPart part) {
   const float w = m == neg_inf() ? 0.f : fast_exp2(m - mm);
   const float sum = wave_sum(l * w);
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < part.slices; s0 += NS) {
-    const int s = s0 + g;
+  const auto add = [&](int s, f32x4 x) {
     const float ws = __shfl(w, s & 63, 64);
     // (a slice of weight 0 holds nothing that the row has seen, or nothing beside the others)
-    if (s < part.slices && d < part.ld && ws != 0.f)
-      o += ws * *reinterpret_cast<const f32x4*>(part.row(row * part.slices + s) + d);
-  }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += ws != 0.f ? ws * x[e] : 0.f;
+  };
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u)
+    if (u * NS < part.slices) add(u * NS + g, v[u]);
+  for (int s0 = kAhead * NS; s0 < part.slices; s0 += NS) add(s0 + g, load(s0 + g));
 #pragma unroll
   for (int step = W; step < 64; step <<= 1)
 #pragma unroll

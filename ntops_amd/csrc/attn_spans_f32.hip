@@ -57,8 +57,6 @@ __global__ __launch_bounds__(64 * NW, 4) void k_span_f32(SpanArgs a, int mode, i
   const bool in_rows = qw + r16 < nrows;
   const SpanRow x = span_row(a, s, min(qw + r16, nrows - 1));
   const int tw0 = front_only ? 0 : min(qw, nrows - 1) / group, tw1 = front_only ? 0 : min(qw + 15, nrows - 1) / group;
-  const int w_hi = s.hi(tw1), w_lo = s.lo(tw0), w_hi_all = s.hi(tw0), w_lo_all = s.lo(tw1);
-  const int my_hi = s.hi(x.t) - 4 * g, my_lo = s.lo(x.t) - 4 * g;
   f32x4 qf[DP / 16];
   {
     const float* Q = static_cast<const float*>(a.q) + x.b * a.qst[0] + x.h * a.qst[1] + x.t * a.qst[2];
@@ -69,26 +67,29 @@ __global__ __launch_bounds__(64 * NW, 4) void k_span_f32(SpanArgs a, int mode, i
     }
   }
 
-  const int nft = (s.n[0] + kKeys - 1) / kKeys, nt = nft + (s.n[1] + kKeys - 1) / kKeys;
+  // the front's keys and the main ones behind them, as one sequence
+  const int nf = s.n[0], keys = nf + s.n[1];
+  const int sinks = nf + max(0, s.sinks);
+  const int w_hi = nf + s.hi(tw1), w_lo = nf + s.lo(tw0), w_hi_all = nf + s.hi(tw0), w_lo_all = nf + s.lo(tw1);
+  const int my_hi = nf + s.hi(x.t) - 4 * g, my_lo = nf + s.lo(x.t) - 4 * g;
+  const int nt = (keys + kKeys - 1) / kKeys;
   const int share = (nt + slices - 1) / slices;
   const int i0 = min(slice * share, nt);
   const int nkv = min(i0 + share, nt) - i0;
 
   f32x4 kst[kLd], vst[kLd];
   const auto load_tile = [&](int t) __attribute__((always_inline)) {
-    const int i = i0 + t, sp = i < nft ? 0 : 1;
-    const int row0 = (sp == 0 ? i : i - nft) * kKeys;
-    const float* K = reinterpret_cast<const float*>(s.k[sp]);
-    const float* V = reinterpret_cast<const float*>(s.v[sp]);
+    const int k0 = (i0 + t) * kKeys;
 #pragma unroll
     for (int j = 0; j < kLd; ++j) {
       const int f = threadIdx.x + kThreads * j;
-      const int key = row0 + f / (DP / 4), d = 4 * (f % (DP / 4));
-      const bool ok = f < kF4 && key < s.n[sp] && d < a.D;
+      const int key = k0 + f / (DP / 4), d = 4 * (f % (DP / 4));
       f32x4 kz = {0.f, 0.f, 0.f, 0.f}, vz = {0.f, 0.f, 0.f, 0.f};
-      if (ok) {
-        kz = *reinterpret_cast<const f32x4*>(K + key * s.kld[sp] + d);
-        vz = *reinterpret_cast<const f32x4*>(V + key * s.vld[sp] + d);
+      if (f < kF4 && key < keys && d < a.D) {
+        const int sp = key < nf ? 0 : 1;
+        const int64_t row = key < nf ? key : key - nf;
+        kz = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(s.k[sp]) + row * s.kld[sp] + d);
+        vz = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(s.v[sp]) + row * s.vld[sp] + d);
       }
       kst[j] = kz;
       vst[j] = vz;
@@ -121,10 +122,8 @@ __global__ __launch_bounds__(64 * NW, 4) void k_span_f32(SpanArgs a, int mode, i
     if (t + 1 < nkv) load_tile(t + 1);
     const float* kt = sm + (t & 1) * kBuf;
     const float* vt = kt + kKTile;
-    const int i = i0 + t;
-    const bool front = i < nft;
-    const int k0 = (front ? i : i - nft) * kKeys;
-    if (active && (front || (k0 < w_hi && (k0 + kKeys > w_lo || k0 < s.sinks)))) {  // wave-uniform
+    const int k0 = (i0 + t) * kKeys;
+    if (active && k0 < w_hi && (k0 + kKeys > w_lo || k0 < sinks)) {  // wave-uniform
       f32x4 sc[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -136,8 +135,9 @@ __global__ __launch_bounds__(64 * NW, 4) void k_span_f32(SpanArgs a, int mode, i
 #pragma unroll
           for (int e = 0; e < 4; ++e) sc[kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[tt][e], sc[kb], 0, 0, 0);
         }
-      const bool whole = front ? k0 + kKeys <= s.n[0] : k0 + kKeys <= w_hi_all && (k0 >= w_lo_all || k0 + kKeys <= s.sinks);
-      const int up = (front ? s.n[0] - 4 * g : my_hi) - k0, down = front ? -4 * g : my_lo - k0, sink = s.sinks - 4 * g - k0;
+      const bool whole = k0 + kKeys <= w_hi_all && (k0 >= w_lo_all || k0 + kKeys <= sinks);
+      const int up = my_hi - k0, sink = sinks - 4 * g - k0;
+      const uint32_t hidden = static_cast<uint32_t>(max(0, my_lo - k0 - sink));  // [sinks, my_lo)
       float mx = neg_inf();
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(64 * NW, 4) void k_span_f32(SpanArgs a, int mode, i
         for (int r = 0; r < 4; ++r) {
           const int k = kb * 16 + r;
           float v = sc[kb][r] * a.scale_log2;
-          if (!whole) v = k < up && (k >= down || k < sink) ? v : neg_inf();
+          if (!whole) v = k < up && static_cast<uint32_t>(k - sink) >= hidden ? v : neg_inf();
           sc[kb][r] = v;
           mx = fmaxf(mx, v);
         }
@@ -213,8 +213,8 @@ __global__ __launch_bounds__(64 * NW, 4) void k_span_f32(SpanArgs a, int mode, i
     rows &= rows - 1;
     const SpanRow y = span_row(a, s, r);
     float ro_[DP / 16], rm, rl;
-    span_attend_row<float, DP / 16, 1>(a, s, y, min(i0 * kKeys, s.n[0]), min((i0 + nkv) * kKeys, s.n[0]),
-                                    max(0, min((i0 - nft) * kKeys, s.n[1])), max(0, min((i0 + nkv - nft) * kKeys, s.n[1])), ro_, rm, rl);
+    const int k0 = i0 * kKeys, k1 = min(k0 + nkv * kKeys, keys);
+    span_attend_row<float, DP / 16, 1>(a, s, y, min(k0, nf), min(k1, nf), max(0, k0 - nf), max(0, k1 - nf), ro_, rm, rl);
     span_write_row<float, DP / 16>(a, part, y, slice, ro_, rm, rl);
   }
 }

@@ -146,24 +146,24 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
   const int set_rows = f.mode == kFront ? ro * (a.B / a.G) : ro;
   const int rows = min(16 * RG, set_rows - r0);
   const int t0 = f.mode == kFront ? 0 : r0 / group, t1 = f.mode == kFront ? 0 : (r0 + rows - 1) / group;
-  const Spans s = make_spans<2>(a, f.mode, set, t0, t1);
   part.first = f.first;
 
+  // The queries are on their way before the lengths are known.
   char* mine = smem + wave * 32768;
   const uint32_t mine_addr = lds_addr(mine);
   char* sq = kShared ? smem + NW * 32768 : mine + 16384 + 8192;  // [rg][ks][lane]
-  int hi[RG], lo[RG];
+  int token[RG];
   {
-    const T* Q = static_cast<const T*>(a.q) + s.b0 * a.qst[0] + static_cast<int64_t>(s.hk) * group * a.qst[1];
+    const SpanSet w = span_set(a, f.mode, set);
+    const T* Q = static_cast<const T*>(a.q) + w.b0 * a.qst[0] + static_cast<int64_t>(w.hk) * group * a.qst[1];
     const u32x4 rq = make_rsrc(Q, 0x7ffffff0);
     const uint32_t sq_addr = lds_addr(sq);
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
       const int r = rg * 16 + c16;
-      const SpanRow x = span_row(a, s, r0 + min(r, rows - 1));
-      hi[rg] = s.hi(x.t);
-      lo[rg] = s.lo(x.t);
-      const uint32_t off = static_cast<uint32_t>(((x.b - s.b0) * a.qst[0] + (x.h - s.hk * group) * a.qst[1] + x.t * a.qst[2]) * 2);
+      const SpanRow x = span_row(a, w, r0 + min(r, rows - 1));
+      token[rg] = x.t;
+      const uint32_t off = static_cast<uint32_t>(((x.b - w.b0) * a.qst[0] + (x.h - w.hk * group) * a.qst[1] + x.t * a.qst[2]) * 2);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const int d0 = ks * 32 + 8 * g;
@@ -171,6 +171,13 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
           dma16(rq, __builtin_amdgcn_readfirstlane(sq_addr + (rg * KS + ks) * 1024), r < rows && d0 < a.D ? off + d0 * 2 : kOOB);
       }
     }
+  }
+  const Spans s = make_spans<2>(a, f.mode, set, t0, t1);
+  int hi[RG], lo[RG];
+#pragma unroll
+  for (int rg = 0; rg < RG; ++rg) {
+    hi[rg] = s.hi(token[rg]);
+    lo[rg] = s.lo(token[rg]);
   }
   // at least the least factor there is, so that a masked score stays -inf under a zero scale
   const float c = fabsf(a.scale_log2) < 0x1p-126f ? 0x1p-126f : fabsf(a.scale_log2);
@@ -250,7 +257,6 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
     const bool front = i < nft;
     const int kt = (front ? i : i - nft) * NK;
     const bool whole = front ? kt + NK <= s.n[0] : kt + NK <= hi_min && (kt >= lo_max || kt + NK <= s.sinks);
-    const bool sinks = !front && kt < s.sinks;
     u32x4 pf[RG][KB / 2];
     // Two groups of rows side by side, which hide each other's latencies: a SIMD has this
     // wave alone.  (The keys' fragments are read again for each pair: there are registers
@@ -285,22 +291,19 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
 #pragma unroll
         for (int u = 0; u < PG; ++u) {
           const int rg = rg0 + u;
-          const int up = (front ? s.n[0] : hi[rg]) - kt - 4 * g, down = front ? -4 * g : lo[rg] - kt - 4 * g;
-          if (sinks) {
-            const int sink = s.sinks - kt - 4 * g;
+          const int up = (front ? s.n[0] : hi[rg]) - kt - 4 * g;
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[u][kb][e] = kb * 16 + e < up ? sc[u][kb][e] : neg_inf();
+          if (!front && kt < lo_max) {  // hidden: [sinks, lo)
+            const int sink = max(0, s.sinks) - kt - 4 * g;
+            const uint32_t hidden = static_cast<uint32_t>(max(0, lo[rg] - kt - 4 * g - sink));
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int k = kb * 16 + e;
-                sc[u][kb][e] = k < up && (k >= down || k < sink) ? sc[u][kb][e] : neg_inf();
-              }
-          } else {
-            const uint32_t seen = static_cast<uint32_t>(max(0, up - down));
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) sc[u][kb][e] = static_cast<uint32_t>(kb * 16 + e - down) < seen ? sc[u][kb][e] : neg_inf();
+              for (int e = 0; e < 4; ++e)
+                sc[u][kb][e] = static_cast<uint32_t>(kb * 16 + e - sink) < hidden ? neg_inf() : sc[u][kb][e];
           }
         }
       }
@@ -482,8 +485,9 @@ int launch_few(const SpanArgs& a, const FewBlocks& front, const FewBlocks& main,
 
 template <typename T, int D, int NW, int RGF>
 int launch_few(const SpanArgs& a, const FewBlocks& front, const FewBlocks& main, int rows, const SpanPart& part, hipStream_t st) {
-  if (rows <= 16) return launch_few<T, D, NW, RGF, 1>(a, front, main, part, st);
-  return launch_few<T, D, NW, RGF, 2>(a, front, main, part, st);
+  if constexpr (RGF != 1 && RGF != 2)  // (a group has more rows than a sequence)
+    if (rows > 16) return launch_few<T, D, NW, RGF, 2>(a, front, main, part, st);
+  return launch_few<T, D, NW, RGF, 1>(a, front, main, part, st);
 }
 
 template <typename T, int D>
@@ -498,11 +502,14 @@ int run_few(const SpanArgs& a, const FewPlan& p, const SpanPart& part, hipStream
   main.blocks = main.sets * main.slices;
   if (p.front_slices > 0) {
     front.mode = kFront;
-    front.row_blocks = static_cast<int>(ceil_div(span_rows(a, kFront), 64));
+    const int64_t front_rows = span_rows(a, kFront);
+    front.row_blocks = static_cast<int>(ceil_div(front_rows, 64));
     front.slices = p.front_slices;
     front.sets = span_sets(a, kFront);
     front.blocks = front.sets * front.slices;
     if (front.row_blocks > 1) front.blocks = ceil_div(front.blocks, 8) * 8 * front.row_blocks;
+    if (front_rows <= 16) return launch_few<T, D, 2, 1>(a, front, main, rows, part, st);
+    if (front_rows <= 32) return launch_few<T, D, 2, 2>(a, front, main, rows, part, st);
     return launch_few<T, D, 2, 4>(a, front, main, rows, part, st);
   }
   return p.waves == 1 ? launch_few<T, D, 1, 0>(a, front, main, rows, part, st) : launch_few<T, D, 2, 0>(a, front, main, rows, part, st);

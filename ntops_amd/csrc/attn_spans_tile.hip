@@ -50,11 +50,28 @@ struct SpanDma {
       voff[i] = c * 8 < dt ? static_cast<uint32_t>(row * ld * 2 + c * 16) : kOOB;
     }
   }
-  // 64 rows from row0 < n on of `n` at `base` (rows past them are zeros) into the LDS
-  __device__ __forceinline__ void issue(const char* base, int64_t ld, int row0, int n, int dt, uint32_t tile) const {
-    const u32x4 r = make_rsrc(base + row0 * ld * 2, ((n - row0 - 1) * ld + dt) * 2);
+  // `n` rows at `base` (those past them are zeros) into the LDS
+  __device__ __forceinline__ void issue(const char* base, int64_t ld, int n, int dt, uint32_t tile) const {
+    const u32x4 r = make_rsrc(base, ((n - 1) * ld + dt) * 2);
 #pragma unroll
     for (int i = 0; i < kInst; ++i) dma16(r, __builtin_amdgcn_readfirstlane(tile + lds_off + i * 1024), voff[i]);
+  }
+  // the same, but the tile's rows below `cut` from `front` and the others from `base`; once
+  // a block, so in few instructions
+  __device__ __forceinline__ void issue_two(const char* front, const char* base, int64_t ld, int cut, int n, int dt, uint32_t tile, int lane) const {
+    constexpr int cpr = D / 8;
+#pragma unroll 1
+    for (int i = 0; i < kInst; ++i) {
+      const int first = lds_off / (D * 2) + i * kRowsPerInst, row = first + lane / cpr;
+      const int c = IS_V ? vslot<D>(row, lane % cpr) : kslot<D>(row, lane % cpr);
+      const uint32_t off = c * 8 < dt ? static_cast<uint32_t>(row * ld * 2 + c * 16) : kOOB;
+      const uint32_t at = __builtin_amdgcn_readfirstlane(tile + first * (D * 2));
+#pragma unroll 1
+      for (int part = 0; part < 2; ++part) {
+        const u32x4 r = make_rsrc(part ? base : front, ((part ? n : cut) - 1) * ld * 2 + dt * 2);
+        if ((row < cut) == (part == 0)) dma16(r, at, off);  // (a lane that is off writes nothing into the LDS)
+      }
+    }
   }
 };
 
@@ -111,8 +128,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_span_tile(SpanArgs a, int mo
   const bool in_rows = my_r < nrows;
   const SpanRow x = span_row(a, s, min(my_r, nrows - 1));
   const int tw0 = front_only ? 0 : min(qw, nrows - 1) / group, tw1 = front_only ? 0 : min(qw + 31, nrows - 1) / group;
-  // main keys [lo, hi) that some row of the wave sees, and between lo_all and hi_all every row
-  const int w_hi = s.hi(tw1), w_lo = s.lo(tw0), w_hi_all = s.hi(tw0), w_lo_all = s.lo(tw1);
+  // The front's keys and the main ones behind them, as one sequence: of it [lo, hi) and
+  // all below `sinks` are seen by some row of the wave, between lo_all and hi_all by every row
+  const int nf = s.n[0], keys = nf + s.n[1];
+  const int sinks = nf + max(0, s.sinks);
+  const int w_hi = nf + s.hi(tw1), w_lo = nf + s.lo(tw0), w_hi_all = nf + s.hi(tw0), w_lo_all = nf + s.lo(tw1);
 
   u32x4 qf[KS];  // Q fragments (A operand of S): row my_r, d = 16 ks + 8 (lane >> 5) .. + 7
   {
@@ -123,13 +143,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_span_tile(SpanArgs a, int mo
       qf[ks] = in_rows && d0 < a.D ? *reinterpret_cast<const u32x4*>(Q + d0) : u32x4{0, 0, 0, 0};
       if (a.scale_log2 < 0.f) qf[ks] ^= 0x80008000u;
     }
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[ks]));
   }
   // at least the least factor there is, so that a masked score stays -inf under a zero scale
   const float c = fabsf(a.scale_log2) < 0x1p-126f ? 0x1p-126f : fabsf(a.scale_log2);
 
-  const int nft = (s.n[0] + kKeys - 1) / kKeys, nt = nft + (s.n[1] + kKeys - 1) / kKeys;
+  const int nt = (keys + kKeys - 1) / kKeys;
   const int share = (nt + slices - 1) / slices;
   const int i0 = min(slice * share, nt);
   const int nkv = min(i0 + share, nt) - i0;  // tiles of this item
@@ -142,21 +160,29 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_span_tile(SpanArgs a, int mo
   // tile g of the item into its stage
   const auto dma = [&](int g) __attribute__((always_inline)) {
     const uint32_t st = smem_addr + static_cast<uint32_t>((g & 1) * kStage);
-    const int i = i0 + g, span = i < nft ? 0 : 1;
-    const int row0 = (span == 0 ? i : i - nft) * kKeys;
-    kd.issue(s.k[span], kld, row0, s.n[span], a.D, st);
-    vd.issue(s.v[span], vld, row0, s.n[span], a.D, st + kTile);
+    const int k0 = (i0 + g) * kKeys;
+    if (k0 < nf && k0 + kKeys > nf && s.n[1] > 0) {  // the front's last keys and the first main ones
+      const int64_t back = nf - k0;
+      kd.issue_two(s.k[0] + k0 * kld * 2, s.k[1] - back * kld * 2, kld, nf - k0, keys - k0, a.D, st, lane);
+      vd.issue_two(s.v[0] + k0 * vld * 2, s.v[1] - back * vld * 2, vld, nf - k0, keys - k0, a.D, st + kTile, lane);
+      return;
+    }
+    const int span = k0 < nf ? 0 : 1, row0 = span == 0 ? k0 : k0 - nf;
+    kd.issue(s.k[span] + row0 * kld * 2, kld, s.n[span] - row0, a.D, st);
+    vd.issue(s.v[span] + row0 * vld * 2, vld, s.n[span] - row0, a.D, st + kTile);
   };
+  if (nkv > 0) dma(0);
+  // the queries settle here, with tile 0
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) asm volatile("" ::"v"(qf[ks]));
   // whether the wave has rows that see keys of tile g
   const auto need = [&](int g) __attribute__((always_inline)) {
-    const int i = i0 + g;
-    if (i < nft) return active;
-    const int k0 = (i - nft) * kKeys;
-    return active && k0 < w_hi && (k0 + kKeys > w_lo || k0 < s.sinks);
+    const int k0 = (i0 + g) * kKeys;
+    return active && k0 < w_hi && (k0 + kKeys > w_lo || k0 < sinks);
   };
   // limits of row my_r relative to this lane's column group: element (u, e) of a tile is
   // its key 32 u + 8 (e >> 2) + (e & 3) past that origin
-  const int my_hi = s.hi(x.t) - 4 * (lane >> 5), my_lo = s.lo(x.t) - 4 * (lane >> 5);
+  const int my_hi = nf + s.hi(x.t) - 4 * (lane >> 5), my_lo = nf + s.lo(x.t) - 4 * (lane >> 5);
 
   f32x16 o[DT];
 #pragma unroll
@@ -204,20 +230,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_span_tile(SpanArgs a, int mo
     __builtin_amdgcn_sched_barrier(0);
   };
   const auto vector_phase = [&](int g) __attribute__((always_inline)) {
-    const int i = i0 + g;
-    const bool front = i < nft;
-    const int k0 = (front ? i : i - nft) * kKeys;
-    const bool whole = front ? k0 + kKeys <= s.n[0] : k0 + kKeys <= w_hi_all && (k0 >= w_lo_all || k0 + kKeys <= s.sinks);
-    if (!whole) {
-      const int up = (front ? s.n[0] - 4 * (lane >> 5) : my_hi) - k0, down = front ? -64 : my_lo - k0;
-      const int sink = s.sinks - 4 * (lane >> 5) - k0;
+    const int k0 = (i0 + g) * kKeys;
+    if (k0 + kKeys > w_hi_all) {
+      const int up = my_hi - k0;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int k = 32 * u + 8 * (e >> 2) + (e & 3);
-          sc[u][e] = k < up && (k >= down || k < sink) ? sc[u][e] : neg_inf();
-        }
+        for (int e = 0; e < 16; ++e) sc[u][e] = 32 * u + 8 * (e >> 2) + (e & 3) < up ? sc[u][e] : neg_inf();
+    }
+    if (k0 < w_lo_all && k0 + kKeys > sinks) {  // hidden: [sinks, my_lo)
+      const int sink = sinks - 4 * (lane >> 5) - k0;
+      const uint32_t hidden = static_cast<uint32_t>(max(0, my_lo - k0 - sink));
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          sc[u][e] = static_cast<uint32_t>(32 * u + 8 * (e >> 2) + (e & 3) - sink) < hidden ? neg_inf() : sc[u][e];
     }
     const float th = max32(sc) * c;  // of this lane's half of the row (base 2)
     if (__any(th > m_run + kSlack)) {
@@ -249,7 +277,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_span_tile(SpanArgs a, int mo
     for (int sl = 0; sl < 4; ++sl) pf[sl] = pack8<T>(&p[sl >> 1][8 * (sl & 1)]);
   };
 
-  if (nkv > 0) dma(0);
   for (int k = 0; k < nkv; ++k) {
     wait_vmcnt<0>();
     block_barrier();  // tile k is in, and every wave is done with tile k - 1
@@ -316,8 +343,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_span_tile(SpanArgs a, int mo
     rows &= rows - 1;
     const SpanRow y = span_row(a, s, r);
     float ro_[DM / 16], rm, rl;
-    span_attend_row<T, DM / 16, 1>(a, s, y, min(i0 * kKeys, s.n[0]), min((i0 + nkv) * kKeys, s.n[0]),
-                               max(0, min((i0 - nft) * kKeys, s.n[1])), max(0, min((i0 + nkv - nft) * kKeys, s.n[1])), ro_, rm, rl);
+    const int k0 = i0 * kKeys, k1 = min(k0 + nkv * kKeys, keys);
+    span_attend_row<T, DM / 16, 1>(a, s, y, min(k0, nf), min(k1, nf), max(0, k0 - nf), max(0, k1 - nf), ro_, rm, rl);
     span_write_row<T, DM / 16>(a, part, y, slice, ro_, rm, rl);
   }
 }
