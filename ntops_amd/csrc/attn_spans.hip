@@ -243,11 +243,22 @@ bool matrix_layout(const SpanArgs& a, int dtype) {
 
 int run(int dtype, SpanArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
   if (ws == nullptr) ws_bytes = 0;
-  // a span without keys has the other's strides
-  for (int i = 0; i < 4; ++i) {
-    if (a.P == 0) a.pkst[i] = a.kst[i], a.pvst[i] = a.vst[i];
-    if (a.C == 0) a.kst[i] = a.pkst[i], a.vst[i] = a.pvst[i];
-  }
+  // Strides that nothing is multiplied with do not decide on the kernel; a span of one key
+  // or none has the other's row stride.
+  const auto quiet = [](int64_t (&s)[4], int64_t n0, int64_t n1, int64_t n2) {
+    if (n0 <= 1) s[0] = 0;
+    if (n1 <= 1) s[1] = 0;
+    if (n2 <= 1) s[2] = 0;
+  };
+  quiet(a.qst, a.B, a.Hq, a.Sq);
+  quiet(a.ost, a.B, a.Hq, a.Sq);
+  const int64_t row = (a.D + 7) / 8 * 8;
+  for (auto* s : {&a.kst, &a.vst}) quiet(*s, a.B, a.Hkv, a.C);
+  for (auto* s : {&a.pkst, &a.pvst}) quiet(*s, a.G, a.Hkv, a.P);
+  if (a.C <= 1) a.kst[2] = a.P > 1 ? a.pkst[2] : row, a.vst[2] = a.P > 1 ? a.pvst[2] : row;
+  if (a.P <= 1) a.pkst[2] = a.kst[2], a.pvst[2] = a.vst[2];
+  if (a.C == 0) a.kst[3] = a.vst[3] = 1;
+  if (a.P == 0) a.pkst[3] = a.pvst[3] = 1;
   Plan p = make_plan(dtype, a);
   if (plan_bytes(a, p) > ws_bytes) {
     p = make_plan(dtype, a, true);

@@ -50,6 +50,8 @@ def multi_axis_rotary_position_embedding_qk(q, k, sin_table, cos_table, position
     for x in (q, k):
         if inplace and any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape)):
             raise RuntimeError(f"{what}: elements that share memory (a stride is 0) cannot be rotated in place")
+    if inplace and q.numel() and k.numel() and q.data_ptr() == k.data_ptr():
+        raise RuntimeError(f"{what}: q and k are one tensor, which would be rotated twice in place")
     dev = _lib.require_cuda(q, k, sin_table, cos_table, positions)
     lib = _lib.load()
     with _DeviceGuard(dev):

@@ -217,6 +217,39 @@ def test_scores_that_rise_and_fall(sq, dtype):
         check_prefix(q, kk, v, kk.flip(2)[:, :, : max(sq, 30)], v[:, :, : max(sq, 30)], scale=0.5)
 
 
+KERNELS = [
+    # tokens, query heads, heads, dim, dtype, kernel of a window, of a shared prefix of few and many keys again
+    (1, 8, 2, 128, torch.bfloat16, "few", "few", "few"), (8, 8, 2, 64, torch.float16, "few", "few", "few"), (9, 8, 2, 128, torch.bfloat16, "tile", "tile", "tile"),
+    (200, 8, 2, 96, torch.float16, "tile", "tile", "tile"), (3, 8, 2, 128, torch.float32, "f32", "f32", "f32"), (2, 8, 2, 100, torch.bfloat16, "rows", "rows", "rows"),
+    (2, 8, 2, 98, torch.float32, "rows", "rows", "rows"), (4, 8, 2, 136, torch.float16, "rows", "rows", "rows"),
+]
+
+
+@pytest.mark.parametrize("sq,hq,hkv,d,dtype,window,short,long", KERNELS)
+def test_kernels(sq, hq, hkv, d, dtype, window, short, long):
+    """Which kernel serves a call: by rows, type and head dim; strides of a dim of one
+    element do not matter."""
+    q, k, v = window_inputs(4, hq, hkv, sq, 300, d, dtype)
+    check_window(q, k, v, 100, 4)
+    assert f" {window} " in _lib.last_kernel()
+    check_prefix(q, k[:1], v[:1], k[:, :, :40], v[:, :, :40])
+    nt.shared_prefix_attention(q, k[:1], v[:1], k, v)
+    k1 = torch.randn(4, hkv, d, 1, device="cuda").to(dtype).transpose(2, 3)  # one token: a row stride of 1
+    assert k1.stride(2) == 1
+    check_window(q[:, :, :1], k1, k1, 5)
+    check_prefix(q, k1[:2], k1[:2], k, v)
+    check_prefix(q, k[:2], v[:2], k1, k1)
+    lengthy = torch.randn(1, hkv, 20000, d, device="cuda").to(dtype)
+    big = q.repeat(16, 1, 1, 1)
+    kk, vv = k.repeat(16, 1, 1, 1), v.repeat(16, 1, 1, 1)
+    out = nt.shared_prefix_attention(big, lengthy, lengthy, kk, vv)
+    assert any(f" {x} " in _lib.last_kernel() for x in (short, long))
+    again = nt.shared_prefix_attention(big[:4], lengthy, lengthy, kk[:4], vv[:4])
+    # the same rows, joined from other slices: each within its roundings
+    u = HALF_STEP[dtype] if dtype != torch.float32 else 2.0**-18
+    assert ((out[:4].double() - again.double()).abs() <= 4 * u * (again.double().abs() + 1)).all()
+
+
 def test_same_results_every_time():
     for sq in (1, 7, 200):
         q, k, v = window_inputs(3, 8, 2, sq, 900, 128, torch.bfloat16)

@@ -86,6 +86,9 @@ def test_rotary_refusals():
     q = zeros(2, 5, 1, 8).expand(2, 5, 4, 8)
     with pytest.raises(RuntimeError, match="share memory"):
         nt.multi_axis_rotary_position_embedding_qk(q, zeros(2, 5, 2, 8), zeros(9, 4), zeros(9, 4), zeros(3, 2, 5, dtype=torch.int64), (1, 1, 2), inplace=True)
+    one = zeros(2, 5, 4, 8)
+    with pytest.raises(RuntimeError, match="twice"):
+        nt.multi_axis_rotary_position_embedding_qk(one, one, zeros(9, 4), zeros(9, 4), zeros(3, 2, 5, dtype=torch.int64), (1, 1, 2), inplace=True)
     with pytest.raises(TypeError):
         rope(sections=(1.5, 2.5))
 
