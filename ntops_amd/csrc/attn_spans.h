@@ -27,6 +27,7 @@ struct SpanArgs {
   const void* plengths;  // tokens of each prefix (null: P)
   int lengths_dtype, plengths_dtype;
   int B, Hq, Hkv, Sq, C, D, G, P;
+  int group, per;  // query heads of a cache head; sequences of a prefix
   int window, sinks;  // at least 1; 0 with a shared prefix
   float scale_log2;   // scale * log2(e)
 };
@@ -51,11 +52,14 @@ struct SpanSet {
   int b0;  // first sequence
   int hk;  // cache head
 };
-__device__ __forceinline__ SpanSet span_set(const SpanArgs& a, int mode, int64_t set) {
+// (Every count of blocks and rows is below 2^32: quotients of 64 bits would cost hundreds
+// of instructions a wave.)
+__device__ __forceinline__ SpanSet span_set(const SpanArgs& a, int mode, uint32_t set) {
   SpanSet s;
-  s.at = static_cast<int>(set / a.Hkv);
-  s.hk = static_cast<int>(set - static_cast<int64_t>(s.at) * a.Hkv);
-  s.b0 = mode == kFront ? s.at * (a.B / a.G) : s.at;
+  const uint32_t at = set / static_cast<uint32_t>(a.Hkv);
+  s.at = static_cast<int>(at);
+  s.hk = static_cast<int>(set - at * a.Hkv);
+  s.b0 = mode == kFront ? s.at * a.per : s.at;
   return s;
 }
 
@@ -78,7 +82,7 @@ __device__ __forceinline__ int span_length(const void* p, int dtype, int i, int 
 
 // Spans of the rows of tokens t0 .. t1 of set `set`; ES: bytes of an element.
 template <int ES>
-__device__ __forceinline__ Spans make_spans(const SpanArgs& a, int mode, int64_t set, int t0, int t1) {
+__device__ __forceinline__ Spans make_spans(const SpanArgs& a, int mode, uint32_t set, int t0, int t1) {
   Spans s;
   static_cast<SpanSet&>(s) = span_set(a, mode, set);
   const int at = s.at;
@@ -108,7 +112,7 @@ __device__ __forceinline__ Spans make_spans(const SpanArgs& a, int mode, int64_t
     }
   }
   if (a.pk != nullptr && mode != kMain) {
-    const int g = mode == kFront ? at : at / (a.B / a.G);
+    const int g = mode == kFront ? at : static_cast<int>(static_cast<uint32_t>(at) / static_cast<uint32_t>(a.per));
     s.n[0] = span_length(a.plengths, a.plengths_dtype, g, a.P);
     s.k[0] = static_cast<const char*>(a.pk) + (g * a.pkst[0] + s.hk * a.pkst[1]) * ES;
     s.v[0] = static_cast<const char*>(a.pv) + (g * a.pvst[0] + s.hk * a.pvst[1]) * ES;
@@ -122,15 +126,16 @@ __device__ __forceinline__ Spans make_spans(const SpanArgs& a, int mode, int64_t
 struct SpanRow {
   int b, t, h;
 };
-__device__ __forceinline__ SpanRow span_row(const SpanArgs& a, const SpanSet& s, int r) {
-  const int group = a.Hq / a.Hkv, ro = group * a.Sq;
-  SpanRow x;
-  x.b = r / ro;
-  r -= x.b * ro;
-  x.t = r / group;
-  x.h = s.hk * group + r - x.t * group;
-  x.b += s.b0;
-  return x;
+__device__ __forceinline__ SpanRow span_row(const SpanArgs& a, int mode, const SpanSet& s, int row) {
+  const uint32_t group = static_cast<uint32_t>(a.group);
+  uint32_t r = static_cast<uint32_t>(row), b = 0;
+  if (mode == kFront) {
+    const uint32_t ro = group * a.Sq;
+    b = r / ro;
+    r -= b * ro;
+  }
+  const uint32_t t = r / group;
+  return {s.b0 + static_cast<int>(b), static_cast<int>(t), s.hk * a.group + static_cast<int>(r - t * group)};
 }
 
 // Partial results of slices: per query row (batch, head, token) and slice the

@@ -22,15 +22,14 @@ constexpr int64_t kMaxCount = 0x7fffffff;
 template <typename T, int EL>
 __global__ __launch_bounds__(256) void k_span_rows(SpanArgs a, int mode, int slices, SpanPart part, int64_t total) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t id = block_id() * 4 + wave;
-  if (id >= total) return;
-  const int64_t rows = static_cast<int64_t>(a.Hq / a.Hkv) * a.Sq * (mode == kFront ? a.B / a.G : 1);
-  const int slice = static_cast<int>(id % slices);
-  const int64_t at = id / slices, set = at / rows;
-  const int r = static_cast<int>(at - set * rows);
-  const int t = r / (a.Hq / a.Hkv) % a.Sq;
+  const int64_t at = block_id() * 4 + wave;
+  if (at >= total) return;
+  const uint32_t id = static_cast<uint32_t>(at), rows = static_cast<uint32_t>(a.group * a.Sq * (mode == kFront ? a.per : 1));
+  const uint32_t row = id / static_cast<uint32_t>(slices), set = row / rows;
+  const int slice = static_cast<int>(id - row * slices), r = static_cast<int>(row - set * rows);
+  const int t = static_cast<int>(static_cast<uint32_t>(r) / static_cast<uint32_t>(a.group) % static_cast<uint32_t>(a.Sq));
   const Spans s = make_spans<sizeof(T)>(a, mode, set, t, t);
-  const SpanRow x = span_row(a, s, r);
+  const SpanRow x = span_row(a, mode, s, r);
   const int fc = (s.n[0] + slices - 1) / slices, mc = (s.n[1] + slices - 1) / slices;
   float o[EL], m, l;
   span_attend_row<T, EL, (EL > 8 ? 2 : 4)>(a, s, x, min(slice * fc, s.n[0]), min(slice * fc + fc, s.n[0]), min(slice * mc, s.n[1]), min(slice * mc + mc, s.n[1]),
@@ -79,9 +78,8 @@ __global__ __launch_bounds__(256) void k_span_merge(SpanArgs a, SpanPart part) {
     for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], step, 64);
   if (g != 0) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int t = static_cast<int>(row % a.Sq);
-  const int64_t bh = row / a.Sq;
-  T* O = static_cast<T*>(a.o) + (bh / a.Hq) * a.ost[0] + (bh % a.Hq) * a.ost[1] + t * a.ost[2];
+  const uint32_t id = static_cast<uint32_t>(row), bh = id / static_cast<uint32_t>(a.Sq), b = bh / static_cast<uint32_t>(a.Hq);
+  T* O = static_cast<T*>(a.o) + b * a.ost[0] + (bh - b * a.Hq) * a.ost[1] + (id - bh * a.Sq) * a.ost[2];
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (d + e < a.D) O[(d + e) * a.ost[3]] = static_cast<T>(o[e] * inv);
@@ -242,6 +240,8 @@ bool matrix_layout(const SpanArgs& a, int dtype) {
 }
 
 int run(int dtype, SpanArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
+  a.group = a.Hq / a.Hkv;
+  a.per = a.B / a.G;
   if (ws == nullptr) ws_bytes = 0;
   // Strides that nothing is multiplied with do not decide on the kernel; a span of one key
   // or none has the other's row stride.

@@ -28,7 +28,7 @@ template <int DP>
 constexpr int kLdsBytes = 2 * (kKeys * (DP + 4) + DP * (kKeys + 4)) * 4;
 
 template <int DP, int NW>
-__global__ __launch_bounds__(64 * NW, 4) void k_span_f32(SpanArgs a, int mode, int nqb, int slices, int64_t total, SpanPart part) {
+__global__ __launch_bounds__(64 * NW, 4) void k_span_f32(SpanArgs a, int mode, int nqb, int slices, uint32_t total, SpanPart part) {
   constexpr int QB = 16 * NW;
   constexpr int KP = DP + 4;     // floats per K row in the LDS
   constexpr int VP = kKeys + 4;  // floats per V^T row
@@ -40,23 +40,24 @@ __global__ __launch_bounds__(64 * NW, 4) void k_span_f32(SpanArgs a, int mode, i
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
-  const int64_t pid = block_id();
-  if (pid >= total) return;  // the tail of a 2-D grid (the whole block)
-  const int per = nqb * slices;
-  const int64_t set = pid / per;
-  const int in = static_cast<int>(pid - set * per);
-  const int qb = nqb - 1 - in / slices, slice = in % slices;
-  const int group = a.Hq / a.Hkv, ro = group * a.Sq;
+  const int64_t all = block_id();
+  if (all >= total) return;  // the tail of a 2-D grid (the whole block)
+  const uint32_t pid = static_cast<uint32_t>(all);
+  const uint32_t per = static_cast<uint32_t>(nqb * slices), set = pid / per, in = pid - set * per;
+  const uint32_t back = in / static_cast<uint32_t>(slices);
+  const int qb = nqb - 1 - static_cast<int>(back), slice = static_cast<int>(in - back * slices);
+  const int group = a.group, ro = group * a.Sq;
   const bool front_only = mode == kFront;
-  const int nrows = front_only ? ro * (a.B / a.G) : ro;
+  const auto token = [&](int row) { return static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(group)); };
+  const int nrows = front_only ? ro * a.per : ro;
   const int r0 = qb * QB, r1 = min(r0 + QB, nrows);
-  const Spans s = make_spans<4>(a, mode, set, front_only ? 0 : r0 / group, front_only ? 0 : (r1 - 1) / group);
+  const Spans s = make_spans<4>(a, mode, set, front_only ? 0 : token(r0), front_only ? 0 : token(r1 - 1));
 
   const int qw = r0 + wave * 16;
   const bool active = qw < nrows;
   const bool in_rows = qw + r16 < nrows;
-  const SpanRow x = span_row(a, s, min(qw + r16, nrows - 1));
-  const int tw0 = front_only ? 0 : min(qw, nrows - 1) / group, tw1 = front_only ? 0 : min(qw + 15, nrows - 1) / group;
+  const SpanRow x = span_row(a, mode, s, min(qw + r16, nrows - 1));
+  const int tw0 = front_only ? 0 : token(min(qw, nrows - 1)), tw1 = front_only ? 0 : token(min(qw + 15, nrows - 1));
   f32x4 qf[DP / 16];
   {
     const float* Q = static_cast<const float*>(a.q) + x.b * a.qst[0] + x.h * a.qst[1] + x.t * a.qst[2];
@@ -211,7 +212,7 @@ __global__ __launch_bounds__(64 * NW, 4) void k_span_f32(SpanArgs a, int mode, i
   while (rows != 0) {
     const int r = qw + __builtin_ctz(rows);
     rows &= rows - 1;
-    const SpanRow y = span_row(a, s, r);
+    const SpanRow y = span_row(a, mode, s, r);
     float ro_[DP / 16], rm, rl;
     const int k0 = i0 * kKeys, k1 = min(k0 + nkv * kKeys, keys);
     span_attend_row<float, DP / 16, 1>(a, s, y, min(k0, nf), min(k1, nf), max(0, k0 - nf), max(0, k1 - nf), ro_, rm, rl);
@@ -229,7 +230,7 @@ int launch_f32(const SpanArgs& a, int mode, int slices, const SpanPart& part, hi
   const int64_t nqb = ceil_div(span_rows(a, mode), 16 * NW);
   const int64_t total = span_sets(a, mode) * nqb * slices;
   note_kernel("%s f32 d%d waves%d mode%d split%d", a.pk ? "shared_prefix" : "sliding_window", DP, NW, mode, slices);
-  hipLaunchKernelGGL(kern, blocks_2d(total), dim3(64 * NW), kLdsBytes<DP>, st, a, mode, static_cast<int>(nqb), slices, total, part);
+  hipLaunchKernelGGL(kern, blocks_2d(total), dim3(64 * NW), kLdsBytes<DP>, st, a, mode, static_cast<int>(nqb), slices, static_cast<uint32_t>(total), part);
   return check_launch("attention");
 }
 

@@ -108,7 +108,7 @@ struct FewBlocks {
   int row_blocks;  // of a set
   int slices;
   int first;       // slice of the rows that slice 0 is
-  int64_t sets, blocks;
+  uint32_t sets, blocks;
 };
 
 // Where the queries lie: up to two groups of rows go to registers, through the LDS of a
@@ -119,7 +119,7 @@ constexpr int kQueryLds = RG > 2 ? RG * (D / 32) * 1024 : 0;
 
 // RG: groups of 16 rows a block has room for.
 template <typename T, int D, int NW, int RG>
-__device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f, SpanPart part, int64_t id, char* smem) {
+__device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f, SpanPart part, uint32_t id, char* smem) {
   constexpr int NK = kTileKeys<D>;
   constexpr int KB = NK / 16;  // 16-key blocks of a tile
   constexpr int KS = D / 32;   // k-steps of S^T = K Q^T
@@ -131,21 +131,25 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
   const int g = lane >> 4, c16 = lane & 15;
   // Blocks of the same keys and other rows run on one XCD (workgroups go round the 8),
   // whose L2 then brings the keys in once.
-  int64_t at = id;
+  uint32_t at = id;
   int rb = 0;
   if (f.row_blocks > 1) {
-    const int64_t t = id >> 3;
-    rb = static_cast<int>(t % f.row_blocks);
-    at = t / f.row_blocks * 8 + (id & 7);
+    const uint32_t t = id >> 3, of = t / static_cast<uint32_t>(f.row_blocks);
+    rb = static_cast<int>(t - of * f.row_blocks);
+    at = of * 8 + (id & 7);
   }
-  const int64_t set = at / f.slices;
+  const uint32_t set = at / static_cast<uint32_t>(f.slices);
   const int slice = static_cast<int>(at - set * f.slices);
   if (set >= f.sets) return;  // (the whole block: the last eight)
   const int r0 = rb * (16 * RG);
-  const int group = a.Hq / a.Hkv, ro = group * a.Sq;
-  const int set_rows = f.mode == kFront ? ro * (a.B / a.G) : ro;
+  const int ro = a.group * a.Sq;
+  const int set_rows = f.mode == kFront ? ro * a.per : ro;
   const int rows = min(16 * RG, set_rows - r0);
-  const int t0 = f.mode == kFront ? 0 : r0 / group, t1 = f.mode == kFront ? 0 : (r0 + rows - 1) / group;
+  int t0 = 0, t1 = 0;
+  if (f.mode != kFront) {
+    t0 = static_cast<int>(static_cast<uint32_t>(r0) / static_cast<uint32_t>(a.group));
+    t1 = static_cast<int>(static_cast<uint32_t>(r0 + rows - 1) / static_cast<uint32_t>(a.group));
+  }
   part.first = f.first;
 
   // The queries are on their way before the lengths are known.
@@ -155,15 +159,15 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
   int token[RG];
   {
     const SpanSet w = span_set(a, f.mode, set);
-    const T* Q = static_cast<const T*>(a.q) + w.b0 * a.qst[0] + static_cast<int64_t>(w.hk) * group * a.qst[1];
+    const T* Q = static_cast<const T*>(a.q) + w.b0 * a.qst[0] + static_cast<int64_t>(w.hk) * a.group * a.qst[1];
     const u32x4 rq = make_rsrc(Q, 0x7ffffff0);
     const uint32_t sq_addr = lds_addr(sq);
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
       const int r = rg * 16 + c16;
-      const SpanRow x = span_row(a, w, r0 + min(r, rows - 1));
+      const SpanRow x = span_row(a, f.mode, w, r0 + min(r, rows - 1));
       token[rg] = x.t;
-      const uint32_t off = static_cast<uint32_t>(((x.b - w.b0) * a.qst[0] + (x.h - w.hk * group) * a.qst[1] + x.t * a.qst[2]) * 2);
+      const uint32_t off = static_cast<uint32_t>(((x.b - w.b0) * a.qst[0] + (x.h - w.hk * a.group) * a.qst[1] + x.t * a.qst[2]) * 2);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const int d0 = ks * 32 + 8 * g;
@@ -376,10 +380,12 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
   wait_dma<0>();  // no DMA may land in the LDS that the joining reuses
 
   // join the waves, a group of rows after the other: [wave][16] maxima, [wave][16]
-  // sums, a bit per row that has to be computed again, then [wave][16][D + 4] O
+  // sums, a bit per row that has to be computed again, the rows' places, then
+  // [wave][16][D + 4] O
   float* sm = reinterpret_cast<float*>(smem);
   uint32_t* again = reinterpret_cast<uint32_t*>(sm + 2 * NW * 16);
-  float* so = sm + 2 * NW * 16 + 4;
+  int64_t* to = reinterpret_cast<int64_t*>(sm + 2 * NW * 16 + 4);  // where each row goes
+  float* so = sm + 2 * NW * 16 + 36;
   constexpr int LD = D + 4;
 #pragma unroll
   for (int rg = 0; rg < RG; ++rg) {
@@ -391,6 +397,10 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
     if (g == 0) {
       sm[wave * 16 + c16] = m[rg];
       sm[(NW + wave) * 16 + c16] = l[rg];
+      if (rg % NW == wave) {
+        const SpanRow x = span_row(a, f.mode, s, r0 + min(rg * 16 + c16, rows - 1));
+        to[c16] = part.p ? part.at(a, x, slice) : x.b * a.ost[0] + x.h * a.ost[1] + x.t * a.ost[2];
+      }
     }
 #pragma unroll
     for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4*>(so + (wave * 16 + c16) * LD + t * 16 + 4 * g) = o[rg][t];
@@ -413,11 +423,10 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] += mw == neg_inf() ? 0.f : ow[e] * fw;
       }
-      const SpanRow x = span_row(a, s, r0 + rg * 16 + row);
       const float any = (v[0] + v[1]) + (v[2] + v[3]);
       if (!(any == any) && sum == sum) atomicOr(&again[rg >> 1], 1u << ((rg & 1) * 16 + row));
       if (part.p) {
-        const int64_t pa = part.at(a, x, slice);
+        const int64_t pa = to[row];
         if (d == 0) {
           float* ml = part.ml(a, pa);
           ml[0] = mm;
@@ -429,7 +438,7 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
         T w4[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) w4[e] = static_cast<T>(v[e] * inv);
-        *reinterpret_cast<u32x2*>(static_cast<T*>(a.o) + x.b * a.ost[0] + x.h * a.ost[1] + x.t * a.ost[2] + d) =
+        *reinterpret_cast<u32x2*>(static_cast<T*>(a.o) + to[row] + d) =
             __builtin_bit_cast(u32x2, w4);
       }
     }
@@ -444,7 +453,7 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
     const int row = __builtin_ctzll(bad);
     bad &= bad - 1;
     if (row % NW != wave) continue;
-    const SpanRow x = span_row(a, s, r0 + row);
+    const SpanRow x = span_row(a, f.mode, s, r0 + row);
     float ro_[D / 16], rm, rl;
     span_attend_row<T, D / 16, 1>(a, s, x, min(i0 * NK, s.n[0]), min(i1 * NK, s.n[0]), max(0, min((i0 - nft) * NK, s.n[1])),
                                max(0, min((i1 - nft) * NK, s.n[1])), ro_, rm, rl);
@@ -457,8 +466,9 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
 template <typename T, int D, int NW, int RGF, int RGM>
 __global__ __launch_bounds__(64 * NW, 2) void k_span_few(SpanArgs a, FewBlocks front, FewBlocks main, SpanPart part) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];  // [wave][2 stages][K, V], queries
-  const int64_t id = block_id();
-  if (id >= front.blocks + main.blocks) return;  // the tail of a 2-D grid (the whole block)
+  const int64_t all = block_id();
+  if (all >= static_cast<int64_t>(front.blocks) + main.blocks) return;  // the tail of a 2-D grid (the whole block)
+  const uint32_t id = static_cast<uint32_t>(all);
   if constexpr (RGF > 0) {
     if (id < front.blocks) {
       few_block<T, D, NW, RGF>(a, front, part, id, smem);
@@ -471,7 +481,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_span_few(SpanArgs a, FewBlocks f
 template <typename T, int D, int NW, int RGF, int RGM>
 int launch_few(const SpanArgs& a, const FewBlocks& front, const FewBlocks& main, const SpanPart& part, hipStream_t st) {
   constexpr int kLds = NW * 32768 + kQueryLds<D, RGF>;
-  static_assert((2 * NW * 16 + 4 + NW * 16 * (D + 4)) * 4 <= NW * 32768, "LDS");
+  static_assert((2 * NW * 16 + 36 + NW * 16 * (D + 4)) * 4 <= NW * 32768, "LDS");
   auto kern = k_span_few<T, D, NW, RGF, RGM>;
   if constexpr (kLds > 65536) {
     static std::atomic<uint64_t> done{0};
@@ -479,7 +489,7 @@ int launch_few(const SpanArgs& a, const FewBlocks& front, const FewBlocks& main,
   }
   note_kernel("%s few d%d waves%d rows%d+%d split%d+%d", a.pk ? "shared_prefix" : "sliding_window", D, NW, 16 * RGF, 16 * RGM, front.slices,
               main.slices);
-  hipLaunchKernelGGL(kern, blocks_2d(front.blocks + main.blocks), dim3(64 * NW), kLds, st, a, front, main, part);
+  hipLaunchKernelGGL(kern, blocks_2d(static_cast<int64_t>(front.blocks) + main.blocks), dim3(64 * NW), kLds, st, a, front, main, part);
   return check_launch("attention");
 }
 
@@ -498,16 +508,16 @@ int run_few(const SpanArgs& a, const FewPlan& p, const SpanPart& part, hipStream
   main.row_blocks = 1;
   main.slices = p.slices;
   main.first = part.first;
-  main.sets = span_sets(a, main.mode);
+  main.sets = static_cast<uint32_t>(span_sets(a, main.mode));
   main.blocks = main.sets * main.slices;
   if (p.front_slices > 0) {
     front.mode = kFront;
     const int64_t front_rows = span_rows(a, kFront);
     front.row_blocks = static_cast<int>(ceil_div(front_rows, 64));
     front.slices = p.front_slices;
-    front.sets = span_sets(a, kFront);
+    front.sets = static_cast<uint32_t>(span_sets(a, kFront));
     front.blocks = front.sets * front.slices;
-    if (front.row_blocks > 1) front.blocks = ceil_div(front.blocks, 8) * 8 * front.row_blocks;
+    if (front.row_blocks > 1) front.blocks = (front.blocks + 7) / 8 * 8 * front.row_blocks;
     if (front_rows <= 16) return launch_few<T, D, 2, 1>(a, front, main, rows, part, st);
     if (front_rows <= 32) return launch_few<T, D, 2, 2>(a, front, main, rows, part, st);
     return launch_few<T, D, 2, 4>(a, front, main, rows, part, st);

@@ -90,7 +90,7 @@ __device__ __forceinline__ float max32(const f32x16 (&s)[2]) {
 
 // D: columns of a row in the LDS; DM: columns that are multiplied, at least the head dim.
 template <typename T, int D, int DM>
-__global__ __launch_bounds__(64 * kWaves, 2) void k_span_tile(SpanArgs a, int mode, int nqb, int slices, int64_t total, SpanPart part) {
+__global__ __launch_bounds__(64 * kWaves, 2) void k_span_tile(SpanArgs a, int mode, int nqb, int slices, uint32_t total, SpanPart part) {
   constexpr int KS = DM / 16;  // k-steps of S = Q K^T
   constexpr int DT = DM / 32;  // 32-column tiles of O
   constexpr int kTile = kKeys * D * 2;
@@ -99,35 +99,37 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_span_tile(SpanArgs a, int mo
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t pid = block_id();
-  if (pid >= total) return;  // the tail of a 2-D grid (the whole block)
+  const int64_t all = block_id();
+  if (all >= total) return;  // the tail of a 2-D grid (the whole block)
+  const uint32_t pid = static_cast<uint32_t>(all);
   // An XCD (workgroups go round them) walks whole sets, every eighth one, the rows with
   // the most keys first.
-  const int per = nqb * slices;
-  int64_t set;
-  int in;
-  if ((total / per & 7) == 0) {
-    const int64_t at = pid >> 3;
-    set = at / per * 8 + (pid & 7);
-    in = static_cast<int>(at % per);
+  const uint32_t per = static_cast<uint32_t>(nqb * slices), sets = total / per;
+  uint32_t set, in;
+  if ((sets & 7) == 0) {
+    const uint32_t at = pid >> 3, of = at / per;
+    set = of * 8 + (pid & 7);
+    in = at - of * per;
   } else {
     set = pid / per;
-    in = static_cast<int>(pid - set * per);
+    in = pid - set * per;
   }
-  const int qb = nqb - 1 - in / slices, slice = in % slices;
-  const int group = a.Hq / a.Hkv, ro = group * a.Sq;
-  const int nrows = mode == kFront ? ro * (a.B / a.G) : ro;
+  const uint32_t back = in / static_cast<uint32_t>(slices);
+  const int qb = nqb - 1 - static_cast<int>(back), slice = static_cast<int>(in - back * slices);
+  const int group = a.group, ro = group * a.Sq;
+  const int nrows = mode == kFront ? ro * a.per : ro;
   const int r0 = qb * kRowsBlock, r1 = min(r0 + kRowsBlock, nrows);
   const bool front_only = mode == kFront;
-  const Spans s = make_spans<2>(a, mode, set, front_only ? 0 : r0 / group, front_only ? 0 : (r1 - 1) / group);
+  const auto token = [&](int row) { return static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(group)); };
+  const Spans s = make_spans<2>(a, mode, set, front_only ? 0 : token(r0), front_only ? 0 : token(r1 - 1));
   const int64_t kld = s.kld[front_only ? 0 : 1], vld = s.vld[front_only ? 0 : 1];  // (equal where there are both)
 
   const int qw = r0 + wave * 32;
   const bool active = qw < nrows;
   const int my_r = qw + (lane & 31);
   const bool in_rows = my_r < nrows;
-  const SpanRow x = span_row(a, s, min(my_r, nrows - 1));
-  const int tw0 = front_only ? 0 : min(qw, nrows - 1) / group, tw1 = front_only ? 0 : min(qw + 31, nrows - 1) / group;
+  const SpanRow x = span_row(a, mode, s, min(my_r, nrows - 1));
+  const int tw0 = front_only ? 0 : token(min(qw, nrows - 1)), tw1 = front_only ? 0 : token(min(qw + 31, nrows - 1));
   // The front's keys and the main ones behind them, as one sequence: of it [lo, hi) and
   // all below `sinks` are seen by some row of the wave, between lo_all and hi_all by every row
   const int nf = s.n[0], keys = nf + s.n[1];
@@ -341,7 +343,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_span_tile(SpanArgs a, int mo
   while (rows != 0) {
     const int r = qw + __builtin_ctz(rows);
     rows &= rows - 1;
-    const SpanRow y = span_row(a, s, r);
+    const SpanRow y = span_row(a, mode, s, r);
     float ro_[DM / 16], rm, rl;
     const int k0 = i0 * kKeys, k1 = min(k0 + nkv * kKeys, keys);
     span_attend_row<T, DM / 16, 1>(a, s, y, min(k0, nf), min(k1, nf), max(0, k0 - nf), max(0, k1 - nf), ro_, rm, rl);
@@ -356,7 +358,7 @@ int launch_tile(const SpanArgs& a, int mode, int slices, const SpanPart& part, h
   const int64_t nqb = ceil_div(span_rows(a, mode), kRowsBlock);
   const int64_t total = span_sets(a, mode) * nqb * slices;
   note_kernel("%s tile d%d mode%d split%d", a.pk ? "shared_prefix" : "sliding_window", DM, mode, slices);
-  hipLaunchKernelGGL((k_span_tile<T, D, DM>), blocks_2d(total), dim3(64 * kWaves), kLds, st, a, mode, static_cast<int>(nqb), slices, total, part);
+  hipLaunchKernelGGL((k_span_tile<T, D, DM>), blocks_2d(total), dim3(64 * kWaves), kLds, st, a, mode, static_cast<int>(nqb), slices, static_cast<uint32_t>(total), part);
   return check_launch("attention");
 }
 
