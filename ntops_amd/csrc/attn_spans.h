@@ -270,8 +270,7 @@ struct FewPlan {
 };
 int span_few_run(int dtype, const SpanArgs& a, const FewPlan& p, const SpanPart& part, hipStream_t st);
 
-// The same for any number of rows, in blocks of kTileRows; kBoth: with equal row strides
-// of both spans.
+// The same for any number of rows, in blocks of kTileRows.
 constexpr int kTileRows = 128;
 int span_tile_run(int dtype, const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st);
 

@@ -243,8 +243,7 @@ int run(int dtype, SpanArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
   a.group = a.Hq / a.Hkv;
   a.per = a.B / a.G;
   if (ws == nullptr) ws_bytes = 0;
-  // Strides that nothing is multiplied with do not decide on the kernel; a span of one key
-  // or none has the other's row stride.
+  // Strides that nothing is multiplied with do not decide on the kernel.
   const auto quiet = [](int64_t (&s)[4], int64_t n0, int64_t n1, int64_t n2) {
     if (n0 <= 1) s[0] = 0;
     if (n1 <= 1) s[1] = 0;
@@ -255,8 +254,8 @@ int run(int dtype, SpanArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
   const int64_t row = (a.D + 7) / 8 * 8;
   for (auto* s : {&a.kst, &a.vst}) quiet(*s, a.B, a.Hkv, a.C);
   for (auto* s : {&a.pkst, &a.pvst}) quiet(*s, a.G, a.Hkv, a.P);
-  if (a.C <= 1) a.kst[2] = a.P > 1 ? a.pkst[2] : row, a.vst[2] = a.P > 1 ? a.pvst[2] : row;
-  if (a.P <= 1) a.pkst[2] = a.kst[2], a.pvst[2] = a.vst[2];
+  if (a.C <= 1) a.kst[2] = a.vst[2] = row;
+  if (a.P <= 1) a.pkst[2] = a.pvst[2] = row;
   if (a.C == 0) a.kst[3] = a.vst[3] = 1;
   if (a.P == 0) a.pkst[3] = a.pvst[3] = 1;
   Plan p = make_plan(dtype, a);
@@ -264,8 +263,7 @@ int run(int dtype, SpanArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
     p = make_plan(dtype, a, true);
     if (plan_bytes(a, p) > ws_bytes) p.slices = 1;
   }
-  const bool one_stride = a.pk == nullptr || (a.kst[2] == a.pkst[2] && a.vst[2] == a.pvst[2]);
-  if (p.main != kRows && (!matrix_layout(a, dtype) || (p.main == kTile && p.front_slices == 0 && !one_stride))) {
+  if (p.main != kRows && !matrix_layout(a, dtype)) {
     p = rows_plan(a);
     if (plan_bytes(a, p) > ws_bytes) p.slices = 1;
   }

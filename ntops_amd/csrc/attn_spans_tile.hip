@@ -56,24 +56,27 @@ struct SpanDma {
 #pragma unroll
     for (int i = 0; i < kInst; ++i) dma16(r, __builtin_amdgcn_readfirstlane(tile + lds_off + i * 1024), voff[i]);
   }
-  // the same, but the tile's rows below `cut` from `front` and the others from `base`; once
-  // a block, so in few instructions
-  __device__ __forceinline__ void issue_two(const char* front, const char* base, int64_t ld, int cut, int n, int dt, uint32_t tile, int lane) const {
-    constexpr int cpr = D / 8;
+};
+
+// A tile whose rows below `cut` come from `front` and the others from `base` (the row
+// that would be the tile's first), `n` rows in all; once a block, so in few instructions.
+template <int D, bool IS_V>
+__device__ __forceinline__ void dma_two(const char* front, int64_t front_ld, const char* base, int64_t ld, int cut, int n, int dt, uint32_t tile,
+                                        int wave, int lane) {
+  constexpr int kInst = SpanDma<D, IS_V>::kInst, kRowsPerInst = SpanDma<D, IS_V>::kRowsPerInst, cpr = D / 8;
 #pragma unroll 1
-    for (int i = 0; i < kInst; ++i) {
-      const int first = lds_off / (D * 2) + i * kRowsPerInst, row = first + lane / cpr;
-      const int c = IS_V ? vslot<D>(row, lane % cpr) : kslot<D>(row, lane % cpr);
-      const uint32_t off = c * 8 < dt ? static_cast<uint32_t>(row * ld * 2 + c * 16) : kOOB;
-      const uint32_t at = __builtin_amdgcn_readfirstlane(tile + first * (D * 2));
+  for (int i = 0; i < kInst; ++i) {
+    const int first = (wave * kInst + i) * kRowsPerInst, row = first + lane / cpr;
+    const int c = IS_V ? vslot<D>(row, lane % cpr) : kslot<D>(row, lane % cpr);
 #pragma unroll 1
-      for (int part = 0; part < 2; ++part) {
-        const u32x4 r = make_rsrc(part ? base : front, ((part ? n : cut) - 1) * ld * 2 + dt * 2);
-        if ((row < cut) == (part == 0)) dma16(r, at, off);  // (a lane that is off writes nothing into the LDS)
-      }
+    for (int part = 0; part < 2; ++part) {
+      const int64_t of = part ? ld : front_ld;
+      const u32x4 r = make_rsrc(part ? base : front, ((part ? n : cut) - 1) * of * 2 + dt * 2);
+      const uint32_t off = c * 8 < dt ? static_cast<uint32_t>(row * of * 2 + c * 16) : kOOB;
+      if ((row < cut) == (part == 0)) dma16(r, __builtin_amdgcn_readfirstlane(tile + first * (D * 2)), off);  // (a lane that is off writes nothing)
     }
   }
-};
+}
 
 __device__ __forceinline__ float max32(const f32x16 (&s)[2]) {
   float v[32];
@@ -122,7 +125,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_span_tile(SpanArgs a, int mo
   const bool front_only = mode == kFront;
   const auto token = [&](int row) { return static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(group)); };
   const Spans s = make_spans<2>(a, mode, set, front_only ? 0 : token(r0), front_only ? 0 : token(r1 - 1));
-  const int64_t kld = s.kld[front_only ? 0 : 1], vld = s.vld[front_only ? 0 : 1];  // (equal where there are both)
 
   const int qw = r0 + wave * 32;
   const bool active = qw < nrows;
@@ -154,24 +156,30 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_span_tile(SpanArgs a, int mo
   const int i0 = min(slice * share, nt);
   const int nkv = min(i0 + share, nt) - i0;  // tiles of this item
 
-  SpanDma<D, false> kd;
-  SpanDma<D, true> vd;
-  kd.init(kld, wave, lane, a.D);
-  vd.init(vld, wave, lane, a.D);
+  SpanDma<D, false> kd[2];  // of the front, of the main span
+  SpanDma<D, true> vd[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    kd[i].init(s.kld[i], wave, lane, a.D);
+    vd[i].init(s.vld[i], wave, lane, a.D);
+  }
   const uint32_t smem_addr = lds_addr(smem);
   // tile g of the item into its stage
   const auto dma = [&](int g) __attribute__((always_inline)) {
     const uint32_t st = smem_addr + static_cast<uint32_t>((g & 1) * kStage);
     const int k0 = (i0 + g) * kKeys;
-    if (k0 < nf && k0 + kKeys > nf && s.n[1] > 0) {  // the front's last keys and the first main ones
-      const int64_t back = nf - k0;
-      kd.issue_two(s.k[0] + k0 * kld * 2, s.k[1] - back * kld * 2, kld, nf - k0, keys - k0, a.D, st, lane);
-      vd.issue_two(s.v[0] + k0 * vld * 2, s.v[1] - back * vld * 2, vld, nf - k0, keys - k0, a.D, st + kTile, lane);
-      return;
+    if (k0 >= nf) {
+      const int row0 = k0 - nf;
+      kd[1].issue(s.k[1] + row0 * s.kld[1] * 2, s.kld[1], s.n[1] - row0, a.D, st);
+      vd[1].issue(s.v[1] + row0 * s.vld[1] * 2, s.vld[1], s.n[1] - row0, a.D, st + kTile);
+    } else if (k0 + kKeys <= nf || s.n[1] == 0) {
+      kd[0].issue(s.k[0] + k0 * s.kld[0] * 2, s.kld[0], nf - k0, a.D, st);
+      vd[0].issue(s.v[0] + k0 * s.vld[0] * 2, s.vld[0], nf - k0, a.D, st + kTile);
+    } else {  // the front's last keys and the first main ones
+      const int cut = nf - k0;
+      dma_two<D, false>(s.k[0] + k0 * s.kld[0] * 2, s.kld[0], s.k[1] - cut * s.kld[1] * 2, s.kld[1], cut, keys - k0, a.D, st, wave, lane);
+      dma_two<D, true>(s.v[0] + k0 * s.vld[0] * 2, s.vld[0], s.v[1] - cut * s.vld[1] * 2, s.vld[1], cut, keys - k0, a.D, st + kTile, wave, lane);
     }
-    const int span = k0 < nf ? 0 : 1, row0 = span == 0 ? k0 : k0 - nf;
-    kd.issue(s.k[span] + row0 * kld * 2, kld, s.n[span] - row0, a.D, st);
-    vd.issue(s.v[span] + row0 * vld * 2, vld, s.n[span] - row0, a.D, st + kTile);
   };
   if (nkv > 0) dma(0);
   // the queries settle here, with tile 0
