@@ -466,10 +466,10 @@ NTOPS_API int64_t ntops_kv_cache_attention_workspace(int dtype, int64_t B, int64
  * h / (Hq / Hkv).  lengths (B values, I32 or I64 by lengths_dtype; NULL: C tokens
  * each) are read on the device and cut to 0 .. C; keys that no row sees are not
  * read.  A row that sees no key is 0, and what a row does not see does not reach
- * it, whatever it holds.  window >= 1, sinks >= 0.  fp32 statistics and sums; F16
- * and BF16 with D a multiple of 8 up to 128, unit strides along D and rows at
- * multiples of 16 bytes run on the matrix cores (probabilities rounded to the
- * type), other layouts, D <= 256 and F32 on a kernel of one wave per row.  The
+ * it, whatever it holds.  window >= 1, sinks >= 0, D <= 256.  fp32 statistics and sums.
+ * On the matrix cores: F16 and BF16 with D a multiple of 8 (probabilities rounded to
+ * the type), F32 with D a multiple of 4, with unit strides along D and rows at
+ * multiples of 16 bytes; other layouts on a kernel of one wave per row.  The
  * workspace (16-byte aligned; may be NULL) spreads the keys of few query rows over
  * the GPU. */
 NTOPS_API int ntops_sliding_window_attention(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t C, int64_t D,

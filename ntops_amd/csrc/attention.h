@@ -28,7 +28,7 @@ __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_ex
 // D / 8 chunks per row), conflict-free for the transposing fragment reads.
 template <int D>
 __device__ __forceinline__ int vslot(int r, int c) {
-  if constexpr (D == 128)
+  if constexpr (D >= 128)
     return mnslot(r, c);
   else
     return c ^ (((r >> 1) & 1) << 2);

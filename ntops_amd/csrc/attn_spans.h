@@ -259,7 +259,7 @@ __device__ __forceinline__ void span_write_row(const SpanArgs& a, const SpanPart
 // Any types, head dims and layouts: a wave per row and slice.
 int span_rows_run(int dtype, const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st);
 
-// 16-bit types, at most kFewRows rows of a sequence a cache head.  front_slices > 0:
+// 16-bit types, head dims up to 128, at most kFewRows rows of a sequence a cache head.  front_slices > 0:
 // with the rows of all sequences of a group over their prefix, in that many slices that
 // come before the others.
 constexpr int kFewRows = 32;
@@ -274,8 +274,8 @@ int span_few_run(int dtype, const SpanArgs& a, const FewPlan& p, const SpanPart&
 constexpr int kTileRows = 128;
 int span_tile_run(int dtype, const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st);
 
-// fp32, head dims up to 128 that are multiples of 4, rows at multiples of 16 bytes: any
-// number of rows, in blocks of kF32Rows.
+// fp32, head dims that are multiples of 4, rows at multiples of 16 bytes: any number of
+// rows, in blocks of kF32Rows.
 constexpr int kF32Rows = 128;
 int span_f32_run(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st);
 

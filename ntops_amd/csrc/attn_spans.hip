@@ -183,10 +183,10 @@ constexpr int64_t kFewFrontRows = 512;
 // The plan for this problem where layouts suit the matrix cores, from sizes alone.
 // `joined`: both spans in one pass (without a workspace, they cannot be parted).
 Plan make_plan(int dtype, const SpanArgs& a, bool joined = false) {
-  if (a.D > 128 || a.D % (dtype == NTOPS_F32 ? 4 : 8) != 0 || static_cast<int64_t>(a.C) + a.P == 0) return rows_plan(a);
+  if (a.D % (dtype == NTOPS_F32 ? 4 : 8) != 0 || static_cast<int64_t>(a.C) + a.P == 0) return rows_plan(a);
   if (dtype == NTOPS_F32) return f32_plan(a, joined);
   const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv, cus = cu_count_cached();
-  const bool few = span_rows(a, kMain) <= kFewRows;
+  const bool few = a.D <= 128 && span_rows(a, kMain) <= kFewRows;
   const int64_t again = static_cast<int64_t>(a.B - a.G) * a.Hkv * a.P * a.D * 4;
   const int64_t blocks = row_blocks(a, kMain, few ? kFewRows : kTileRows);
   if (!joined && a.P > 0 && a.B > a.G) {

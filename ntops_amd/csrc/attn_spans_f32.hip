@@ -10,8 +10,15 @@
 // as d = 16 t + 4 g + e (g = l >> 4, e the step of four), so a lane reads four floats per
 // four MFMAs.  K and V^T tiles are double-buffered in the LDS; a tile's loads go to
 // registers before the previous tile's products and are stored after them, one barrier a
-// tile.  Bound by the fp32 matrix rate, a sixteenth of the 16-bit one, and, with few
-// rows, by the loads.
+// tile.  Two blocks a CU (over 128 columns, whose tiles fill the LDS: one), 4 waves a SIMD.
+//
+// Bound by the fp32 matrix rate, a tenth of the 16-bit one here (154 against 1513
+// TFLOP/s), and, with few rows, by the loads.  Measured: (3, 12 / 4, 333 over up to 1501,
+// window 500 and 8 sinks) of 96 49 us, the matrix cores half busy -- 21 us of products,
+// those of masked keys in edge tiles among them -- and 9 of the 49 the merge of two
+// slices; blocks of 64 rows gained nothing.  Over 128 columns (1, 16 / 4, 500 behind 500) of
+// 256 123 us, by the kernel of one wave per row 1158; (16, 16 / 4, 1 over 4100) of 256 267
+// against 319.
 //
 // What a row does not see: as in attn_spans_tile.hip.
 #include <algorithm>
@@ -28,7 +35,7 @@ template <int DP>
 constexpr int kLdsBytes = 2 * (kKeys * (DP + 4) + DP * (kKeys + 4)) * 4;
 
 template <int DP, int NW>
-__global__ __launch_bounds__(64 * NW, 4) void k_span_f32(SpanArgs a, int mode, int nqb, int slices, uint32_t total, SpanPart part) {
+__global__ __launch_bounds__(64 * NW, DP > 128 ? 2 : 4) void k_span_f32(SpanArgs a, int mode, int nqb, int slices, uint32_t total, SpanPart part) {
   constexpr int QB = 16 * NW;
   constexpr int KP = DP + 4;     // floats per K row in the LDS
   constexpr int VP = kKeys + 4;  // floats per V^T row
@@ -244,7 +251,8 @@ int run_f32(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipSt
 int span_f32_run(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
   if (a.D <= 64) return run_f32<64>(a, mode, slices, part, st);
   if (a.D <= 96) return run_f32<96>(a, mode, slices, part, st);
-  return run_f32<128>(a, mode, slices, part, st);
+  if (a.D <= 128) return run_f32<128>(a, mode, slices, part, st);
+  return run_f32<256>(a, mode, slices, part, st);
 }
 
 }  // namespace ntops

@@ -6,8 +6,9 @@
 // window -- over the 64-key tiles of both spans, or a slice of them.  Wave w owns rows
 // 32 w .. + 31 with their queries in registers and skips the tiles that none of them
 // sees; tiles go global -> LDS by direct DMA into one of two stages while the other is
-// used, one barrier a tile.  Two blocks a CU (64 columns: three) that nothing
-// synchronizes: the maxima and exponentials of one run under the MFMAs of the other.
+// used, one barrier a tile.  Two blocks a CU (64 columns: three; over 128, whose stages
+// fill the LDS: one) that nothing synchronizes: the maxima and exponentials of one run
+// under the MFMAs of the other.
 // Eight waves of 32 rows that alternate the two kinds of phase between barriers (256
 // rows, four stages, one block a CU) took 2 % less for long rows of 128 columns -- (16,
 // 32 / 8, 500 over a shared 8192) bf16 1070 against 1088 us -- 28 % more of 64 columns,
@@ -18,6 +19,16 @@
 // is past it by more than 2^8.  Masked scores are -inf whatever their key holds; a
 // value that is not finite times P = 0 is NaN, so a row whose result is NaN under a sum
 // that is none is computed again by itself, from the keys that it sees.
+//
+// Bound by the vector instructions of the softmax beside the matrix cores (55 % busy over
+// long rows of 128 columns), at few tiles a block by its start and end, and of one row a
+// head over 128 columns by the loads.  Measured, bf16: (1, 32 / 8, 16384 tokens, window
+// 4096 and 4 sinks) of 128 930 us, 1.03 PFLOP/s; (16, 32 / 8, 500 over a shared 8192) of 128
+// 1029 us, 1.05 PFLOP/s; (7, 16, 2001, window 255) of 80 55 us; (1, 16 / 4, 1000 behind 1000)
+// of 192 42 us, of 256 50 us; (64, 32 / 8, 1 over 4100) of 256 381 us, 5.6 TB/s, by the
+// kernel of one wave per row 8.4 ms.
+#include <atomic>
+
 #include "attn_spans.h"
 
 namespace ntops {
@@ -93,7 +104,7 @@ __device__ __forceinline__ float max32(const f32x16 (&s)[2]) {
 
 // D: columns of a row in the LDS; DM: columns that are multiplied, at least the head dim.
 template <typename T, int D, int DM>
-__global__ __launch_bounds__(64 * kWaves, 2) void k_span_tile(SpanArgs a, int mode, int nqb, int slices, uint32_t total, SpanPart part) {
+__global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void k_span_tile(SpanArgs a, int mode, int nqb, int slices, uint32_t total, SpanPart part) {
   constexpr int KS = DM / 16;  // k-steps of S = Q K^T
   constexpr int DT = DM / 32;  // 32-column tiles of O
   constexpr int kTile = kKeys * D * 2;
@@ -362,11 +373,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_span_tile(SpanArgs a, int mo
 template <typename T, int D, int DM>
 int launch_tile(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
   constexpr int kLds = 2 * 2 * kKeys * D * 2;
-  static_assert(kLds <= 65536, "LDS");
+  auto kern = k_span_tile<T, D, DM>;
+  if constexpr (kLds > 65536) {
+    static std::atomic<uint64_t> done{0};
+    if (int e = reserve_lds(reinterpret_cast<const void*>(kern), kLds, done, "attention")) return e;
+  }
   const int64_t nqb = ceil_div(span_rows(a, mode), kRowsBlock);
   const int64_t total = span_sets(a, mode) * nqb * slices;
   note_kernel("%s tile d%d mode%d split%d", a.pk ? "shared_prefix" : "sliding_window", DM, mode, slices);
-  hipLaunchKernelGGL((k_span_tile<T, D, DM>), blocks_2d(total), dim3(64 * kWaves), kLds, st, a, mode, static_cast<int>(nqb), slices, static_cast<uint32_t>(total), part);
+  hipLaunchKernelGGL(kern, blocks_2d(total), dim3(64 * kWaves), kLds, st, a, mode, static_cast<int>(nqb), slices, static_cast<uint32_t>(total), part);
   return check_launch("attention");
 }
 
@@ -374,7 +389,9 @@ template <typename T>
 int run_tile(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
   if (a.D <= 64) return launch_tile<T, 64, 64>(a, mode, slices, part, st);
   if (a.D <= 96) return launch_tile<T, 128, 96>(a, mode, slices, part, st);
-  return launch_tile<T, 128, 128>(a, mode, slices, part, st);
+  if (a.D <= 128) return launch_tile<T, 128, 128>(a, mode, slices, part, st);
+  if (a.D <= 192) return launch_tile<T, 256, 192>(a, mode, slices, part, st);
+  return launch_tile<T, 256, 256>(a, mode, slices, part, st);
 }
 
 }  // namespace

@@ -38,7 +38,7 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // c ^ ((r >> 2) & 7) each conflict on every read (256 vs 414 B per clock).
 template <int BK>
 __device__ __forceinline__ int kslot(int r, int c) {
-  if constexpr (BK == 128)
+  if constexpr (BK >= 128)
     return c ^ (r & 15);
   else if constexpr (BK == 64)
     return c ^ ((r >> 1) & 7);

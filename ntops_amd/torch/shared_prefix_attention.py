@@ -16,8 +16,8 @@ head h // (query heads / heads).  A row that sees no key is 0; what a row does n
 see does not reach it, NaNs and infinities included.  scale defaults to
 1 / sqrt(head_dim).
 
-float16, bfloat16 or float32, head dims up to 256; 16-bit head dims that are
-multiples of 8 up to 128 run on the matrix cores."""
+float16, bfloat16 or float32, head dims up to 256; multiples of 8 (float32: of 4) run
+on the matrix cores."""
 
 import math
 

@@ -9,10 +9,12 @@ all; read on the device and cut to the capacity).  The last query row is the
 sequence's last token: row i is its token p = lengths[b] - tokens + i, and sees the
 keys j <= p with j > p - window or j < sinks.  Query head h reads head h // (query
 heads / heads).  A row that sees no key is 0; what a row does not see does not reach
-it, NaNs and infinities included.  scale defaults to 1 / sqrt(head_dim).
+it, NaNs and infinities included.  Prompts that are padded in front have rows before
+their first token, which are 0; for prompts padded at their end, lengths of `tokens`
+leave token i at row i.  scale defaults to 1 / sqrt(head_dim).
 
-float16, bfloat16 or float32, head dims up to 256; 16-bit head dims that are
-multiples of 8 up to 128 run on the matrix cores."""
+float16, bfloat16 or float32, head dims up to 256; multiples of 8 (float32: of 4) run
+on the matrix cores."""
 
 import math
 import operator
