@@ -30,6 +30,8 @@ template <int D>
 __device__ __forceinline__ int vslot(int r, int c) {
   if constexpr (D >= 128)
     return mnslot(r, c);
+  else if constexpr (D == 96)
+    return c;
   else
     return c ^ (((r >> 1) & 1) << 2);
 }

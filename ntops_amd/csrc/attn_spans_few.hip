@@ -42,6 +42,7 @@ constexpr int kTileKeys = 4096 / D;  // keys of a wave's tile
 // is past it by more than this (base 2): the largest probability is then at most 2^8,
 // in fp32 sums and in 16-bit products as good as 1, and O is rescaled on few tiles.
 constexpr float kSlack = 8.f;
+constexpr int kAhead = 4;  // fragments of V read ahead of the MFMAs that use them
 
 // The copy of a 16-byte chunk a lane with the non-temporal hint (mfma.h: dma16): each
 // byte is read once.
@@ -274,18 +275,27 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
       for (int u = 0; u < PG; ++u)
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) sc[u][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+      // the fragments of k-step ks + 1 are read while the MFMAs of ks run
+      u32x4 q[2][PG], kf[2][KB];
+      const auto read = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        u32x4 q[PG];
-#pragma unroll
-        for (int u = 0; u < PG; ++u) q[u] = kShared ? query(rg0 + u, ks) : qf[kShared ? 0 : rg0 + u][ks];
+        for (int u = 0; u < PG; ++u) q[ks & 1][u] = kShared ? query(rg0 + u, ks) : qf[kShared ? 0 : rg0 + u][ks];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           const int row = kb * 16 + c16;
-          const u32x4 kf = *reinterpret_cast<const u32x4*>(sk + row * (D * 2) + kslot<D>(row, ks * 4 + g) * 16);
-#pragma unroll
-          for (int u = 0; u < PG; ++u) sc[u][kb] = mfma16<T>(kf, q[u], sc[u][kb]);
+          kf[ks & 1][kb] = *reinterpret_cast<const u32x4*>(sk + row * (D * 2) + kslot<D>(row, ks * 4 + g) * 16);
         }
+      };
+      read(0);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if (ks + 1 < KS) read(ks + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int u = 0; u < PG; ++u) sc[u][kb] = mfma16<T>(kf[ks & 1][kb], q[ks & 1][u], sc[u][kb]);
+        __builtin_amdgcn_sched_barrier(0);
       }
       if (rg0 + PG == RG) {
         wait_lgkmcnt0();
@@ -356,24 +366,32 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
     }
 
     wait_dma<24>();  // V of tile j is in
+    // V^T: lane row 16 t + (l & 15) at the keys of pf[p]; fragment i + kAhead is read
+    // while the MFMAs of i run
+    const auto read_v = [&](int i) __attribute__((always_inline)) {
+      const int col = (i % DT) * 16 + (c16 & 3) * 4;
+      s16x4 w[2];
 #pragma unroll
-    for (int p = 0; p < KB / 2; ++p)
-#pragma unroll
-      for (int t = 0; t < DT; ++t) {
-        // V^T: lane row 16 t + (l & 15) at the keys of pf[p]
-        const int col = t * 16 + (c16 & 3) * 4;
-        s16x4 w[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int row = p * 32 + u * 16 + g * 4 + (c16 >> 2);
-          w[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lds_s16x4_t*)(sv + row * (D * 2) + vslot<D>(row, col >> 3) * 16 + ((col >> 2) & 1) * 8));
-        }
-        const u32x2 lw = __builtin_bit_cast(u32x2, w[0]), hw = __builtin_bit_cast(u32x2, w[1]);
-        const u32x4 vf = {lw.x, lw.y, hw.x, hw.y};
-#pragma unroll
-        for (int rg = 0; rg < RG; ++rg) o[rg][t] = mfma16<T>(vf, pf[rg][p], o[rg][t]);
+      for (int u = 0; u < 2; ++u) {
+        const int row = (i / DT) * 32 + u * 16 + g * 4 + (c16 >> 2);
+        w[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s16x4_t*)(sv + row * (D * 2) + vslot<D>(row, col >> 3) * 16 + ((col >> 2) & 1) * 8));
       }
+      const u32x2 lw = __builtin_bit_cast(u32x2, w[0]), hw = __builtin_bit_cast(u32x2, w[1]);
+      return u32x4{lw.x, lw.y, hw.x, hw.y};
+    };
+    constexpr int nv = KB / 2 * DT;
+    u32x4 vf[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) vf[i] = read_v(i);
+#pragma unroll
+    for (int i = 0; i < nv; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int rg = 0; rg < RG; ++rg) o[rg][i % DT] = mfma16<T>(vf[i % kAhead], pf[rg][i / DT], o[rg][i % DT]);
+      if (i + kAhead < nv) vf[i % kAhead] = read_v(i + kAhead);
+    }
+    __builtin_amdgcn_sched_barrier(0);
     wait_lgkmcnt0();
     issue_v(j + 2);
   }

@@ -6,14 +6,15 @@
 // window -- over the 64-key tiles of both spans, or a slice of them.  Wave w owns rows
 // 32 w .. + 31 with their queries in registers and skips the tiles that none of them
 // sees; tiles go global -> LDS by direct DMA into one of two stages while the other is
-// used, one barrier a tile.  Two blocks a CU (64 columns: three; over 128, whose stages
-// fill the LDS: one) that nothing synchronizes: the maxima and exponentials of one run
-// under the MFMAs of the other.
+// used, one barrier a tile.  Two blocks a CU (up to 96 columns: three; over 128, whose
+// stages fill the LDS: one) that nothing synchronizes: the maxima and exponentials of one
+// run under the MFMAs of the other.  (Rows of 96 columns in the LDS of 128, two blocks: 57
+// against 49 us for narrow windows, 840 against 777 for long rows.)
 // Eight waves of 32 rows that alternate the two kinds of phase between barriers (256
 // rows, four stages, one block a CU) took 2 % less for long rows of 128 columns -- (16,
 // 32 / 8, 500 over a shared 8192) bf16 1070 against 1088 us -- 28 % more of 64 columns,
 // (1, 32 / 8, 16384, window 4096) 748 against 583, and half as long again for narrow
-// windows, (7, 16, 2001, window 255) of 80 columns 100 against 65.
+// windows, (7, 16, 2001, window 255) of 80 columns 100 against 57.
 //
 // A row's reference (from which its exponents are taken) follows its maximum when that
 // is past it by more than 2^8.  Masked scores are -inf whatever their key holds; a
@@ -24,7 +25,7 @@
 // long rows of 128 columns), at few tiles a block by its start and end, and of one row a
 // head over 128 columns by the loads.  Measured, bf16: (1, 32 / 8, 16384 tokens, window
 // 4096 and 4 sinks) of 128 930 us, 1.03 PFLOP/s; (16, 32 / 8, 500 over a shared 8192) of 128
-// 1029 us, 1.05 PFLOP/s; (7, 16, 2001, window 255) of 80 55 us; (1, 16 / 4, 1000 behind 1000)
+// 1029 us, 1.05 PFLOP/s; (7, 16, 2001, window 255) of 80 49 us; (1, 16 / 4, 1000 behind 1000)
 // of 192 42 us, of 256 50 us; (64, 32 / 8, 1 over 4100) of 256 381 us, 5.6 TB/s, by the
 // kernel of one wave per row 8.4 ms.
 #include <atomic>
@@ -44,19 +45,17 @@ constexpr float kSlack = 8.f;
 // DMA of one tile of 64 keys of D: 1 KiB an instruction, spread evenly over the waves.
 template <int D, bool IS_V>
 struct SpanDma {
-  static constexpr int kRowsPerInst = 1024 / (D * 2);
-  static constexpr int kInst = kKeys / kRowsPerInst / kWaves;
-  static_assert(kInst >= 1 && kInst * kWaves * kRowsPerInst == kKeys, "tile must split evenly over the waves");
+  static constexpr int kChunks = D / 8;  // of a row
+  static constexpr int kInst = kKeys * kChunks / 64 / kWaves;
+  static_assert(kInst * kWaves * 64 == kKeys * kChunks, "tile must split evenly over the waves");
   uint32_t voff[kInst];
   int lds_off;
 
   __device__ __forceinline__ void init(int64_t ld, int wave, int lane, int dt) {
     lds_off = wave * kInst * 1024;
-    constexpr int cpr = D / 8;
 #pragma unroll
     for (int i = 0; i < kInst; ++i) {
-      const int row = (wave * kInst + i) * kRowsPerInst + lane / cpr;
-      const int slot = lane % cpr;
+      const int id = (wave * kInst + i) * 64 + lane, row = id / kChunks, slot = id % kChunks;
       const int c = IS_V ? vslot<D>(row, slot) : kslot<D>(row, slot);
       voff[i] = c * 8 < dt ? static_cast<uint32_t>(row * ld * 2 + c * 16) : kOOB;
     }
@@ -74,17 +73,17 @@ struct SpanDma {
 template <int D, bool IS_V>
 __device__ __forceinline__ void dma_two(const char* front, int64_t front_ld, const char* base, int64_t ld, int cut, int n, int dt, uint32_t tile,
                                         int wave, int lane) {
-  constexpr int kInst = SpanDma<D, IS_V>::kInst, kRowsPerInst = SpanDma<D, IS_V>::kRowsPerInst, cpr = D / 8;
+  constexpr int kInst = SpanDma<D, IS_V>::kInst, kChunks = SpanDma<D, IS_V>::kChunks;
 #pragma unroll 1
   for (int i = 0; i < kInst; ++i) {
-    const int first = (wave * kInst + i) * kRowsPerInst, row = first + lane / cpr;
-    const int c = IS_V ? vslot<D>(row, lane % cpr) : kslot<D>(row, lane % cpr);
+    const int inst = wave * kInst + i, row = (inst * 64 + lane) / kChunks, slot = (inst * 64 + lane) % kChunks;
+    const int c = IS_V ? vslot<D>(row, slot) : kslot<D>(row, slot);
 #pragma unroll 1
     for (int part = 0; part < 2; ++part) {
       const int64_t of = part ? ld : front_ld;
       const u32x4 r = make_rsrc(part ? base : front, ((part ? n : cut) - 1) * of * 2 + dt * 2);
       const uint32_t off = c * 8 < dt ? static_cast<uint32_t>(row * of * 2 + c * 16) : kOOB;
-      if ((row < cut) == (part == 0)) dma16(r, __builtin_amdgcn_readfirstlane(tile + first * (D * 2)), off);  // (a lane that is off writes nothing)
+      if ((row < cut) == (part == 0)) dma16(r, __builtin_amdgcn_readfirstlane(tile + inst * 1024), off);  // (a lane that is off writes nothing)
     }
   }
 }
@@ -104,7 +103,7 @@ __device__ __forceinline__ float max32(const f32x16 (&s)[2]) {
 
 // D: columns of a row in the LDS; DM: columns that are multiplied, at least the head dim.
 template <typename T, int D, int DM>
-__global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : 2) void k_span_tile(SpanArgs a, int mode, int nqb, int slices, uint32_t total, SpanPart part) {
+__global__ __launch_bounds__(64 * kWaves, D > 128 ? 1 : D > 96 ? 2 : 3) void k_span_tile(SpanArgs a, int mode, int nqb, int slices, uint32_t total, SpanPart part) {
   constexpr int KS = DM / 16;  // k-steps of S = Q K^T
   constexpr int DT = DM / 32;  // 32-column tiles of O
   constexpr int kTile = kKeys * D * 2;
@@ -388,7 +387,7 @@ int launch_tile(const SpanArgs& a, int mode, int slices, const SpanPart& part, h
 template <typename T>
 int run_tile(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
   if (a.D <= 64) return launch_tile<T, 64, 64>(a, mode, slices, part, st);
-  if (a.D <= 96) return launch_tile<T, 128, 96>(a, mode, slices, part, st);
+  if (a.D <= 96) return launch_tile<T, 96, 96>(a, mode, slices, part, st);
   if (a.D <= 128) return launch_tile<T, 128, 128>(a, mode, slices, part, st);
   if (a.D <= 192) return launch_tile<T, 256, 192>(a, mode, slices, part, st);
   return launch_tile<T, 256, 256>(a, mode, slices, part, st);

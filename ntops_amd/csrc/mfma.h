@@ -40,6 +40,8 @@ template <int BK>
 __device__ __forceinline__ int kslot(int r, int c) {
   if constexpr (BK >= 128)
     return c ^ (r & 15);
+  else if constexpr (BK == 96)
+    return c ^ ((r >> 2) & 3);
   else if constexpr (BK == 64)
     return c ^ ((r >> 1) & 7);
   else

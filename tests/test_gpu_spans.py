@@ -86,6 +86,7 @@ WINDOWS = [
     (2, 4, 4, 40, 100, 128, 16, 0), (8, 3, 3, 65, 65, 64, 20, 5), (2, 8, 2, 130, 400, 128, 128, 4), (1, 4, 2, 300, 300, 72, 1, 0),
     (2, 5, 5, 333, 500, 120, 64, 100), (1, 2, 1, 700, 700, 64, 255, 1), (1, 12, 3, 270, 900, 128, 1000, 10), (8, 2, 2, 17, 40, 16, 12, 3),
     (2, 2, 1, 9, 60, 200, 20, 2), (2, 3, 1, 4, 50, 37, 9, 1), (1, 2, 2, 3, 20, 256, 6, 0), (1, 1, 1, 600, 600, 128, 100, 0), (2, 4, 2, 150, 400, 256, 100, 5), (2, 2, 1, 300, 500, 160, 130, 70),
+    (2, 4, 2, 150, 400, 96, 100, 5), (3, 2, 2, 333, 600, 88, 130, 70), (1, 3, 1, 700, 700, 80, 255, 1),
 ]
 
 
