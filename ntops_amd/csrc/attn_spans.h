@@ -259,9 +259,9 @@ __device__ __forceinline__ void span_write_row(const SpanArgs& a, const SpanPart
 // Any types, head dims and layouts: a wave per row and slice.
 int span_rows_run(int dtype, const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st);
 
-// 16-bit types, head dims up to 128, at most kFewRows rows of a sequence a cache head.  front_slices > 0:
-// with the rows of all sequences of a group over their prefix, in that many slices that
-// come before the others.
+// 16-bit types, head dims up to 128, at most kFewRows rows of a sequence a cache head.
+// front_slices > 0: with the rows of all sequences of a group (span_few_run: at most 16)
+// over their prefix, in that many slices that come before the others.
 constexpr int kFewRows = 32;
 struct FewPlan {
   int waves;  // a block, 1 or 2
@@ -269,8 +269,10 @@ struct FewPlan {
   int front_slices, slices;
 };
 int span_few_run(int dtype, const SpanArgs& a, const FewPlan& p, const SpanPart& part, hipStream_t st);
+int span_mixed_run(int dtype, const SpanArgs& a, const FewPlan& p, const SpanPart& part, hipStream_t st);
 
-// The same for any number of rows, in blocks of kTileRows.
+// 16-bit types, head dims that are multiples of 8: any number of rows, in blocks of
+// kTileRows.
 constexpr int kTileRows = 128;
 int span_tile_run(int dtype, const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st);
 

@@ -115,7 +115,7 @@ int64_t main_keys(const SpanArgs& a) { return std::min<int64_t>(a.C, static_cast
 // keys in `slices`; without, each sequence's rows go over both spans.
 enum Path { kRows, kFew, kTile, kF32 };
 struct Plan {
-  Path front, main;  // front: kFew (in one launch with a main of kFew) or kTile
+  Path front, main;  // (in one launch where the main one is kFew)
   int front_slices, slices;
   int waves;  // of a block of kFew
 };
@@ -169,16 +169,18 @@ int tile_slices(const SpanArgs& a, int64_t items, int64_t keys, int most) {
   return static_cast<int>(std::max<int64_t>(1, std::min({static_cast<int64_t>(most), n, ceil_div(keys, 128)})));
 }
 
+// Rows of a group up to which kFew takes the prefix, from more on kTile, both in one
+// launch with the sequences' own keys: 4 over 32768 with 4 heads (16 rows) 38 / 41 us, 8 over
+// 8192 (32 rows) 26.8 / 21.9, 16 over 8192 34.0 / 23.0, 64 over 8192 52.6 / 49.7.
+constexpr int64_t kFewFrontRows = 16;
 // Prefix keys and values that sequences may read again through the caches before the
 // prefix is better attended by itself, and the two results joined.  bf16, 32 / 8 heads of
 // 128, one token over a prefix and up to 512 of its own, each sequence over both / apart:
-// 4 over 8192 (100 MB again) 23.3 / 26.5 us, 8 over 8192 (235 MB) 33.9 / 29.7, 16 over 2048
-// (126 MB) 24.1 / 25.5, 64 over 512 (132 MB) 28.9 / 29.2, 2 over 32768 (134 MB) 35.8 / 44.6, 4 over
-// 32768 (403 MB) 56.9 / 46.0, 64 over 2048 (528 MB) 50.5 / 36.5.
-constexpr int64_t kReadAgain = 140 << 20;
-// Rows of a group up to which kFew takes the prefix, in the launch of the sequences' own
-// keys: 256 / 1024 rows over 2048 36.5 / 89.7 us, by kTile 44.3 / 93.2.
-constexpr int64_t kFewFrontRows = 512;
+// by kFew 2 over 32768 (134 MB again) 33 / 41 us, 4 over 32768 (403 MB) 54 / 38; by kTile 4 over
+// 8192 (101 MB) 21.0 / 21.6, 16 over 1024 (63 MB) 16.6 / 19.2, 16 over 2048 (126 MB) 22.0 /
+// 19.8, 64 over 512 (132 MB) 28.8 / 26.3, 8 over 8192 (235 MB) 32.6 / 21.9, 64 over 2048 (528
+// MB) 50.8 / 31.5.
+int64_t read_again(bool few_front) { return (few_front ? int64_t{140} : int64_t{110}) << 20; }
 
 // The plan for this problem where layouts suit the matrix cores, from sizes alone.
 // `joined`: both spans in one pass (without a workspace, they cannot be parted).
@@ -191,12 +193,18 @@ Plan make_plan(int dtype, const SpanArgs& a, bool joined = false) {
   const int64_t blocks = row_blocks(a, kMain, few ? kFewRows : kTileRows);
   if (!joined && a.P > 0 && a.B > a.G) {
     const int64_t front = row_blocks(a, kFront, kTileRows);
+    const bool few_front = few && span_rows(a, kFront) <= kFewFrontRows;
     // many rows: where the rows of a group fill blocks that those of a sequence leave empty
-    const bool apart = few ? again > kReadAgain : blocks * (a.P + a.C) > (front * a.P + blocks * a.C) * 7 / 4 && again > kReadAgain;
+    const bool apart = again > read_again(few_front) && (few || blocks * (a.P + a.C) > (front * a.P + blocks * a.C) * 7 / 4);
     if (apart) {
-      const bool few_front = few && span_rows(a, kFront) <= kFewFrontRows;
-      const int64_t keys = std::max<int64_t>(128, ceil_div(a.P * (few_front ? row_blocks(a, kFront, 64) : front), cus));
-      const int fs = static_cast<int>(std::min<int64_t>(kMaxSlices / 2, ceil_div(a.P, keys)));
+      // A front block a CU; beside blocks of few rows half as many, but of no more than
+      // 1024 keys, so that the others find room (64 sequences over 8192 of their group and
+      // up to 1024 of their own, 4 / 8 / 12 / 16 slices: 58 / 50 / 55 / 58 us; 16 over 32768, 16 /
+      // 32: 56 / 46).
+      const bool mixed = few && !few_front;
+      const int64_t most = ceil_div(a.P, mixed ? 512 : 128), wide = std::max<int64_t>(1, (mixed ? cus / 2 : cus) / front);
+      const int64_t cut = std::max<int64_t>(mixed ? ceil_div(a.P, 1024) : 1, std::min(most, wide));
+      const int fs = static_cast<int>(std::min<int64_t>(kMaxSlices / 2, cut));
       // own keys: slices no longer than twice the prefix's
       const int64_t ms = std::min({static_cast<int64_t>(kMaxSlices / 2), ceil_div(a.C, 2 * ceil_div(a.P, fs)), 2 * cus / blocks});
       return {few_front ? kFew : kTile, few ? kFew : kTile, fs, static_cast<int>(std::max<int64_t>(1, ms)), 2};
@@ -270,7 +278,7 @@ int run(int dtype, SpanArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
   const int n = p.front_slices + p.slices;
   SpanPart part{n > 1 ? static_cast<float*>(ws) : nullptr, n, 0, (a.D + 3) / 4 * 4};
   const int mode = p.front_slices > 0 ? kMain : kBoth;
-  if (p.front_slices > 0 && p.front != kFew)
+  if (p.front_slices > 0 && p.main != kFew)
     if (int e = p.front == kF32 ? span_f32_run(a, kFront, p.front_slices, part, st) : span_tile_run(dtype, a, kFront, p.front_slices, part, st))
       return e;
   part.first = p.front_slices;
@@ -278,7 +286,7 @@ int run(int dtype, SpanArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
   if (p.main == kRows)
     e = span_rows_run(dtype, a, mode, p.slices, part, st);
   else if (p.main == kFew)
-    e = span_few_run(dtype, a, {p.waves, mode, p.front == kFew ? p.front_slices : 0, p.slices}, part, st);
+    e = (p.front == kFew ? span_few_run : span_mixed_run)(dtype, a, {p.waves, mode, p.front_slices, p.slices}, part, st);
   else if (p.main == kF32)
     e = span_f32_run(a, mode, p.slices, part, st);
   else
