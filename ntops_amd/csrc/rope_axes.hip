@@ -288,7 +288,7 @@ extern "C" int ntops_rope_axes_qk(int dtype, int64_t B, int64_t S, int64_t Hq, i
       (Hq > 0 && (!q || !q_out || !q_strides || !q_out_strides)) || (Hk > 0 && (!k || !k_out || !k_strides || !k_out_strides)))
     return set_error(NTOPS_ERR_INVALID, "%s: null pointer", what);
   constexpr int64_t kMost = int64_t(1) << 40;
-  if (B > kMost || S > kMost || Hq > kMost || Hk > kMost || B * S > kMost || (Hq + Hk) > kMost / (B * S))
+  if (B > kMost || S > kMost / B || Hq > kMost || Hk > kMost || (Hq + Hk) > kMost / (B * S))
     return set_error(NTOPS_ERR_UNSUPPORTED, "%s: problem too large", what);
   a.B = B;
   a.S = S;

@@ -133,6 +133,14 @@ def test_c_entries_refuse():
     assert rot(s=0) == 0
 
 
+def test_rotary_sizes_whose_product_passes_64_bits():
+    lib, p, st = _lib.load(), ctypes.c_void_p(256), _lib.i64_array((8, 8, 8, 1))
+    for b, s in ((1 << 40, 1 << 24), (1 << 24, 1 << 40), (1 << 32, 1 << 32), (1 << 40, 1 << 40), (1 << 20, (1 << 20) + 1)):
+        rc = lib.ntops_rope_axes_qk(
+            _lib.BF16, b, s, 4, 2, 8, p, st, p, st, _lib.F32, p, 4, p, 4, 9, 4, 3, p, _lib.I64, st, 3, _lib.i64_array((1, 1, 2)), 0, p, st, p, st, None)
+        assert rc == 2 and "too large" in _err()
+
+
 def test_workspaces_of_refused_calls_are_empty():
     lib = _lib.load()
     for b, hq, hkv, sq, c, d, w, s in ((0, 4, 2, 1, 9, 8, 5, 0), (2, 3, 2, 1, 9, 8, 5, 0), (2, 4, 2, 1, 9, 300, 5, 0), (2, 4, 2, 1, 9, 8, 0, 0), (1 << 40, 4, 2, 1, 9, 8, 5, 0), (2, 4, 0, 1, 9, 8, 5, 0)):
