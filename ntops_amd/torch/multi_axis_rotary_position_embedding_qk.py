@@ -24,6 +24,17 @@ from ntops_amd import _lib
 from ntops_amd.torch.utils import _DeviceGuard, _contiguous, _strides, _to_dtype
 
 
+def _share_heads(q, k):
+    """Whether q and k are the same memory, or slices of one tensor along its heads that overlap."""
+    if not q.numel() or not k.numel():
+        return False
+    apart = k.data_ptr() - q.data_ptr()
+    step = q.stride(2) * q.element_size()
+    if apart == 0 or q.stride() != k.stride() or step == 0 or apart % step:
+        return apart == 0
+    return -k.shape[2] < apart // step < q.shape[2]
+
+
 def multi_axis_rotary_position_embedding_qk(q, k, sin_table, cos_table, positions, sections, interleaved=True, inplace=False):
     if _lib.fast is not None and not inplace:
         r = _lib.fast.rope_axes_qk(q, k, sin_table, cos_table, positions, sections, interleaved)
@@ -50,8 +61,8 @@ def multi_axis_rotary_position_embedding_qk(q, k, sin_table, cos_table, position
     for x in (q, k):
         if inplace and any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape)):
             raise RuntimeError(f"{what}: elements that share memory (a stride is 0) cannot be rotated in place")
-    if inplace and q.numel() and k.numel() and q.data_ptr() == k.data_ptr():
-        raise RuntimeError(f"{what}: q and k are one tensor, which would be rotated twice in place")
+    if inplace and _share_heads(q, k):
+        raise RuntimeError(f"{what}: q and k share heads, which would be rotated twice in place")
     dev = _lib.require_cuda(q, k, sin_table, cos_table, positions)
     lib = _lib.load()
     with _DeviceGuard(dev):

@@ -93,6 +93,19 @@ def test_rotary_refusals():
         rope(sections=(1.5, 2.5))
 
 
+def test_rotary_in_place_refuses_heads_of_both():
+    rest = (zeros(9, 4), zeros(9, 4), zeros(3, 2, 5, dtype=torch.int64), (1, 1, 2))
+    both = zeros(2, 5, 7, 8)
+    for q, k in ((both[:, :, :5], both[:, :, 4:]), (both[:, :, 3:], both[:, :, :4]), (both, both[:, :, 2:3]), (both[:, :, :2], both[:, :, :1])):
+        with pytest.raises(RuntimeError, match="twice"):
+            nt.multi_axis_rotary_position_embedding_qk(q, k, *rest, inplace=True)
+        with pytest.raises(RuntimeError, match="GPU tensor"):
+            nt.multi_axis_rotary_position_embedding_qk(q, k, *rest)
+    for q, k in ((both[:, :, :5], both[:, :, 5:]), (both[:, :, 4:], both[:, :, :4]), (both[:, :, :3], both.clone()[:, :, :3])):
+        with pytest.raises(RuntimeError, match="GPU tensor"):
+            nt.multi_axis_rotary_position_embedding_qk(q, k, *rest, inplace=True)
+
+
 def _err():
     return _lib.load().ntops_last_error().decode()
 
