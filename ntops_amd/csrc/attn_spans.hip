@@ -189,13 +189,15 @@ Plan make_plan(int dtype, const SpanArgs& a, bool joined = false) {
   if (dtype == NTOPS_F32) return f32_plan(a, joined);
   const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv, cus = cu_count_cached();
   const bool few = a.D <= 128 && span_rows(a, kMain) <= kFewRows;
-  const int64_t again = static_cast<int64_t>(a.B - a.G) * a.Hkv * a.P * a.D * 4;
+  const double again = static_cast<double>(a.B - a.G) * a.Hkv * a.P * a.D * 4;  // (no size overflows it)
   const int64_t blocks = row_blocks(a, kMain, few ? kFewRows : kTileRows);
   if (!joined && a.P > 0 && a.B > a.G) {
     const int64_t front = row_blocks(a, kFront, kTileRows);
     const bool few_front = few && span_rows(a, kFront) <= kFewFrontRows;
     // many rows: where the rows of a group fill blocks that those of a sequence leave empty
-    const bool apart = again > read_again(few_front) && (few || blocks * (a.P + a.C) > (front * a.P + blocks * a.C) * 7 / 4);
+    const auto walked = [](int64_t n, int64_t keys) { return static_cast<double>(n) * static_cast<double>(keys); };
+    const bool apart = again > read_again(few_front) &&
+                       (few || walked(blocks, static_cast<int64_t>(a.P) + a.C) > 1.75 * (walked(front, a.P) + walked(blocks, a.C)));
     if (apart) {
       // A front block a CU; beside blocks of few rows half as many, but of no more than
       // 1024 keys, so that the others find room (64 sequences over 8192 of their group and
@@ -223,6 +225,8 @@ int64_t plan_bytes(const SpanArgs& a, const Plan& p) {
   if (n <= 1) return 0;
   return static_cast<int64_t>(a.B) * a.Hq * a.Sq * n * ((a.D + 3) / 4 * 4 + 2) * 4;
 }
+// The workspace of a call whose layouts are not known yet.
+int64_t workspace_bytes(int dtype, const SpanArgs& a) { return std::max(plan_bytes(a, make_plan(dtype, a)), plan_bytes(a, rows_plan(a))); }
 
 // What the matrix cores' kernels read: unit strides along the head dim, rows at
 // multiples of 16 bytes that do not overlap, and for 16-bit types every offset within a
@@ -386,7 +390,7 @@ extern "C" int64_t ntops_sliding_window_attention_workspace(int dtype, int64_t B
   if (!span_sizes(a, B, Hq, Hkv, Sq, C, D, 0) || window < 1 || sinks < 0) return 0;
   a.window = clamp_count(window);
   a.sinks = clamp_count(sinks);
-  return plan_bytes(a, make_plan(dtype, a));
+  return workspace_bytes(dtype, a);
 }
 
 extern "C" int ntops_sliding_window_attention(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t C, int64_t D,
@@ -414,7 +418,7 @@ extern "C" int64_t ntops_shared_prefix_attention_workspace(int dtype, int64_t G,
   if (!span_sizes(a, B, Hq, Hkv, Sq, C, D, P) || G <= 0 || B % G != 0) return 0;
   a.G = static_cast<int>(G);
   a.pk = &a;  // (a prefix there is)
-  return plan_bytes(a, make_plan(dtype, a));
+  return workspace_bytes(dtype, a);
 }
 
 extern "C" int ntops_shared_prefix_attention(int dtype, int64_t G, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t P,

@@ -15,7 +15,7 @@
 // Bound by the fp32 matrix rate, a tenth of the 16-bit one here (154 against 1513
 // TFLOP/s), and, with few rows, by the loads.  Measured: (3, 12 / 4, 333 over up to 1501,
 // window 500 and 8 sinks) of 96 49 us, the matrix cores half busy -- 21 us of products,
-// those of masked keys in edge tiles among them -- and 9 of the 49 the merge of two
+// those of masked keys in edge tiles among them -- and 8 of the 49 the merge of five
 // slices; blocks of 64 rows gained nothing.  Over 128 columns (1, 16 / 4, 500 behind 500) of
 // 256 123 us, by the kernel of one wave per row 1158; (16, 16 / 4, 1 over 4100) of 256 267
 // against 319.
