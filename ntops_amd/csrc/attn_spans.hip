@@ -120,20 +120,24 @@ struct Plan {
   int waves;  // of a block of kFew
 };
 
+// Eight waves a CU, none of less than 32 keys: fp32 (1, 8, 1 over 200) of 128 11.6 us, of 128
+// keys at least 26.8, (1, 8, 1 over 1000) 16.7 / 23.9, (1, 8, 1 over 2048) 19.8 / 23.3.
 Plan rows_plan(const SpanArgs& a) {
   const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
-  const int64_t n = std::min({static_cast<int64_t>(kMaxSlices), cu_count_cached() * 8 / rows, (a.P + main_keys(a)) / 128});
+  const int64_t n = std::min({static_cast<int64_t>(kMaxSlices), cu_count_cached() * 8 / rows, (a.P + main_keys(a)) / 32});
   return {kRows, kRows, 0, static_cast<int>(std::max<int64_t>(1, n)), 0};
 }
 
 // Blocks of `rows` rows.
 int64_t row_blocks(const SpanArgs& a, int mode, int rows) { return span_sets(a, mode) * ceil_div(span_rows(a, mode), rows); }
 
-// fp32: blocks of kF32Rows rows, two a CU.
+// fp32: blocks of kF32Rows rows, two a CU, or single rows; slices of no less than two tiles
+// ((1, 32 / 8, 1 over 1024) of 128, one / two / four 17.4 / 18.6 / 24.4 us, (2, 12 / 4, 100 over 600)
+// of 96 27.2 / 24.0 / 29.2, (4, 12 / 4, 30 over 1200) of 64 26.3 / 24.0 / 22.2).
 Plan f32_plan(const SpanArgs& a, bool joined) {
   const int64_t blocks = 2 * cu_count_cached();
   const auto slices = [&](int64_t items, int64_t keys, int most) {
-    const int64_t n = std::min({static_cast<int64_t>(most), blocks / items, ceil_div(keys, 128)});
+    const int64_t n = std::min({static_cast<int64_t>(most), blocks / items, ceil_div(keys, 64)});
     return static_cast<int>(std::max<int64_t>(n, 1));
   };
   const int64_t main = row_blocks(a, kMain, kF32Rows);
@@ -142,17 +146,23 @@ Plan f32_plan(const SpanArgs& a, bool joined) {
     if (main * a.P > front * a.P + (front * a.P + main * a.C) / 4)
       return {kF32, kF32, slices(front, a.P, kMaxSlices / 2), slices(main, a.C, kMaxSlices / 2), 0};
   }
+  // (a row alone at its cache head needs no keys kept for others: (32, 8, 1 over 4096) of
+  // 128 by kF32 310 us, by kRows 202, 5.3 TB/s; four rows a head 311 / 342)
+  if (span_rows(a, kMain) == 1) return rows_plan(a);
   return {kF32, kF32, 0, slices(main, a.P + std::min<int64_t>(a.C, main_keys(a) + a.Sq), kMaxSlices), 0};
 }
 
 // Slices of kFew for `heads` sets of rows over `keys` keys: a block of two waves a CU,
-// none of less than four tiles a wave, below which the partial results and the merge
-// cost what the slices gain; blocks of one wave (two heads a CU or more) are not split.
-// bf16, 128 columns, 4100 keys, 1 / 2 / 4 / 8 / 16 / 32 slices: 8 heads of 8 rows - / - / - /
-// 17.0 / 16.0 / 16.3 us, 64 heads - / 33.4 / 29.7 / 33.9, 256 heads 91.2 / 98.6.
+// none of less than two tiles a wave, past sixteen slices of four, below which the partial
+// results and the merge cost what the slices gain; blocks of one wave (two heads a CU or
+// more) are not split.  bf16, 128 columns, 4100 keys, 1 / 2 / 4 / 8 / 16 / 32 slices: 8 heads of
+// 8 rows - / - / - / 17.0 / 16.0 / 16.3 us, 64 heads - / 33.4 / 29.7 / 33.9, 256 heads 91.2 / 98.6;
+// two / four tiles a wave: 8 heads over 1024 9.6 / 10.8, over 500 9.3 / 10.7, of 64 columns over
+// 1024 9.1 / 10.8, one head over 8192 21.6 / 18.6.
 int few_slices(const SpanArgs& a, int64_t heads, int64_t keys, int waves) {
   const int step = (a.D > 64 ? 32 : 64) * waves;
-  int64_t n = waves == 1 ? 1 : std::min({static_cast<int64_t>(kMaxSlices), cu_count_cached() / heads, ceil_div(keys, 4 * step)});
+  const int64_t most = std::max(std::min<int64_t>(16, ceil_div(keys, 2 * step)), ceil_div(keys, 4 * step));
+  int64_t n = waves == 1 ? 1 : std::min({static_cast<int64_t>(kMaxSlices), cu_count_cached() / heads, most});
   if (n <= 2 && keys <= 8 * step) n = 1;  // two short slices gain what the merge's launch costs
   return static_cast<int>(std::max<int64_t>(n, 1));
 }

@@ -245,7 +245,7 @@ KERNELS = [
     (1, 8, 2, 128, torch.bfloat16, "few", "few", "mixed"), (8, 8, 2, 64, torch.float16, "few", "few", "mixed"), (9, 8, 2, 128, torch.bfloat16, "tile", "tile", "tile"),
     (200, 8, 2, 96, torch.float16, "tile", "tile", "tile"), (3, 8, 2, 128, torch.float32, "f32", "f32", "f32"), (2, 8, 2, 100, torch.bfloat16, "rows", "rows", "rows"),
     (2, 8, 2, 98, torch.float32, "rows", "rows", "rows"), (4, 8, 2, 136, torch.float16, "tile", "tile", "tile"), (5, 8, 2, 256, torch.bfloat16, "tile", "tile", "tile"),
-    (5, 8, 2, 252, torch.float32, "f32", "f32", "f32"), (3, 8, 2, 250, torch.bfloat16, "rows", "rows", "rows"),
+    (1, 4, 4, 128, torch.float32, "rows", "rows", "f32"), (1, 8, 4, 128, torch.float32, "f32", "f32", "f32"), (5, 8, 2, 252, torch.float32, "f32", "f32", "f32"), (3, 8, 2, 250, torch.bfloat16, "rows", "rows", "rows"),
 ]
 
 
