@@ -168,14 +168,18 @@ int few_slices(const SpanArgs& a, int64_t heads, int64_t keys, int waves) {
 }
 
 // Slices of kTile for `items` blocks of rows over `keys` keys: a block a CU, two of 64
-// columns or where each still has 4000 keys (two run side by side, but the partial
-// results cost), none under two tiles.  4100 keys of 128 columns, 1 / 2 / 4 / 8 / 16 / 32
-// slices: 8 blocks of 64 rows 95 / 57 / 37 / 24.8 / 21.5 / 21.1 us, 64 blocks - / 56.6 / 39.5 /
-// 41.3, 256 blocks 110.6 / 113.3; 1100 keys, 256 blocks of 128 rows 36.1 / 46.7; 8700 keys 172 /
-// 148; 2100 keys of 64 columns, 128 blocks - / 30.1 / 26.2 / 32.5.
+// columns, of up to 128 where each still has 2048 keys (two run side by side, but the partial results
+// cost), or where `uneven` rows, those of a prompt from its start, leave CUs without work;
+// none under two tiles.  4100 keys of 128 columns, 1 / 2 / 4 / 8 / 16 / 32 slices: 8 blocks of
+// 64 rows 95 / 57 / 37 / 24.8 / 21.5 / 21.1 us, 64 blocks - / 56.6 / 39.5 / 41.3, 256 blocks 110.6
+// / 113.3; 1100 keys, 256 blocks of 128 rows 36.1 / 46.7; 8700 keys 172 / 148; 8192 keys, 128
+// blocks - / 92.9 / 83.7; uneven: 4096 keys, 256 blocks 82 / 67, 2048 keys, 128 blocks - / 37.5 /
+// 33.3; 2100 keys of 64 columns, 128 blocks - / 30.1 / 26.2 / 32.5.
 int tile_slices(const SpanArgs& a, int64_t items, int64_t keys, int most) {
   const int64_t cus = cu_count_cached();
-  const int64_t two = 2 * cus / items, n = a.D <= 64 || (two > 1 && keys / two >= 4000) ? two : cus / items;
+  const bool uneven = span_rows(a, kMain) > kTileRows && main_keys(a) > a.Sq / 2 && a.P + a.C <= 2 * static_cast<int64_t>(a.Sq);
+  const int64_t two = 2 * cus / items;
+  const int64_t n = a.D <= 64 || (a.D <= 128 && two > 1 && (uneven || keys / two >= 2048)) ? two : cus / items;
   return static_cast<int>(std::max<int64_t>(1, std::min({static_cast<int64_t>(most), n, ceil_div(keys, 128)})));
 }
 
@@ -222,7 +226,8 @@ Plan make_plan(int dtype, const SpanArgs& a, bool joined = false) {
       return {few_front ? kFew : kTile, few ? kFew : kTile, fs, static_cast<int>(std::max<int64_t>(1, ms)), 2};
     }
   }
-  const int64_t keys = a.P + std::min<int64_t>(a.C, main_keys(a) + (few ? 0 : a.Sq));
+  const int64_t tokens = few ? 0 : std::min<int64_t>(a.Sq, ceil_div(kTileRows, a.Hq / a.Hkv));  // of a block past its first
+  const int64_t keys = a.P + std::min<int64_t>(a.C, main_keys(a) + tokens);
   if (few) {
     const int waves = heads < 2 * cus ? 2 : 1;
     return {kFew, kFew, 0, few_slices(a, heads, keys, waves), waves};

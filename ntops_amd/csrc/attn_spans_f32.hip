@@ -18,7 +18,8 @@
 // those of masked keys in edge tiles among them -- and 8 of the 49 the merge of five
 // slices; blocks of 64 rows gained nothing.  Over 128 columns (1, 16 / 4, 500 behind 500) of
 // 256 123 us, by the kernel of one wave per row 1158; (16, 16 / 4, 1 over 4100) of 256 267
-// against 319.
+// against 319.  (1, 16 / 4, 4096 causal) of 128 738 us, 93 TFLOP/s -- 1220 with blocks of one
+// set after the other, which leave the longest two of a CU to end alone.
 //
 // What a row does not see: as in attn_spans_tile.hip.
 #include <algorithm>
@@ -30,6 +31,7 @@ namespace ntops {
 namespace {
 
 constexpr int kKeys = 32;
+constexpr uint32_t kCus = 256;
 
 template <int DP>
 constexpr int kLdsBytes = 2 * (kKeys * (DP + 4) + DP * (kKeys + 4)) * 4;
@@ -50,7 +52,10 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 2 : 4) void k_span_f32(SpanArgs
   const int64_t all = block_id();
   if (all >= total) return;  // the tail of a 2-D grid (the whole block)
   const uint32_t pid = static_cast<uint32_t>(all);
-  const uint32_t per = static_cast<uint32_t>(nqb * slices), set = pid / per, in = pid - set * per;
+  // Long rows of keys first; up to two blocks a CU, which all start at once, the CUs with
+  // the longest of the first half get the shortest of the second.
+  const uint32_t sets = total / static_cast<uint32_t>(nqb * slices);
+  const uint32_t order = total <= 2 * kCus && pid >= kCus ? total - 1 - (pid - kCus) : pid, in = order / sets, set = order - in * sets;
   const uint32_t back = in / static_cast<uint32_t>(slices);
   const int qb = nqb - 1 - static_cast<int>(back), slice = static_cast<int>(in - back * slices);
   const int group = a.group, ro = group * a.Sq;

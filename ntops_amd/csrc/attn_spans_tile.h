@@ -10,6 +10,10 @@
 // stages fill the LDS: one) that nothing synchronizes: the maxima and exponentials of one
 // run under the MFMAs of the other.  (Rows of 96 columns in the LDS of 128, two blocks: 57
 // against 49 us for narrow windows, 840 against 777 for long rows.)
+//
+// Blocks see few keys at a prompt's start and many at its end, so the order in which they
+// are handed out decides where two a CU start at once: (1, 16 / 4, 4096 causal) of 128 97 us,
+// set after set 119.
 // Eight waves of 32 rows that alternate the two kinds of phase between barriers (256
 // rows, four stages, one block a CU) took 2 % less for long rows of 128 columns -- (16,
 // 32 / 8, 500 over a shared 8192) bf16 1070 against 1088 us -- 28 % more of 64 columns,
@@ -39,6 +43,7 @@ constexpr int kWaves = 4;
 constexpr int kRowsBlock = 32 * kWaves;
 static_assert(kRowsBlock == kTileRows, "the plans count on it");
 constexpr int kKeys = 64;
+constexpr uint32_t kCus = 256;
 constexpr int kAhead = 4;  // fragments read ahead of the MFMA that uses them
 constexpr float kSlack = 8.f;
 
@@ -115,17 +120,19 @@ __device__ __forceinline__ void tile_block(const SpanArgs& a, int mode, int nqb,
   constexpr int kStage = 2 * kTile;                      // K tile, then V tile
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // An XCD (workgroups go round them) walks whole sets, every eighth one, the rows with
-  // the most keys first.
+  // Long rows of keys first.  An XCD (workgroups go round them) walks whole sets, every
+  // eighth one; up to two blocks a CU, which all start at once, the CUs with the longest
+  // of the first half get the shortest of the second.
   const uint32_t per = static_cast<uint32_t>(nqb * slices), sets = total / per;
   uint32_t set, in;
-  if ((sets & 7) == 0) {
+  if (total > 2 * kCus && (sets & 7) == 0) {
     const uint32_t at = pid >> 3, of = at / per;
     set = of * 8 + (pid & 7);
     in = at - of * per;
   } else {
-    set = pid / per;
-    in = pid - set * per;
+    const uint32_t at = total <= 2 * kCus && pid >= kCus ? total - 1 - (pid - kCus) : pid;
+    in = at / sets;
+    set = at - in * sets;
   }
   const uint32_t back = in / static_cast<uint32_t>(slices);
   const int qb = nqb - 1 - static_cast<int>(back), slice = static_cast<int>(in - back * slices);
