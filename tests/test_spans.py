@@ -189,3 +189,33 @@ def test_oracle_identities():
     assert np.allclose(one, three) and np.allclose((one**2).sum(-1), (x**2).sum(-1))
     bad = S.multi_axis_rotary_position_embedding(x, np.sin(angles), np.cos(angles), np.stack([row, row + 99]), (3, 1), False)
     assert np.isnan(bad).sum() == 2 * 5 * 3 * 2 and np.isnan(bad[..., [3, 7]]).all()
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (3, 0), (4, 2), (99, 0), (2, 99)])
+def test_oracle_against_torch(window, sinks):
+    """Both operators against torch's attention in 64 bits under a mask written key by key."""
+    rng = np.random.default_rng(window)
+    b, hq, h, sq, c, p, d = 3, 4, 2, 4, 9, 6, 8
+    q, k, v = rng.normal(size=(b, hq, sq, d)), rng.normal(size=(b, h, c, d)), rng.normal(size=(b, h, c, d))
+    pk, pv = rng.normal(size=(1, h, p, d)), rng.normal(size=(1, h, p, d))
+    lengths, plen = [9, 2, 5], [4]
+
+    def torch_attention(keys, vals, mask):
+        keys, vals = (torch.from_numpy(np.repeat(t, hq // h, 1)) for t in (keys, vals))
+        out = torch.nn.functional.scaled_dot_product_attention(torch.from_numpy(q), keys, vals, torch.from_numpy(mask[:, None]), scale=0.7)
+        return np.where(mask.any(-1)[:, None, :, None], out.numpy(), 0)
+
+    mask = np.zeros((b, sq, c), bool)
+    both = np.zeros((b, sq, p + c), bool)
+    for i in range(b):
+        for t in range(sq):
+            at = lengths[i] - sq + t
+            for j in range(c):
+                mask[i, t, j] = j <= at and (j > at - window or j < sinks)
+                both[i, t, p + j] = j <= at
+            both[i, t, : plen[0]] = True
+    got = S.sliding_window_attention(q, k, v, window, sinks, lengths, 0.7)[0]
+    assert np.allclose(got, torch_attention(k, v, mask), atol=1e-12)
+    got = S.shared_prefix_attention(q, pk, pv, k, v, plen, lengths, 0.7)[0]
+    want = torch_attention(np.concatenate([np.repeat(pk, b, 0), k], 2), np.concatenate([np.repeat(pv, b, 0), v], 2), both)
+    assert np.allclose(got, want, atol=1e-12)
