@@ -279,6 +279,7 @@ int span_tile_run(int dtype, const SpanArgs& a, int mode, int slices, const Span
 // fp32, head dims that are multiples of 4, rows at multiples of 16 bytes: any number of
 // rows, in blocks of kF32Rows.
 constexpr int kF32Rows = 128;
+constexpr int kF32FewRows = 16;  // head dims up to 128: a set with no more is one block's
 int span_f32_run(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st);
 
 }  // namespace ntops

@@ -131,9 +131,25 @@ Plan rows_plan(const SpanArgs& a) {
 // Blocks of `rows` rows.
 int64_t row_blocks(const SpanArgs& a, int mode, int rows) { return span_sets(a, mode) * ceil_div(span_rows(a, mode), rows); }
 
-// fp32: blocks of kF32Rows rows, two a CU, or single rows; slices of no less than two tiles
-// ((1, 32 / 8, 1 over 1024) of 128, one / two / four 17.4 / 18.6 / 24.4 us, (2, 12 / 4, 100 over 600)
-// of 96 27.2 / 24.0 / 29.2, (4, 12 / 4, 30 over 1200) of 64 26.3 / 24.0 / 22.2).
+// Slices of few rows for `heads` sets of them over `keys` keys, in tiles of `tile` keys a
+// wave: a block a CU, none of less than two tiles a wave, past sixteen slices of four,
+// below which the partial results and the merge cost what the slices gain.  bf16, 128
+// columns, 4100 keys, 1 / 2 / 4 / 8 / 16 / 32 slices: 8 heads of 8 rows - / - / - / 17.0 / 16.0 /
+// 16.3 us, 64 heads - / 33.4 / 29.7 / 33.9, 256 heads 91.2 / 98.6; two / four tiles a wave: 8
+// heads over 1024 9.6 / 10.8, over 500 9.3 / 10.7, of 64 columns over 1024 9.1 / 10.8, one head
+// over 8192 21.6 / 18.6.  fp32 (whose tiles are half as large) one / two tiles: 8 heads over
+// 1024 12.1 / 13.0, over 4096 22.6 / 18.2; 64 heads over 4096, 4 / 8 / 16 slices 47.8 / 50.1 / 52.2.
+int few_slices(int64_t heads, int64_t keys, int waves, int tile) {
+  const int64_t step = static_cast<int64_t>(tile) * waves;
+  const int64_t most = std::max(std::min<int64_t>(16, ceil_div(keys, 2 * step)), ceil_div(keys, 4 * step));
+  int64_t n = std::min({static_cast<int64_t>(kMaxSlices), cu_count_cached() / heads, most});
+  if (n <= 2 && keys <= 8 * step) n = 1;  // two short slices gain what the merge's launch costs
+  return static_cast<int>(std::max<int64_t>(n, 1));
+}
+
+// fp32: few rows as few_slices has them; blocks of kF32Rows rows, two a CU, in slices of no
+// less than two tiles (one / two / four: (1, 12 / 4, 30 over 200) of 96 13.3 / 16.6 / 23.6 us, (2, 12
+// / 4, 100 over 600) of 96 27.2 / 24.0 / 29.2, (4, 12 / 4, 30 over 1200) of 64 26.3 / 24.0 / 22.2).
 Plan f32_plan(const SpanArgs& a, bool joined) {
   const int64_t blocks = 2 * cu_count_cached();
   const auto slices = [&](int64_t items, int64_t keys, int most) {
@@ -141,36 +157,27 @@ Plan f32_plan(const SpanArgs& a, bool joined) {
     return static_cast<int>(std::max<int64_t>(n, 1));
   };
   const int64_t main = row_blocks(a, kMain, kF32Rows);
+  const bool few = a.D <= 128 && span_rows(a, kMain) <= kF32FewRows;
   if (!joined && a.P > 0 && a.B > a.G) {
     const int64_t front = row_blocks(a, kFront, kF32Rows);
-    if (main * a.P > front * a.P + (front * a.P + main * a.C) / 4)
+    // few rows: by the bytes read again, as in read_again below: (4, 32 / 8, 1 over 2048) of 128
+    // (50 MB) joined / apart 21.0 / 25.9 us, 16 over 1024 (126 MB) 31.7 / 35.3, 4 over 8192 (201
+    // MB) 44.7 / 35.0, 4 over 32768 137 / 62, 64 over 2048 144 / 82
+    const double again = static_cast<double>(a.B - a.G) * a.Hkv * a.P * a.D * 8;
+    if (few ? again > (128 << 20) : main * a.P > front * a.P + (front * a.P + main * a.C) / 4)
       return {kF32, kF32, slices(front, a.P, kMaxSlices / 2), slices(main, a.C, kMaxSlices / 2), 0};
   }
-  // (a row alone at its cache head needs no keys kept for others: (32, 8, 1 over 4096) of
-  // 128 by kF32 310 us, by kRows 202, 5.3 TB/s; four rows a head 311 / 342)
+  if (few) return {kF32, kF32, 0, few_slices(main, a.P + std::min<int64_t>(a.C, main_keys(a) + a.Sq), 4, 8), 0};
+  // (a row alone at its cache head needs no keys kept for others: (8, 8, 1 over 8192) of 256
+  // by kF32 267 us, by kRows 227)
   if (span_rows(a, kMain) == 1) return rows_plan(a);
   return {kF32, kF32, 0, slices(main, a.P + std::min<int64_t>(a.C, main_keys(a) + a.Sq), kMaxSlices), 0};
 }
 
-// Slices of kFew for `heads` sets of rows over `keys` keys: a block of two waves a CU,
-// none of less than two tiles a wave, past sixteen slices of four, below which the partial
-// results and the merge cost what the slices gain; blocks of one wave (two heads a CU or
-// more) are not split.  bf16, 128 columns, 4100 keys, 1 / 2 / 4 / 8 / 16 / 32 slices: 8 heads of
-// 8 rows - / - / - / 17.0 / 16.0 / 16.3 us, 64 heads - / 33.4 / 29.7 / 33.9, 256 heads 91.2 / 98.6;
-// two / four tiles a wave: 8 heads over 1024 9.6 / 10.8, over 500 9.3 / 10.7, of 64 columns over
-// 1024 9.1 / 10.8, one head over 8192 21.6 / 18.6.
-int few_slices(const SpanArgs& a, int64_t heads, int64_t keys, int waves) {
-  const int step = (a.D > 64 ? 32 : 64) * waves;
-  const int64_t most = std::max(std::min<int64_t>(16, ceil_div(keys, 2 * step)), ceil_div(keys, 4 * step));
-  int64_t n = waves == 1 ? 1 : std::min({static_cast<int64_t>(kMaxSlices), cu_count_cached() / heads, most});
-  if (n <= 2 && keys <= 8 * step) n = 1;  // two short slices gain what the merge's launch costs
-  return static_cast<int>(std::max<int64_t>(n, 1));
-}
-
 // Slices of kTile for `items` blocks of rows over `keys` keys: a block a CU, two of 64
-// columns, of up to 128 where each still has 2048 keys (two run side by side, but the partial results
-// cost), or where `uneven` rows, those of a prompt from its start, leave CUs without work;
-// none under two tiles.  4100 keys of 128 columns, 1 / 2 / 4 / 8 / 16 / 32 slices: 8 blocks of
+// columns, of up to 128 where each still has 2048 keys (two run side by side, but the
+// partial results cost), or where `uneven` rows, those of a prompt from its start, leave
+// CUs without work; none under two tiles.  4100 keys of 128 columns, 1 / 2 / 4 / 8 / 16 / 32 slices: 8 blocks of
 // 64 rows 95 / 57 / 37 / 24.8 / 21.5 / 21.1 us, 64 blocks - / 56.6 / 39.5 / 41.3, 256 blocks 110.6
 // / 113.3; 1100 keys, 256 blocks of 128 rows 36.1 / 46.7; 8700 keys 172 / 148; 8192 keys, 128
 // blocks - / 92.9 / 83.7; uneven: 4096 keys, 256 blocks 82 / 67, 2048 keys, 128 blocks - / 37.5 /
@@ -230,7 +237,8 @@ Plan make_plan(int dtype, const SpanArgs& a, bool joined = false) {
   const int64_t keys = a.P + std::min<int64_t>(a.C, main_keys(a) + tokens);
   if (few) {
     const int waves = heads < 2 * cus ? 2 : 1;
-    return {kFew, kFew, 0, few_slices(a, heads, keys, waves), waves};
+    // (blocks of one wave are not split)
+    return {kFew, kFew, 0, waves == 1 ? 1 : few_slices(heads, keys, waves, a.D > 64 ? 32 : 64), waves};
   }
   return {kTile, kTile, 0, tile_slices(a, blocks, keys, kMaxSlices), 0};
 }
@@ -316,7 +324,7 @@ int run(int dtype, SpanArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
 
 bool sizes_fit(int64_t B, int64_t Hq, int64_t Sq, int64_t C, int64_t P) {
   return B <= kMaxCount && Hq <= kMaxCount && Sq <= kMaxCount / 2 && C <= kMaxCount / 2 && P <= kMaxCount / 2 && B * Hq <= kMaxCount &&
-         B * Hq * Sq <= kMaxCount - 4096;
+         B * Hq * Sq <= kMaxCount - 4096 && C + P <= kMaxCount - 4096;
 }
 
 }  // namespace

@@ -1,5 +1,5 @@
 // fp32 windowed and shared-prefix attention on the matrix cores: IEEE fp32 products
-// (v_mfma_f32_16x16x4_f32) with fp32 sums.
+// (v_mfma_f32_16x16x4_f32) with fp32 sums.  Here for many rows; few ones further down.
 //
 // A block is 16 rows a wave of those that share a cache head, over the 32-key tiles of
 // both spans or a slice of them.  The scores are computed transposed, S^T = K Q^T: lane
@@ -32,6 +32,7 @@ namespace {
 
 constexpr int kKeys = 32;
 constexpr uint32_t kCus = 256;
+constexpr int kFewWaves = 4;
 
 template <int DP>
 constexpr int kLdsBytes = 2 * (kKeys * (DP + 4) + DP * (kKeys + 4)) * 4;
@@ -232,6 +233,216 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 2 : 4) void k_span_f32(SpanArgs
   }
 }
 
+// Up to 16 rows of a set, head dims up to DP: each wave streams tiles of 16 keys of its own,
+// global -> registers, one tile ahead, without the LDS: lane (g, r16) reads of K what the
+// first product takes, key r16's columns 16 t + 4 g .. + 3, and of V columns 64 w + 4 r16 ..
+// + 3 of the keys 4 g + e, the operand of O^T rows 4 r16 + c (an order of O's columns
+// that the result undoes).  The waves are joined through the LDS at the end.
+//
+// Bound by the loads: (32, 32 / 8, 1 over 4096) of 128 164 us, 6.5 TB/s, where blocks of 128
+// rows, of whose eight waves one has rows, took 311; (8, 32 / 8, 1 over 4096) 49 against 89,
+// (1, 32 / 8, 1 over 1024) 12.0 against 17.8, a row alone at its head (32, 8, 1 over 4096) 164,
+// by the kernel of one wave per row 199.
+template <int DP>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void k_span_f32_few(SpanArgs a, int mode, int slices, uint32_t total, SpanPart part) {
+  constexpr int NW = kFewWaves, KT = DP / 16, VW = DP / 64, LD = DP + 4;
+  __shared__ __attribute__((aligned(16))) float so[NW * 16 * LD];
+  __shared__ float sm[2 * NW * 16];
+  __shared__ uint32_t again;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, g = lane >> 4;
+  const int64_t all = block_id();
+  if (all >= total) return;  // the tail of a 2-D grid (the whole block)
+  const uint32_t pid = static_cast<uint32_t>(all);
+  const uint32_t set = pid / static_cast<uint32_t>(slices);
+  const int slice = static_cast<int>(pid - set * slices);
+  const bool front_only = mode == kFront;
+  const int rows = a.group * a.Sq * (front_only ? a.per : 1), t1 = front_only ? 0 : a.Sq - 1;
+  const Spans s = make_spans<4>(a, mode, set, 0, t1);
+  const bool in_rows = r16 < rows;
+  const SpanRow x = span_row(a, mode, s, min(r16, rows - 1));
+
+  f32x4 qf[KT];
+  {
+    const float* Q = static_cast<const float*>(a.q) + x.b * a.qst[0] + x.h * a.qst[1] + x.t * a.qst[2];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      const int d = 16 * t + 4 * g;
+      qf[t] = in_rows && d < a.D ? *reinterpret_cast<const f32x4*>(Q + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
+  // the front's keys and the main ones behind them, as one sequence
+  const int nf = s.n[0], keys = nf + s.n[1];
+  const int sinks = nf + max(0, s.sinks);
+  const int hi_all = nf + s.hi(0), lo_all = nf + s.lo(t1);
+  const int my_hi = nf + s.hi(x.t) - 4 * g, my_lo = nf + s.lo(x.t) - 4 * g;
+  const int nt = (keys + 15) / 16, share = (nt + slices - 1) / slices;
+  const int i0 = min(slice * share, nt), i1 = min(i0 + share, nt);
+
+  // (past the last key: that key again, and past the last column the first ones, whose
+  // scores are masked, whose queries are 0 and which are not stored)
+  const auto row_of = [&](int key, int which) __attribute__((always_inline)) {
+    const int k = min(key, keys - 1), sp = k < nf ? 0 : 1;
+    const int64_t row = sp ? k - nf : k;
+    return which ? reinterpret_cast<const float*>(s.v[sp]) + row * s.vld[sp] : reinterpret_cast<const float*>(s.k[sp]) + row * s.kld[sp];
+  };
+  struct Tile {
+    f32x4 k[KT], v[4][VW];
+  };
+  const auto load = [&](int i, Tile& t) __attribute__((always_inline)) {
+    const float* K = row_of(16 * i + r16, 0);
+#pragma unroll
+    for (int u = 0; u < KT; ++u) {
+      const int d = 16 * u + 4 * g;
+      t.k[u] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(K + (d < a.D ? d : 0)));
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float* V = row_of(16 * i + 4 * g + e, 1);
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        const int d = 64 * w + 4 * r16;
+        t.v[e][w] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(V + (d < a.D ? d : 0)));
+      }
+    }
+  };
+
+  f32x4 o[VW][4];
+#pragma unroll
+  for (int w = 0; w < VW; ++w)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[w][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = neg_inf(), l = 0.f;  // of row r16; this lane's part of its sum
+  const auto attend = [&](int i, Tile& t) __attribute__((always_inline)) {
+    if (a.D < DP) {
+#pragma unroll
+      for (int u = 0; u < KT; ++u)
+        if (16 * u + 4 * g >= a.D) t.k[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    f32x4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int u = 0; u < KT; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(t.k[u][e], qf[u][e], sc[e & 1], 0, 0, 0);
+    const int k0 = 16 * i;
+    const bool whole = k0 + 16 <= hi_all && (k0 >= lo_all || k0 + 16 <= sinks);
+    const int up = my_hi - k0, sink = sinks - 4 * g - k0;
+    const uint32_t hidden = static_cast<uint32_t>(max(0, my_lo - k0 - sink));  // [sinks, my_lo)
+    float p[4], mx = neg_inf();
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      p[r] = (sc[0][r] + sc[1][r]) * a.scale_log2;
+      if (!whole) p[r] = r < up && static_cast<uint32_t>(r - sink) >= hidden ? p[r] : neg_inf();
+      mx = fmaxf(mx, p[r]);
+    }
+    if (__any(mx > m)) {
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float m_new = fmaxf(m, mx);
+      const float alpha = m_new == neg_inf() ? 1.f : fast_exp2(m - m_new);
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int w = 0; w < VW; ++w)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[w][c] *= alpha;
+    }
+    const float m_use = m == neg_inf() ? 0.f : m;  // nothing seen so far: P = 0
+#pragma unroll
+    for (int r = 0; r < 4; ++r) p[r] = fast_exp2(p[r] - m_use);
+    l += (p[0] + p[1]) + (p[2] + p[3]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int w = 0; w < VW; ++w)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[w][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(t.v[e][w][c], p[e], o[w][c], 0, 0, 0);
+  };
+  Tile ta, tb;
+  int i = i0 + wave;
+  if (i < i1) load(i, ta);
+  for (; i < i1; i += 2 * NW) {
+    if (i + NW < i1) load(i + NW, tb);
+    attend(i, ta);
+    if (i + NW >= i1) break;
+    if (i + 2 * NW < i1) load(i + 2 * NW, ta);
+    attend(i + NW, tb);
+  }
+
+  // join the waves
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (threadIdx.x == 0) again = 0;
+  if (g == 0) {
+    sm[wave * 16 + r16] = m;
+    sm[(NW + wave) * 16 + r16] = l;
+  }
+#pragma unroll
+  for (int w = 0; w < VW; ++w)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<f32x4*>(so + (wave * 16 + r16) * LD + 64 * w + 16 * g + 4 * r) = f32x4{o[w][0][r], o[w][1][r], o[w][2][r], o[w][3][r]};
+  __syncthreads();
+  for (int it = threadIdx.x; it < 16 * (DP / 4); it += 64 * NW) {
+    const int row = it / (DP / 4), d = (it - row * (DP / 4)) * 4;
+    if (row >= rows || d >= a.D) continue;
+    float mm = sm[row];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) mm = fmaxf(mm, sm[w * 16 + row]);
+    float sum = 0.f;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float mw = sm[w * 16 + row];
+      // (a wave of which the row has seen nothing but NaN scores: its sum alone)
+      const float fw = mw == neg_inf() ? 0.f : fast_exp2(mw - mm);
+      sum += sm[(NW + w) * 16 + row] * fw;
+      const f32x4 ow = *reinterpret_cast<const f32x4*>(so + (w * 16 + row) * LD + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += mw == neg_inf() ? 0.f : ow[e] * fw;
+    }
+    const float any = (v[0] + v[1]) + (v[2] + v[3]);
+    if (!(any == any) && sum == sum) atomicOr(&again, 1u << row);
+    const SpanRow y = span_row(a, mode, s, row);
+    if (part.p) {
+      const int64_t at = part.at(a, y, slice);
+      if (d == 0) {
+        float* ml = part.ml(a, at);
+        ml[0] = mm;
+        ml[1] = sum;
+      }
+      *reinterpret_cast<f32x4*>(part.row(at) + d) = v;
+    } else {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (a NaN sum passes through)
+      *reinterpret_cast<f32x4*>(static_cast<float*>(a.o) + y.b * a.ost[0] + y.h * a.ost[1] + y.t * a.ost[2] + d) = v * inv;
+    }
+  }
+  __syncthreads();
+  uint32_t bad = __builtin_amdgcn_readfirstlane(again);
+  if (bad == 0) return;  // (the same for every wave)
+  wait_vmcnt<0>();       // what has been written of these rows is written before what follows
+  __syncthreads();
+  while (bad != 0) {
+    const int row = __builtin_ctz(bad);
+    bad &= bad - 1;
+    if (row % NW != wave) continue;
+    const SpanRow y = span_row(a, mode, s, row);
+    float ro_[KT], rm, rl;
+    span_attend_row<float, KT, 1>(a, s, y, min(16 * i0, nf), min(16 * i1, nf), max(0, 16 * i0 - nf), max(0, min(16 * i1, keys) - nf), ro_, rm, rl);
+    span_write_row<float, KT>(a, part, y, slice, ro_, rm, rl);
+  }
+}
+
+template <int DP>
+int launch_f32_few(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
+  const int64_t total = span_sets(a, mode) * slices;
+  note_kernel("%s f32 few d%d mode%d split%d", a.pk ? "shared_prefix" : "sliding_window", DP, mode, slices);
+  hipLaunchKernelGGL((k_span_f32_few<DP>), blocks_2d(total), dim3(64 * kFewWaves), 0, st, a, mode, slices, static_cast<uint32_t>(total), part);
+  return check_launch("attention");
+}
+
 template <int DP, int NW>
 int launch_f32(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
   auto kern = k_span_f32<DP, NW>;
@@ -254,6 +465,8 @@ int run_f32(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipSt
 }  // namespace
 
 int span_f32_run(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
+  if (a.D <= 128 && span_rows(a, mode) <= kF32FewRows)
+    return a.D <= 64 ? launch_f32_few<64>(a, mode, slices, part, st) : launch_f32_few<128>(a, mode, slices, part, st);
   if (a.D <= 64) return run_f32<64>(a, mode, slices, part, st);
   if (a.D <= 96) return run_f32<96>(a, mode, slices, part, st);
   if (a.D <= 128) return run_f32<128>(a, mode, slices, part, st);

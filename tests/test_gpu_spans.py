@@ -85,7 +85,7 @@ WINDOWS = [
     (4, 32, 8, 1, 1000, 128, 333, 70), (2, 32, 1, 1, 700, 80, 129, 33), (1, 6, 2, 5, 900, 64, 200, 3), (3, 8, 1, 8, 257, 128, 31, 4),
     (2, 4, 4, 40, 100, 128, 16, 0), (8, 3, 3, 65, 65, 64, 20, 5), (2, 8, 2, 130, 400, 128, 128, 4), (1, 4, 2, 300, 300, 72, 1, 0),
     (2, 5, 5, 333, 500, 120, 64, 100), (1, 2, 1, 700, 700, 64, 255, 1), (1, 12, 3, 270, 900, 128, 1000, 10), (8, 2, 2, 17, 40, 16, 12, 3),
-    (2, 2, 1, 9, 60, 200, 20, 2), (2, 3, 1, 4, 50, 37, 9, 1), (1, 2, 2, 3, 20, 256, 6, 0), (1, 1, 1, 600, 600, 128, 100, 0), (2, 4, 2, 150, 400, 256, 100, 5), (2, 2, 1, 300, 500, 160, 130, 70),
+    (2, 2, 1, 9, 60, 200, 20, 2), (2, 3, 1, 4, 50, 37, 9, 1), (1, 2, 2, 3, 20, 256, 6, 0), (1, 1, 1, 600, 600, 128, 100, 0), (3, 4, 2, 7, 333, 128, 50, 9), (2, 16, 1, 1, 700, 92, 300, 40), (2, 4, 2, 150, 400, 256, 100, 5), (2, 2, 1, 300, 500, 160, 130, 70),
     (2, 4, 2, 150, 400, 96, 100, 5), (3, 2, 2, 333, 600, 88, 130, 70), (1, 3, 1, 700, 700, 80, 255, 1),
 ]
 
@@ -245,7 +245,8 @@ KERNELS = [
     (1, 8, 2, 128, torch.bfloat16, "few", "few", "mixed"), (8, 8, 2, 64, torch.float16, "few", "few", "mixed"), (9, 8, 2, 128, torch.bfloat16, "tile", "tile", "tile"),
     (200, 8, 2, 96, torch.float16, "tile", "tile", "tile"), (3, 8, 2, 128, torch.float32, "f32", "f32", "f32"), (2, 8, 2, 100, torch.bfloat16, "rows", "rows", "rows"),
     (2, 8, 2, 98, torch.float32, "rows", "rows", "rows"), (4, 8, 2, 136, torch.float16, "tile", "tile", "tile"), (5, 8, 2, 256, torch.bfloat16, "tile", "tile", "tile"),
-    (1, 4, 4, 128, torch.float32, "rows", "rows", "f32"), (1, 8, 4, 128, torch.float32, "f32", "f32", "f32"), (5, 8, 2, 252, torch.float32, "f32", "f32", "f32"), (3, 8, 2, 250, torch.bfloat16, "rows", "rows", "rows"),
+    (1, 4, 4, 128, torch.float32, "f32 few", "f32 few", "f32 few"), (8, 8, 4, 92, torch.float32, "f32 few", "f32 few", "f32 few"),
+    (1, 4, 4, 160, torch.float32, "rows", "rows", "f32"), (9, 8, 4, 128, torch.float32, "f32 d128", "f32 d128", "f32 d128"), (5, 8, 2, 252, torch.float32, "f32", "f32", "f32"), (3, 8, 2, 250, torch.bfloat16, "rows", "rows", "rows"),
 ]
 
 
