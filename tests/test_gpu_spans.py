@@ -323,6 +323,38 @@ def test_captured_and_replayed(sq):
             assert torch.equal(x, y), step
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("g,b,hq,hkv,sq,p,c,d", APART)
+def test_captured_apart(g, b, hq, hkv, sq, p, c, d, dtype):
+    """Prefixes attended apart, in a graph replayed with new lengths; twice at once, on two
+    streams, beside it."""
+    q, k, v = window_inputs(b, hq, hkv, sq, c, d, dtype)
+    pk, pv = values(g, hkv, p, d, dtype=dtype), values(g, hkv, p, d, dtype=dtype)
+    n, pn = spread(b, c), spread(g, p)
+
+    def call():
+        return nt.shared_prefix_attention(q, pk, pv, k, v, pn, n)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        call()
+        with torch.cuda.graph(graph, stream=side):
+            out = call()
+    torch.cuda.current_stream().wait_stream(side)
+    for step in range(3):
+        n.copy_(torch.randint(0, c + 1, (b,), dtype=torch.int32))
+        pn.copy_(torch.randint(0, p + 1, (g,), dtype=torch.int32))
+        side.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        want = call()
+        with torch.cuda.stream(side):
+            beside = call()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(beside, want), step
+
+
 def test_on_another_stream():
     q, k, v = window_inputs(8, 8, 2, 3, 900, 128, torch.float16)
     want = nt.sliding_window_attention(q, k, v, 500, 2), nt.shared_prefix_attention(q, k[:2], v[:2], k, v)

@@ -125,7 +125,7 @@ def test_c_entries_refuse():
         (win(lengths=p, ldt=_lib.F32), 1, "lengths"), (win(b=1 << 40), 2, "too large"), (win(c=1 << 31), 2, "too large"),
         (win(b=1 << 16, hq=1 << 16), 2, "too large"), (win(ws=ctypes.c_void_p(8), nws=64), 1, "workspace"), (win(ws=p, nws=-1), 1, "workspace"),
         (pre(g=0), 1, "multiple"), (pre(g=3), 1, "multiple"), (pre(pl=-1), 1, "negative"), (pre(pk=None), 1, "null"), (pre(pl=1 << 31), 2, "too large"),
-        (pre(plen=p, pdt=_lib.BOOL), 1, "prefix lengths"),
+        (pre(plen=p, pdt=_lib.BOOL), 1, "prefix lengths"), (pre(pl=(1 << 30) - 1, c=(1 << 30) - 1), 2, "too large"),
     ]:
         assert rc == code, (rc, code, text)
     assert win(w=0) == 1 and "window" in _err()
