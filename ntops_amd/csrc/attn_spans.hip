@@ -169,7 +169,7 @@ Plan f32_plan(const SpanArgs& a, bool joined) {
   }
   if (few) return {kF32, kF32, 0, few_slices(main, a.P + std::min<int64_t>(a.C, main_keys(a) + a.Sq), 4, 8), 0};
   // (a row alone at its cache head needs no keys kept for others: (8, 8, 1 over 8192) of 256
-  // by kF32 267 us, by kRows 227)
+  // by kF32 381 us, by kRows 212; (64, 8, 1 over 1000) 381 / 201)
   if (span_rows(a, kMain) == 1) return rows_plan(a);
   return {kF32, kF32, 0, slices(main, a.P + std::min<int64_t>(a.C, main_keys(a) + a.Sq), kMaxSlices), 0};
 }

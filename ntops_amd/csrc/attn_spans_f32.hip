@@ -7,21 +7,24 @@
 // the B operand of O^T += V^T P^T for MFMA step r when the keys of that step are taken as
 // 4 (l >> 4) + r (a sum over keys does not depend on their order), so P never leaves the
 // registers, and every accumulator of a lane belongs to one row.  The head dim is walked
-// as d = 16 t + 4 g + e (g = l >> 4, e the step of four), so a lane reads four floats per
-// four MFMAs.  K and V^T tiles are double-buffered in the LDS; a tile's loads go to
-// registers before the previous tile's products and are stored after them, one barrier a
-// tile.  Two blocks a CU (over 128 columns, whose tiles fill the LDS: one), 4 waves a SIMD.
+// as d = 16 t + 4 g + e (g = l >> 4, e the step of four), so a lane reads four floats of K
+// per four MFMAs; of V, whose rows stay as they are, the four columns side by side that
+// four accumulators take, in an order in which the results lie side by side, too.  (With
+// V transposed on its way into the LDS, whose stores then collide, long rows took 8 to 15 %
+// more.)  Tiles are double-buffered; a tile's loads go to registers before the previous
+// tile's products and are stored after them, one barrier a tile.  Two blocks a CU (over 128
+// columns, whose tiles fill the LDS: one), 4 waves a SIMD.
 //
 // Bound by the fp32 matrix rate, a tenth of the 16-bit one here (154 against 1513
-// TFLOP/s), and, with few rows, by the loads.  Measured: (3, 12 / 4, 333 over up to 1501,
-// window 500 and 8 sinks) of 96 49 us, the matrix cores half busy -- 21 us of products,
-// those of masked keys in edge tiles among them -- and 8 of the 49 the merge of five
-// slices; blocks of 64 rows gained nothing.  Over 128 columns (1, 16 / 4, 500 behind 500) of
-// 256 123 us, by the kernel of one wave per row 1158; (16, 16 / 4, 1 over 4100) of 256 267
-// against 319.  (1, 16 / 4, 4096 causal) of 128 738 us, 93 TFLOP/s -- 1220 with blocks of one
-// set after the other, which leave the longest two of a CU to end alone.
+// TFLOP/s).  Measured: (1, 16 / 4, 4096 causal) of 128 638 us, 108 TFLOP/s -- nearly twice as
+// long with blocks of one set after the other, which leave the longest two of a CU to end
+// alone; (3, 12 / 4, 333 over up to 1501, window 500 and 8 sinks) of 96 47 us, the matrix
+// cores half busy: 21 us of products, those of masked keys in edge tiles among them, the
+// starts and ends of blocks of four tiles, and 8 us the merge of five slices; blocks of 64
+// rows gained nothing.  Over 128 columns (1, 16 / 4, 500 behind 500) of 256 102 us, by the
+// kernel of one wave per row 1151; (16, 16 / 4, 1 over 4100) of 256 216 against 319.
 //
-// What a row does not see: as in attn_spans_tile.hip.
+// What a row does not see: as in attn_spans_tile.h.
 #include <algorithm>
 #include <atomic>
 
@@ -35,14 +38,15 @@ constexpr uint32_t kCus = 256;
 constexpr int kFewWaves = 4;
 
 template <int DP>
-constexpr int kLdsBytes = 2 * (kKeys * (DP + 4) + DP * (kKeys + 4)) * 4;
+constexpr int kLdsBytes = 2 * kKeys * (DP + 4 + DP) * 4;
 
 template <int DP, int NW>
 __global__ __launch_bounds__(64 * NW, DP > 128 ? 2 : 4) void k_span_f32(SpanArgs a, int mode, int nqb, int slices, uint32_t total, SpanPart part) {
   constexpr int QB = 16 * NW;
   constexpr int KP = DP + 4;     // floats per K row in the LDS
-  constexpr int VP = kKeys + 4;  // floats per V^T row
-  constexpr int kKTile = kKeys * KP, kBuf = kKTile + DP * VP;
+  constexpr int VP = DP;         // per V row (those 4 apart, read side by side, start at the same bank)
+  constexpr int kKTile = kKeys * KP, kBuf = kKTile + kKeys * VP;
+  constexpr int NC = DP / 16;    // columns of V of a lane
   constexpr int kThreads = 64 * NW;
   constexpr int kF4 = kKeys * DP / 4;                   // 16-byte chunks per operand and tile
   constexpr int kLd = (kF4 + kThreads - 1) / kThreads;  // per thread
@@ -118,11 +122,13 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 2 : 4) void k_span_f32(SpanArgs
       if (f >= kF4) break;
       const int kl = f / (DP / 4), d = 4 * (f % (DP / 4));
       *reinterpret_cast<f32x4*>(kt + kl * KP + d) = kst[j];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) vt[(d + e) * VP + kl] = vst[j][e];
+      *reinterpret_cast<f32x4*>(vt + kl * VP + d) = vst[j];
     }
   };
 
+  // Columns of V that lane r16 multiplies, in fours of 64 and in twos of the last 32 of 96:
+  // what a lane gets of O then lies side by side in fours, and so do those of g = 0 .. 3.
+  const int at4 = (r16 >> 2) + 4 * (r16 & 3), at2 = 2 * (r16 >> 2) + (r16 & 1) + 8 * (r16 >> 1 & 1);
   f32x4 o[DP / 16];
 #pragma unroll
   for (int i = 0; i < DP / 16; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -142,13 +148,15 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 2 : 4) void k_span_f32(SpanArgs
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int tt = 0; tt < DP / 16; ++tt)
+      for (int tt = 0; tt < DP / 16; ++tt) {
+        f32x4 kf[2];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const f32x4 kf = *reinterpret_cast<const f32x4*>(kt + (kb * 16 + r16) * KP + 16 * tt + 4 * g);
+        for (int kb = 0; kb < 2; ++kb) kf[kb] = *reinterpret_cast<const f32x4*>(kt + (kb * 16 + r16) * KP + 16 * tt + 4 * g);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[tt][e], sc[kb], 0, 0, 0);
-        }
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) sc[kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[kb][e], qf[tt][e], sc[kb], 0, 0, 0);
+      }
       const bool whole = k0 + kKeys <= w_hi_all && (k0 >= w_lo_all || k0 + kKeys <= sinks);
       const int up = my_hi - k0, sink = sinks - 4 * g - k0;
       const uint32_t hidden = static_cast<uint32_t>(max(0, my_lo - k0 - sink));  // [sinks, my_lo)
@@ -182,12 +190,24 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 2 : 4) void k_span_f32(SpanArgs
 #pragma unroll
       for (int u = 0; u < DP / 16; ++u) o[u] *= alpha;
 #pragma unroll
-      for (int u = 0; u < DP / 16; ++u)
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const f32x4 vf = *reinterpret_cast<const f32x4*>(vt + (16 * u + r16) * VP + kb * 16 + 4 * g);
+        for (int e = 0; e < 4; ++e) {
+          const float* row = vt + (kb * 16 + 4 * g + e) * VP;
+          float v[NC];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[e], sc[kb][e], o[u], 0, 0, 0);
+          for (int u = 0; u + 4 <= NC; u += 4) {
+            const f32x4 y = *reinterpret_cast<const f32x4*>(row + 16 * u + 4 * at4);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[u + c] = y[c];
+          }
+          if constexpr (NC % 4 == 2) {
+            const f32x2 y = *reinterpret_cast<const f32x2*>(row + 64 + 2 * at2);
+            v[4] = y.x;
+            v[5] = y.y;
+          }
+#pragma unroll
+          for (int u = 0; u < NC; ++u) o[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[u], sc[kb][e], o[u], 0, 0, 0);
         }
     }
     if (t + 1 < nkv) store_tile((t + 1) & 1);  // read last in tile t - 1, before the barrier that ended it
@@ -197,14 +217,22 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 2 : 4) void k_span_f32(SpanArgs
   l += __shfl_xor(l, 32, 64);
   const bool none = m == neg_inf();
   const float inv = l == 0.f ? 0.f : 1.f / l;  // (a NaN sum passes through)
+  // runs of four columns: `first(i)` and the accumulators
+  const auto first = [&](int i) { return i < NC / 4 * 4 ? i / 4 * 64 + i % 4 * 16 + 4 * g : 64 + 16 * (i - 4) + 4 * g; };
+  const auto run = [&](int i) {
+    if (i < NC / 4 * 4) {
+      const int u = i / 4 * 4, r = i % 4;
+      return f32x4{o[u][r], o[u + 1][r], o[u + 2][r], o[u + 3][r]};
+    }
+    const int r = 2 * (i - 4);
+    return f32x4{o[NC - 2][r], o[NC - 1][r], o[NC - 2][r + 1], o[NC - 1][r + 1]};
+  };
   float any = 0.f;
 #pragma unroll
-  for (int u = 0; u < DP / 16; ++u)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      o[u][e] = none ? 0.f : o[u][e];
-      any += 16 * u + 4 * g < a.D ? o[u][e] : 0.f;
-    }
+  for (int i = 0; i < NC; ++i) {
+    const f32x4 y = run(i);
+    any += first(i) < a.D ? (y[0] + y[1]) + (y[2] + y[3]) : 0.f;
+  }
   if (in_rows) {
     const int64_t at = part.p ? part.at(a, x, slice) : 0;
     if (part.p && g == 0) {
@@ -213,13 +241,12 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 2 : 4) void k_span_f32(SpanArgs
       ml[1] = l;
     }
     float* O = part.p ? part.row(at) : static_cast<float*>(a.o) + x.b * a.ost[0] + x.h * a.ost[1] + x.t * a.ost[2];
+    const float f = part.p ? 1.f : inv;
 #pragma unroll
-    for (int u = 0; u < DP / 16; ++u) {
-      const int d = 16 * u + 4 * g;
-      if (d < a.D) *reinterpret_cast<f32x4*>(O + d) = part.p ? o[u] : o[u] * inv;
-    }
+    for (int i = 0; i < NC; ++i)
+      if (first(i) < a.D) *reinterpret_cast<f32x4*>(O + first(i)) = (none ? f32x4{0.f, 0.f, 0.f, 0.f} : run(i)) * f;
   }
-  const uint64_t bad = __ballot(in_rows && !(any == any) && l == l);
+  const uint64_t bad = __ballot(in_rows && !none && !(any == any) && l == l);
   uint32_t rows = static_cast<uint32_t>(bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffffu;
   if (rows != 0) wait_vmcnt<0>();  // what has been written of these rows is written before what follows
   while (rows != 0) {
