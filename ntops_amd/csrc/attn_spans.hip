@@ -38,20 +38,20 @@ __global__ __launch_bounds__(256) void k_span_rows(SpanArgs a, int mode, int sli
 }
 
 // Combines the slices of every query row in slice order: one wave per row, W lanes
-// a slice and 64 / W slices side by side.
-template <typename T, int W>
+// a slice and 64 / W slices side by side, AHEAD times as many in flight.
+template <typename T, int W, int AHEAD>
 __global__ __launch_bounds__(256) void k_span_merge(SpanArgs a, SpanPart part) {
   const int lane = threadIdx.x & 63;
   const int64_t row = block_id() * 4 + (threadIdx.x >> 6);
   if (row >= static_cast<int64_t>(a.B) * a.Hq * a.Sq) return;
-  constexpr int NS = 64 / W, kAhead = 4;
+  constexpr int NS = 64 / W;
   const int d = (lane % W) * 4, g = lane / W;
   const auto load = [&](int s) {
     return s < part.slices && d < part.ld ? *reinterpret_cast<const f32x4*>(part.row(row * part.slices + s) + d) : f32x4{0.f, 0.f, 0.f, 0.f};
   };
-  f32x4 v[kAhead];  // in flight while the weights are formed
+  f32x4 v[AHEAD];  // in flight while the weights are formed
 #pragma unroll
-  for (int u = 0; u < kAhead; ++u) v[u] = load(u * NS + g);
+  for (int u = 0; u < AHEAD; ++u) v[u] = load(u * NS + g);
   float m = neg_inf(), l = 0.f;
   if (lane < part.slices) {
     const float* ml = part.ml(a, row * part.slices + lane);
@@ -68,10 +68,15 @@ __global__ __launch_bounds__(256) void k_span_merge(SpanArgs a, SpanPart part) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += ws != 0.f ? ws * x[e] : 0.f;
   };
+  for (int s0 = 0; s0 < part.slices; s0 += AHEAD * NS) {
+    if (s0 > 0) {
 #pragma unroll
-  for (int u = 0; u < kAhead; ++u)
-    if (u * NS < part.slices) add(u * NS + g, v[u]);
-  for (int s0 = kAhead * NS; s0 < part.slices; s0 += NS) add(s0 + g, load(s0 + g));
+      for (int u = 0; u < AHEAD; ++u) v[u] = load(s0 + u * NS + g);
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (s0 + u * NS < part.slices) add(s0 + u * NS + g, v[u]);
+  }
 #pragma unroll
   for (int step = W; step < 64; step <<= 1)
 #pragma unroll
@@ -85,18 +90,23 @@ __global__ __launch_bounds__(256) void k_span_merge(SpanArgs a, SpanPart part) {
     if (d + e < a.D) O[(d + e) * a.ost[3]] = static_cast<T>(o[e] * inv);
 }
 
+template <typename T, int W>
+int launch_merge(const SpanArgs& a, const SpanPart& part, hipStream_t st) {
+  const dim3 grid = blocks_2d(ceil_div(static_cast<int64_t>(a.B) * a.Hq * a.Sq, 4)), block(256);
+  // (33 slices of 128 columns, 8 or 4 times 2 in flight: (1, 32 / 8, 1 over 32768) 29.5 / 31.5 us)
+  if (part.slices > 4 * (64 / W))
+    hipLaunchKernelGGL((k_span_merge<T, W, 8>), grid, block, 0, st, a, part);
+  else
+    hipLaunchKernelGGL((k_span_merge<T, W, 4>), grid, block, 0, st, a, part);
+  return check_launch("attention");
+}
+
 int merge(int dtype, const SpanArgs& a, const SpanPart& part, hipStream_t st) {
-  const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Sq;
   return dispatch_float16_32(dtype, "attention", [&](auto tag) {
     using T = decltype(tag);
-    const dim3 grid = blocks_2d(ceil_div(rows, 4)), block(256);
-    if (part.ld <= 64)
-      hipLaunchKernelGGL((k_span_merge<T, 16>), grid, block, 0, st, a, part);
-    else if (part.ld <= 128)
-      hipLaunchKernelGGL((k_span_merge<T, 32>), grid, block, 0, st, a, part);
-    else
-      hipLaunchKernelGGL((k_span_merge<T, 64>), grid, block, 0, st, a, part);
-    return check_launch("attention");
+    if (part.ld <= 64) return launch_merge<T, 16>(a, part, st);
+    if (part.ld <= 128) return launch_merge<T, 32>(a, part, st);
+    return launch_merge<T, 64>(a, part, st);
   });
 }
 
