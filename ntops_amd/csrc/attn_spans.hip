@@ -230,12 +230,15 @@ Plan make_plan(int dtype, const SpanArgs& a, bool joined = false) {
     const bool apart = again > read_again(few_front) &&
                        (few || walked(blocks, static_cast<int64_t>(a.P) + a.C) > 1.75 * (walked(front, a.P) + walked(blocks, a.C)));
     if (apart) {
-      // A front block a CU; beside blocks of few rows half as many, but of no more than
-      // 1024 keys, so that the others find room (64 sequences over 8192 of their group and
-      // up to 1024 of their own, 4 / 8 / 12 / 16 slices: 58 / 50 / 55 / 58 us; 16 over 32768, 16 /
-      // 32: 56 / 46).
+      // A front block a CU; of kFew on three of four (4 sequences over 32768 with 8 heads, 16 /
+      // 24 / 32 slices: 33.7 / 31.1 / 36.4 us, 2 over 100000 80 / 70 / 78; 32 over four of up to 5001
+      // with 16 heads, 2 / 3 / 4 slices 28.6 / 27.5 / 28.4); of kTile beside blocks of few rows on
+      // half, but of no more than 1024 keys, so that the others find room (64 sequences over
+      // 8192 of their group and up to 1024 of their own, 4 / 8 / 12 / 16 slices: 58 / 50 / 55 / 58
+      // us; 16 over 32768, 16 / 32: 56 / 46).
       const bool mixed = few && !few_front;
-      const int64_t most = ceil_div(a.P, mixed ? 512 : 128), wide = std::max<int64_t>(1, (mixed ? cus / 2 : cus) / front);
+      const int64_t most = ceil_div(a.P, mixed ? 512 : 128);
+      const int64_t wide = std::max<int64_t>(1, (mixed ? cus / 2 : few ? cus * 3 / 4 : cus) / front);
       const int64_t cut = std::max<int64_t>(mixed ? ceil_div(a.P, 1024) : 1, std::min(most, wide));
       const int fs = static_cast<int>(std::min<int64_t>(kMaxSlices / 2, cut));
       // own keys: slices no longer than twice the prefix's
