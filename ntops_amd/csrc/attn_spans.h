@@ -160,8 +160,10 @@ struct SpanPart {
 // each; the four streams of keys are joined at the end.  Every lane ends with the
 // whole row: o[u] of column (lane & 15) + 16 u.
 //
-// Front keys [f0, f1) and main keys [m0, m1) of what the row sees.
-template <typename T, int EL, int UNROLL>
+// Front keys [f0, f1) and main keys [m0, m1) of what the row sees.  MEAN: o is divided by
+// the sum at every step, so that it never passes the largest value; without, o is the sum
+// of values times weights, which may where the result does not.
+template <typename T, int EL, int UNROLL, bool MEAN>
 __device__ __forceinline__ void span_attend_row(const SpanArgs& a, const Spans& s, const SpanRow x, int f0, int f1, int m0,
                                              int m1, float (&o)[EL], float& m, float& l) {
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
@@ -209,8 +211,14 @@ __device__ __forceinline__ void span_attend_row(const SpanArgs& a, const Spans& 
         const float sc = k + 4 * w < k1 ? d * a.scale_log2 : neg_inf();
         const float m_new = fmaxf(m, sc);
         const float m_use = m_new == neg_inf() ? 0.f : m_new;
-        const float alpha = fast_exp2(m - m_use), p = fast_exp2(sc - m_use);
-        l = l * alpha + p;
+        float alpha = fast_exp2(m - m_use), p = fast_exp2(sc - m_use);
+        const float l_new = l * alpha + p;
+        if (MEAN) {
+          const float by = l_new == 0.f ? 0.f : 1.f / l_new;
+          alpha *= l * by;
+          p *= by;
+        }
+        l = l_new;
 #pragma unroll
         for (int u = 0; u < EL; ++u) o[u] = fmaf(p, vv[w][u], o[u] * alpha);
         m = m_new;
@@ -221,22 +229,34 @@ __device__ __forceinline__ void span_attend_row(const SpanArgs& a, const Spans& 
   for (int step = 16; step <= 32; step <<= 1) {
     const float m2 = __shfl_xor(m, step, 64);
     const float mm = fmaxf(m, m2), m_use = mm == neg_inf() ? 0.f : mm;
-    const float f = fast_exp2(m - m_use), f2 = fast_exp2(m2 - m_use);
-    l = l * f + __shfl_xor(l, step, 64) * f2;
+    float f = fast_exp2(m - m_use), f2 = fast_exp2(m2 - m_use);
+    const float l2 = __shfl_xor(l, step, 64), l_new = l * f + l2 * f2;
+    if (MEAN) {
+      const float by = l_new == 0.f ? 0.f : 1.f / l_new;
+      f *= l * by;
+      f2 *= l2 * by;
+    }
+    l = l_new;
 #pragma unroll
     for (int u = 0; u < EL; ++u) o[u] = o[u] * f + __shfl_xor(o[u], step, 64) * f2;
     m = mm;
   }
 }
 
-// Writes such a row: to the output, or as slice `slice` of the partial results.
-template <typename T, int EL>
+// Writes such a row: to the output, or as slice `slice` of the partial results -- a mean
+// under a sum and a weight of it in (0.5, 1] with a power of two taken into the maximum.
+template <typename T, int EL, bool MEAN>
 __device__ __forceinline__ void span_write_row(const SpanArgs& a, const SpanPart& part, const SpanRow& x, int slice,
                                                const float (&o)[EL], float m, float l) {
   const int lane = threadIdx.x & 63;
   if (lane >= 16) return;
   if (part.p) {
     const int64_t at = part.at(a, x, slice);
+    float f = 1.f;
+    if (MEAN && l > 0.f) {
+      m += static_cast<float>(__builtin_amdgcn_frexp_expf(l));
+      l = f = __builtin_amdgcn_frexp_mantf(l);
+    }
     if (lane == 0) {
       float* ml = part.ml(a, at);
       ml[0] = m;
@@ -244,14 +264,26 @@ __device__ __forceinline__ void span_write_row(const SpanArgs& a, const SpanPart
     }
 #pragma unroll
     for (int u = 0; u < EL; ++u)
-      if (lane + 16 * u < a.D) part.row(at)[lane + 16 * u] = o[u];
+      if (lane + 16 * u < a.D) part.row(at)[lane + 16 * u] = o[u] * f;
     return;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // (a NaN sum, from a NaN score, passes through)
+  const float inv = l == 0.f ? 0.f : MEAN ? 1.f : 1.f / l;  // (a NaN sum, from a NaN score, passes through)
   T* O = static_cast<T*>(a.o) + x.b * a.ost[0] + x.h * a.ost[1] + x.t * a.ost[2];
 #pragma unroll
   for (int u = 0; u < EL; ++u)
     if (lane + 16 * u < a.D) O[(lane + 16 * u) * a.ost[3]] = static_cast<T>(o[u] * inv);
+}
+
+// What has to be computed again by itself: a sum of a row's columns that is no number, or
+// none that fp32 holds, under a sum of weights that is one.
+__device__ __forceinline__ bool span_again(float any, float l) { return !(any - any == 0.f) && l == l; }
+// The row again, from keys [f0, f1) of the front and [m0, m1) of the main span.
+template <typename T, int EL>
+__device__ __forceinline__ void span_row_again(const SpanArgs& a, const Spans& s, const SpanPart& part, const SpanRow& x, int slice, int f0, int f1,
+                                               int m0, int m1) {
+  float o[EL], m, l;
+  span_attend_row<T, EL, 1, true>(a, s, x, f0, f1, m0, m1, o, m, l);
+  span_write_row<T, EL, true>(a, part, x, slice, o, m, l);
 }
 
 // ---- paths (host) ------------------------------------------------------------

@@ -31,10 +31,16 @@ __global__ __launch_bounds__(256) void k_span_rows(SpanArgs a, int mode, int sli
   const Spans s = make_spans<sizeof(T)>(a, mode, set, t, t);
   const SpanRow x = span_row(a, mode, s, r);
   const int fc = (s.n[0] + slices - 1) / slices, mc = (s.n[1] + slices - 1) / slices;
+  const int f0 = min(slice * fc, s.n[0]), f1 = min(slice * fc + fc, s.n[0]), m0 = min(slice * mc, s.n[1]), m1 = min(slice * mc + mc, s.n[1]);
   float o[EL], m, l;
-  span_attend_row<T, EL, (EL > 8 ? 2 : 4)>(a, s, x, min(slice * fc, s.n[0]), min(slice * fc + fc, s.n[0]), min(slice * mc, s.n[1]), min(slice * mc + mc, s.n[1]),
-                         o, m, l);
-  span_write_row<T, EL>(a, part, x, slice, o, m, l);
+  span_attend_row<T, EL, (EL > 8 ? 2 : 4), false>(a, s, x, f0, f1, m0, m1, o, m, l);
+  float any = 0.f;
+#pragma unroll
+  for (int u = 0; u < EL; ++u) any += o[u];
+  if (__any(span_again(any, l)))
+    span_row_again<T, EL>(a, s, part, x, slice, f0, f1, m0, m1);
+  else
+    span_write_row<T, EL, false>(a, part, x, slice, o, m, l);
 }
 
 // Combines the slices of every query row in slice order: one wave per row, W lanes
@@ -59,8 +65,10 @@ __global__ __launch_bounds__(256) void k_span_merge(SpanArgs a, SpanPart part) {
     l = ml[1];
   }
   const float mm = wave_max(m);
-  const float w = m == neg_inf() ? 0.f : fast_exp2(m - mm);
+  float w = m == neg_inf() ? 0.f : fast_exp2(m - mm);
   const float sum = wave_sum(l * w);
+  // (divided first: sums of slices may pass fp32's range where the result does not)
+  w *= sum == 0.f ? 0.f : 1.f / sum;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   const auto add = [&](int s, f32x4 x) {
     const float ws = __shfl(w, s & 63, 64);
@@ -82,12 +90,11 @@ __global__ __launch_bounds__(256) void k_span_merge(SpanArgs a, SpanPart part) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], step, 64);
   if (g != 0) return;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const uint32_t id = static_cast<uint32_t>(row), bh = id / static_cast<uint32_t>(a.Sq), b = bh / static_cast<uint32_t>(a.Hq);
   T* O = static_cast<T*>(a.o) + b * a.ost[0] + (bh - b * a.Hq) * a.ost[1] + (id - bh * a.Sq) * a.ost[2];
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (d + e < a.D) O[(d + e) * a.ost[3]] = static_cast<T>(o[e] * inv);
+    if (d + e < a.D) O[(d + e) * a.ost[3]] = static_cast<T>(o[e]);
 }
 
 template <typename T, int W>

@@ -246,17 +246,15 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 2 : 4) void k_span_f32(SpanArgs
     for (int i = 0; i < NC; ++i)
       if (first(i) < a.D) *reinterpret_cast<f32x4*>(O + first(i)) = (none ? f32x4{0.f, 0.f, 0.f, 0.f} : run(i)) * f;
   }
-  const uint64_t bad = __ballot(in_rows && !none && !(any == any) && l == l);
+  const uint64_t bad = __ballot(in_rows && !none && span_again(any, l));
   uint32_t rows = static_cast<uint32_t>(bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffffu;
   if (rows != 0) wait_vmcnt<0>();  // what has been written of these rows is written before what follows
   while (rows != 0) {
     const int r = qw + __builtin_ctz(rows);
     rows &= rows - 1;
     const SpanRow y = span_row(a, mode, s, r);
-    float ro_[DP / 16], rm, rl;
     const int k0 = i0 * kKeys, k1 = min(k0 + nkv * kKeys, keys);
-    span_attend_row<float, DP / 16, 1>(a, s, y, min(k0, nf), min(k1, nf), max(0, k0 - nf), max(0, k1 - nf), ro_, rm, rl);
-    span_write_row<float, DP / 16>(a, part, y, slice, ro_, rm, rl);
+    span_row_again<float, DP / 16>(a, s, part, y, slice, min(k0, nf), min(k1, nf), max(0, k0 - nf), max(0, k1 - nf));
   }
 }
 
@@ -431,7 +429,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_span_f32_few(SpanArgs a, 
       for (int e = 0; e < 4; ++e) v[e] += mw == neg_inf() ? 0.f : ow[e] * fw;
     }
     const float any = (v[0] + v[1]) + (v[2] + v[3]);
-    if (!(any == any) && sum == sum) atomicOr(&again, 1u << row);
+    if (span_again(any, sum)) atomicOr(&again, 1u << row);
     const SpanRow y = span_row(a, mode, s, row);
     if (part.p) {
       const int64_t at = part.at(a, y, slice);
@@ -456,9 +454,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_span_f32_few(SpanArgs a, 
     bad &= bad - 1;
     if (row % NW != wave) continue;
     const SpanRow y = span_row(a, mode, s, row);
-    float ro_[KT], rm, rl;
-    span_attend_row<float, KT, 1>(a, s, y, min(16 * i0, nf), min(16 * i1, nf), max(0, 16 * i0 - nf), max(0, min(16 * i1, keys) - nf), ro_, rm, rl);
-    span_write_row<float, KT>(a, part, y, slice, ro_, rm, rl);
+    span_row_again<float, KT>(a, s, part, y, slice, min(16 * i0, nf), min(16 * i1, nf), max(0, 16 * i0 - nf), max(0, min(16 * i1, keys) - nf));
   }
 }
 

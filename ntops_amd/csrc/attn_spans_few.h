@@ -17,8 +17,9 @@
 // that follow from them and the first tile take most, one after the other.
 //
 // What a row does not see: masked scores are -inf whatever their key holds.  A
-// value that is not finite times P = 0 is NaN, though; a row whose result is NaN under
-// a sum that is none is computed again by itself, from the keys that it sees.
+// value that is not finite times P = 0 is NaN, though; a row whose result is NaN, or past
+// fp32's range, under a sum that is a number is computed again by itself, from the keys
+// that it sees.
 #pragma once
 
 #include "attn_spans.h"
@@ -107,15 +108,14 @@ __device__ __forceinline__ void wait_dma() {
 
 // One kind of blocks of a launch.
 struct FewBlocks {
-  int mode;       // SpanMode
+  int mode;  // SpanMode
   int slices;
-  int first;       // slice of the rows that slice 0 is
-  uint32_t sets, blocks;
+  int first;  // slice of the rows that slice 0 is
+  uint32_t blocks;
 };
 
 inline FewBlocks few_blocks(const SpanArgs& a, int mode, int slices, int first) {
-  const uint32_t sets = static_cast<uint32_t>(span_sets(a, mode));
-  return {mode, slices, first, sets, sets * slices};
+  return {mode, slices, first, static_cast<uint32_t>(span_sets(a, mode)) * static_cast<uint32_t>(slices)};
 }
 
 // RG: groups of 16 rows a block has room for.
@@ -398,7 +398,7 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
         for (int e = 0; e < 4; ++e) v[e] += mw == neg_inf() ? 0.f : ow[e] * fw;
       }
       const float any = (v[0] + v[1]) + (v[2] + v[3]);
-      if (!(any == any) && sum == sum) atomicOr(again, 1u << (rg * 16 + row));
+      if (span_again(any, sum)) atomicOr(again, 1u << (rg * 16 + row));
       if (part.p) {
         const int64_t pa = to[row];
         if (d == 0) {
@@ -427,10 +427,8 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
     bad &= bad - 1;
     if (row % NW != wave) continue;
     const SpanRow x = span_row(a, f.mode, s, row);
-    float ro_[D / 16], rm, rl;
-    span_attend_row<T, D / 16, 1>(a, s, x, min(i0 * NK, s.n[0]), min(i1 * NK, s.n[0]), max(0, min((i0 - nft) * NK, s.n[1])),
-                               max(0, min((i1 - nft) * NK, s.n[1])), ro_, rm, rl);
-    span_write_row<T, D / 16>(a, part, x, slice, ro_, rm, rl);
+    span_row_again<T, D / 16>(a, s, part, x, slice, min(i0 * NK, s.n[0]), min(i1 * NK, s.n[0]), max(0, min((i0 - nft) * NK, s.n[1])),
+                              max(0, min((i1 - nft) * NK, s.n[1])));
   }
 }
 

@@ -14,6 +14,7 @@
 // Blocks see few keys at a prompt's start and many at its end, so the order in which they
 // are handed out decides where two a CU start at once: (1, 16 / 4, 4096 causal) of 128 97 us,
 // set after set 119.
+//
 // Eight waves of 32 rows that alternate the two kinds of phase between barriers (256
 // rows, four stages, one block a CU) took 2 % less for long rows of 128 columns -- (16,
 // 32 / 8, 500 over a shared 8192) bf16 1070 against 1088 us -- 28 % more of 64 columns,
@@ -22,8 +23,9 @@
 //
 // A row's reference (from which its exponents are taken) follows its maximum when that
 // is past it by more than 2^8.  Masked scores are -inf whatever their key holds; a
-// value that is not finite times P = 0 is NaN, so a row whose result is NaN under a sum
-// that is none is computed again by itself, from the keys that it sees.
+// value that is not finite times P = 0 is NaN, so a row whose result is NaN, or past fp32's
+// range, under a sum that is a number is computed again by itself, from the keys that it
+// sees.
 //
 // Bound by the vector instructions of the softmax beside the matrix cores (55 % busy over
 // long rows of 128 columns), at few tiles a block by its start and end, and of one row a
@@ -363,16 +365,14 @@ __device__ __forceinline__ void tile_block(const SpanArgs& a, int mode, int nqb,
     }
   }
   wait_vmcnt<0>();  // no DMA may land after the workgroup ends
-  const uint64_t bad = __ballot(in_rows && !(any == any) && l == l);
+  const uint64_t bad = __ballot(in_rows && span_again(any, l));
   uint32_t rows = static_cast<uint32_t>(bad) | static_cast<uint32_t>(bad >> 32);
   while (rows != 0) {
     const int r = qw + __builtin_ctz(rows);
     rows &= rows - 1;
     const SpanRow y = span_row(a, mode, s, r);
-    float ro_[DM / 16], rm, rl;
     const int k0 = i0 * kKeys, k1 = min(k0 + nkv * kKeys, keys);
-    span_attend_row<T, DM / 16, 1>(a, s, y, min(k0, nf), min(k1, nf), max(0, k0 - nf), max(0, k1 - nf), ro_, rm, rl);
-    span_write_row<T, DM / 16>(a, part, y, slice, ro_, rm, rl);
+    span_row_again<T, DM / 16>(a, s, part, y, slice, min(k0, nf), min(k1, nf), max(0, k0 - nf), max(0, k1 - nf));
   }
 }
 

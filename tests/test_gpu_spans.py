@@ -217,6 +217,33 @@ def test_what_a_row_does_not_see_does_not_reach_it_apart(g, b, hq, hkv, sq, p, c
     check_prefix(q, pk, pv, k, v, torch.tensor(seen[:g]).cuda(), torch.full((b,), c - 3).cuda())
 
 
+def huge(*shape, dtype, signs):
+    """Values up to the type's largest, sums of which no fp32 holds."""
+    t = (torch.rand(*shape) * 0.7 + 0.25) * torch.finfo(dtype).max
+    return (t * (torch.randint(0, 2, shape) * 2 - 1) if signs else t).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("signs", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sq,hkv,d", [(1, 2, 128), (1, 4, 64), (3, 2, 128), (7, 1, 64), (70, 2, 128), (300, 2, 96), (300, 4, 128), (9, 1, 200), (5, 2, 38)])
+def test_values_whose_sum_is_past_the_range(sq, hkv, d, dtype, signs):
+    b, hq, c = 2, 4, 400
+    q, k, _ = window_inputs(b, hq, hkv, sq, c, d, dtype)
+    v = huge(b, hkv, c, d, dtype=dtype, signs=signs)
+    for kk in (k, k * 0, k * 4):
+        check_window(q, kk, v, 150, 3, torch.tensor([c - 20, c // 2]).cuda())
+        check_prefix(q, kk[:1], v[:1], k[:, :, :90], v[:, :, :90])
+
+
+@pytest.mark.parametrize("signs", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("g,b,hq,hkv,sq,p,c,d", APART)
+def test_values_whose_sum_is_past_the_range_apart(g, b, hq, hkv, sq, p, c, d, dtype, signs):
+    q, k, _ = window_inputs(b, hq, hkv, sq, c, d, dtype)
+    pk = values(g, hkv, p, d, dtype=dtype)
+    check_prefix(q, pk, huge(g, hkv, p, d, dtype=dtype, signs=signs), k, huge(b, hkv, c, d, dtype=dtype, signs=signs))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("sq", [1, 5, 120])
 def test_scales(sq, dtype):
