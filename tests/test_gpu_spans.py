@@ -109,7 +109,7 @@ PREFIXES = [
 # groups whose rows attend to their prefix apart from their own keys
 APART = [
     (1, 16, 2, 2, 1, 10007, 30, 128), (2, 32, 4, 4, 1, 5001, 9, 64), (1, 40, 4, 2, 3, 3001, 50, 128), (2, 60, 4, 2, 10, 4003, 33, 80),
-    (1, 33, 8, 8, 1, 2100, 600, 64), (1, 30, 2, 2, 40, 8001, 30, 64),
+    (1, 33, 8, 8, 1, 2100, 600, 64), (1, 16, 2, 2, 33, 8001, 30, 128),
 ]
 
 
