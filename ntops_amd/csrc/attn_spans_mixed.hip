@@ -25,7 +25,7 @@ __global__ __launch_bounds__(64 * span_tile::kWaves, 2) void k_span_mixed(SpanAr
   if (id < front) {
     part.first = 0;
     span_tile::tile_block<T, DT, DT>(a, kFront, nqb, slices, front, part, id, smem);
-  } else if (threadIdx.x < 64 * kFewWaves) {
+  } else if (threadIdx.x < 64 * kFewWaves) {  // (whole waves, which a branch takes past the barriers; as a scalar condition 3 % slower)
     span_few::few_block<T, D, kFewWaves, RGM>(a, main, part, id - front, smem);
   }
 }
