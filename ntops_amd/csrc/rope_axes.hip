@@ -214,7 +214,8 @@ template <typename T, typename TT>
 int run_axes(const AxesArgs& a, hipStream_t st) {
   constexpr int V = Pack16<T>::N;
   const int64_t tokens = a.B * a.S, heads = a.t[0].H + a.t[1].H;
-  bool vec = (a.D / 2) % (a.interleaved ? V / 2 : V) == 0;
+  // (the vector path's heads are 32-bit: parts <= heads, so h + kUnroll * parts < 3 * 2^29)
+  bool vec = (a.D / 2) % (a.interleaved ? V / 2 : V) == 0 && heads <= (int64_t(1) << 29);
   for (const AxesTensor& d : a.t) {
     if (d.H == 0) continue;
     vec = vec && d.xs[3] == 1 && d.ys[3] == 1 && aligned16(d.x) && aligned16(d.y);
