@@ -540,7 +540,9 @@ NTOPS_API int ntops_rope_qk(int dtype, int64_t B, int64_t S, int64_t Hq, int64_t
  * positions (axes, B, S) by 3 element strides, I32 or I64, are read on the device; a
  * pair whose position lies outside of the table_rows rows is NaN.  Tables of F32 or
  * of dtype, of D / 2 columns (column i) or D (each element its own).  fp32, one
- * rounding.  D <= 512.  In place per tensor with equal strides. */
+ * rounding.  D <= 512.  In place per tensor with equal strides; elements of a result
+ * that share memory with each other, with the other tensor or otherwise with their own
+ * are refused. */
 NTOPS_API int ntops_rope_axes_qk(int dtype, int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D,
                const void* q, const int64_t* q_strides,
                const void* k, const int64_t* k_strides,

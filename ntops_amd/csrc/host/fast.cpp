@@ -879,10 +879,10 @@ PyObject* shared_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NTOPS_END
 }
 
-// rope_axes_qk(q, k, sin, cos, positions, sections (a list or tuple of ints), interleaved)
+// rope_axes_qk(q, k, sin, cos, positions, sections (a list or tuple of ints), interleaved, inplace = False)
 PyObject* rope_axes_qk(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NTOPS_TRY
-  if (n != 7 || !usable() || !PyBool_Check(a[6]) || (!PyTuple_CheckExact(a[5]) && !PyList_CheckExact(a[5]))) return none();
+  if ((n != 7 && n != 8) || !usable() || !PyBool_Check(a[6]) || (n == 8 && !PyBool_Check(a[7])) || (!PyTuple_CheckExact(a[5]) && !PyList_CheckExact(a[5]))) return none();
   const at::Tensor* t[5];
   int64_t dev;
   void* st;
@@ -904,12 +904,13 @@ PyObject* rope_axes_qk(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (count > 256) return none();
   for (Py_ssize_t i = 0; i < count; ++i)
     if (!integer(PySequence_Fast_GET_ITEM(a[5], i), sections[i])) return none();
+  const bool inplace = n == 8 && a[7] == Py_True;
   at::Tensor qo, ko;
   int rc;
   {
     NoGil free;
-    qo = new_like(q, q.sizes());
-    ko = new_like(k, k.sizes());
+    qo = inplace ? q : new_like(q, q.sizes());
+    ko = inplace ? k : new_like(k, k.sizes());
     rc = f_rope_axes_qk(code, B, S, q.size(2), k.size(2), D, q.data_ptr(), q.strides().data(), k.data_ptr(), k.strides().data(), tcode,
                         sn.data_ptr(), sn.stride(0), cs.data_ptr(), cs.stride(0), sn.size(0), tw, pos.size(0), pos.data_ptr(), pcode,
                         pos.strides().data(), count, sections, a[6] == Py_True ? 1 : 0, qo.data_ptr(), qo.strides().data(),

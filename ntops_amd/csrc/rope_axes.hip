@@ -12,6 +12,7 @@
 // bytes, fp32 and from a row of its own for each axis, would otherwise pass the L1 as
 // often as the heads' own.  Generic path: a thread per pair, any strides.
 #include <algorithm>
+#include <cstdlib>
 
 #include "dispatch.h"
 #include "kv_cache.h"
@@ -252,6 +253,98 @@ int run_axes(const AxesArgs& a, hipStream_t st) {
   return check_launch("rope_axes");
 }
 
+// ---- what tensors share (host) ------------------------------------------------
+
+using Wide = __int128;  // sums of strides times sizes, whatever the caller gives
+
+// Steps n of 0 .. most of a dim, or of one dim of each of two tensors together.
+struct Steps {
+  int64_t step, most;
+};
+struct Layout {
+  Steps s[8];
+  int n = 0;
+  Wide before = 0;  // what steps below zero take from the first element's place
+  void add(int64_t step, int64_t most) {
+    if (most <= 0 || step == 0) return;
+    if (step < 0) {
+      before += static_cast<Wide>(step) * most;
+      step = -step;
+    }
+    for (int i = 0; i < n; ++i)
+      if (s[i].step == step) {
+        s[i].most += most;
+        return;
+      }
+    s[n++] = {step, most};
+  }
+  Wide reach() const {
+    Wide r = 0;
+    for (int i = 0; i < n; ++i) r += static_cast<Wide>(s[i].step) * s[i].most;
+    return r;
+  }
+};
+
+// Whether `left` is a sum of step * n over the layout's steps, largest first, which leaves
+// few n where strides are those of nested dims; true where `trials` do not tell.
+bool reaches(const Layout& a, int i, Wide rest, Wide left, int& trials) {
+  if (left == 0) return true;
+  if (left < 0 || left > rest) return false;
+  const Wide step = a.s[i].step, behind = rest - step * a.s[i].most;
+  const Wide last = std::min<Wide>(a.s[i].most, left / step);
+  for (Wide n = left > behind ? (left - behind + step - 1) / step : 0; n <= last; ++n) {
+    if (--trials < 0 || reaches(a, i + 1, behind, left - n * step, trials)) return true;
+  }
+  return false;
+}
+bool reaches(Layout& a, Wide target) {
+  std::sort(a.s, a.s + a.n, [](const Steps& x, const Steps& y) { return x.step > y.step; });
+  int trials = 10000;
+  return reaches(a, 0, a.reach(), target, trials);
+}
+
+struct Strided {
+  const void* p;
+  const int64_t* st;
+  int64_t size[4];
+};
+
+// Whether two elements of x are the same memory.
+bool meets_itself(const Strided& x) {
+  for (int i = 0; i < 4; ++i) {
+    // index vectors that differ first in dim i, by n + 1, and by -most .. most behind it
+    const int64_t most = x.size[i] - 1, step = std::abs(x.st[i]);
+    if (most <= 0) continue;
+    if (step == 0) return true;
+    Layout a;
+    a.add(step, most - 1);
+    Wide target = -static_cast<Wide>(step);
+    for (int j = i + 1; j < 4; ++j) {
+      const int64_t s = std::abs(x.st[j]);
+      a.add(s, 2 * (x.size[j] - 1));
+      target += static_cast<Wide>(s) * (x.size[j] - 1);
+    }
+    if (reaches(a, target)) return true;
+  }
+  return false;
+}
+
+// Whether an element of x and one of y, of `es` bytes each, are the same memory.
+bool meet(const Strided& x, const Strided& y, int es) {
+  Layout a, b;
+  for (int i = 0; i < 4; ++i) a.add(x.st[i], x.size[i] - 1);
+  for (int i = 0; i < 4; ++i) b.add(y.st[i], y.size[i] - 1);
+  const Wide apart = static_cast<Wide>(reinterpret_cast<intptr_t>(y.p)) - reinterpret_cast<intptr_t>(x.p);
+  // in elements: the places of x are lowest + 0 .. reach, those of y likewise
+  const Wide x_low = a.before * es, y_low = apart + b.before * es;
+  const Wide x_high = x_low + a.reach() * es, y_high = y_low + b.reach() * es;
+  if (y_low >= x_high + es || x_low >= y_high + es) return false;
+  if (apart % es != 0) return true;
+  // x's steps from its lowest place, and y's down from its highest
+  for (int i = 0; i < b.n; ++i) a.add(b.s[i].step, b.s[i].most);
+  return reaches(a, (y_high - x_low) / es);
+}
+
 }  // namespace
 }  // namespace ntops
 
@@ -312,6 +405,20 @@ extern "C" int ntops_rope_axes_qk(int dtype, int64_t B, int64_t S, int64_t Hq, i
       for (int d = 0; d < 4; ++d)
         if (xst[t][d] != yst[t][d]) return set_error(NTOPS_ERR_INVALID, "%s: in place needs equal strides", what);
   }
+  // What one thread writes, no other may read or write.
+  Strided x[2], y[2];
+  for (int t = 0; t < 2; ++t) {
+    x[t] = {xs[t], xst[t], {B, S, hs[t], D}};
+    y[t] = {ys[t], yst[t], {B, S, hs[t], D}};
+  }
+  const int es = dtype == NTOPS_F32 ? 4 : 2;
+  for (int t = 0; t < 2; ++t) {
+    if (hs[t] == 0) continue;
+    if (meets_itself(y[t])) return set_error(NTOPS_ERR_INVALID, "%s: elements of a result share memory", what);
+    if (xs[t] != ys[t] && meet(x[t], y[t], es)) return set_error(NTOPS_ERR_INVALID, "%s: a result and its tensor share elements", what);
+  }
+  if (Hq > 0 && Hk > 0 && (meet(y[0], y[1], es) || meet(y[0], x[1], es) || meet(x[0], y[1], es)))
+    return set_error(NTOPS_ERR_INVALID, "%s: q and k share elements that are written", what);
   a.sn = sin_table;
   a.cs = cos_table;
   a.srs = sin_row_stride;

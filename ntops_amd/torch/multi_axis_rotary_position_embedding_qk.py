@@ -14,7 +14,8 @@ interleaved=False (i, i + dim / 2).
 
 Computed in fp32 and rounded once.  A pair whose position lies outside of the tables
 is NaN (positions are read on the device).  Returns (q_out, k_out); inplace=True
-rotates q and k in place."""
+rotates q and k in place, where each element is one of its own: tensors that share
+elements with each other or with themselves are refused."""
 
 import operator
 
@@ -24,20 +25,74 @@ from ntops_amd import _lib
 from ntops_amd.torch.utils import _DeviceGuard, _contiguous, _strides, _to_dtype
 
 
-def _share_heads(q, k):
-    """Whether q and k are the same memory, or slices of one tensor along its heads that overlap."""
+def _reaches(target, terms):
+    """Whether `target` is the sum of step * n over the (step, most) of `terms`, for some n of 0 .. most
+    each.  Largest steps first, which leave few n where strides are those of nested dims; True
+    where 10000 trials do not tell."""
+    most_of = {}
+    for step, most in terms:
+        if step and most:
+            most_of[step] = most_of.get(step, 0) + most
+    steps = sorted(most_of.items(), reverse=True)
+    rest = [0]
+    for step, most in reversed(steps):
+        rest.append(rest[-1] + step * most)
+    rest.reverse()
+    todo = [(0, target)]
+    for _ in range(10000):
+        if not todo:
+            return False
+        i, left = todo.pop()
+        if left == 0:
+            return True
+        if left < 0 or left > rest[i]:
+            continue
+        step, most = steps[i]
+        first, last = max(0, -((rest[i + 1] - left) // step)), min(most, left // step)
+        if last - first > 10000:
+            return True
+        todo += [(i + 1, left - n * step) for n in range(first, last + 1)]
+    return True
+
+
+def _dims(x):
+    return [(s, n - 1) for s, n in zip(x.stride(), x.shape) if n > 1]
+
+
+def _meets_itself(x):
+    """Whether two elements of x are the same memory."""
+    if not x.numel():
+        return False
+    end = 1
+    for step, most in sorted(_dims(x)):
+        if step < end:
+            break
+        end += step * most
+    else:
+        return False  # each dim's step passes all that the smaller ones reach
+    # index vectors that differ first in dim i, by n + 1, and by -most .. most behind it
+    dims = _dims(x)
+    return any(
+        step == 0 or _reaches(sum(s * m for s, m in dims[i + 1 :]) - step, [(step, most - 1)] + [(s, 2 * m) for s, m in dims[i + 1 :]])
+        for i, (step, most) in enumerate(dims))
+
+
+def _meet(q, k):
+    """Whether an element of q and one of k are the same memory (both of one type)."""
     if not q.numel() or not k.numel():
         return False
+    size = q.element_size()
     apart = k.data_ptr() - q.data_ptr()
-    step = q.stride(2) * q.element_size()
-    if apart == 0 or q.stride() != k.stride() or step == 0 or apart % step:
-        return apart == 0
-    return -k.shape[2] < apart // step < q.shape[2]
+    q_end, k_end = (sum(s * m for s, m in _dims(x)) for x in (q, k))
+    if apart > q_end * size or -apart > k_end * size:
+        return False
+    # q's index vector, and k's counted from its last element
+    return apart % size != 0 or _reaches(apart // size + k_end, _dims(q) + _dims(k))
 
 
 def multi_axis_rotary_position_embedding_qk(q, k, sin_table, cos_table, positions, sections, interleaved=True, inplace=False):
-    if _lib.fast is not None and not inplace:
-        r = _lib.fast.rope_axes_qk(q, k, sin_table, cos_table, positions, sections, interleaved)
+    if _lib.fast is not None:
+        r = _lib.fast.rope_axes_qk(q, k, sin_table, cos_table, positions, sections, interleaved, inplace)
         if r is not None:
             return r
     what = "multi_axis_rotary_position_embedding_qk"
@@ -58,11 +113,10 @@ def multi_axis_rotary_position_embedding_qk(q, k, sin_table, cos_table, position
     if sin_table.dim() != 2 or sin_table.shape != cos_table.shape or sin_table.shape[1] not in (dim // 2, dim):
         raise RuntimeError(
             f"{what}: the tables must both be (positions, {dim // 2}) or (positions, {dim}), got {tuple(sin_table.shape)} and {tuple(cos_table.shape)}")
-    for x in (q, k):
-        if inplace and any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape)):
-            raise RuntimeError(f"{what}: elements that share memory (a stride is 0) cannot be rotated in place")
-    if inplace and _share_heads(q, k):
-        raise RuntimeError(f"{what}: q and k share heads, which would be rotated twice in place")
+    if inplace and (_meets_itself(q) or _meets_itself(k)):
+        raise RuntimeError(f"{what}: elements that share memory cannot be rotated in place")
+    if inplace and _meet(q, k):
+        raise RuntimeError(f"{what}: q and k share elements, which would be rotated twice in place")
     dev = _lib.require_cuda(q, k, sin_table, cos_table, positions)
     lib = _lib.load()
     with _DeviceGuard(dev):
