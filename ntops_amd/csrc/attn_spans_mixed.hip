@@ -3,7 +3,7 @@
 // their prefix, blocks of attn_spans_few.h each sequence's rows over its own keys, in one
 // launch, so that the first, bound by the matrix cores and vector instructions, run beside
 // the second, bound by streaming.  bf16, 32 / 8 heads of 128, 64 sequences of one token
-// over a shared 8192 and up to 1024 of their own: 49 us, of which 4.5 the merge (168 MB of
+// over a shared 8192 and up to 1024 of their own: 50 us, of which 4.5 the merge (168 MB of
 // own keys and 34 of the prefix: 41 at 4.95 TB/s), 53 with the prefix by blocks of few rows,
 // 63 by a launch of its own; 16 sequences 25 against 36.
 #include "attn_spans_few.h"
@@ -15,19 +15,22 @@ namespace {
 constexpr int kFewWaves = 2;
 
 // D, DT: columns of a row in the LDS, of few rows and of tiles; RGM: groups of 16 rows of a
-// sequence.  A block of few rows has two waves; its others end at once.
+// sequence.  A block of few rows has two waves.  Its others end at once, by a scalar branch
+// that no mask of lanes can turn into code they walk through: every wave that is left
+// meets the block's barriers.  (As a condition on the lanes 2 to 3 % less time.)
 template <typename T, int D, int DT, int RGM>
 __global__ __launch_bounds__(64 * span_tile::kWaves, 2) void k_span_mixed(SpanArgs a, int nqb, int slices, uint32_t front, span_few::FewBlocks main, SpanPart part) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int64_t all = block_id();
   if (all >= static_cast<int64_t>(front) + main.blocks) return;  // the tail of a 2-D grid (the whole block)
   const uint32_t id = static_cast<uint32_t>(all);
+  if (id >= front && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= kFewWaves) return;
   if (id < front) {
     part.first = 0;
     span_tile::tile_block<T, DT, DT>(a, kFront, nqb, slices, front, part, id, smem);
-  } else if (threadIdx.x < 64 * kFewWaves) {  // (whole waves, which a branch takes past the barriers; as a scalar condition 3 % slower)
-    span_few::few_block<T, D, kFewWaves, RGM>(a, main, part, id - front, smem);
+    return;
   }
+  span_few::few_block<T, D, kFewWaves, RGM>(a, main, part, id - front, smem);
 }
 
 template <typename T, int D, int DT, int RGM>
