@@ -289,7 +289,9 @@ bool matrix_layout(const SpanArgs& a, int dtype) {
     const int64_t sinks = std::min<int64_t>(a.C, a.sinks);
     if (!span(a.kst, sinks) || !span(a.vst, sinks)) return false;
   }
+  // (the kernel of few rows adds 32-bit offsets to a set's first query)
   const int64_t per = a.pk ? a.B / a.G : 1;
+  if (!f32 && (a.qst[0] < 0 || a.qst[1] < 0 || a.qst[2] < 0)) return false;
   if (!f32 && (per - 1) * a.qst[0] + (a.Hq / a.Hkv - 1) * a.qst[1] + (a.Sq - 1) * a.qst[2] + a.D >= 0x3fffffffLL) return false;
   return a.P == 0 || (rows16(a.pkst) && rows16(a.pvst) && aligned16(a.pk) && aligned16(a.pv) && span(a.pkst, a.P) && span(a.pvst, a.P));
 }
