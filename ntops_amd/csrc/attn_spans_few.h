@@ -167,8 +167,8 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
     hi[rg] = s.hi(token[rg]);
     lo[rg] = s.lo(token[rg]);
   }
-  // at least the least factor there is, so that a masked score stays -inf under a zero scale
-  const float c = fabsf(a.scale_log2) < 0x1p-126f ? 0x1p-126f : fabsf(a.scale_log2);
+  // (under a zero scale the least factor there is, so that a masked score stays -inf)
+  const float c = a.scale_log2 == 0.f ? 0x1p-149f : fabsf(a.scale_log2);
   const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // a negative scale: -Q
   const int hi_min = s.hi(0), lo_max = s.lo(t1);  // a main tile between them is seen whole by every row
 

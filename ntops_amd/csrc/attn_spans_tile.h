@@ -167,8 +167,8 @@ __device__ __forceinline__ void tile_block(const SpanArgs& a, int mode, int nqb,
       if (a.scale_log2 < 0.f) qf[ks] ^= 0x80008000u;
     }
   }
-  // at least the least factor there is, so that a masked score stays -inf under a zero scale
-  const float c = fabsf(a.scale_log2) < 0x1p-126f ? 0x1p-126f : fabsf(a.scale_log2);
+  // (under a zero scale the least factor there is, so that a masked score stays -inf)
+  const float c = a.scale_log2 == 0.f ? 0x1p-149f : fabsf(a.scale_log2);
 
   const int nt = (keys + kKeys - 1) / kKeys;
   const int share = (nt + slices - 1) / slices;
