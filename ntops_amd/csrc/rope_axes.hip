@@ -44,9 +44,15 @@ struct AxesArgs {
   alignas(8) uint8_t axis[kMaxPairs];
 };
 
-__device__ __forceinline__ void rotate_pair(float x0, float x1, float c0, float s0, float c1, float s1, float& o0, float& o1) {
-  o0 = fmaf(x0, c0, -(x1 * s0));
-  o1 = fmaf(x1, c1, x0 * s1);
+template <typename T>
+__device__ __forceinline__ void rotate_pair(float x0, float x1, float c0, float s0, float c1, float s1, T& y0, T& y1) {
+  float o0 = fmaf(x0, c0, -(x1 * s0)), o1 = fmaf(x1, c1, x0 * s1);
+  // One rounding to fp32, then one to the type, wherever a pair comes in the code: else some
+  // f16 results are rounded from the exact sum by a mixed-precision fma and others are not,
+  // and a head's last bit depends on which thread has it.
+  if constexpr (std::is_same<T, _Float16>::value) asm("" : "+v"(o0), "+v"(o1));
+  y0 = static_cast<T>(o0);
+  y1 = static_cast<T>(o1);
 }
 
 // Row of the tables of pair i's axis at token (b, s); -1: outside.
@@ -101,10 +107,7 @@ __global__ __launch_bounds__(256) void k_rope_axes_generic(AxesArgs a, int64_t p
     table_at<TT>(a, row, a.wide ? d0 : i, s0, c0);
     table_at<TT>(a, row, a.wide ? d1 : i, s1, c1);
     const float x0 = static_cast<float>(x[d0 * d.xs[3]]), x1 = static_cast<float>(x[d1 * d.xs[3]]);
-    float o0, o1;
-    rotate_pair(x0, x1, c0, s0, c1, s1, o0, o1);
-    y[d0 * d.ys[3]] = static_cast<T>(o0);
-    y[d1 * d.ys[3]] = static_cast<T>(o1);
+    rotate_pair(x0, x1, c0, s0, c1, s1, y[d0 * d.ys[3]], y[d1 * d.ys[3]]);
   }
 }
 
@@ -194,16 +197,10 @@ __global__ __launch_bounds__(256) void k_rope_axes(AxesArgs a, int parts, uint32
       Pack16<T> o0, o1;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        float r0, r1;
-        if constexpr (INTER) {
-          rotate_pair(static_cast<float>(v0.v[2 * i]), static_cast<float>(v0.v[2 * i + 1]), c0[i], s0[i], c1[i], s1[i], r0, r1);
-          o0.v[2 * i] = static_cast<T>(r0);
-          o0.v[2 * i + 1] = static_cast<T>(r1);
-        } else {
-          rotate_pair(static_cast<float>(v0.v[i]), static_cast<float>(v1.v[i]), c0[i], s0[i], c1[i], s1[i], r0, r1);
-          o0.v[i] = static_cast<T>(r0);
-          o1.v[i] = static_cast<T>(r1);
-        }
+        if constexpr (INTER)
+          rotate_pair(static_cast<float>(v0.v[2 * i]), static_cast<float>(v0.v[2 * i + 1]), c0[i], s0[i], c1[i], s1[i], o0.v[2 * i], o0.v[2 * i + 1]);
+        else
+          rotate_pair(static_cast<float>(v0.v[i]), static_cast<float>(v1.v[i]), c0[i], s0[i], c1[i], s1[i], o0.v[i], o1.v[i]);
       }
       store16_nt(p, o0);
       if constexpr (!INTER) store16_nt(p + half, o1);
