@@ -154,6 +154,19 @@ struct SpanPart {
   }
 };
 
+// A product rounded by itself, which no fma takes in.  Scores that are compared as rounded
+// products have their exponents from the same ones: an fma against a maximum that was rounded is
+// off by half a unit of the maximum, which past 2^24 is a factor of two and soon all there is.
+__device__ __forceinline__ float product(float a, float b) {
+  float p = a * b;
+  asm("" : "+v"(p));
+  return p;
+}
+// References (base 2) from which on the 16-bit kernels of the matrix cores take exponents so, by
+// two instructions a score; below, one fma, off by a factor under two that all of a row's
+// probabilities share.
+__device__ __forceinline__ bool span_far(float m) { return fabsf(m) >= 0x1p24f && m != neg_inf(); }
+
 // One query row by one wave, fp32 throughout, any head dim up to 16 EL and any
 // strides; reads nothing that the row does not see.  Sixteen lanes share a key
 // (lane i the columns i + 16 u), four keys side by side, UNROLL of them in flight
@@ -208,7 +221,7 @@ __device__ __forceinline__ void span_attend_row(const SpanArgs& a, const Spans& 
         d += dpp_mov<kDppXor2>(d);
         d += dpp_mov<kDppHalfMirror>(d);
         d += dpp_mov<kDppMirror>(d);
-        const float sc = k + 4 * w < k1 ? d * a.scale_log2 : neg_inf();
+        const float sc = k + 4 * w < k1 ? product(d, a.scale_log2) : neg_inf();
         const float m_new = fmaxf(m, sc);
         const float m_use = m_new == neg_inf() ? 0.f : m_new;
         float alpha = fast_exp2(m - m_use), p = fast_exp2(sc - m_use);

@@ -166,7 +166,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 2 : 4) void k_span_f32(SpanArgs
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int k = kb * 16 + r;
-          float v = sc[kb][r] * a.scale_log2;
+          float v = product(sc[kb][r], a.scale_log2);
           if (!whole) v = k < up && static_cast<uint32_t>(k - sink) >= hidden ? v : neg_inf();
           sc[kb][r] = v;
           mx = fmaxf(mx, v);
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_span_f32_few(SpanArgs a, 
     float p[4], mx = neg_inf();
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      p[r] = (sc[0][r] + sc[1][r]) * a.scale_log2;
+      p[r] = product(sc[0][r] + sc[1][r], a.scale_log2);
       if (!whole) p[r] = r < up && static_cast<uint32_t>(r - sink) >= hidden ? p[r] : neg_inf();
       mx = fmaxf(mx, p[r]);
     }

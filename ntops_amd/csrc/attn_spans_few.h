@@ -202,9 +202,14 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
 
   f32x4 o[RG][DT];
   float m[RG], l[RG];  // reference (base 2) of the lane's row; this lane's part of its sum
+  // exponents are by * score - mb: of c and the reference (0: nothing seen so far, P = 0), or
+  // where `far` (span_far of some row's reference, wave-uniform) of scores that are exponents
+  float by = c, mb[RG];
+  bool far = false;
 #pragma unroll
   for (int rg = 0; rg < RG; ++rg) {
     m[rg] = neg_inf();
+    mb[rg] = 0.f;
     l[rg] = 0.f;
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[rg][t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -293,29 +298,45 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
       mx[rg] = top[KB - 1] * c;
       raise = raise || mx[rg] > m[rg] + kSlack;
     }
-    if (__any(raise)) {
+    raise = __any(raise);
+    if (raise || far) {
+      if (raise) {
 #pragma unroll
-      for (int rg = 0; rg < RG; ++rg) {
-        mx[rg] = fmaxf(mx[rg], __shfl_xor(mx[rg], 16, 64));
-        mx[rg] = fmaxf(mx[rg], __shfl_xor(mx[rg], 32, 64));
-        const bool up = mx[rg] > m[rg] + kSlack;
-        const float alpha = up ? fast_exp2(m[rg] - mx[rg]) : 1.f;
-        m[rg] = up ? mx[rg] : m[rg];
-        l[rg] *= alpha;
+        for (int rg = 0; rg < RG; ++rg) {
+          mx[rg] = fmaxf(mx[rg], __shfl_xor(mx[rg], 16, 64));
+          mx[rg] = fmaxf(mx[rg], __shfl_xor(mx[rg], 32, 64));
+          const bool up = mx[rg] > m[rg] + kSlack;
+          const float alpha = up ? fast_exp2(m[rg] - mx[rg]) : 1.f;
+          m[rg] = up ? mx[rg] : m[rg];
+          l[rg] *= alpha;
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+          for (int t = 0; t < DT; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[rg][t][e] *= alpha;
+            for (int e = 0; e < 4; ++e) o[rg][t][e] *= alpha;
+          mb[rg] = m[rg] == neg_inf() ? 0.f : m[rg];
+          far = far || __any(span_far(m[rg]));
+        }
+      }
+      if (far) {
+#pragma unroll
+        for (int rg = 0; rg < RG; ++rg) {
+          const float ref = m[rg] == neg_inf() ? 0.f : m[rg];
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[rg][kb][e] = product(sc[rg][kb][e], c) - ref;
+          mb[rg] = 0.f;
+        }
+        by = 1.f;
       }
     }
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
-      const float mb = m[rg] == neg_inf() ? 0.f : m[rg];  // nothing seen so far: P = 0
 #pragma unroll
       for (int p = 0; p < KB / 2; ++p) {
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = fast_exp2(fmaf(sc[rg][2 * p + (e >> 2)][e & 3], c, -mb));
+        for (int e = 0; e < 8; ++e) x[e] = fast_exp2(fmaf(sc[rg][2 * p + (e >> 2)][e & 3], by, -mb[rg]));
         l[rg] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
         pf[rg][p] = pack8<T>(x);  // keys 32 p + 4 g + 0..3 and 32 p + 16 + 4 g + 0..3
       }

@@ -220,6 +220,7 @@ __device__ __forceinline__ void tile_block(const SpanArgs& a, int mode, int nqb,
     for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
   float m_run = neg_inf();  // reference (base 2) of row my_r
   float l_half = 0.f;       // this lane's half of the row's sum of exponentials
+  uint32_t far = 0;         // span_far of some row's reference, wave-uniform
   f32x16 sc[2];             // S of the tile being softmaxed
   u32x4 pf[4];              // P of that tile, as MFMA A operands per 16-key slice
 
@@ -287,13 +288,23 @@ __device__ __forceinline__ void tile_block(const SpanArgs& a, int mode, int nqb,
       for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[t][e] *= alpha;
+      far |= __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(__ballot(span_far(m_run)) != 0));
     }
-    const float mb = m_run == neg_inf() ? 0.f : m_run;  // nothing seen so far: P = 0
+    float mb = m_run == neg_inf() ? 0.f : m_run;  // nothing seen so far: P = 0
+    float by = c;
+    if (far != 0) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[u][e] = product(sc[u][e], c) - mb;
+      by = 1.f;
+      mb = 0.f;
+    }
     float p[2][16];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) p[u][e] = fast_exp2(fmaf(sc[u][e], c, -mb));
+      for (int e = 0; e < 16; ++e) p[u][e] = fast_exp2(fmaf(sc[u][e], by, -mb));
     float r[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) r[e] = p[0][e] + p[1][e];

@@ -145,3 +145,24 @@ def test_infinite_keys(g, b, hq, hkv, sq, p, c, d, dtype, bad):
     k[:, :, c - 2 :] = bad
     prefix_twice(q, pk, pv, k, v, None, torch.full((b,), c - 2).cuda())
     window_twice(q, k, v, c, 0, torch.full((b,), c - 2).cuda())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,hq,hkv,sq,c,d", [(2, 8, 2, 1, 700, 128), (1, 8, 2, 5, 500, 64), (2, 4, 2, 150, 300, 128), (1, 4, 2, 80, 300, 256), (2, 2, 1, 3, 200, 37), (64, 8, 8, 1, 200, 128), (40, 4, 2, 3, 40, 128)])
+def test_scores_of_any_size(b, hq, hkv, sq, c, d, dtype):
+    """Whole scores (exact in fp32) from 2^10 to 2^37, of which a row's largest, or those that
+    tie for it, have all the weight."""
+    q, k, v = window_inputs(b, hq, hkv, sq, c, d, dtype)
+    k[..., 0] = torch.randint(-90, 120, (b, hkv, c)).to(dtype).cuda()
+    p = 3001 if b == 40 else 60
+    pk, pv, _ = window_inputs(1, hkv, hkv, p, p, d, dtype)
+    pk[..., 0] = torch.randint(-90, 121, pk.shape[:3]).to(dtype).cuda()
+    for power in (10, 16, 20, 24, 26, 30):
+        for sign in (1, -1):
+            q.zero_()
+            q[..., 0], scale = sign * 2.0 ** min(power, 15), 2.0 ** max(0, power - 15)
+            args = doubles(q), doubles(k), doubles(v)
+            out, size, reach = S.sliding_window_attention(*args, 90, 4, None, scale)
+            check(nt.sliding_window_attention(q, k, v, 90, 4, scale=scale), (out, size, 0 * reach), 94, d, scale)
+            out, size, reach = S.shared_prefix_attention(args[0], doubles(pk), doubles(pv), *args[1:], scale=scale)
+            check(nt.shared_prefix_attention(q, pk, pv, k, v, scale=scale), (out, size, 0 * reach), pk.shape[2] + c, d, scale)
