@@ -308,11 +308,23 @@ struct Strided {
 
 // Whether two elements of x are the same memory.
 bool meets_itself(const Strided& x) {
+  // no, where each dim's step passes all that the smaller ones reach
+  Steps own[4];
+  int n = 0;
+  for (int i = 0; i < 4; ++i) {
+    if (x.size[i] <= 1) continue;
+    if (x.st[i] == 0) return true;
+    own[n++] = {std::abs(x.st[i]), x.size[i] - 1};
+  }
+  std::sort(own, own + n, [](const Steps& x, const Steps& y) { return x.step < y.step; });
+  Wide end = 1;
+  int nested = 0;
+  for (; nested < n && own[nested].step >= end; ++nested) end += static_cast<Wide>(own[nested].step) * own[nested].most;
+  if (nested == n) return false;
   for (int i = 0; i < 4; ++i) {
     // index vectors that differ first in dim i, by n + 1, and by -most .. most behind it
     const int64_t most = x.size[i] - 1, step = std::abs(x.st[i]);
     if (most <= 0) continue;
-    if (step == 0) return true;
     Layout a;
     a.add(step, most - 1);
     Wide target = -static_cast<Wide>(step);
