@@ -290,12 +290,17 @@ __device__ __forceinline__ void span_write_row(const SpanArgs& a, const SpanPart
 // What has to be computed again by itself: a sum of a row's columns that is no number, or
 // none that fp32 holds, under a sum of weights that is one.
 __device__ __forceinline__ bool span_again(float any, float l) { return !(any - any == 0.f) && l == l; }
-// The row again, from keys [f0, f1) of the front and [m0, m1) of the main span.
+// The row again, from keys [f0, f1) of the front and [m0, m1) of the main span.  A row that sees
+// an infinity or a NaN itself comes here too, for the result that it had: a wave takes such
+// rows one after the other, 100 to 200 times as long as the matrix cores.  (1, 32 / 8,
+// 4096, window 1024) bf16 of 128 with one infinite value among a head's sinks 15.4 ms (90 us
+// without), with one key in flight instead of four 22.7; fp32 6.5 (four keys: 16.8) against 0.61;
+// (64, 32 / 8, 1 over 4096) with one in every head 7.4 ms against 0.16.
 template <typename T, int EL>
 __device__ __forceinline__ void span_row_again(const SpanArgs& a, const Spans& s, const SpanPart& part, const SpanRow& x, int slice, int f0, int f1,
                                                int m0, int m1) {
   float o[EL], m, l;
-  span_attend_row<T, EL, 1, true>(a, s, x, f0, f1, m0, m1, o, m, l);
+  span_attend_row<T, EL, (sizeof(T) == 2 && EL == 8 ? 4 : 1), true>(a, s, x, f0, f1, m0, m1, o, m, l);
   span_write_row<T, EL, true>(a, part, x, slice, o, m, l);
 }
 
