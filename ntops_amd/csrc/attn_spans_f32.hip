@@ -480,6 +480,8 @@ int launch_f32(const SpanArgs& a, int mode, int slices, const SpanPart& part, hi
   return check_launch("attention");
 }
 
+// Over 128 columns all 256 are multiplied: (1, 16 / 4, 4096 causal) of 136 / 192 / 256 1578 /
+// 1584 / 1592 us, (1, 16 / 4, 500 behind 500) 90 / 95 / 102.  A form of 192 is not built.
 template <int DP>
 int run_f32(const SpanArgs& a, int mode, int slices, const SpanPart& part, hipStream_t st) {
   return launch_f32<DP, 8>(a, mode, slices, part, st);

@@ -12,7 +12,7 @@
 // more).
 //
 // Bound by the HBM where there are keys for every CU: bf16 (64, 32 / 8, 1 over up to 8192,
-// window 4096) of 128 columns 157 us, 6.3 TB/s; few keys by latency: (1, 32 / 8, 1 over 4096,
+// window 4096) of 128 columns 150 to 154 us, 6.4 TB/s; few keys by latency: (1, 32 / 8, 1 over 4096,
 // window 1024) 9.2 us and 3.5 the merge, of which the start, the lengths, the addresses
 // that follow from them and the first tile take most, one after the other.
 //
@@ -77,7 +77,9 @@ struct TileDma {
   }
   // rows `row0` and on into LDS at `dst`; !valid: loads of nothing, which still count in
   // vmcnt.  Columns past the head dim: of K zeros; of V whatever follows, which reaches
-  // nothing but the columns of O past the head dim.
+  // nothing but the columns of O past the head dim.  That is the next key, which is read
+  // anyway, where a head's keys lie side by side, but another head's where a token's heads do:
+  // (64, 32 / 8, 1 over 8192, window 4096) of 80 columns 101 / 189 us, of 128 160 / 169.
   __device__ __forceinline__ void issue(uint32_t dst, int row0, bool valid, int dt) const {
     u32x4 r = rsrc;
     r.z = valid ? r.z : 0u;
@@ -338,6 +340,7 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = fast_exp2(fmaf(sc[rg][2 * p + (e >> 2)][e & 3], by, -mb[rg]));
         l[rg] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        // (rounded to the type for the second product, the sum above not: attn_spans_tile.h)
         pf[rg][p] = pack8<T>(x);  // keys 32 p + 4 g + 0..3 and 32 p + 16 + 4 g + 0..3
       }
     }
