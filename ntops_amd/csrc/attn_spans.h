@@ -167,6 +167,15 @@ __device__ __forceinline__ float product(float a, float b) {
 // probabilities share.
 __device__ __forceinline__ bool span_far(float m) { return fabsf(m) >= 0x1p24f && m != neg_inf(); }
 
+// A mean of values as the type.  It passes none of them, but where probabilities were rounded up
+// together it does by up to half a step, and next to f16's largest value that is infinity.
+// (bf16 sums of such values pass fp32's range: such rows are computed again, unrounded.)
+template <typename T>
+__device__ __forceinline__ T mean_as(float x) {
+  if constexpr (std::is_same<T, _Float16>::value) x = fabsf(x) < __builtin_huge_valf() ? __builtin_amdgcn_fmed3f(x, -65504.f, 65504.f) : x;
+  return static_cast<T>(x);
+}
+
 // One query row by one wave, fp32 throughout, any head dim up to 16 EL and any
 // strides; reads nothing that the row does not see.  Sixteen lanes share a key
 // (lane i the columns i + 16 u), four keys side by side, UNROLL of them in flight
@@ -284,7 +293,7 @@ __device__ __forceinline__ void span_write_row(const SpanArgs& a, const SpanPart
   T* O = static_cast<T*>(a.o) + x.b * a.ost[0] + x.h * a.ost[1] + x.t * a.ost[2];
 #pragma unroll
   for (int u = 0; u < EL; ++u)
-    if (lane + 16 * u < a.D) O[(lane + 16 * u) * a.ost[3]] = static_cast<T>(o[u] * inv);
+    if (lane + 16 * u < a.D) O[(lane + 16 * u) * a.ost[3]] = mean_as<T>(o[u] * inv);
 }
 
 // What has to be computed again by itself: a sum of a row's columns that is no number, or

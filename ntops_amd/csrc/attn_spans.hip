@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void k_span_merge(SpanArgs a, SpanPart part) {
   T* O = static_cast<T*>(a.o) + b * a.ost[0] + (bh - b * a.Hq) * a.ost[1] + (id - bh * a.Sq) * a.ost[2];
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (d + e < a.D) O[(d + e) * a.ost[3]] = static_cast<T>(o[e]);
+    if (d + e < a.D) O[(d + e) * a.ost[3]] = mean_as<T>(o[e]);
 }
 
 template <typename T, int W>

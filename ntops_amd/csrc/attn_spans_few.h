@@ -435,7 +435,7 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
         const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (a NaN sum passes through)
         T w4[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w4[e] = static_cast<T>(v[e] * inv);
+        for (int e = 0; e < 4; ++e) w4[e] = mean_as<T>(v[e] * inv);
         *reinterpret_cast<u32x2*>(static_cast<T*>(a.o) + to[row] + d) =
             __builtin_bit_cast(u32x2, w4);
       }

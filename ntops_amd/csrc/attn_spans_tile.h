@@ -367,13 +367,25 @@ __device__ __forceinline__ void tile_block(const SpanArgs& a, int mode, int nqb,
         }
     } else {
       T* O = static_cast<T*>(a.o) + x.b * a.ost[0] + x.h * a.ost[1] + x.t * a.ost[2];
+      float by_sum = inv;
+      if constexpr (std::is_same<T, _Float16>::value) {
+        // as mean_as, in fewer instructions: the row is divided by what its probabilities were rounded up by
+        // (f16 (7, 16, 2001, window 255) of 80 columns 47.1 us, each value cut by itself 47.9, neither 46.2)
+        float top = 0.f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) top = max3(fabsf(o[t][e]), fabsf(o[t][e + 1]), top);
+        const float past = top * inv;
+        if (past > 65504.f && past < __builtin_huge_valf()) by_sum *= 65504.f / past;
+      }
 #pragma unroll
       for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           T v4[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v4[e] = static_cast<T>(o[t][4 * q + e] * inv);
+          for (int e = 0; e < 4; ++e) v4[e] = static_cast<T>(o[t][4 * q + e] * by_sum);
           const int col = t * 32 + 8 * q + 4 * (lane >> 5);
           if (col < a.D)  // a.D % 8 == 0: the 4 columns are all in or all out
             *reinterpret_cast<u32x2*>(O + col) = __builtin_bit_cast(u32x2, v4);

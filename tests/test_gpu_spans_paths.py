@@ -1,12 +1,14 @@
 """Paths of sliding_window_attention and shared_prefix_attention that the main uses take
 and small problems do not, against the 64-bit oracle (tolerances: test_gpu_spans.py)."""
 
+import math
+
 import pytest
 import torch
 
 import ntops_amd.torch as nt
 from ntops_amd import _lib
-from tests.test_gpu_spans import DTYPES, check, doubles, window_inputs
+from tests.test_gpu_spans import DTYPES, HALF_STEP, check, doubles, window_inputs
 from oracle import spans as S
 
 pytestmark = pytest.mark.gpu
@@ -166,3 +168,23 @@ def test_scores_of_any_size(b, hq, hkv, sq, c, d, dtype):
             check(nt.sliding_window_attention(q, k, v, 90, 4, scale=scale), (out, size, 0 * reach), 94, d, scale)
             out, size, reach = S.shared_prefix_attention(args[0], doubles(pk), doubles(pv), *args[1:], scale=scale)
             check(nt.shared_prefix_attention(q, pk, pv, k, v, scale=scale), (out, size, 0 * reach), pk.shape[2] + c, d, scale)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("b,hq,hkv,sq,c,d", [(1, 4, 2, 1, 900, 128), (2, 8, 2, 3, 200, 64), (1, 4, 2, 150, 600, 128), (1, 2, 1, 2, 300, 36), (64, 8, 8, 1, 120, 64), (2, 4, 2, 80, 400, 200)])
+def test_means_of_the_largest_value(b, hq, hkv, sq, c, d, dtype):
+    """All values the type's largest: so is every mean of them, though probabilities that are
+    rounded up together would pass it."""
+    q, k = (torch.zeros(b, h, n, d, dtype=dtype, device="cuda") for h, n in ((hq, sq), (hkv, c)))
+    v = torch.full_like(k, torch.finfo(dtype).max)
+    v[..., 1::2] *= -1
+    q[..., 0], k[..., 1] = 1, 0
+    k[:, :, 0, 0] = 1
+    half = HALF_STEP[dtype]
+    for p in (0.5 * (1 + 1.01 * half), 0.25 * (1 + 1.2 * half), 1 - 0.4 * half):  # every other key's probability, of a first key's 1
+        scale = -math.log(p)
+        want = S.sliding_window_attention(doubles(q), doubles(k), doubles(v), c, 0, None, scale)
+        check(nt.sliding_window_attention(q, k, v, c, scale=scale), want, c, d, scale)
+        front, own = (k[:1, :, : c // 2], v[:1, :, : c // 2]), (k[:, :, c // 2 :], v[:, :, c // 2 :])
+        want = S.shared_prefix_attention(doubles(q), *(doubles(t) for t in front + own), scale=scale)
+        check(nt.shared_prefix_attention(q, *front, *own, scale=scale), want, c, d, scale)
