@@ -44,6 +44,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
+// Of results of matrix instructions, which the compiler keeps only its own instructions from
+// reading too early: not before `seen`, what one of those has read from the last of them.
+__device__ __forceinline__ float max3_after(float a, float b, float c, uint32_t seen) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c), "v"(seen));
+  return r;
+}
+__device__ __forceinline__ uint32_t read_of(float a, float b) { return __float_as_uint(a) | __float_as_uint(b); }
 
 // From here on a result cut to [0, 1] keeps a NaN (it is 0 by default): the
 // wave's MODE register, bit 8 (DX10_CLAMP).

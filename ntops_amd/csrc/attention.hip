@@ -67,9 +67,13 @@ __device__ __forceinline__ float max32(const f32x16 (&s)[2]) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[16 * u + e] = s[u][e];
   float m1[11];
+  const uint32_t seen = read_of(v[15], v[31]);
+  m1[10] = max3_after(v[15], v[31], v[31], seen);
 #pragma unroll
-  for (int i = 0; i < 10; ++i) m1[i] = max3(v[3 * i], v[3 * i + 1], v[3 * i + 2]);
-  m1[10] = max3(v[30], v[31], v[31]);
+  for (int i = 0; i < 5; ++i) {
+    m1[i] = max3_after(v[3 * i], v[3 * i + 1], v[3 * i + 2], seen);
+    m1[5 + i] = max3_after(v[16 + 3 * i], v[17 + 3 * i], v[18 + 3 * i], seen);
+  }
   const float m2a = max3(m1[0], m1[1], m1[2]), m2b = max3(m1[3], m1[4], m1[5]);
   const float m2c = max3(m1[6], m1[7], m1[8]), m2d = max3(m1[9], m1[10], m1[10]);
   return max3(m2a, m2b, max3(m2c, m2d, m2d));

@@ -61,8 +61,8 @@ __device__ __forceinline__ void widen16(u32x4 c, float scale, u32x4 (&o)[2]) {
                  widen2<T, false>(c[2 * i + 1], scale), widen2<T, true>(c[2 * i + 1], scale)};
 }
 
-__device__ __forceinline__ float max8(const float* v) {
-  return max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[7]));
+__device__ __forceinline__ float max8(const float* v, uint32_t seen) {
+  return max3(max3_after(v[0], v[1], v[2], seen), max3_after(v[3], v[4], v[5], seen), max3_after(v[6], v[7], v[7], seen));
 }
 
 // Blocks that a CU holds: by registers.
@@ -299,7 +299,8 @@ __global__ __launch_bounds__(256, blocks_per_cu(std::is_same<T, __bf16>::value, 
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[t][e] = s[t][e];
-    const float th = fmaxf(max3(max8(&x[0][0]) * c[0], max8(&x[0][8]) * c[1], max8(&x[1][0]) * c[2]), max8(&x[1][8]) * c[3]);
+    const uint32_t seen = read_of(x[0][15], x[1][15]);
+    const float th = fmaxf(max3(max8(&x[0][0], seen) * c[0], max8(&x[0][8], seen) * c[1], max8(&x[1][0], seen) * c[2]), max8(&x[1][8], seen) * c[3]);
     if (__any(th > m_i + kSlack)) {
       const auto h2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(th), __float_as_uint(th), false, false);
       const float tmax = fmaxf(__uint_as_float(h2[0]), __uint_as_float(h2[1]));  // of lanes l and l ^ 32

@@ -289,12 +289,13 @@ __device__ __forceinline__ void few_block(const SpanArgs& a, const FewBlocks& f,
     }
     float mx[RG];
     bool raise = false;
+    const uint32_t seen = read_of(sc[0][KB - 1][3], sc[RG - 1][KB - 1][3]);
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
       float top[KB];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
-        top[kb] = max3(sc[rg][kb][0], sc[rg][kb][1], sc[rg][kb][2]);
+        top[kb] = max3_after(sc[rg][kb][0], sc[rg][kb][1], sc[rg][kb][2], seen);
         top[kb] = max3(top[kb], sc[rg][kb][3], kb > 0 ? top[kb - 1] : top[kb]);
       }
       mx[rg] = top[KB - 1] * c;

@@ -102,9 +102,13 @@ __device__ __forceinline__ float max32(const f32x16 (&s)[2]) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[16 * u + e] = s[u][e];
   float m[11];
+  const uint32_t seen = read_of(v[15], v[31]);
+  m[10] = max3_after(v[15], v[31], v[31], seen);
 #pragma unroll
-  for (int i = 0; i < 10; ++i) m[i] = max3(v[3 * i], v[3 * i + 1], v[3 * i + 2]);
-  m[10] = max3(v[30], v[31], v[31]);
+  for (int i = 0; i < 5; ++i) {
+    m[i] = max3_after(v[3 * i], v[3 * i + 1], v[3 * i + 2], seen);
+    m[5 + i] = max3_after(v[16 + 3 * i], v[17 + 3 * i], v[18 + 3 * i], seen);
+  }
   return max3(max3(max3(m[0], m[1], m[2]), max3(m[3], m[4], m[5]), m[6]), max3(m[7], m[8], m[9]), m[10]);
 }
 
